@@ -53,8 +53,10 @@
 extern "C" {
 #endif
 
-#define PA_ABI_VERSION 8
+#define PA_ABI_VERSION 9
 #define PA_MAX_ORDER 8
+#define PA_MAX_DRAFTS 64   /* drafted tokens per row of one step */
+#define PA_MAX_MOVES 128   /* array pairs of one pa_draft_commit */
 
 /* status codes (0 = success, negative = failure) */
 #define PA_OK            0
@@ -335,13 +337,146 @@ typedef struct pa_linear {
     pa_linear_out out[PA_LINEAR_MAX_OUT];
 } pa_linear;
 
+/* ---- drafted tokens (no counterpart in the reference) ------------------------------------
+ * A decode step that looks at several new tokens per row at once: `drafts` (T <= PA_MAX_DRAFTS)
+ * nodes per batch row behind a cache whose rows hold counts[b] positions each.  The nodes of a row
+ * form a tree: parents[b * parents_stride + t] is the node that t follows (lower than t), or -1
+ * for a node that follows the cached positions; parents == NULL is a chain (0, 1, 2, ...).  Any
+ * other value, and a parent that is itself absent, makes the node absent: nothing attends to it,
+ * its outputs are 0 and the walk of pa_draft_verify never reaches it.
+ * The drafted tokens' keys, values, level outputs and logsumexps lie in draft slots [B, kv_heads,
+ * T, dim] beside the cache until pa_draft_commit moves the kept ones behind the cached positions.
+ * A count below 0 or above the capacity is taken as that bound. */
+
+/* One level of pa_draft_attend. */
+typedef struct pa_draft_level {
+    pa_view k;            /* [B, kv_heads, capacity, dim]: the cached keys */
+    pa_view v;            /* cached values; at the final level the outputs of the level below */
+    pa_view vmul;         /* middle levels: the cached outputs of the level below */
+    pa_view bias;         /* every level but the deepest: fp32 [B, kv_heads, capacity], the cached
+                           * logsumexps of the level below (unit position stride) */
+    pa_view q;            /* [B, heads, T, dim] at the final level, else [B, kv_heads, T, dim] */
+    pa_view dk;           /* [B, kv_heads, T, dim]: the drafted tokens' keys */
+    pa_view dv;           /* their values (not at the final level) */
+    pa_view out;          /* like q: this level's output for every node */
+    pa_view lse;          /* fp32 [B, kv_heads, T] (not at the final level; unit position stride) */
+} pa_draft_level;
+
+/* Every level of an order-`order` poly attention for all nodes of a step, levels[0] the deepest:
+ *   s_ij  = softclamp(scale <q_i, k_j>) + bias_j      j a cached position of the row, an ancestor of
+ *   out_i = sum_j softmax_j(s_ij) v_j                  node i, or i itself
+ *   lse_i = logsumexp_j(s_ij)
+ * with the values of pa_poly_decode (v; round(v * out of the level below); out of the level below);
+ * the ancestors' level outputs are used as computed, in fp32.  Rows and views start on 16 bytes. */
+typedef struct pa_draft {
+    int32_t batch, kv_heads, heads, drafts, dim, order, capacity;
+    float   scale, softclamp;
+    const int32_t* counts;      /* device [B] */
+    const int32_t* parents;     /* device, or NULL: a chain */
+    int64_t        parents_stride;  /* elements between rows (0: one tree for all rows) */
+    pa_draft_level levels[PA_MAX_ORDER];
+    void*   workspace;
+    size_t  workspace_bytes;
+} pa_draft;
+
+/* One tensor of pa_draft_append. */
+typedef struct pa_draft_item {
+    pa_view     src;            /* [B, heads, T, dim]: the projection (unit feature stride) */
+    const void* norm_weight;    /* [dim] RMSNorm weight, or NULL: no normalisation */
+    int32_t     weight_dtype;
+    int32_t     rotate;         /* nonzero: rotate the leading rot_dim features after the norm */
+    pa_view     out;            /* [B, heads, T, dim] */
+} pa_draft_item;
+
+/* The q RMSNorms and the rotary embedding of a step's drafted tokens, written to their draft slots:
+ *   y = round(rotate(x * rsqrt(mean(x^2) + eps) * w))
+ * rounded once (pa_decode_prologue also rounds between the norm and the rotation).  The angles are
+ * angles[b * angles_sb + t * angles_sn + feature], or with inv_freq those of pa_decode_prologue at
+ * the node's position counts[b] + (its number of ancestors). */
+typedef struct pa_draft_rows {
+    int32_t        batch, drafts, dim, count;
+    float          eps;
+    const int32_t* counts;      /* device [B] (read with inv_freq) */
+    const int32_t* parents;     /* device, or NULL: a chain (read with inv_freq) */
+    int64_t        parents_stride;
+    const void*    angles;      /* or NULL */
+    int32_t        angles_dtype;
+    int32_t        rot_dim;     /* even, <= dim */
+    int64_t        angles_sb, angles_sn;
+    const float*   inv_freq;    /* [rot_dim / 2], or NULL */
+    float          interp;
+    pa_draft_item  items[2 * PA_MAX_ORDER];
+} pa_draft_rows;
+
+/* The walk over a row's tree against the target's probabilities.  logits[b, t] is the target's
+ * prediction behind node t; p_t = softmax(logits[b, t] / temperature[b]), and where the temperature
+ * is not above 0 (or uniforms is NULL) all of p_t is on the first of the largest logits.  The walk
+ * starts at node 0, which is kept, and takes the nodes in order: a child t of the current node
+ * with token x is kept, and becomes the current node, when uniforms[b, t] * q(x) < p(x); otherwise
+ *   p := max(p - q, 0) / sum   with draft_probs, q = draft_probs[b, current node] the distribution
+ *                              that the children of that node were drawn from, independently
+ *   p := p without x / sum     without: the children were chosen, q(x) = 1
+ * (p stays as it is where the sum is 0).  At the end token[b] is the i with the largest
+ * p_i / noise[b, i] among p_i > 0, the lowest of equals: with noise drawn from Exp(1) a sample of p.
+ * path[b] lists the kept nodes in order, then -1; kept[b] is their number.  A row whose node 0 is
+ * absent keeps nothing and gets token -1, and a p without a positive entry (logits that are NaN or
+ * all -inf) gives token -1.  A token outside the vocabulary is not kept (and without
+ * draft_probs removes nothing from p). */
+typedef struct pa_verify {
+    int32_t        batch, drafts, vocab;
+    int32_t        dtype;       /* of logits: PA_F32 / PA_F16 / PA_BF16 */
+    const void*    logits;      /* [B, T, vocab] (unit vocab stride) */
+    int64_t        logits_sb, logits_sn;
+    const int64_t* tokens;      /* [B, T] */
+    int64_t        tokens_stride;
+    const int32_t* parents;     /* or NULL: a chain */
+    int64_t        parents_stride;
+    const float*   uniforms;    /* [B, T] in [0, 1), or NULL: every row takes the largest logits */
+    int64_t        uniforms_stride;
+    const float*   noise;       /* [B, vocab] > 0; required with uniforms */
+    int64_t        noise_stride;
+    const float*   temperature; /* [B], or NULL: 1 */
+    const float*   draft_probs; /* [B, T, vocab], or NULL */
+    int64_t        probs_sb, probs_sn;
+    int32_t*       path;        /* [B, T] */
+    int32_t*       kept;        /* [B] */
+    int64_t*       token;       /* [B] */
+    void*          workspace;
+    size_t         workspace_bytes;
+} pa_verify;
+
+/* One pair of arrays of pa_draft_commit: src [B, kv_heads, slots, row_bytes] and
+ * dst [B, kv_heads, capacity, row_bytes], contiguous; row_bytes a multiple of 4 (rows of whole 16
+ * bytes start on 16 bytes). */
+typedef struct pa_draft_move {
+    const void* src;
+    void*       dst;
+    int32_t     row_bytes;
+    int32_t     pad;
+} pa_draft_move;
+
+/* dst[b, h, counts[b] + i] = src[b, h, path[b, i]] for i < kept[b] and every move, then, with
+ * `advance`, counts[b] += the number moved.  A path ends early at an entry outside [0, slots);
+ * positions past the capacity are not written nor counted, and overflow[0] (when given) is set. */
+typedef struct pa_commit {
+    int32_t        batch, kv_heads, slots, capacity, count, advance;
+    const int32_t* path;        /* device [B, path_stride] */
+    int64_t        path_stride;
+    int32_t        path_len;    /* entries per row */
+    const int32_t* kept;        /* device [B] */
+    int32_t*       counts;      /* device [B] */
+    int32_t*       overflow;    /* device [1], or NULL */
+    pa_draft_move  moves[PA_MAX_MOVES];
+} pa_commit;
+
 int         pa_abi_version(void);
 const char* pa_strerror(int status);
 int         pa_last_hip_error(void);   /* hipError_t of the last PA_EHIP on this thread */
 /* sizeof of the ABI structs, for binding checks: 0 pa_view, 1 pa_mask, 2 pa_pass,
  * 3 pa_pass_grad, 4 pa_decode_level, 5 pa_decode, 6 pa_prologue_item, 7 pa_prologue,
- * 8 pa_rmsnorm, 9 pa_linear, 10 pa_linear_out, 11 pa_epilogue, 12 pa_qk_norm; 0 for other
- * values */
+ * 8 pa_rmsnorm, 9 pa_linear, 10 pa_linear_out, 11 pa_epilogue, 12 pa_qk_norm, 13 pa_draft_level,
+ * 14 pa_draft, 15 pa_draft_item, 16 pa_draft_rows, 17 pa_verify, 18 pa_draft_move, 19 pa_commit;
+ * 0 for other values */
 size_t      pa_struct_size(int which);
 
 /* Kernel timing (no counterpart in the reference: a measurement facility for benchmarks).
@@ -413,6 +548,14 @@ int    pa_linear_small(const pa_linear* l, void* stream);
 /* The same without input steps, activations and residuals, for 16-bit types, up to 64 rows and
  * any in_features that is a multiple of 8 (the projections of a step over a larger batch). */
 int    pa_linear_rows(const pa_linear* l, void* stream);
+
+/* A step over drafted tokens: append, attend (per layer), verify, commit (per model). */
+int    pa_draft_append(const pa_draft_rows* r, void* stream);
+size_t pa_draft_attend_workspace(const pa_draft* d);
+int    pa_draft_attend(const pa_draft* d, void* stream);
+size_t pa_draft_verify_workspace(const pa_verify* v);
+int    pa_draft_verify(const pa_verify* v, void* stream);
+int    pa_draft_commit(const pa_commit* c, void* stream);
 
 #ifdef __cplusplus
 }

@@ -267,6 +267,13 @@ size_t pa_struct_size(int which) {
         case 10: return sizeof(pa_linear_out);
         case 11: return sizeof(pa_epilogue);
         case 12: return sizeof(pa_qk_norm);
+        case 13: return sizeof(pa_draft_level);
+        case 14: return sizeof(pa_draft);
+        case 15: return sizeof(pa_draft_item);
+        case 16: return sizeof(pa_draft_rows);
+        case 17: return sizeof(pa_verify);
+        case 18: return sizeof(pa_draft_move);
+        case 19: return sizeof(pa_commit);
         default: return 0;
     }
 }
@@ -686,5 +693,37 @@ int pa_linear_small(const pa_linear* l, void* stream) {
     if (st != PA_OK) return st;
     return finish_launch();
 }
+
+int pa_draft_append(const pa_draft_rows* x, void* stream) {
+    if (!x) return PA_EINVAL;
+    const int st = launch_draft_append(x, static_cast<hipStream_t>(stream));
+    if (st != PA_OK) return st;
+    return finish_launch();
+}
+
+int pa_draft_attend(const pa_draft* x, void* stream) {
+    if (!x) return PA_EINVAL;
+    const int st = launch_draft_attend(x, static_cast<hipStream_t>(stream));
+    if (st != PA_OK) return st;
+    return finish_launch();
+}
+
+int pa_draft_verify(const pa_verify* x, void* stream) {
+    if (!x) return PA_EINVAL;
+    const int st = launch_draft_verify(x, static_cast<hipStream_t>(stream));
+    if (st != PA_OK) return st;
+    return finish_launch();
+}
+
+int pa_draft_commit(const pa_commit* x, void* stream) {
+    if (!x) return PA_EINVAL;
+    const int st = launch_draft_commit(x, static_cast<hipStream_t>(stream));
+    if (st != PA_OK) return st;
+    return finish_launch();
+}
+
+size_t pa_draft_attend_workspace(const pa_draft* d) { return d ? draft_attend_workspace(d) : 0; }
+
+size_t pa_draft_verify_workspace(const pa_verify* v) { return v ? draft_verify_workspace(v) : 0; }
 
 }  // extern "C"

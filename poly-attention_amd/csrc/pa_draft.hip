@@ -1,0 +1,631 @@
+// pa_draft.hip -- the rest of a drafted step: the join of the units with the tree part
+// (k_draft_combine), norms, rotary and draft slots (k_draft_append), the move of the kept nodes
+// (k_draft_commit), and the host side of these entry points.
+#include <algorithm>
+
+#include "pa_draft_partial.h"
+
+namespace pa {
+
+// ---------------------------------------------------------------------------------------
+// One workgroup per (batch row and key head, P.cols columns of the head, up to 64 rows of the
+// final level).  Per level, deepest first: the scores of the rows against the T drafted keys
+// (16x16 tiles), masked to each node's ancestors; their softmax joined with the units' maxima and
+// sums; the workgroup's columns of the output from the units' weighted values and the tree's
+// values.  The levels below the final one have at most 64 rows and are repeated by every row block.
+template <typename T, int D>
+__global__ __launch_bounds__(kDraftThreads) void k_draft_combine(const DraftDev P) {
+    typedef DraftGeo<T, D> G;
+    constexpr int KS = G::KS, KE = G::KE;
+    extern __shared__ float smem[];
+    const int T16 = (P.T + 15) & ~15;
+    const int spitch = T16 + 1, vpitch = P.cols + 4;
+    float* s_s = smem;                         // [64][spitch]: scores, then probabilities
+    float* s_in = s_s + ((64 * spitch + 3) & ~3);  // [T16][vpitch]: this level's tree values
+    float* s_out = s_in + T16 * vpitch;        // [T16][vpitch]: its outputs
+    __shared__ uint64_t s_anc[64];
+    __shared__ float s_bias[64], s_nbias[64], s_top[64], s_sum[64];
+    __shared__ float4 s_red[kDraftThreads];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int b = blockIdx.x / P.kv_heads, hk = blockIdx.x % P.kv_heads;
+    const int col0 = blockIdx.y * P.cols, ncol = min(P.cols, P.dim - col0);
+    const int64_t size = draft_unit_size(P, lane);
+    const int first = draft_first_unit(P, size, b, lane);
+    const int units = (int)((draft_count(P, b) + size - 1) / size);
+    if (wave == 0)
+        s_anc[lane] = draft_ancestors(P.parents ? P.parents + b * P.parents_stride : nullptr, P.T, lane);
+    const float sl2 = P.scale * kLog2e, cl2 = P.softclamp * kLog2e;
+    const float cinv = P.softclamp > 0.f ? P.scale / P.softclamp : 0.f;
+    const int quads = ncol / 4;  // dim and cols are multiples of 4
+
+    for (int t = 0; t < P.order; ++t) {
+        const DraftLevelDev& L = P.L[t];
+        const bool last = t == P.order - 1;
+        const int r0 = last ? blockIdx.z * 64 : 0;
+        if (r0 >= L.rows) return;  // the final level: nothing follows
+        const int rows = min(64, L.rows - r0);
+        const int64_t rec = ((int64_t)first * P.kv_heads + hk) * P.rec_rows + L.row0 + r0;
+        const int64_t urec = (int64_t)P.kv_heads * P.rec_rows;  // records between units
+
+        // the tree's values: v, v * msg, or msg (already in s_in, as the level below left it)
+        if (!last)
+            for (int x = tid; x < P.T * quads; x += kDraftThreads) {
+                const int n = x / quads, d = 4 * (x % quads);
+                const T* row = L.dv.at<T>(b, hk) + n * L.dv.sn + col0 + d;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float* at = &s_in[n * vpitch + d + e];
+                    *at = t == 0 ? to_f(row[e]) : *at * to_f(row[e]);
+                }
+            }
+        __syncthreads();  // s_anc and the level below's results are in place
+
+        const int nrt = (rows + 15) / 16, nkt = T16 / 16;
+        for (int pair = wave; pair < nrt * nkt; pair += 4) {
+            const int rt = pair / nkt, kt = pair % nkt;
+            const int r = r0 + min(16 * rt + c, rows - 1), n = min(16 * kt + c, P.T - 1);
+            const T* qrow = L.q.at<T>(b, hk * L.rep + r / P.T) + (r % P.T) * L.q.sn;
+            const T* krow = L.dk.at<T>(b, hk) + n * L.dk.sn;
+            f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int d = KE * 4 * s + KE * g;
+                const bool in = d < P.dim;
+                const u32x4_d q = in ? load16u(qrow + d) : u32x4_d{0u, 0u, 0u, 0u};
+                const u32x4_d k = in ? load16u(krow + d) : u32x4_d{0u, 0u, 0u, 0u};
+                if constexpr (G::F32) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) a = mma_f32(q[j], k[j], a);
+                } else {
+                    a = Mma16<T>::run(q, k, a);
+                }
+            }
+            const int key = 16 * kt + c;
+            const float bz = t == 0 ? 0.f : s_bias[key];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 16 * rt + 4 * g + i;
+                const bool sees = row < rows && ((s_anc[(r0 + row) % P.T] >> key) & 1);
+                const float y = P.softclamp > 0.f ? cl2 * tanhf(a[i] * cinv) : a[i] * sl2;
+                s_s[row * spitch + key] = sees ? y + bz : -INFINITY;
+            }
+        }
+        __syncthreads();
+
+        {   // four threads per row: maximum and sum over the units and the tree
+            const int row = tid >> 2, sub = tid & 3;
+            float top = -INFINITY, sum = 0.f;
+            if (row < rows) {
+                for (int k = sub; k < P.T; k += 4) top = fmaxf(top, s_s[row * spitch + k]);
+                for (int u = sub; u < units; u += 4) top = fmaxf(top, P.ws_s[rec + row + u * urec].x);
+            }
+            top = fmaxf(top, __shfl_xor(top, 1));
+            top = fmaxf(top, __shfl_xor(top, 2));
+            if (row < rows) {
+                for (int k = sub; k < P.T; k += 4) {
+                    const float x = s_s[row * spitch + k];
+                    const float p = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - top);
+                    s_s[row * spitch + k] = p;
+                    sum += p;
+                }
+                for (int u = sub; u < units; u += 4) {
+                    const float2 ms = P.ws_s[rec + row + u * urec];
+                    sum += ms.x == -INFINITY ? 0.f : ms.y * __builtin_amdgcn_exp2f(ms.x - top);
+                }
+            }
+            sum += __shfl_xor(sum, 1);
+            sum += __shfl_xor(sum, 2);
+            if (row < rows && sub == 0) {
+                const bool live = s_anc[(r0 + row) % P.T] != 0;
+                s_top[row] = top;
+                s_sum[row] = live ? sum : 0.f;
+                if (!last) {
+                    const float lse = live ? top + log2f(sum) : 0.f;
+                    s_nbias[row] = lse;
+                    if (blockIdx.y == 0 && blockIdx.z == 0) L.lse.at<float>(b, hk)[row] = lse * kLn2;
+                }
+            }
+        }
+        __syncthreads();
+
+        // the outputs: one (row, four columns) item per thread; with few items the units are dealt out
+        // over `parts` threads per item
+        const int rp = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+        const int items = rp * quads;
+        const int parts = items * 8 <= kDraftThreads ? 8 : items * 4 <= kDraftThreads ? 4
+                          : items * 2 <= kDraftThreads ? 2 : 1;
+        for (int x0 = 0; x0 < items; x0 += kDraftThreads) {
+            const int part = parts > 1 ? tid / items : 0;
+            const int item = parts > 1 ? tid % items : x0 + tid;
+            const int row = item / quads, d = 4 * (item % quads);
+            const bool on = item < items && part < parts && row < rows && s_sum[row] != 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (on) {
+                const float top = s_top[row];
+                const float* src = P.ws_o + (rec + row) * P.dim + col0 + d;
+                for (int u = part; u < units; u += parts) {
+                    const float mu = P.ws_s[rec + row + u * urec].x;
+                    const float w = mu == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mu - top);
+                    const float4 y = *reinterpret_cast<const float4*>(src + u * urec * P.dim);
+                    acc.x += w * y.x;
+                    acc.y += w * y.y;
+                    acc.z += w * y.z;
+                    acc.w += w * y.w;
+                }
+                if (part == 0) {
+                    // only what the node sees: another branch's value may be anything
+                    for (uint64_t see = s_anc[(r0 + row) % P.T]; see; see &= see - 1) {
+                        const int k = __ffsll((unsigned long long)see) - 1;
+                        const float p = s_s[row * spitch + k];
+                        const float* y = &s_in[k * vpitch + d];
+                        acc.x += p * y[0];
+                        acc.y += p * y[1];
+                        acc.z += p * y[2];
+                        acc.w += p * y[3];
+                    }
+                }
+            }
+            if (parts > 1) {
+                s_red[tid] = acc;
+                __syncthreads();
+                if (part == 0)
+                    for (int k = 1; k < parts; ++k) {
+                        const float4 y = s_red[tid + k * items];
+                        acc.x += y.x;
+                        acc.y += y.y;
+                        acc.z += y.z;
+                        acc.w += y.w;
+                    }
+            }
+            if (part == 0 && item < items && row < rows) {
+                const float inv = s_sum[row] != 0.f ? 1.f / s_sum[row] : 0.f;
+                const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+                if (!last) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s_out[row * vpitch + d + e] = y[e];
+                }
+                if (last || blockIdx.z == 0) {
+                    const int r = r0 + row;
+                    T* to = L.out.at<T>(b, hk * L.rep + r / P.T) + (r % P.T) * L.out.sn + col0 + d;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) to[e] = from_f<T>(y[e]);
+                }
+            }
+        }
+        __syncthreads();
+        if (tid < 64) s_bias[tid] = s_nbias[tid];
+        float* const done = s_out;  // this level's outputs are the next one's values
+        s_out = s_in;
+        s_in = done;
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Norms and rotary of a step's nodes into their draft slots.  One workgroup per (node, part of its
+// rows), a lane holding 16 bytes of a row: a lane's features are the same in all its rows, so the
+// sines and cosines are computed once per lane (they cost more than the rows).
+
+struct DraftItemDev {
+    DraftRow src, out;
+    const void* w;
+    int32_t wdt, rotate, row0;
+};
+struct DraftRowsDev {
+    int32_t batch, T, dim, count, rows, rot_dim, adt, lpr;
+    float eps, interp;
+    const int32_t* counts;
+    const int32_t* parents;
+    int64_t parents_stride, angles_sb, angles_sn;
+    const void* angles;
+    const float* inv_freq;
+    DraftItemDev it[2 * PA_MAX_ORDER];
+};
+
+template <typename T>
+__global__ __launch_bounds__(kDraftThreads) void k_draft_append(const DraftRowsDev P) {
+    constexpr int E = 16 / sizeof(T);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int b = blockIdx.x / P.T, t = blockIdx.x % P.T;
+    const int sub = tid & (P.lpr - 1), d0 = sub * E;
+    const bool in = d0 < P.dim;
+    float cs[E], sn[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        cs[e] = 1.f;
+        sn[e] = 0.f;
+    }
+    if (P.rot_dim > 0) {
+        float pos = 0.f;
+        if (!P.angles) {  // the position as the rotary module builds it, rounded to the rows' type
+            const uint64_t anc = draft_ancestors(P.parents ? P.parents + b * P.parents_stride : nullptr,
+                                                 P.T, lane);
+            const int depth = __popcll(anc) - 1;
+            const int mine = max(0, __shfl(depth, t));
+            pos = round_to<T>(round_to<T>((float)(P.counts[b] + mine)) / P.interp);
+        }
+        const int64_t at = b * P.angles_sb + t * P.angles_sn;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (d0 + e < P.rot_dim) {
+                const float a = P.angles ? load_any(P.angles, P.adt, at + d0 + e)
+                                         : pos * P.inv_freq[(d0 + e) >> 1];
+                cs[e] = cosf(a);
+                sn[e] = sinf(a);
+            }
+    }
+    const int per = kDraftThreads / P.lpr;  // rows at a time
+    for (int row = blockIdx.y * per + tid / P.lpr; row - tid / P.lpr < P.rows; row += gridDim.y * per) {
+        const bool on = row < P.rows;
+        int k = 0;
+        while (k + 1 < P.count && row >= P.it[k + 1].row0) ++k;
+        const DraftItemDev& I = P.it[k];
+        const int h = (on ? row : P.rows - 1) - I.row0;
+        float x[E];
+        u32x4_d raw = {0u, 0u, 0u, 0u};
+        if (in) raw = load16u(I.src.at<T>(b, h) + t * I.src.sn + d0);
+        if constexpr (E == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(raw[e]);
+        } else {
+            typedef T t2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t word = raw[e];  // a value: a bit cast of the element itself reads element 0
+                const t2 y = __builtin_bit_cast(t2, word);
+                x[2 * e] = (float)y[0];
+                x[2 * e + 1] = (float)y[1];
+            }
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) ss += x[e] * x[e];
+        for (int off = 1; off < P.lpr; off <<= 1) ss += __shfl_xor(ss, off);
+        if (I.w && in) {
+            const float r = rsqrtf(ss / (float)P.dim + P.eps);
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = x[e] * r * load_any(I.w, I.wdt, d0 + e);
+        }
+        if (I.rotate && P.rot_dim > 0) {
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float y0 = x[e] * cs[e] - x[e + 1] * sn[e];
+                x[e + 1] = x[e + 1] * cs[e + 1] + x[e] * sn[e + 1];
+                x[e] = y0;
+            }
+        }
+        if (on && in) {
+            u32x4_d y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (E == 4) y[e] = __float_as_uint(x[e]);
+                else y[e] = draft_pack2<T>(x[2 * e], x[2 * e + 1]);
+            }
+            *reinterpret_cast<u32x4_d*>(I.out.at<T>(b, h) + t * I.out.sn + d0) = y;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// The kept nodes of a row, from their draft slots to the positions behind the cached ones.
+
+struct DraftCommitDev {
+    int32_t batch, kv_heads, slots, capacity, path_len;
+    const int32_t* path;
+    int64_t path_stride;
+    const int32_t* kept;
+    int32_t* counts;
+    int32_t* overflow;
+    pa_draft_move mv[PA_MAX_MOVES];
+};
+
+// entries of row b's path that are moved: up to the first one outside the slots, within the capacity
+__device__ __forceinline__ int commit_length(const DraftCommitDev& P, int b, int lane, int& n, bool& over) {
+    n = min(max(P.counts[b], 0), P.capacity);
+    const int want = min(max(P.kept[b], 0), P.path_len);
+    int bad = want;
+    if (lane < want) {
+        const int p = P.path[b * P.path_stride + lane];
+        if (p < 0 || p >= P.slots) bad = lane;
+    }
+    for (int off = 32; off > 0; off >>= 1) bad = min(bad, __shfl_xor(bad, off));
+    over = bad > P.capacity - n;
+    return min(bad, P.capacity - n);
+}
+
+__global__ __launch_bounds__(kDraftThreads) void k_draft_commit(const DraftCommitDev P) {
+    const int tid = threadIdx.x;
+    const int b = blockIdx.x / P.kv_heads;
+    int n;
+    bool over;
+    const int len = commit_length(P, b, tid & 63, n, over);
+    const pa_draft_move& M = P.mv[blockIdx.y];
+    const int64_t bh = blockIdx.x;
+    const char* src = static_cast<const char*>(M.src) + bh * P.slots * M.row_bytes;
+    char* dst = static_cast<char*>(M.dst) + (bh * P.capacity + n) * M.row_bytes;
+    if (M.row_bytes % 16 == 0) {
+        const int per = M.row_bytes / 16;
+        for (int x = tid; x < len * per; x += kDraftThreads) {
+            const int i = x / per, w = x % per;
+            reinterpret_cast<uint4*>(dst)[x] =
+                reinterpret_cast<const uint4*>(src + (int64_t)P.path[b * P.path_stride + i] * M.row_bytes)[w];
+        }
+    } else {
+        const int per = M.row_bytes / 4;
+        for (int x = tid; x < len * per; x += kDraftThreads) {
+            const int i = x / per, w = x % per;
+            reinterpret_cast<uint32_t*>(dst)[x] =
+                reinterpret_cast<const uint32_t*>(src + (int64_t)P.path[b * P.path_stride + i] * M.row_bytes)[w];
+        }
+    }
+}
+
+// the counts advance after every move has read them: a launch of its own
+__global__ __launch_bounds__(kDraftThreads) void k_draft_advance(const DraftCommitDev P) {
+    const int b = blockIdx.x * (kDraftThreads / 64) + (threadIdx.x >> 6);
+    if (b >= P.batch) return;
+    int n;
+    bool over;
+    const int len = commit_length(P, b, threadIdx.x & 63, n, over);
+    if ((threadIdx.x & 63) == 0) {
+        P.counts[b] = n + len;
+        if (over && P.overflow) *P.overflow = 1;
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// host side
+
+namespace {
+
+bool draft_dtype(int d) { return d == PA_F32 || d == PA_F16 || d == PA_BF16; }
+int draft_size(int dtype) { return dtype == PA_F32 ? 4 : 2; }
+
+// rows of 16-byte aligned starts (E elements); a stride of 0 broadcasts
+bool rows16(const pa_view& v) {
+    const int E = 16 / draft_size(v.dtype);
+    return (uintptr_t)v.ptr % 16 == 0 && v.sb % E == 0 && v.sh % E == 0 && v.sn % E == 0;
+}
+DraftRow draft_row(const pa_view& v) {
+    DraftRow r;
+    r.p = static_cast<char*>(v.ptr);
+    r.sb = v.sb;
+    r.sh = v.sh;
+    r.sn = v.sn;
+    return r;
+}
+
+// head dims: multiples of 8, of 16 above 128 (a lane's features are whole: dim / 16 of the padded dim)
+bool draft_dim(int d) { return d >= 8 && d <= 256 && d % 8 == 0 && (d <= 128 || d % 16 == 0); }
+
+constexpr int64_t kDraftGoal = 1024;  // workgroups of the partial launch aimed at
+
+// geometry shared by the workspace query and the launch; false where the request is malformed
+bool draft_plan(const pa_draft* d, DraftDev& P, int& units) {
+    if (d->batch < 1 || d->kv_heads < 1 || d->heads < 1 || d->heads % d->kv_heads != 0) return false;
+    if (d->drafts < 1 || d->drafts > PA_MAX_DRAFTS || d->order < 2 || d->order > PA_MAX_ORDER) return false;
+    if (d->capacity < 1 || !draft_dim(d->dim) || !draft_dtype(d->levels[0].k.dtype)) return false;
+    const int rep = d->heads / d->kv_heads;
+    if ((int64_t)rep * d->drafts > (1 << 20)) return false;
+    P.batch = d->batch;
+    P.kv_heads = d->kv_heads;
+    P.T = d->drafts;
+    P.dim = d->dim;
+    P.order = d->order;
+    P.capacity = d->capacity;
+    const bool f32 = d->levels[0].k.dtype == PA_F32;
+    const int D = d->dim <= 64 ? 64 : d->dim <= 128 ? 128 : 256;
+    const int tiles = f32 ? draft_row_tiles<float>(D) : draft_row_tiles<bf16>(D);
+    const int most = d->drafts * rep;
+    const int block = 16 * (most <= 16 ? 1 : std::min(tiles, most <= 32 ? 2 : 4));
+    P.row_blocks = (most + block - 1) / block;
+    P.rec_rows = d->drafts * (d->order - 1) + most;
+    const int64_t per = (int64_t)d->kv_heads * d->order * P.row_blocks;
+    int64_t target = std::max<int64_t>(1, kDraftGoal / per);
+    // no more units than the capacity has chunks
+    const int64_t chunks = ((int64_t)d->capacity + kDraftChunk - 1) / kDraftChunk * d->batch;
+    target = std::min(target, chunks);
+    P.target = (int)target;
+    units = (int)std::min(target + d->batch, chunks);
+    return (int64_t)d->kv_heads * P.row_blocks <= 65535;
+}
+
+size_t draft_ws_bytes(const DraftDev& P, int units) {
+    const size_t rec = (size_t)units * P.kv_heads * P.rec_rows;
+    return ((rec * P.dim * 4 + 255) & ~size_t(255)) + rec * sizeof(float2);
+}
+
+template <typename T>
+void launch_combine(const DraftDev& P, dim3 grid, size_t lds, hipStream_t s) {
+    if (P.dim <= 64) hipLaunchKernelGGL((k_draft_combine<T, 64>), grid, dim3(kDraftThreads), lds, s, P);
+    else if (P.dim <= 128) hipLaunchKernelGGL((k_draft_combine<T, 128>), grid, dim3(kDraftThreads), lds, s, P);
+    else hipLaunchKernelGGL((k_draft_combine<T, 256>), grid, dim3(kDraftThreads), lds, s, P);
+}
+
+}  // namespace
+
+size_t draft_attend_workspace(const pa_draft* d) {
+    DraftDev P;
+    int units = 0;
+    return draft_plan(d, P, units) ? draft_ws_bytes(P, units) : 0;
+}
+
+int launch_draft_attend(const pa_draft* d, hipStream_t s) {
+    if (d->batch < 1 || d->kv_heads < 1 || d->heads < 1 || d->heads % d->kv_heads != 0 ||
+        d->drafts < 1 || d->drafts > PA_MAX_DRAFTS || d->order < 2 || d->order > PA_MAX_ORDER ||
+        d->capacity < 1 || d->dim < 1 || !d->counts)
+        return PA_EINVAL;
+    const int T = d->levels[0].k.dtype;
+    if (!draft_dtype(T)) return PA_EINVAL;
+    if (!draft_dim(d->dim)) return PA_EUNSUPPORTED;
+    DraftDev P;
+    int units = 0;
+    if (!draft_plan(d, P, units)) return PA_EUNSUPPORTED;
+    if (!d->workspace || (uintptr_t)d->workspace % 16 != 0 ||
+        d->workspace_bytes < draft_ws_bytes(P, units))
+        return PA_EWORKSPACE;
+    P.scale = d->scale;
+    P.softclamp = d->softclamp > 0.f ? d->softclamp : 0.f;
+    P.counts = d->counts;
+    P.parents = d->parents;
+    P.parents_stride = d->parents_stride;
+    const size_t rec = (size_t)units * P.kv_heads * P.rec_rows;
+    P.ws_o = static_cast<float*>(d->workspace);
+    P.ws_s = reinterpret_cast<float2*>(static_cast<char*>(d->workspace) +
+                                       ((rec * P.dim * 4 + 255) & ~size_t(255)));
+    const int rep = d->heads / d->kv_heads;
+    bool vmul = false;
+    for (int t = 0; t < d->order; ++t) {
+        const pa_draft_level& l = d->levels[t];
+        const bool last = t == d->order - 1, middle = t > 0 && !last;
+        const int h = last ? d->heads : d->kv_heads;
+        auto need = [&](const pa_view& v, bool want, int heads, int dtype) {
+            if (!v.ptr) return !want;
+            return want && v.heads == heads && v.dtype == dtype;
+        };
+        if (!need(l.k, true, d->kv_heads, T) || !need(l.v, true, d->kv_heads, T) ||
+            !need(l.vmul, middle, d->kv_heads, T) || !need(l.bias, t > 0, d->kv_heads, PA_F32) ||
+            !need(l.q, true, h, T) || !need(l.dk, true, d->kv_heads, T) ||
+            !need(l.dv, !last, d->kv_heads, T) || !need(l.out, true, h, T) ||
+            !need(l.lse, !last, d->kv_heads, PA_F32))
+            return PA_EINVAL;
+        const pa_view* vecs[7] = {&l.k, &l.v, &l.vmul, &l.q, &l.dk, &l.dv, &l.out};
+        for (const pa_view* v : vecs)
+            if (v->ptr && !rows16(*v)) return PA_EUNSUPPORTED;
+        if ((l.bias.ptr && l.bias.sn != 1) || (l.lse.ptr && l.lse.sn != 1)) return PA_EUNSUPPORTED;
+        DraftLevelDev& L = P.L[t];
+        L.k = draft_row(l.k);
+        L.v = draft_row(l.v);
+        L.m = draft_row(l.vmul);
+        L.bias = draft_row(l.bias);
+        L.q = draft_row(l.q);
+        L.dk = draft_row(l.dk);
+        L.dv = draft_row(l.dv);
+        L.out = draft_row(l.out);
+        L.lse = draft_row(l.lse);
+        L.rep = last ? rep : 1;
+        L.rows = d->drafts * L.rep;
+        L.row0 = t * d->drafts;
+        vmul = vmul || middle;
+    }
+    {
+        ProfScope ps("draft_partial", s);
+        if (T == PA_F32) launch_draft_partial<float>(P, units, vmul, s);
+        else if (T == PA_F16) launch_draft_partial<f16>(P, units, vmul, s);
+        else launch_draft_partial<bf16>(P, units, vmul, s);
+    }
+    // columns per workgroup: few where the grid is small, all where it is not
+    const int blocks = (d->drafts * rep + 63) / 64;
+    P.cols = 16;
+    while (P.cols < 64 && P.cols < P.dim &&
+           (int64_t)P.batch * P.kv_heads * blocks * ((P.dim + P.cols - 1) / P.cols) > 2048)
+        P.cols *= 2;
+    const int T16 = (P.T + 15) & ~15;
+    const size_t lds = 4 * (((64 * (T16 + 1) + 3) & ~3) + 2 * (size_t)T16 * (P.cols + 4));
+    const dim3 grid(P.batch * P.kv_heads, (P.dim + P.cols - 1) / P.cols, blocks);
+    ProfScope ps("draft_combine", s);
+    if (T == PA_F32) launch_combine<float>(P, grid, lds, s);
+    else if (T == PA_F16) launch_combine<f16>(P, grid, lds, s);
+    else launch_combine<bf16>(P, grid, lds, s);
+    return PA_OK;
+}
+
+int launch_draft_append(const pa_draft_rows* r, hipStream_t s) {
+    if (r->batch < 1 || r->drafts < 1 || r->drafts > PA_MAX_DRAFTS || r->dim < 1 || r->count < 1 ||
+        r->count > 2 * PA_MAX_ORDER)
+        return PA_EINVAL;
+    const int T = r->items[0].src.dtype;
+    if (!draft_dtype(T)) return PA_EINVAL;
+    if (!draft_dim(r->dim)) return PA_EUNSUPPORTED;
+    const bool rotary = r->angles || r->inv_freq;
+    if (rotary && (r->rot_dim < 0 || r->rot_dim > r->dim || r->rot_dim % 2 != 0)) return PA_EINVAL;
+    if (r->angles && !draft_dtype(r->angles_dtype)) return PA_EINVAL;
+    if (!r->angles && r->inv_freq && (!(r->interp > 0.f) || !r->counts)) return PA_EINVAL;
+    DraftRowsDev P;
+    const int E = 16 / draft_size(T);
+    P.batch = r->batch;
+    P.T = r->drafts;
+    P.dim = r->dim;
+    P.count = r->count;
+    P.rot_dim = rotary ? r->rot_dim : 0;
+    P.adt = r->angles_dtype;
+    P.eps = r->eps;
+    P.interp = r->interp;
+    P.counts = r->counts;
+    P.parents = r->parents;
+    P.parents_stride = r->parents_stride;
+    P.angles_sb = r->angles_sb;
+    P.angles_sn = r->angles_sn;
+    P.angles = r->angles;
+    P.inv_freq = r->inv_freq;
+    P.lpr = 1;
+    while (P.lpr * E < r->dim) P.lpr <<= 1;
+    P.rows = 0;
+    for (int k = 0; k < r->count; ++k) {
+        const pa_draft_item& it = r->items[k];
+        if (!it.src.ptr || !it.out.ptr || it.src.heads < 1 || it.src.dtype != T || it.out.dtype != T ||
+            it.out.heads != it.src.heads || (it.norm_weight && !draft_dtype(it.weight_dtype)))
+            return PA_EINVAL;
+        if (!rows16(it.src) || !rows16(it.out)) return PA_EUNSUPPORTED;
+        DraftItemDev& I = P.it[k];
+        I.src = draft_row(it.src);
+        I.out = draft_row(it.out);
+        I.w = it.norm_weight;
+        I.wdt = it.weight_dtype;
+        I.rotate = it.rotate;
+        I.row0 = P.rows;
+        P.rows += it.src.heads;
+    }
+    const int per = kDraftThreads / P.lpr;
+    const int64_t nodes = (int64_t)r->batch * r->drafts;
+    if (nodes > (1 << 30)) return PA_EUNSUPPORTED;
+    // parts of a node's rows: enough workgroups to fill the GPU, each with at least one sweep of rows
+    int parts = (int)std::max<int64_t>(1, std::min<int64_t>((P.rows + per - 1) / per, 1024 / nodes));
+    const dim3 grid((unsigned)nodes, parts);
+    ProfScope ps("draft_append", s);
+    if (T == PA_F32) hipLaunchKernelGGL((k_draft_append<float>), grid, dim3(kDraftThreads), 0, s, P);
+    else if (T == PA_F16) hipLaunchKernelGGL((k_draft_append<f16>), grid, dim3(kDraftThreads), 0, s, P);
+    else hipLaunchKernelGGL((k_draft_append<bf16>), grid, dim3(kDraftThreads), 0, s, P);
+    return PA_OK;
+}
+
+int launch_draft_commit(const pa_commit* c, hipStream_t s) {
+    if (c->batch < 1 || c->kv_heads < 1 || c->slots < 1 || c->slots > PA_MAX_DRAFTS || c->capacity < 1 ||
+        c->count < 0 || c->count > PA_MAX_MOVES || c->path_len < 0 || c->path_len > PA_MAX_DRAFTS ||
+        !c->path || !c->kept || !c->counts)
+        return PA_EINVAL;
+    if ((int64_t)c->batch * c->kv_heads > (1 << 30)) return PA_EUNSUPPORTED;
+    DraftCommitDev P;
+    P.batch = c->batch;
+    P.kv_heads = c->kv_heads;
+    P.slots = c->slots;
+    P.capacity = c->capacity;
+    P.path_len = c->path_len;
+    P.path = c->path;
+    P.path_stride = c->path_stride;
+    P.kept = c->kept;
+    P.counts = c->counts;
+    P.overflow = c->overflow;
+    for (int k = 0; k < c->count; ++k) {
+        const pa_draft_move& m = c->moves[k];
+        const int a = m.row_bytes % 16 == 0 ? 16 : 4;
+        if (!m.src || !m.dst || m.row_bytes < 4 || m.row_bytes % 4 != 0 || (uintptr_t)m.src % a != 0 ||
+            (uintptr_t)m.dst % a != 0)
+            return PA_EINVAL;
+        P.mv[k] = m;
+    }
+    if (c->count > 0) {
+        ProfScope ps("draft_commit", s);
+        hipLaunchKernelGGL(k_draft_commit, dim3(c->batch * c->kv_heads, c->count), dim3(kDraftThreads), 0, s, P);
+    }
+    if (c->advance) {
+        ProfScope ps("draft_advance", s);
+        constexpr int per = kDraftThreads / 64;
+        hipLaunchKernelGGL(k_draft_advance, dim3((c->batch + per - 1) / per), dim3(kDraftThreads), 0, s, P);
+    }
+    return PA_OK;
+}
+
+}  // namespace pa

@@ -1,0 +1,6 @@
+// pa_draft_f16.hip -- k_draft_partial for f16 (a source file of its own: compile time).
+#include "pa_draft_partial.h"
+
+namespace pa {
+template void launch_draft_partial<f16>(const DraftDev& P, int units, bool vmul, hipStream_t s);
+}  // namespace pa

@@ -1,0 +1,353 @@
+// pa_draft_partial.h -- k_draft_partial: the cached positions of a drafted step.
+//
+// One workgroup per (unit of positions, key head and block of rows, level), four waves, each on its
+// own 32 (fp32: 16) positions at a time; nothing is shared until the end, so there is no barrier in
+// the loop and no LDS between memory and the matrix cores.
+//
+// S^T = K Q^T with 16x16 tiles (A: 16 positions, lane l holds position l % 16; B: 16 rows): lane l =
+// 16 g + c gets row c and the positions 4 g .. 4 g + 3 of a tile.  A second product over those
+// positions, O^T = V^T P^T, wants from lane l row c and the positions of group g: exactly the
+// probabilities it holds, if V^T's operand takes the same positions.  So a lane loads, for its
+// group's eight positions (4 g + e of both tiles), the dim / 16 features it owns: 16 lanes cover a
+// whole row, and the transposition that the operand needs is inside the lane (one v_perm_b32 for
+// two values).  fp32 takes v_mfma_f32_16x16x4_f32, whose operands are single values: no
+// transposition at all.  In O^T a lane holds one row, so the running maximum's rescale is one
+// factor per lane; it moves only past kDraftTau (lazy), so exp2(s - m) is at most 2^8.
+#pragma once
+
+#include "pa_draft.h"
+
+namespace pa {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_d __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_d __attribute__((ext_vector_type(2)));
+
+template <typename T> struct Mma16;
+template <> struct Mma16<bf16> {
+    typedef __bf16 frag __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x4_t run(u32x4_d a, u32x4_d b, f32x4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(frag, a),
+                                                       __builtin_bit_cast(frag, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mma16<f16> {
+    typedef _Float16 frag __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x4_t run(u32x4_d a, u32x4_d b, f32x4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(frag, a),
+                                                      __builtin_bit_cast(frag, b), c, 0, 0, 0);
+    }
+};
+__device__ __forceinline__ f32x4_t mma_f32(uint32_t a, uint32_t b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a), __uint_as_float(b), c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t draft_pack2(float lo, float hi) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    const f2 v = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, t2));
+}
+// two 16-bit products, each rounded
+template <typename T>
+__device__ __forceinline__ uint32_t draft_mul2(uint32_t a, uint32_t b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    const f2 x = __builtin_convertvector(__builtin_bit_cast(t2, a), f2);
+    const f2 y = __builtin_convertvector(__builtin_bit_cast(t2, b), f2);
+    return draft_pack2<T>(x[0] * y[0], x[1] * y[1]);
+}
+
+__device__ __forceinline__ u32x4_d load16u(const void* p) { return *reinterpret_cast<const u32x4_d*>(p); }
+
+// Fragment geometry of a head dim padded to D: S words of a row's contraction per lane, W words of
+// values per lane and position.
+template <typename T, int D> struct DraftGeo {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int KT = F32 ? 1 : 2;         // 16-position tiles per step
+    static constexpr int NP = 4 * KT;              // a lane's positions per step
+    static constexpr int KS = F32 ? D / 16 : D / 32;  // 16-byte loads of a key row per lane
+    static constexpr int VE = D / 16;              // features per lane of a value row
+    static constexpr int VW = F32 ? VE : VE / 2;   // the same in 32-bit words
+    static constexpr int KE = F32 ? 4 : 8;         // elements of a 16-byte load
+};
+
+// a value row's features VE*c .. of one position
+template <int VW>
+__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[VW]) {
+    if constexpr (VW == 2) {
+        const u32x2_d x = *reinterpret_cast<const u32x2_d*>(p);
+        w[0] = x[0];
+        w[1] = x[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < VW; i += 4) {
+            const u32x4_d x = load16u(static_cast<const char*>(p) + 4 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[i + j] = x[j];
+        }
+    }
+}
+
+template <typename T, int D, int RT, bool VM>
+__global__ __launch_bounds__(kDraftThreads) void k_draft_partial(const DraftDev P) {
+    typedef DraftGeo<T, D> G;
+    constexpr int KT = G::KT, NP = G::NP, KS = G::KS, VE = G::VE, VW = G::VW, KE = G::KE;
+    constexpr int PITCH = D + 4;
+    __shared__ float s_o[16 * RT * PITCH];
+    __shared__ float s_m[4][16 * RT], s_l[4][16 * RT];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int hk = blockIdx.y / P.row_blocks, r0 = (blockIdx.y % P.row_blocks) * 16 * RT;
+    const DraftLevelDev& L = P.L[blockIdx.z];
+    if (r0 >= L.rows) return;
+    const int64_t size = draft_unit_size(P, lane);
+    int b = 0, place = 0;
+    if (!draft_find_unit(P, size, blockIdx.x, lane, b, place)) return;
+    b = __builtin_amdgcn_readfirstlane(b);
+    place = __builtin_amdgcn_readfirstlane(place);
+    const int len = draft_count(P, b);
+    const int64_t begin = place * size;
+    const int cnt = (int)(len - begin < size ? len - begin : size);  // >= 1
+    const int nrows = min(16 * RT, L.rows - r0);
+    const int nrt = (nrows + 15) / 16;
+
+    // the queries: row r of the block is node r % T of the group's head r / T
+    u32x4_d qf[RT][KS];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = min(r0 + 16 * rt + c, L.rows - 1);
+        const T* row = L.q.at<T>(b, hk * L.rep + r / P.T) + (int64_t)(r % P.T) * L.q.sn;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = (KE * 4) * s + KE * g;
+            qf[rt][s] = d < P.dim ? load16u(row + d) : u32x4_d{0u, 0u, 0u, 0u};
+        }
+    }
+    f32x4_t o[RT][VE];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt] = -INFINITY;
+        l[rt] = 0.f;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) o[rt][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const T* kb = L.k.at<T>(b, hk) + begin * L.k.sn;
+    const T* vb = L.v.at<T>(b, hk) + begin * L.v.sn;
+    const T* mb = VM && L.m.p ? L.m.at<T>(b, hk) + begin * L.m.sn : nullptr;
+    const float* bias = L.bias.p ? L.bias.at<float>(b, hk) + begin : nullptr;
+    const float sl2 = P.scale * kLog2e, cl2 = P.softclamp * kLog2e;
+    const float cinv = P.softclamp > 0.f ? P.scale / P.softclamp : 0.f;
+    // Features past the head dim (one that is not D): the loads fall back to the row's last 16
+    // bytes; the queries are 0 there, and those columns of the output are not stored.
+    int kd[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) kd[s] = min((KE * 4) * s + KE * g, P.dim - KE);
+    const int vd = min(VE * c, P.dim - VE);  // dim is a multiple of 8 (fp32: 4), and see the host
+
+    const int steps = (cnt + 64 * KT - 1) / (64 * KT);  // the workgroup's: 4 waves x KT tiles
+    for (int st = 0; st < steps; ++st) {
+        const int j0 = (4 * st + wave) * 16 * KT;
+        if (j0 >= cnt) break;
+        // positions past the unit's end read its last one; their scores become -inf
+        u32x4_d kf[KT][KS];
+        uint32_t v[NP][VW];
+        float bz[KT][4];
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            const T* row = kb + (int64_t)min(j0 + 16 * t + c, cnt - 1) * L.k.sn;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) kf[t][s] = load16u(row + kd[s]);
+        }
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t j = min(j0 + 16 * t + 4 * g + i, cnt - 1);
+                load_words<VW>(vb + j * L.v.sn + vd, v[4 * t + i]);
+                bz[t][i] = bias ? bias[j] * kLog2e : 0.f;
+                if constexpr (VM) {
+                    if (mb) {
+                        uint32_t x[VW];
+                        load_words<VW>(mb + j * L.m.sn + vd, x);
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) {
+                            if constexpr (G::F32)
+                                v[4 * t + i][w] = __float_as_uint(__uint_as_float(v[4 * t + i][w]) *
+                                                                  __uint_as_float(x[w]));
+                            else
+                                v[4 * t + i][w] = draft_mul2<T>(v[4 * t + i][w], x[w]);
+                        }
+                    }
+                }
+            }
+        // scores and probabilities
+        uint32_t pf[RT][4];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            if (rt >= nrt) break;
+            float x[KT][4];
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    if constexpr (G::F32) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) a = mma_f32(kf[t][s][j], qf[rt][s][j], a);
+                    } else {
+                        a = Mma16<T>::run(kf[t][s], qf[rt][s], a);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float y = P.softclamp > 0.f ? cl2 * tanhf(a[i] * cinv) : a[i] * sl2;
+                    x[t][i] = j0 + 16 * t + 4 * g + i < cnt ? y + bz[t][i] : -INFINITY;
+                }
+            }
+            float top = x[0][0];
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, x[t][i]);
+            if (__any(top > m[rt] + kDraftTau)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float mn = fmaxf(m[rt], top);
+                const float al = mn == m[rt] ? 1.f : __builtin_amdgcn_exp2f(m[rt] - mn);
+                m[rt] = mn;
+                l[rt] *= al;
+#pragma unroll
+                for (int j = 0; j < VE; ++j) o[rt][j] *= al;
+            }
+            const float ms = m[rt] == -INFINITY ? 0.f : m[rt];
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[t][i] = __builtin_amdgcn_exp2f(x[t][i] - ms);
+                    l[rt] += x[t][i];
+                }
+            if constexpr (G::F32) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pf[rt][i] = __float_as_uint(x[0][i]);
+            } else {
+                // rounded to the value type for the product: 2^-9 of a term, averaged over the row
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    pf[rt][2 * t] = draft_pack2<T>(x[t][0], x[t][1]);
+                    pf[rt][2 * t + 1] = draft_pack2<T>(x[t][2], x[t][3]);
+                }
+            }
+        }
+        // O^T += V^T P^T, feature j of every lane's VE per tile
+#pragma unroll
+        for (int j = 0; j < VE; ++j) {
+            if constexpr (G::F32) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    if (rt >= nrt) break;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[rt][j] = mma_f32(v[i][j], pf[rt][i], o[rt][j]);
+                }
+            } else {
+                const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
+                u32x4_d a;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    a[e] = __builtin_amdgcn_perm(v[2 * e + 1][j / 2], v[2 * e][j / 2], sel);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    if (rt >= nrt) break;
+                    o[rt][j] = Mma16<T>::run(a, u32x4_d{pf[rt][0], pf[rt][1], pf[rt][2], pf[rt][3]},
+                                             o[rt][j]);
+                }
+            }
+        }
+    }
+
+    // join the four waves: maxima and sums first, then the outputs one wave after another
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        l[rt] += __shfl_xor(l[rt], 16);
+        l[rt] += __shfl_xor(l[rt], 32);
+        if (g == 0) {
+            s_m[wave][16 * rt + c] = m[rt];
+            s_l[wave][16 * rt + c] = l[rt];
+        }
+    }
+    __syncthreads();
+    float f[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        float top = s_m[0][16 * rt + c];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][16 * rt + c]);
+        f[rt] = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - top);
+    }
+    for (int w = 0; w < 4; ++w) {
+        if (wave == w) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < VE; j += 4) {
+                        float4* at = reinterpret_cast<float4*>(&s_o[(16 * rt + c) * PITCH + VE * (4 * g + i) + j]);
+                        float4 x = w ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+                        x.x += f[rt] * o[rt][j][i];
+                        x.y += f[rt] * o[rt][j + 1][i];
+                        x.z += f[rt] * o[rt][j + 2][i];
+                        x.w += f[rt] * o[rt][j + 3][i];
+                        *at = x;
+                    }
+        }
+        __syncthreads();
+    }
+    const int64_t rec = ((int64_t)blockIdx.x * P.kv_heads + hk) * P.rec_rows + L.row0 + r0;
+    if (tid < nrows) {
+        float top = s_m[0][tid], sum = 0.f;
+        for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][tid]);
+        for (int w = 0; w < 4; ++w)
+            sum += s_m[w][tid] == -INFINITY ? 0.f : s_l[w][tid] * __builtin_amdgcn_exp2f(s_m[w][tid] - top);
+        P.ws_s[rec + tid] = make_float2(top, sum);
+    }
+    const int quads = P.dim / 4;
+    for (int x = tid; x < nrows * quads; x += kDraftThreads) {
+        const int r = x / quads, d = x % quads * 4;
+        *reinterpret_cast<float4*>(P.ws_o + (rec + r) * P.dim + d) =
+            *reinterpret_cast<const float4*>(&s_o[r * PITCH + d]);
+    }
+}
+
+template <typename T, int D, int RT>
+void launch_draft_partial_rt(const DraftDev& P, int units, bool vmul, hipStream_t s) {
+    const dim3 grid(units, P.kv_heads * P.row_blocks, P.order);
+    if (vmul) hipLaunchKernelGGL((k_draft_partial<T, D, RT, true>), grid, dim3(kDraftThreads), 0, s, P);
+    else hipLaunchKernelGGL((k_draft_partial<T, D, RT, false>), grid, dim3(kDraftThreads), 0, s, P);
+}
+
+template <typename T, int D>
+void launch_draft_partial_d(const DraftDev& P, int units, bool vmul, hipStream_t s) {
+    int rows = 0;
+    for (int t = 0; t < P.order; ++t) rows = P.L[t].rows > rows ? P.L[t].rows : rows;
+    constexpr int most = draft_row_tiles<T>(D);
+    if (rows <= 16 || most == 1) return launch_draft_partial_rt<T, D, 1>(P, units, vmul, s);
+    if constexpr (most >= 2)
+        if (rows <= 32 || most == 2) return launch_draft_partial_rt<T, D, 2>(P, units, vmul, s);
+    if constexpr (most >= 4) launch_draft_partial_rt<T, D, 4>(P, units, vmul, s);
+}
+
+template <typename T>
+void launch_draft_partial(const DraftDev& P, int units, bool vmul, hipStream_t s) {
+    if (P.dim <= 64) launch_draft_partial_d<T, 64>(P, units, vmul, s);
+    else if (P.dim <= 128) launch_draft_partial_d<T, 128>(P, units, vmul, s);
+    else launch_draft_partial_d<T, 256>(P, units, vmul, s);
+}
+
+}  // namespace pa

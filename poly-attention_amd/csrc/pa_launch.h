@@ -76,6 +76,13 @@ size_t rms_many_workspace(const pa_rmsnorm* items, int count);
 int launch_rms_many(const pa_rmsnorm* items, int count, bool bwd, hipStream_t s);
 size_t rms_bwd_workspace(const pa_rmsnorm* p);
 int launch_rms_bwd(const pa_rmsnorm* p, hipStream_t s);
+// drafted tokens
+size_t draft_attend_workspace(const pa_draft* d);
+int launch_draft_attend(const pa_draft* d, hipStream_t s);
+int launch_draft_append(const pa_draft_rows* r, hipStream_t s);
+int launch_draft_commit(const pa_commit* c, hipStream_t s);
+size_t draft_verify_workspace(const pa_verify* v);
+int launch_draft_verify(const pa_verify* v, hipStream_t s);
 int launch_linear_small(const pa_linear* l, hipStream_t s);
 int launch_linear_rows(const pa_linear* l, hipStream_t s);
 

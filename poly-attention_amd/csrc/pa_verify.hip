@@ -1,0 +1,443 @@
+// pa_verify.hip -- the walk of drafted tokens against the target's probabilities.
+//
+// Two launches.  k_verify_stats reads every node's logits once: per chunk of the vocabulary the
+// maximum, its first position and the sum of exp(x - max), a chunk held in registers between the
+// two.  k_verify_walk runs one workgroup per (row, chunk): each joins the chunks' statistics and
+// walks the row's tree for itself (a few values per node; the same result in every workgroup, so
+// none waits for another), then takes its chunk of the last node's distribution for the token; the
+// workgroup that finishes a row last joins the chunks.
+//
+// The token is the largest p_i / noise_i: one pass, no cumulative sums, and p's common factor drops
+// out.  Only a test of a further child after a rejection needs the residual's sum; without a draft
+// distribution that is 1 - (rejected probabilities), with one a pass over the row.
+#include "pa_draft.h"
+
+namespace pa {
+
+namespace {
+
+constexpr int kVerThreads = 256;
+constexpr int kVerChunk = 8192;  // entries of a workgroup: 32 per thread, held in registers
+
+struct VerifyDev {
+    int32_t batch, T, vocab, chunks;
+    const void* logits;
+    int64_t logits_sb, logits_sn;
+    const int64_t* tokens;
+    int64_t tokens_stride;
+    const int32_t* parents;
+    int64_t parents_stride;
+    const float* uniforms;
+    int64_t uniforms_stride;
+    const float* noise;
+    int64_t noise_stride;
+    const float* temperature;
+    const float* probs;
+    int64_t probs_sb, probs_sn;
+    int32_t* path;
+    int32_t* kept;
+    int64_t* token;
+    float4* stats;       // [B][T][chunks]: maximum, sum, first position of the maximum (as bits)
+    uint64_t* best;      // [B][chunks][2]
+    uint32_t* ticket;    // [B]
+};
+
+__device__ __forceinline__ float row_temperature(const VerifyDev& P, int b) {
+    if (!P.uniforms) return 0.f;
+    const float t = P.temperature ? P.temperature[b] : 1.f;
+    return t > 0.f ? t : 0.f;
+}
+
+// the larger value, the lower position of equals; NaN loses
+__device__ __forceinline__ void take_first(float& x, int& i, float y, int j) {
+    if (y > x || (y == x && j < i)) {
+        x = y;
+        i = j;
+    }
+}
+
+// Entry `32-entry group` access: vector k of thread tid covers E entries of the 16-byte aligned run
+// that holds the row, so an unaligned row costs a few masked entries at its ends and no more.
+template <typename T> struct VerVec {
+    static constexpr int E = 16 / sizeof(T);
+    static constexpr int N = kVerChunk / (kVerThreads * E);
+};
+
+// E entries of a row of n, starting at entry i (which may be negative or past the end), as floats;
+// entries outside are `fill`.  `row + i` is 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void load_entries(const T* row, int64_t i, int n, float fill,
+                                             float (&x)[VerVec<T>::E]) {
+    constexpr int E = VerVec<T>::E;
+    if (i >= 0 && i + E <= n) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(row + i);
+        const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int k = 0; k < E; ++k) x[k] = to_f(e[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < E; ++k) x[k] = i + k >= 0 && i + k < n ? to_f(row[i + k]) : fill;
+    }
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+    for (int off = 32; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off));
+    return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off);
+    return x;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kVerThreads) void k_verify_stats(const VerifyDev P) {
+    constexpr int E = VerVec<T>::E, N = VerVec<T>::N;
+    __shared__ float s_x[4], s_sum[4];
+    __shared__ int s_i[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int chunk = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
+    if (chunk == 0 && t == 0 && tid == 0) P.ticket[b] = 0;  // before the walk's launch begins
+    const float temp = row_temperature(P, b);
+    const T* row = reinterpret_cast<const T*>(P.logits) + b * P.logits_sb + t * P.logits_sn;
+    const int shift = (int)(((uintptr_t)row & 15) / sizeof(T));  // entries before the row in its run
+    const int64_t i0 = (int64_t)chunk * kVerChunk - shift;
+    float x[N][E];
+    float top = -INFINITY;
+    int at = P.vocab;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int64_t i = i0 + (int64_t)(k * kVerThreads + tid) * E;
+        load_entries<T>(row, i, P.vocab, -INFINITY, x[k]);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (x[k][e] > top) {
+                top = x[k][e];
+                at = (int)(i + e);
+            }
+    }
+    for (int off = 32; off > 0; off >>= 1) take_first(top, at, __shfl_xor(top, off), __shfl_xor(at, off));
+    if (lane == 0) {
+        s_x[wave] = top;
+        s_i[wave] = at;
+    }
+    __syncthreads();
+    top = s_x[0];
+    at = s_i[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) take_first(top, at, s_x[w], s_i[w]);
+    float sum = 0.f;
+    if (temp > 0.f) {
+        const float c = kLog2e / temp, base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum += __builtin_amdgcn_exp2f((x[k][e] - base) * c);
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) s_sum[wave] = sum;
+    __syncthreads();
+    if (tid == 0)
+        P.stats[((int64_t)b * P.T + t) * P.chunks + chunk] =
+            make_float4(top, s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3], __int_as_float(at), 0.f);
+}
+
+// the residual after `n` rejections of one entry's probability p with draft probability q: inv[k] is
+// one over the sum of the k-th residual, 0 where that sum was 0 (p stays as it was)
+__device__ __forceinline__ float residual(float p, float q, const float* inv, int n) {
+    for (int k = 0; k < n; ++k) p = inv[k] != 0.f ? fmaxf(p - q, 0.f) * inv[k] : p;
+    return p;
+}
+
+__device__ __forceinline__ uint64_t best_key(float w, float noise, int64_t i) {
+    if (!(w > 0.f)) return 0;
+    const float key = w / noise;
+    if (!(key >= 0.f)) return 0;
+    // +1: a key of 0 (underflow) still is a candidate
+    return ((uint64_t)(__float_as_uint(key) + 1u) << 32) | (0xffffffffu - (uint32_t)i);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) {
+    constexpr int E = VerVec<T>::E, N = VerVec<T>::N;
+    __shared__ float s_top[64], s_inv[64], s_px[64], s_qx[64], s_u[64], s_rinv[64];
+    __shared__ int s_arg[64], s_parent[64], s_path[64], s_rej[64];
+    __shared__ int64_t s_tok[64];
+    __shared__ uint64_t s_live, s_best[4][2];
+    __shared__ float s_wave[4];
+    __shared__ int s_last;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int chunk = blockIdx.x, b = blockIdx.y;
+    const float temp = row_temperature(P, b);
+    const bool greedy = !(temp > 0.f);
+    const float c = greedy ? 0.f : kLog2e / temp;
+    const int32_t* parents = P.parents ? P.parents + b * P.parents_stride : nullptr;
+
+    // the nodes: statistics over the chunks (four threads each), tokens, random numbers
+    {
+        const int t = tid >> 2, sub = tid & 3;
+        float top = -INFINITY, sum = 0.f;
+        int at = P.vocab;
+        if (t < P.T) {
+            const float4* st = P.stats + ((int64_t)b * P.T + t) * P.chunks;
+            for (int k = sub; k < P.chunks; k += 4) take_first(top, at, st[k].x, __float_as_int(st[k].z));
+        }
+        for (int off = 1; off < 4; off <<= 1) take_first(top, at, __shfl_xor(top, off), __shfl_xor(at, off));
+        if (t < P.T && !greedy) {
+            const float4* st = P.stats + ((int64_t)b * P.T + t) * P.chunks;
+            for (int k = sub; k < P.chunks; k += 4)
+                sum += st[k].x == -INFINITY ? st[k].y  // 0, or NaN
+                                            : st[k].y * __builtin_amdgcn_exp2f((st[k].x - top) * c);
+        }
+        sum += __shfl_xor(sum, 1);
+        sum += __shfl_xor(sum, 2);
+        if (t < P.T && sub == 0) {
+            s_top[t] = top;
+            s_inv[t] = 1.f / sum;
+            s_arg[t] = at;
+            s_parent[t] = parents ? parents[t] : t - 1;
+            s_tok[t] = P.tokens[b * P.tokens_stride + t];
+            s_u[t] = greedy ? 0.f : P.uniforms[b * P.uniforms_stride + t];
+        }
+    }
+    if (wave == 0) {
+        const uint64_t anc = draft_ancestors(parents, P.T, lane);
+        const uint64_t live = __ballot(anc != 0);
+        if (lane == 0) s_live = live;
+    }
+    __syncthreads();
+    const uint64_t live = s_live;
+    // each node's own probabilities under its parent
+    if (tid < P.T) {
+        const int p = s_parent[tid];
+        const int64_t tok = s_tok[tid];
+        float px = 0.f, qx = 1.f;
+        if (((live >> tid) & 1) && p >= 0 && tok >= 0 && tok < P.vocab) {
+            if (greedy) {
+                px = tok == s_arg[p] ? 1.f : 0.f;
+            } else {
+                const float x = to_f(reinterpret_cast<const T*>(P.logits)[b * P.logits_sb + p * P.logits_sn + tok]);
+                px = __builtin_amdgcn_exp2f((x - s_top[p]) * c) * s_inv[p];
+            }
+            if (P.probs) qx = P.probs[b * P.probs_sb + p * P.probs_sn + tok];
+        }
+        s_px[tid] = px;
+        s_qx[tid] = qx;
+    }
+    __syncthreads();
+
+    // the walk, the same in every thread
+    int cur = 0, kept = live & 1 ? 1 : 0, nrej = 0;  // rejected children of cur
+    float left = 1.f;                                 // without probs: 1 - their probabilities
+    if (tid == 0) s_path[0] = kept ? 0 : -1;
+    const T* row = reinterpret_cast<const T*>(P.logits) + b * P.logits_sb;
+    const float* qrow = P.probs ? P.probs + b * P.probs_sb : nullptr;
+    for (int t = 1; kept && t < P.T; ++t) {
+        if (!((live >> t) & 1) || s_parent[t] != cur) continue;
+        const int64_t tok = s_tok[t];
+        float px = s_px[t], qx = s_qx[t];
+        if (!greedy && nrej > 0) {
+            if (P.probs) {
+                // the sum of the newest residual, now that a further child needs it
+                float part = 0.f;
+                for (int64_t i = tid; i < P.vocab; i += kVerThreads) {
+                    const float p = __builtin_amdgcn_exp2f((to_f(row[cur * P.logits_sn + i]) - s_top[cur]) * c) * s_inv[cur];
+                    const float q = qrow[cur * P.probs_sn + i];
+                    part += fmaxf(residual(p, q, s_rinv, nrej - 1) - q, 0.f);
+                }
+                part = wave_sum(part);
+                __syncthreads();
+                if (lane == 0) s_wave[wave] = part;
+                __syncthreads();
+                const float sum = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
+                if (tid == 0) s_rinv[nrej - 1] = sum > 0.f ? 1.f / sum : 0.f;
+                __syncthreads();
+                px = tok >= 0 && tok < P.vocab ? residual(px, qx, s_rinv, nrej) : 0.f;
+            } else {
+                for (int k = 0; k < nrej; ++k)
+                    if (s_tok[s_rej[k]] == tok) px = 0.f;
+                px /= left;
+            }
+        }
+        if (s_u[t] * qx < px) {
+            cur = t;
+            if (tid == 0) s_path[kept] = t;
+            ++kept;
+            nrej = 0;
+            left = 1.f;
+        } else if (!greedy) {
+            if (P.probs) {
+                ++nrej;
+            } else if (px > 0.f) {
+                // removed from p, unless it was all of p
+                const float rest = left - px * left;
+                if (rest > 0.f) {
+                    if (tid == 0) s_rej[nrej] = t;
+                    ++nrej;
+                    left = rest;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    __syncthreads();
+    if (chunk == 0) {
+        for (int t = tid; t < P.T; t += kVerThreads) P.path[(int64_t)b * P.T + t] = t < kept ? s_path[t] : -1;
+        if (tid == 0) P.kept[b] = kept;
+    }
+    if (!kept || greedy) {
+        if (chunk == 0 && tid == 0)
+            P.token[b] = kept && s_arg[cur] < P.vocab ? (int64_t)s_arg[cur] : (int64_t)-1;
+        return;
+    }
+
+    // this chunk of the last node's distribution.  With probs the last rejection's residual is taken
+    // without its sum (a common factor); `alt` is the candidate before it, for a sum of 0.
+    row += cur * P.logits_sn;
+    const float top = s_top[cur], inv = s_inv[cur];
+    const float* q = P.probs && nrej > 0 ? qrow + cur * P.probs_sn : nullptr;
+    const float* noise = P.noise + b * P.noise_stride;
+    const int shift = (int)(((uintptr_t)row & 15) / sizeof(T));
+    const int64_t i0 = (int64_t)chunk * kVerChunk - shift;
+    uint64_t best = 0, alt = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int64_t i = i0 + (int64_t)(k * kVerThreads + tid) * E;
+        if (i >= P.vocab) continue;
+        float x[E];
+        load_entries<T>(row, i, P.vocab, -INFINITY, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int64_t j = i + e;
+            if (j < 0 || j >= P.vocab) continue;
+            float w = __builtin_amdgcn_exp2f((x[e] - top) * c) * inv;
+            const float nz = noise[j];
+            uint64_t key;
+            if (q) {
+                const float qj = q[j];
+                w = residual(w, qj, s_rinv, nrej - 1);
+                key = best_key(w, nz, j);
+                alt = key > alt ? key : alt;
+                w = fmaxf(w - qj, 0.f);
+            } else {
+                for (int r = 0; r < nrej; ++r)
+                    if (s_tok[s_rej[r]] == j) w = 0.f;
+            }
+            key = best_key(w, nz, j);
+            best = key > best ? key : best;
+        }
+    }
+    for (int off = 32; off > 0; off >>= 1) {
+        const uint64_t y = __shfl_xor((unsigned long long)best, off), z = __shfl_xor((unsigned long long)alt, off);
+        best = y > best ? y : best;
+        alt = z > alt ? z : alt;
+    }
+    if (lane == 0) {
+        s_best[wave][0] = best;
+        s_best[wave][1] = alt;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < 4; ++w) {
+            best = s_best[w][0] > best ? s_best[w][0] : best;
+            alt = s_best[w][1] > alt ? s_best[w][1] : alt;
+        }
+        uint64_t* to = P.best + ((int64_t)b * P.chunks + chunk) * 2;
+        __hip_atomic_store(to, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(to + 1, alt, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // the release orders the two stores before the ticket, the acquire the others' before the reads
+        const uint32_t n = __hip_atomic_fetch_add(P.ticket + b, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        s_last = n == (uint32_t)P.chunks - 1;
+    }
+    __syncthreads();
+    if (!s_last || wave != 0) return;
+    best = 0;
+    alt = 0;
+    for (int k = lane; k < P.chunks; k += 64) {
+        uint64_t* from = P.best + ((int64_t)b * P.chunks + k) * 2;
+        const uint64_t y = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint64_t z = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        best = y > best ? y : best;
+        alt = z > alt ? z : alt;
+    }
+    for (int off = 32; off > 0; off >>= 1) {
+        const uint64_t y = __shfl_xor((unsigned long long)best, off), z = __shfl_xor((unsigned long long)alt, off);
+        best = y > best ? y : best;
+        alt = z > alt ? z : alt;
+    }
+    if (lane == 0) {
+        const uint64_t pick = best ? best : alt;
+        P.token[b] = pick ? (int64_t)(0xffffffffu - (uint32_t)pick) : (int64_t)-1;
+    }
+}
+
+int verify_chunks(const pa_verify* v) {
+    // a row's 16-byte aligned run may begin up to 7 entries before the row
+    return (int)(((int64_t)v->vocab + 7 + kVerChunk - 1) / kVerChunk);
+}
+
+bool verify_sizes(const pa_verify* v) {
+    return v->batch >= 1 && v->batch <= 65535 && v->drafts >= 1 && v->drafts <= PA_MAX_DRAFTS &&
+           v->vocab >= 1 && v->vocab <= (1 << 30);
+}
+
+}  // namespace
+
+size_t draft_verify_workspace(const pa_verify* v) {
+    if (!verify_sizes(v)) return 0;
+    const size_t chunks = verify_chunks(v), b = v->batch;
+    return b * v->drafts * chunks * sizeof(float4) + b * chunks * 16 + b * 4;
+}
+
+int launch_draft_verify(const pa_verify* v, hipStream_t s) {
+    if (!verify_sizes(v)) return v->batch > 65535 || v->vocab > (1 << 30) ? PA_EUNSUPPORTED : PA_EINVAL;
+    if (v->dtype != PA_F32 && v->dtype != PA_F16 && v->dtype != PA_BF16) return PA_EINVAL;
+    if (!v->logits || !v->tokens || !v->path || !v->kept || !v->token || (v->uniforms && !v->noise) ||
+        (uintptr_t)v->logits % (v->dtype == PA_F32 ? 4 : 2) != 0)
+        return PA_EINVAL;
+    if (!v->workspace || (uintptr_t)v->workspace % 16 != 0 || v->workspace_bytes < draft_verify_workspace(v))
+        return PA_EWORKSPACE;
+    VerifyDev P;
+    P.batch = v->batch;
+    P.T = v->drafts;
+    P.vocab = v->vocab;
+    P.chunks = verify_chunks(v);
+    P.logits = v->logits;
+    P.logits_sb = v->logits_sb;
+    P.logits_sn = v->logits_sn;
+    P.tokens = v->tokens;
+    P.tokens_stride = v->tokens_stride;
+    P.parents = v->parents;
+    P.parents_stride = v->parents_stride;
+    P.uniforms = v->uniforms;
+    P.uniforms_stride = v->uniforms_stride;
+    P.noise = v->noise;
+    P.noise_stride = v->noise_stride;
+    P.temperature = v->temperature;
+    P.probs = v->uniforms ? v->draft_probs : nullptr;
+    P.probs_sb = v->probs_sb;
+    P.probs_sn = v->probs_sn;
+    P.path = v->path;
+    P.kept = v->kept;
+    P.token = v->token;
+    char* ws = static_cast<char*>(v->workspace);
+    P.stats = reinterpret_cast<float4*>(ws);
+    ws += (size_t)P.batch * P.T * P.chunks * sizeof(float4);
+    P.best = reinterpret_cast<uint64_t*>(ws);
+    ws += (size_t)P.batch * P.chunks * 16;
+    P.ticket = reinterpret_cast<uint32_t*>(ws);
+    auto go = [&](auto tag) {
+        typedef decltype(tag) T;
+        {
+            ProfScope ps("verify_stats", s);
+            hipLaunchKernelGGL((k_verify_stats<T>), dim3(P.chunks, P.T, P.batch), dim3(kVerThreads), 0, s, P);
+        }
+        ProfScope ps("verify_walk", s);
+        hipLaunchKernelGGL((k_verify_walk<T>), dim3(P.chunks, P.batch), dim3(kVerThreads), 0, s, P);
+    };
+    if (v->dtype == PA_F32) go(float{});
+    else if (v->dtype == PA_F16) go(f16{});
+    else go(bf16{});
+    return PA_OK;
+}
+
+}  // namespace pa

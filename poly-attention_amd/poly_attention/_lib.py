@@ -16,8 +16,10 @@ import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libpolyattn.so"
 
-PA_ABI_VERSION = 8
+PA_ABI_VERSION = 9
 PA_MAX_ORDER = 8
+PA_MAX_DRAFTS = 64
+PA_MAX_MOVES = 128
 
 PA_OK = 0
 PA_EINVAL = -1
@@ -67,6 +69,12 @@ EXPORTED_SYMBOLS = (
     "pa_rmsnorm_bwd",
     "pa_linear_small",
     "pa_linear_rows",
+    "pa_draft_append",
+    "pa_draft_attend_workspace",
+    "pa_draft_attend",
+    "pa_draft_verify_workspace",
+    "pa_draft_verify",
+    "pa_draft_commit",
 )
 
 
@@ -261,12 +269,119 @@ class PaLinear(ctypes.Structure):
     ]
 
 
+class PaDraftLevel(ctypes.Structure):
+    _fields_ = [(name, PaView) for name in ("k", "v", "vmul", "bias", "q", "dk", "dv", "out", "lse")]
+
+
+class PaDraft(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int32),
+        ("kv_heads", c_int32),
+        ("heads", c_int32),
+        ("drafts", c_int32),
+        ("dim", c_int32),
+        ("order", c_int32),
+        ("capacity", c_int32),
+        ("scale", c_float),
+        ("softclamp", c_float),
+        ("counts", c_void_p),
+        ("parents", c_void_p),
+        ("parents_stride", c_int64),
+        ("levels", PaDraftLevel * PA_MAX_ORDER),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+    ]
+
+
+class PaDraftItem(ctypes.Structure):
+    _fields_ = [
+        ("src", PaView),
+        ("norm_weight", c_void_p),
+        ("weight_dtype", c_int32),
+        ("rotate", c_int32),
+        ("out", PaView),
+    ]
+
+
+class PaDraftRows(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int32),
+        ("drafts", c_int32),
+        ("dim", c_int32),
+        ("count", c_int32),
+        ("eps", c_float),
+        ("counts", c_void_p),
+        ("parents", c_void_p),
+        ("parents_stride", c_int64),
+        ("angles", c_void_p),
+        ("angles_dtype", c_int32),
+        ("rot_dim", c_int32),
+        ("angles_sb", c_int64),
+        ("angles_sn", c_int64),
+        ("inv_freq", c_void_p),
+        ("interp", c_float),
+        ("items", PaDraftItem * (2 * PA_MAX_ORDER)),
+    ]
+
+
+class PaVerify(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int32),
+        ("drafts", c_int32),
+        ("vocab", c_int32),
+        ("dtype", c_int32),
+        ("logits", c_void_p),
+        ("logits_sb", c_int64),
+        ("logits_sn", c_int64),
+        ("tokens", c_void_p),
+        ("tokens_stride", c_int64),
+        ("parents", c_void_p),
+        ("parents_stride", c_int64),
+        ("uniforms", c_void_p),
+        ("uniforms_stride", c_int64),
+        ("noise", c_void_p),
+        ("noise_stride", c_int64),
+        ("temperature", c_void_p),
+        ("draft_probs", c_void_p),
+        ("probs_sb", c_int64),
+        ("probs_sn", c_int64),
+        ("path", c_void_p),
+        ("kept", c_void_p),
+        ("token", c_void_p),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+    ]
+
+
+class PaDraftMove(ctypes.Structure):
+    _fields_ = [("src", c_void_p), ("dst", c_void_p), ("row_bytes", c_int32), ("pad", c_int32)]
+
+
+class PaCommit(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int32),
+        ("kv_heads", c_int32),
+        ("slots", c_int32),
+        ("capacity", c_int32),
+        ("count", c_int32),
+        ("advance", c_int32),
+        ("path", c_void_p),
+        ("path_stride", c_int64),
+        ("path_len", c_int32),
+        ("kept", c_void_p),
+        ("counts", c_void_p),
+        ("overflow", c_void_p),
+        ("moves", PaDraftMove * PA_MAX_MOVES),
+    ]
+
+
 class PaKernelTime(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("launches", c_int64), ("total_ms", ctypes.c_double)]
 
 
 STRUCTS = (PaView, PaMask, PaPass, PaPassGrad, PaDecodeLevel, PaDecode, PaPrologueItem,
-           PaPrologue, PaRmsNorm, PaLinear, PaLinearOut, PaEpilogue, PaQkNorm)
+           PaPrologue, PaRmsNorm, PaLinear, PaLinearOut, PaEpilogue, PaQkNorm,
+           PaDraftLevel, PaDraft, PaDraftItem, PaDraftRows, PaVerify, PaDraftMove, PaCommit)
 
 
 # The hot structs as one struct.pack each (assigning ctypes fields one by one was half of a pass's
@@ -343,6 +458,18 @@ def _configure(lib) -> None:
     lib.pa_rmsnorm_bwd.argtypes = [ctypes.POINTER(PaRmsNorm), c_void_p]
     lib.pa_linear_rows.restype = c_int
     lib.pa_linear_rows.argtypes = [ctypes.POINTER(PaLinear), c_void_p]
+    lib.pa_draft_append.restype = c_int
+    lib.pa_draft_append.argtypes = [ctypes.POINTER(PaDraftRows), c_void_p]
+    lib.pa_draft_attend_workspace.restype = c_size_t
+    lib.pa_draft_attend_workspace.argtypes = [ctypes.POINTER(PaDraft)]
+    lib.pa_draft_attend.restype = c_int
+    lib.pa_draft_attend.argtypes = [ctypes.POINTER(PaDraft), c_void_p]
+    lib.pa_draft_verify_workspace.restype = c_size_t
+    lib.pa_draft_verify_workspace.argtypes = [ctypes.POINTER(PaVerify)]
+    lib.pa_draft_verify.restype = c_int
+    lib.pa_draft_verify.argtypes = [ctypes.POINTER(PaVerify), c_void_p]
+    lib.pa_draft_commit.restype = c_int
+    lib.pa_draft_commit.argtypes = [ctypes.POINTER(PaCommit), c_void_p]
     lib.pa_linear_small.restype = c_int
     lib.pa_linear_small.argtypes = [ctypes.POINTER(PaLinear), c_void_p]
 

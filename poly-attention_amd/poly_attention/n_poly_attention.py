@@ -30,7 +30,8 @@ from ._helpers import (
     where_keys,
     where_queries,
 )
-from .poly_attention import (_DECODE_ROWS, _compute_dtype, _module_angles, _q_norms,
+from .drafts import DraftCache
+from .poly_attention import (_DECODE_ROWS, _compute_dtype, _draft_step, _module_angles, _q_norms,
                              _static_decode_step, fused_available)
 from .rotary import RotaryEmbedding, apply_rotary_emb
 
@@ -144,11 +145,14 @@ class NPolyAttention(Module):
 
     def forward(self, x, context: Tensor | tuple[Tensor, ...] | None = None, mask=None,
                 context_mask: Tensor | tuple[Tensor | None, ...] | None = None,
-                rotary_pos_emb=None, cache=None, return_cache=False):
+                rotary_pos_emb=None, cache=None, return_cache=False, parents=None):
+        """``parents``: the tree of the drafted tokens ``x`` (with a DraftCache; see drafts.py)."""
         seq_len, device = x.shape[-2], x.device
 
         has_cache = exists(cache)
-        if has_cache:
+        drafted = isinstance(cache, DraftCache)
+        assert drafted or not exists(parents), "parents describe drafted tokens: pass a DraftCache"
+        if has_cache and not drafted:
             assert seq_len == 1, "sequence length must be 1 when using kv cache"
 
         orig_x = x
@@ -216,10 +220,13 @@ class NPolyAttention(Module):
                     gates if self.attn_gate else None, self.use_root_value_as_attn_gate)
         epilogue_done = False
 
-        if isinstance(cache, _cache.StaticCache):
+        if drafted or isinstance(cache, _cache.StaticCache):
             # fixed-capacity cache: norms, rotary and appends fused into the decode step
-            out = _static_decode_step(self, qs, vs_for_aggregation, mask, context_mask,
-                                      rotary_pos_emb, cache)
+            step = _static_decode_step
+            if drafted:
+                step = partial(_draft_step, parents=parents)
+            out = step(self, qs, vs_for_aggregation, mask, context_mask, rotary_pos_emb,
+                       cache=cache)
             new_cache = cache
             if exists(root_value) and self.is_gqa:
                 root_value = repeat_kv(root_value, self.num_rep)

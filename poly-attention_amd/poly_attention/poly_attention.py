@@ -19,6 +19,7 @@ from torch.nn import Module, RMSNorm
 from einops.layers.torch import Rearrange
 
 from . import _cache, _lib
+from .drafts import DraftCache
 from ._helpers import (
     add_key_bias,
     cast_tuple,
@@ -215,6 +216,43 @@ def _static_decode_step(module, qs, vs, mask, context_mask, rotary_pos_emb,
     return out
 
 
+def _draft_step(module, qs, vs, mask, context_mask, rotary_pos_emb, cache: DraftCache,
+                parents) -> Tensor:
+    """A step over drafted tokens on a DraftCache, for both module orders: the norms and the rotary
+    into the draft slots, then every level of the attention (each in one call of the library).
+    ``qs`` = (q1, ..., q_{order+1}) are the raw projections [B, h, T, d], ``vs`` the aggregation
+    values.  Returns the output [B, heads, T, d]; ``commit_drafts`` keeps the tokens afterwards."""
+    q1 = qs[0]
+    if not (module.use_flash_kernel and q1.is_cuda):
+        raise RuntimeError("a DraftCache needs the fused GPU path (libpolyattn)")
+    _lib.load()
+    if exists(mask) or any(exists(m) for m in context_mask):
+        raise NotImplementedError("masks are not supported with a DraftCache: rows hold their own counts")
+    if cache.order != len(qs) - 1:
+        raise ValueError(f"DraftCache of order {cache.order} passed to an order-{len(qs) - 1} module")
+    norms = list(module.q_norms)
+    if len({n.eps for n in norms}) != 1:
+        raise NotImplementedError("q norms with different eps")
+    eps = norms[0].eps
+    if eps is None:  # torch's rms_norm default: epsilon of the op-math type (fp32)
+        eps = torch.finfo(torch.float32).eps
+    weights = [n.weight if n.weight is not None else torch.ones(q1.shape[-1], device=q1.device)
+               for n in norms]
+    kwargs = {}
+    if exists(rotary_pos_emb):
+        # a table of more positions is read from its end, as apply_rotary_emb does
+        T = q1.shape[-2]
+        kwargs["angles"] = (rotary_pos_emb[-T:] if rotary_pos_emb.dim() == 2 else rotary_pos_emb)
+    elif exists(module.rotary_emb):
+        # a module's own rotary (poly_attention.py:302-304, n_poly_attention.py:224-229): the cache
+        # holds its keys rotated, as a StaticCache does
+        cache.rotate_prefix(module.rotary_emb)
+        kwargs["inv_freq"] = module.rotary_emb.freqs
+        kwargs["interp"] = module.rotary_emb.interpolate_factor
+    q1 = cache.append(qs, vs, weights, eps=eps, parents=parents, **kwargs)
+    return cache.attend(q1, parents=parents, scale=module.scale, softclamp=module.softclamp_value)
+
+
 # attention
 
 
@@ -386,11 +424,14 @@ class Order2PolyAttention(Module):
 
     def forward(self, x, context: Tensor | tuple[Tensor, ...] | None = None, mask=None,
                 context_mask: Tensor | tuple[Tensor | None, ...] | None = None,
-                rotary_pos_emb=None, cache=None, return_cache=False):
+                rotary_pos_emb=None, cache=None, return_cache=False, parents=None):
+        """``parents``: the tree of the drafted tokens ``x`` (with a DraftCache; see drafts.py)."""
         seq_len, device = x.shape[-2], x.device
 
         has_cache = exists(cache)
-        if has_cache:
+        drafted = isinstance(cache, DraftCache)
+        assert drafted or not exists(parents), "parents describe drafted tokens: pass a DraftCache"
+        if has_cache and not drafted:
             assert seq_len == 1, "sequence length must be 1 when using kv cache"
 
         orig_x = x
@@ -459,10 +500,13 @@ class Order2PolyAttention(Module):
                     gates if self.attn_gate else None, self.use_root_value_as_attn_gate)
         epilogue_done = False
 
-        if isinstance(cache, _cache.StaticCache):
+        if drafted or isinstance(cache, _cache.StaticCache):
             # fixed-capacity cache: norms, rotary and appends fused into the decode step
-            out = _static_decode_step(self, qs, (v3,), mask, context_mask, rotary_pos_emb,
-                                      cache)
+            if drafted:
+                out = _draft_step(self, qs, (v3,), mask, context_mask, rotary_pos_emb, cache, parents)
+            else:
+                out = _static_decode_step(self, qs, (v3,), mask, context_mask, rotary_pos_emb,
+                                          cache)
             new_cache = cache
             v2 = repeat_kv(v2, self.num_rep) if self.is_gqa and exists(v2) else v2
         else:
