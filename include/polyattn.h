@@ -366,8 +366,9 @@ typedef struct pa_draft_level {
  *   s_ij  = softclamp(scale <q_i, k_j>) + bias_j      j a cached position of the row, an ancestor of
  *   out_i = sum_j softmax_j(s_ij) v_j                  node i, or i itself
  *   lse_i = logsumexp_j(s_ij)
- * with the values of pa_poly_decode (v; round(v * out of the level below); out of the level below);
- * the ancestors' level outputs are used as computed, in fp32.  Rows and views start on 16 bytes. */
+ * with the values of pa_poly_decode, a middle level's product not rounded (v; v * out of the level
+ * below; out of the level below); the ancestors' level outputs are used as computed, in fp32.
+ * Rows and views start on 16 bytes; cached positions lie at most 2^22 elements apart. */
 typedef struct pa_draft {
     int32_t batch, kv_heads, heads, drafts, dim, order, capacity;
     float   scale, softclamp;

@@ -125,7 +125,7 @@ extern template void launch_draft_partial<f16>(const DraftDev& P, int units, boo
 extern template void launch_draft_partial<float>(const DraftDev& P, int units, bool vmul, hipStream_t s);
 template <typename T> constexpr int draft_row_tiles(int D) {
     // 16-row tiles that a wave's accumulators hold
-    return sizeof(T) == 4 ? (D > 128 ? 1 : 2) : (D > 128 ? 2 : 4);
+    return D > 128 ? 1 : sizeof(T) == 4 ? 2 : 4;
 }
 
 }  // namespace pa

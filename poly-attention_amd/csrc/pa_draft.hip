@@ -494,6 +494,9 @@ int launch_draft_attend(const pa_draft* d, hipStream_t s) {
         const pa_view* vecs[7] = {&l.k, &l.v, &l.vmul, &l.q, &l.dk, &l.dv, &l.out};
         for (const pa_view* v : vecs)
             if (v->ptr && !rows16(*v)) return PA_EUNSUPPORTED;
+        // a step's offsets are 32-bit: positions at most 2^22 elements apart
+        for (const pa_view* v : {&l.k, &l.v, &l.vmul})
+            if (v->ptr && (v->sn < 0 || v->sn > (1 << 22))) return PA_EUNSUPPORTED;
         if ((l.bias.ptr && l.bias.sn != 1) || (l.lse.ptr && l.lse.sn != 1)) return PA_EUNSUPPORTED;
         DraftLevelDev& L = P.L[t];
         L.k = draft_row(l.k);

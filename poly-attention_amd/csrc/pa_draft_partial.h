@@ -49,14 +49,17 @@ __device__ __forceinline__ uint32_t draft_pack2(float lo, float hi) {
     const f2 v = {lo, hi};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, t2));
 }
-// two 16-bit products, each rounded
+// two 16-bit products: word e of hi the rounded ones, of lo what the rounding left
 template <typename T>
-__device__ __forceinline__ uint32_t draft_mul2(uint32_t a, uint32_t b) {
+__device__ __forceinline__ void draft_mul2(uint32_t a, uint32_t b, u32x4_d& hi, u32x4_d& lo, int e) {
     typedef float f2 __attribute__((ext_vector_type(2)));
     typedef T t2 __attribute__((ext_vector_type(2)));
     const f2 x = __builtin_convertvector(__builtin_bit_cast(t2, a), f2);
     const f2 y = __builtin_convertvector(__builtin_bit_cast(t2, b), f2);
-    return draft_pack2<T>(x[0] * y[0], x[1] * y[1]);
+    const uint32_t h = draft_pack2<T>(x[0] * y[0], x[1] * y[1]);
+    const f2 r = __builtin_convertvector(__builtin_bit_cast(t2, h), f2);
+    hi[e] = h;
+    lo[e] = draft_pack2<T>(fmaf(x[0], y[0], -r[0]), fmaf(x[1], y[1], -r[1]));
 }
 
 __device__ __forceinline__ u32x4_d load16u(const void* p) { return *reinterpret_cast<const u32x4_d*>(p); }
@@ -73,29 +76,44 @@ template <typename T, int D> struct DraftGeo {
     static constexpr int KE = F32 ? 4 : 8;         // elements of a 16-byte load
 };
 
-// a value row's features VE*c .. of one position
+// A buffer over the rest of a unit: loads past its end (and at kDraftOut) give 0 without touching memory,
+// so neither the last step nor a head dim below D needs a test.
+constexpr int kDraftOut = 0x7ffffff0;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t draft_buffer(const char* p, int64_t bytes) {
+    const int n = bytes <= 0 ? 0 : bytes > 0x40000000 ? 0x40000000 : (int)bytes;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, n, 0x00027000);
+}
 template <int VW>
-__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[VW]) {
+__device__ __forceinline__ void buffer_words(__amdgpu_buffer_rsrc_t r, int off, int more, uint32_t (&w)[VW]) {
     if constexpr (VW == 2) {
-        const u32x2_d x = *reinterpret_cast<const u32x2_d*>(p);
+        const u32x2_d x = __builtin_amdgcn_raw_buffer_load_b64(r, off, more, 0);
         w[0] = x[0];
         w[1] = x[1];
     } else {
 #pragma unroll
         for (int i = 0; i < VW; i += 4) {
-            const u32x4_d x = load16u(static_cast<const char*>(p) + 4 * i);
+            const u32x4_d x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * i, more, 0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[i + j] = x[j];
         }
     }
 }
 
+// waves per SIMD to hold registers for: two hide each other's waits and ends
+template <typename T, bool VM> constexpr int draft_waves(int D, int RT) {
+    return D <= 128 && D * RT <= (VM && D == 128 ? 128 : 256) ? 2 : 1;
+}
+
 template <typename T, int D, int RT, bool VM>
-__global__ __launch_bounds__(kDraftThreads) void k_draft_partial(const DraftDev P) {
+__global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_draft_partial(const DraftDev P) {
     typedef DraftGeo<T, D> G;
-    constexpr int KT = G::KT, NP = G::NP, KS = G::KS, VE = G::VE, VW = G::VW, KE = G::KE;
+    constexpr int KT = G::KT, KS = G::KS, VE = G::VE, KE = G::KE;
     constexpr int PITCH = D + 4;
-    __shared__ float s_o[16 * RT * PITCH];
+    // a query row's fragments stay in registers where those are few
+    constexpr bool QLDS = RT * KS * 4 > 32;
+    constexpr int OWORDS = 16 * RT * PITCH, QWORDS = QLDS ? RT * KS * 256 : 0;
+    __shared__ __align__(16) float s_o[OWORDS > QWORDS ? OWORDS : QWORDS];  // the queries, then the outputs
+    u32x4_d* const s_q = reinterpret_cast<u32x4_d*>(s_o);
     __shared__ float s_m[4][16 * RT], s_l[4][16 * RT];
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -111,21 +129,31 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_partial(const DraftDev 
     place = __builtin_amdgcn_readfirstlane(place);
     const int len = draft_count(P, b);
     const int64_t begin = place * size;
-    const int cnt = (int)(len - begin < size ? len - begin : size);  // >= 1
+    const int cnt = __builtin_amdgcn_readfirstlane((int)(len - begin < size ? len - begin : size));  // >= 1
     const int nrows = min(16 * RT, L.rows - r0);
     const int nrt = (nrows + 15) / 16;
 
     // the queries: row r of the block is node r % T of the group's head r / T
-    u32x4_d qf[RT][KS];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
+    auto query = [&](int rt, int s) __attribute__((always_inline)) -> u32x4_d {
         const int r = min(r0 + 16 * rt + c, L.rows - 1);
         const T* row = L.q.at<T>(b, hk * L.rep + r / P.T) + (int64_t)(r % P.T) * L.q.sn;
+        const int d = (KE * 4) * s + KE * g;
+        return d < P.dim ? load16u(row + d) : u32x4_d{0u, 0u, 0u, 0u};
+    };
+    u32x4_d qf[QLDS ? 1 : RT][KS];
+    if constexpr (QLDS) {  // fragments in LDS, in the order of the lanes
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int d = (KE * 4) * s + KE * g;
-            qf[rt][s] = d < P.dim ? load16u(row + d) : u32x4_d{0u, 0u, 0u, 0u};
-        }
+        for (int rt = 0; rt < RT; ++rt)
+            if (rt % 4 == wave || RT < 4)
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+                    if (RT >= 4 || s % 4 == wave) s_q[(rt * KS + s) * 64 + lane] = query(rt, s);
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) qf[rt][s] = query(rt, s);
     }
     f32x4_t o[RT][VE];
     float m[RT], l[RT];
@@ -137,84 +165,139 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_partial(const DraftDev 
         for (int j = 0; j < VE; ++j) o[rt][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    const T* kb = L.k.at<T>(b, hk) + begin * L.k.sn;
-    const T* vb = L.v.at<T>(b, hk) + begin * L.v.sn;
-    const T* mb = VM && L.m.p ? L.m.at<T>(b, hk) + begin * L.m.sn : nullptr;
-    const float* bias = L.bias.p ? L.bias.at<float>(b, hk) + begin : nullptr;
+    const bool has_m = VM && L.m.p;
+    const char* kb = reinterpret_cast<const char*>(L.k.at<T>(b, hk) + begin * L.k.sn);
+    const char* vb = reinterpret_cast<const char*>(L.v.at<T>(b, hk) + begin * L.v.sn);
+    const char* mb = has_m ? reinterpret_cast<const char*>(L.m.at<T>(b, hk) + begin * L.m.sn) : nullptr;
+    const char* bb = L.bias.p ? reinterpret_cast<const char*>(L.bias.at<float>(b, hk) + begin) : nullptr;
+    const int64_t kp = L.k.sn * (int64_t)sizeof(T), vp = L.v.sn * (int64_t)sizeof(T),
+                  mp = has_m ? L.m.sn * (int64_t)sizeof(T) : 0;  // bytes between positions
+    const int rowb = P.dim * (int)sizeof(T);
+    // a lane's offsets inside a step do not change: positions 16 t + c of the keys, 16 t + 4 g + i
+    // of the values
+    int ko[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        const int d = (KE * 4) * s + KE * g;
+        ko[s] = d < P.dim ? c * (int)kp + d * (int)sizeof(T) : kDraftOut;
+    }
+    const bool vin = VE * c < P.dim;
+    const int vo = vin ? 4 * g * (int)vp + VE * c * (int)sizeof(T) : kDraftOut;
+    const int mo = vin ? 4 * g * (int)mp + VE * c * (int)sizeof(T) : kDraftOut;
     const float sl2 = P.scale * kLog2e, cl2 = P.softclamp * kLog2e;
-    const float cinv = P.softclamp > 0.f ? P.scale / P.softclamp : 0.f;
-    // Features past the head dim (one that is not D): the loads fall back to the row's last 16
-    // bytes; the queries are 0 there, and those columns of the output are not stored.
-    int kd[KS];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) kd[s] = min((KE * 4) * s + KE * g, P.dim - KE);
-    const int vd = min(VE * c, P.dim - VE);  // dim is a multiple of 8 (fp32: 4), and see the host
+    const float unclamped = P.softclamp > 0.f ? P.scale / P.softclamp : sl2;
 
-    const int steps = (cnt + 64 * KT - 1) / (64 * KT);  // the workgroup's: 4 waves x KT tiles
-    for (int st = 0; st < steps; ++st) {
-        const int j0 = (4 * st + wave) * 16 * KT;
-        if (j0 >= cnt) break;
-        // positions past the unit's end read its last one; their scores become -inf
-        u32x4_d kf[KT][KS];
-        uint32_t v[NP][VW];
-        float bz[KT][4];
-#pragma unroll
-        for (int t = 0; t < KT; ++t) {
-            const T* row = kb + (int64_t)min(j0 + 16 * t + c, cnt - 1) * L.k.sn;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) kf[t][s] = load16u(row + kd[s]);
-        }
+    // One set of registers for the keys and one for the values: the next step's keys are loaded as soon as
+    // this step's scores are formed, its values as soon as they have been summed, so that loads are in
+    // flight all the time (and twice the waves fit, against two sets).
+    u32x4_d kf[KT][KS];
+    uint32_t v[G::NP][G::VW];
+    uint32_t mv[VM ? G::NP : 1][VM ? G::VW : 1];
+    uint32_t bz[KT][4];
+    auto load_k = [&](int j0) __attribute__((always_inline)) {
+        const int left = cnt - j0;  // positions of the unit from here; none past its last step
+        const auto rk = draft_buffer(kb + j0 * kp, left > 0 ? (left - 1) * kp + rowb : 0);
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int64_t j = min(j0 + 16 * t + 4 * g + i, cnt - 1);
-                load_words<VW>(vb + j * L.v.sn + vd, v[4 * t + i]);
-                bz[t][i] = bias ? bias[j] * kLog2e : 0.f;
-                if constexpr (VM) {
-                    if (mb) {
-                        uint32_t x[VW];
-                        load_words<VW>(mb + j * L.m.sn + vd, x);
+            for (int s = 0; s < KS; ++s)
+                kf[t][s] = __builtin_amdgcn_raw_buffer_load_b128(rk, ko[s], 16 * t * (int)kp, 0);
+        if (bb) {
+            const auto rb = draft_buffer(bb + 4ll * j0, 4ll * left);
 #pragma unroll
-                        for (int w = 0; w < VW; ++w) {
-                            if constexpr (G::F32)
-                                v[4 * t + i][w] = __float_as_uint(__uint_as_float(v[4 * t + i][w]) *
-                                                                  __uint_as_float(x[w]));
-                            else
-                                v[4 * t + i][w] = draft_mul2<T>(v[4 * t + i][w], x[w]);
-                        }
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    bz[t][i] = __builtin_amdgcn_raw_buffer_load_b32(rb, 16 * g, 64 * t + 4 * i, 0);
+        }
+    };
+    auto load_v = [&](int j0) __attribute__((always_inline)) {
+        const int left = cnt - j0;
+        const auto rv = draft_buffer(vb + j0 * vp, left > 0 ? (left - 1) * vp + rowb : 0);
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                buffer_words<G::VW>(rv, vo, (16 * t + i) * (int)vp, v[4 * t + i]);
+        if constexpr (VM)
+            if (has_m) {
+                const auto rm = draft_buffer(mb + j0 * mp, left > 0 ? (left - 1) * mp + rowb : 0);
+#pragma unroll
+                for (int t = 0; t < KT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        buffer_words<G::VW>(rm, mo, (16 * t + i) * (int)mp, mv[4 * t + i]);
+            }
+    };
+
+    constexpr int STEP = 64 * KT;  // the workgroup's positions per round of steps
+    const int first = wave * 16 * KT;
+    load_k(first);
+    load_v(first);
+    for (int j0 = first; j0 < cnt; j0 += STEP) {
+        float x[RT][KT][4];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            if (rt >= nrt) break;
+            f32x4_t a[KT];
+#pragma unroll
+            for (int t = 0; t < KT; ++t) a[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const u32x4_d q = QLDS ? s_q[(rt * KS + s) * 64 + lane] : qf[QLDS ? 0 : rt][s];
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    if constexpr (G::F32) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) a[t] = mma_f32(kf[t][s][j], q[j], a[t]);
+                    } else {
+                        a[t] = Mma16<T>::run(kf[t][s], q, a[t]);
                     }
                 }
             }
-        // scores and probabilities
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[rt][t][i] = a[t][i] * unclamped;
+        }
+        if (P.softclamp > 0.f) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int t = 0; t < KT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[rt][t][i] = cl2 * tanhf(x[rt][t][i]);
+        }
+        if (bb) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+                        x[rt][t][i] = fmaf(__uint_as_float(bz[t][i]), kLog2e, x[rt][t][i]);
+        }
+        if (j0 + 16 * KT > cnt) {  // the unit's last positions
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+                        if (j0 + 16 * t + 4 * g + i >= cnt) x[rt][t][i] = -INFINITY;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(j0 + STEP);
+        __builtin_amdgcn_sched_barrier(0);
         uint32_t pf[RT][4];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             if (rt >= nrt) break;
-            float x[KT][4];
-#pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                f32x4_t a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    if constexpr (G::F32) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) a = mma_f32(kf[t][s][j], qf[rt][s][j], a);
-                    } else {
-                        a = Mma16<T>::run(kf[t][s], qf[rt][s], a);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float y = P.softclamp > 0.f ? cl2 * tanhf(a[i] * cinv) : a[i] * sl2;
-                    x[t][i] = j0 + 16 * t + 4 * g + i < cnt ? y + bz[t][i] : -INFINITY;
-                }
-            }
-            float top = x[0][0];
+            float top = x[rt][0][0];
 #pragma unroll
             for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, x[t][i]);
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, x[rt][t][i]);
             if (__any(top > m[rt] + kDraftTau)) {
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
@@ -230,18 +313,18 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_partial(const DraftDev 
             for (int t = 0; t < KT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[t][i] = __builtin_amdgcn_exp2f(x[t][i] - ms);
-                    l[rt] += x[t][i];
+                    x[rt][t][i] = __builtin_amdgcn_exp2f(x[rt][t][i] - ms);
+                    l[rt] += x[rt][t][i];
                 }
             if constexpr (G::F32) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) pf[rt][i] = __float_as_uint(x[0][i]);
+                for (int i = 0; i < 4; ++i) pf[rt][i] = __float_as_uint(x[rt][0][i]);
             } else {
-                // rounded to the value type for the product: 2^-9 of a term, averaged over the row
+                // rounded to the value type for the product: half a step of a term, averaged over the row
 #pragma unroll
                 for (int t = 0; t < KT; ++t) {
-                    pf[rt][2 * t] = draft_pack2<T>(x[t][0], x[t][1]);
-                    pf[rt][2 * t + 1] = draft_pack2<T>(x[t][2], x[t][3]);
+                    pf[rt][2 * t] = draft_pack2<T>(x[rt][t][0], x[rt][t][1]);
+                    pf[rt][2 * t + 1] = draft_pack2<T>(x[rt][t][2], x[rt][t][3]);
                 }
             }
         }
@@ -250,25 +333,43 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_partial(const DraftDev 
         for (int j = 0; j < VE; ++j) {
             if constexpr (G::F32) {
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    if (rt >= nrt) break;
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t a = v[i][j];
+                    if constexpr (VM)
+                        if (has_m) a = __float_as_uint(__uint_as_float(a) * __uint_as_float(mv[i][j]));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[rt][j] = mma_f32(v[i][j], pf[rt][i], o[rt][j]);
+                    for (int rt = 0; rt < RT; ++rt)
+                        if (rt < nrt) o[rt][j] = mma_f32(a, pf[rt][i], o[rt][j]);
                 }
             } else {
                 const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
-                u32x4_d a;
+                u32x4_d a, a2 = {0u, 0u, 0u, 0u};
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     a[e] = __builtin_amdgcn_perm(v[2 * e + 1][j / 2], v[2 * e][j / 2], sel);
+                if constexpr (VM)
+                    if (has_m) {
+                        // v * m as two values of the type, the rounded product and what it leaves: one
+                        // rounding of the product was most of a middle level's error
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t y = __builtin_amdgcn_perm(mv[2 * e + 1][j / 2], mv[2 * e][j / 2], sel);
+                            draft_mul2<T>(a[e], y, a, a2, e);
+                        }
+                    }
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
                     if (rt >= nrt) break;
-                    o[rt][j] = Mma16<T>::run(a, u32x4_d{pf[rt][0], pf[rt][1], pf[rt][2], pf[rt][3]},
-                                             o[rt][j]);
+                    const u32x4_d p = {pf[rt][0], pf[rt][1], pf[rt][2], pf[rt][3]};
+                    o[rt][j] = Mma16<T>::run(a, p, o[rt][j]);
+                    if constexpr (VM)
+                        if (has_m) o[rt][j] = Mma16<T>::run(a2, p, o[rt][j]);
                 }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(j0 + STEP);
+        __builtin_amdgcn_sched_barrier(0);
     }
 
     // join the four waves: maxima and sums first, then the outputs one wave after another
