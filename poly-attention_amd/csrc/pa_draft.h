@@ -5,13 +5,13 @@
 // them read the same keys and values, so the scores and the weighted sums are matrix products with
 // R rows: the cached positions are read from memory once for all nodes and heads of a group.
 //
-// Two launches.  k_draft_partial covers the cached positions of every level: they do not depend on the
-// step's results, so all levels run at once, split over positions ("units": chunks of one size in
-// all rows, whose number follows the counts on the device); it leaves (max, sum, weighted values)
-// per unit.  k_draft_combine walks the levels, deepest first: it joins the units and adds the tree
-// part, where the deeper level's result is the bias and the value.  Values enter linearly, column by
-// column, and the scores need no values: a workgroup of the combine owns some columns of the head
-// and repeats the (small) scores of the tree, so no workgroup waits for another.
+// Two launches.  k_draft_partial covers what does not depend on the step's results, so all levels run
+// at once: the cached positions, split into units (chunks of one size in all rows, whose number
+// follows the counts on the device), each leaving (max, sum, weighted values), and the scores of
+// the drafted tokens among themselves.  k_draft_combine walks the levels, deepest first: it joins the
+// units and the tree part, where the deeper level's result is the bias and the value.  Values enter
+// linearly, column by column, and the scores need no values: a workgroup of the combine owns some
+// columns of the head and repeats the (few) weights, so no workgroup waits for another.
 #pragma once
 
 #include "pa_common.h"
@@ -48,6 +48,9 @@ struct DraftDev {
     int64_t parents_stride;
     float* ws_o;   // [unit][kv head][rec_rows][dim]
     float2* ws_s;  // [unit][kv head][rec_rows]: running maximum (log2 units) and sum
+    float* ws_t;   // [row][kv head][rec_rows][t16]: scores of the tree without biases (log2 units), -inf
+                   // where a node does not see another
+    int32_t t16;   // T in whole sixteens
     DraftLevelDev L[PA_MAX_ORDER];
 };
 
@@ -55,46 +58,62 @@ __device__ __forceinline__ int draft_count(const DraftDev& P, int b) {
     const int n = P.counts[b];
     return n < 0 ? 0 : (n > P.capacity ? P.capacity : n);
 }
+__device__ __forceinline__ int draft_chunks(const DraftDev& P, int b) {
+    return (int)(((unsigned)draft_count(P, b) + kDraftChunk - 1) / kDraftChunk);
+}
 
-// Positions per unit: the batch's positions over the units aimed at, in whole kDraftChunk.  The sum
-// of ceil(n_b / size) is then at most target + batch.
-__device__ __forceinline__ int64_t draft_unit_size(const DraftDev& P, int lane) {
-    int64_t total = 0;
-    for (int b = lane; b < P.batch; b += 64) total += draft_count(P, b);
+// How the cached positions are split: units of `size` chunks in all rows, so many that there are about
+// `target` of them (at most target + batch), counted on the device.
+struct DraftUnits {
+    int size;    // chunks per unit
+    int b;       // the row of the unit asked for
+    int place;   // its place among the row's units
+    int first;   // the first unit of row b
+    int number;  // the units of row b
+};
+
+__device__ __forceinline__ unsigned draft_ceil(unsigned n, unsigned d) { return d == 1 ? n : (n + d - 1) / d; }
+
+// The units of row `want` (want >= 0), or the row of unit u (want < 0; false past the last unit).
+// The whole wave takes part.  One row needs no sums.
+__device__ __forceinline__ bool draft_units(const DraftDev& P, int want, int u, int lane, DraftUnits& r) {
+    if (P.batch == 1) {
+        const unsigned n = draft_chunks(P, 0);
+        r.size = max(1u, draft_ceil(n, P.target));
+        r.b = 0;
+        r.first = 0;
+        r.place = u;
+        r.number = draft_ceil(n, r.size);
+        return want >= 0 || u < r.number;
+    }
+    unsigned total = 0, n0 = 0;  // n0: this lane's row of the first 64
+    for (int b = lane; b < P.batch; b += 64) {
+        const unsigned n = draft_chunks(P, b);
+        total += n;
+        if (b < 64) n0 = n;
+    }
     for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off);
-    const int64_t c = (total + P.target - 1) / P.target;
-    const int64_t size = (c + kDraftChunk - 1) / kDraftChunk * kDraftChunk;
-    return size > 0 ? size : kDraftChunk;
-}
-
-// number of units of the rows before b (the whole wave takes part)
-__device__ __forceinline__ int draft_first_unit(const DraftDev& P, int64_t size, int b, int lane) {
-    int sum = 0;
-    for (int r = lane; r < b; r += 64) sum += (int)((draft_count(P, r) + size - 1) / size);
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-    return sum;
-}
-
-// the row of unit u and its place among that row's units; false past the last unit
-__device__ __forceinline__ bool draft_find_unit(const DraftDev& P, int64_t size, int u, int lane, int& b,
-                                                int& place) {
+    r.size = max(1u, draft_ceil(total, P.target));
     int before = 0;
     for (int r0 = 0; r0 < P.batch; r0 += 64) {
-        const int r = r0 + lane;
-        const int mine = r < P.batch ? (int)((draft_count(P, r) + size - 1) / size) : 0;
+        const int row = r0 + lane;
+        const int mine = draft_ceil(r0 == 0 ? n0 : row < P.batch ? draft_chunks(P, row) : 0, r.size);
         int incl = mine;
         for (int off = 1; off < 64; off <<= 1) {
             const int y = __shfl_up(incl, off);
             if (lane >= off) incl += y;
         }
-        const uint64_t past = __ballot(before + incl > u);
+        const uint64_t past = want >= 0 ? (want < r0 + 64 ? 1ull << (want - r0) : 0ull)
+                                        : __ballot(before + incl > u);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
-            b = r0 + l;
-            place = u - (before + __shfl(incl, l) - __shfl(mine, l));
+            r.b = __builtin_amdgcn_readfirstlane(r0 + l);
+            r.number = __builtin_amdgcn_readlane(mine, l);
+            r.first = before + __builtin_amdgcn_readlane(incl, l) - r.number;
+            r.place = u - r.first;
             return true;
         }
-        before += __shfl(incl, 63);
+        before += __builtin_amdgcn_readlane(incl, 63);
     }
     return false;
 }

@@ -8,195 +8,218 @@
 namespace pa {
 
 // ---------------------------------------------------------------------------------------
-// One workgroup per (batch row and key head, P.cols columns of the head, up to 64 rows of the
-// final level).  Per level, deepest first: the scores of the rows against the T drafted keys
-// (16x16 tiles), masked to each node's ancestors; their softmax joined with the units' maxima and
-// sums; the workgroup's columns of the output from the units' weighted values and the tree's
+// One workgroup per (batch row and key head, P.cols columns of the head, up to 64 rows of the final
+// level).  First, for all levels at once, the units of the cached positions are joined (a row's
+// maximum, sum and the workgroup's columns); then the levels, deepest first: the tree's scores get the
+// deeper level's logsumexps, their softmax is joined with the units' and the columns with the tree's
 // values.  The levels below the final one have at most 64 rows and are repeated by every row block.
-template <typename T, int D>
-__global__ __launch_bounds__(kDraftThreads) void k_draft_combine(const DraftDev P) {
-    typedef DraftGeo<T, D> G;
-    constexpr int KS = G::KS, KE = G::KE;
-    extern __shared__ float smem[];
-    const int T16 = (P.T + 15) & ~15;
-    const int spitch = T16 + 1, vpitch = P.cols + 4;
-    float* s_s = smem;                         // [64][spitch]: scores, then probabilities
-    float* s_in = s_s + ((64 * spitch + 3) & ~3);  // [T16][vpitch]: this level's tree values
-    float* s_out = s_in + T16 * vpitch;        // [T16][vpitch]: its outputs
-    __shared__ uint64_t s_anc[64];
-    __shared__ float s_bias[64], s_nbias[64], s_top[64], s_sum[64];
-    __shared__ float4 s_red[kDraftThreads];
+// What bounds it is latency: loads are issued in batches and the next level's scores are loaded before
+// this one's are used.
+constexpr int kDraftBatch = 8;  // units whose records a thread loads together
 
+struct JoinedRow {
+    float top, sum;
+    float4 acc;
+};
+__device__ __forceinline__ void join(JoinedRow& a, float top, float sum, const float4& acc) {
+    const float t = fmaxf(a.top, top);
+    const float f = a.top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.top - t);
+    const float h = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t);
+    a.top = t;
+    a.sum = a.sum * f + sum * h;
+    a.acc.x = a.acc.x * f + acc.x * h;
+    a.acc.y = a.acc.y * f + acc.y * h;
+    a.acc.z = a.acc.z * f + acc.z * h;
+    a.acc.w = a.acc.w * f + acc.w * h;
+}
+
+template <typename T>
+__device__ __forceinline__ float4 load4f(const T* p) {
+    if constexpr (sizeof(T) == 4) {
+        return *reinterpret_cast<const float4*>(p);
+    } else {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        const t4 x = *reinterpret_cast<const t4*>(p);
+        return make_float4((float)x[0], (float)x[1], (float)x[2], (float)x[3]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store4f(T* p, const float4& y) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = y;
+    } else {
+        u32x2_d w;
+        w[0] = draft_pack2<T>(y.x, y.y);
+        w[1] = draft_pack2<T>(y.z, y.w);
+        *reinterpret_cast<u32x2_d*>(p) = w;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kDraftThreads) void k_draft_combine(const DraftDev P) {
+    extern __shared__ __align__(16) float smem[];
+    __shared__ uint64_t s_anc[64];
+    __shared__ float s_bias[64], s_top[64], s_inv[64], s_utop[64 * PA_MAX_ORDER], s_usum[64 * PA_MAX_ORDER];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int c = lane & 15, g = lane >> 4;
     const int b = blockIdx.x / P.kv_heads, hk = blockIdx.x % P.kv_heads;
     const int col0 = blockIdx.y * P.cols, ncol = min(P.cols, P.dim - col0);
-    const int64_t size = draft_unit_size(P, lane);
-    const int first = draft_first_unit(P, size, b, lane);
-    const int units = (int)((draft_count(P, b) + size - 1) / size);
+    const int quads = ncol / 4;  // dim and cols are multiples of 8
+    const int last = P.order - 1, low = P.T * last;  // rows of the levels below the final one
+    const int r0 = blockIdx.z * 64, frows = min(64, P.L[last].rows - r0);
+    const int rows_all = low + frows;
+    const int spitch = P.t16 + 1, vpitch = P.cols + 4;
+    float* const s_acc = smem;                                  // [rows_all][cols]: the joined units
+    float* const s_p = s_acc + rows_all * P.cols;               // [64][spitch]: weights of the tree
+    float* s_in = s_p + ((64 * spitch + 3) & ~3);               // [t16][vpitch]: a level's tree values
+    float* s_out = s_in + P.t16 * vpitch;                       // [t16][vpitch]: its outputs
+    float* const s_red = s_in;                                  // before the levels: 256 JoinedRow
+
+    // four threads per row take the tree's scores of a level, every fourth one each
+    const int row = tid >> 2, sub = tid & 3;
+    float s[16];
+    auto load_scores = [&](int t) __attribute__((always_inline)) {
+        const int n = t == last ? frows : P.T;
+        const float* from = P.ws_t + (((int64_t)b * P.kv_heads + hk) * P.rec_rows + P.L[t].row0 +
+                                      (t == last ? r0 : 0) + row) * P.t16 + sub;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) s[k] = row < n && 4 * k + sub < P.T ? from[4 * k] : -INFINITY;
+    };
+    load_scores(0);
+    DraftUnits U;
+    draft_units(P, b, 0, lane, U);
     if (wave == 0)
         s_anc[lane] = draft_ancestors(P.parents ? P.parents + b * P.parents_stride : nullptr, P.T, lane);
-    const float sl2 = P.scale * kLog2e, cl2 = P.softclamp * kLog2e;
-    const float cinv = P.softclamp > 0.f ? P.scale / P.softclamp : 0.f;
-    const int quads = ncol / 4;  // dim and cols are multiples of 4
 
-    for (int t = 0; t < P.order; ++t) {
-        const DraftLevelDev& L = P.L[t];
-        const bool last = t == P.order - 1;
-        const int r0 = last ? blockIdx.z * 64 : 0;
-        if (r0 >= L.rows) return;  // the final level: nothing follows
-        const int rows = min(64, L.rows - r0);
-        const int64_t rec = ((int64_t)first * P.kv_heads + hk) * P.rec_rows + L.row0 + r0;
+    {   // the units: an item is a row and four columns, dealt out over `parts` threads where there are few
         const int64_t urec = (int64_t)P.kv_heads * P.rec_rows;  // records between units
-
-        // the tree's values: v, v * msg, or msg (already in s_in, as the level below left it)
-        if (!last)
-            for (int x = tid; x < P.T * quads; x += kDraftThreads) {
-                const int n = x / quads, d = 4 * (x % quads);
-                const T* row = L.dv.at<T>(b, hk) + n * L.dv.sn + col0 + d;
+        const int64_t rec0 = ((int64_t)U.first * P.kv_heads + hk) * P.rec_rows;
+        const int items = rows_all * quads;
+        int parts = 1;
+        while (parts < 16 && items * parts * 2 <= kDraftThreads && parts * 2 <= U.number) parts *= 2;
+        for (int x0 = 0; x0 < items; x0 += kDraftThreads) {
+            const int part = parts > 1 ? tid / items : 0, item = parts > 1 ? tid % items : x0 + tid;
+            JoinedRow a = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+            const int ra = item / quads, d = 4 * (item % quads);
+            if (item < items && part < parts) {
+                const int64_t rec = rec0 + ra + (ra < low ? 0 : r0);
+                for (int u = part; u < U.number; u += parts * kDraftBatch) {
+                    float2 ms[kDraftBatch];
+                    float4 y[kDraftBatch];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float* at = &s_in[n * vpitch + d + e];
-                    *at = t == 0 ? to_f(row[e]) : *at * to_f(row[e]);
+                    for (int k = 0; k < kDraftBatch; ++k) {
+                        const int64_t at = rec + (int64_t)min(u + k * parts, U.number - 1) * urec;
+                        ms[k] = P.ws_s[at];
+                        y[k] = *reinterpret_cast<const float4*>(P.ws_o + at * P.dim + col0 + d);
+                        if (u + k * parts >= U.number) ms[k].x = -INFINITY;
+                    }
+#pragma unroll
+                    for (int k = 0; k < kDraftBatch; ++k) join(a, ms[k].x, ms[k].y, y[k]);
                 }
             }
-        __syncthreads();  // s_anc and the level below's results are in place
-
-        const int nrt = (rows + 15) / 16, nkt = T16 / 16;
-        for (int pair = wave; pair < nrt * nkt; pair += 4) {
-            const int rt = pair / nkt, kt = pair % nkt;
-            const int r = r0 + min(16 * rt + c, rows - 1), n = min(16 * kt + c, P.T - 1);
-            const T* qrow = L.q.at<T>(b, hk * L.rep + r / P.T) + (r % P.T) * L.q.sn;
-            const T* krow = L.dk.at<T>(b, hk) + n * L.dk.sn;
-            f32x4_t a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const int d = KE * 4 * s + KE * g;
-                const bool in = d < P.dim;
-                const u32x4_d q = in ? load16u(qrow + d) : u32x4_d{0u, 0u, 0u, 0u};
-                const u32x4_d k = in ? load16u(krow + d) : u32x4_d{0u, 0u, 0u, 0u};
-                if constexpr (G::F32) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) a = mma_f32(q[j], k[j], a);
-                } else {
-                    a = Mma16<T>::run(q, k, a);
-                }
+            if (parts > 1) {
+                float* r = s_red + tid * 6;
+                r[0] = a.top;
+                r[1] = a.sum;
+                r[2] = a.acc.x;
+                r[3] = a.acc.y;
+                r[4] = a.acc.z;
+                r[5] = a.acc.w;
+                __syncthreads();
+                if (part == 0)
+                    for (int k = 1; k < parts; ++k) {
+                        const float* z = s_red + (tid + k * items) * 6;
+                        join(a, z[0], z[1], make_float4(z[2], z[3], z[4], z[5]));
+                    }
             }
-            const int key = 16 * kt + c;
-            const float bz = t == 0 ? 0.f : s_bias[key];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 16 * rt + 4 * g + i;
-                const bool sees = row < rows && ((s_anc[(r0 + row) % P.T] >> key) & 1);
-                const float y = P.softclamp > 0.f ? cl2 * tanhf(a[i] * cinv) : a[i] * sl2;
-                s_s[row * spitch + key] = sees ? y + bz : -INFINITY;
+            if (part == 0 && item < items) {
+                *reinterpret_cast<float4*>(s_acc + ra * P.cols + d) = a.acc;
+                if (d == 0) {
+                    s_utop[ra] = a.top;
+                    s_usum[ra] = a.sum;
+                }
             }
         }
-        __syncthreads();
+    }
+    __syncthreads();
 
-        {   // four threads per row: maximum and sum over the units and the tree
-            const int row = tid >> 2, sub = tid & 3;
-            float top = -INFINITY, sum = 0.f;
-            if (row < rows) {
-                for (int k = sub; k < P.T; k += 4) top = fmaxf(top, s_s[row * spitch + k]);
-                for (int u = sub; u < units; u += 4) top = fmaxf(top, P.ws_s[rec + row + u * urec].x);
+    for (int t = 0; t <= last; ++t) {
+        const DraftLevelDev& L = P.L[t];
+        const bool fin = t == last;
+        const int rows = fin ? frows : P.T, ra0 = t * P.T, rr = fin ? r0 : 0;
+        // the tree's values: v, v * msg, or msg (already in s_in, as the level below left it)
+        if (!fin)
+            for (int x = tid; x < P.T * quads; x += kDraftThreads) {
+                const int n = x / quads, d = 4 * (x % quads);
+                float4 y = load4f<T>(L.dv.at<T>(b, hk) + n * L.dv.sn + col0 + d);
+                float4* at = reinterpret_cast<float4*>(&s_in[n * vpitch + d]);
+                if (t > 0) {
+                    const float4 z = *at;
+                    y = make_float4(y.x * z.x, y.y * z.y, y.z * z.z, y.w * z.w);
+                }
+                *at = y;
+            }
+        {   // maximum and sum over the units and the tree
+            float top = row < rows ? s_utop[ra0 + row] : -INFINITY, sum = 0.f;
+            const float utop = top;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                if (t > 0 && 4 * k + sub < P.T) s[k] += s_bias[4 * k + sub];
+                top = fmaxf(top, s[k]);
             }
             top = fmaxf(top, __shfl_xor(top, 1));
             top = fmaxf(top, __shfl_xor(top, 2));
-            if (row < rows) {
-                for (int k = sub; k < P.T; k += 4) {
-                    const float x = s_s[row * spitch + k];
-                    const float p = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - top);
-                    s_s[row * spitch + k] = p;
-                    sum += p;
-                }
-                for (int u = sub; u < units; u += 4) {
-                    const float2 ms = P.ws_s[rec + row + u * urec];
-                    sum += ms.x == -INFINITY ? 0.f : ms.y * __builtin_amdgcn_exp2f(ms.x - top);
-                }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const float p = s[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[k] - top);
+                if (row < rows && 4 * k + sub < P.T) s_p[row * spitch + 4 * k + sub] = p;
+                sum += p;
             }
             sum += __shfl_xor(sum, 1);
             sum += __shfl_xor(sum, 2);
+            const float f = utop == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(utop - top);
+            __syncthreads();  // every s_bias has been read
             if (row < rows && sub == 0) {
-                const bool live = s_anc[(r0 + row) % P.T] != 0;
-                s_top[row] = top;
-                s_sum[row] = live ? sum : 0.f;
-                if (!last) {
+                sum += s_usum[ra0 + row] * f;
+                const bool live = s_anc[(rr + row) % P.T] != 0;
+                s_top[row] = f;
+                s_inv[row] = live ? 1.f / sum : 0.f;
+                if (!fin) {
                     const float lse = live ? top + log2f(sum) : 0.f;
-                    s_nbias[row] = lse;
+                    s_bias[row] = lse;
                     if (blockIdx.y == 0 && blockIdx.z == 0) L.lse.at<float>(b, hk)[row] = lse * kLn2;
                 }
             }
         }
+        if (!fin) load_scores(t + 1);
         __syncthreads();
-
-        // the outputs: one (row, four columns) item per thread; with few items the units are dealt out
-        // over `parts` threads per item
-        const int rp = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-        const int items = rp * quads;
-        const int parts = items * 8 <= kDraftThreads ? 8 : items * 4 <= kDraftThreads ? 4
-                          : items * 2 <= kDraftThreads ? 2 : 1;
-        for (int x0 = 0; x0 < items; x0 += kDraftThreads) {
-            const int part = parts > 1 ? tid / items : 0;
-            const int item = parts > 1 ? tid % items : x0 + tid;
-            const int row = item / quads, d = 4 * (item % quads);
-            const bool on = item < items && part < parts && row < rows && s_sum[row] != 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (on) {
-                const float top = s_top[row];
-                const float* src = P.ws_o + (rec + row) * P.dim + col0 + d;
-                for (int u = part; u < units; u += parts) {
-                    const float mu = P.ws_s[rec + row + u * urec].x;
-                    const float w = mu == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mu - top);
-                    const float4 y = *reinterpret_cast<const float4*>(src + u * urec * P.dim);
-                    acc.x += w * y.x;
-                    acc.y += w * y.y;
-                    acc.z += w * y.z;
-                    acc.w += w * y.w;
+        for (int x = tid; x < rows * quads; x += kDraftThreads) {
+            const int r = x / quads, d = 4 * (x % quads);
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            const uint64_t anc = s_anc[(rr + r) % P.T];
+            if (anc) {
+                const float f = s_top[r], inv = s_inv[r];
+                const float4 u = *reinterpret_cast<const float4*>(s_acc + (ra0 + r) * P.cols + d);
+                if (f != 0.f) y = make_float4(u.x * f, u.y * f, u.z * f, u.w * f);
+                // only what the node sees: another branch's value may be anything
+                for (uint64_t see = anc; see; see &= see - 1) {
+                    const int k = __ffsll((unsigned long long)see) - 1;
+                    const float p = s_p[r * spitch + k];
+                    const float4 z = *reinterpret_cast<const float4*>(&s_in[k * vpitch + d]);
+                    y.x += p * z.x;
+                    y.y += p * z.y;
+                    y.z += p * z.z;
+                    y.w += p * z.w;
                 }
-                if (part == 0) {
-                    // only what the node sees: another branch's value may be anything
-                    for (uint64_t see = s_anc[(r0 + row) % P.T]; see; see &= see - 1) {
-                        const int k = __ffsll((unsigned long long)see) - 1;
-                        const float p = s_s[row * spitch + k];
-                        const float* y = &s_in[k * vpitch + d];
-                        acc.x += p * y[0];
-                        acc.y += p * y[1];
-                        acc.z += p * y[2];
-                        acc.w += p * y[3];
-                    }
-                }
+                y = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
             }
-            if (parts > 1) {
-                s_red[tid] = acc;
-                __syncthreads();
-                if (part == 0)
-                    for (int k = 1; k < parts; ++k) {
-                        const float4 y = s_red[tid + k * items];
-                        acc.x += y.x;
-                        acc.y += y.y;
-                        acc.z += y.z;
-                        acc.w += y.w;
-                    }
-            }
-            if (part == 0 && item < items && row < rows) {
-                const float inv = s_sum[row] != 0.f ? 1.f / s_sum[row] : 0.f;
-                const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-                if (!last) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s_out[row * vpitch + d + e] = y[e];
-                }
-                if (last || blockIdx.z == 0) {
-                    const int r = r0 + row;
-                    T* to = L.out.at<T>(b, hk * L.rep + r / P.T) + (r % P.T) * L.out.sn + col0 + d;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) to[e] = from_f<T>(y[e]);
-                }
+            if (!fin) *reinterpret_cast<float4*>(&s_out[r * vpitch + d]) = y;
+            if (fin || blockIdx.z == 0) {
+                const int n = (rr + r) % P.T, h = (rr + r) / P.T;
+                store4f<T>(L.out.at<T>(b, hk * L.rep + h) + n * L.out.sn + col0 + d, y);
             }
         }
         __syncthreads();
-        if (tid < 64) s_bias[tid] = s_nbias[tid];
         float* const done = s_out;  // this level's outputs are the next one's values
         s_out = s_in;
         s_in = done;
@@ -422,6 +445,7 @@ bool draft_plan(const pa_draft* d, DraftDev& P, int& units) {
     const int block = 16 * (most <= 16 ? 1 : std::min(tiles, most <= 32 ? 2 : 4));
     P.row_blocks = (most + block - 1) / block;
     P.rec_rows = d->drafts * (d->order - 1) + most;
+    P.t16 = (d->drafts + 15) & ~15;
     const int64_t per = (int64_t)d->kv_heads * d->order * P.row_blocks;
     int64_t target = std::max<int64_t>(1, kDraftGoal / per);
     // no more units than the capacity has chunks
@@ -432,16 +456,25 @@ bool draft_plan(const pa_draft* d, DraftDev& P, int& units) {
     return (int64_t)d->kv_heads * P.row_blocks <= 65535;
 }
 
-size_t draft_ws_bytes(const DraftDev& P, int units) {
+// the workspace's three arrays, and its size
+size_t draft_ws(DraftDev& P, int units, void* base) {
+    auto whole = [](size_t n) { return (n + 255) & ~size_t(255); };
     const size_t rec = (size_t)units * P.kv_heads * P.rec_rows;
-    return ((rec * P.dim * 4 + 255) & ~size_t(255)) + rec * sizeof(float2);
+    char* at = static_cast<char*>(base);
+    P.ws_o = reinterpret_cast<float*>(at);
+    size_t n = whole(rec * P.dim * 4);
+    P.ws_s = reinterpret_cast<float2*>(at + n);
+    n += whole(rec * sizeof(float2));
+    P.ws_t = reinterpret_cast<float*>(at + n);
+    return n + (size_t)P.batch * P.kv_heads * P.rec_rows * P.t16 * 4;
 }
 
-template <typename T>
-void launch_combine(const DraftDev& P, dim3 grid, size_t lds, hipStream_t s) {
-    if (P.dim <= 64) hipLaunchKernelGGL((k_draft_combine<T, 64>), grid, dim3(kDraftThreads), lds, s, P);
-    else if (P.dim <= 128) hipLaunchKernelGGL((k_draft_combine<T, 128>), grid, dim3(kDraftThreads), lds, s, P);
-    else hipLaunchKernelGGL((k_draft_combine<T, 256>), grid, dim3(kDraftThreads), lds, s, P);
+// LDS of the combine with `cols` columns
+size_t combine_lds(const DraftDev& P, int cols) {
+    const int rows = P.T * (P.order - 1) + 64;
+    const size_t values = 2 * (size_t)P.t16 * (cols + 4);
+    return 4 * ((size_t)rows * cols + ((64 * (P.t16 + 1) + 3) & ~3) +
+                std::max(values, (size_t)kDraftThreads * 6));
 }
 
 }  // namespace
@@ -449,7 +482,7 @@ void launch_combine(const DraftDev& P, dim3 grid, size_t lds, hipStream_t s) {
 size_t draft_attend_workspace(const pa_draft* d) {
     DraftDev P;
     int units = 0;
-    return draft_plan(d, P, units) ? draft_ws_bytes(P, units) : 0;
+    return draft_plan(d, P, units) ? draft_ws(P, units, nullptr) : 0;
 }
 
 int launch_draft_attend(const pa_draft* d, hipStream_t s) {
@@ -464,17 +497,13 @@ int launch_draft_attend(const pa_draft* d, hipStream_t s) {
     int units = 0;
     if (!draft_plan(d, P, units)) return PA_EUNSUPPORTED;
     if (!d->workspace || (uintptr_t)d->workspace % 16 != 0 ||
-        d->workspace_bytes < draft_ws_bytes(P, units))
+        d->workspace_bytes < draft_ws(P, units, d->workspace))
         return PA_EWORKSPACE;
     P.scale = d->scale;
     P.softclamp = d->softclamp > 0.f ? d->softclamp : 0.f;
     P.counts = d->counts;
     P.parents = d->parents;
     P.parents_stride = d->parents_stride;
-    const size_t rec = (size_t)units * P.kv_heads * P.rec_rows;
-    P.ws_o = static_cast<float*>(d->workspace);
-    P.ws_s = reinterpret_cast<float2*>(static_cast<char*>(d->workspace) +
-                                       ((rec * P.dim * 4 + 255) & ~size_t(255)));
     const int rep = d->heads / d->kv_heads;
     bool vmul = false;
     for (int t = 0; t < d->order; ++t) {
@@ -519,19 +548,18 @@ int launch_draft_attend(const pa_draft* d, hipStream_t s) {
         else if (T == PA_F16) launch_draft_partial<f16>(P, units, vmul, s);
         else launch_draft_partial<bf16>(P, units, vmul, s);
     }
-    // columns per workgroup: few where the grid is small, all where it is not
+    // columns per workgroup: few where the grid is small; LDS of two workgroups a CU at least
     const int blocks = (d->drafts * rep + 63) / 64;
     P.cols = 16;
-    while (P.cols < 64 && P.cols < P.dim &&
-           (int64_t)P.batch * P.kv_heads * blocks * ((P.dim + P.cols - 1) / P.cols) > 2048)
+    while (P.cols < P.dim && combine_lds(P, 2 * P.cols) <= 56 * 1024 &&
+           (int64_t)P.batch * P.kv_heads * blocks * ((P.dim + P.cols - 1) / P.cols) > 1024)
         P.cols *= 2;
-    const int T16 = (P.T + 15) & ~15;
-    const size_t lds = 4 * (((64 * (T16 + 1) + 3) & ~3) + 2 * (size_t)T16 * (P.cols + 4));
+    const size_t lds = combine_lds(P, P.cols);
     const dim3 grid(P.batch * P.kv_heads, (P.dim + P.cols - 1) / P.cols, blocks);
     ProfScope ps("draft_combine", s);
-    if (T == PA_F32) launch_combine<float>(P, grid, lds, s);
-    else if (T == PA_F16) launch_combine<f16>(P, grid, lds, s);
-    else launch_combine<bf16>(P, grid, lds, s);
+    if (T == PA_F32) hipLaunchKernelGGL((k_draft_combine<float>), grid, dim3(kDraftThreads), lds, s, P);
+    else if (T == PA_F16) hipLaunchKernelGGL((k_draft_combine<f16>), grid, dim3(kDraftThreads), lds, s, P);
+    else hipLaunchKernelGGL((k_draft_combine<bf16>), grid, dim3(kDraftThreads), lds, s, P);
     return PA_OK;
 }
 

@@ -112,7 +112,9 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
     // a query row's fragments stay in registers where those are few
     constexpr bool QLDS = RT * KS * 4 > 32;
     constexpr int OWORDS = 16 * RT * PITCH, QWORDS = QLDS ? RT * KS * 256 : 0;
-    __shared__ __align__(16) float s_o[OWORDS > QWORDS ? OWORDS : QWORDS];  // the queries, then the outputs
+    // the waves' outputs meet in NB buffers, four where they are small
+    constexpr int NB = OWORDS <= 2304 ? 4 : OWORDS <= 4608 ? 2 : 1;
+    __shared__ __align__(16) float s_o[NB * OWORDS > QWORDS ? NB * OWORDS : QWORDS];  // the queries, then these
     u32x4_d* const s_q = reinterpret_cast<u32x4_d*>(s_o);
     __shared__ float s_m[4][16 * RT], s_l[4][16 * RT];
 
@@ -122,16 +124,16 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
     const int hk = blockIdx.y / P.row_blocks, r0 = (blockIdx.y % P.row_blocks) * 16 * RT;
     const DraftLevelDev& L = P.L[blockIdx.z];
     if (r0 >= L.rows) return;
-    const int64_t size = draft_unit_size(P, lane);
-    int b = 0, place = 0;
-    if (!draft_find_unit(P, size, blockIdx.x, lane, b, place)) return;
-    b = __builtin_amdgcn_readfirstlane(b);
-    place = __builtin_amdgcn_readfirstlane(place);
-    const int len = draft_count(P, b);
-    const int64_t begin = place * size;
-    const int cnt = __builtin_amdgcn_readfirstlane((int)(len - begin < size ? len - begin : size));  // >= 1
     const int nrows = min(16 * RT, L.rows - r0);
     const int nrt = (nrows + 15) / 16;
+    const bool tree = (int)blockIdx.x < P.batch;  // the first workgroups: a row's drafted tokens
+    const int unit = blockIdx.x - P.batch;
+    DraftUnits U;
+    if (!tree && !draft_units(P, -1, unit, lane, U)) return;
+    const int b = tree ? (int)blockIdx.x : U.b;
+    const int64_t begin = tree ? 0 : (int64_t)U.place * U.size * kDraftChunk;
+    // >= 1: a unit begins inside its row
+    const int cnt = tree ? 0 : __builtin_amdgcn_readfirstlane((int)min((int64_t)U.size * kDraftChunk, draft_count(P, b) - begin));
 
     // the queries: row r of the block is node r % T of the group's head r / T
     auto query = [&](int rt, int s) __attribute__((always_inline)) -> u32x4_d {
@@ -155,6 +157,49 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
 #pragma unroll
             for (int s = 0; s < KS; ++s) qf[rt][s] = query(rt, s);
     }
+    const float sl2 = P.scale * kLog2e, cl2 = P.softclamp * kLog2e;
+    const float unclamped = P.softclamp > 0.f ? P.scale / P.softclamp : sl2;
+
+    if (tree) {  // 16 drafted keys per wave
+        if (16 * wave >= P.T) return;
+        const uint64_t anc = draft_ancestors(P.parents ? P.parents + b * P.parents_stride : nullptr, P.T, lane);
+        const uint32_t anc_lo = (uint32_t)anc, anc_hi = (uint32_t)(anc >> 32);
+        const T* row = L.dk.at<T>(b, hk) + min(16 * wave + c, P.T - 1) * L.dk.sn;
+        u32x4_d kf[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = (KE * 4) * s + KE * g;
+            kf[s] = d < P.dim ? load16u(row + d) : u32x4_d{0u, 0u, 0u, 0u};
+        }
+        float* to = P.ws_t + (((int64_t)b * P.kv_heads + hk) * P.rec_rows + L.row0 + r0) * P.t16;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            if (rt >= nrt) break;
+            f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const u32x4_d q = QLDS ? s_q[(rt * KS + s) * 64 + lane] : qf[QLDS ? 0 : rt][s];
+                if constexpr (G::F32) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) a = mma_f32(kf[s][j], q[j], a);
+                } else {
+                    a = Mma16<T>::run(kf[s], q, a);
+                }
+            }
+            const int r = r0 + 16 * rt + c;
+            const uint64_t sees = ((uint64_t)__shfl(anc_hi, r % P.T) << 32) | __shfl(anc_lo, r % P.T);
+            f32x4_t y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = a[i] * unclamped;
+                y[i] = (sees >> (16 * wave + 4 * g + i)) & 1 ? (P.softclamp > 0.f ? cl2 * tanhf(x) : x) : -INFINITY;
+            }
+            if (16 * rt + c < nrows)
+                *reinterpret_cast<f32x4_t*>(to + (int64_t)(16 * rt + c) * P.t16 + 16 * wave + 4 * g) = y;
+        }
+        return;
+    }
+
     f32x4_t o[RT][VE];
     float m[RT], l[RT];
 #pragma unroll
@@ -184,8 +229,6 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
     const bool vin = VE * c < P.dim;
     const int vo = vin ? 4 * g * (int)vp + VE * c * (int)sizeof(T) : kDraftOut;
     const int mo = vin ? 4 * g * (int)mp + VE * c * (int)sizeof(T) : kDraftOut;
-    const float sl2 = P.scale * kLog2e, cl2 = P.softclamp * kLog2e;
-    const float unclamped = P.softclamp > 0.f ? P.scale / P.softclamp : sl2;
 
     // One set of registers for the keys and one for the values: the next step's keys are loaded as soon as
     // this step's scores are formed, its values as soon as they have been summed, so that loads are in
@@ -391,15 +434,18 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
         for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][16 * rt + c]);
         f[rt] = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - top);
     }
-    for (int w = 0; w < 4; ++w) {
-        if (wave == w) {
+    // in NB buffers: as many waves at a time
+#pragma unroll
+    for (int w = 0; w < 4; w += NB) {
+        if (wave / NB == w / NB) {
+            float* const buf = s_o + (wave % NB) * OWORDS;
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < VE; j += 4) {
-                        float4* at = reinterpret_cast<float4*>(&s_o[(16 * rt + c) * PITCH + VE * (4 * g + i) + j]);
+                        float4* at = reinterpret_cast<float4*>(&buf[(16 * rt + c) * PITCH + VE * (4 * g + i) + j]);
                         float4 x = w ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
                         x.x += f[rt] * o[rt][j][i];
                         x.y += f[rt] * o[rt][j + 1][i];
@@ -410,7 +456,7 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
         }
         __syncthreads();
     }
-    const int64_t rec = ((int64_t)blockIdx.x * P.kv_heads + hk) * P.rec_rows + L.row0 + r0;
+    const int64_t rec = ((int64_t)unit * P.kv_heads + hk) * P.rec_rows + L.row0 + r0;
     if (tid < nrows) {
         float top = s_m[0][tid], sum = 0.f;
         for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][tid]);
@@ -421,14 +467,22 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
     const int quads = P.dim / 4;
     for (int x = tid; x < nrows * quads; x += kDraftThreads) {
         const int r = x / quads, d = x % quads * 4;
-        *reinterpret_cast<float4*>(P.ws_o + (rec + r) * P.dim + d) =
-            *reinterpret_cast<const float4*>(&s_o[r * PITCH + d]);
+        float4 y = *reinterpret_cast<const float4*>(&s_o[r * PITCH + d]);
+#pragma unroll
+        for (int k = 1; k < NB; ++k) {
+            const float4 z = *reinterpret_cast<const float4*>(&s_o[k * OWORDS + r * PITCH + d]);
+            y.x += z.x;
+            y.y += z.y;
+            y.z += z.z;
+            y.w += z.w;
+        }
+        *reinterpret_cast<float4*>(P.ws_o + (rec + r) * P.dim + d) = y;
     }
 }
 
 template <typename T, int D, int RT>
 void launch_draft_partial_rt(const DraftDev& P, int units, bool vmul, hipStream_t s) {
-    const dim3 grid(units, P.kv_heads * P.row_blocks, P.order);
+    const dim3 grid(P.batch + units, P.kv_heads * P.row_blocks, P.order);
     if (vmul) hipLaunchKernelGGL((k_draft_partial<T, D, RT, true>), grid, dim3(kDraftThreads), 0, s, P);
     else hipLaunchKernelGGL((k_draft_partial<T, D, RT, false>), grid, dim3(kDraftThreads), 0, s, P);
 }
