@@ -458,7 +458,9 @@ typedef struct pa_draft_move {
 
 /* dst[b, h, counts[b] + i] = src[b, h, path[b, i]] for i < kept[b] and every move, then, with
  * `advance`, counts[b] += the number moved.  A path ends early at an entry outside [0, slots);
- * positions past the capacity are not written nor counted, and overflow[0] (when given) is set. */
+ * positions past the capacity are not written nor counted, and overflow[0] (when given) is set.
+ * `tickets` (0 before the call and again after it) tell the last workgroup of a row that the count
+ * may advance; the library reads `count` moves and no more of the array. */
 typedef struct pa_commit {
     int32_t        batch, kv_heads, slots, capacity, count, advance;
     const int32_t* path;        /* device [B, path_stride] */
@@ -467,6 +469,7 @@ typedef struct pa_commit {
     const int32_t* kept;        /* device [B] */
     int32_t*       counts;      /* device [B] */
     int32_t*       overflow;    /* device [1], or NULL */
+    int32_t*       tickets;     /* device [B]; required with advance */
     pa_draft_move  moves[PA_MAX_MOVES];
 } pa_commit;
 

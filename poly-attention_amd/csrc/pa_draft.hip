@@ -335,12 +335,13 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_append(const DraftRowsD
 // The kept nodes of a row, from their draft slots to the positions behind the cached ones.
 
 struct DraftCommitDev {
-    int32_t batch, kv_heads, slots, capacity, path_len;
+    int32_t batch, kv_heads, slots, capacity, path_len, count, advance;
     const int32_t* path;
     int64_t path_stride;
     const int32_t* kept;
     int32_t* counts;
     int32_t* overflow;
+    int32_t* tickets;
     pa_draft_move mv[PA_MAX_MOVES];
 };
 
@@ -358,43 +359,40 @@ __device__ __forceinline__ int commit_length(const DraftCommitDev& P, int b, int
     return min(bad, P.capacity - n);
 }
 
+// One workgroup per (row, move).  With advance the workgroup of a row that finishes last counts the kept
+// nodes: by then every other one has read the count (its ticket comes after), so one launch does both.
 __global__ __launch_bounds__(kDraftThreads) void k_draft_commit(const DraftCommitDev P) {
-    const int tid = threadIdx.x;
-    const int b = blockIdx.x / P.kv_heads;
+    const int tid = threadIdx.x, b = blockIdx.x;
     int n;
     bool over;
     const int len = commit_length(P, b, tid & 63, n, over);
     const pa_draft_move& M = P.mv[blockIdx.y];
-    const int64_t bh = blockIdx.x;
-    const char* src = static_cast<const char*>(M.src) + bh * P.slots * M.row_bytes;
-    char* dst = static_cast<char*>(M.dst) + (bh * P.capacity + n) * M.row_bytes;
-    if (M.row_bytes % 16 == 0) {
-        const int per = M.row_bytes / 16;
-        for (int x = tid; x < len * per; x += kDraftThreads) {
-            const int i = x / per, w = x % per;
-            reinterpret_cast<uint4*>(dst)[x] =
-                reinterpret_cast<const uint4*>(src + (int64_t)P.path[b * P.path_stride + i] * M.row_bytes)[w];
-        }
-    } else {
-        const int per = M.row_bytes / 4;
-        for (int x = tid; x < len * per; x += kDraftThreads) {
-            const int i = x / per, w = x % per;
-            reinterpret_cast<uint32_t*>(dst)[x] =
-                reinterpret_cast<const uint32_t*>(src + (int64_t)P.path[b * P.path_stride + i] * M.row_bytes)[w];
+    const int32_t* path = P.path + b * P.path_stride;
+    const int unit = M.row_bytes % 16 == 0 ? 16 : 4;
+    const int per = M.row_bytes / unit, head = len * per;
+    if (P.count > 0) {
+        const int64_t bh = (int64_t)b * P.kv_heads;
+        const char* src = static_cast<const char*>(M.src) + bh * P.slots * M.row_bytes;
+        char* dst = static_cast<char*>(M.dst) + (bh * P.capacity + n) * M.row_bytes;
+        const int64_t sh = (int64_t)P.slots * M.row_bytes, dh = (int64_t)P.capacity * M.row_bytes;
+        for (int64_t x = tid; x < (int64_t)head * P.kv_heads; x += kDraftThreads) {
+            const int64_t h = x / head;
+            const int y = (int)(x - h * head), i = y / per;
+            const char* from = src + h * sh + (int64_t)path[i] * M.row_bytes + (y - i * per) * unit;
+            char* to = dst + h * dh + (int64_t)y * unit;
+            if (unit == 16) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+            else *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
         }
     }
-}
-
-// the counts advance after every move has read them: a launch of its own
-__global__ __launch_bounds__(kDraftThreads) void k_draft_advance(const DraftCommitDev P) {
-    const int b = blockIdx.x * (kDraftThreads / 64) + (threadIdx.x >> 6);
-    if (b >= P.batch) return;
-    int n;
-    bool over;
-    const int len = commit_length(P, b, threadIdx.x & 63, n, over);
-    if ((threadIdx.x & 63) == 0) {
-        P.counts[b] = n + len;
-        if (over && P.overflow) *P.overflow = 1;
+    if (!P.advance) return;
+    __syncthreads();  // every wave has read the count
+    if (tid == 0) {
+        const int done = __hip_atomic_fetch_add(P.tickets + b, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        if (done == (int)gridDim.y - 1) {
+            P.counts[b] = n + len;
+            P.tickets[b] = 0;
+            if (over && P.overflow) *P.overflow = 1;
+        }
     }
 }
 
@@ -625,9 +623,8 @@ int launch_draft_append(const pa_draft_rows* r, hipStream_t s) {
 int launch_draft_commit(const pa_commit* c, hipStream_t s) {
     if (c->batch < 1 || c->kv_heads < 1 || c->slots < 1 || c->slots > PA_MAX_DRAFTS || c->capacity < 1 ||
         c->count < 0 || c->count > PA_MAX_MOVES || c->path_len < 0 || c->path_len > PA_MAX_DRAFTS ||
-        !c->path || !c->kept || !c->counts)
+        !c->path || !c->kept || !c->counts || (c->advance && !c->tickets))
         return PA_EINVAL;
-    if ((int64_t)c->batch * c->kv_heads > (1 << 30)) return PA_EUNSUPPORTED;
     DraftCommitDev P;
     P.batch = c->batch;
     P.kv_heads = c->kv_heads;
@@ -647,14 +644,12 @@ int launch_draft_commit(const pa_commit* c, hipStream_t s) {
             return PA_EINVAL;
         P.mv[k] = m;
     }
-    if (c->count > 0) {
+    P.count = c->count;
+    P.advance = c->advance;
+    P.tickets = c->tickets;
+    if (c->count > 0 || c->advance) {
         ProfScope ps("draft_commit", s);
-        hipLaunchKernelGGL(k_draft_commit, dim3(c->batch * c->kv_heads, c->count), dim3(kDraftThreads), 0, s, P);
-    }
-    if (c->advance) {
-        ProfScope ps("draft_advance", s);
-        constexpr int per = kDraftThreads / 64;
-        hipLaunchKernelGGL(k_draft_advance, dim3((c->batch + per - 1) / per), dim3(kDraftThreads), 0, s, P);
+        hipLaunchKernelGGL(k_draft_commit, dim3(c->batch, std::max(c->count, 1)), dim3(kDraftThreads), 0, s, P);
     }
     return PA_OK;
 }

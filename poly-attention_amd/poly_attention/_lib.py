@@ -371,6 +371,7 @@ class PaCommit(ctypes.Structure):
         ("kept", c_void_p),
         ("counts", c_void_p),
         ("overflow", c_void_p),
+        ("tickets", c_void_p),
         ("moves", PaDraftMove * PA_MAX_MOVES),
     ]
 
@@ -393,7 +394,10 @@ _PASS_FMT = "5i2f2i4x" + 5 * _VIEW_FMT + 2 * "Q2q" + 2 * _VIEW_FMT + "4Q"
 PACK_PASS = struct.Struct("@" + _PASS_FMT)
 PACK_PASS_GRAD = struct.Struct("@" + _PASS_FMT + 7 * _VIEW_FMT + "i4x2Q" + 2 * _VIEW_FMT)
 PACK_RMS = struct.Struct("@4if4x" + _VIEW_FMT + "Qi4x" + _VIEW_FMT + "Q" + 2 * _VIEW_FMT + "4Q2iq")
-for _pack, _cls in ((PACK_PASS, PaPass), (PACK_PASS_GRAD, PaPassGrad), (PACK_RMS, PaRmsNorm)):
+PACK_VERIFY = struct.Struct("@4iQ2qQqQqQqQqQQ2q5Q")
+PACK_COMMIT = struct.Struct("@6iQqi4x4Q")  # the moves follow
+assert PACK_COMMIT.size == PaCommit.moves.offset
+for _pack, _cls in ((PACK_VERIFY, PaVerify), (PACK_PASS, PaPass), (PACK_PASS_GRAD, PaPassGrad), (PACK_RMS, PaRmsNorm)):
     assert _pack.size == ctypes.sizeof(_cls), _cls.__name__
 
 
@@ -467,9 +471,9 @@ def _configure(lib) -> None:
     lib.pa_draft_verify_workspace.restype = c_size_t
     lib.pa_draft_verify_workspace.argtypes = [ctypes.POINTER(PaVerify)]
     lib.pa_draft_verify.restype = c_int
-    lib.pa_draft_verify.argtypes = [ctypes.POINTER(PaVerify), c_void_p]
+    lib.pa_draft_verify.argtypes = [c_void_p, c_void_p]  # packed structures
     lib.pa_draft_commit.restype = c_int
-    lib.pa_draft_commit.argtypes = [ctypes.POINTER(PaCommit), c_void_p]
+    lib.pa_draft_commit.argtypes = [c_void_p, c_void_p]
     lib.pa_linear_small.restype = c_int
     lib.pa_linear_small.argtypes = [ctypes.POINTER(PaLinear), c_void_p]
 

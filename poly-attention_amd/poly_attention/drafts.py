@@ -22,6 +22,7 @@ captured into a HIP graph.  The calls are for the GPU and for inference.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Sequence
 
 import torch
@@ -29,6 +30,18 @@ from torch import Tensor
 
 from . import _lib
 from ._lib import DTYPE_CODE, PA_MAX_DRAFTS, PA_MAX_MOVES
+
+
+def _call(fn, t: Tensor, what: str, *args) -> None:
+    """fn(*args, stream) on t's device and its current stream; raises on a failure status."""
+    index = t.device.index
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, what)
 
 
 def _need(ok: bool, what: str, error=ValueError) -> None:
@@ -44,18 +57,23 @@ def _set_view(v, t: Tensor) -> None:
     v.dtype = DTYPE_CODE[t.dtype]
 
 
-def _rows16(t: Tensor) -> bool:
-    """Unit feature stride and every row on 16 bytes."""
-    e = 16 // t.element_size()
-    s = t.stride()
-    return (s[3] == 1 and s[0] % e == 0 and s[1] % e == 0 and s[2] % e == 0
-            and t.data_ptr() % 16 == 0)
+def _rows16(t: Tensor) -> Tensor:
+    """``t`` [batch, heads, n, dim] with a unit feature stride and every row on 16 bytes, copied where it
+    has not."""
+    s0, s1, s2, s3 = t.stride()
+    if s3 == 1 and not ((s0 | s1 | s2) * t.element_size() | t.data_ptr()) & 15:
+        return t
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
 
 
 def _parents(parents: Optional[Tensor], batch: int, drafts: int, device) -> tuple:
     """(tensor to keep alive, address, elements between rows); a chain is (None, None, 0)."""
     if parents is None:
         return None, None, 0
+    if (parents.dtype is torch.int32 and parents.device == device and parents.shape == (batch, drafts)
+            and parents.stride(1) == 1):
+        return parents, parents.data_ptr(), parents.stride(0)
     _need(parents.device == device, "parents: on another device than the cache")
     _need(not parents.is_floating_point() and parents.dtype != torch.bool,
           "parents: an integer tensor", TypeError)
@@ -177,7 +195,10 @@ class DraftCache:
             mv.src, mv.dst = src.data_ptr(), dst.data_ptr()
             mv.row_bytes = src.element_size() * (dim_head if src.dim() == 4 else 1)
         self._moves = bytes(moves)
-        self._plans = {}
+        self._geometry = (batch, kv_heads, max_drafts, capacity)
+        # rows' tickets of a commit, 0 between calls
+        self._tickets = torch.zeros(batch, dtype=torch.int32, device=device)
+        self._plans = {}  # the calls' structures, by the shape of q1
 
     # -------------------------------------------------------------------------------------
 
@@ -189,6 +210,18 @@ class DraftCache:
               f"{what}: [{self.batch}, {heads}, {drafts}, {self.dim_head}], not {list(t.shape)}")
         _need(t.dtype == self.dtype, f"{what}: {t.dtype}, the cache holds {self.dtype}", TypeError)
         _need(t.device == self.device, f"{what}: on another device than the cache")
+
+    def _plan(self, kind: str, q1: Tensor):
+        """The call's structure for q1's shape, whose constant fields are set once."""
+        self._check_gpu()
+        _need(q1.dim() == 4, "q1: [batch, heads, drafts, dim_head]")
+        T, H = q1.shape[2], q1.shape[1]
+        _need(1 <= T <= self.max_drafts, f"{T} tokens: 1 to max_drafts = {self.max_drafts}")
+        _need(H >= 1 and H % self.kv_heads == 0, f"{H} heads over {self.kv_heads} kv_heads")
+        self._check_rows(q1, "q1", T, H)
+        plan = self._append_plan(T, H) if kind == "append" else self._attend_plan(T, H)
+        self._plans[kind, q1.shape] = plan
+        return plan
 
     def positions(self, drafts: int, parents: Optional[Tensor] = None) -> Tensor:
         """Positions [B, drafts] of a step's nodes: the row's count plus the node's depth (for
@@ -213,78 +246,90 @@ class DraftCache:
         a rotary module's frequencies at the nodes' positions, with its ``interp``olation factor.
         The result is rounded once.  Returns q1 [B, heads, T, d]; the others go to ``draft_qs`` and
         ``draft_vs``."""
-        self._check_gpu()
         q1 = qs[0]
         _need(len(qs) == self.order + 1 and len(vs) == self.order - 1 and len(weights) == len(qs),
               f"order {self.order}: {self.order + 1} qs and weights, {self.order - 1} vs")
-        _need(q1.dim() == 4, "q1: [batch, heads, drafts, dim_head]")
-        T, H = q1.shape[2], q1.shape[1]
-        _need(1 <= T <= self.max_drafts, f"{T} tokens: 1 to max_drafts = {self.max_drafts}")
-        _need(H >= 1 and H % self.kv_heads == 0, f"{H} heads over {self.kv_heads} kv_heads")
-        _need(angles is None or inv_freq is None, "angles or inv_freq, not both")
-        if torch.is_grad_enabled() and any(t.requires_grad for t in (*qs, *vs)):
-            raise RuntimeError("DraftCache steps are inference-only: run them under torch.no_grad()")
-        plan = self._plans.get(("append", T, H))
-        if plan is None:
-            plan = self._plans[("append", T, H)] = _lib.PaDraftRows()
-            plan.batch, plan.drafts, plan.dim, plan.count = self.batch, T, self.dim_head, 2 * self.order
-            plan.counts = self.counts.data_ptr()
-            for it, out in zip(plan.items[1:], (*self.draft_qs, *self.draft_vs)):
-                _set_view(it.out, out)
+        plan = self._plans.get(("append", q1.shape)) or self._plan("append", q1)
+        B, H, T, d = q1.shape
+        dtype, device, grad = self.dtype, self.device, torch.is_grad_enabled()
+        P, items = plan
         keep = []
-        out = torch.empty(self.batch, H, T, self.dim_head, dtype=self.dtype, device=self.device)
-        plan.eps = eps
-        _, plan.parents, plan.parents_stride = p = _parents(parents, self.batch, T, self.device)
-        keep.append(p[0])
-        plan.angles = plan.inv_freq = None
-        plan.rot_dim = 0
-        if angles is not None:
-            a = angles.detach()
-            _need(a.device == self.device, "angles: on another device than the cache")
-            r = a.shape[-1]
-            _need(a.shape in ((self.batch, T, r), (T, r), (r,)),
-                  f"angles: [{self.batch}, {T}, r], [{T}, r] or [r], not {list(a.shape)}")
-            if a.dtype not in DTYPE_CODE or (a.stride(-1) != 1 and r > 1):
-                a = a.to(a.dtype if a.dtype in DTYPE_CODE else torch.float32).contiguous()
-            keep.append(a)
-            plan.angles, plan.angles_dtype, plan.rot_dim = a.data_ptr(), DTYPE_CODE[a.dtype], r
-            plan.angles_sb = a.stride(0) if a.dim() == 3 else 0
-            plan.angles_sn = a.stride(-2) if a.dim() >= 2 else 0
-        elif inv_freq is not None:
-            _need(inv_freq.device == self.device and inv_freq.dim() == 1,
-                  "inv_freq: [r / 2] on the cache's device")
-            _need(interp > 0, "interp: above 0")
-            f = inv_freq.detach().to(torch.float32).contiguous()
-            keep.append(f)
-            plan.inv_freq, plan.rot_dim, plan.interp = f.data_ptr(), 2 * f.numel(), interp
-        _need(plan.rot_dim % 2 == 0 and plan.rot_dim <= self.dim_head,
-              f"{plan.rot_dim} angles: an even number up to dim_head = {self.dim_head}")
-        for k, src in enumerate((*qs, *vs)):
-            self._check_rows(src, "q%d" % (k + 1) if k <= self.order else "v%d" % (k - self.order + 2),
-                             T, H if k == 0 else self.kv_heads)
-            if not _rows16(src):
-                src = src.contiguous()
-                if src.data_ptr() % 16:
-                    src = src.clone()
-                keep.append(src)
-            it = plan.items[k]
-            _set_view(it.src, src)
-            w = weights[k] if k <= self.order else None
-            it.rotate = 1 if k <= self.order else 0
-            if w is None:
-                it.norm_weight = None
-            else:
-                _need(w.shape == (self.dim_head,) and w.device == self.device and w.dtype in DTYPE_CODE,
-                      f"norm weight {k}: [{self.dim_head}] on the cache's device")
+        P.eps = eps
+        parents, P.parents, P.parents_stride = _parents(parents, B, T, device)
+        self._set_angles(P, angles, inv_freq, interp, T, keep)
+        shape, kv = q1.shape, (B, self.kv_heads, T, d)
+        for k, (it, view) in enumerate(items):
+            norm = k <= self.order
+            src = qs[k] if norm else vs[k - self.order - 1]
+            if src.shape != shape or src.dtype is not dtype or src.device != device:
+                self._check_rows(src, "q%d" % (k + 1) if norm else "v%d" % (k - self.order + 2), T, shape[1])
+            if grad and src.requires_grad:
+                raise RuntimeError("DraftCache steps are inference-only: run them under torch.no_grad()")
+            shape = kv
+            rows = _rows16(src)
+            keep.append(rows)
+            view.ptr = rows.data_ptr()
+            view.sb, view.sh, view.sn, _ = rows.stride()
+            if norm:
+                w = weights[k]
+                if w is None:
+                    it.norm_weight = None
+                    continue
+                _need(w.shape == (d,) and w.device == device and w.dtype in DTYPE_CODE,
+                      f"norm weight {k}: [{d}] on the cache's device")
                 if w.stride(0) != 1:
                     w = w.contiguous()
                     keep.append(w)
                 it.norm_weight, it.weight_dtype = w.data_ptr(), DTYPE_CODE[w.dtype]
-        _set_view(plan.items[0].out, out)
-        from . import _ops
-
-        _ops._call(_lib.load().pa_draft_append, out, "pa_draft_append", ctypes.byref(plan))
+        out = torch.empty((B, H, T, d), dtype=dtype, device=device)
+        P.items[0].out.ptr = out.data_ptr()
+        _call(_lib.load().pa_draft_append, out, "pa_draft_append", ctypes.byref(P))
         return out
+
+    def _append_plan(self, T: int, H: int):
+        P = _lib.PaDraftRows()
+        P.batch, P.drafts, P.dim, P.count = self.batch, T, self.dim_head, 2 * self.order
+        P.counts = self.counts.data_ptr()
+        items = []
+        for k, (it, out) in enumerate(zip(P.items, (None, *self.draft_qs, *self.draft_vs))):
+            it.src.heads = it.out.heads = H if k == 0 else self.kv_heads
+            it.src.dtype = it.out.dtype = DTYPE_CODE[self.dtype]
+            it.rotate = 1 if k <= self.order else 0
+            if k:
+                _set_view(it.out, out)
+            else:
+                it.out.sb, it.out.sh, it.out.sn = H * T * self.dim_head, T * self.dim_head, self.dim_head
+            items.append((it, it.src))
+        return P, items
+
+    def _set_angles(self, P, angles, inv_freq, interp, T, keep) -> None:
+        if angles is None and inv_freq is None:
+            P.angles = P.inv_freq = None
+            P.rot_dim = 0
+            return
+        _need(angles is None or inv_freq is None, "angles or inv_freq, not both")
+        if angles is not None:
+            a, r = angles, angles.shape[-1]
+            _need(a.device == self.device, "angles: on another device than the cache")
+            _need(a.shape == (self.batch, T, r) or a.shape == (T, r) or a.shape == (r,),
+                  f"angles: [{self.batch}, {T}, r], [{T}, r] or [r], not {list(a.shape)}")
+            if a.dtype not in DTYPE_CODE or (a.stride(-1) != 1 and r > 1):
+                a = a.detach().to(a.dtype if a.dtype in DTYPE_CODE else torch.float32).contiguous()
+            P.inv_freq, P.angles, P.angles_dtype = None, a.data_ptr(), DTYPE_CODE[a.dtype]
+            s = a.stride()
+            P.angles_sb = s[0] if len(s) == 3 else 0
+            P.angles_sn = s[-2] if len(s) >= 2 else 0
+        else:
+            _need(inv_freq.device == self.device and inv_freq.dim() == 1,
+                  "inv_freq: [r / 2] on the cache's device")
+            _need(interp > 0, "interp: above 0")
+            a = inv_freq.detach().to(torch.float32).contiguous()
+            r = 2 * a.numel()
+            P.angles, P.inv_freq, P.interp = None, a.data_ptr(), interp
+        keep.append(a)
+        _need(r % 2 == 0 and r <= self.dim_head,
+              f"{r} angles: an even number up to dim_head = {self.dim_head}")
+        P.rot_dim = r
 
     def attend(self, q1: Tensor, *, parents: Optional[Tensor] = None, scale: Optional[float] = None,
                softclamp: Optional[float] = None) -> Tensor:
@@ -293,36 +338,26 @@ class DraftCache:
         the other levels' queries, keys and values are in the draft slots.  Writes ``draft_msgs`` and
         ``draft_lses`` and returns the output [B, heads, T, d].  ``scale`` defaults to
         dim_head ** -0.5."""
-        self._check_gpu()
-        _need(q1.dim() == 4, "q1: [batch, heads, drafts, dim_head]")
-        T, H = q1.shape[2], q1.shape[1]
-        _need(1 <= T <= self.max_drafts, f"{T} tokens: 1 to max_drafts = {self.max_drafts}")
-        _need(H >= 1 and H % self.kv_heads == 0, f"{H} heads over {self.kv_heads} kv_heads")
-        self._check_rows(q1, "q1", T, H)
-        if torch.is_grad_enabled() and q1.requires_grad:
+        plan = self._plans.get(("attend", q1.shape)) or self._plan("attend", q1)
+        B, H, T, d = q1.shape
+        dtype, device = self.dtype, self.device
+        if q1.dtype is not dtype or q1.device != device:
+            self._check_rows(q1, "q1", T, H)
+        if q1.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("DraftCache steps are inference-only: run them under torch.no_grad()")
-        lib = _lib.load()
-        plan = self._plans.get(("attend", T, H))
-        if plan is None:
-            plan = self._plans[("attend", T, H)] = self._attend_plan(T, H)
-        if not _rows16(q1):
-            q1 = q1.contiguous()
-            if q1.data_ptr() % 16:
-                q1 = q1.clone()
+        D, q, y, size, strides = plan
+        rows = _rows16(q1)
         # heads inner in memory: merging the heads afterwards is a view
-        out = torch.empty(self.batch, T, H, self.dim_head, dtype=self.dtype,
-                          device=self.device).permute(0, 2, 1, 3)
-        keep, plan.parents, plan.parents_stride = _parents(parents, self.batch, T, self.device)
-        last = plan.levels[self.order - 1]
-        _set_view(last.q, q1)
-        _set_view(last.out, out)
-        plan.scale = self.dim_head ** -0.5 if scale is None else scale
-        plan.softclamp = softclamp if softclamp else 0.0
-        ws = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=self.device)
-        plan.workspace = ws.data_ptr()
-        from . import _ops
-
-        _ops._call(lib.pa_draft_attend, out, "pa_draft_attend", ctypes.byref(plan))
+        out = torch.empty_strided((B, H, T, d), strides, dtype=dtype, device=device)
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        parents, D.parents, D.parents_stride = _parents(parents, B, T, device)
+        q.ptr = rows.data_ptr()
+        q.sb, q.sh, q.sn, _ = rows.stride()
+        y.ptr = out.data_ptr()
+        D.scale = d ** -0.5 if scale is None else scale
+        D.softclamp = softclamp if softclamp else 0.0
+        D.workspace = ws.data_ptr()
+        _call(_lib.load().pa_draft_attend, out, "pa_draft_attend", ctypes.byref(D))
         return out
 
     def _attend_plan(self, T: int, H: int):
@@ -354,7 +389,12 @@ class DraftCache:
         D.workspace_bytes = _lib.load().pa_draft_attend_workspace(ctypes.byref(D))
         _need(D.workspace_bytes > 0, f"{H} heads, {T} tokens over {self.kv_heads} kv_heads: too many",
               NotImplementedError)
-        return D
+        last = D.levels[self.order - 1]
+        strides = (T * H * self.dim_head, self.dim_head, H * self.dim_head, 1)
+        for v in (last.q, last.out):
+            v.heads, v.dtype = H, DTYPE_CODE[self.dtype]
+        last.out.sb, last.out.sh, last.out.sn, _ = strides
+        return D, last.q, last.out, D.workspace_bytes, strides
 
     def rotate_prefix(self, rotary) -> None:
         """Rotate the keys copied from a module's tuple cache in place, as the module's rotary rotates
@@ -389,36 +429,33 @@ def commit_drafts(caches: Sequence[DraftCache], path: Tensor, kept: Tensor) -> N
     slot; kept 0 leaves a row as it is).  Tokens past the capacity are dropped and flagged
     (``overflow``)."""
     c0 = caches[0]
-    c0._check_gpu()
+    counts, geometry, device = c0.counts, c0._geometry, c0.device
     for c in caches:
-        _need(c.counts is c0.counts, "caches of one commit share one counts tensor")
-        _need((c.batch, c.kv_heads, c.capacity, c.max_drafts) ==
-              (c0.batch, c0.kv_heads, c0.capacity, c0.max_drafts),
-              "caches of one commit have the same batch, kv_heads, capacity and max_drafts")
-    for t, what in ((path, "path"), (kept, "kept")):
-        _need(t.dtype == torch.int32, f"{what}: int32, not {t.dtype}", TypeError)
-        _need(t.device == c0.device, f"{what}: on another device than the caches")
-    _need(path.dim() == 2 and path.shape[0] == c0.batch and 1 <= path.shape[1] <= PA_MAX_DRAFTS,
-          f"path: [{c0.batch}, 1 to {PA_MAX_DRAFTS}], not {list(path.shape)}")
-    _need(kept.shape == (c0.batch,), f"kept: [{c0.batch}], not {list(kept.shape)}")
-    if path.stride(1) != 1 and path.shape[1] > 1:
-        path = path.contiguous()
-    kept = kept.contiguous()
-    C = _lib.PaCommit()
-    C.batch, C.kv_heads, C.slots, C.capacity = c0.batch, c0.kv_heads, c0.max_drafts, c0.capacity
-    C.path, C.path_stride, C.path_len = path.data_ptr(), path.stride(0), path.shape[1]
-    C.kept, C.counts, C.overflow = kept.data_ptr(), c0.counts.data_ptr(), c0.overflow.data_ptr()
-    moves = b"".join([c._moves for c in caches])
-    size = ctypes.sizeof(_lib.PaDraftMove)
-    total = len(moves) // size
-    from . import _ops
-
+        if c.counts is not counts or c._geometry != geometry:
+            _need(c.counts is counts, "caches of one commit share one counts tensor")
+            _need(False, "caches of one commit have the same batch, kv_heads, capacity and max_drafts")
+    B, hk, slots, capacity = geometry
+    if not (path.dtype is torch.int32 and kept.dtype is torch.int32 and path.device == device == kept.device
+            and path.dim() == 2 and path.shape[0] == B and 1 <= path.shape[1] <= PA_MAX_DRAFTS
+            and kept.shape == (B,) and path.stride(1) == 1 and kept.is_contiguous() and device.type == "cuda"):
+        c0._check_gpu()
+        for t, what in ((path, "path"), (kept, "kept")):
+            _need(t.dtype == torch.int32, f"{what}: int32, not {t.dtype}", TypeError)
+            _need(t.device == device, f"{what}: on another device than the caches")
+        _need(path.dim() == 2 and path.shape[0] == B and 1 <= path.shape[1] <= PA_MAX_DRAFTS,
+              f"path: [{B}, 1 to {PA_MAX_DRAFTS}], not {list(path.shape)}")
+        _need(kept.shape == (B,), f"kept: [{B}], not {list(kept.shape)}")
+        path, kept = path.contiguous(), kept.contiguous()
+    moves = c0._moves if len(caches) == 1 else b"".join([c._moves for c in caches])
+    size = PA_MAX_MOVES * ctypes.sizeof(_lib.PaDraftMove)
     fn = _lib.load().pa_draft_commit
-    for k in range(0, total, PA_MAX_MOVES):
-        C.count = min(PA_MAX_MOVES, total - k)
-        C.advance = 1 if k + PA_MAX_MOVES >= total else 0
-        ctypes.memmove(C.moves, moves[k * size:(k + C.count) * size], C.count * size)
-        _ops._call(fn, kept, "pa_draft_commit", ctypes.byref(C))
+    for k in range(0, len(moves), size):
+        part = moves if len(moves) <= size else moves[k:k + size]
+        head = _lib.PACK_COMMIT.pack(
+            B, hk, slots, capacity, len(part) // ctypes.sizeof(_lib.PaDraftMove), k + size >= len(moves),
+            path.data_ptr(), path.stride(0), path.shape[1], kept.data_ptr(), counts.data_ptr(),
+            c0.overflow.data_ptr(), c0._tickets.data_ptr())
+        _call(fn, kept, "pa_draft_commit", head + part)
 
 
 def verify_drafts(logits: Tensor, tokens: Tensor, parents: Optional[Tensor] = None, *,
@@ -454,47 +491,47 @@ def verify_drafts(logits: Tensor, tokens: Tensor, parents: Optional[Tensor] = No
     _need((uniforms is None) == (noise is None), "uniforms and noise go together")
     _need(uniforms is not None or (temperature is None and draft_probs is None),
           "temperature and draft_probs need uniforms and noise")
-    P = _lib.PaVerify()
-    keep = []
-
-    def fixed(t, what, shape, dtype):
-        _need(t.dtype == dtype, f"{what}: {dtype}, not {t.dtype}", TypeError)
-        _need(t.shape == shape, f"{what}: {list(shape)}, not {list(t.shape)}")
-        _need(t.device == dev, f"{what}: on another device than logits")
-        if t.stride(-1) != 1 and t.shape[-1] > 1:
-            t = t.contiguous()
-            keep.append(t)
-        return t
-
-    logits = logits.detach()
     if logits.stride(2) != 1 and V > 1:
         logits = logits.contiguous()
-    P.batch, P.drafts, P.vocab, P.dtype = B, T, V, DTYPE_CODE[logits.dtype]
-    P.logits, P.logits_sb, P.logits_sn = logits.data_ptr(), logits.stride(0), logits.stride(1)
-    tokens = fixed(tokens, "tokens", (B, T), torch.int64)
-    P.tokens, P.tokens_stride = tokens.data_ptr(), tokens.stride(0)
-    parents, P.parents, P.parents_stride = _parents(parents, B, T, dev)
-    if uniforms is not None:
-        uniforms = fixed(uniforms, "uniforms", (B, T), torch.float32)
-        P.uniforms, P.uniforms_stride = uniforms.data_ptr(), uniforms.stride(0)
-        noise = fixed(noise, "noise", (B, V), torch.float32)
-        P.noise, P.noise_stride = noise.data_ptr(), noise.stride(0)
-    if temperature is not None:
-        temperature = fixed(temperature, "temperature", (B,), torch.float32)
-        P.temperature = temperature.data_ptr()
-    if draft_probs is not None:
-        draft_probs = fixed(draft_probs.detach(), "draft_probs", (B, T, V), torch.float32)
-        P.draft_probs = draft_probs.data_ptr()
-        P.probs_sb, P.probs_sn = draft_probs.stride(0), draft_probs.stride(1)
-    path = torch.empty(B, T, dtype=torch.int32, device=dev)
+    keep = [logits]
+
+    def fixed(t, what, shape, dtype):
+        """Address and leading strides of an optional tensor that has to be of this shape and type."""
+        if t is None:
+            return (0,) * len(shape)
+        if t.dtype is not dtype or t.shape != shape or t.device != dev:
+            _need(t.dtype == dtype, f"{what}: {dtype}, not {t.dtype}", TypeError)
+            _need(t.shape == shape, f"{what}: {list(shape)}, not {list(t.shape)}")
+            _need(False, f"{what}: on another device than logits")
+        strides = t.stride()
+        if strides[-1] != 1 and shape[-1] > 1:
+            t = t.contiguous()
+            keep.append(t)
+            strides = t.stride()
+        return (t.data_ptr(), *strides[:-1])
+
+    parents, par_ptr, par_stride = _parents(parents, B, T, dev)
+    path = torch.empty((B, T), dtype=torch.int32, device=dev)
     kept = torch.empty(B, dtype=torch.int32, device=dev)
     token = torch.empty(B, dtype=torch.int64, device=dev)
-    P.path, P.kept, P.token = path.data_ptr(), kept.data_ptr(), token.data_ptr()
-    lib = _lib.load()
-    size = lib.pa_draft_verify_workspace(ctypes.byref(P))
+    size = _verify_workspace(B, T, V)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    P.workspace, P.workspace_bytes = ws.data_ptr(), size
-    from . import _ops
-
-    _ops._call(lib.pa_draft_verify, logits, "pa_draft_verify", ctypes.byref(P))
+    sb, sn, _ = logits.stride()
+    packed = _lib.PACK_VERIFY.pack(
+        B, T, V, DTYPE_CODE[logits.dtype], logits.data_ptr(), sb, sn,
+        *fixed(tokens, "tokens", (B, T), torch.int64), par_ptr or 0, par_stride,
+        *fixed(uniforms, "uniforms", (B, T), torch.float32), *fixed(noise, "noise", (B, V), torch.float32),
+        *fixed(temperature, "temperature", (B,), torch.float32),
+        *fixed(draft_probs, "draft_probs", (B, T, V), torch.float32),
+        path.data_ptr(), kept.data_ptr(), token.data_ptr(), ws.data_ptr(), size)
+    _call(_lib.load().pa_draft_verify, logits, "pa_draft_verify", packed)
     return path, kept, token
+
+
+@functools.lru_cache(maxsize=256)
+def _verify_workspace(B: int, T: int, V: int) -> int:
+    P = _lib.PaVerify()
+    P.batch, P.drafts, P.vocab = B, T, V
+    size = _lib.load().pa_draft_verify_workspace(ctypes.byref(P))
+    _need(size > 0, f"logits [{B}, {T}, {V}]: at most 65535 rows and 2^30 tokens", NotImplementedError)
+    return size

@@ -208,7 +208,7 @@ def test_verify_entry_refuses(path, value, want):
 def commit_args():
     C = _lib.PaCommit()
     C.batch, C.kv_heads, C.slots, C.capacity, C.count, C.advance, C.path_len = 2, 2, 8, 32, 1, 1, 8
-    C.path = C.kept = C.counts = FAKE
+    C.path = C.kept = C.counts = C.tickets = FAKE
     C.moves[0].src = C.moves[0].dst = FAKE
     C.moves[0].row_bytes = 128
     return C
@@ -216,7 +216,7 @@ def commit_args():
 
 @param("path,value", [
     ("batch", 0), ("kv_heads", 0), ("slots", 0), ("slots", 65), ("capacity", 0), ("count", 129), ("count", -1),
-    ("path_len", 65), ("path", None), ("kept", None), ("counts", None), ("moves.0.src", None),
+    ("path_len", 65), ("path", None), ("kept", None), ("counts", None), ("tickets", None), ("moves.0.src", None),
     ("moves.0.dst", None), ("moves.0.row_bytes", 0), ("moves.0.row_bytes", 6), ("moves.0.src", FAKE + 8),
 ])
 def test_commit_entry_refuses(path, value):
