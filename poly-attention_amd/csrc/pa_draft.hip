@@ -254,6 +254,19 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_append(const DraftRowsD
     const int b = blockIdx.x / P.T, t = blockIdx.x % P.T;
     const int sub = tid & (P.lpr - 1), d0 = sub * E;
     const bool in = d0 < P.dim;
+    const int per = kDraftThreads / P.lpr;  // rows at a time
+    auto item = [&](int row) __attribute__((always_inline)) -> const DraftItemDev& {
+        int k = 0;
+        while (k + 1 < P.count && row >= P.it[k + 1].row0) ++k;
+        return P.it[k];
+    };
+    auto fetch = [&](int row) __attribute__((always_inline)) -> u32x4_d {
+        if (!in || row >= P.rows) return u32x4_d{0u, 0u, 0u, 0u};
+        const DraftItemDev& I = item(row);
+        return load16u(I.src.at<T>(b, row - I.row0) + t * I.src.sn + d0);
+    };
+    const int row0 = blockIdx.y * per + tid / P.lpr;
+    u32x4_d next = fetch(row0);  // in flight over the sines
     float cs[E], sn[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -270,25 +283,29 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_append(const DraftRowsD
             pos = round_to<T>(round_to<T>((float)(P.counts[b] + mine)) / P.interp);
         }
         const int64_t at = b * P.angles_sb + t * P.angles_sn;
+        float a[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e)
+        for (int e = 0; e < E; ++e) {
+            const int d = min(d0 + e, P.rot_dim - 1);
+            a[e] = P.angles ? load_any(P.angles, P.adt, at + d) : pos * P.inv_freq[d >> 1];
+        }
+#pragma unroll
+        for (int e = 0; e < E; e += 2)
             if (d0 + e < P.rot_dim) {
-                const float a = P.angles ? load_any(P.angles, P.adt, at + d0 + e)
-                                         : pos * P.inv_freq[(d0 + e) >> 1];
-                cs[e] = cosf(a);
-                sn[e] = sinf(a);
+                sincosf(a[e], &sn[e], &cs[e]);
+                sn[e + 1] = sn[e];
+                cs[e + 1] = cs[e];
+                // a pair's features usually turn by one angle
+                if (a[e + 1] != a[e]) sincosf(a[e + 1], &sn[e + 1], &cs[e + 1]);
             }
     }
-    const int per = kDraftThreads / P.lpr;  // rows at a time
-    for (int row = blockIdx.y * per + tid / P.lpr; row - tid / P.lpr < P.rows; row += gridDim.y * per) {
+    for (int row = row0; row - tid / P.lpr < P.rows; row += gridDim.y * per) {
+        const u32x4_d raw = next;
         const bool on = row < P.rows;
-        int k = 0;
-        while (k + 1 < P.count && row >= P.it[k + 1].row0) ++k;
-        const DraftItemDev& I = P.it[k];
+        const DraftItemDev& I = item(row);
         const int h = (on ? row : P.rows - 1) - I.row0;
+        next = fetch(row + gridDim.y * per);
         float x[E];
-        u32x4_d raw = {0u, 0u, 0u, 0u};
-        if (in) raw = load16u(I.src.at<T>(b, h) + t * I.src.sn + d0);
         if constexpr (E == 4) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(raw[e]);
@@ -375,9 +392,9 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_commit(const DraftCommi
         const char* src = static_cast<const char*>(M.src) + bh * P.slots * M.row_bytes;
         char* dst = static_cast<char*>(M.dst) + (bh * P.capacity + n) * M.row_bytes;
         const int64_t sh = (int64_t)P.slots * M.row_bytes, dh = (int64_t)P.capacity * M.row_bytes;
-        for (int64_t x = tid; x < (int64_t)head * P.kv_heads; x += kDraftThreads) {
-            const int64_t h = x / head;
-            const int y = (int)(x - h * head), i = y / per;
+        const unsigned all = (unsigned)head * P.kv_heads;  // at most 64 rows of 256 units per head
+        for (unsigned x = tid; x < all; x += kDraftThreads) {
+            const unsigned h = x / (unsigned)head, y = x - h * head, i = y / (unsigned)per;
             const char* from = src + h * sh + (int64_t)path[i] * M.row_bytes + (y - i * per) * unit;
             char* to = dst + h * dh + (int64_t)y * unit;
             if (unit == 16) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
@@ -387,7 +404,9 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_commit(const DraftCommi
     if (!P.advance) return;
     __syncthreads();  // every wave has read the count
     if (tid == 0) {
-        const int done = __hip_atomic_fetch_add(P.tickets + b, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        // relaxed: nothing that another workgroup wrote is read after it, and this one's read of the count has
+        // returned (the length depends on it); a release would write the L2 back, at several us
+        const int done = __hip_atomic_fetch_add(P.tickets + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (done == (int)gridDim.y - 1) {
             P.counts[b] = n + len;
             P.tickets[b] = 0;
@@ -625,6 +644,7 @@ int launch_draft_commit(const pa_commit* c, hipStream_t s) {
         c->count < 0 || c->count > PA_MAX_MOVES || c->path_len < 0 || c->path_len > PA_MAX_DRAFTS ||
         !c->path || !c->kept || !c->counts || (c->advance && !c->tickets))
         return PA_EINVAL;
+    if (c->kv_heads > (1 << 15)) return PA_EUNSUPPORTED;  // 32-bit indexes of a row's vectors
     DraftCommitDev P;
     P.batch = c->batch;
     P.kv_heads = c->kv_heads;
@@ -639,7 +659,7 @@ int launch_draft_commit(const pa_commit* c, hipStream_t s) {
     for (int k = 0; k < c->count; ++k) {
         const pa_draft_move& m = c->moves[k];
         const int a = m.row_bytes % 16 == 0 ? 16 : 4;
-        if (!m.src || !m.dst || m.row_bytes < 4 || m.row_bytes % 4 != 0 || (uintptr_t)m.src % a != 0 ||
+        if (!m.src || !m.dst || m.row_bytes < 4 || m.row_bytes > 4096 || m.row_bytes % 4 != 0 || (uintptr_t)m.src % a != 0 ||
             (uintptr_t)m.dst % a != 0)
             return PA_EINVAL;
         P.mv[k] = m;

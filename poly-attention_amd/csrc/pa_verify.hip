@@ -17,7 +17,7 @@ namespace pa {
 namespace {
 
 constexpr int kVerThreads = 256;
-constexpr int kVerChunk = 8192;  // entries of a workgroup: 32 per thread, held in registers
+constexpr int kVerChunk = 4096;  // entries of a workgroup: 16 per thread, held in registers
 
 struct VerifyDev {
     int32_t batch, T, vocab, chunks;
@@ -80,10 +80,17 @@ __device__ __forceinline__ void load_entries(const T* row, int64_t i, int n, flo
     }
 }
 
-__device__ __forceinline__ float wave_max(float x) {
-    for (int off = 32; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off));
-    return x;
+// E floats of a row of n at entry i, of any alignment; what lies outside is 1
+template <int E>
+__device__ __forceinline__ void load_floats(const float* row, int64_t i, int n, float (&x)[E]) {
+    if (i >= 0 && i + E <= n) {
+        __builtin_memcpy(x, row + i, sizeof(x));
+    } else {
+#pragma unroll
+        for (int k = 0; k < E; ++k) x[k] = i + k >= 0 && i + k < n ? row[i + k] : 1.f;
+    }
 }
+
 __device__ __forceinline__ float wave_sum(float x) {
     for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off);
     return x;
@@ -159,11 +166,10 @@ __device__ __forceinline__ uint64_t best_key(float w, float noise, int64_t i) {
 template <typename T>
 __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) {
     constexpr int E = VerVec<T>::E, N = VerVec<T>::N;
-    __shared__ float s_top[64], s_inv[64], s_px[64], s_qx[64], s_u[64], s_rinv[64];
-    __shared__ int s_arg[64], s_parent[64], s_path[64], s_rej[64];
-    __shared__ int64_t s_tok[64];
-    __shared__ uint64_t s_live, s_best[4][2];
-    __shared__ float s_wave[4];
+    __shared__ float s_top[64], s_inv[64], s_rinv[64], s_wave[4];
+    __shared__ int s_arg[64];
+    __shared__ int64_t s_rej[64];
+    __shared__ uint64_t s_best[4][2];
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int chunk = blockIdx.x, b = blockIdx.y;
@@ -172,117 +178,113 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
     const float c = greedy ? 0.f : kLog2e / temp;
     const int32_t* parents = P.parents ? P.parents + b * P.parents_stride : nullptr;
 
-    // the nodes: statistics over the chunks (four threads each), tokens, random numbers
-    {
+    // every wave holds the nodes, one per lane, and walks for itself
+    const bool node = lane < P.T;
+    const int parent = node ? (parents ? parents[lane] : lane - 1) : -2;
+    const int64_t tok = node ? P.tokens[b * P.tokens_stride + lane] : -1;
+    const float u = node && !greedy ? P.uniforms[b * P.uniforms_stride + lane] : 0.f;
+    {   // statistics over the chunks, four threads per node
         const int t = tid >> 2, sub = tid & 3;
         float top = -INFINITY, sum = 0.f;
         int at = P.vocab;
-        if (t < P.T) {
-            const float4* st = P.stats + ((int64_t)b * P.T + t) * P.chunks;
-            for (int k = sub; k < P.chunks; k += 4) take_first(top, at, st[k].x, __float_as_int(st[k].z));
+        const float4* st = P.stats + ((int64_t)b * P.T + t) * P.chunks;
+        if (t < P.T)
+#pragma unroll 4
+            for (int k = sub; k < P.chunks; k += 4) {
+                const float4 x = st[k];
+                const float was = top;
+                take_first(top, at, x.x, __float_as_int(x.z));
+                if (!greedy) {
+                    sum = was == -INFINITY ? sum : sum * __builtin_amdgcn_exp2f((was - top) * c);
+                    sum += x.x == -INFINITY ? x.y : x.y * __builtin_amdgcn_exp2f((x.x - top) * c);  // y: 0, or NaN
+                }
+            }
+        for (int off = 1; off < 4; off <<= 1) {
+            const float was = top, x = __shfl_xor(top, off), y = __shfl_xor(sum, off);
+            take_first(top, at, x, __shfl_xor(at, off));
+            if (!greedy)
+                sum = (was == -INFINITY ? sum : sum * __builtin_amdgcn_exp2f((was - top) * c)) +
+                      (x == -INFINITY ? y : y * __builtin_amdgcn_exp2f((x - top) * c));
         }
-        for (int off = 1; off < 4; off <<= 1) take_first(top, at, __shfl_xor(top, off), __shfl_xor(at, off));
-        if (t < P.T && !greedy) {
-            const float4* st = P.stats + ((int64_t)b * P.T + t) * P.chunks;
-            for (int k = sub; k < P.chunks; k += 4)
-                sum += st[k].x == -INFINITY ? st[k].y  // 0, or NaN
-                                            : st[k].y * __builtin_amdgcn_exp2f((st[k].x - top) * c);
-        }
-        sum += __shfl_xor(sum, 1);
-        sum += __shfl_xor(sum, 2);
         if (t < P.T && sub == 0) {
             s_top[t] = top;
             s_inv[t] = 1.f / sum;
             s_arg[t] = at;
-            s_parent[t] = parents ? parents[t] : t - 1;
-            s_tok[t] = P.tokens[b * P.tokens_stride + t];
-            s_u[t] = greedy ? 0.f : P.uniforms[b * P.uniforms_stride + t];
         }
     }
-    if (wave == 0) {
-        const uint64_t anc = draft_ancestors(parents, P.T, lane);
-        const uint64_t live = __ballot(anc != 0);
-        if (lane == 0) s_live = live;
-    }
+    const uint64_t live = __ballot(draft_ancestors(parents, P.T, lane) != 0);
     __syncthreads();
-    const uint64_t live = s_live;
-    // each node's own probabilities under its parent
-    if (tid < P.T) {
-        const int p = s_parent[tid];
-        const int64_t tok = s_tok[tid];
-        float px = 0.f, qx = 1.f;
-        if (((live >> tid) & 1) && p >= 0 && tok >= 0 && tok < P.vocab) {
-            if (greedy) {
-                px = tok == s_arg[p] ? 1.f : 0.f;
-            } else {
-                const float x = to_f(reinterpret_cast<const T*>(P.logits)[b * P.logits_sb + p * P.logits_sn + tok]);
-                px = __builtin_amdgcn_exp2f((x - s_top[p]) * c) * s_inv[p];
-            }
-            if (P.probs) qx = P.probs[b * P.probs_sb + p * P.probs_sn + tok];
+    // each node's own probability under its parent
+    float px = 0.f, qx = 1.f;
+    if (((live >> lane) & 1) && parent >= 0 && tok >= 0 && tok < P.vocab) {
+        if (greedy) {
+            px = tok == s_arg[parent] ? 1.f : 0.f;
+        } else {
+            const float x = to_f(reinterpret_cast<const T*>(P.logits)[b * P.logits_sb + parent * P.logits_sn + tok]);
+            px = __builtin_amdgcn_exp2f((x - s_top[parent]) * c) * s_inv[parent];
         }
-        s_px[tid] = px;
-        s_qx[tid] = qx;
+        if (P.probs) qx = P.probs[b * P.probs_sb + parent * P.probs_sn + tok];
     }
-    __syncthreads();
 
-    // the walk, the same in every thread
+    // the walk: the current node's children in order.  All of it is the same in every wave.
     int cur = 0, kept = live & 1 ? 1 : 0, nrej = 0;  // rejected children of cur
+    uint64_t path = kept, rejected = 0;               // kept nodes, rejected children whose token is out of p
     float left = 1.f;                                 // without probs: 1 - their probabilities
-    if (tid == 0) s_path[0] = kept ? 0 : -1;
     const T* row = reinterpret_cast<const T*>(P.logits) + b * P.logits_sb;
     const float* qrow = P.probs ? P.probs + b * P.probs_sb : nullptr;
-    for (int t = 1; kept && t < P.T; ++t) {
-        if (!((live >> t) & 1) || s_parent[t] != cur) continue;
-        const int64_t tok = s_tok[t];
-        float px = s_px[t], qx = s_qx[t];
-        if (!greedy && nrej > 0) {
+    uint64_t children = kept ? __ballot(((live >> lane) & 1) && parent == 0) : 0;
+    while (children) {
+        const int t = __ffsll((unsigned long long)children) - 1;
+        children &= children - 1;
+        float pt = __shfl(px, t);
+        const float qt = __shfl(qx, t), ut = __shfl(u, t);
+        const int64_t xt = __shfl((long long)tok, t);
+        if (nrej > 0) {
             if (P.probs) {
                 // the sum of the newest residual, now that a further child needs it
+                const float top = s_top[cur], inv = s_inv[cur];
                 float part = 0.f;
                 for (int64_t i = tid; i < P.vocab; i += kVerThreads) {
-                    const float p = __builtin_amdgcn_exp2f((to_f(row[cur * P.logits_sn + i]) - s_top[cur]) * c) * s_inv[cur];
+                    const float p = __builtin_amdgcn_exp2f((to_f(row[cur * P.logits_sn + i]) - top) * c) * inv;
                     const float q = qrow[cur * P.probs_sn + i];
                     part += fmaxf(residual(p, q, s_rinv, nrej - 1) - q, 0.f);
                 }
                 part = wave_sum(part);
-                __syncthreads();
                 if (lane == 0) s_wave[wave] = part;
                 __syncthreads();
                 const float sum = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
                 if (tid == 0) s_rinv[nrej - 1] = sum > 0.f ? 1.f / sum : 0.f;
                 __syncthreads();
-                px = tok >= 0 && tok < P.vocab ? residual(px, qx, s_rinv, nrej) : 0.f;
+                pt = xt >= 0 && xt < P.vocab ? residual(pt, qt, s_rinv, nrej) : 0.f;
             } else {
-                for (int k = 0; k < nrej; ++k)
-                    if (s_tok[s_rej[k]] == tok) px = 0.f;
-                px /= left;
+                if (__any(((rejected >> lane) & 1) && tok == xt)) pt = 0.f;
+                pt /= left;
             }
         }
-        if (s_u[t] * qx < px) {
+        if (ut * qt < pt) {
             cur = t;
-            if (tid == 0) s_path[kept] = t;
             ++kept;
+            path |= 1ull << t;
             nrej = 0;
+            rejected = 0;
             left = 1.f;
+            children = __ballot(((live >> lane) & 1) && parent == t);
         } else if (!greedy) {
             if (P.probs) {
                 ++nrej;
-            } else if (px > 0.f) {
-                // removed from p, unless it was all of p
-                const float rest = left - px * left;
-                if (rest > 0.f) {
-                    if (tid == 0) s_rej[nrej] = t;
-                    ++nrej;
-                    left = rest;
-                }
+            } else if (pt > 0.f && left - pt * left > 0.f) {  // out of p, unless it was all of p
+                rejected |= 1ull << t;
+                left -= pt * left;
+                ++nrej;
             }
         }
-        __syncthreads();
     }
-    __syncthreads();
-    if (chunk == 0) {
-        for (int t = tid; t < P.T; t += kVerThreads) P.path[(int64_t)b * P.T + t] = t < kept ? s_path[t] : -1;
-        if (tid == 0) P.kept[b] = kept;
+    if (chunk == 0 && wave == 0) {
+        int32_t* to = P.path + (int64_t)b * P.T;
+        const uint64_t below = path & ((1ull << lane) - 1);
+        if ((path >> lane) & 1) to[__popcll(below)] = lane;
+        if (node && lane >= kept) to[lane] = -1;
+        if (lane == 0) P.kept[b] = kept;
     }
     if (!kept || greedy) {
         if (chunk == 0 && tid == 0)
@@ -298,31 +300,42 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
     const float* noise = P.noise + b * P.noise_stride;
     const int shift = (int)(((uintptr_t)row & 15) / sizeof(T));
     const int64_t i0 = (int64_t)chunk * kVerChunk - shift;
+    const int nout = P.probs ? 0 : nrej;
+    if (wave == 0 && ((rejected >> lane) & 1)) s_rej[__popcll(rejected & ((1ull << lane) - 1))] = tok;
+    float x[N][E], nz[N][E];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int64_t i = i0 + (int64_t)(k * kVerThreads + tid) * E;
+        load_entries<T>(row, i, P.vocab, -INFINITY, x[k]);
+        load_floats<E>(noise, i, P.vocab, nz[k]);
+    }
+    __syncthreads();
     uint64_t best = 0, alt = 0;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         const int64_t i = i0 + (int64_t)(k * kVerThreads + tid) * E;
-        if (i >= P.vocab) continue;
-        float x[E];
-        load_entries<T>(row, i, P.vocab, -INFINITY, x);
+        float w[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[e] = __builtin_amdgcn_exp2f((x[k][e] - top) * c) * inv;  // 0 outside
+        if (q) {
+            float qj[E];
+            load_floats<E>(q, i, P.vocab, qj);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                w[e] = residual(w[e], qj[e], s_rinv, nrej - 1);
+                const uint64_t key = best_key(w[e], nz[k][e], i + e);
+                alt = key > alt ? key : alt;
+                w[e] = fmaxf(w[e] - qj[e], 0.f);
+            }
+        }
+        for (int r = 0; r < nout; ++r) {
+            const int64_t out = s_rej[r] - i;
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[e] = out == e ? 0.f : w[e];
+        }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int64_t j = i + e;
-            if (j < 0 || j >= P.vocab) continue;
-            float w = __builtin_amdgcn_exp2f((x[e] - top) * c) * inv;
-            const float nz = noise[j];
-            uint64_t key;
-            if (q) {
-                const float qj = q[j];
-                w = residual(w, qj, s_rinv, nrej - 1);
-                key = best_key(w, nz, j);
-                alt = key > alt ? key : alt;
-                w = fmaxf(w - qj, 0.f);
-            } else {
-                for (int r = 0; r < nrej; ++r)
-                    if (s_tok[s_rej[r]] == j) w = 0.f;
-            }
-            key = best_key(w, nz, j);
+            const uint64_t key = best_key(w[e], nz[k][e], i + e);
             best = key > best ? key : best;
         }
     }
@@ -344,8 +357,10 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
         uint64_t* to = P.best + ((int64_t)b * P.chunks + chunk) * 2;
         __hip_atomic_store(to, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __hip_atomic_store(to + 1, alt, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        // the release orders the two stores before the ticket, the acquire the others' before the reads
-        const uint32_t n = __hip_atomic_fetch_add(P.ticket + b, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        // The stores and the loads below act at the level that all of the GPU shares, so it is enough that the
+        // stores have ended before the ticket is drawn; a release would write the L2 back, at several us.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const uint32_t n = __hip_atomic_fetch_add(P.ticket + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         s_last = n == (uint32_t)P.chunks - 1;
     }
     __syncthreads();
