@@ -57,6 +57,7 @@ extern "C" {
 #define PA_MAX_ORDER 8
 #define PA_MAX_DRAFTS 64   /* drafted tokens per row of one step */
 #define PA_MAX_MOVES 128   /* array pairs of one pa_draft_commit */
+#define PA_TICKET_STRIDE 32  /* int32 per row of its tickets */
 
 /* status codes (0 = success, negative = failure) */
 #define PA_OK            0
@@ -469,7 +470,7 @@ typedef struct pa_commit {
     const int32_t* kept;        /* device [B] */
     int32_t*       counts;      /* device [B] */
     int32_t*       overflow;    /* device [1], or NULL */
-    int32_t*       tickets;     /* device [B]; required with advance */
+    int32_t*       tickets;     /* device [B * PA_TICKET_STRIDE]; required with advance */
     pa_draft_move  moves[PA_MAX_MOVES];
 } pa_commit;
 

@@ -21,6 +21,9 @@ namespace pa {
 
 constexpr int kDraftThreads = 256;
 constexpr int kDraftChunk = 128;  // a unit covers a multiple of this many positions (4 waves x 32)
+// tickets of different rows lie on cache lines of their own: atomics on one line follow one another (432 of
+// them on one line took 4 us)
+constexpr int kTicketStride = PA_TICKET_STRIDE;
 constexpr float kDraftTau = 8.f;  // lazy-rescale headroom of the running maximum (log2 units)
 
 struct DraftRow {  // a [B, h, n, dim] array: base and element strides

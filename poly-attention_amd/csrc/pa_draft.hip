@@ -227,17 +227,17 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_combine(const DraftDev 
 }
 
 // ---------------------------------------------------------------------------------------
-// Norms and rotary of a step's nodes into their draft slots.  One workgroup per (node, part of its
-// rows), a lane holding 16 bytes of a row: a lane's features are the same in all its rows, so the
-// sines and cosines are computed once per lane (they cost more than the rows).
+// Norms and rotary of a step's nodes into their draft slots.  One workgroup per (node, tensor), a lane
+// holding 16 bytes of a row: a lane's features are the same in all its rows, so the sines and cosines
+// are computed once per lane (they cost more than the rows), while the first rows are on their way.
 
 struct DraftItemDev {
     DraftRow src, out;
     const void* w;
-    int32_t wdt, rotate, row0;
+    int32_t wdt, rotate, heads;
 };
 struct DraftRowsDev {
-    int32_t batch, T, dim, count, rows, rot_dim, adt, lpr;
+    int32_t batch, T, dim, count, rot_dim, adt, lpr;
     float eps, interp;
     const int32_t* counts;
     const int32_t* parents;
@@ -247,103 +247,128 @@ struct DraftRowsDev {
     DraftItemDev it[2 * PA_MAX_ORDER];
 };
 
+// E values of any of the types from p[i]
+template <int E>
+__device__ __forceinline__ void load_row(const void* p, int dtype, int64_t i, float (&x)[E]) {
+    if (dtype == PA_F32) {
+        __builtin_memcpy(x, static_cast<const float*>(p) + i, sizeof(x));
+    } else if (dtype == PA_F16) {
+        f16 r[E];
+        __builtin_memcpy(r, static_cast<const f16*>(p) + i, sizeof(r));
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = to_f(r[e]);
+    } else {
+        bf16 r[E];
+        __builtin_memcpy(r, static_cast<const bf16*>(p) + i, sizeof(r));
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = to_f(r[e]);
+    }
+}
+
 template <typename T>
 __global__ __launch_bounds__(kDraftThreads) void k_draft_append(const DraftRowsDev P) {
-    constexpr int E = 16 / sizeof(T);
+    constexpr int E = 16 / sizeof(T), U = 2;  // rows of a thread in flight
     const int tid = threadIdx.x, lane = tid & 63;
     const int b = blockIdx.x / P.T, t = blockIdx.x % P.T;
+    const DraftItemDev& I = P.it[blockIdx.y];
     const int sub = tid & (P.lpr - 1), d0 = sub * E;
     const bool in = d0 < P.dim;
-    const int per = kDraftThreads / P.lpr;  // rows at a time
-    auto item = [&](int row) __attribute__((always_inline)) -> const DraftItemDev& {
-        int k = 0;
-        while (k + 1 < P.count && row >= P.it[k + 1].row0) ++k;
-        return P.it[k];
+    const int per = kDraftThreads / P.lpr, first = tid / P.lpr;  // rows (heads) at a time
+    const T* src = I.src.at<T>(b, 0) + t * I.src.sn + d0;
+    T* out = I.out.at<T>(b, 0) + t * I.out.sn + d0;
+    u32x4_d raw[U];
+    auto fetch = [&](int h0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            raw[u] = u32x4_d{0u, 0u, 0u, 0u};
+            if (in && h0 + u * per < I.heads) raw[u] = load16u(src + (h0 + u * per) * I.src.sh);
+        }
     };
-    auto fetch = [&](int row) __attribute__((always_inline)) -> u32x4_d {
-        if (!in || row >= P.rows) return u32x4_d{0u, 0u, 0u, 0u};
-        const DraftItemDev& I = item(row);
-        return load16u(I.src.at<T>(b, row - I.row0) + t * I.src.sn + d0);
-    };
-    const int row0 = blockIdx.y * per + tid / P.lpr;
-    u32x4_d next = fetch(row0);  // in flight over the sines
-    float cs[E], sn[E];
+    fetch(first);
+    float w[E], cs[E], sn[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
+        w[e] = 0.f;
         cs[e] = 1.f;
         sn[e] = 0.f;
     }
-    if (P.rot_dim > 0) {
-        float pos = 0.f;
-        if (!P.angles) {  // the position as the rotary module builds it, rounded to the rows' type
+    if (I.w && in) load_row<E>(I.w, I.wdt, d0, w);
+    const bool turn = I.rotate && P.rot_dim > 0;
+    if (turn) {
+        float a[E];
+        if (P.angles) {
+            const int64_t at = b * P.angles_sb + t * P.angles_sn;
+            if (d0 + E <= P.rot_dim) {
+                load_row<E>(P.angles, P.adt, at + d0, a);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    a[e] = d0 + e < P.rot_dim ? load_any(P.angles, P.adt, at + d0 + e) : 0.f;
+            }
+        } else {  // the position as the rotary module builds it, rounded to the rows' type
             const uint64_t anc = draft_ancestors(P.parents ? P.parents + b * P.parents_stride : nullptr,
                                                  P.T, lane);
             const int depth = __popcll(anc) - 1;
             const int mine = max(0, __shfl(depth, t));
-            pos = round_to<T>(round_to<T>((float)(P.counts[b] + mine)) / P.interp);
-        }
-        const int64_t at = b * P.angles_sb + t * P.angles_sn;
-        float a[E];
+            const float pos = round_to<T>(round_to<T>((float)(P.counts[b] + mine)) / P.interp);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int d = min(d0 + e, P.rot_dim - 1);
-            a[e] = P.angles ? load_any(P.angles, P.adt, at + d) : pos * P.inv_freq[d >> 1];
+            for (int e = 0; e < E; ++e) a[e] = d0 + e < P.rot_dim ? pos * P.inv_freq[(d0 + e) >> 1] : 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < E; e += 2)
-            if (d0 + e < P.rot_dim) {
-                sincosf(a[e], &sn[e], &cs[e]);
-                sn[e + 1] = sn[e];
-                cs[e + 1] = cs[e];
-                // a pair's features usually turn by one angle
-                if (a[e + 1] != a[e]) sincosf(a[e + 1], &sn[e + 1], &cs[e + 1]);
-            }
+        for (int e = 0; e < E; e += 2) {
+            sincosf(a[e], &sn[e], &cs[e]);
+            sn[e + 1] = sn[e];
+            cs[e + 1] = cs[e];
+            // a pair's features usually turn by one angle
+            if (a[e + 1] != a[e]) sincosf(a[e + 1], &sn[e + 1], &cs[e + 1]);
+        }
     }
-    for (int row = row0; row - tid / P.lpr < P.rows; row += gridDim.y * per) {
-        const u32x4_d raw = next;
-        const bool on = row < P.rows;
-        const DraftItemDev& I = item(row);
-        const int h = (on ? row : P.rows - 1) - I.row0;
-        next = fetch(row + gridDim.y * per);
-        float x[E];
-        if constexpr (E == 4) {
+    for (int h0 = 0; h0 < I.heads; h0 += U * per) {
+        u32x4_d y[U];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(raw[e]);
-        } else {
-            typedef T t2 __attribute__((ext_vector_type(2)));
+        for (int u = 0; u < U; ++u) {
+            float x[E];
+            if constexpr (E == 4) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(raw[u][e]);
+            } else {
+                typedef T t2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t word = raw[u][e];  // a value: a bit cast of the element reads element 0
+                    const t2 z = __builtin_bit_cast(t2, word);
+                    x[2 * e] = (float)z[0];
+                    x[2 * e + 1] = (float)z[1];
+                }
+            }
+            if (I.w) {
+                float ss = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) ss += x[e] * x[e];
+                for (int off = 1; off < P.lpr; off <<= 1) ss += __shfl_xor(ss, off);
+                const float r = rsqrtf(ss / (float)P.dim + P.eps);
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[e] = x[e] * r * w[e];
+            }
+            if (turn) {
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    const float z = x[e] * cs[e] - x[e + 1] * sn[e];
+                    x[e + 1] = x[e + 1] * cs[e + 1] + x[e] * sn[e + 1];
+                    x[e] = z;
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t word = raw[e];  // a value: a bit cast of the element itself reads element 0
-                const t2 y = __builtin_bit_cast(t2, word);
-                x[2 * e] = (float)y[0];
-                x[2 * e + 1] = (float)y[1];
+                if constexpr (E == 4) y[u][e] = __float_as_uint(x[e]);
+                else y[u][e] = draft_pack2<T>(x[2 * e], x[2 * e + 1]);
             }
         }
-        float ss = 0.f;
+        fetch(first + h0 + U * per);
 #pragma unroll
-        for (int e = 0; e < E; ++e) ss += x[e] * x[e];
-        for (int off = 1; off < P.lpr; off <<= 1) ss += __shfl_xor(ss, off);
-        if (I.w && in) {
-            const float r = rsqrtf(ss / (float)P.dim + P.eps);
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = x[e] * r * load_any(I.w, I.wdt, d0 + e);
-        }
-        if (I.rotate && P.rot_dim > 0) {
-#pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                const float y0 = x[e] * cs[e] - x[e + 1] * sn[e];
-                x[e + 1] = x[e + 1] * cs[e + 1] + x[e] * sn[e + 1];
-                x[e] = y0;
-            }
-        }
-        if (on && in) {
-            u32x4_d y;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if constexpr (E == 4) y[e] = __float_as_uint(x[e]);
-                else y[e] = draft_pack2<T>(x[2 * e], x[2 * e + 1]);
-            }
-            *reinterpret_cast<u32x4_d*>(I.out.at<T>(b, h) + t * I.out.sn + d0) = y;
+        for (int u = 0; u < U; ++u) {
+            const int h = first + h0 + u * per;
+            if (in && h < I.heads) *reinterpret_cast<u32x4_d*>(out + h * I.out.sh) = y[u];
         }
     }
 }
@@ -363,55 +388,70 @@ struct DraftCommitDev {
 };
 
 // entries of row b's path that are moved: up to the first one outside the slots, within the capacity
-__device__ __forceinline__ int commit_length(const DraftCommitDev& P, int b, int lane, int& n, bool& over) {
+// (lane i's entry in p)
+__device__ __forceinline__ int commit_length(const DraftCommitDev& P, int b, int lane, int& n, int& p, bool& over) {
+    p = lane < P.path_len ? P.path[b * P.path_stride + lane] : -1;
     n = min(max(P.counts[b], 0), P.capacity);
     const int want = min(max(P.kept[b], 0), P.path_len);
-    int bad = want;
-    if (lane < want) {
-        const int p = P.path[b * P.path_stride + lane];
-        if (p < 0 || p >= P.slots) bad = lane;
-    }
-    for (int off = 32; off > 0; off >>= 1) bad = min(bad, __shfl_xor(bad, off));
+    const uint64_t outside = __ballot(p < 0 || p >= P.slots);
+    const int bad = min(want, outside ? __ffsll((unsigned long long)outside) - 1 : 64);
     over = bad > P.capacity - n;
     return min(bad, P.capacity - n);
 }
 
-// One workgroup per (row, move).  With advance the workgroup of a row that finishes last counts the kept
-// nodes: by then every other one has read the count (its ticket comes after), so one launch does both.
+// `len` rows of every head, four vectors of a thread in flight; lane i of a wave holds the slot of row i
+template <typename V>
+__device__ __forceinline__ void move_rows(const char* src, char* dst, int64_t sh, int64_t dh, int row_bytes, int len,
+                                          int heads, int slot, int tid) {
+    const unsigned per = row_bytes / sizeof(V), head = len * per;
+    const unsigned all = head * heads;  // at most 64 rows of 1024 vectors and 2^14 heads
+    constexpr int U = 4;
+    for (unsigned x0 = 0; x0 < all; x0 += U * kDraftThreads) {
+        V v[U];
+        unsigned h[U], y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const unsigned x = min(x0 + u * kDraftThreads + tid, all - 1);
+            h[u] = x / head;
+            y[u] = x - h[u] * head;
+            const unsigned i = y[u] / per;
+            v[u] = *reinterpret_cast<const V*>(src + h[u] * sh + (int64_t)__shfl(slot, (int)i) * row_bytes +
+                                               (y[u] - i * per) * sizeof(V));
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (x0 + u * kDraftThreads + tid < all)
+                *reinterpret_cast<V*>(dst + h[u] * dh + y[u] * sizeof(V)) = v[u];
+    }
+}
+
+// One workgroup per (row, move).  With advance the workgroup of a row that draws the last ticket counts the
+// kept nodes: by then every other one has read the count, so one launch does both.
 __global__ __launch_bounds__(kDraftThreads) void k_draft_commit(const DraftCommitDev P) {
     const int tid = threadIdx.x, b = blockIdx.x;
-    int n;
+    int n, slot;
     bool over;
-    const int len = commit_length(P, b, tid & 63, n, over);
+    const int len = commit_length(P, b, tid & 63, n, slot, over);
     const pa_draft_move& M = P.mv[blockIdx.y];
-    const int32_t* path = P.path + b * P.path_stride;
-    const int unit = M.row_bytes % 16 == 0 ? 16 : 4;
-    const int per = M.row_bytes / unit, head = len * per;
-    if (P.count > 0) {
+    __syncthreads();  // every wave has read the count
+    int done = 0;     // drawn now, looked at after the moves
+    // relaxed: nothing that another workgroup wrote is read after it, and this one's reads of the count have
+    // returned (the length depends on them); a release would write the L2 back, at several us
+    if (P.advance && tid == 0)
+        done = __hip_atomic_fetch_add(P.tickets + b * kTicketStride, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (P.count > 0 && len > 0) {
+        const int unit = M.row_bytes % 16 == 0 ? 16 : 4;
         const int64_t bh = (int64_t)b * P.kv_heads;
         const char* src = static_cast<const char*>(M.src) + bh * P.slots * M.row_bytes;
         char* dst = static_cast<char*>(M.dst) + (bh * P.capacity + n) * M.row_bytes;
         const int64_t sh = (int64_t)P.slots * M.row_bytes, dh = (int64_t)P.capacity * M.row_bytes;
-        const unsigned all = (unsigned)head * P.kv_heads;  // at most 64 rows of 256 units per head
-        for (unsigned x = tid; x < all; x += kDraftThreads) {
-            const unsigned h = x / (unsigned)head, y = x - h * head, i = y / (unsigned)per;
-            const char* from = src + h * sh + (int64_t)path[i] * M.row_bytes + (y - i * per) * unit;
-            char* to = dst + h * dh + (int64_t)y * unit;
-            if (unit == 16) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
-            else *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
-        }
+        if (unit == 16) move_rows<u32x4_d>(src, dst, sh, dh, M.row_bytes, len, P.kv_heads, slot, tid);
+        else move_rows<uint32_t>(src, dst, sh, dh, M.row_bytes, len, P.kv_heads, slot, tid);
     }
-    if (!P.advance) return;
-    __syncthreads();  // every wave has read the count
-    if (tid == 0) {
-        // relaxed: nothing that another workgroup wrote is read after it, and this one's read of the count has
-        // returned (the length depends on it); a release would write the L2 back, at several us
-        const int done = __hip_atomic_fetch_add(P.tickets + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (done == (int)gridDim.y - 1) {
-            P.counts[b] = n + len;
-            P.tickets[b] = 0;
-            if (over && P.overflow) *P.overflow = 1;
-        }
+    if (P.advance && tid == 0 && done == (int)gridDim.y - 1) {
+        P.counts[b] = n + len;
+        P.tickets[b * kTicketStride] = 0;
+        if (over && P.overflow) *P.overflow = 1;
     }
 }
 
@@ -610,7 +650,6 @@ int launch_draft_append(const pa_draft_rows* r, hipStream_t s) {
     P.inv_freq = r->inv_freq;
     P.lpr = 1;
     while (P.lpr * E < r->dim) P.lpr <<= 1;
-    P.rows = 0;
     for (int k = 0; k < r->count; ++k) {
         const pa_draft_item& it = r->items[k];
         if (!it.src.ptr || !it.out.ptr || it.src.heads < 1 || it.src.dtype != T || it.out.dtype != T ||
@@ -623,15 +662,11 @@ int launch_draft_append(const pa_draft_rows* r, hipStream_t s) {
         I.w = it.norm_weight;
         I.wdt = it.weight_dtype;
         I.rotate = it.rotate;
-        I.row0 = P.rows;
-        P.rows += it.src.heads;
+        I.heads = it.src.heads;
     }
-    const int per = kDraftThreads / P.lpr;
     const int64_t nodes = (int64_t)r->batch * r->drafts;
     if (nodes > (1 << 30)) return PA_EUNSUPPORTED;
-    // parts of a node's rows: enough workgroups to fill the GPU, each with at least one sweep of rows
-    int parts = (int)std::max<int64_t>(1, std::min<int64_t>((P.rows + per - 1) / per, 1024 / nodes));
-    const dim3 grid((unsigned)nodes, parts);
+    const dim3 grid((unsigned)nodes, r->count);
     ProfScope ps("draft_append", s);
     if (T == PA_F32) hipLaunchKernelGGL((k_draft_append<float>), grid, dim3(kDraftThreads), 0, s, P);
     else if (T == PA_F16) hipLaunchKernelGGL((k_draft_append<f16>), grid, dim3(kDraftThreads), 0, s, P);
@@ -644,7 +679,7 @@ int launch_draft_commit(const pa_commit* c, hipStream_t s) {
         c->count < 0 || c->count > PA_MAX_MOVES || c->path_len < 0 || c->path_len > PA_MAX_DRAFTS ||
         !c->path || !c->kept || !c->counts || (c->advance && !c->tickets))
         return PA_EINVAL;
-    if (c->kv_heads > (1 << 15)) return PA_EUNSUPPORTED;  // 32-bit indexes of a row's vectors
+    if (c->kv_heads > (1 << 14)) return PA_EUNSUPPORTED;  // 32-bit indexes of a row's vectors
     DraftCommitDev P;
     P.batch = c->batch;
     P.kv_heads = c->kv_heads;

@@ -39,7 +39,7 @@ struct VerifyDev {
     int64_t* token;
     float4* stats;       // [B][T][chunks]: maximum, sum, first position of the maximum (as bits)
     uint64_t* best;      // [B][chunks][2]
-    uint32_t* ticket;    // [B]
+    uint32_t* ticket;    // [B][kTicketStride]
 };
 
 __device__ __forceinline__ float row_temperature(const VerifyDev& P, int b) {
@@ -56,38 +56,24 @@ __device__ __forceinline__ void take_first(float& x, int& i, float y, int j) {
     }
 }
 
-// Entry `32-entry group` access: vector k of thread tid covers E entries of the 16-byte aligned run
-// that holds the row, so an unaligned row costs a few masked entries at its ends and no more.
+// vector k of thread tid: E entries (16 bytes of T) of its chunk
 template <typename T> struct VerVec {
     static constexpr int E = 16 / sizeof(T);
     static constexpr int N = kVerChunk / (kVerThreads * E);
 };
 
-// E entries of a row of n, starting at entry i (which may be negative or past the end), as floats;
-// entries outside are `fill`.  `row + i` is 16-byte aligned.
-template <typename T>
-__device__ __forceinline__ void load_entries(const T* row, int64_t i, int n, float fill,
-                                             float (&x)[VerVec<T>::E]) {
-    constexpr int E = VerVec<T>::E;
-    if (i >= 0 && i + E <= n) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(row + i);
-        const T* e = reinterpret_cast<const T*>(&raw);
+// E entries of a row of n at entry i >= 0; what lies past the end is `fill`.  Rows start anywhere (a
+// vocabulary need not be a multiple of 8): global loads of 16 bytes may be unaligned.
+template <typename T, int E>
+__device__ __forceinline__ void load_entries(const T* row, int64_t i, int n, float fill, float (&x)[E]) {
+    T raw[E];
+    if (i + E <= n) {
+        __builtin_memcpy(raw, row + i, sizeof(raw));
 #pragma unroll
-        for (int k = 0; k < E; ++k) x[k] = to_f(e[k]);
+        for (int k = 0; k < E; ++k) x[k] = to_f(raw[k]);
     } else {
 #pragma unroll
-        for (int k = 0; k < E; ++k) x[k] = i + k >= 0 && i + k < n ? to_f(row[i + k]) : fill;
-    }
-}
-
-// E floats of a row of n at entry i, of any alignment; what lies outside is 1
-template <int E>
-__device__ __forceinline__ void load_floats(const float* row, int64_t i, int n, float (&x)[E]) {
-    if (i >= 0 && i + E <= n) {
-        __builtin_memcpy(x, row + i, sizeof(x));
-    } else {
-#pragma unroll
-        for (int k = 0; k < E; ++k) x[k] = i + k >= 0 && i + k < n ? row[i + k] : 1.f;
+        for (int k = 0; k < E; ++k) x[k] = i + k < n ? to_f(row[i + k]) : fill;
     }
 }
 
@@ -103,26 +89,32 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_stats(const VerifyDev P)
     __shared__ int s_i[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int chunk = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
-    if (chunk == 0 && t == 0 && tid == 0) P.ticket[b] = 0;  // before the walk's launch begins
+    if (chunk == 0 && t == 0 && tid == 0) P.ticket[b * kTicketStride] = 0;  // before the walk's launch begins
     const float temp = row_temperature(P, b);
     const T* row = reinterpret_cast<const T*>(P.logits) + b * P.logits_sb + t * P.logits_sn;
-    const int shift = (int)(((uintptr_t)row & 15) / sizeof(T));  // entries before the row in its run
-    const int64_t i0 = (int64_t)chunk * kVerChunk - shift;
+    const int i0 = chunk * kVerChunk + tid * E;
     float x[N][E];
     float top = -INFINITY;
     int at = P.vocab;
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-        const int64_t i = i0 + (int64_t)(k * kVerThreads + tid) * E;
-        load_entries<T>(row, i, P.vocab, -INFINITY, x[k]);
+    for (int k = 0; k < N; ++k) load_entries<T, E>(row, i0 + k * kVerThreads * E, P.vocab, -INFINITY, x[k]);
+    if (temp > 0.f) {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (x[k][e] > top) {
-                top = x[k][e];
-                at = (int)(i + e);
-            }
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int e = 0; e < E; ++e) top = fmaxf(top, x[k][e]);  // NaN loses, and shows in the sum
+        for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (x[k][e] > top) {
+                    top = x[k][e];
+                    at = i0 + k * kVerThreads * E + e;
+                }
+        for (int off = 32; off > 0; off >>= 1) take_first(top, at, __shfl_xor(top, off), __shfl_xor(at, off));
     }
-    for (int off = 32; off > 0; off >>= 1) take_first(top, at, __shfl_xor(top, off), __shfl_xor(at, off));
     if (lane == 0) {
         s_x[wave] = top;
         s_i[wave] = at;
@@ -139,13 +131,13 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_stats(const VerifyDev P)
         for (int k = 0; k < N; ++k)
 #pragma unroll
             for (int e = 0; e < E; ++e) sum += __builtin_amdgcn_exp2f((x[k][e] - base) * c);
+        sum = wave_sum(sum);
+        if (lane == 0) s_sum[wave] = sum;
+        __syncthreads();
+        sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
     }
-    sum = wave_sum(sum);
-    if (lane == 0) s_sum[wave] = sum;
-    __syncthreads();
     if (tid == 0)
-        P.stats[((int64_t)b * P.T + t) * P.chunks + chunk] =
-            make_float4(top, s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3], __int_as_float(at), 0.f);
+        P.stats[((int64_t)b * P.T + t) * P.chunks + chunk] = make_float4(top, sum, __int_as_float(at), 0.f);
 }
 
 // the residual after `n` rejections of one entry's probability p with draft probability q: inv[k] is
@@ -163,6 +155,17 @@ __device__ __forceinline__ uint64_t best_key(float w, float noise, int64_t i) {
     return ((uint64_t)(__float_as_uint(key) + 1u) << 32) | (0xffffffffu - (uint32_t)i);
 }
 
+__device__ __forceinline__ uint64_t wave_best(uint64_t x) {
+    for (int off = 32; off > 0; off >>= 1) {
+        const uint64_t y = __shfl_xor((unsigned long long)x, off);
+        x = y > x ? y : x;
+    }
+    return x;
+}
+__device__ __forceinline__ int64_t best_token(uint64_t key) {
+    return key ? (int64_t)(0xffffffffu - (uint32_t)key) : (int64_t)-1;
+}
+
 template <typename T>
 __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) {
     constexpr int E = VerVec<T>::E, N = VerVec<T>::N;
@@ -177,6 +180,15 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
     const bool greedy = !(temp > 0.f);
     const float c = greedy ? 0.f : kLog2e / temp;
     const int32_t* parents = P.parents ? P.parents + b * P.parents_stride : nullptr;
+
+    // this chunk's random numbers are in flight over the walk
+    const int i0 = chunk * kVerChunk + tid * E;
+    float nz[N][E];
+    if (!greedy) {
+        const float* noise = P.noise + b * P.noise_stride;
+#pragma unroll
+        for (int k = 0; k < N; ++k) load_entries<float, E>(noise, i0 + k * kVerThreads * E, P.vocab, 1.f, nz[k]);
+    }
 
     // every wave holds the nodes, one per lane, and walks for itself
     const bool node = lane < P.T;
@@ -297,29 +309,22 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
     row += cur * P.logits_sn;
     const float top = s_top[cur], inv = s_inv[cur];
     const float* q = P.probs && nrej > 0 ? qrow + cur * P.probs_sn : nullptr;
-    const float* noise = P.noise + b * P.noise_stride;
-    const int shift = (int)(((uintptr_t)row & 15) / sizeof(T));
-    const int64_t i0 = (int64_t)chunk * kVerChunk - shift;
     const int nout = P.probs ? 0 : nrej;
     if (wave == 0 && ((rejected >> lane) & 1)) s_rej[__popcll(rejected & ((1ull << lane) - 1))] = tok;
-    float x[N][E], nz[N][E];
+    float x[N][E];
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-        const int64_t i = i0 + (int64_t)(k * kVerThreads + tid) * E;
-        load_entries<T>(row, i, P.vocab, -INFINITY, x[k]);
-        load_floats<E>(noise, i, P.vocab, nz[k]);
-    }
+    for (int k = 0; k < N; ++k) load_entries<T, E>(row, i0 + k * kVerThreads * E, P.vocab, -INFINITY, x[k]);
     __syncthreads();
     uint64_t best = 0, alt = 0;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const int64_t i = i0 + (int64_t)(k * kVerThreads + tid) * E;
+        const int i = i0 + k * kVerThreads * E;
         float w[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) w[e] = __builtin_amdgcn_exp2f((x[k][e] - top) * c) * inv;  // 0 outside
         if (q) {
             float qj[E];
-            load_floats<E>(q, i, P.vocab, qj);
+            load_entries<float, E>(q, i, P.vocab, 1.f, qj);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 w[e] = residual(w[e], qj[e], s_rinv, nrej - 1);
@@ -339,11 +344,8 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
             best = key > best ? key : best;
         }
     }
-    for (int off = 32; off > 0; off >>= 1) {
-        const uint64_t y = __shfl_xor((unsigned long long)best, off), z = __shfl_xor((unsigned long long)alt, off);
-        best = y > best ? y : best;
-        alt = z > alt ? z : alt;
-    }
+    best = wave_best(best);
+    if (q) alt = wave_best(alt);
     if (lane == 0) {
         s_best[wave][0] = best;
         s_best[wave][1] = alt;
@@ -354,15 +356,20 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
             best = s_best[w][0] > best ? s_best[w][0] : best;
             alt = s_best[w][1] > alt ? s_best[w][1] : alt;
         }
+        if (P.chunks == 1) {
+            P.token[b] = best_token(best ? best : alt);
+            return;
+        }
         uint64_t* to = P.best + ((int64_t)b * P.chunks + chunk) * 2;
         __hip_atomic_store(to, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __hip_atomic_store(to + 1, alt, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         // The stores and the loads below act at the level that all of the GPU shares, so it is enough that the
         // stores have ended before the ticket is drawn; a release would write the L2 back, at several us.
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        const uint32_t n = __hip_atomic_fetch_add(P.ticket + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint32_t n = __hip_atomic_fetch_add(P.ticket + b * kTicketStride, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         s_last = n == (uint32_t)P.chunks - 1;
     }
+    if (P.chunks == 1) return;
     __syncthreads();
     if (!s_last || wave != 0) return;
     best = 0;
@@ -374,20 +381,13 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
         best = y > best ? y : best;
         alt = z > alt ? z : alt;
     }
-    for (int off = 32; off > 0; off >>= 1) {
-        const uint64_t y = __shfl_xor((unsigned long long)best, off), z = __shfl_xor((unsigned long long)alt, off);
-        best = y > best ? y : best;
-        alt = z > alt ? z : alt;
-    }
-    if (lane == 0) {
-        const uint64_t pick = best ? best : alt;
-        P.token[b] = pick ? (int64_t)(0xffffffffu - (uint32_t)pick) : (int64_t)-1;
-    }
+    best = wave_best(best);
+    alt = wave_best(alt);
+    if (lane == 0) P.token[b] = best_token(best ? best : alt);
 }
 
 int verify_chunks(const pa_verify* v) {
-    // a row's 16-byte aligned run may begin up to 7 entries before the row
-    return (int)(((int64_t)v->vocab + 7 + kVerChunk - 1) / kVerChunk);
+    return (v->vocab + kVerChunk - 1) / kVerChunk;
 }
 
 bool verify_sizes(const pa_verify* v) {
@@ -400,7 +400,7 @@ bool verify_sizes(const pa_verify* v) {
 size_t draft_verify_workspace(const pa_verify* v) {
     if (!verify_sizes(v)) return 0;
     const size_t chunks = verify_chunks(v), b = v->batch;
-    return b * v->drafts * chunks * sizeof(float4) + b * chunks * 16 + b * 4;
+    return b * v->drafts * chunks * sizeof(float4) + b * chunks * 16 + b * kTicketStride * 4;
 }
 
 int launch_draft_verify(const pa_verify* v, hipStream_t s) {

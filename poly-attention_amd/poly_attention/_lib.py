@@ -20,6 +20,7 @@ PA_ABI_VERSION = 9
 PA_MAX_ORDER = 8
 PA_MAX_DRAFTS = 64
 PA_MAX_MOVES = 128
+PA_TICKET_STRIDE = 32
 
 PA_OK = 0
 PA_EINVAL = -1

@@ -197,7 +197,7 @@ class DraftCache:
         self._moves = bytes(moves)
         self._geometry = (batch, kv_heads, max_drafts, capacity)
         # rows' tickets of a commit, 0 between calls
-        self._tickets = torch.zeros(batch, dtype=torch.int32, device=device)
+        self._tickets = torch.zeros(batch * _lib.PA_TICKET_STRIDE, dtype=torch.int32, device=device)
         self._plans = {}  # the calls' structures, by the shape of q1
 
     # -------------------------------------------------------------------------------------
