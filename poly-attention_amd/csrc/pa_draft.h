@@ -34,18 +34,14 @@ struct DraftRow {  // a [B, h, n, dim] array: base and element strides
     }
 };
 
-struct DraftLevelDev {
-    DraftRow k, v, m, bias, q, dk, dv, out, lse;
-    int32_t rows, rep, row0;  // rows per key head, heads per key head, first row in a unit's record
-};
-
-struct DraftDev {
+// What the two launches share.
+struct DraftCommon {
     int32_t batch, kv_heads, T, dim, order, capacity;
-    int32_t target;      // units aimed at over the whole batch
-    int32_t row_blocks;  // partial: blocks of rows per key head (of the level that has most)
     int32_t rec_rows;    // rows of a unit's record, all levels
-    int32_t cols;        // combine: columns per workgroup
-    float scale, softclamp;
+    int32_t t16;         // T in whole sixteens
+    int32_t target;      // units aimed at over the whole batch ...
+    int32_t target_min;  // ... or this many, where units are smaller than
+    int32_t least;       // this many chunks
     const int32_t* counts;
     const int32_t* parents;
     int64_t parents_stride;
@@ -53,15 +49,35 @@ struct DraftDev {
     float2* ws_s;  // [unit][kv head][rec_rows]: running maximum (log2 units) and sum
     float* ws_t;   // [row][kv head][rec_rows][t16]: scores of the tree without biases (log2 units), -inf
                    // where a node does not see another
-    int32_t t16;   // T in whole sixteens
+    int4* ws_u;    // [row]: the row's first unit, its units, and which of its nodes are there (64 bits)
+};
+
+struct DraftLevelDev {
+    DraftRow q, k, v, bias, m, dk;
+    int32_t rows, rep, row0;  // rows per key head, heads per key head, first row in a unit's record
+};
+struct DraftDev : DraftCommon {
+    int32_t row_blocks;  // blocks of rows per key head (of the level that has most)
+    float scale, softclamp;
     DraftLevelDev L[PA_MAX_ORDER];
 };
 
-__device__ __forceinline__ int draft_count(const DraftDev& P, int b) {
+struct DraftJoinLevel {
+    DraftRow dv, out;
+    float* lse;
+    int64_t lse_sb, lse_sh;
+};
+struct DraftJoin : DraftCommon {
+    int32_t lgcols;  // log2 of the columns per workgroup
+    int32_t rep;     // heads per key head at the final level
+    DraftJoinLevel L[PA_MAX_ORDER];
+};
+
+__device__ __forceinline__ int draft_count(const DraftCommon& P, int b) {
     const int n = P.counts[b];
     return n < 0 ? 0 : (n > P.capacity ? P.capacity : n);
 }
-__device__ __forceinline__ int draft_chunks(const DraftDev& P, int b) {
+__device__ __forceinline__ int draft_chunks(const DraftCommon& P, int b) {
     return (int)(((unsigned)draft_count(P, b) + kDraftChunk - 1) / kDraftChunk);
 }
 
@@ -77,12 +93,18 @@ struct DraftUnits {
 
 __device__ __forceinline__ unsigned draft_ceil(unsigned n, unsigned d) { return d == 1 ? n : (n + d - 1) / d; }
 
+// chunks per unit for a batch of `total` chunks
+__device__ __forceinline__ int draft_unit_size(const DraftCommon& P, unsigned total) {
+    const unsigned many = draft_ceil(total, P.target), few = draft_ceil(total, P.target_min);
+    return max(max(1u, many), min(few, (unsigned)P.least));
+}
+
 // The units of row `want` (want >= 0), or the row of unit u (want < 0; false past the last unit).
 // The whole wave takes part.  One row needs no sums.
-__device__ __forceinline__ bool draft_units(const DraftDev& P, int want, int u, int lane, DraftUnits& r) {
+__device__ __forceinline__ bool draft_units(const DraftCommon& P, int want, int u, int lane, DraftUnits& r) {
     if (P.batch == 1) {
         const unsigned n = draft_chunks(P, 0);
-        r.size = max(1u, draft_ceil(n, P.target));
+        r.size = draft_unit_size(P, n);
         r.b = 0;
         r.first = 0;
         r.place = u;
@@ -96,7 +118,7 @@ __device__ __forceinline__ bool draft_units(const DraftDev& P, int want, int u, 
         if (b < 64) n0 = n;
     }
     for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off);
-    r.size = max(1u, draft_ceil(total, P.target));
+    r.size = draft_unit_size(P, total);
     int before = 0;
     for (int r0 = 0; r0 < P.batch; r0 += 64) {
         const int row = r0 + lane;
@@ -140,11 +162,11 @@ __device__ __forceinline__ uint64_t draft_ancestors(const int32_t* parents, int 
     return dead ? 0ull : ((uint64_t)hi << 32) | lo;
 }
 
-template <typename T> void launch_draft_partial(const DraftDev& P, int units, bool vmul, hipStream_t s);
+template <typename T> void launch_draft_partial(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
 // in source files of their own
-extern template void launch_draft_partial<bf16>(const DraftDev& P, int units, bool vmul, hipStream_t s);
-extern template void launch_draft_partial<f16>(const DraftDev& P, int units, bool vmul, hipStream_t s);
-extern template void launch_draft_partial<float>(const DraftDev& P, int units, bool vmul, hipStream_t s);
+extern template void launch_draft_partial<bf16>(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
+extern template void launch_draft_partial<f16>(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
+extern template void launch_draft_partial<float>(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
 template <typename T> constexpr int draft_row_tiles(int D) {
     // 16-row tiles that a wave's accumulators hold
     return D > 128 ? 1 : sizeof(T) == 4 ? 2 : 4;

@@ -15,22 +15,30 @@ namespace pa {
 // values.  The levels below the final one have at most 64 rows and are repeated by every row block.
 // What bounds it is latency: loads are issued in batches and the next level's scores are loaded before
 // this one's are used.
+// Code that runs for the first time waits for its instructions too, and a level's arguments for the
+// scalar cache: the score loops are as long as the tree needs (NK), the arguments are read into LDS
+// beside the first loads, and nothing divides by a number that is not known before.
 constexpr int kDraftBatch = 8;  // units whose records a thread loads together
 
 struct JoinedRow {
     float top, sum;
     float4 acc;
 };
-__device__ __forceinline__ void join(JoinedRow& a, float top, float sum, const float4& acc) {
-    const float t = fmaxf(a.top, top);
-    const float f = a.top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.top - t);
-    const float h = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t);
-    a.top = t;
-    a.sum = a.sum * f + sum * h;
-    a.acc.x = a.acc.x * f + acc.x * h;
-    a.acc.y = a.acc.y * f + acc.y * h;
-    a.acc.z = a.acc.z * f + acc.z * h;
-    a.acc.w = a.acc.w * f + acc.w * h;
+__device__ __forceinline__ float exp2_or_0(float x, float top) {
+    return x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - top);
+}
+__device__ __forceinline__ void join(JoinedRow& a, float f, float sum, const float4& acc) {
+    a.sum += sum * f;
+    a.acc.x += acc.x * f;
+    a.acc.y += acc.y * f;
+    a.acc.z += acc.z * f;
+    a.acc.w += acc.w * f;
+}
+__device__ __forceinline__ void raise(JoinedRow& a, float top) {
+    const float f = exp2_or_0(a.top, top);
+    a.top = top;
+    a.sum *= f;
+    a.acc = make_float4(a.acc.x * f, a.acc.y * f, a.acc.z * f, a.acc.w * f);
 }
 
 template <typename T>
@@ -55,69 +63,81 @@ __device__ __forceinline__ void store4f(T* p, const float4& y) {
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kDraftThreads) void k_draft_combine(const DraftDev P) {
+template <typename T, int NK>
+__global__ __launch_bounds__(kDraftThreads) void k_draft_combine(const DraftJoin P) {
     extern __shared__ __align__(16) float smem[];
-    __shared__ uint64_t s_anc[64];
     __shared__ float s_bias[64], s_top[64], s_inv[64], s_utop[64 * PA_MAX_ORDER], s_usum[64 * PA_MAX_ORDER];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    __shared__ __align__(16) DraftJoinLevel s_lvl[PA_MAX_ORDER];
+    const int tid = threadIdx.x;
     const int b = blockIdx.x / P.kv_heads, hk = blockIdx.x % P.kv_heads;
-    const int col0 = blockIdx.y * P.cols, ncol = min(P.cols, P.dim - col0);
-    const int quads = ncol / 4;  // dim and cols are multiples of 8
+    const int col0 = blockIdx.y << P.lgcols, ncol = min(1 << P.lgcols, P.dim - col0);
     const int last = P.order - 1, low = P.T * last;  // rows of the levels below the final one
-    const int r0 = blockIdx.z * 64, frows = min(64, P.L[last].rows - r0);
+    const int r0 = blockIdx.z * 64, frows = min(64, P.T * P.rep - r0);
     const int rows_all = low + frows;
-    const int spitch = P.t16 + 1, vpitch = P.cols + 4;
-    float* const s_acc = smem;                                  // [rows_all][cols]: the joined units
-    float* const s_p = s_acc + rows_all * P.cols;               // [64][spitch]: weights of the tree
-    float* s_in = s_p + ((64 * spitch + 3) & ~3);               // [t16][vpitch]: a level's tree values
-    float* s_out = s_in + P.t16 * vpitch;                       // [t16][vpitch]: its outputs
-    float* const s_red = s_in;                                  // before the levels: 256 JoinedRow
+    const int lgq = P.lgcols - 2;                  // a row's items: four columns each
+    const int spitch = P.t16 + 4, vpitch = (1 << P.lgcols) + 4;
+    float* const s_acc = smem;                     // [rows_all][cols]: the joined units
+    float* const s_p = s_acc + (rows_all << P.lgcols);  // [64][spitch]: weights of the tree
+    float* s_in = s_p + 64 * spitch;               // [t16][vpitch]: a level's tree values
+    float* s_out = s_in + P.t16 * vpitch;          // [t16][vpitch]: its outputs
+    float* const s_red = s_in;                     // before the levels: 256 x 6
 
-    // four threads per row take the tree's scores of a level, every fourth one each
+    const int4 units = P.ws_u[b];
+    // Four threads per row take the tree's scores of a level, every fourth one each; a thread's item is a
+    // row and four columns.  Both for a level ahead.
     const int row = tid >> 2, sub = tid & 3;
-    float s[16];
+    const int ir = tid >> lgq, id = (tid & ((1 << lgq) - 1)) * 4;
+    const float* const scores = P.ws_t + ((int64_t)blockIdx.x * P.rec_rows + row) * P.t16 + sub;
+    float s[NK];
     auto load_scores = [&](int t) __attribute__((always_inline)) {
         const int n = t == last ? frows : P.T;
-        const float* from = P.ws_t + (((int64_t)b * P.kv_heads + hk) * P.rec_rows + P.L[t].row0 +
-                                      (t == last ? r0 : 0) + row) * P.t16 + sub;
+        const float* from = scores + (t * P.T + (t == last ? r0 : 0)) * P.t16;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) s[k] = row < n && 4 * k + sub < P.T ? from[4 * k] : -INFINITY;
+        for (int k = 0; k < NK; ++k) s[k] = row < n && 4 * k < P.t16 ? from[4 * k] : -INFINITY;
     };
     load_scores(0);
-    DraftUnits U;
-    draft_units(P, b, 0, lane, U);
-    if (wave == 0)
-        s_anc[lane] = draft_ancestors(P.parents ? P.parents + b * P.parents_stride : nullptr, P.T, lane);
+    float4 val = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (ir < P.T && id < ncol) val = load4f<T>(P.L[0].dv.template at<T>(b, hk) + ir * P.L[0].dv.sn + col0 + id);
+    {
+        constexpr int W = sizeof(DraftJoinLevel) / 4;
+        static_assert(W * PA_MAX_ORDER <= kDraftThreads, "one word per thread");
+        if (tid < W * P.order)
+            reinterpret_cast<uint32_t*>(s_lvl)[tid] = reinterpret_cast<const uint32_t*>(P.L)[tid];
+    }
 
-    {   // the units: an item is a row and four columns, dealt out over `parts` threads where there are few
+    {   // the units: an item's are dealt out over `parts` threads where there are few items
         const int64_t urec = (int64_t)P.kv_heads * P.rec_rows;  // records between units
-        const int64_t rec0 = ((int64_t)U.first * P.kv_heads + hk) * P.rec_rows;
-        const int items = rows_all * quads;
-        int parts = 1;
-        while (parts < 16 && items * parts * 2 <= kDraftThreads && parts * 2 <= U.number) parts *= 2;
-        for (int x0 = 0; x0 < items; x0 += kDraftThreads) {
-            const int part = parts > 1 ? tid / items : 0, item = parts > 1 ? tid % items : x0 + tid;
+        const int64_t rec0 = ((int64_t)units.x * P.kv_heads + hk) * P.rec_rows;
+        const int items = rows_all << lgq;
+        int lgp = 0;
+        while (lgp < 4 && items << (lgp + 1) <= kDraftThreads && 2 << lgp <= units.y) ++lgp;
+        // with parts, a part's items lie in `stride` threads
+        const int stride = kDraftThreads >> lgp, part = tid / stride;  // a power of two
+        for (int x0 = 0; x0 < items; x0 += stride) {
+            const int item = x0 + (tid & (stride - 1)), ra = item >> lgq, d = (item & ((1 << lgq) - 1)) * 4;
             JoinedRow a = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-            const int ra = item / quads, d = 4 * (item % quads);
-            if (item < items && part < parts) {
+            if (item < items && d < ncol) {
                 const int64_t rec = rec0 + ra + (ra < low ? 0 : r0);
-                for (int u = part; u < U.number; u += parts * kDraftBatch) {
+                const float* const from = P.ws_o + col0 + d;
+                for (int u = part; u < units.y; u += kDraftBatch << lgp) {
                     float2 ms[kDraftBatch];
                     float4 y[kDraftBatch];
 #pragma unroll
                     for (int k = 0; k < kDraftBatch; ++k) {
-                        const int64_t at = rec + (int64_t)min(u + k * parts, U.number - 1) * urec;
+                        const int64_t at = rec + (int64_t)min(u + (k << lgp), units.y - 1) * urec;
                         ms[k] = P.ws_s[at];
-                        y[k] = *reinterpret_cast<const float4*>(P.ws_o + at * P.dim + col0 + d);
-                        if (u + k * parts >= U.number) ms[k].x = -INFINITY;
+                        y[k] = *reinterpret_cast<const float4*>(from + at * P.dim);
+                        if (u + (k << lgp) >= units.y) ms[k].x = -INFINITY;
                     }
+                    float top = a.top;
 #pragma unroll
-                    for (int k = 0; k < kDraftBatch; ++k) join(a, ms[k].x, ms[k].y, y[k]);
+                    for (int k = 0; k < kDraftBatch; ++k) top = fmaxf(top, ms[k].x);
+                    raise(a, top);
+#pragma unroll
+                    for (int k = 0; k < kDraftBatch; ++k) join(a, exp2_or_0(ms[k].x, top), ms[k].y, y[k]);
                 }
             }
-            if (parts > 1) {
+            if (lgp) {
                 float* r = s_red + tid * 6;
                 r[0] = a.top;
                 r[1] = a.sum;
@@ -126,14 +146,18 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_combine(const DraftDev 
                 r[4] = a.acc.z;
                 r[5] = a.acc.w;
                 __syncthreads();
-                if (part == 0)
-                    for (int k = 1; k < parts; ++k) {
-                        const float* z = s_red + (tid + k * items) * 6;
-                        join(a, z[0], z[1], make_float4(z[2], z[3], z[4], z[5]));
+                if (part == 0 && item < items) {
+                    float top = a.top;
+                    for (int k = 1; k < 1 << lgp; ++k) top = fmaxf(top, s_red[(tid + k * stride) * 6]);
+                    raise(a, top);
+                    for (int k = 1; k < 1 << lgp; ++k) {
+                        const float* z = s_red + (tid + k * stride) * 6;
+                        join(a, exp2_or_0(z[0], top), z[1], make_float4(z[2], z[3], z[4], z[5]));
                     }
+                }
             }
-            if (part == 0 && item < items) {
-                *reinterpret_cast<float4*>(s_acc + ra * P.cols + d) = a.acc;
+            if (part == 0 && item < items && d < ncol) {
+                *reinterpret_cast<float4*>(s_acc + (ra << P.lgcols) + d) = a.acc;
                 if (d == 0) {
                     s_utop[ra] = a.top;
                     s_usum[ra] = a.sum;
@@ -141,82 +165,101 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_combine(const DraftDev 
             }
         }
     }
+    const uint64_t live = ((uint64_t)(uint32_t)units.w << 32) | (uint32_t)units.z;
     __syncthreads();
 
     for (int t = 0; t <= last; ++t) {
-        const DraftLevelDev& L = P.L[t];
+        const DraftJoinLevel& L = s_lvl[t];
         const bool fin = t == last;
         const int rows = fin ? frows : P.T, ra0 = t * P.T, rr = fin ? r0 : 0;
         // the tree's values: v, v * msg, or msg (already in s_in, as the level below left it)
         if (!fin)
-            for (int x = tid; x < P.T * quads; x += kDraftThreads) {
-                const int n = x / quads, d = 4 * (x % quads);
-                float4 y = load4f<T>(L.dv.at<T>(b, hk) + n * L.dv.sn + col0 + d);
-                float4* at = reinterpret_cast<float4*>(&s_in[n * vpitch + d]);
+            for (int n = ir; n < P.T; n += kDraftThreads >> lgq) {
+                if (id >= ncol) break;
+                float4 y = val;
+                if (n != ir) y = load4f<T>(L.dv.template at<T>(b, hk) + n * L.dv.sn + col0 + id);
+                float4* at = reinterpret_cast<float4*>(&s_in[n * vpitch + id]);
                 if (t > 0) {
                     const float4 z = *at;
                     y = make_float4(y.x * z.x, y.y * z.y, y.z * z.z, y.w * z.w);
                 }
                 *at = y;
             }
-        {   // maximum and sum over the units and the tree
-            float top = row < rows ? s_utop[ra0 + row] : -INFINITY, sum = 0.f;
-            const float utop = top;
+        // maximum and sum over the units and the tree
+        const float utop = row < rows ? s_utop[ra0 + row] : -INFINITY;
+        float top = utop, sum = 0.f;
+        if (t > 0) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                if (t > 0 && 4 * k + sub < P.T) s[k] += s_bias[4 * k + sub];
-                top = fmaxf(top, s[k]);
-            }
-            top = fmaxf(top, __shfl_xor(top, 1));
-            top = fmaxf(top, __shfl_xor(top, 2));
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const float p = s[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[k] - top);
-                if (row < rows && 4 * k + sub < P.T) s_p[row * spitch + 4 * k + sub] = p;
-                sum += p;
-            }
-            sum += __shfl_xor(sum, 1);
-            sum += __shfl_xor(sum, 2);
-            const float f = utop == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(utop - top);
-            __syncthreads();  // every s_bias has been read
-            if (row < rows && sub == 0) {
-                sum += s_usum[ra0 + row] * f;
-                const bool live = s_anc[(rr + row) % P.T] != 0;
-                s_top[row] = f;
-                s_inv[row] = live ? 1.f / sum : 0.f;
-                if (!fin) {
-                    const float lse = live ? top + log2f(sum) : 0.f;
-                    s_bias[row] = lse;
-                    if (blockIdx.y == 0 && blockIdx.z == 0) L.lse.at<float>(b, hk)[row] = lse * kLn2;
-                }
-            }
+            for (int k = 0; k < NK; ++k) s[k] += s_bias[4 * k + sub];  // past T: s is -inf, the bias 0
         }
-        if (!fin) load_scores(t + 1);
-        __syncthreads();
-        for (int x = tid; x < rows * quads; x += kDraftThreads) {
-            const int r = x / quads, d = 4 * (x % quads);
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-            const uint64_t anc = s_anc[(rr + r) % P.T];
-            if (anc) {
-                const float f = s_top[r], inv = s_inv[r];
-                const float4 u = *reinterpret_cast<const float4*>(s_acc + (ra0 + r) * P.cols + d);
-                if (f != 0.f) y = make_float4(u.x * f, u.y * f, u.z * f, u.w * f);
-                // only what the node sees: another branch's value may be anything
-                for (uint64_t see = anc; see; see &= see - 1) {
-                    const int k = __ffsll((unsigned long long)see) - 1;
-                    const float p = s_p[r * spitch + k];
-                    const float4 z = *reinterpret_cast<const float4*>(&s_in[k * vpitch + d]);
-                    y.x += p * z.x;
-                    y.y += p * z.y;
-                    y.z += p * z.z;
-                    y.w += p * z.w;
-                }
-                y = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+#pragma unroll
+        for (int k = 0; k < NK; ++k) top = fmaxf(top, s[k]);
+        top = fmaxf(top, __shfl_xor(top, 1));
+        top = fmaxf(top, __shfl_xor(top, 2));
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            const float p = exp2_or_0(s[k], top);
+            if (row < rows && 4 * k < P.t16) s_p[row * spitch + 4 * k + sub] = p;
+            sum += p;
+        }
+        if (!fin) {
+            load_scores(t + 1);
+            const DraftJoinLevel& N = s_lvl[t + 1];
+            if (t + 1 < last && ir < P.T && id < ncol)
+                val = load4f<T>(N.dv.template at<T>(b, hk) + ir * N.dv.sn + col0 + id);
+        }
+        sum += __shfl_xor(sum, 1);
+        sum += __shfl_xor(sum, 2);
+        __syncthreads();  // every s_bias has been read
+        if (sub == 0) {
+            float lse = 0.f;
+            if (row < rows) {
+                const float f = exp2_or_0(utop, top);
+                sum += s_usum[ra0 + row] * f;
+                int n = row;
+                if (fin) n = (rr + row) % P.T;
+                const bool here = (live >> n) & 1;
+                s_top[row] = f;
+                s_inv[row] = here ? 1.f / sum : 0.f;
+                if (!fin && here) lse = top + log2f(sum);
+                if (!fin && blockIdx.y == 0 && blockIdx.z == 0) L.lse[b * L.lse_sb + hk * L.lse_sh + row] = lse * kLn2;
             }
-            if (!fin) *reinterpret_cast<float4*>(&s_out[r * vpitch + d]) = y;
+            s_bias[row] = lse;
+        }
+        __syncthreads();
+        for (int r = ir; r < rows; r += kDraftThreads >> lgq) {
+            if (id >= ncol) break;
+            const float f = s_top[r], inv = s_inv[r];
+            const float4 u = *reinterpret_cast<const float4*>(s_acc + ((ra0 + r) << P.lgcols) + id);
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (f != 0.f) y = make_float4(u.x * f, u.y * f, u.z * f, u.w * f);
+            for (int k0 = 0; k0 < P.T; k0 += 4) {
+                const float4 p = *reinterpret_cast<const float4*>(&s_p[r * spitch + k0]);
+                const float w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float4 z = *reinterpret_cast<const float4*>(&s_in[(k0 + k) * vpitch + id]);
+                    // what a node does not see (another branch, a slot past the nodes) may hold anything
+                    const bool see = w[k] != 0.f;
+                    y.x += w[k] * (see ? z.x : 0.f);
+                    y.y += w[k] * (see ? z.y : 0.f);
+                    y.z += w[k] * (see ? z.z : 0.f);
+                    y.w += w[k] * (see ? z.w : 0.f);
+                }
+            }
+            // an absent node's row: 0, whatever its query was
+            y = inv != 0.f ? make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (!fin) *reinterpret_cast<float4*>(&s_out[r * vpitch + id]) = y;
             if (fin || blockIdx.z == 0) {
-                const int n = (rr + r) % P.T, h = (rr + r) / P.T;
-                store4f<T>(L.out.at<T>(b, hk * L.rep + h) + n * L.out.sn + col0 + d, y);
+                int h = 0, n = r;
+                if (fin) {
+                    h = (rr + r) / P.T;
+                    n = rr + r - h * P.T;
+                    h += hk * P.rep;
+                } else {
+                    h = hk;
+                }
+                store4f<T>(L.out.template at<T>(b, h) + n * L.out.sn + col0 + id, y);
             }
         }
         __syncthreads();
@@ -224,6 +267,13 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_combine(const DraftDev 
         s_out = s_in;
         s_in = done;
     }
+}
+
+template <typename T>
+void launch_combine(const DraftJoin& P, dim3 grid, size_t lds, hipStream_t s) {
+    if (P.t16 == 16) hipLaunchKernelGGL((k_draft_combine<T, 4>), grid, dim3(kDraftThreads), lds, s, P);
+    else if (P.t16 == 32) hipLaunchKernelGGL((k_draft_combine<T, 8>), grid, dim3(kDraftThreads), lds, s, P);
+    else hipLaunchKernelGGL((k_draft_combine<T, 16>), grid, dim3(kDraftThreads), lds, s, P);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -480,10 +530,13 @@ DraftRow draft_row(const pa_view& v) {
 // head dims: multiples of 8, of 16 above 128 (a lane's features are whole: dim / 16 of the padded dim)
 bool draft_dim(int d) { return d >= 8 && d <= 256 && d % 8 == 0 && (d <= 128 || d % 16 == 0); }
 
-constexpr int64_t kDraftGoal = 1024;  // workgroups of the partial launch aimed at
+// Workgroups of the first launch aimed at: kDraftMany, but kDraftFew where a unit's keys are below
+// kDraftUnitBytes (a workgroup's start and end cost as much as some 30 KB).  32 x 8192 positions of 128:
+// 272 us with 1024, 249 with 2048; order 3, 8 x 2048 of 64: 41 with 1024, 45 with 2048.
+constexpr int64_t kDraftMany = 2048, kDraftFew = 1024, kDraftUnitBytes = 64 * 1024;
 
 // geometry shared by the workspace query and the launch; false where the request is malformed
-bool draft_plan(const pa_draft* d, DraftDev& P, int& units) {
+bool draft_plan(const pa_draft* d, DraftDev& P, int& units, int& tiles) {
     if (d->batch < 1 || d->kv_heads < 1 || d->heads < 1 || d->heads % d->kv_heads != 0) return false;
     if (d->drafts < 1 || d->drafts > PA_MAX_DRAFTS || d->order < 2 || d->order > PA_MAX_ORDER) return false;
     if (d->capacity < 1 || !draft_dim(d->dim) || !draft_dtype(d->levels[0].k.dtype)) return false;
@@ -497,24 +550,25 @@ bool draft_plan(const pa_draft* d, DraftDev& P, int& units) {
     P.capacity = d->capacity;
     const bool f32 = d->levels[0].k.dtype == PA_F32;
     const int D = d->dim <= 64 ? 64 : d->dim <= 128 ? 128 : 256;
-    const int tiles = f32 ? draft_row_tiles<float>(D) : draft_row_tiles<bf16>(D);
     const int most = d->drafts * rep;
-    const int block = 16 * (most <= 16 ? 1 : std::min(tiles, most <= 32 ? 2 : 4));
-    P.row_blocks = (most + block - 1) / block;
+    const int64_t chunks = ((int64_t)d->capacity + kDraftChunk - 1) / kDraftChunk * d->batch;
+    // rows of a workgroup: as many as its registers hold
+    tiles = most <= 16 ? 1 : std::min(f32 ? draft_row_tiles<float>(D) : draft_row_tiles<bf16>(D), most <= 32 ? 2 : 4);
+    P.row_blocks = (most + 16 * tiles - 1) / (16 * tiles);
     P.rec_rows = d->drafts * (d->order - 1) + most;
     P.t16 = (d->drafts + 15) & ~15;
     const int64_t per = (int64_t)d->kv_heads * d->order * P.row_blocks;
-    int64_t target = std::max<int64_t>(1, kDraftGoal / per);
     // no more units than the capacity has chunks
-    const int64_t chunks = ((int64_t)d->capacity + kDraftChunk - 1) / kDraftChunk * d->batch;
-    target = std::min(target, chunks);
+    const int64_t target = std::min(std::max<int64_t>(1, kDraftMany / per), chunks);
     P.target = (int)target;
+    P.target_min = (int)std::min(std::max<int64_t>(1, kDraftFew / per), chunks);
+    P.least = std::max(1, (int)(kDraftUnitBytes / ((int64_t)kDraftChunk * d->dim * (f32 ? 4 : 2))));
     units = (int)std::min(target + d->batch, chunks);
     return (int64_t)d->kv_heads * P.row_blocks <= 65535;
 }
 
-// the workspace's three arrays, and its size
-size_t draft_ws(DraftDev& P, int units, void* base) {
+// the workspace's arrays, and its size
+size_t draft_ws(DraftCommon& P, int units, void* base) {
     auto whole = [](size_t n) { return (n + 255) & ~size_t(255); };
     const size_t rec = (size_t)units * P.kv_heads * P.rec_rows;
     char* at = static_cast<char*>(base);
@@ -523,23 +577,25 @@ size_t draft_ws(DraftDev& P, int units, void* base) {
     P.ws_s = reinterpret_cast<float2*>(at + n);
     n += whole(rec * sizeof(float2));
     P.ws_t = reinterpret_cast<float*>(at + n);
-    return n + (size_t)P.batch * P.kv_heads * P.rec_rows * P.t16 * 4;
+    n += whole((size_t)P.batch * P.kv_heads * P.rec_rows * P.t16 * 4);
+    P.ws_u = reinterpret_cast<int4*>(at + n);
+    return n + (size_t)P.batch * sizeof(int4);
 }
 
-// LDS of the combine with `cols` columns
-size_t combine_lds(const DraftDev& P, int cols) {
+// LDS of the combine with 2^lg columns
+size_t combine_lds(const DraftCommon& P, int lg) {
+    const int cols = 1 << lg;
     const int rows = P.T * (P.order - 1) + 64;
     const size_t values = 2 * (size_t)P.t16 * (cols + 4);
-    return 4 * ((size_t)rows * cols + ((64 * (P.t16 + 1) + 3) & ~3) +
-                std::max(values, (size_t)kDraftThreads * 6));
+    return 4 * ((size_t)rows * cols + 64 * (P.t16 + 4) + std::max(values, (size_t)kDraftThreads * 6));
 }
 
 }  // namespace
 
 size_t draft_attend_workspace(const pa_draft* d) {
     DraftDev P;
-    int units = 0;
-    return draft_plan(d, P, units) ? draft_ws(P, units, nullptr) : 0;
+    int units = 0, tiles = 0;
+    return draft_plan(d, P, units, tiles) ? draft_ws(P, units, nullptr) : 0;
 }
 
 int launch_draft_attend(const pa_draft* d, hipStream_t s) {
@@ -551,8 +607,8 @@ int launch_draft_attend(const pa_draft* d, hipStream_t s) {
     if (!draft_dtype(T)) return PA_EINVAL;
     if (!draft_dim(d->dim)) return PA_EUNSUPPORTED;
     DraftDev P;
-    int units = 0;
-    if (!draft_plan(d, P, units)) return PA_EUNSUPPORTED;
+    int units = 0, tiles = 0;
+    if (!draft_plan(d, P, units, tiles)) return PA_EUNSUPPORTED;
     if (!d->workspace || (uintptr_t)d->workspace % 16 != 0 ||
         d->workspace_bytes < draft_ws(P, units, d->workspace))
         return PA_EWORKSPACE;
@@ -563,6 +619,9 @@ int launch_draft_attend(const pa_draft* d, hipStream_t s) {
     P.parents_stride = d->parents_stride;
     const int rep = d->heads / d->kv_heads;
     bool vmul = false;
+    DraftJoin J;
+    static_cast<DraftCommon&>(J) = P;
+    J.rep = rep;
     for (int t = 0; t < d->order; ++t) {
         const pa_draft_level& l = d->levels[t];
         const bool last = t == d->order - 1, middle = t > 0 && !last;
@@ -591,9 +650,11 @@ int launch_draft_attend(const pa_draft* d, hipStream_t s) {
         L.bias = draft_row(l.bias);
         L.q = draft_row(l.q);
         L.dk = draft_row(l.dk);
-        L.dv = draft_row(l.dv);
-        L.out = draft_row(l.out);
-        L.lse = draft_row(l.lse);
+        J.L[t].dv = draft_row(l.dv);
+        J.L[t].out = draft_row(l.out);
+        J.L[t].lse = static_cast<float*>(l.lse.ptr);
+        J.L[t].lse_sb = l.lse.sb;
+        J.L[t].lse_sh = l.lse.sh;
         L.rep = last ? rep : 1;
         L.rows = d->drafts * L.rep;
         L.row0 = t * d->drafts;
@@ -601,22 +662,23 @@ int launch_draft_attend(const pa_draft* d, hipStream_t s) {
     }
     {
         ProfScope ps("draft_partial", s);
-        if (T == PA_F32) launch_draft_partial<float>(P, units, vmul, s);
-        else if (T == PA_F16) launch_draft_partial<f16>(P, units, vmul, s);
-        else launch_draft_partial<bf16>(P, units, vmul, s);
+        if (T == PA_F32) launch_draft_partial<float>(P, units, tiles, vmul, s);
+        else if (T == PA_F16) launch_draft_partial<f16>(P, units, tiles, vmul, s);
+        else launch_draft_partial<bf16>(P, units, tiles, vmul, s);
     }
     // columns per workgroup: few where the grid is small; LDS of two workgroups a CU at least
     const int blocks = (d->drafts * rep + 63) / 64;
-    P.cols = 16;
-    while (P.cols < P.dim && combine_lds(P, 2 * P.cols) <= 56 * 1024 &&
-           (int64_t)P.batch * P.kv_heads * blocks * ((P.dim + P.cols - 1) / P.cols) > 1024)
-        P.cols *= 2;
-    const size_t lds = combine_lds(P, P.cols);
-    const dim3 grid(P.batch * P.kv_heads, (P.dim + P.cols - 1) / P.cols, blocks);
+    J.lgcols = combine_lds(P, 4) <= 52 * 1024 ? 4 : 3;
+    auto groups = [&]() { return (P.dim + (1 << J.lgcols) - 1) >> J.lgcols; };
+    while ((1 << J.lgcols) < P.dim && combine_lds(P, J.lgcols + 1) <= 52 * 1024 &&
+           (int64_t)P.batch * P.kv_heads * blocks * groups() > 1024)
+        ++J.lgcols;
+    const size_t lds = combine_lds(P, J.lgcols);
+    const dim3 grid(P.batch * P.kv_heads, groups(), blocks);
     ProfScope ps("draft_combine", s);
-    if (T == PA_F32) hipLaunchKernelGGL((k_draft_combine<float>), grid, dim3(kDraftThreads), lds, s, P);
-    else if (T == PA_F16) hipLaunchKernelGGL((k_draft_combine<f16>), grid, dim3(kDraftThreads), lds, s, P);
-    else hipLaunchKernelGGL((k_draft_combine<bf16>), grid, dim3(kDraftThreads), lds, s, P);
+    if (T == PA_F32) launch_combine<float>(J, grid, lds, s);
+    else if (T == PA_F16) launch_combine<f16>(J, grid, lds, s);
+    else launch_combine<bf16>(J, grid, lds, s);
     return PA_OK;
 }
 

@@ -2,5 +2,5 @@
 #include "pa_draft_partial.h"
 
 namespace pa {
-template void launch_draft_partial<f16>(const DraftDev& P, int units, bool vmul, hipStream_t s);
+template void launch_draft_partial<f16>(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
 }  // namespace pa
