@@ -167,9 +167,9 @@ template <typename T> void launch_draft_partial(const DraftDev& P, int units, in
 extern template void launch_draft_partial<bf16>(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
 extern template void launch_draft_partial<f16>(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
 extern template void launch_draft_partial<float>(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
-template <typename T> constexpr int draft_row_tiles(int D) {
-    // 16-row tiles that a wave's accumulators hold
-    return D > 128 ? 1 : sizeof(T) == 4 ? 2 : 4;
+// 16-row tiles that a wave's accumulators leave room for, `middle` with a middle level's third stream
+template <typename T> constexpr int draft_row_tiles(int D, bool middle) {
+    return D > 128 ? 1 : sizeof(T) == 4 || (middle && D == 128) ? 2 : 4;
 }
 
 }  // namespace pa

@@ -553,7 +553,8 @@ bool draft_plan(const pa_draft* d, DraftDev& P, int& units, int& tiles) {
     const int most = d->drafts * rep;
     const int64_t chunks = ((int64_t)d->capacity + kDraftChunk - 1) / kDraftChunk * d->batch;
     // rows of a workgroup: as many as its registers hold
-    tiles = most <= 16 ? 1 : std::min(f32 ? draft_row_tiles<float>(D) : draft_row_tiles<bf16>(D), most <= 32 ? 2 : 4);
+    tiles = most <= 16 ? 1 : std::min(f32 ? draft_row_tiles<float>(D, d->order > 2) : draft_row_tiles<bf16>(D, d->order > 2),
+                                              most <= 32 ? 2 : 4);
     P.row_blocks = (most + 16 * tiles - 1) / (16 * tiles);
     P.rec_rows = d->drafts * (d->order - 1) + most;
     P.t16 = (d->drafts + 15) & ~15;

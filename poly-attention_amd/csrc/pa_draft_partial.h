@@ -2,7 +2,7 @@
 //
 // One workgroup per (unit of positions, key head and block of rows, level), four waves, each on its
 // own 32 (fp32: 16) positions at a time; nothing is shared until the end, so there is no barrier in
-// the loop and no LDS between memory and the matrix cores.
+// the loop.
 //
 // S^T = K Q^T with 16x16 tiles (A: 16 positions, lane l holds position l % 16; B: 16 rows): lane l =
 // 16 g + c gets row c and the positions 4 g .. 4 g + 3 of a tile.  A second product over those
@@ -13,6 +13,9 @@
 // two values).  fp32 takes v_mfma_f32_16x16x4_f32, whose operands are single values: no
 // transposition at all.  In O^T a lane holds one row, so the running maximum's rescale is one
 // factor per lane; it moves only past kDraftTau (lazy), so exp2(s - m) is at most 2^8.
+//
+// Bound by memory while the rows are few: 16 rows of a step cost about a tenth of its 16 KB at the
+// memory's rate, 64 rows about as much as them.
 #pragma once
 
 #include "pa_draft.h"
@@ -74,6 +77,8 @@ template <typename T, int D> struct DraftGeo {
     static constexpr int VE = D / 16;              // features per lane of a value row
     static constexpr int VW = F32 ? VE : VE / 2;   // the same in 32-bit words
     static constexpr int KE = F32 ? 4 : 8;         // elements of a 16-byte load
+    static constexpr int CPR = D / KE;             // 16-byte chunks of a row
+    static constexpr int STEP = 16 * KT;           // a wave's positions per step
 };
 
 // A buffer over the rest of a unit: loads past its end (and at kDraftOut) give 0 without touching memory,
@@ -114,11 +119,14 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
     constexpr int KT = G::KT, KS = G::KS, VE = G::VE, KE = G::KE;
     constexpr int PITCH = D + 4;
     // a query row's fragments stay in registers where those are few
-    constexpr bool QLDS = RT * KS * 4 > 32;
+    constexpr bool QLDS = RT * KS * 4 > (G::F32 ? 32 : 16);
     constexpr int OWORDS = 16 * RT * PITCH, QWORDS = QLDS ? RT * KS * 256 : 0;
     // the waves' outputs meet in NB buffers, four where they are small
     constexpr int NB = OWORDS <= 2304 ? 4 : OWORDS <= 4608 ? 2 : 1;
-    __shared__ __align__(16) float s_o[NB * OWORDS > QWORDS ? NB * OWORDS : QWORDS];  // the queries, then these
+    // keys pass through LDS (KLDS) where four waves' steps fit
+    constexpr bool KLDS = D <= 128;
+    constexpr int KWORDS = KLDS ? 4 * G::STEP * G::CPR * 4 : 0, INWORDS = QWORDS + KWORDS;
+    __shared__ __align__(16) float s_o[NB * OWORDS > INWORDS ? NB * OWORDS : INWORDS];  // queries and keys, then these
     u32x4_d* const s_q = reinterpret_cast<u32x4_d*>(s_o);
     __shared__ float s_m[4][16 * RT], s_l[4][16 * RT];
 
@@ -227,14 +235,27 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
     const int64_t kp = L.k.sn * (int64_t)sizeof(T), vp = L.v.sn * (int64_t)sizeof(T),
                   mp = has_m ? L.m.sn * (int64_t)sizeof(T) : 0;  // bytes between positions
     const int rowb = P.dim * (int)sizeof(T);
-    // a lane's offsets inside a step do not change: positions 16 t + c of the keys, 16 t + 4 g + i
-    // of the values
-    int ko[KS];
+    // A lane's offsets inside a step do not change.  Keys: with KLDS a load takes whole rows, 64 / CPR of
+    // them, which the wave turns in its own part of LDS (position c, 16-byte chunk 4 s + g; chunks are
+    // permuted by the position so that neither side meets bank conflicts); loaded as the operand wants
+    // them, 64 bytes of each of 16 rows at a time, they come 8 to 12% slower (32 x 8192: 278 -> 244 us).
+    // Values: positions 16 t + 4 g + i.
+    constexpr int CPR = G::CPR, LOADS = KT * KS;
+    int ko[KLDS ? 1 : KS];
+    if constexpr (KLDS) {
+        ko[0] = lane % CPR * KE < P.dim ? lane / CPR * (int)kp + lane % CPR * 16 : kDraftOut;
+    } else {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        const int d = (KE * 4) * s + KE * g;
-        ko[s] = d < P.dim ? c * (int)kp + d * (int)sizeof(T) : kDraftOut;
+        for (int s = 0; s < KS; ++s) {
+            const int d = (KE * 4) * s + KE * g;
+            ko[s] = d < P.dim ? c * (int)kp + d * (int)sizeof(T) : kDraftOut;
+        }
     }
+    u32x4_d* const s_k = s_q + QWORDS / 4 + wave * (G::STEP * CPR);
+    constexpr int CMASK = CPR < 16 ? CPR - 1 : 15;
+    auto chunk = [](int position, int ch) __attribute__((always_inline)) -> int {
+        return position * CPR + (ch ^ (position & CMASK));
+    };
     const bool vin = VE * c < P.dim;
     const int vo = vin ? 4 * g * (int)vp + VE * c * (int)sizeof(T) : kDraftOut;
     const int mo = vin ? 4 * g * (int)mp + VE * c * (int)sizeof(T) : kDraftOut;
@@ -242,7 +263,7 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
     // One set of registers for the keys and one for the values: the next step's keys are loaded as soon as
     // this step's scores are formed, its values as soon as they have been summed, so that loads are in
     // flight all the time (and twice the waves fit, against two sets).
-    u32x4_d kf[KT][KS];
+    u32x4_d kr[LOADS];
     uint32_t v[G::NP][G::VW];
     uint32_t mv[VM ? G::NP : 1][VM ? G::VW : 1];
     uint32_t bz[KT][4];
@@ -250,18 +271,18 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
         const int left = cnt - j0;  // positions of the unit from here; none past its last step
         const auto rk = draft_buffer(kb + j0 * kp, left > 0 ? (left - 1) * kp + rowb : 0);
 #pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            kr[i] = KLDS ? __builtin_amdgcn_raw_buffer_load_b128(rk, ko[0], i * (64 / CPR) * (int)kp, kDraftStream)
+                         : __builtin_amdgcn_raw_buffer_load_b128(rk, ko[KLDS ? 0 : i % KS], i / KS * 16 * (int)kp, kDraftStream);
+    };
+    auto load_bias = [&](int j0) __attribute__((always_inline)) {
+        if (!bb) return;
+        const auto rb = draft_buffer(bb + 4ll * j0, 4ll * (cnt - j0));
+#pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-                kf[t][s] = __builtin_amdgcn_raw_buffer_load_b128(rk, ko[s], 16 * t * (int)kp, kDraftStream);
-        if (bb) {
-            const auto rb = draft_buffer(bb + 4ll * j0, 4ll * left);
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    bz[t][i] = __builtin_amdgcn_raw_buffer_load_b32(rb, 16 * g, 64 * t + 4 * i, 0);
-        }
+            for (int i = 0; i < 4; ++i)
+                bz[t][i] = __builtin_amdgcn_raw_buffer_load_b32(rb, 16 * g, 64 * t + 4 * i, 0);
     };
     auto load_v = [&](int j0) __attribute__((always_inline)) {
         const int left = cnt - j0;
@@ -285,33 +306,47 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
     constexpr int STEP = 64 * KT;  // the workgroup's positions per round of steps
     const int first = wave * 16 * KT;
     load_k(first);
+    load_bias(first);
     load_v(first);
     for (int j0 = first; j0 < cnt; j0 += STEP) {
-        float x[RT][KT][4];
+        if constexpr (KLDS) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            if (rt >= nrt) break;
-            f32x4_t a[KT];
+            for (int i = 0; i < LOADS; ++i) s_k[chunk(i * (64 / CPR) + lane / CPR, lane % CPR)] = kr[i];
+            // other lanes of the wave read them: LDS keeps a wave's order, the compiler has to as well
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            load_k(j0 + STEP);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        f32x4_t x[RT][KT];
 #pragma unroll
-            for (int t = 0; t < KT; ++t) a[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
+            for (int t = 0; t < KT; ++t) x[rt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            u32x4_d k[KT];
+#pragma unroll
+            for (int t = 0; t < KT; ++t) k[t] = KLDS ? s_k[chunk(16 * t + c, 4 * s + g)] : kr[t * KS + s];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                if (rt >= nrt) break;
                 const u32x4_d q = QLDS ? s_q[(rt * KS + s) * 64 + lane] : qf[QLDS ? 0 : rt][s];
 #pragma unroll
                 for (int t = 0; t < KT; ++t) {
                     if constexpr (G::F32) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) a[t] = mma_f32(kf[t][s][j], q[j], a[t]);
+                        for (int j = 0; j < 4; ++j) x[rt][t] = mma_f32(k[t][j], q[j], x[rt][t]);
                     } else {
-                        a[t] = Mma16<T>::run(kf[t][s], q, a[t]);
+                        x[rt][t] = Mma16<T>::run(k[t], q, x[rt][t]);
                     }
                 }
             }
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[rt][t][i] = a[t][i] * unclamped;
         }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int t = 0; t < KT; ++t) x[rt][t] *= unclamped;
         if (P.softclamp > 0.f) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
@@ -339,7 +374,8 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
                         if (j0 + 16 * t + 4 * g + i >= cnt) x[rt][t][i] = -INFINITY;
         }
         __builtin_amdgcn_sched_barrier(0);
-        load_k(j0 + STEP);
+        if constexpr (!KLDS) load_k(j0 + STEP);
+        load_bias(j0 + STEP);
         __builtin_amdgcn_sched_barrier(0);
         uint32_t pf[RT][4];
 #pragma unroll
@@ -489,20 +525,24 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
     }
 }
 
-template <typename T, int D, int RT>
+template <typename T, int D, int RT, bool MIDDLE>
 void launch_draft_partial_rt(const DraftDev& P, int units, bool vmul, hipStream_t s) {
     const dim3 grid(P.batch + units, P.kv_heads * P.row_blocks, P.order);
-    if (vmul) hipLaunchKernelGGL((k_draft_partial<T, D, RT, true>), grid, dim3(kDraftThreads), 0, s, P);
-    else hipLaunchKernelGGL((k_draft_partial<T, D, RT, false>), grid, dim3(kDraftThreads), 0, s, P);
+    if constexpr (MIDDLE)
+        if (vmul) {
+            hipLaunchKernelGGL((k_draft_partial<T, D, RT, true>), grid, dim3(kDraftThreads), 0, s, P);
+            return;
+        }
+    hipLaunchKernelGGL((k_draft_partial<T, D, RT, false>), grid, dim3(kDraftThreads), 0, s, P);
 }
 
 template <typename T, int D>
 void launch_draft_partial_d(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s) {
-    constexpr int most = draft_row_tiles<T>(D);
-    if (most == 1 || tiles == 1) return launch_draft_partial_rt<T, D, 1>(P, units, vmul, s);
+    constexpr int most = draft_row_tiles<T>(D, false), most_m = draft_row_tiles<T>(D, true);
+    if (tiles == 1) return launch_draft_partial_rt<T, D, 1, (most_m >= 1)>(P, units, vmul, s);
     if constexpr (most >= 2)
-        if (most == 2 || tiles == 2) return launch_draft_partial_rt<T, D, 2>(P, units, vmul, s);
-    if constexpr (most >= 4) launch_draft_partial_rt<T, D, 4>(P, units, vmul, s);
+        if (tiles == 2) return launch_draft_partial_rt<T, D, 2, (most_m >= 2)>(P, units, vmul, s);
+    if constexpr (most >= 4) launch_draft_partial_rt<T, D, 4, (most_m >= 4)>(P, units, vmul, s);
 }
 
 template <typename T>
