@@ -154,79 +154,20 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
         const int d = (KE * 4) * s + KE * g;
         return d < P.dim ? load16u(row + d) : u32x4_d{0u, 0u, 0u, 0u};
     };
-    u32x4_d qf[QLDS ? 1 : RT][KS];
-    if constexpr (QLDS) {  // fragments in LDS, in the order of the lanes
+    u32x4_d qf[QLDS ? 1 : RT][KS], qt[QLDS ? RT * KS / 4 : 1];
+    if constexpr (QLDS) {  // a quarter of the fragments per wave
+        static_assert(RT * KS % 4 == 0, "four waves");
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-            if (rt % 4 == wave || RT < 4)
-#pragma unroll
-                for (int s = 0; s < KS; ++s)
-                    if (RT >= 4 || s % 4 == wave) s_q[(rt * KS + s) * 64 + lane] = query(rt, s);
-        __syncthreads();
+        for (int k = 0; k < RT * KS / 4; ++k) {
+            const int f = wave * (RT * KS / 4) + k;
+            qt[k] = query(f / KS, f % KS);
+        }
     } else {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int s = 0; s < KS; ++s) qf[rt][s] = query(rt, s);
     }
-    const float sl2 = P.scale * kLog2e, cl2 = P.softclamp * kLog2e;
-    const float unclamped = P.softclamp > 0.f ? P.scale / P.softclamp : sl2;
-
-    if (tree) {  // 16 drafted keys per wave
-        if (16 * wave >= P.T) return;
-        const uint64_t anc = draft_ancestors(P.parents ? P.parents + b * P.parents_stride : nullptr, P.T, lane);
-        const uint32_t anc_lo = (uint32_t)anc, anc_hi = (uint32_t)(anc >> 32);
-        const T* row = L.dk.at<T>(b, hk) + min(16 * wave + c, P.T - 1) * L.dk.sn;
-        u32x4_d kf[KS];
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int d = (KE * 4) * s + KE * g;
-            kf[s] = d < P.dim ? load16u(row + d) : u32x4_d{0u, 0u, 0u, 0u};
-        }
-        if (blockIdx.y == 0 && blockIdx.z == 0 && wave == 0) {  // for the join
-            const uint64_t live = __ballot(anc != 0);
-            draft_units(P, b, 0, lane, U);
-            if (lane == 0) P.ws_u[b] = make_int4(U.first, U.number, (int)(uint32_t)live, (int)(live >> 32));
-        }
-        float* to = P.ws_t + (((int64_t)b * P.kv_heads + hk) * P.rec_rows + L.row0 + r0) * P.t16;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            if (rt >= nrt) break;
-            f32x4_t a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const u32x4_d q = QLDS ? s_q[(rt * KS + s) * 64 + lane] : qf[QLDS ? 0 : rt][s];
-                if constexpr (G::F32) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) a = mma_f32(kf[s][j], q[j], a);
-                } else {
-                    a = Mma16<T>::run(kf[s], q, a);
-                }
-            }
-            const int r = r0 + 16 * rt + c;
-            const uint64_t sees = ((uint64_t)__shfl(anc_hi, r % P.T) << 32) | __shfl(anc_lo, r % P.T);
-            f32x4_t y;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = a[i] * unclamped;
-                y[i] = (sees >> (16 * wave + 4 * g + i)) & 1 ? (P.softclamp > 0.f ? cl2 * tanhf(x) : x) : -INFINITY;
-            }
-            if (16 * rt + c < nrows)
-                *reinterpret_cast<f32x4_t*>(to + (int64_t)(16 * rt + c) * P.t16 + 16 * wave + 4 * g) = y;
-        }
-        return;
-    }
-
-    f32x4_t o[RT][VE];
-    float m[RT], l[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        m[rt] = -INFINITY;
-        l[rt] = 0.f;
-#pragma unroll
-        for (int j = 0; j < VE; ++j) o[rt][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
-
     const bool has_m = VM && L.m.p;
     const char* kb = reinterpret_cast<const char*>(L.k.at<T>(b, hk) + begin * L.k.sn);
     const char* vb = reinterpret_cast<const char*>(L.v.at<T>(b, hk) + begin * L.v.sn);
@@ -305,9 +246,73 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
 
     constexpr int STEP = 64 * KT;  // the workgroup's positions per round of steps
     const int first = wave * 16 * KT;
+    // the first step is on its way before the queries are needed (a tree's workgroup has none)
     load_k(first);
     load_bias(first);
     load_v(first);
+    if constexpr (QLDS) {
+#pragma unroll
+        for (int k = 0; k < RT * KS / 4; ++k) s_q[(wave * (RT * KS / 4) + k) * 64 + lane] = qt[k];
+        __syncthreads();
+    }
+    const float sl2 = P.scale * kLog2e, cl2 = P.softclamp * kLog2e;
+    const float unclamped = P.softclamp > 0.f ? P.scale / P.softclamp : sl2;
+
+    if (tree) {  // 16 drafted keys per wave
+        if (16 * wave >= P.T) return;
+        const uint64_t anc = draft_ancestors(P.parents ? P.parents + b * P.parents_stride : nullptr, P.T, lane);
+        const uint32_t anc_lo = (uint32_t)anc, anc_hi = (uint32_t)(anc >> 32);
+        const T* row = L.dk.at<T>(b, hk) + min(16 * wave + c, P.T - 1) * L.dk.sn;
+        u32x4_d kf[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = (KE * 4) * s + KE * g;
+            kf[s] = d < P.dim ? load16u(row + d) : u32x4_d{0u, 0u, 0u, 0u};
+        }
+        if (blockIdx.y == 0 && blockIdx.z == 0 && wave == 0) {  // for the join
+            const uint64_t live = __ballot(anc != 0);
+            draft_units(P, b, 0, lane, U);
+            if (lane == 0) P.ws_u[b] = make_int4(U.first, U.number, (int)(uint32_t)live, (int)(live >> 32));
+        }
+        float* to = P.ws_t + (((int64_t)b * P.kv_heads + hk) * P.rec_rows + L.row0 + r0) * P.t16;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            if (rt >= nrt) break;
+            f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const u32x4_d q = QLDS ? s_q[(rt * KS + s) * 64 + lane] : qf[QLDS ? 0 : rt][s];
+                if constexpr (G::F32) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) a = mma_f32(kf[s][j], q[j], a);
+                } else {
+                    a = Mma16<T>::run(kf[s], q, a);
+                }
+            }
+            const int r = r0 + 16 * rt + c;
+            const uint64_t sees = ((uint64_t)__shfl(anc_hi, r % P.T) << 32) | __shfl(anc_lo, r % P.T);
+            f32x4_t y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = a[i] * unclamped;
+                y[i] = (sees >> (16 * wave + 4 * g + i)) & 1 ? (P.softclamp > 0.f ? cl2 * tanhf(x) : x) : -INFINITY;
+            }
+            if (16 * rt + c < nrows)
+                *reinterpret_cast<f32x4_t*>(to + (int64_t)(16 * rt + c) * P.t16 + 16 * wave + 4 * g) = y;
+        }
+        return;
+    }
+
+    f32x4_t o[RT][VE];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt] = -INFINITY;
+        l[rt] = 0.f;
+#pragma unroll
+        for (int j = 0; j < VE; ++j) o[rt][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
     for (int j0 = first; j0 < cnt; j0 += STEP) {
         if constexpr (KLDS) {
 #pragma unroll

@@ -397,7 +397,8 @@ PACK_PASS_GRAD = struct.Struct("@" + _PASS_FMT + 7 * _VIEW_FMT + "i4x2Q" + 2 * _
 PACK_RMS = struct.Struct("@4if4x" + _VIEW_FMT + "Qi4x" + _VIEW_FMT + "Q" + 2 * _VIEW_FMT + "4Q2iq")
 PACK_VERIFY = struct.Struct("@4iQ2qQqQqQqQqQQ2q5Q")
 PACK_COMMIT = struct.Struct("@6iQqi4x4Q")  # the moves follow
-assert PACK_COMMIT.size == PaCommit.moves.offset
+PACK_MOVE = struct.Struct("@2Q2i")
+assert PACK_COMMIT.size == PaCommit.moves.offset and PACK_MOVE.size == ctypes.sizeof(PaDraftMove)
 for _pack, _cls in ((PACK_VERIFY, PaVerify), (PACK_PASS, PaPass), (PACK_PASS_GRAD, PaPassGrad), (PACK_RMS, PaRmsNorm)):
     assert _pack.size == ctypes.sizeof(_cls), _cls.__name__
 

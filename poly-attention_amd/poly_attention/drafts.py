@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 from typing import Optional, Sequence
 
 import torch
@@ -30,6 +31,12 @@ from torch import Tensor
 
 from . import _lib
 from ._lib import DTYPE_CODE, PA_MAX_DRAFTS, PA_MAX_MOVES
+
+
+# the fields of a PaDraftItem that change from call to call
+_PACK_SRC = struct.Struct("@Q3q").pack_into
+_PACK_NORM = struct.Struct("@Qi").pack_into
+_NORM_AT = _lib.PaDraftItem.norm_weight.offset
 
 
 def _call(fn, t: Tensor, what: str, *args) -> None:
@@ -171,7 +178,6 @@ class DraftCache:
         self.order, self.batch, self.kv_heads, self.dim_head = order, batch, kv_heads, dim_head
         self.capacity, self.max_drafts, self.dtype, self.device = capacity, max_drafts, dtype, device
         self.counts = counts
-        self.overflow = torch.zeros(1, dtype=torch.int32, device=device)
         self.keys_rotated = False
 
         def rows(n, m):
@@ -188,16 +194,15 @@ class DraftCache:
         self.draft_qs, self.draft_vs = rows(max_drafts, order), rows(max_drafts, m)
         self.draft_msgs, self.draft_lses = rows(max_drafts, m), sums(max_drafts)
         # the moves of a commit, laid out once: the buffers stay where they are
-        moves = (_lib.PaDraftMove * (4 * order - 3))()
-        for mv, (src, dst) in zip(moves, zip(
-                (*self.draft_qs, *self.draft_vs, *self.draft_msgs, *self.draft_lses),
-                (*self.qs, *self.vs, *self.msgs, *self.lses))):
-            mv.src, mv.dst = src.data_ptr(), dst.data_ptr()
-            mv.row_bytes = src.element_size() * (dim_head if src.dim() == 4 else 1)
-        self._moves = bytes(moves)
+        row = dtype.itemsize * dim_head
+        pairs = zip((*self.draft_qs, *self.draft_vs, *self.draft_msgs, *self.draft_lses),
+                    (*self.qs, *self.vs, *self.msgs, *self.lses))
+        self._moves = b"".join([_lib.PACK_MOVE.pack(src.data_ptr(), dst.data_ptr(), row if src.dim() == 4 else 4, 0)
+                                for src, dst in pairs])
         self._geometry = (batch, kv_heads, max_drafts, capacity)
-        # rows' tickets of a commit, 0 between calls
-        self._tickets = torch.zeros(batch * _lib.PA_TICKET_STRIDE, dtype=torch.int32, device=device)
+        # rows' tickets of a commit, 0 between calls, and the flag of tokens past the capacity
+        zeros = torch.zeros((batch + 1) * _lib.PA_TICKET_STRIDE, dtype=torch.int32, device=device)
+        self._tickets, self.overflow = zeros[_lib.PA_TICKET_STRIDE:], zeros[:1]
         self._plans = {}  # the calls' structures, by the shape of q1
 
     # -------------------------------------------------------------------------------------
@@ -252,36 +257,40 @@ class DraftCache:
         plan = self._plans.get(("append", q1.shape)) or self._plan("append", q1)
         B, H, T, d = q1.shape
         dtype, device, grad = self.dtype, self.device, torch.is_grad_enabled()
-        P, items = plan
-        keep = []
+        P, buf, offsets = plan
+        keep = [qs, vs, weights]
         P.eps = eps
         parents, P.parents, P.parents_stride = _parents(parents, B, T, device)
         self._set_angles(P, angles, inv_freq, interp, T, keep)
-        shape, kv = q1.shape, (B, self.kv_heads, T, d)
-        for k, (it, view) in enumerate(items):
-            norm = k <= self.order
-            src = qs[k] if norm else vs[k - self.order - 1]
+        es, index, shape, kv, order = dtype.itemsize, device.index, q1.shape, self._kv_shape(T), self.order
+        for k, off in enumerate(offsets):
+            src = qs[k] if k <= order else vs[k - order - 1]
             if src.shape != shape or src.dtype is not dtype or src.device != device:
-                self._check_rows(src, "q%d" % (k + 1) if norm else "v%d" % (k - self.order + 2), T, shape[1])
+                self._check_rows(src, f"q{k + 1}" if k <= order else f"v{k - order + 2}", T, shape[1])
             if grad and src.requires_grad:
                 raise RuntimeError("DraftCache steps are inference-only: run them under torch.no_grad()")
             shape = kv
-            rows = _rows16(src)
-            keep.append(rows)
-            view.ptr = rows.data_ptr()
-            view.sb, view.sh, view.sn, _ = rows.stride()
-            if norm:
+            ptr = src.data_ptr()
+            s0, s1, s2, s3 = src.stride()
+            if s3 != 1 or ((s0 | s1 | s2) * es | ptr) & 15:
+                src = _rows16(src)
+                keep.append(src)
+                ptr = src.data_ptr()
+                s0, s1, s2, s3 = src.stride()
+            _PACK_SRC(buf, off, ptr, s0, s1, s2)
+            if k <= order:
                 w = weights[k]
                 if w is None:
-                    it.norm_weight = None
+                    _PACK_NORM(buf, off + _NORM_AT, 0, 0)
                     continue
-                _need(w.shape == (d,) and w.device == device and w.dtype in DTYPE_CODE,
-                      f"norm weight {k}: [{d}] on the cache's device")
+                code = DTYPE_CODE.get(w.dtype)
+                if code is None or w.dim() != 1 or w.numel() != d or w.device != device:
+                    _need(False, f"norm weight {k}: [{d}] on the cache's device")
                 if w.stride(0) != 1:
                     w = w.contiguous()
                     keep.append(w)
-                it.norm_weight, it.weight_dtype = w.data_ptr(), DTYPE_CODE[w.dtype]
-        out = torch.empty((B, H, T, d), dtype=dtype, device=device)
+                _PACK_NORM(buf, off + _NORM_AT, w.data_ptr(), code)
+        out = torch.empty(B, H, T, d, dtype=dtype, device=device)
         P.items[0].out.ptr = out.data_ptr()
         _call(_lib.load().pa_draft_append, out, "pa_draft_append", ctypes.byref(P))
         return out
@@ -290,7 +299,6 @@ class DraftCache:
         P = _lib.PaDraftRows()
         P.batch, P.drafts, P.dim, P.count = self.batch, T, self.dim_head, 2 * self.order
         P.counts = self.counts.data_ptr()
-        items = []
         for k, (it, out) in enumerate(zip(P.items, (None, *self.draft_qs, *self.draft_vs))):
             it.src.heads = it.out.heads = H if k == 0 else self.kv_heads
             it.src.dtype = it.out.dtype = DTYPE_CODE[self.dtype]
@@ -299,8 +307,11 @@ class DraftCache:
                 _set_view(it.out, out)
             else:
                 it.out.sb, it.out.sh, it.out.sn = H * T * self.dim_head, T * self.dim_head, self.dim_head
-            items.append((it, it.src))
-        return P, items
+        step, base = ctypes.sizeof(_lib.PaDraftItem), _lib.PaDraftRows.items.offset
+        return P, memoryview(P).cast("B"), [base + k * step for k in range(2 * self.order)]
+
+    def _kv_shape(self, T: int) -> tuple:
+        return (self.batch, self.kv_heads, T, self.dim_head)
 
     def _set_angles(self, P, angles, inv_freq, interp, T, keep) -> None:
         if angles is None and inv_freq is None:
@@ -495,23 +506,9 @@ def verify_drafts(logits: Tensor, tokens: Tensor, parents: Optional[Tensor] = No
         logits = logits.contiguous()
     keep = [logits]
 
-    def fixed(t, what, shape, dtype):
-        """Address and leading strides of an optional tensor that has to be of this shape and type."""
-        if t is None:
-            return (0,) * len(shape)
-        if t.dtype is not dtype or t.shape != shape or t.device != dev:
-            _need(t.dtype == dtype, f"{what}: {dtype}, not {t.dtype}", TypeError)
-            _need(t.shape == shape, f"{what}: {list(shape)}, not {list(t.shape)}")
-            _need(False, f"{what}: on another device than logits")
-        strides = t.stride()
-        if strides[-1] != 1 and shape[-1] > 1:
-            t = t.contiguous()
-            keep.append(t)
-            strides = t.stride()
-        return (t.data_ptr(), *strides[:-1])
-
     parents, par_ptr, par_stride = _parents(parents, B, T, dev)
-    path = torch.empty((B, T), dtype=torch.int32, device=dev)
+    bt = (B, T)
+    path = torch.empty(B, T, dtype=torch.int32, device=dev)
     kept = torch.empty(B, dtype=torch.int32, device=dev)
     token = torch.empty(B, dtype=torch.int64, device=dev)
     size = _verify_workspace(B, T, V)
@@ -519,13 +516,33 @@ def verify_drafts(logits: Tensor, tokens: Tensor, parents: Optional[Tensor] = No
     sb, sn, _ = logits.stride()
     packed = _lib.PACK_VERIFY.pack(
         B, T, V, DTYPE_CODE[logits.dtype], logits.data_ptr(), sb, sn,
-        *fixed(tokens, "tokens", (B, T), torch.int64), par_ptr or 0, par_stride,
-        *fixed(uniforms, "uniforms", (B, T), torch.float32), *fixed(noise, "noise", (B, V), torch.float32),
-        *fixed(temperature, "temperature", (B,), torch.float32),
-        *fixed(draft_probs, "draft_probs", (B, T, V), torch.float32),
+        *_fixed(tokens, "tokens", bt, torch.int64, dev, keep), par_ptr or 0, par_stride,
+        *_fixed(uniforms, "uniforms", bt, torch.float32, dev, keep),
+        *_fixed(noise, "noise", (B, V), torch.float32, dev, keep),
+        *_fixed(temperature, "temperature", (B,), torch.float32, dev, keep),
+        *_fixed(draft_probs, "draft_probs", (B, T, V), torch.float32, dev, keep),
         path.data_ptr(), kept.data_ptr(), token.data_ptr(), ws.data_ptr(), size)
     _call(_lib.load().pa_draft_verify, logits, "pa_draft_verify", packed)
     return path, kept, token
+
+
+def _fixed(t: Optional[Tensor], what: str, shape: tuple, dtype, dev, keep: list) -> tuple:
+    """Address and leading strides of an optional tensor that has to be of this shape and type."""
+    if t is None:
+        return _NOTHING[len(shape)]
+    if t.dtype is not dtype or t.shape != shape or t.device != dev:
+        _need(t.dtype == dtype, f"{what}: {dtype}, not {t.dtype}", TypeError)
+        _need(t.shape == shape, f"{what}: {list(shape)}, not {list(t.shape)}")
+        _need(False, f"{what}: on another device than logits")
+    strides = t.stride()
+    if strides[-1] != 1 and shape[-1] > 1:
+        t = t.contiguous()
+        keep.append(t)
+        strides = t.stride()
+    return (t.data_ptr(), *strides[:-1])
+
+
+_NOTHING = tuple((0,) * n for n in range(4))
 
 
 @functools.lru_cache(maxsize=256)
