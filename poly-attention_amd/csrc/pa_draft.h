@@ -167,6 +167,11 @@ template <typename T> void launch_draft_partial(const DraftDev& P, int units, in
 extern template void launch_draft_partial<bf16>(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
 extern template void launch_draft_partial<f16>(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
 extern template void launch_draft_partial<float>(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
+// Waves per SIMD that the first launch's registers are held to, with RT tiles of 16 rows and, for a middle
+// level, a third stream: two where they fit, which hide each other's waits and ends.
+constexpr int draft_waves(int D, int RT, bool middle) {
+    return D <= 128 && D * RT <= (middle && D == 128 ? 128 : 256) ? 2 : 1;
+}
 // 16-row tiles that a wave's accumulators leave room for, `middle` with a middle level's third stream
 template <typename T> constexpr int draft_row_tiles(int D, bool middle) {
     return D > 128 ? 1 : sizeof(T) == 4 || (middle && D == 128) ? 2 : 4;

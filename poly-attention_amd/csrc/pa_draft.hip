@@ -530,10 +530,12 @@ DraftRow draft_row(const pa_view& v) {
 // head dims: multiples of 8, of 16 above 128 (a lane's features are whole: dim / 16 of the padded dim)
 bool draft_dim(int d) { return d >= 8 && d <= 256 && d % 8 == 0 && (d <= 128 || d % 16 == 0); }
 
-// Workgroups of the first launch aimed at: kDraftMany, but kDraftFew where a unit's keys are below
-// kDraftUnitBytes (a workgroup's start and end cost as much as some 30 KB).  32 x 8192 positions of 128:
-// 272 us with 1024, 249 with 2048; order 3, 8 x 2048 of 64: 41 with 1024, 45 with 2048.
-constexpr int64_t kDraftMany = 2048, kDraftFew = 1024, kDraftUnitBytes = 64 * 1024;
+// Workgroups of the first launch aimed at, as multiples of those that are in flight together: kDraftMany,
+// but kDraftFew where a unit's keys are below kDraftUnitBytes per 16 rows, since a workgroup's start
+// and end and its record cost the more the more rows it has.  Behind cold caches: 32 x 8192 positions of
+// 128, 32 rows: 272 us with few, 249 with many; 8 x 4096, 64 rows: 85 with few, 137 with four times as
+// many; order 3, 8 x 2048 of 64, 16 rows: 41 with few, 45 with many.
+constexpr int64_t kDraftMany = 4, kDraftFew = 2, kDraftUnitBytes = 64 * 1024, kDraftCus = 256;
 
 // geometry shared by the workspace query and the launch; false where the request is malformed
 bool draft_plan(const pa_draft* d, DraftDev& P, int& units, int& tiles) {
@@ -560,10 +562,11 @@ bool draft_plan(const pa_draft* d, DraftDev& P, int& units, int& tiles) {
     P.t16 = (d->drafts + 15) & ~15;
     const int64_t per = (int64_t)d->kv_heads * d->order * P.row_blocks;
     // no more units than the capacity has chunks
-    const int64_t target = std::min(std::max<int64_t>(1, kDraftMany / per), chunks);
+    const int64_t flight = kDraftCus * draft_waves(D, tiles, d->order > 2);
+    const int64_t target = std::min(std::max<int64_t>(1, kDraftMany * flight / per), chunks);
     P.target = (int)target;
-    P.target_min = (int)std::min(std::max<int64_t>(1, kDraftFew / per), chunks);
-    P.least = std::max(1, (int)(kDraftUnitBytes / ((int64_t)kDraftChunk * d->dim * (f32 ? 4 : 2))));
+    P.target_min = (int)std::min(std::max<int64_t>(1, kDraftFew * flight / per), chunks);
+    P.least = std::max(1, (int)(kDraftUnitBytes * tiles / ((int64_t)kDraftChunk * d->dim * (f32 ? 4 : 2))));
     units = (int)std::min(target + d->batch, chunks);
     return (int64_t)d->kv_heads * P.row_blocks <= 65535;
 }

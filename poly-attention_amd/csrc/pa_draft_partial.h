@@ -108,21 +108,15 @@ __device__ __forceinline__ void buffer_words(__amdgpu_buffer_rsrc_t r, int off, 
     }
 }
 
-// waves per SIMD to hold registers for: two hide each other's waits and ends
-template <typename T, bool VM> constexpr int draft_waves(int D, int RT) {
-    return D <= 128 && D * RT <= (VM && D == 128 ? 128 : 256) ? 2 : 1;
-}
-
 template <typename T, int D, int RT, bool VM>
-__global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_draft_partial(const DraftDev P) {
+__global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft_partial(const DraftDev P) {
     typedef DraftGeo<T, D> G;
     constexpr int KT = G::KT, KS = G::KS, VE = G::VE, KE = G::KE;
     constexpr int PITCH = D + 4;
     // a query row's fragments stay in registers where those are few
     constexpr bool QLDS = RT * KS * 4 > (G::F32 ? 32 : 16);
-    constexpr int OWORDS = 16 * RT * PITCH, QWORDS = QLDS ? RT * KS * 256 : 0;
-    // the waves' outputs meet in NB buffers, four where they are small
-    constexpr int NB = OWORDS <= 2304 ? 4 : OWORDS <= 4608 ? 2 : 1;
+    // the waves' outputs meet in NB buffers of 16 rows
+    constexpr int OWORDS = 16 * PITCH, QWORDS = QLDS ? RT * KS * 256 : 0, NB = D <= 128 ? 4 : 2;
     // keys pass through LDS (KLDS) where four waves' steps fit
     constexpr bool KLDS = D <= 128;
     constexpr int KWORDS = KLDS ? 4 * G::STEP * G::CPR * 4 : 0, INWORDS = QWORDS + KWORDS;
@@ -465,7 +459,7 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // join the four waves: maxima and sums first, then the outputs one wave after another
+    // join the four waves: maxima and sums first, then the outputs
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         l[rt] += __shfl_xor(l[rt], 16);
@@ -484,28 +478,6 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
         for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][16 * rt + c]);
         f[rt] = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - top);
     }
-    // in NB buffers: as many waves at a time
-#pragma unroll
-    for (int w = 0; w < 4; w += NB) {
-        if (wave / NB == w / NB) {
-            float* const buf = s_o + (wave % NB) * OWORDS;
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < VE; j += 4) {
-                        float4* at = reinterpret_cast<float4*>(&buf[(16 * rt + c) * PITCH + VE * (4 * g + i) + j]);
-                        float4 x = w ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
-                        x.x += f[rt] * o[rt][j][i];
-                        x.y += f[rt] * o[rt][j + 1][i];
-                        x.z += f[rt] * o[rt][j + 2][i];
-                        x.w += f[rt] * o[rt][j + 3][i];
-                        *at = x;
-                    }
-        }
-        __syncthreads();
-    }
     const int64_t rec = ((int64_t)unit * P.kv_heads + hk) * P.rec_rows + L.row0 + r0;
     if (tid < nrows) {
         float top = s_m[0][tid], sum = 0.f;
@@ -514,19 +486,46 @@ __global__ __launch_bounds__(kDraftThreads, (draft_waves<T, VM>(D, RT))) void k_
             sum += s_m[w][tid] == -INFINITY ? 0.f : s_l[w][tid] * __builtin_amdgcn_exp2f(s_m[w][tid] - top);
         P.ws_s[rec + tid] = make_float2(top, sum);
     }
-    const int quads = P.dim / 4;
-    for (int x = tid; x < nrows * quads; x += kDraftThreads) {
-        const int r = x / quads, d = x % quads * 4;
-        float4 y = *reinterpret_cast<const float4*>(&s_o[r * PITCH + d]);
+    // 16 rows at a time, the waves side by side in NB buffers
 #pragma unroll
-        for (int k = 1; k < NB; ++k) {
-            const float4 z = *reinterpret_cast<const float4*>(&s_o[k * OWORDS + r * PITCH + d]);
-            y.x += z.x;
-            y.y += z.y;
-            y.z += z.z;
-            y.w += z.w;
+    for (int rt = 0; rt < RT; ++rt) {
+        if (rt >= nrt) break;
+#pragma unroll
+        for (int w = 0; w < 4; w += NB) {
+            if (NB == 4 || wave / NB == w / NB) {
+                float* const buf = s_o + (wave % NB) * OWORDS + c * PITCH + 4 * VE * g;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < VE; j += 4) {
+                        float4* at = reinterpret_cast<float4*>(buf + VE * i + j);
+                        float4 x = w ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+                        x.x += f[rt] * o[rt][j][i];
+                        x.y += f[rt] * o[rt][j + 1][i];
+                        x.z += f[rt] * o[rt][j + 2][i];
+                        x.w += f[rt] * o[rt][j + 3][i];
+                        *at = x;
+                    }
+            }
+            __syncthreads();
         }
-        *reinterpret_cast<float4*>(P.ws_o + (rec + r) * P.dim + d) = y;
+        const int r = tid >> 4;
+        if (16 * rt + r < nrows)
+#pragma unroll
+            for (int d = 4 * (tid & 15); d < D; d += 64) {
+                if (d >= P.dim) break;
+                float4 y = *reinterpret_cast<const float4*>(&s_o[r * PITCH + d]);
+#pragma unroll
+                for (int k = 1; k < NB; ++k) {
+                    const float4 z = *reinterpret_cast<const float4*>(&s_o[k * OWORDS + r * PITCH + d]);
+                    y.x += z.x;
+                    y.y += z.y;
+                    y.z += z.z;
+                    y.w += z.w;
+                }
+                *reinterpret_cast<float4*>(P.ws_o + (rec + 16 * rt + r) * P.dim + d) = y;
+            }
+        if (rt + 1 < RT) __syncthreads();
     }
 }
 
