@@ -82,7 +82,8 @@ template <typename T, int D> struct DraftGeo {
 };
 
 // A buffer over the rest of a unit: loads past its end (and at kDraftOut) give 0 without touching memory,
-// so neither the last step nor a head dim below D needs a test.
+// so neither the last step nor a head dim below D needs a test.  The whole offset goes into the address
+// that is checked against the end (a scalar offset need not be).
 // They are marked as streaming: a cached position is read once a step, and by the other blocks of rows at
 // about the same time.  Behind a kernel that leaves the caches full of its own data that is worth 20 to
 // 40% (7 rows of up to 21333 positions 147 -> 91 us, 8 x 2048 of order 3 66 -> 41).
@@ -93,15 +94,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t draft_buffer(const char* p, in
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, n, 0x00027000);
 }
 template <int VW>
-__device__ __forceinline__ void buffer_words(__amdgpu_buffer_rsrc_t r, int off, int more, uint32_t (&w)[VW]) {
+__device__ __forceinline__ void buffer_words(__amdgpu_buffer_rsrc_t r, int off, uint32_t (&w)[VW]) {
     if constexpr (VW == 2) {
-        const u32x2_d x = __builtin_amdgcn_raw_buffer_load_b64(r, off, more, kDraftStream);
+        const u32x2_d x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, kDraftStream);
         w[0] = x[0];
         w[1] = x[1];
     } else {
 #pragma unroll
         for (int i = 0; i < VW; i += 4) {
-            const u32x4_d x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * i, more, kDraftStream);
+            const u32x4_d x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * i, 0, kDraftStream);
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[i + j] = x[j];
         }
@@ -207,8 +208,8 @@ __global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft
         const auto rk = draft_buffer(kb + j0 * kp, left > 0 ? (left - 1) * kp + rowb : 0);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
-            kr[i] = KLDS ? __builtin_amdgcn_raw_buffer_load_b128(rk, ko[0], i * (64 / CPR) * (int)kp, kDraftStream)
-                         : __builtin_amdgcn_raw_buffer_load_b128(rk, ko[KLDS ? 0 : i % KS], i / KS * 16 * (int)kp, kDraftStream);
+            kr[i] = __builtin_amdgcn_raw_buffer_load_b128(
+                rk, KLDS ? ko[0] + i * (64 / CPR) * (int)kp : ko[KLDS ? 0 : i % KS] + i / KS * 16 * (int)kp, 0, kDraftStream);
     };
     auto load_bias = [&](int j0) __attribute__((always_inline)) {
         if (!bb) return;
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft
         for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                bz[t][i] = __builtin_amdgcn_raw_buffer_load_b32(rb, 16 * g, 64 * t + 4 * i, 0);
+                bz[t][i] = __builtin_amdgcn_raw_buffer_load_b32(rb, 16 * g + 64 * t + 4 * i, 0, 0);
     };
     auto load_v = [&](int j0) __attribute__((always_inline)) {
         const int left = cnt - j0;
@@ -226,7 +227,7 @@ __global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft
         for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                buffer_words<G::VW>(rv, vo, (16 * t + i) * (int)vp, v[4 * t + i]);
+                buffer_words<G::VW>(rv, vo + (16 * t + i) * (int)vp, v[4 * t + i]);
         if constexpr (VM)
             if (has_m) {
                 const auto rm = draft_buffer(mb + j0 * mp, left > 0 ? (left - 1) * mp + rowb : 0);
@@ -234,7 +235,7 @@ __global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft
                 for (int t = 0; t < KT; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        buffer_words<G::VW>(rm, mo, (16 * t + i) * (int)mp, mv[4 * t + i]);
+                        buffer_words<G::VW>(rm, mo + (16 * t + i) * (int)mp, mv[4 * t + i]);
             }
     };
 

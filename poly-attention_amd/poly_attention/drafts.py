@@ -82,8 +82,8 @@ def _parents(parents: Optional[Tensor], batch: int, drafts: int, device) -> tupl
             and parents.stride(1) == 1):
         return parents, parents.data_ptr(), parents.stride(0)
     _need(parents.device == device, "parents: on another device than the cache")
-    _need(not parents.is_floating_point() and parents.dtype != torch.bool,
-          "parents: an integer tensor", TypeError)
+    _need(parents.dtype in (torch.int64, torch.int32, torch.int16, torch.int8),
+          f"parents: a signed integer tensor, not {parents.dtype}", TypeError)
     _need(parents.shape == (batch, drafts) or parents.shape == (drafts,),
           f"parents: [{batch}, {drafts}] or [{drafts}], not {list(parents.shape)}")
     if parents.dtype != torch.int32:
@@ -120,6 +120,9 @@ class DraftCache:
     dim_head] and ``lses`` fp32 [B, kv_heads, capacity] -- one copy per key head, where the tuple cache
     repeats msg and lse for the query heads of a group, which are equal -- and ``draft_qs``,
     ``draft_vs``, ``draft_msgs``, ``draft_lses`` with ``max_drafts`` slots in place of the capacity.
+
+    The buffers and ``counts`` are written in place and stay the same objects.  A cache takes one step at
+    a time; caches of their own may be used at once, on any streams.
 
     A count reaches the capacity at most: tokens that do not fit are dropped by ``commit_drafts``, which
     sets the device flag ``overflow``; ``check_overflow()`` reads it.
@@ -439,6 +442,7 @@ def commit_drafts(caches: Sequence[DraftCache], path: Tensor, kept: Tensor) -> N
     [B, n] and ``kept`` int32 [B] as ``verify_drafts`` returns them (a path ends early at an entry that is no
     slot; kept 0 leaves a row as it is).  Tokens past the capacity are dropped and flagged
     (``overflow``)."""
+    _need(len(caches) > 0, "a commit needs at least one cache")
     c0 = caches[0]
     counts, geometry, device = c0.counts, c0._geometry, c0.device
     for c in caches:

@@ -180,6 +180,23 @@ def test_attend_is_deterministic_and_follows_its_stream():
         assert torch.equal(o, out)
 
 
+def test_two_caches_at_once_on_two_streams():
+    """Each step's workspace is its own: interleaved launches on two streams give each cache's result."""
+    a, qa, outa = check_attend(2, 2, [700, 90], 8, 4, 2, 64, "bf16", "chain")
+    b, qb, outb = check_attend(3, 3, [300, 0, 41], 8, 4, 2, 64, "bf16", "chain")
+    qa, qb = qa.to(dev()), qb.to(dev())
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(20):
+        for s, c, q in zip(streams, (a, b), (qa, qb)):
+            with torch.cuda.stream(s):
+                outs.append(c.attend(q))
+    torch.cuda.synchronize()
+    for k, o in enumerate(outs):
+        assert torch.equal(o, outb if k % 2 else outa)
+
+
 def test_attend_takes_any_strides_of_q1():
     from poly_attention import DraftCache
 
@@ -379,6 +396,23 @@ def test_verify_logits_without_a_number():
     assert kept.tolist() == [1, 1, 2, 1] and token.tolist() == [-1, 0, 8500, 0]
 
 
+def test_verify_residual_of_nothing():
+    """A draft distribution equal to the target's leaves nothing of p after a rejection (which a number
+    below 1 never causes): p then stays as it was, with one child and with two."""
+    from poly_attention import verify_drafts
+
+    d = dev()
+    for V in (8, 8192):
+        logits, probs = torch.zeros(2, 3, V, device=d), torch.full((2, 3, V), 1.0 / V, device=d)
+        tokens = torch.tensor([[0, 3, 5], [0, 5, 3]], device=d)
+        noise = torch.ones(2, V, device=d)
+        noise[0, 6] = noise[1, 5] = 0.5
+        parents = torch.tensor([[-1, 0, 0], [-1, 0, -2]], device=d)
+        path, kept, token = verify_drafts(logits, tokens, parents, uniforms=torch.ones(2, 3, device=d), noise=noise,
+                                          draft_probs=probs)
+        assert kept.tolist() == [1, 1] and token.tolist() == [6, 5]
+
+
 def test_verify_keeps_the_target_distribution():
     """Over many rows with their own random numbers the first token behind node 0 is distributed as the
     target's softmax, with drafts chosen and with drafts drawn (two children each): with 40000 rows a
@@ -505,6 +539,8 @@ def test_refusals():
     bad(RuntimeError, c.attend, q.clone().requires_grad_())
     bad(ValueError, c.attend, q, parents=torch.zeros(2, 4, dtype=torch.int32, device=d))
     bad(TypeError, c.attend, q, parents=torch.zeros(2, 3, device=d))
+    bad(TypeError, c.attend, q, parents=torch.zeros(2, 3, dtype=torch.uint8, device=d))
+    bad(ValueError, commit_drafts, [], torch.zeros(2, 4, dtype=torch.int32, device=d), torch.zeros(2, dtype=torch.int32, device=d))
     bad(ValueError, c.attend, q, parents=torch.zeros(3, dtype=torch.int32))
     for change in (dict(qs=[q, kv]), dict(vs=[kv, kv]), dict(weights=[None]), dict(qs=[q, q, kv]),
                    dict(angles=torch.zeros(3, 65, device=d)), dict(angles=torch.zeros(3, 66, device=d)),
