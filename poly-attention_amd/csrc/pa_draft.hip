@@ -568,7 +568,7 @@ bool draft_plan(const pa_draft* d, DraftDev& P, int& units, int& tiles) {
     P.target_min = (int)std::min(std::max<int64_t>(1, kDraftFew * flight / per), chunks);
     P.least = std::max(1, (int)(kDraftUnitBytes * tiles / ((int64_t)kDraftChunk * d->dim * (f32 ? 4 : 2))));
     units = (int)std::min(target + d->batch, chunks);
-    return (int64_t)d->kv_heads * P.row_blocks <= 65535;
+    return (int64_t)d->kv_heads * P.row_blocks <= 65535 && (int64_t)d->batch * d->kv_heads <= INT32_MAX / 64;
 }
 
 // the workspace's arrays, and its size

@@ -48,6 +48,12 @@ __device__ __forceinline__ float row_temperature(const VerifyDev& P, int b) {
     return t > 0.f ? t : 0.f;
 }
 
+// log2(e) / temperature as a finite number above 0: a difference of logits of 0 stays 0 and one of
+// -inf stays -inf where the quotient would be infinite or 0
+__device__ __forceinline__ float logit_scale(float temp) {
+    return fminf(fmaxf(kLog2e / temp, FLT_MIN), FLT_MAX);
+}
+
 // the larger value, the lower position of equals; NaN loses
 __device__ __forceinline__ void take_first(float& x, int& i, float y, int j) {
     if (y > x || (y == x && j < i)) {
@@ -126,7 +132,7 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_stats(const VerifyDev P)
     for (int w = 1; w < 4; ++w) take_first(top, at, s_x[w], s_i[w]);
     float sum = 0.f;
     if (temp > 0.f) {
-        const float c = kLog2e / temp, base = top == -INFINITY ? 0.f : top;
+        const float c = logit_scale(temp), base = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int k = 0; k < N; ++k)
 #pragma unroll
@@ -179,7 +185,7 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
     const int chunk = blockIdx.x, b = blockIdx.y;
     const float temp = row_temperature(P, b);
     const bool greedy = !(temp > 0.f);
-    const float c = greedy ? 0.f : kLog2e / temp;
+    const float c = greedy ? 0.f : logit_scale(temp);
     const int32_t* parents = P.parents ? P.parents + b * P.parents_stride : nullptr;
 
     // this chunk's random numbers are in flight over the walk
@@ -466,7 +472,7 @@ int launch_draft_verify(const pa_verify* v, hipStream_t s) {
     ws += (size_t)P.batch * P.chunks * 16;
     P.ticket = reinterpret_cast<uint32_t*>(ws);
     // One launch where a workgroup reads a row's logits in little more time than a launch takes: 64 KB
-    // of fp32 (one row of 5 nodes over 256 tokens: 7.3 -> 4.6 us, and one launch less for the host).
+    // of fp32 (one row of 5 nodes over 256 tokens: 7.3 -> 5.0 us, and one launch less for the host).
     const bool small = P.chunks == 1 && (int64_t)P.T * P.vocab <= 16384;
     auto go = [&](auto tag) {
         typedef decltype(tag) T;

@@ -37,6 +37,7 @@ from ._lib import DTYPE_CODE, PA_MAX_DRAFTS, PA_MAX_MOVES
 _PACK_SRC = struct.Struct("@Q3q").pack_into
 _PACK_NORM = struct.Struct("@Qi").pack_into
 _NORM_AT = _lib.PaDraftItem.norm_weight.offset
+_NO_GRAD = "DraftCache steps are inference-only: run them under torch.no_grad()"
 
 
 def _call(fn, t: Tensor, what: str, *args) -> None:
@@ -151,7 +152,7 @@ class DraftCache:
         self.prefix = n
         for to, src in zip((*self.qs, *self.vs, *self.msgs, *self.lses), (*qs, *vs, *msgs, *lses)):
             rep = src.shape[1] // hk  # query heads of a group hold equal rows
-            to.narrow(2, 0, n).copy_(src[:, ::rep])
+            to.narrow(2, 0, n).copy_(src.detach()[:, ::rep])
 
     @classmethod
     def empty(cls, *, order: int, batch: int, kv_heads: int, dim_head: int, capacity: int,
@@ -271,7 +272,7 @@ class DraftCache:
             if src.shape != shape or src.dtype is not dtype or src.device != device:
                 self._check_rows(src, f"q{k + 1}" if k <= order else f"v{k - order + 2}", T, shape[1])
             if grad and src.requires_grad:
-                raise RuntimeError("DraftCache steps are inference-only: run them under torch.no_grad()")
+                raise RuntimeError(_NO_GRAD)
             shape = kv
             ptr = src.data_ptr()
             s0, s1, s2, s3 = src.stride()
@@ -289,6 +290,8 @@ class DraftCache:
                 code = DTYPE_CODE.get(w.dtype)
                 if code is None or w.dim() != 1 or w.numel() != d or w.device != device:
                     _need(False, f"norm weight {k}: [{d}] on the cache's device")
+                if grad and w.requires_grad:
+                    raise RuntimeError(_NO_GRAD)
                 if w.stride(0) != 1:
                     w = w.contiguous()
                     keep.append(w)
@@ -323,6 +326,7 @@ class DraftCache:
             return
         _need(angles is None or inv_freq is None, "angles or inv_freq, not both")
         if angles is not None:
+            _need(angles.dim() >= 1, "angles: at least one dimension")
             a, r = angles, angles.shape[-1]
             _need(a.device == self.device, "angles: on another device than the cache")
             _need(a.shape == (self.batch, T, r) or a.shape == (T, r) or a.shape == (r,),
@@ -358,7 +362,7 @@ class DraftCache:
         if q1.dtype is not dtype or q1.device != device:
             self._check_rows(q1, "q1", T, H)
         if q1.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("DraftCache steps are inference-only: run them under torch.no_grad()")
+            raise RuntimeError(_NO_GRAD)
         D, q, y, size, strides = plan
         rows = _rows16(q1)
         # heads inner in memory: merging the heads afterwards is a view
@@ -421,7 +425,7 @@ class DraftCache:
                                    "capturing steps (the cached prefix is rotated once, in place)")
             for q in self.qs:
                 head = q.narrow(2, 0, self.prefix)
-                head.copy_(rotary.rotate_queries_or_keys(head))
+                head.copy_(rotary.rotate_queries_or_keys(head).detach())
         self.keys_rotated = True
 
     def check_overflow(self) -> None:

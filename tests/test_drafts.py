@@ -36,6 +36,14 @@ def test_oracle_tree():
     assert DO.walk_tree([-1, 0, 1, 0, 5, 4, -2, 6]) == [[0], [0, 1], [0, 1, 2], [0, 3], None, None, None, None]
 
 
+def test_cache_of_tensors_with_a_gradient():
+    """A prefill outside torch.no_grad(): the buffers hold values, no graph."""
+    q, v = (torch.randn(1, 2, 3, 8, requires_grad=True) * 1 for _ in range(2))
+    c = DraftCache((q, q, v, v[..., 0], v), 5)
+    assert not any(t.requires_grad for t in (*c.qs, *c.vs, *c.msgs, *c.lses))
+    assert torch.equal(c.qs[0][:, :, :3], q) and torch.equal(c.lses[0][:, :, :3], v[..., 0])
+
+
 def test_cache_from_tuples():
     q2, q3, v3 = (torch.randn(2, 2, 5, 64) for _ in range(3))
     lse, msg = torch.randn(2, 2, 5), torch.randn(2, 2, 5, 64)

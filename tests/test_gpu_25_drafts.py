@@ -255,6 +255,24 @@ def test_append(dtype, order, B, T, H, hk, D, rot, shape):
         assert bool((t[:, :, T:] == 7.0).all())
 
 
+def test_append_refuses_to_drop_a_gradient():
+    from poly_attention import DraftCache
+
+    c = DraftCache.empty(order=2, batch=1, kv_heads=2, dim_head=64, capacity=9, dtype=torch.float32, device=dev())
+    row = lambda h: torch.zeros(1, h, 3, 64, device=dev())  # noqa: E731
+    for k in (0, 2, "weight"):
+        qs, vs = [row(2), row(2), row(2)], [row(2)]
+        weights = [torch.ones(64, device=dev()) for _ in qs]
+        if k == "weight":
+            weights[1].requires_grad_()
+        else:
+            qs[k].requires_grad_()
+        with pytest.raises(RuntimeError, match="inference-only"):
+            c.append(qs, vs, weights, eps=1e-6)
+        with torch.no_grad():
+            c.append(qs, vs, weights, eps=1e-6)
+
+
 def test_append_positions_of_a_rotary_module():
     """inv_freq: the angle of a node is its row's count plus its depth, as the single-token prologue
     forms it (fp32 here: the position is exact)."""
@@ -394,6 +412,24 @@ def test_verify_logits_without_a_number():
     assert kept.tolist() == [1, 1, 2, 1] and token.tolist() == [-1, -1, 8500, 2]
     path, kept, token = verify_drafts(logits.to(d), tokens.to(d))
     assert kept.tolist() == [1, 1, 2, 1] and token.tolist() == [-1, 0, 8500, 0]
+
+
+def test_verify_temperatures_near_zero_and_infinite():
+    """A temperature so small that 1 / temperature is infinite puts all of p on the largest logit; an
+    infinite one spreads it over every logit that is not -inf."""
+    from poly_attention import verify_drafts
+
+    d = dev()
+    for V in (16, 8192):
+        logits = torch.arange(V, dtype=torch.float32, device=d).expand(2, 1, V).contiguous()
+        logits[:, :, 0] = -float("inf")
+        noise = torch.ones(2, V, device=d)
+        noise[:, 5] = 0.5
+        noise[:, 0] = 0.25
+        path, kept, token = verify_drafts(
+            logits, torch.zeros(2, 1, dtype=torch.int64, device=d), uniforms=torch.zeros(2, 1, device=d),
+            noise=noise, temperature=torch.tensor([1e-40, float("inf")], device=d))
+        assert kept.tolist() == [1, 1] and token.tolist() == [V - 1, 5]
 
 
 def test_verify_residual_of_nothing():
