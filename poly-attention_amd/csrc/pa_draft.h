@@ -81,10 +81,10 @@ __device__ __forceinline__ int draft_chunks(const DraftCommon& P, int b) {
     return (int)(((unsigned)draft_count(P, b) + kDraftChunk - 1) / kDraftChunk);
 }
 
-// How the cached positions are split: units of `size` chunks in all rows, so many that there are about
-// `target` of them (at most target + batch), counted on the device.
+// How the cached positions are split: units of at most so many chunks in all rows that there are about
+// `target` of them (at most target + batch), counted on the device; a row's units are of one size.
 struct DraftUnits {
-    int size;    // chunks per unit
+    int size;    // chunks per unit of row b
     int b;       // the row of the unit asked for
     int place;   // its place among the row's units
     int first;   // the first unit of row b
@@ -109,6 +109,7 @@ __device__ __forceinline__ bool draft_units(const DraftCommon& P, int want, int 
         r.first = 0;
         r.place = u;
         r.number = draft_ceil(n, r.size);
+        if (r.number > 0) r.size = draft_ceil(n, r.number);
         return want >= 0 || u < r.number;
     }
     unsigned total = 0, n0 = 0;  // n0: this lane's row of the first 64
@@ -122,7 +123,8 @@ __device__ __forceinline__ bool draft_units(const DraftCommon& P, int want, int 
     int before = 0;
     for (int r0 = 0; r0 < P.batch; r0 += 64) {
         const int row = r0 + lane;
-        const int mine = draft_ceil(r0 == 0 ? n0 : row < P.batch ? draft_chunks(P, row) : 0, r.size);
+        const unsigned n = r0 == 0 ? n0 : row < P.batch ? draft_chunks(P, row) : 0;
+        const int mine = draft_ceil(n, r.size);
         int incl = mine;
         for (int off = 1; off < 64; off <<= 1) {
             const int y = __shfl_up(incl, off);
@@ -136,6 +138,7 @@ __device__ __forceinline__ bool draft_units(const DraftCommon& P, int want, int 
             r.number = __builtin_amdgcn_readlane(mine, l);
             r.first = before + __builtin_amdgcn_readlane(incl, l) - r.number;
             r.place = u - r.first;
+            if (r.number > 0) r.size = draft_ceil(__builtin_amdgcn_readlane(n, l), r.number);
             return true;
         }
         before += __builtin_amdgcn_readlane(incl, 63);
@@ -167,14 +170,29 @@ template <typename T> void launch_draft_partial(const DraftDev& P, int units, in
 extern template void launch_draft_partial<bf16>(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
 extern template void launch_draft_partial<f16>(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
 extern template void launch_draft_partial<float>(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);
+// the same for 16-bit types where draft_wide says so
+template <typename T> void launch_draft_wide(const DraftDev& P, int units, bool vmul, hipStream_t s);
+extern template void launch_draft_wide<bf16>(const DraftDev& P, int units, bool vmul, hipStream_t s);
+extern template void launch_draft_wide<f16>(const DraftDev& P, int units, bool vmul, hipStream_t s);
+// its waves, and their 16-row tiles: what two waves per SIMD have registers for
+constexpr int kDraftWideWaves = 4;
+// Whether a group of `rows` rows at the final level goes to k_draft_wide (D: the padded head dim).  Both, in
+// us, behind cold caches: 40 rows of 128, 8 x 4096 positions 83 here, 68 there, 64 rows 85 and 69, 20 x 500
+// 48 rows 49 and 31; 64 rows of 64, 8 x 4096 48 and 48, 48 rows 20 x 500 26 and 24.  With a middle level
+// 64 rows of 64 (order 3, 8 x 2048) 84 and 105, 128 rows 33 and 31; 64 rows of 128 72 and 69.
+constexpr bool draft_wide(int D, bool f32, bool middle, int rows) {
+    return !f32 && D <= 128 && rows > (D == 64 && middle ? 64 : 32);
+}
+constexpr int draft_wide_tiles(int D) { return D <= 64 ? 4 : 2; }
 // Waves per SIMD that the first launch's registers are held to, with RT tiles of 16 rows and, for a middle
 // level, a third stream: two where they fit, which hide each other's waits and ends.
 constexpr int draft_waves(int D, int RT, bool middle) {
     return D <= 128 && D * RT <= (middle && D == 128 ? 128 : 256) ? 2 : 1;
 }
-// 16-row tiles that a wave's accumulators leave room for, `middle` with a middle level's third stream
+// 16-row tiles of a workgroup of that kernel, at most: what a wave's accumulators leave room for, and 16-bit
+// blocks of more rows are the other kernel's (draft_wide); `middle` with a middle level's third stream
 template <typename T> constexpr int draft_row_tiles(int D, bool middle) {
-    return D > 128 ? 1 : sizeof(T) == 4 || (middle && D == 128) ? 2 : 4;
+    return D > 128 ? 1 : sizeof(T) == 2 && D == 64 && middle ? 4 : 2;
 }
 
 }  // namespace pa

@@ -533,9 +533,9 @@ bool draft_dim(int d) { return d >= 8 && d <= 256 && d % 8 == 0 && (d <= 128 || 
 // Workgroups of the first launch aimed at, as multiples of those that are in flight together: kDraftMany,
 // but kDraftFew where a unit's keys are below kDraftUnitBytes per 16 rows, since a workgroup's start
 // and end and its record cost the more the more rows it has.  Behind cold caches: 32 x 8192 positions of
-// 128, 32 rows: 272 us with few, 249 with many; 8 x 4096, 64 rows: 85 with few, 137 with four times as
-// many; order 3, 8 x 2048 of 64, 16 rows: 41 with few, 45 with many.
-constexpr int64_t kDraftMany = 4, kDraftFew = 2, kDraftUnitBytes = 64 * 1024, kDraftCus = 256;
+// 128, 32 rows: 272 us with few, 249 with many; order 3, 8 x 2048 of 64, 16 rows: 41 with few, 45 with many.
+// k_draft_wide: 8 x 4096 of 128 in one round 69, in two 79 (64 rows), 84 and 90 (128 rows).
+constexpr int64_t kDraftMany = 4, kDraftFew = 2, kDraftWideMany = 2, kDraftUnitBytes = 64 * 1024, kDraftCus = 256;
 
 // geometry shared by the workspace query and the launch; false where the request is malformed
 bool draft_plan(const pa_draft* d, DraftDev& P, int& units, int& tiles) {
@@ -557,15 +557,20 @@ bool draft_plan(const pa_draft* d, DraftDev& P, int& units, int& tiles) {
     // rows of a workgroup: as many as its registers hold
     tiles = most <= 16 ? 1 : std::min(f32 ? draft_row_tiles<float>(D, d->order > 2) : draft_row_tiles<bf16>(D, d->order > 2),
                                               most <= 32 ? 2 : 4);
+    const bool wide = draft_wide(D, f32, d->order > 2, most);
+    if (wide) tiles = kDraftWideWaves * draft_wide_tiles(D);
     P.row_blocks = (most + 16 * tiles - 1) / (16 * tiles);
     P.rec_rows = d->drafts * (d->order - 1) + most;
     P.t16 = (d->drafts + 15) & ~15;
-    const int64_t per = (int64_t)d->kv_heads * d->order * P.row_blocks;
+    const int low = (d->drafts + 16 * tiles - 1) / (16 * tiles);  // blocks of a level below the final one
+    const int64_t per = (int64_t)d->kv_heads * (P.row_blocks + (d->order - 1) * low);  // workgroups per unit
     // no more units than the capacity has chunks
-    const int64_t flight = kDraftCus * draft_waves(D, tiles, d->order > 2);
-    const int64_t target = std::min(std::max<int64_t>(1, kDraftMany * flight / per), chunks);
+    const int64_t flight = kDraftCus * (wide ? 2 : draft_waves(D, tiles, d->order > 2));
+    const int64_t target = std::min(std::max<int64_t>(1, (wide ? kDraftWideMany : kDraftMany) * flight / per), chunks);
     P.target = (int)target;
-    P.target_min = (int)std::min(std::max<int64_t>(1, kDraftFew * flight / per), chunks);
+    // in one round of workgroups, with half a unit per row that the rows' ends add
+    const int64_t few = wide ? flight / per - d->batch / 2 : kDraftFew * flight / per;
+    P.target_min = (int)std::min(std::max<int64_t>(1, few), chunks);
     P.least = std::max(1, (int)(kDraftUnitBytes * tiles / ((int64_t)kDraftChunk * d->dim * (f32 ? 4 : 2))));
     units = (int)std::min(target + d->batch, chunks);
     return (int64_t)d->kv_heads * P.row_blocks <= 65535 && (int64_t)d->batch * d->kv_heads <= INT32_MAX / 64;
@@ -666,7 +671,10 @@ int launch_draft_attend(const pa_draft* d, hipStream_t s) {
     }
     {
         ProfScope ps("draft_partial", s);
-        if (T == PA_F32) launch_draft_partial<float>(P, units, tiles, vmul, s);
+        if (tiles >= kDraftWideWaves * draft_wide_tiles(128)) {
+            if (T == PA_F16) launch_draft_wide<f16>(P, units, vmul, s);
+            else launch_draft_wide<bf16>(P, units, vmul, s);
+        } else if (T == PA_F32) launch_draft_partial<float>(P, units, tiles, vmul, s);
         else if (T == PA_F16) launch_draft_partial<f16>(P, units, tiles, vmul, s);
         else launch_draft_partial<bf16>(P, units, tiles, vmul, s);
     }

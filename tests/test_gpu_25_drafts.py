@@ -122,6 +122,24 @@ def test_attend(dtype, order, B, counts, T, H, hk, D, kind):
     check_attend(order, B, counts, T, H, hk, D, dtype, kind)
 
 
+@param("dtype", ("bf16", "f16"))
+@param("order,B,counts,T,H,hk,D,kind", [
+    (2, 2, [0, 1], 64, 8, 4, 64, "tree"),         # blocks of more than 64 rows: nothing cached, one position
+    (2, 2, [127, 1000], 33, 4, 2, 128, "holes"),  # 66 rows: 32, 32, 2 and none per wave
+    (2, 3, [33, 64, 2500], 13, 8, 1, 96, "forest"),
+    (3, 2, [600, 5], 40, 8, 2, 64, "tree"),       # a middle level of fewer rows than a block holds
+    (4, 1, [300], 64, 8, 1, 128, "tree"),         # several blocks
+    (3, 1, [1500], 64, 5, 1, 40, "chain"),        # 320 rows of 64 padded columns
+    (2, 70, [7 * b % 90 for b in range(70)], 17, 4, 1, 8, "holes"),
+])
+def test_attend_wide_blocks(dtype, order, B, counts, T, H, hk, D, kind):
+    check_attend(order, B, counts, T, H, hk, D, dtype, kind)
+
+
+def test_attend_wide_blocks_softclamp():
+    check_attend(3, 2, [100, 3], 24, 6, 2, 128, "bf16", "tree", softclamp=5.0)
+
+
 @param("dtype,softclamp,scale", [("bf16", 5.0, None), ("f32", 30.0, 0.05), ("f16", 0.5, 1.0), ("f32", None, 0.0)])
 def test_attend_softclamp_and_scale(dtype, softclamp, scale):
     check_attend(3, 2, [100, 3], 6, 4, 2, 64, dtype, "tree", softclamp=softclamp, scale=scale)
