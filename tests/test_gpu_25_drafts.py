@@ -215,6 +215,29 @@ def test_two_caches_at_once_on_two_streams():
         assert torch.equal(o, outb if k % 2 else outa)
 
 
+@param("value", (float("nan"), float("inf")))
+@param("dtype,T,H,D", [("f32", 5, 2, 64), ("f32", 40, 4, 64), ("bf16", 20, 8, 128), ("f16", 64, 2, 64)])
+def test_attend_what_another_branch_holds(dtype, T, H, D, value):
+    """A node's key, query and value that are no numbers leave the outputs of all nodes that do not see it
+    as they were: the same sums in the same order."""
+    cache, q1, _ = check_attend(3, 2, [130, 3], T, H, 2, D, dtype, "chain")
+    parents = torch.zeros(T, dtype=torch.int32, device=dev())
+    parents[0] = -1
+    q1, bad = q1.to(dev()), T // 2
+    others = [t for t in range(T) if t != bad]
+
+    def step():
+        out = cache.attend(q1, parents=parents)
+        return [x[:, :, others].clone() for x in (out, *cache.draft_msgs, *cache.draft_lses)]
+
+    want = step()
+    q1[:, :, bad] = value
+    for t in (*cache.draft_qs, *cache.draft_vs):
+        t[:, :, bad] = value
+    for x, y in zip(step(), want):
+        assert bool(y.isfinite().all()) and torch.equal(x, y)
+
+
 def test_attend_takes_any_strides_of_q1():
     from poly_attention import DraftCache
 
