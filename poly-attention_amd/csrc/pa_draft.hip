@@ -339,7 +339,8 @@ void launch_combine(const DraftJoin& P, dim3 grid, size_t lds, hipStream_t s) {
 // ---------------------------------------------------------------------------------------
 // Norms and rotary of a step's nodes into their draft slots.  One workgroup per (node, tensor), a lane
 // holding 16 bytes of a row: a lane's features are the same in all its rows, so the sines and cosines
-// are computed once per lane (they cost more than the rows), while the first rows are on their way.
+// are computed once per lane (they cost more than the rows), while the first rows are on their way.  Bound by
+// that one chain: 32 x 8 nodes of 32 + 3 x 8 heads of 128 take 5.8 us, 5 nodes of 8 heads of 64 5.2.
 
 struct DraftItemDev {
     DraftRow src, out;
@@ -535,7 +536,8 @@ __device__ __forceinline__ void move_rows(const char* src, char* dst, int64_t sh
     }
 }
 
-// One workgroup per (row, move).  With advance the workgroup of a row that draws the last ticket counts the
+// One workgroup per (row, move): 8 rows of 54 buffers 4.9 us, one of 5 3.9 (paths, rows, counts: three dependent
+// trips to memory).  With advance the workgroup of a row that draws the last ticket counts the
 // kept nodes: by then every other one has read the count, so one launch does both.
 __global__ __launch_bounds__(kDraftThreads) void k_draft_commit(const DraftCommitDev P) {
     const int tid = threadIdx.x, b = blockIdx.x;

@@ -10,6 +10,10 @@
 // The token is the largest p_i / noise_i: one pass, no cumulative sums, and p's common factor drops
 // out.  Only a test of a further child after a rejection needs the residual's sum; without a draft
 // distribution that is 1 - (rejected probabilities), with one a pass over the row.
+//
+// 32 trees of 16 nodes over 32000 tokens (bf16): 10.2 us for the statistics (3.6 TB/s: 4096 short workgroups),
+// 10.0 for the walk (dependent trips to memory).  8 chains of 6 over 128256 (fp32) with the drafts'
+// distributions: 6.0 and 12.8.
 #include "pa_draft.h"
 
 namespace pa {
