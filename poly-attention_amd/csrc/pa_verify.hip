@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kVerThreads = 256;
 constexpr int kVerChunk = 4096;  // entries of a workgroup: 16 per thread, held in registers
+constexpr int kVerSmallNodes = 8, kVerSmallLoads = 2;  // what the single launch takes: 16-byte loads of a row per lane
 
 struct VerifyDev {
     int32_t batch, T, vocab, chunks;
@@ -206,25 +207,39 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
     const int parent = node ? (parents ? parents[lane] : lane - 1) : -2;
     const int64_t tok = node ? P.tokens[b * P.tokens_stride + lane] : -1;
     const float u = node && !greedy ? P.uniforms[b * P.uniforms_stride + lane] : 0.f;
-    if constexpr (SMALL) {
-        for (int t = wave; t < P.T; t += kVerThreads / 64) {
-            const T* x = reinterpret_cast<const T*>(P.logits) + b * P.logits_sb + t * P.logits_sn;
+    if constexpr (SMALL) {  // a row in a wave's registers, all rows on their way at once
+        constexpr int R = kVerSmallNodes * 64 / kVerThreads;
+        float x[R][kVerSmallLoads][E];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int t = min(wave + r * (kVerThreads / 64), P.T - 1);
+            const T* from = reinterpret_cast<const T*>(P.logits) + b * P.logits_sb + t * P.logits_sn;
+#pragma unroll
+            for (int k = 0; k < kVerSmallLoads; ++k) load_entries<T, E>(from, (k * 64 + lane) * E, P.vocab, -INFINITY, x[r][k]);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int t = wave + r * (kVerThreads / 64);
             float top = -INFINITY, sum = 0.f;
             int at = P.vocab;
-            for (int i = lane; i < P.vocab; i += 64) {
-                const float y = to_f(x[i]);
-                if (y > top) {
-                    top = y;
-                    at = i;
-                }
-            }
+#pragma unroll
+            for (int k = 0; k < kVerSmallLoads; ++k)
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (x[r][k][e] > top) {
+                        top = x[r][k][e];
+                        at = (k * 64 + lane) * E + e;
+                    }
             for (int off = 32; off > 0; off >>= 1) take_first(top, at, __shfl_xor(top, off), __shfl_xor(at, off));
             if (!greedy) {
                 const float base = top == -INFINITY ? 0.f : top;
-                for (int i = lane; i < P.vocab; i += 64) sum += __builtin_amdgcn_exp2f((to_f(x[i]) - base) * c);
+#pragma unroll
+                for (int k = 0; k < kVerSmallLoads; ++k)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) sum += __builtin_amdgcn_exp2f((x[r][k][e] - base) * c);  // 0 past the end
                 sum = wave_sum(sum);
             }
-            if (lane == 0) {
+            if (t < P.T && lane == 0) {
                 s_top[t] = top;
                 s_inv[t] = 1.f / sum;
                 s_arg[t] = at;
@@ -291,10 +306,31 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
                 // the sum of the newest residual, now that a further child needs it
                 const float top = s_top[cur], inv = s_inv[cur];
                 float part = 0.f;
-                for (int64_t i = tid; i < P.vocab; i += kVerThreads) {
-                    const float p = __builtin_amdgcn_exp2f((to_f(row[cur * P.logits_sn + i]) - top) * c) * inv;
-                    const float q = qrow[cur * P.probs_sn + i];
-                    part += fmaxf(residual(p, q, s_rinv, nrej - 1) - q, 0.f);
+                float x[2][N][E], q[2][N][E];
+                auto fetch = [&](int i, float (&x)[N][E], float (&q)[N][E]) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        const int64_t at = i + (int64_t)k * kVerThreads * E;
+                        load_entries<T, E>(row + cur * P.logits_sn, at, P.vocab, -INFINITY, x[k]);
+                        load_entries<float, E>(qrow + cur * P.probs_sn, at, P.vocab, 1.f, q[k]);
+                    }
+                };
+                auto add = [&](float (&x)[N][E], float (&q)[N][E]) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            const float p = __builtin_amdgcn_exp2f((x[k][e] - top) * c) * inv;  // 0 past the end
+                            part += fmaxf(residual(p, q[k][e], s_rinv, nrej - 1) - q[k][e], 0.f);
+                        }
+                };
+                // two chunks in turn, one on its way
+                fetch(tid * E, x[0], q[0]);
+                for (int i = tid * E; i - tid * E < P.vocab; i += 2 * kVerChunk) {
+                    fetch(i + kVerChunk, x[1], q[1]);
+                    add(x[0], q[0]);
+                    fetch(i + 2 * kVerChunk, x[0], q[0]);
+                    add(x[1], q[1]);
                 }
                 part = wave_sum(part);
                 if (lane == 0) s_wave[wave] = part;
@@ -475,9 +511,9 @@ int launch_draft_verify(const pa_verify* v, hipStream_t s) {
     P.best = reinterpret_cast<uint64_t*>(ws);
     ws += (size_t)P.batch * P.chunks * 16;
     P.ticket = reinterpret_cast<uint32_t*>(ws);
-    // One launch where a workgroup reads a row's logits in little more time than a launch takes: 64 KB
-    // of fp32 (one row of 5 nodes over 256 tokens: 7.3 -> 5.0 us, and one launch less for the host).
-    const bool small = P.chunks == 1 && (int64_t)P.T * P.vocab <= 16384;
+    // One launch where a row's logits fit the registers of a wave and a wave has two nodes at most (one row of 5
+    // nodes over 256 tokens: 13.7 us behind cold caches, 5 else; two launches 17.4).
+    const bool small = P.T <= kVerSmallNodes && P.vocab <= 64 * kVerSmallLoads * (v->dtype == PA_F32 ? 4 : 8);
     auto go = [&](auto tag) {
         typedef decltype(tag) T;
         if (small) {
