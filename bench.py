@@ -447,9 +447,9 @@ class _Block(torch.nn.Module):
         self.ffn = torch.nn.Sequential(torch.nn.Linear(dim, 4 * dim), torch.nn.GELU(),
                                        torch.nn.Linear(4 * dim, dim))
 
-    def forward(self, x, rotary_pos_emb=None, cache=None):
+    def forward(self, x, rotary_pos_emb=None, cache=None, parents=None):
         attn_out, new_cache = self.attn(self.norm1(x), rotary_pos_emb=rotary_pos_emb,
-                                        cache=cache, return_cache=True)
+                                        cache=cache, return_cache=True, parents=parents)
         if x.is_cuda:
             # decode-sized inputs: the residual add, the norm, the GELU and the second residual
             # add ride in the projections' launches (pa_linear_small), rounded as the separate
@@ -477,8 +477,9 @@ class _PolyLM(torch.nn.Module):
         self.norm = torch.nn.RMSNorm(dim)
         self.to_logits = torch.nn.Linear(dim, num_tokens, bias=False)
 
-    def forward(self, x, cache=None, pos=None):
-        """``pos``: the positions as a device tensor (a captured step has no host count)."""
+    def forward(self, x, cache=None, pos=None, parents=None):
+        """``pos``: the positions as a device tensor (a captured step has no host count);
+        ``parents``: the tree of a drafted step's tokens (DraftCaches)."""
         seq_len = x.shape[1]
         past = 0 if cache is None else cache[1]
         layer_caches = [None] * len(self.layers) if cache is None else cache[0]
@@ -488,7 +489,7 @@ class _PolyLM(torch.nn.Module):
         x = self.token_emb(x)
         new = []
         for layer, lc in zip(self.layers, layer_caches):
-            x, nc = layer(x, rotary_pos_emb=rot, cache=lc)
+            x, nc = layer(x, rotary_pos_emb=rot, cache=lc, parents=parents)
             new.append(nc)
         if x.is_cuda:
             from poly_attention import _ops
@@ -707,6 +708,62 @@ def decode_order3_bench(dev, cpu, steps=512, prefill=2048, batch=8, warm=2, eage
     return res
 
 
+def drafted_decode_bench(dev, drafts, steps=256, prefill=2048, batch=8, warm=2):
+    """Config 4's stack with ``drafts`` tokens a row and step: the last decided one and drafts that
+    follow it, each the token that last followed the one before in its row (prompt and output).
+    One step -- drafting, the model, verification (greedy), commit -- is one HIP graph."""
+    from poly_attention import DraftCache, commit_drafts, verify_drafts
+
+    lm, prompt = make_lm(dev, batch=batch, prefill=prefill)
+    with torch.no_grad():
+        logits, (layer_caches, n) = lm(prompt)
+        counts = torch.full((batch,), n, dtype=torch.int32, device=dev)
+        caches = [DraftCache(c, n + (steps + warm) * drafts, max_drafts=drafts, counts=counts)
+                  for c in layer_caches]
+        del layer_caches
+        last = logits[:, -1].argmax(-1)
+        follow = torch.zeros(batch, 256, dtype=torch.int64, device=dev)
+        follow.scatter_(1, prompt[:, :-1], prompt[:, 1:])
+        tokens = torch.zeros(batch, drafts, dtype=torch.int64, device=dev)
+        slot = torch.arange(drafts, device=dev)
+
+        def step():
+            tokens[:, 0] = last
+            for t in range(1, drafts):
+                tokens[:, t:t + 1] = follow.gather(1, tokens[:, t - 1:t])
+            lg, _ = lm(tokens, (caches, None), pos=caches[0].positions(drafts))
+            path, kept, token = verify_drafts(lg, tokens)
+            commit_drafts(caches, path, kept)
+            after = torch.where(slot + 1 == kept[:, None], token[:, None], tokens.roll(-1, 1))
+            follow.scatter_(1, tokens, torch.where(slot < kept[:, None], after, follow.gather(1, tokens)))
+            last.copy_(token)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(warm):
+                step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        torch.cuda.synchronize()
+        before = counts.sum().item()
+        t0 = time.perf_counter()
+        for _ in range(steps):
+            graph.replay()
+        torch.cuda.synchronize()
+        seconds = time.perf_counter() - t0
+        for c in caches:
+            c.check_overflow()
+        kept = counts.sum().item() - before
+    return {"workload": f"order-3 drafted decode, config 4's stack, batch {batch}, prefill {prefill}, {drafts} tokens "
+                        f"per row and step, {steps} greedy steps",
+            "ms_per_step": round(seconds / steps * 1e3, 4), "tokens_per_s": round(kept / seconds, 1),
+            "kept_per_row_and_step": round(kept / steps / batch, 3),
+            "mode": "DraftCache + one HIP graph per step"}
+
+
 def _lib():
     from poly_attention import _lib as lib
 
@@ -835,6 +892,8 @@ def main():
     ap.add_argument("--no-vit", action="store_true", help="skip config 3 (PolyViT forward)")
     ap.add_argument("--no-lm", action="store_true", help="skip config 4 (order-3 decode loop)")
     ap.add_argument("--lm-steps", type=int, default=512, help="config 4: greedy decode steps")
+    ap.add_argument("--lm-drafts", type=int, default=0,
+                    help="config 4 with this many drafted tokens per row and step, beside it (0: off)")
     ap.add_argument("--lm-no-eager", action="store_true",
                     help="config 4: skip the eager tuple-cache loop (profiling runs)")
     ap.add_argument("--calib-copy", action="store_true",
@@ -953,6 +1012,9 @@ def main():
         lm = decode_order3_bench(dev, cpu=not args.no_cpu, steps=args.lm_steps,
                                  eager=not args.lm_no_eager)
         log(f"[bench] config 4 {lm}")
+        if args.lm_drafts:
+            lm["drafted"] = drafted_decode_bench(dev, args.lm_drafts)
+            log(f"[bench] config 4 drafted {lm['drafted']}")
 
     cpu = None
     if not args.no_cpu:

@@ -347,7 +347,7 @@ typedef struct pa_linear {
  * its outputs are 0 and the walk of pa_draft_verify never reaches it.
  * The drafted tokens' keys, values, level outputs and logsumexps lie in draft slots [B, kv_heads,
  * T, dim] beside the cache until pa_draft_commit moves the kept ones behind the cached positions.
- * A count below 0 or above the capacity is taken as that bound. */
+ * A count below 0 or above the capacity (at most 2^30) is taken as that bound. */
 
 /* One level of pa_draft_attend. */
 typedef struct pa_draft_level {

@@ -676,7 +676,7 @@ int launch_draft_attend(const pa_draft* d, hipStream_t s) {
         return PA_EINVAL;
     const int T = d->levels[0].k.dtype;
     if (!draft_dtype(T)) return PA_EINVAL;
-    if (!draft_dim(d->dim)) return PA_EUNSUPPORTED;
+    if (!draft_dim(d->dim) || d->capacity > (1 << 30)) return PA_EUNSUPPORTED;  // 32-bit positions, a step ahead
     DraftDev P;
     int units = 0, tiles = 0;
     if (!draft_plan(d, P, units, tiles)) return PA_EUNSUPPORTED;

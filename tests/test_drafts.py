@@ -140,7 +140,7 @@ def broken(fn, args, path, value):
 
 @param("path,value,want", [
     ("batch", 0, "EINVAL"), ("kv_heads", 0, "EINVAL"), ("heads", 3, "EINVAL"), ("drafts", 0, "EINVAL"),
-    ("drafts", 65, "EINVAL"), ("order", 1, "EINVAL"), ("order", 9, "EINVAL"), ("capacity", 0, "EINVAL"),
+    ("drafts", 65, "EINVAL"), ("order", 1, "EINVAL"), ("order", 9, "EINVAL"), ("capacity", 0, "EINVAL"), ("capacity", 2 ** 30 + 1, "EUNSUPPORTED"),
     ("counts", None, "EINVAL"), ("dim", 0, "EINVAL"), ("dim", 60, "EUNSUPPORTED"),
     ("dim", 264, "EUNSUPPORTED"), ("dim", 136, "EUNSUPPORTED"), ("workspace", None, "EWORKSPACE"),
     ("workspace", FAKE + 4, "EWORKSPACE"), ("workspace_bytes", 16, "EWORKSPACE"),

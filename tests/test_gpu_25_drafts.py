@@ -355,6 +355,12 @@ VERIFY_CASES = [
     (9, 2, 4, 50257, "f32", "tree", True, "ones"),
     (10, 2, 5, 24577, "bf16", "tree", False, "greedy"),
     (11, 3, 8, 4099, "f16", "holes", True, "greedy"),
+    (12, 4, 8, 1024, "bf16", "tree", True, "mixed"),  # the most that one launch takes, and one more
+    (13, 4, 8, 1025, "f16", "tree", False, "ones"),
+    (14, 3, 8, 512, "f32", "holes", True, "mixed"),
+    (15, 3, 9, 512, "f32", "tree", False, "mixed"),
+    (16, 2, 24, 40001, "bf16", "tree", True, "ones"),
+    (17, 3, 7, 9001, "f16", "forest", True, "mixed"),
 ]
 
 
