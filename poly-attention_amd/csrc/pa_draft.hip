@@ -596,7 +596,7 @@ bool draft_dim(int d) { return d >= 8 && d <= 256 && d % 8 == 0 && (d <= 128 || 
 // but kDraftFew where a unit's keys are below kDraftUnitBytes per 16 rows, since a workgroup's start
 // and end and its record cost the more the more rows it has.  Behind cold caches: 32 x 8192 positions of
 // 128, 32 rows: 272 us with few, 249 with many; order 3, 8 x 2048 of 64, 16 rows: 41 with few, 45 with many.
-// k_draft_wide: 8 x 4096 of 128 in one round 69, in two 79 (64 rows), 84 and 90 (128 rows).
+// k_draft_wide, 8 x 4096 of 128: as many as are in flight 69, twice as many 79 (64 rows); 84 and 90 (128 rows).
 constexpr int64_t kDraftMany = 4, kDraftFew = 2, kDraftWideMany = 2, kDraftUnitBytes = 64 * 1024, kDraftCus = 256;
 
 // geometry shared by the workspace query and the launch; false where the request is malformed
@@ -630,7 +630,7 @@ bool draft_plan(const pa_draft* d, DraftDev& P, int& units, int& tiles) {
     const int64_t flight = kDraftCus * (wide ? 2 : draft_waves(D, tiles, d->order > 2));
     const int64_t target = std::min(std::max<int64_t>(1, (wide ? kDraftWideMany : kDraftMany) * flight / per), chunks);
     P.target = (int)target;
-    // in one round of workgroups, with half a unit per row that the rows' ends add
+    // as many as are in flight, with half a unit per row that the ends of rows add
     const int64_t few = wide ? flight / per - d->batch / 2 : kDraftFew * flight / per;
     P.target_min = (int)std::min(std::max<int64_t>(1, few), chunks);
     P.least = std::max(1, (int)(kDraftUnitBytes * tiles / ((int64_t)kDraftChunk * d->dim * (f32 ? 4 : 2))));
