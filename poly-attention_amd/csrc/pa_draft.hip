@@ -538,17 +538,30 @@ __device__ __forceinline__ void move_rows(const char* src, char* dst, int64_t sh
 
 // One workgroup per (row, move): 8 rows of 54 buffers 4.9 us, one of 5 3.9 (paths, rows, counts: three dependent
 // trips to memory).  With advance the workgroup of a row that draws the last ticket counts the
-// kept nodes: by then every other one has read the count, so one launch does both.
+// kept nodes: by then every other one has read the count, so one launch does both.  The first wave reads it
+// for the workgroup: a barrier does not wait for another wave's loads from memory, so a wave that read the
+// count for itself might read the advanced one.
 __global__ __launch_bounds__(kDraftThreads) void k_draft_commit(const DraftCommitDev P) {
+    __shared__ int s_slot[64], s_n, s_len, s_over;
     const int tid = threadIdx.x, b = blockIdx.x;
-    int n, slot;
-    bool over;
-    const int len = commit_length(P, b, tid & 63, n, slot, over);
+    if (tid < 64) {
+        int at, p;
+        bool past;
+        const int moved = commit_length(P, b, tid, at, p, past);
+        s_slot[tid] = p;
+        if (tid == 0) {
+            s_n = at;
+            s_len = moved;
+            s_over = past;
+        }
+    }
+    __syncthreads();  // past it the count has been read: the length in LDS depends on it
+    const int n = s_n, len = s_len, slot = s_slot[tid & 63];
+    const bool over = s_over;
     const pa_draft_move& M = P.mv[blockIdx.y];
-    __syncthreads();  // every wave has read the count
-    int done = 0;     // drawn now, looked at after the moves
-    // relaxed: nothing that another workgroup wrote is read after it, and this one's reads of the count have
-    // returned (the length depends on them); a release would write the L2 back, at several us
+    int done = 0;  // drawn now, looked at after the moves
+    // relaxed: nothing that another workgroup wrote is read after it, and this one's read of the count has
+    // returned; a release would write the L2 back, at several us
     if (P.advance && tid == 0)
         done = __hip_atomic_fetch_add(P.tickets + b * kTicketStride, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (P.count > 0 && len > 0) {
