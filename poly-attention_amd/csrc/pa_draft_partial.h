@@ -18,6 +18,8 @@
 // memory's rate.  32 x 8192 positions of 128, 32 rows: 240 us, 5.6 TB/s.
 #pragma once
 
+#include <type_traits>
+
 #include "pa_draft.h"
 
 namespace pa {
@@ -51,6 +53,26 @@ __device__ __forceinline__ uint32_t draft_pack2(float lo, float hi) {
     typedef T t2 __attribute__((ext_vector_type(2)));
     const f2 v = {lo, hi};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, t2));
+}
+// The probabilities of cached positions as two numbers of the type each, the leading bits (cut off, not rounded) and
+// what those leave: 16 bits of a bf16 weight and 22 of an fp16 one, against 8 and 11.  One of them alone was the
+// largest error of a 16-bit step (bf16 0.0021 to 0.0025 relative to the output against 0.0017, the rounding of the
+// output).  The lowest bit set keeps the rest above 0: an infinite value then gives inf, not inf * 0.
+template <typename T>
+__device__ __forceinline__ void draft_split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const uint32_t ia = __float_as_uint(a), ib = __float_as_uint(b);
+    float ha, hb;
+    if constexpr (std::is_same_v<T, bf16>) {
+        hi = __builtin_amdgcn_perm(ib, ia, 0x07060302u);
+        ha = __uint_as_float(ia & 0xffff0000u);
+        hb = __uint_as_float(ib & 0xffff0000u);
+    } else {
+        const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+        hi = __builtin_bit_cast(uint32_t, h);
+        ha = (float)h[0];
+        hb = (float)h[1];
+    }
+    lo = draft_pack2<T>(__uint_as_float(ia | 1u) - ha, __uint_as_float(ib | 1u) - hb);
 }
 // two 16-bit products: word e of hi the rounded ones, of lo what the rounding left
 template <typename T>
@@ -377,7 +399,9 @@ __global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft
         if constexpr (!KLDS) load_k(j0 + STEP);
         load_bias(j0 + STEP);
         __builtin_amdgcn_sched_barrier(0);
-        uint32_t pf[RT][4];
+        // probabilities (16-bit types: their leading bits, and the rest); 0 for a tile without rows, whose test would
+        // else keep the scores alive beside them (52 spilled registers with four tiles)
+        uint32_t pf[RT][4] = {}, pl[RT][4] = {};
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             if (rt >= nrt) break;
@@ -408,11 +432,10 @@ __global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft
 #pragma unroll
                 for (int i = 0; i < 4; ++i) pf[rt][i] = __float_as_uint(x[rt][0][i]);
             } else {
-                // rounded to the value type for the product: half a step of a term, averaged over the row
 #pragma unroll
                 for (int t = 0; t < KT; ++t) {
-                    pf[rt][2 * t] = draft_pack2<T>(x[rt][t][0], x[rt][t][1]);
-                    pf[rt][2 * t + 1] = draft_pack2<T>(x[rt][t][2], x[rt][t][3]);
+                    draft_split2<T>(x[rt][t][0], x[rt][t][1], pf[rt][2 * t], pl[rt][2 * t]);
+                    draft_split2<T>(x[rt][t][2], x[rt][t][3], pf[rt][2 * t + 1], pl[rt][2 * t + 1]);
                 }
             }
         }
@@ -449,9 +472,11 @@ __global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft
                 for (int rt = 0; rt < RT; ++rt) {
                     if (rt >= nrt) break;
                     const u32x4_d p = {pf[rt][0], pf[rt][1], pf[rt][2], pf[rt][3]};
+                    const u32x4_d p2 = {pl[rt][0], pl[rt][1], pl[rt][2], pl[rt][3]};
                     o[rt][j] = Mma16<T>::run(a, p, o[rt][j]);
                     if constexpr (VM)
                         if (has_m) o[rt][j] = Mma16<T>::run(a2, p, o[rt][j]);
+                    o[rt][j] = Mma16<T>::run(a, p2, o[rt][j]);
                 }
             }
         }

@@ -243,7 +243,7 @@ __global__ __launch_bounds__(64 * kDraftWideWaves, 2) void k_draft_wide(const Dr
                             for (int rt = 0; rt < NR; ++rt)
                                 if (j0 + 16 * t + 4 * g + i >= cnt) x[rt][t][i] = -INFINITY;
                 }
-                u32x4_d pf[NR + 1];
+                u32x4_d pf[NR + 1], pl[NR + 1];  // leading bits and the rest
 #pragma unroll
                 for (int rt = 0; rt < NR; ++rt) {
                     float top = x[rt][0][0];
@@ -269,12 +269,15 @@ __global__ __launch_bounds__(64 * kDraftWideWaves, 2) void k_draft_wide(const Dr
                             x[rt][t][i] = __builtin_amdgcn_exp2f(x[rt][t][i] - ms);
                             l[rt] += x[rt][t][i];
                         }
-                    // rounded to the value type for the product: half a step of a term, averaged over the row
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        pf[rt][2 * t] = draft_pack2<T>(x[rt][t][0], x[rt][t][1]);
-                        pf[rt][2 * t + 1] = draft_pack2<T>(x[rt][t][2], x[rt][t][3]);
-                    }
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            uint32_t hi, lo;
+                            draft_split2<T>(x[rt][t][2 * i], x[rt][t][2 * i + 1], hi, lo);
+                            pf[rt][2 * t + i] = hi;
+                            pl[rt][2 * t + i] = lo;
+                        }
                 }
                 // O^T += V^T P^T, features 16 j + c; lane L of a group of 16 reads position L / 4, columns 4 (L % 4)
                 const int vrow = 4 * g + (c >> 2), vch = (c >> 1) & 1, vlow = (c & 1) * 8;
@@ -303,6 +306,7 @@ __global__ __launch_bounds__(64 * kDraftWideWaves, 2) void k_draft_wide(const Dr
                         o[rt][j] = Mma16<T>::run(a, pf[rt], o[rt][j]);
                         if constexpr (VM)
                             if (has_m) o[rt][j] = Mma16<T>::run(a2, pf[rt], o[rt][j]);
+                        o[rt][j] = Mma16<T>::run(a, pl[rt], o[rt][j]);
                     }
                 }
             }

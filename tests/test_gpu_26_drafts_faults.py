@@ -3,7 +3,8 @@
 import pytest
 import torch
 
-from test_gpu_25_drafts import BUFS, dev, random_caches
+import drafts_oracle as DO
+from test_gpu_25_drafts import BUFS, DT, assert_within, dev, fill_cache, make_tree, random_caches
 
 pytestmark = pytest.mark.gpu
 param = pytest.mark.parametrize
@@ -33,3 +34,70 @@ def test_commit_many_buffers_at_one_count():
         assert caches[0].lengths() == counts
         for w, (dst, _) in zip(want, bufs):
             assert torch.equal(dst, w), step
+
+
+# A weight of a cached position, and a middle level's v * msg, enter the products as two numbers of the type,
+# the second of what the first leaves: bf16 is off by at most 2^-16 of the value (8 bits cut off, the rest below 2^-7
+# rounded to 8), fp16 by 2^-21 (11, 2^-10 and 11) and, below 2^-14, by 2^-25.  The oracle's bound takes one rounding to
+# the type for each (2^-9, 2^-12); in its place, of a weight's value:
+def pair(dtype, order):
+    return 2.0 ** -15 if dtype == "bf16" or order > 2 else 2.0 ** -18
+
+
+def attend_pairs(u, q1, host, lens, trees, scale, softclamp=None):
+    """The oracle's results, with bounds that one rounding of a weight or of a product does not fit."""
+    unit = DO.unit
+    try:
+        DO.unit = lambda dtype: u
+        want, tol = DO.attend(q1, host, lens, trees, scale, softclamp)
+    finally:
+        DO.unit = unit
+    sums = len(want) - len(host["lses"])  # the logsumexps are stored in fp32
+    return want, [e + DO.stored(w, q1.dtype) if k < sums else e for k, (w, e) in enumerate(zip(want, tol))]
+
+
+@param("dtype", ("bf16", "f16"))
+@param("order,B,counts,T,H,hk,D,kind", [
+    (2, 1, [700], 1, 2, 2, 64, "chain"),
+    (2, 2, [300, 41], 5, 8, 2, 128, "tree"),      # 20 rows
+    (3, 1, [500], 7, 4, 2, 64, "tree"),
+    (4, 2, [129, 350], 3, 2, 1, 40, "forest"),
+    (3, 1, [300], 40, 2, 2, 64, "tree"),          # four tiles of a middle level
+    (3, 1, [257], 20, 2, 1, 256, "tree"),
+    (2, 1, [400], 33, 4, 2, 64, "tree"),          # the blocks of many rows
+    (3, 1, [310], 48, 3, 1, 128, "holes"),
+])
+def test_attend_holds_more_than_one_rounding(dtype, order, B, counts, T, H, hk, D, kind):
+    """The outputs are those of fp32 weights and products, rounded once: with weights rounded to the type the
+    error was 1.2 to 1.5 times that of the output's rounding alone."""
+    from poly_attention import DraftCache
+
+    d = dev()
+    g = torch.Generator().manual_seed(order * 100 + T)
+    cache = DraftCache.empty(order=order, batch=B, kv_heads=hk, dim_head=D, capacity=max(counts), max_drafts=T,
+                             dtype=DT[dtype], device=d, counts=torch.tensor(counts, dtype=torch.int32, device=d))
+    host = fill_cache(cache, g, d)
+    trees = [make_tree(T, g, kind) for _ in range(B)]
+    q1 = torch.randn(B, H, T, D, generator=g).to(DT[dtype])
+    out = cache.attend(q1.to(d), parents=torch.tensor(trees, device=d))
+    want, tol = attend_pairs(pair(dtype, order), q1, host, counts, trees, D ** -0.5)
+    for k, (x, w, e) in enumerate(zip((out, *cache.draft_msgs, *cache.draft_lses), want, tol)):
+        assert_within(x, w, e, f"output {k}")
+
+
+@param("dtype", ("bf16", "f16"))
+@param("T,H,D", [(1, 16, 64), (5, 8, 128), (1, 48, 128)])
+def test_attend_weights_of_few_positions(dtype, T, H, D):
+    """Queries of 0: the weights are those of the logsumexps alone, and the scores' own error hides nothing."""
+    from poly_attention import DraftCache
+
+    d = dev()
+    g = torch.Generator().manual_seed(T)
+    cache = DraftCache.empty(order=2, batch=4, kv_heads=1, dim_head=D, capacity=6, max_drafts=T, dtype=DT[dtype],
+                             device=d, counts=torch.tensor([2, 3, 5, 6], dtype=torch.int32, device=d))
+    host = fill_cache(cache, g, d)
+    q1 = torch.zeros(4, H, T, D, dtype=DT[dtype])
+    chain = [list(range(-1, T - 1))] * 4
+    out = cache.attend(q1.to(d))
+    want, tol = attend_pairs(pair(dtype, 2), q1, host, [2, 3, 5, 6], chain, D ** -0.5)
+    assert_within(out, want[0], tol[0], "out")
