@@ -14,6 +14,8 @@
 // columns of the head and repeats the (few) weights, so no workgroup waits for another.
 #pragma once
 
+#include <type_traits>
+
 #include "pa_common.h"
 #include "pa_launch.h"
 
@@ -24,7 +26,12 @@ constexpr int kDraftChunk = 128;  // a unit covers a multiple of this many posit
 // tickets of different rows lie on cache lines of their own: atomics on one line follow one another (432 of
 // them on one line took 4 us)
 constexpr int kTicketStride = PA_TICKET_STRIDE;
-constexpr float kDraftTau = 8.f;  // lazy-rescale headroom of the running maximum (log2 units)
+// A row's weights are exp2(score - m), log2 units, with m its running maximum or less: m is raised where a score passes
+// it by more than draft_tau, to draft_lift below that score.  fp16's smallest number is 2^-24: against a largest
+// weight of 1 those below 2^-25 vanish, of which a long cache holds as many as to matter (20000 of 2^-25.5 beside
+// one of 1: 0.04%, times their values).  Against a largest weight of 2^7 to 2^15 those below 2^-32 do.
+template <typename T> __device__ constexpr float draft_lift() { return std::is_same_v<T, f16> ? 7.f : 0.f; }
+template <typename T> __device__ constexpr float draft_tau() { return std::is_same_v<T, f16> ? 15.f : 8.f; }
 
 struct DraftRow {  // a [B, h, n, dim] array: base and element strides
     char* p;

@@ -12,7 +12,8 @@
 // whole row, and the transposition that the operand needs is inside the lane (one v_perm_b32 for
 // two values).  fp32 takes v_mfma_f32_16x16x4_f32, whose operands are single values: no
 // transposition at all.  In O^T a lane holds one row, so the running maximum's rescale is one
-// factor per lane; it moves only past kDraftTau (lazy), so exp2(s - m) is at most 2^8.
+// factor per lane; it moves only past draft_tau (lazy), so exp2(s - m) is at most 2^8
+// (fp16 2^15).
 //
 // Bound by memory while the rows are few: 16 rows of a step cost about a tenth of its 16 KB at the
 // memory's rate.  32 x 8192 positions of 128, 32 rows: 240 us, 5.6 TB/s.
@@ -410,10 +411,10 @@ __global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft
             for (int t = 0; t < KT; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, x[rt][t][i]);
-            if (__any(top > m[rt] + kDraftTau)) {
+            if (__any(top > m[rt] + draft_tau<T>())) {
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
-                const float mn = fmaxf(m[rt], top);
+                const float mn = fmaxf(m[rt], top - draft_lift<T>());
                 const float al = mn == m[rt] ? 1.f : __builtin_amdgcn_exp2f(m[rt] - mn);
                 m[rt] = mn;
                 l[rt] *= al;

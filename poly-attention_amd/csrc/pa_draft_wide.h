@@ -251,10 +251,10 @@ __global__ __launch_bounds__(64 * kDraftWideWaves, 2) void k_draft_wide(const Dr
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) top = fmaxf(top, x[rt][t][i]);
-                    if (__any(top > m[rt] + kDraftTau)) {
+                    if (__any(top > m[rt] + draft_tau<T>())) {
                         top = fmaxf(top, __shfl_xor(top, 16));
                         top = fmaxf(top, __shfl_xor(top, 32));
-                        const float mn = fmaxf(m[rt], top);
+                        const float mn = fmaxf(m[rt], top - draft_lift<T>());
                         const float al = mn == m[rt] ? 1.f : __builtin_amdgcn_exp2f(m[rt] - mn);
                         m[rt] = mn;
                         l[rt] *= al;

@@ -38,7 +38,7 @@ def test_commit_many_buffers_at_one_count():
 
 # A weight of a cached position, and a middle level's v * msg, enter the products as two numbers of the type,
 # the second of what the first leaves: bf16 is off by at most 2^-16 of the value (8 bits cut off, the rest below 2^-7
-# rounded to 8), fp16 by 2^-21 (11, 2^-10 and 11) and, below 2^-14, by 2^-25.  The oracle's bound takes one rounding to
+# rounded to 8), fp16 by 2^-21 (11, 2^-10 and 11) where it is not among the smallest numbers.  The oracle's bound takes one rounding to
 # the type for each (2^-9, 2^-12); in its place, of a weight's value:
 def pair(dtype, order):
     return 2.0 ** -15 if dtype == "bf16" or order > 2 else 2.0 ** -18
@@ -101,3 +101,32 @@ def test_attend_weights_of_few_positions(dtype, T, H, D):
     out = cache.attend(q1.to(d))
     want, tol = attend_pairs(pair(dtype, 2), q1, host, [2, 3, 5, 6], chain, D ** -0.5)
     assert_within(out, want[0], tol[0], "out")
+
+
+@param("dtype", ("bf16", "f16", "f32"))
+@param("T", (1, 20, 40))
+def test_attend_small_weights_beside_a_large_one(dtype, T):
+    """One position takes nearly all of the weight and has a value of 0: what is left are 4000 weights of 2^-25.6,
+    below fp16's smallest number where the largest is 1.  So many key heads that one workgroup holds a row."""
+    from poly_attention import DraftCache
+
+    d = dev()
+    g = torch.Generator().manual_seed(T)
+    hk, n, D = 600, 4000, 8
+    cache = DraftCache.empty(order=2, batch=1, kv_heads=hk, dim_head=D, capacity=n, max_drafts=T, dtype=DT[dtype],
+                             device=d, counts=torch.tensor([n], dtype=torch.int32, device=d))
+    host = fill_cache(cache, g, d)
+    host["lses"][0].zero_()
+    host["lses"][0][:, :, 100] = 25.6 * 0.6931471805599453
+    host["msgs"][0].add_(1.0)
+    host["msgs"][0][:, :, 100] = 0.0
+    cache.lses[0].copy_(host["lses"][0])
+    cache.msgs[0].copy_(host["msgs"][0])
+    q1 = torch.zeros(1, hk, T, D, dtype=DT[dtype])
+    out = cache.attend(q1.to(d))
+    two = {k: [t[:, :2] for t in ts] for k, ts in host.items()}
+    want, tol = attend_pairs(pair(dtype, 2), q1[:, :2], two, [n], [list(range(-1, T - 1))], D ** -0.5)
+    # below 2^-14 fp16's steps stop shrinking: a weight is off by up to 2^-25, where the largest is at least 2^7
+    floor = 2.0 ** -32 if dtype == "f16" else 0.0
+    tol[0] += floor * host["msgs"][0][:, :2].double().abs().sum(2)[:, :, None]
+    assert_within(out[:, :2], want[0], tol[0], "out")
