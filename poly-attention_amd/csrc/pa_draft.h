@@ -54,6 +54,7 @@ struct DraftCommon {
     int64_t parents_stride;
     float* ws_o;   // [unit][kv head][rec_rows][dim]
     float2* ws_s;  // [unit][kv head][rec_rows]: running maximum (log2 units) and sum
+    int64_t none;  // the record behind those of the units: maximum -inf, sum and values 0
     float* ws_t;   // [row][kv head][rec_rows][t16]: scores of the tree without biases (log2 units), -inf
                    // where a node does not see another
     int4* ws_u;    // [row]: the row's first unit, its units, and which of its nodes are there (64 bits)
@@ -170,6 +171,13 @@ __device__ __forceinline__ uint64_t draft_ancestors(const int32_t* parents, int 
         up = u2;
     }
     return dead ? 0ull : ((uint64_t)hi << 32) | lo;
+}
+
+// The record of no unit, by one wave: the join reads it where it has fewer units than loads.  A unit's record in its
+// place would do for finite values, but 0 times an infinite one is no 0.
+__device__ __forceinline__ void draft_none(const DraftCommon& P, int lane) {
+    for (int d = lane; d < P.dim; d += 64) P.ws_o[P.none * P.dim + d] = 0.f;
+    if (lane == 0) P.ws_s[P.none] = make_float2(-INFINITY, 0.f);
 }
 
 template <typename T> void launch_draft_partial(const DraftDev& P, int units, int tiles, bool vmul, hipStream_t s);

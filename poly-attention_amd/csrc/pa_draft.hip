@@ -136,10 +136,9 @@ __global__ __launch_bounds__(kDraftThreads) void k_draft_combine(const DraftJoin
                     float4 y[kDraftBatch];
 #pragma unroll
                     for (int k = 0; k < kDraftBatch; ++k) {
-                        const int64_t at = rec + (int64_t)min(u + (k << lgp), units.y - 1) * urec;
+                        const int64_t at = u + (k << lgp) < units.y ? rec + (int64_t)(u + (k << lgp)) * urec : P.none;
                         ms[k] = P.ws_s[at];
                         y[k] = *reinterpret_cast<const float4*>(from + at * P.dim);
-                        if (u + (k << lgp) >= units.y) ms[k].x = -INFINITY;
                     }
                     float top = a.top;
 #pragma unroll
@@ -654,7 +653,8 @@ bool draft_plan(const pa_draft* d, DraftDev& P, int& units, int& tiles) {
 // the workspace's arrays, and its size
 size_t draft_ws(DraftCommon& P, int units, void* base) {
     auto whole = [](size_t n) { return (n + 255) & ~size_t(255); };
-    const size_t rec = (size_t)units * P.kv_heads * P.rec_rows;
+    P.none = (int64_t)units * P.kv_heads * P.rec_rows;
+    const size_t rec = (size_t)P.none + 1;
     char* at = static_cast<char*>(base);
     P.ws_o = reinterpret_cast<float*>(at);
     size_t n = whole(rec * P.dim * 4);

@@ -58,34 +58,60 @@ __device__ __forceinline__ uint32_t draft_pack2(float lo, float hi) {
 // The probabilities of cached positions as two numbers of the type each, the leading bits (cut off, not rounded) and
 // what those leave: 16 bits of a bf16 weight and 22 of an fp16 one, against 8 and 11.  One of them alone was the
 // largest error of a 16-bit step (bf16 0.0021 to 0.0025 relative to the output against 0.0017, the rounding of the
-// output).  The lowest bit set keeps the rest above 0: an infinite value then gives inf, not inf * 0.
+// output).  The leading bits are those of a number 2^-12 smaller, so that the rest is above 0: an infinite value then
+// gives inf, not inf * 0.
 template <typename T>
 __device__ __forceinline__ void draft_split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const uint32_t ia = __float_as_uint(a), ib = __float_as_uint(b);
-    float ha, hb;
+    constexpr float kLess = 1.f - 1.f / 4096.f;
+    float ha = a * kLess, hb = b * kLess;
     if constexpr (std::is_same_v<T, bf16>) {
+        const uint32_t ia = __float_as_uint(ha), ib = __float_as_uint(hb);
         hi = __builtin_amdgcn_perm(ib, ia, 0x07060302u);
         ha = __uint_as_float(ia & 0xffff0000u);
         hb = __uint_as_float(ib & 0xffff0000u);
     } else {
-        const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+        const auto h = __builtin_amdgcn_cvt_pkrtz(ha, hb);
         hi = __builtin_bit_cast(uint32_t, h);
         ha = (float)h[0];
         hb = (float)h[1];
     }
-    lo = draft_pack2<T>(__uint_as_float(ia | 1u) - ha, __uint_as_float(ib | 1u) - hb);
+    lo = draft_pack2<T>(a - ha, b - hb);
 }
-// two 16-bit products: word e of hi the rounded ones, of lo what the rounding left
+// A middle level's values v * msg, two at a time, as two bf16 numbers each whatever the type: word e of hi their
+// leading bits, of lo what those leave (16 bits together).  bf16 has fp32's range, where a product of two fp16
+// numbers passes fp16's at both ends.  An infinite product leaves its infinity to lo, beside the largest number
+// in hi: the rest of an infinity would be inf - inf.
 template <typename T>
 __device__ __forceinline__ void draft_mul2(uint32_t a, uint32_t b, u32x4_d& hi, u32x4_d& lo, int e) {
     typedef float f2 __attribute__((ext_vector_type(2)));
     typedef T t2 __attribute__((ext_vector_type(2)));
+    constexpr float kMost = 0x1.fep127f;  // the largest bf16
     const f2 x = __builtin_convertvector(__builtin_bit_cast(t2, a), f2);
     const f2 y = __builtin_convertvector(__builtin_bit_cast(t2, b), f2);
-    const uint32_t h = draft_pack2<T>(x[0] * y[0], x[1] * y[1]);
-    const f2 r = __builtin_convertvector(__builtin_bit_cast(t2, h), f2);
-    hi[e] = h;
-    lo[e] = draft_pack2<T>(fmaf(x[0], y[0], -r[0]), fmaf(x[1], y[1], -r[1]));
+    const uint32_t i0 = __float_as_uint(__builtin_amdgcn_fmed3f(x[0] * y[0], -kMost, kMost)),
+                   i1 = __float_as_uint(__builtin_amdgcn_fmed3f(x[1] * y[1], -kMost, kMost));
+    hi[e] = __builtin_amdgcn_perm(i1, i0, 0x07060302u);
+    lo[e] = draft_pack2<bf16>(fmaf(x[0], y[0], -__uint_as_float(i0 & 0xffff0000u)),
+                              fmaf(x[1], y[1], -__uint_as_float(i1 & 0xffff0000u)));
+}
+
+// the weights p + p2 times the values a, of a middle level (middle) a + a2
+template <typename T, bool VM>
+__device__ __forceinline__ f32x4_t draft_weigh(u32x4_d a, u32x4_d a2, u32x4_d p, u32x4_d p2, f32x4_t o, bool middle) {
+    if constexpr (VM)
+        if (middle) {
+            o = Mma16<bf16>::run(a, p, o);
+            o = Mma16<bf16>::run(a2, p, o);
+            return Mma16<bf16>::run(a, p2, o);
+        }
+    o = Mma16<T>::run(a, p, o);
+    return Mma16<T>::run(a, p2, o);
+}
+// as draft_split2, the numbers of the type, of a middle level bf16
+template <typename T, bool VM>
+__device__ __forceinline__ void draft_weights2(float a, float b, uint32_t& hi, uint32_t& lo, bool middle) {
+    if (VM && middle) draft_split2<bf16>(a, b, hi, lo);
+    else draft_split2<T>(a, b, hi, lo);
 }
 
 __device__ __forceinline__ u32x4_d load16u(const void* p) { return *reinterpret_cast<const u32x4_d*>(p); }
@@ -277,6 +303,7 @@ __global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft
     const float unclamped = P.softclamp > 0.f ? P.scale / P.softclamp : sl2;
 
     if (tree) {  // 16 drafted keys per wave
+        if (blockIdx.x + blockIdx.y + blockIdx.z == 0 && wave == 3) draft_none(P, lane);
         if (16 * wave >= P.T) return;
         const uint64_t anc = draft_ancestors(P.parents ? P.parents + b * P.parents_stride : nullptr, P.T, lane);
         const uint32_t anc_lo = (uint32_t)anc, anc_hi = (uint32_t)(anc >> 32);
@@ -435,8 +462,8 @@ __global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft
             } else {
 #pragma unroll
                 for (int t = 0; t < KT; ++t) {
-                    draft_split2<T>(x[rt][t][0], x[rt][t][1], pf[rt][2 * t], pl[rt][2 * t]);
-                    draft_split2<T>(x[rt][t][2], x[rt][t][3], pf[rt][2 * t + 1], pl[rt][2 * t + 1]);
+                    draft_weights2<T, VM>(x[rt][t][0], x[rt][t][1], pf[rt][2 * t], pl[rt][2 * t], has_m);
+                    draft_weights2<T, VM>(x[rt][t][2], x[rt][t][3], pf[rt][2 * t + 1], pl[rt][2 * t + 1], has_m);
                 }
             }
         }
@@ -461,8 +488,7 @@ __global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft
                     a[e] = __builtin_amdgcn_perm(v[2 * e + 1][j / 2], v[2 * e][j / 2], sel);
                 if constexpr (VM)
                     if (has_m) {
-                        // v * m as two values of the type, the rounded product and what it leaves: one
-                        // rounding of the product was most of a middle level's error
+                        // one rounding of the product was most of a middle level's error
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const uint32_t y = __builtin_amdgcn_perm(mv[2 * e + 1][j / 2], mv[2 * e][j / 2], sel);
@@ -474,10 +500,7 @@ __global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft
                     if (rt >= nrt) break;
                     const u32x4_d p = {pf[rt][0], pf[rt][1], pf[rt][2], pf[rt][3]};
                     const u32x4_d p2 = {pl[rt][0], pl[rt][1], pl[rt][2], pl[rt][3]};
-                    o[rt][j] = Mma16<T>::run(a, p, o[rt][j]);
-                    if constexpr (VM)
-                        if (has_m) o[rt][j] = Mma16<T>::run(a2, p, o[rt][j]);
-                    o[rt][j] = Mma16<T>::run(a, p2, o[rt][j]);
+                    o[rt][j] = draft_weigh<T, VM>(a, a2, p, p2, o[rt][j], has_m);
                 }
             }
         }

@@ -94,6 +94,7 @@ __global__ __launch_bounds__(64 * kDraftWideWaves, 2) void k_draft_wide(const Dr
     const float unclamped = P.softclamp > 0.f ? P.scale / P.softclamp : sl2;
 
     if (tree) {  // a wave's rows against all drafted keys
+        if (blockIdx.x + blockIdx.y + blockIdx.z == 0 && wave == 3) draft_none(P, lane);
         const uint64_t anc = draft_ancestors(P.parents ? P.parents + b * P.parents_stride : nullptr, P.T, lane);
         const uint32_t anc_lo = (uint32_t)anc, anc_hi = (uint32_t)(anc >> 32);
         if (blockIdx.y == 0 && blockIdx.z == 0 && wave == 0) {  // for the join
@@ -173,8 +174,10 @@ __global__ __launch_bounds__(64 * kDraftWideWaves, 2) void k_draft_wide(const Dr
     for (int st = 0; st < NS - 1; ++st) load(st);
 
     // NR: the wave's tiles, a compile-time number (a test per tile keeps the reads of LDS from running ahead)
-    auto run = [&](auto tiles) __attribute__((always_inline)) {
+    // and whether the level is a middle one, for the same reason
+    auto run = [&](auto tiles, auto middle) __attribute__((always_inline)) {
         constexpr int NR = decltype(tiles)::value;
+        constexpr bool MID = decltype(middle)::value;
         f32x4_t o[NR + 1][VE];
         float m[NR + 1], l[NR + 1];
 #pragma unroll
@@ -274,7 +277,7 @@ __global__ __launch_bounds__(64 * kDraftWideWaves, 2) void k_draft_wide(const Dr
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             uint32_t hi, lo;
-                            draft_split2<T>(x[rt][t][2 * i], x[rt][t][2 * i + 1], hi, lo);
+                            draft_weights2<T, MID>(x[rt][t][2 * i], x[rt][t][2 * i + 1], hi, lo, MID);
                             pf[rt][2 * t + i] = hi;
                             pl[rt][2 * t + i] = lo;
                         }
@@ -294,20 +297,13 @@ __global__ __launch_bounds__(64 * kDraftWideWaves, 2) void k_draft_wide(const Dr
 #pragma unroll
                 for (int j = 0; j < VE; ++j) {
                     u32x4_d a = turned(tv, j), a2 = {0u, 0u, 0u, 0u};
-                    if constexpr (VM)
-                        if (has_m) {
-                            // v * m as two values of the type, the rounded product and what it leaves
-                            const u32x4_d y = turned(tm, j), x1 = a;
+                    if constexpr (MID) {
+                        const u32x4_d y = turned(tm, j), x1 = a;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) draft_mul2<T>(x1[e], y[e], a, a2, e);
-                        }
-#pragma unroll
-                    for (int rt = 0; rt < NR; ++rt) {
-                        o[rt][j] = Mma16<T>::run(a, pf[rt], o[rt][j]);
-                        if constexpr (VM)
-                            if (has_m) o[rt][j] = Mma16<T>::run(a2, pf[rt], o[rt][j]);
-                        o[rt][j] = Mma16<T>::run(a, pl[rt], o[rt][j]);
+                        for (int e = 0; e < 4; ++e) draft_mul2<T>(x1[e], y[e], a, a2, e);
                     }
+#pragma unroll
+                    for (int rt = 0; rt < NR; ++rt) o[rt][j] = draft_weigh<T, MID>(a, a2, pf[rt], pl[rt], o[rt][j], MID);
                 }
             }
         }
@@ -326,10 +322,16 @@ __global__ __launch_bounds__(64 * kDraftWideWaves, 2) void k_draft_wide(const Dr
                 if (16 * j + 4 * g < P.dim) *reinterpret_cast<f32x4_t*>(P.ws_o + (rec + r) * P.dim + 16 * j + 4 * g) = o[rt][j];
         }
     };
-    if (nrt == 0) run(std::integral_constant<int, 0>{});
-    else if (nrt == 1) run(std::integral_constant<int, 1>{});
-    else if (RT == 2 || nrt == 2) run(std::integral_constant<int, 2>{});
-    else run(std::integral_constant<int, RT>{});
+    auto level = [&](auto middle) __attribute__((always_inline)) {
+        if (nrt == 0) run(std::integral_constant<int, 0>{}, middle);
+        else if (nrt == 1) run(std::integral_constant<int, 1>{}, middle);
+        else if (RT == 2 || nrt == 2) run(std::integral_constant<int, 2>{}, middle);
+        else run(std::integral_constant<int, RT>{}, middle);
+    };
+    if constexpr (VM) {
+        if (has_m) return level(std::true_type{});
+    }
+    level(std::false_type{});
 }
 
 template <typename T, int D>

@@ -130,3 +130,70 @@ def test_attend_small_weights_beside_a_large_one(dtype, T):
     floor = 2.0 ** -32 if dtype == "f16" else 0.0
     tol[0] += floor * host["msgs"][0][:, :2].double().abs().sum(2)[:, :, None]
     assert_within(out[:, :2], want[0], tol[0], "out")
+def middle_case(dtype, T, H, D, g, d):
+    """An order-3 cache of 64 positions a row, and one query tensor."""
+    from poly_attention import DraftCache
+
+    cache = DraftCache.empty(order=3, batch=2, kv_heads=1, dim_head=D, capacity=64, max_drafts=T, dtype=DT[dtype],
+                             device=d, counts=torch.tensor([64, 50], dtype=torch.int32, device=d))
+    host = fill_cache(cache, g, d)
+    return cache, host, torch.randn(2, H, T, D, generator=g).to(DT[dtype])
+
+
+MIDDLE = [(1, 2, 64), (9, 2, 128), (3, 1, 144), (13, 3, 64), (20, 4, 64), (12, 4, 128)]
+
+
+@param("T,H,D", MIDDLE)
+def test_attend_middle_products_beyond_fp16(T, H, D):
+    """v * msg of a middle level passes fp16's largest and smallest numbers at some positions, their weighted mean
+    mostly does not: the product is not rounded to the type.  One such position has weight 0."""
+    d = dev()
+    g = torch.Generator().manual_seed(T + D)
+    cache, host, q1 = middle_case("f16", T, H, D, g, d)
+    # chain level 1 scores q2 . q3 over v = vs[0], multiplied by the deepest level's outputs
+    for at, v, m in ((7, 300.0, 1500.0), (11, -60000.0, 60.0), (40, 2.0 ** -14, 2.0 ** -10)):
+        host["vs"][0][:, :, at, 3:6] = v
+        host["msgs"][0][:, :, at, 3:6] = m
+    host["lses"][0][:, :, 11] = -torch.finfo(torch.float32).max
+    for name in ("vs", "msgs", "lses"):
+        getattr(cache, name)[0].copy_(host[name][0])
+    out = cache.attend(q1.to(d))
+    host["lses"][0].clamp_(min=-1e30)  # the oracle's bounds stay finite; the weight is 0 as well
+    want, tol = attend_pairs(pair("f16", 3), q1, host, [64, 50], [list(range(-1, T - 1))] * 2, D ** -0.5)
+    assert all(bool(w.isfinite().all()) for w in want)
+    for k, (x, w, e) in enumerate(zip((out, *cache.draft_msgs, *cache.draft_lses), want, tol)):
+        x = x.double().cpu()
+        past = w.abs() >= 65520.0  # a mean that rounds to fp16's infinity (the last of the cases: 116916)
+        assert bool((x.isinf() == past).all()) and bool((x.sign() == w.sign())[past].all())
+        assert_within(x.masked_fill(past, 0.0), w.masked_fill(past, 0.0), e.masked_fill(past, 0.0), f"output {k}")
+
+
+@param("dtype", ("bf16", "f16", "f32"))
+@param("T,H,D", MIDDLE)
+def test_attend_infinite_values(dtype, T, H, D):
+    """An infinite value or level output of a position with a weight gives an infinite output of its sign at
+    its feature, no NaN, and leaves the other features' bits as they were."""
+    d = dev()
+    g = torch.Generator().manual_seed(T + D)
+    cache, host, q1 = middle_case(dtype, T, H, D, g, d)
+    q1 = q1.to(d)
+    clean = [x.clone() for x in (cache.attend(q1), *cache.draft_msgs)]
+    inf = float("inf")
+    cache.vs[0][:, :, 5, 2], cache.msgs[0][:, :, 5, 2] = inf, -0.5     # the middle level: either factor,
+    cache.vs[0][:, :, 17, 9], cache.msgs[0][:, :, 17, 9] = -2.0, -inf  # both
+    cache.vs[0][:, :, 33, 12], cache.msgs[0][:, :, 33, 12] = inf, inf
+    cache.vs[1][:, :, 5, 20] = -inf                                     # the deepest one's values
+    cache.msgs[1][:, :, 8, 30] = inf                                    # and the final one's
+    out = cache.attend(q1)
+    signs = {2: -inf, 9: inf, 12: inf}
+    deepest, middle, final = cache.draft_msgs[0], cache.draft_msgs[1], out
+    same = [c for c in range(D) if c not in (2, 9, 12, 20, 30)]
+    for x, y in ((deepest, clean[1]), (middle, clean[2]), (final, clean[0])):
+        assert torch.equal(x[..., same], y[..., same])
+    for c, s in signs.items():
+        assert bool((middle[..., c] == s).all() and (final[..., c] == s).all()), c
+    assert bool((deepest[..., 20] == -inf).all() and (final[..., 30] == inf).all())
+    # the middle level's drafted values are v * -inf: of one sign up to the first v of the other, then inf - inf
+    own = cache.draft_vs[0][..., 20].double().cumsum(-1) * 0 - cache.draft_vs[0][..., 20].double().sign() * inf
+    one = (own.cummax(-1).values == own.cummin(-1).values)
+    assert torch.equal(middle[..., 20].double().nan_to_num(0, 7, -7), own.masked_fill(~one, 0.0).nan_to_num(0, 7, -7))
