@@ -123,7 +123,9 @@ class DraftCache:
     ``draft_vs``, ``draft_msgs``, ``draft_lses`` with ``max_drafts`` slots in place of the capacity.
 
     The buffers and ``counts`` are written in place and stay the same objects.  A cache takes one step at
-    a time; caches of their own may be used at once, on any streams.
+    a time; caches of their own may be used at once, on any streams.  ``copy.deepcopy`` between two steps gives a
+    cache of its own, to follow two continuations; caches that share a ``counts`` are copied together
+    (``copy.deepcopy(caches)``), and their copies share one.
 
     A count reaches the capacity at most: tokens that do not fit are dropped by ``commit_drafts``, which
     sets the device flag ``overflow``; ``check_overflow()`` reads it.
@@ -197,17 +199,29 @@ class DraftCache:
                                                   rows(capacity, m), sums(capacity))
         self.draft_qs, self.draft_vs = rows(max_drafts, order), rows(max_drafts, m)
         self.draft_msgs, self.draft_lses = rows(max_drafts, m), sums(max_drafts)
-        # the moves of a commit, laid out once: the buffers stay where they are
-        row = dtype.itemsize * dim_head
-        pairs = zip((*self.draft_qs, *self.draft_vs, *self.draft_msgs, *self.draft_lses),
-                    (*self.qs, *self.vs, *self.msgs, *self.lses))
-        self._moves = b"".join([_lib.PACK_MOVE.pack(src.data_ptr(), dst.data_ptr(), row if src.dim() == 4 else 4, 0)
-                                for src, dst in pairs])
         self._geometry = (batch, kv_heads, max_drafts, capacity)
         # rows' tickets of a commit, 0 between calls, and the flag of tokens past the capacity
         zeros = torch.zeros((batch + 1) * _lib.PA_TICKET_STRIDE, dtype=torch.int32, device=device)
         self._tickets, self.overflow = zeros[_lib.PA_TICKET_STRIDE:], zeros[:1]
-        self._plans = {}  # the calls' structures, by the shape of q1
+        self._lay_out()
+
+    def _lay_out(self) -> None:
+        """What holds addresses of the buffers, which stay where they are: a commit's moves, and the other calls'
+        structures."""
+        row = self.dtype.itemsize * self.dim_head
+        pairs = zip((*self.draft_qs, *self.draft_vs, *self.draft_msgs, *self.draft_lses),
+                    (*self.qs, *self.vs, *self.msgs, *self.lses))
+        self._moves = b"".join([_lib.PACK_MOVE.pack(src.data_ptr(), dst.data_ptr(), row if src.dim() == 4 else 4, 0)
+                                for src, dst in pairs])
+        self._plans = {}  # by the shape of q1
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in ("_moves", "_plans")}
+
+    def __setstate__(self, state) -> None:
+        self.__dict__.update(state)
+        self.device = self.counts.device  # a load may have moved the buffers
+        self._lay_out()
 
     # -------------------------------------------------------------------------------------
 

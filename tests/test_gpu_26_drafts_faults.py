@@ -197,3 +197,40 @@ def test_attend_infinite_values(dtype, T, H, D):
     own = cache.draft_vs[0][..., 20].double().cumsum(-1) * 0 - cache.draft_vs[0][..., 20].double().sign() * inf
     one = (own.cummax(-1).values == own.cummin(-1).values)
     assert torch.equal(middle[..., 20].double().nan_to_num(0, 7, -7), own.masked_fill(~one, 0.0).nan_to_num(0, 7, -7))
+
+
+def test_a_forked_cache_goes_its_own_way():
+    """Two caches of one prompt, copied before a step and after one: steps and commits of one leave the other as it
+    is, also when the other is gone."""
+    import copy
+
+    from poly_attention import commit_drafts
+
+    d = dev()
+    g = torch.Generator().manual_seed(8)
+    caches = random_caches(2, 3, 2, 2, 64, 40, 4, [7, 3], "bf16", d, g)
+    bufs = lambda cs: [t for c in cs for name in BUFS for t in getattr(c, name)]  # noqa: E731
+    q1 = torch.randn(2, 4, 3, 64, generator=g).bfloat16().to(d)
+    path = torch.tensor([[0, 2, 1], [1, 0, 2]], dtype=torch.int32, device=d)
+    kept = torch.tensor([3, 1], dtype=torch.int32, device=d)
+
+    def step(cs):
+        outs = [c.attend(q1).clone() for c in cs]
+        commit_drafts(cs, path, kept)
+        return outs
+
+    fork = copy.deepcopy(caches)
+    before = [t.clone() for t in bufs(caches)]
+    first = step(fork)
+    assert fork[0].lengths() == [10, 4] and caches[0].lengths() == [7, 3]
+    for a, b in zip(bufs(caches), before):
+        assert torch.equal(a, b)
+    for a, b in zip(step(caches), first):
+        assert torch.equal(a, b)
+    again = copy.deepcopy(caches)  # after a step
+    del caches
+    for a, b in zip(step(again), step(fork)):
+        assert torch.equal(a, b)
+    for a, b in zip(bufs(again), bufs(fork)):
+        assert torch.equal(a, b)
+    assert again[1].lengths() == fork[1].lengths() == [13, 5]
