@@ -128,7 +128,8 @@ class DraftCache:
     (``copy.deepcopy(caches)``), and their copies share one.
 
     A count reaches the capacity at most: tokens that do not fit are dropped by ``commit_drafts``, which
-    sets the device flag ``overflow``; ``check_overflow()`` reads it.
+    sets the device flag ``overflow``; ``check_overflow()`` reads it.  Caches that are committed together
+    share the flag of the first of them from then on.
     """
 
     def __init__(self, cache, capacity: int, *, max_drafts: int = 16, lengths=None,
@@ -203,6 +204,7 @@ class DraftCache:
         # rows' tickets of a commit, 0 between calls, and the flag of tokens past the capacity
         zeros = torch.zeros((batch + 1) * _lib.PA_TICKET_STRIDE, dtype=torch.int32, device=device)
         self._tickets, self.overflow = zeros[_lib.PA_TICKET_STRIDE:], zeros[:1]
+        self._earlier = ()  # flags of commits with another first cache
         self._lay_out()
 
     def _lay_out(self) -> None:
@@ -444,7 +446,7 @@ class DraftCache:
 
     def check_overflow(self) -> None:
         """Raise if a commit ran past the capacity (reads the device flag: synchronises)."""
-        if int(self.overflow.item()):
+        if any(int(flag.item()) for flag in (self.overflow, *self._earlier)):
             raise RuntimeError(f"DraftCache overflow: tokens past the capacity {self.capacity} were "
                                "dropped")
 
@@ -462,7 +464,7 @@ def commit_drafts(caches: Sequence[DraftCache], path: Tensor, kept: Tensor) -> N
     (``overflow``)."""
     _need(len(caches) > 0, "a commit needs at least one cache")
     c0 = caches[0]
-    counts, geometry, device = c0.counts, c0._geometry, c0.device
+    counts, geometry, device, flag = c0.counts, c0._geometry, c0.device, c0.overflow
     for c in caches:
         if c.counts is not counts or c._geometry != geometry:
             _need(c.counts is counts, "caches of one commit share one counts tensor")
@@ -479,6 +481,9 @@ def commit_drafts(caches: Sequence[DraftCache], path: Tensor, kept: Tensor) -> N
               f"path: [{B}, 1 to {PA_MAX_DRAFTS}], not {list(path.shape)}")
         _need(kept.shape == (B,), f"kept: [{B}], not {list(kept.shape)}")
         path, kept = path.contiguous(), kept.contiguous()
+    for c in caches:  # all of them lose what does not fit
+        if c.overflow is not flag:
+            c._earlier, c.overflow = (*c._earlier, c.overflow), flag
     moves = c0._moves if len(caches) == 1 else b"".join([c._moves for c in caches])
     size = PA_MAX_MOVES * ctypes.sizeof(_lib.PaDraftMove)
     fn = _lib.load().pa_draft_commit
@@ -487,7 +492,7 @@ def commit_drafts(caches: Sequence[DraftCache], path: Tensor, kept: Tensor) -> N
         head = _lib.PACK_COMMIT.pack(
             B, hk, slots, capacity, len(part) // ctypes.sizeof(_lib.PaDraftMove), k + size >= len(moves),
             path.data_ptr(), path.stride(0), path.shape[1], kept.data_ptr(), counts.data_ptr(),
-            c0.overflow.data_ptr(), c0._tickets.data_ptr())
+            flag.data_ptr(), c0._tickets.data_ptr())
         _call(fn, kept, "pa_draft_commit", head + part)
 
 

@@ -234,3 +234,32 @@ def test_a_forked_cache_goes_its_own_way():
     for a, b in zip(bufs(again), bufs(fork)):
         assert torch.equal(a, b)
     assert again[1].lengths() == fork[1].lengths() == [13, 5]
+
+
+def test_overflow_shows_on_every_cache_of_a_commit():
+    """Tokens past the capacity are dropped from all layers: each of their caches says so, a copy too, and still does
+    after a commit with another cache first."""
+    import copy
+
+    from poly_attention import commit_drafts
+
+    d = dev()
+    a, b, c = random_caches(3, 2, 2, 1, 64, 8, 4, [7, 2], "bf16", d, torch.Generator().manual_seed(1))
+    path = torch.tensor([[0, 1, 2, 3]] * 2, dtype=torch.int32, device=d)
+    two = torch.tensor([2, 2], dtype=torch.int32, device=d)
+    none = torch.zeros(2, dtype=torch.int32, device=d)
+    commit_drafts([a, b], path, none)
+    for x in (a, b, c):
+        x.check_overflow()
+    commit_drafts([a, b], path, two)
+    assert a.lengths() == [8, 4]
+    c.check_overflow()  # not of that commit
+    commit_drafts([c, b, a], path, none)
+    c.check_overflow()
+    for x in (a, b, *copy.deepcopy([a, b])):
+        with pytest.raises(RuntimeError, match="overflow"):
+            x.check_overflow()
+    commit_drafts([b, c], path, two)
+    for x in (a, b, c):
+        with pytest.raises(RuntimeError, match="overflow"):
+            x.check_overflow()
