@@ -8,8 +8,10 @@
 // workgroup that finishes a row last joins the chunks.
 //
 // The token is the largest p_i / noise_i: one pass, no cumulative sums, and p's common factor drops
-// out.  Only a test of a further child after a rejection needs the residual's sum; without a draft
-// distribution that is 1 - (rejected probabilities), with one a pass over the row.
+// out.  Only a test of a further child after a rejection needs the residual's sum.  With a draft
+// distribution that is a pass over the row.  Without, it is the sum of what no child of the node holds, which the
+// statistics keep beside the whole sum, and of the children that are left: sums of positive numbers, where
+// 1 - (rejected probabilities) would lose all its digits next to 0.
 //
 // 32 trees of 16 nodes over 32000 tokens (bf16): 10.2 us for the statistics (3.6 TB/s: 4096 short workgroups),
 // 10.0 for the walk (dependent trips to memory).  8 chains of 6 over 128256 (fp32) with the drafts'
@@ -42,7 +44,8 @@ struct VerifyDev {
     int32_t* path;
     int32_t* kept;
     int64_t* token;
-    float4* stats;       // [B][T][chunks]: maximum, sum, first position of the maximum (as bits)
+    float4* stats;       // [B][T][chunks]: maximum, sum, first position of the maximum (as bits), sum without
+                         // the tokens of the node's children
     uint64_t* best;      // [B][chunks][2]
     uint32_t* ticket;    // [B][kTicketStride]
 };
@@ -93,15 +96,34 @@ __device__ __forceinline__ float wave_sum(float x) {
     return x;
 }
 
+// lane's node: its parent (-2 past the nodes) and its token (-1 where it is none of the vocabulary)
+__device__ __forceinline__ int node_parent(const VerifyDev& P, int b, int lane) {
+    return lane >= P.T ? -2 : P.parents ? P.parents[b * P.parents_stride + lane] : lane - 1;
+}
+__device__ __forceinline__ int node_token(const VerifyDev& P, int b, int lane) {
+    const int64_t tok = lane < P.T ? P.tokens[b * P.tokens_stride + lane] : -1;
+    return tok >= 0 && tok < P.vocab ? (int)tok : -1;
+}
+
 template <typename T>
 __global__ __launch_bounds__(kVerThreads) void k_verify_stats(const VerifyDev P) {
     constexpr int E = VerVec<T>::E, N = VerVec<T>::N;
-    __shared__ float s_x[4], s_sum[4];
+    __shared__ float s_x[4], s_sum[4], s_rest[4];
     __shared__ int s_i[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int chunk = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
     if (chunk == 0 && t == 0 && tid == 0) P.ticket[b * kTicketStride] = 0;  // before the walk's launch begins
     const float temp = row_temperature(P, b);
+    // without a draft distribution the walk may take tokens out of p one by one: the node's children, whose loads are
+    // on their way before the logits and looked at when the sum is known (1 us of 19 for 32 trees of 16 over 32000)
+    const bool apart = P.uniforms && !P.probs;
+    const int lt = min(lane, P.T - 1);
+    int64_t kid = -1;
+    int kid_of = lt - 1;
+    if (apart) {
+        kid = P.tokens[b * P.tokens_stride + lt];
+        if (P.parents) kid_of = P.parents[b * P.parents_stride + lt];
+    }
     const T* row = reinterpret_cast<const T*>(P.logits) + b * P.logits_sb + t * P.logits_sn;
     const int i0 = chunk * kVerChunk + tid * E;
     float x[N][E];
@@ -135,20 +157,41 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_stats(const VerifyDev P)
     at = s_i[0];
 #pragma unroll
     for (int w = 1; w < 4; ++w) take_first(top, at, s_x[w], s_i[w]);
-    float sum = 0.f;
+    float sum = 0.f, rest = 0.f;
     if (temp > 0.f) {
         const float c = logit_scale(temp), base = top == -INFINITY ? 0.f : top;
+        auto weights = [&]() __attribute__((always_inline)) -> float {
+            float y = 0.f;
 #pragma unroll
-        for (int k = 0; k < N; ++k)
+            for (int k = 0; k < N; ++k)
 #pragma unroll
-            for (int e = 0; e < E; ++e) sum += __builtin_amdgcn_exp2f((x[k][e] - base) * c);
-        sum = wave_sum(sum);
-        if (lane == 0) s_sum[wave] = sum;
+                for (int e = 0; e < E; ++e) y += __builtin_amdgcn_exp2f((x[k][e] - base) * c);
+            return wave_sum(y);
+        };
+        sum = rest = weights();
+        // a token outside the vocabulary lies in no chunk, or behind the last one's entries
+        const uint64_t in = (uint64_t)kid - (uint64_t)chunk * kVerChunk;
+        uint64_t kids = __ballot(apart && lane > t && lane < P.T && kid_of == t && in < kVerChunk);
+        if (kids) {
+            for (; kids; kids &= kids - 1) {
+                const int out = __builtin_amdgcn_readlane((int)in, __ffsll((unsigned long long)kids) - 1) - tid * E;
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x[k][e] = out == k * kVerThreads * E + e ? -INFINITY : x[k][e];
+            }
+            rest = weights();
+        }
+        if (lane == 0) {
+            s_sum[wave] = sum;
+            s_rest[wave] = rest;
+        }
         __syncthreads();
         sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+        rest = s_rest[0] + s_rest[1] + s_rest[2] + s_rest[3];
     }
     if (tid == 0)
-        P.stats[((int64_t)b * P.T + t) * P.chunks + chunk] = make_float4(top, sum, __int_as_float(at), 0.f);
+        P.stats[((int64_t)b * P.T + t) * P.chunks + chunk] = make_float4(top, sum, __int_as_float(at), rest);
 }
 
 // the residual after `n` rejections of one entry's probability p with draft probability q: inv[k] is
@@ -181,9 +224,8 @@ __device__ __forceinline__ int64_t best_token(uint64_t key) {
 template <typename T, bool SMALL>
 __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) {
     constexpr int E = VerVec<T>::E, N = VerVec<T>::N;
-    __shared__ float s_top[64], s_inv[64], s_rinv[64], s_wave[4];
-    __shared__ int s_arg[64];
-    __shared__ int64_t s_rej[64];
+    __shared__ float s_top[64], s_inv[64], s_rest[64], s_rinv[64], s_wave[4];
+    __shared__ int s_arg[64], s_rej[64];
     __shared__ uint64_t s_best[4][2];
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -204,8 +246,7 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
 
     // every wave holds the nodes, one per lane, and walks for itself
     const bool node = lane < P.T;
-    const int parent = node ? (parents ? parents[lane] : lane - 1) : -2;
-    const int64_t tok = node ? P.tokens[b * P.tokens_stride + lane] : -1;
+    const int parent = node_parent(P, b, lane), tok = node_token(P, b, lane);
     const float u = node && !greedy ? P.uniforms[b * P.uniforms_stride + lane] : 0.f;
     if constexpr (SMALL) {  // a row in a wave's registers, all rows on their way at once
         constexpr int R = kVerSmallNodes * 64 / kVerThreads;
@@ -220,7 +261,7 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int t = wave + r * (kVerThreads / 64);
-            float top = -INFINITY, sum = 0.f;
+            float top = -INFINITY, sum = 0.f, rest = 0.f;
             int at = P.vocab;
 #pragma unroll
             for (int k = 0; k < kVerSmallLoads; ++k)
@@ -233,21 +274,37 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
             for (int off = 32; off > 0; off >>= 1) take_first(top, at, __shfl_xor(top, off), __shfl_xor(at, off));
             if (!greedy) {
                 const float base = top == -INFINITY ? 0.f : top;
+                auto weights = [&]() __attribute__((always_inline)) -> float {
+                    float y = 0.f;
 #pragma unroll
-                for (int k = 0; k < kVerSmallLoads; ++k)
+                    for (int k = 0; k < kVerSmallLoads; ++k)
 #pragma unroll
-                    for (int e = 0; e < E; ++e) sum += __builtin_amdgcn_exp2f((x[r][k][e] - base) * c);  // 0 past the end
-                sum = wave_sum(sum);
+                        for (int e = 0; e < E; ++e) y += __builtin_amdgcn_exp2f((x[r][k][e] - base) * c);  // 0 past the end
+                    return wave_sum(y);
+                };
+                sum = rest = weights();
+                uint64_t kids = P.probs ? 0 : __ballot(lane > t && parent == t && tok >= 0);
+                if (kids) {
+                    for (; kids; kids &= kids - 1) {
+                        const int out = __builtin_amdgcn_readlane(tok, __ffsll((unsigned long long)kids) - 1) - lane * E;
+#pragma unroll
+                        for (int k = 0; k < kVerSmallLoads; ++k)
+#pragma unroll
+                            for (int e = 0; e < E; ++e) x[r][k][e] = out == k * 64 * E + e ? -INFINITY : x[r][k][e];
+                    }
+                    rest = weights();
+                }
             }
             if (t < P.T && lane == 0) {
                 s_top[t] = top;
                 s_inv[t] = 1.f / sum;
+                s_rest[t] = rest;
                 s_arg[t] = at;
             }
         }
     } else {  // statistics over the chunks, four threads per node
         const int t = tid >> 2, sub = tid & 3;
-        float top = -INFINITY, sum = 0.f;
+        float top = -INFINITY, sum = 0.f, rest = 0.f;
         int at = P.vocab;
         const float4* st = P.stats + ((int64_t)b * P.T + t) * P.chunks;
         if (t < P.T)
@@ -257,33 +314,40 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
                 const float was = top;
                 take_first(top, at, x.x, __float_as_int(x.z));
                 if (!greedy) {
-                    sum = was == -INFINITY ? sum : sum * __builtin_amdgcn_exp2f((was - top) * c);
-                    sum += x.x == -INFINITY ? x.y : x.y * __builtin_amdgcn_exp2f((x.x - top) * c);  // y: 0, or NaN
+                    const float f = was == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((was - top) * c),
+                                g = x.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((x.x - top) * c);  // of 0, or NaN
+                    sum = sum * f + x.y * g;
+                    rest = rest * f + x.w * g;
                 }
             }
         for (int off = 1; off < 4; off <<= 1) {
-            const float was = top, x = __shfl_xor(top, off), y = __shfl_xor(sum, off);
+            const float was = top, x = __shfl_xor(top, off), y = __shfl_xor(sum, off), z = __shfl_xor(rest, off);
             take_first(top, at, x, __shfl_xor(at, off));
-            if (!greedy)
-                sum = (was == -INFINITY ? sum : sum * __builtin_amdgcn_exp2f((was - top) * c)) +
-                      (x == -INFINITY ? y : y * __builtin_amdgcn_exp2f((x - top) * c));
+            if (!greedy) {
+                const float f = was == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((was - top) * c),
+                            g = x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((x - top) * c);
+                sum = sum * f + y * g;
+                rest = rest * f + z * g;
+            }
         }
         if (t < P.T && sub == 0) {
             s_top[t] = top;
             s_inv[t] = 1.f / sum;
+            s_rest[t] = rest;
             s_arg[t] = at;
         }
     }
     const uint64_t live = __ballot(draft_ancestors(parents, P.T, lane) != 0);
     __syncthreads();
-    // each node's own probability under its parent
-    float px = 0.f, qx = 1.f;
-    if (((live >> lane) & 1) && parent >= 0 && tok >= 0 && tok < P.vocab) {
+    // each node's own probability under its parent, and its weight there (the largest logit's is 1)
+    float px = 0.f, qx = 1.f, ex = 0.f;
+    if (((live >> lane) & 1) && parent >= 0 && tok >= 0) {
         if (greedy) {
             px = tok == s_arg[parent] ? 1.f : 0.f;
         } else {
             const float x = to_f(reinterpret_cast<const T*>(P.logits)[b * P.logits_sb + parent * P.logits_sn + tok]);
-            px = __builtin_amdgcn_exp2f((x - s_top[parent]) * c) * s_inv[parent];
+            ex = __builtin_amdgcn_exp2f((x - s_top[parent]) * c);
+            px = ex * s_inv[parent];
         }
         if (P.probs) qx = P.probs[b * P.probs_sb + parent * P.probs_sn + tok];
     }
@@ -291,7 +355,10 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
     // the walk: the current node's children in order.  All of it is the same in every wave.
     int cur = 0, kept = live & 1 ? 1 : 0, nrej = 0;  // rejected children of cur
     uint64_t path = kept, rejected = 0;               // kept nodes, rejected children whose token is out of p
-    float left = 1.f;                                 // without probs: 1 - their probabilities
+    // without probs: children of cur whose token no earlier one has, what those behind this lane's weigh, and the
+    // weights that a rejection left
+    uint64_t first = 0;
+    float behind = 0.f, left = 0.f;
     const T* row = reinterpret_cast<const T*>(P.logits) + b * P.logits_sb;
     const float* qrow = P.probs ? P.probs + b * P.probs_sb : nullptr;
     uint64_t children = kept ? __ballot(((live >> lane) & 1) && parent == 0) : 0;
@@ -300,7 +367,7 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
         children &= children - 1;
         float pt = __shfl(px, t);
         const float qt = __shfl(qx, t), ut = __shfl(u, t);
-        const int64_t xt = __shfl((long long)tok, t);
+        const int xt = __shfl(tok, t);
         if (nrej > 0) {
             if (P.probs) {
                 // the sum of the newest residual, now that a further child needs it
@@ -338,10 +405,10 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
                 const float sum = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
                 if (tid == 0) s_rinv[nrej - 1] = sum > 0.f ? 1.f / sum : 0.f;
                 __syncthreads();
-                pt = xt >= 0 && xt < P.vocab ? residual(pt, qt, s_rinv, nrej) : 0.f;
+                pt = xt >= 0 ? residual(pt, qt, s_rinv, nrej) : 0.f;
             } else {
-                if (__any(((rejected >> lane) & 1) && tok == xt)) pt = 0.f;
-                pt /= left;
+                const bool out = __any(((rejected >> lane) & 1) && tok == xt);
+                pt = out ? 0.f : __shfl(ex, t) / left;
             }
         }
         if (ut * qt < pt) {
@@ -350,15 +417,29 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
             path |= 1ull << t;
             nrej = 0;
             rejected = 0;
-            left = 1.f;
+            first = 0;
             children = __ballot(((live >> lane) & 1) && parent == t);
         } else if (!greedy) {
             if (P.probs) {
                 ++nrej;
-            } else if (pt > 0.f && left - pt * left > 0.f) {  // out of p, unless it was all of p
-                rejected |= 1ull << t;
-                left -= pt * left;
-                ++nrej;
+            } else if (pt > 0.f) {  // out of p, unless it was all of p
+                if (!first) {
+                    uint64_t more = __ballot(((live >> lane) & 1) && parent == cur && tok >= 0);
+                    behind = 0.f;
+                    while (more) {
+                        const int j = __ffsll((unsigned long long)more) - 1;
+                        first |= 1ull << j;
+                        more &= ~__ballot(tok == __builtin_amdgcn_readlane(tok, j));
+                        behind += lane < j ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ex), j)) : 0.f;
+                    }
+                }
+                // children before t are rejected and out of p, or had no part of it
+                const float rest = s_rest[cur] + __int_as_float(__builtin_amdgcn_readlane(__float_as_int(behind), t));
+                if (rest > 0x1p-64f) {  // of a weight of 1: what 2^30 tokens hold of it is above fp32's smallest number
+                    rejected |= 1ull << t;
+                    left = rest;
+                    ++nrej;
+                }
             }
         }
     }
@@ -405,7 +486,7 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_walk(const VerifyDev P) 
             }
         }
         for (int r = 0; r < nout; ++r) {
-            const int64_t out = s_rej[r] - i;
+            const int out = s_rej[r] - i;
 #pragma unroll
             for (int e = 0; e < E; ++e) w[e] = out == e ? 0.f : w[e];
         }

@@ -263,3 +263,68 @@ def test_overflow_shows_on_every_cache_of_a_commit():
     for x in (a, b, c):
         with pytest.raises(RuntimeError, match="overflow"):
             x.check_overflow()
+
+
+# (children's tokens in order, vocabulary, gaps between the two logits that hold all of p)
+COVERED = [((0, 1), 2), ((1, 0), 2), ((0, 1), 300), ((1, 0), 5000), ((0, 0, 1), 40000), ((1, 5, 0), 700)]
+
+
+def covered_inputs(tokens, V):
+    """Rows whose p is two tokens', 0 below 1 by a gap, both of them children of node 0, and the largest uniforms."""
+    gaps = torch.linspace(0.0, 15.0, 121)
+    B, T = len(gaps), 1 + len(tokens)
+    logits = torch.full((B, T, V), -2000.0)  # 0 in fp32
+    logits[:, :, 1] = 3.0
+    logits[:, :, 0] = 3.0 - gaps[:, None]
+    u = torch.full((B, T), 1.0 - 2.0 ** -24)
+    g = torch.Generator().manual_seed(V)
+    noise = -torch.log(torch.rand(B, V, generator=g).clamp(min=1e-30))
+    return (logits, torch.tensor([[0, *tokens]] * B), [[-1] + [0] * len(tokens)] * B, u, noise, None, None)
+
+
+@param("tokens,V", COVERED)
+def test_verify_children_that_hold_all_of_p(tokens, V):
+    """What is left after the first is rejected is the other's, so that is kept whatever its number (below 1); the row
+    always has a token."""
+    from test_gpu_25_drafts import run_verify
+
+    path, kept, token = (t.cpu() for t in run_verify(covered_inputs(tokens, V), dev()))
+    last = max(i for i, x in enumerate(tokens) if x == [y for y in tokens if y < 2][-1] and x not in tokens[:i]) + 1
+    assert kept.tolist() == [2] * len(kept) and path[:, 1].tolist() == [last] * len(kept)
+    assert bool(((token == 0) | (token == 1)).all())
+
+
+SHARES = [(2 ** -k, s, V, order) for k in (4, 7, 11, 16) for s in (0.3, 0.8) for V in (3, 40, 6000)
+          for order in ((0, 1), (0, 2, 1))]
+
+
+def share_inputs(below):
+    """Per case of SHARES a row of each of its vocabularies: token 0 has all but a small part of p, token 1 a share of
+    that part.  The child with token 0 is rejected; that with token 1 gets a number 2^-14 below its share, or above."""
+    rows = []
+    for part, share, V, order in SHARES:
+        p = torch.full((V,), part * (1 - share) / (V - 2), dtype=torch.float64)
+        p[0], p[1] = 1 - part, part * share
+        x = p.log().float()
+        p = torch.softmax(x.double(), 0)
+        out = [t for t in order if t != 1]
+        now = p[1] / (p.sum() - p[out].sum())
+        T = 1 + len(order)
+        u = torch.full((1, T), 1.0 - 2.0 ** -24)
+        u[0, T - 1] = float(now) * (1 - below * 2.0 ** -14)
+        noise = -torch.log(torch.rand(1, V, generator=torch.Generator().manual_seed(T)).clamp(min=1e-30))
+        rows.append((x.expand(1, T, V).contiguous(), torch.tensor([[0, *order]]), [[-1] + [0] * len(order)], u, noise, None,
+                     None))
+    return rows
+
+
+@param("below", (1, -1))
+def test_verify_share_of_a_small_remainder(below):
+    """A child's probability after a rejection that leaves down to 2^-16 of p is exact to fp32's few last digits."""
+    from test_gpu_25_drafts import assert_walk, run_verify
+
+    for inputs in share_inputs(below):
+        want, margin = DO.verify(*inputs)
+        assert margin > 2.0 ** -17  # the kernel's probabilities are within 2^-20
+        assert len(want[0][0]) == (2 if below > 0 else 1)
+        assert_walk(run_verify(inputs, dev()), want)
