@@ -246,9 +246,13 @@ def _draft_step(module, qs, vs, mask, context_mask, rotary_pos_emb, cache: Draft
     elif exists(module.rotary_emb):
         # a module's own rotary (poly_attention.py:302-304, n_poly_attention.py:224-229): the cache
         # holds its keys rotated, as a StaticCache does
-        cache.rotate_prefix(module.rotary_emb)
-        kwargs["inv_freq"] = module.rotary_emb.freqs
-        kwargs["interp"] = module.rotary_emb.interpolate_factor
+        rot = module.rotary_emb
+        cache.rotate_prefix(rot)
+        if type(rot) is RotaryEmbedding and rot.freqs.dtype == torch.float32:
+            kwargs["inv_freq"], kwargs["interp"] = rot.freqs, rot.interpolate_factor
+        else:  # frequencies of 16 bits (a layer cast whole) give angles of 16 bits, to the cached keys too
+            pos = cache.positions(q1.shape[-2], parents).to(q1.dtype) / rot.interpolate_factor
+            kwargs["angles"] = rot(pos).detach()
     q1 = cache.append(qs, vs, weights, eps=eps, parents=parents, **kwargs)
     return cache.attend(q1, parents=parents, scale=module.scale, softclamp=module.softclamp_value)
 

@@ -328,3 +328,41 @@ def test_verify_share_of_a_small_remainder(below):
         assert margin > 2.0 ** -17  # the kernel's probabilities are within 2^-20
         assert len(want[0][0]) == (2 if below > 0 else 1)
         assert_walk(run_verify(inputs, dev()), want)
+
+
+@param("order", (2, 3))
+@param("dtype", (torch.bfloat16, torch.float16))
+@param("freqs_too", (True, False))
+def test_module_rotary_of_a_layer_cast_whole(order, dtype, freqs_too):
+    """A layer cast to 16 bits with its rotary frequencies rotates by angles of 16 bits, up to a radian off behind a few
+    hundred positions: a drafted step's keys are turned by the same ones as the cached keys."""
+    from parity import assert_parity
+    from poly_attention import DraftCache, commit_drafts
+    from poly_attention.rotary import RotaryEmbedding
+    from test_gpu_25_drafts import make_module
+
+    d = dev()
+    torch.manual_seed(5)
+    m, _, _ = make_module(order, 4, d, dtype, use_rotary_embed=True)
+    if not freqs_too:
+        m.rotary_emb.freqs.data = RotaryEmbedding(2 * m.rotary_emb.freqs.numel()).freqs.data.to(d)
+    x = torch.randn(2, 404, 64, generator=torch.Generator().manual_seed(2)).to(d, dtype)
+    with torch.no_grad():
+        _, cache = m(x[:, :400], return_cache=True)
+        dc = DraftCache(cache, capacity=410)
+        got = m(x[:, 400:], cache=dc)
+        commit_drafts([dc], torch.arange(4, dtype=torch.int32, device=d).expand(2, 4).contiguous(),
+                      torch.full((2,), 4, dtype=torch.int32, device=d))
+        want = []
+        for i in range(400, 404):
+            y, cache = m(x[:, i:i + 1], cache=cache, return_cache=True)
+            want.append(y)
+        assert_parity(got, torch.cat(want, 1), dtype, "a chain", roundings=3)
+        # the tuple cache holds its keys unrotated.  Rounded on the module's way: the norm, cos, sin, both products and
+        # their sum, and the draft's one: each half a step of the pair's values
+        half = torch.finfo(dtype).eps / 2
+        for q, raw in zip(dc.qs, cache[:2] if order == 2 else cache[0]):
+            turned = m.rotary_emb.rotate_queries_or_keys(raw)
+            pair = raw.float().abs().unflatten(-1, (-1, 2)).sum(-1, keepdim=True).expand(*raw.shape[:-1], -1, 2).flatten(-2)
+            off = (q[:, :, :404].float() - turned.float()).abs()
+            assert bool((off <= 7 * half * pair).all()), float((off / pair).max())
