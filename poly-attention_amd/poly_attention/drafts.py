@@ -71,8 +71,7 @@ def _rows16(t: Tensor) -> Tensor:
     s0, s1, s2, s3 = t.stride()
     if s3 == 1 and not ((s0 | s1 | s2) * t.element_size() | t.data_ptr()) & 15:
         return t
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() & 15 else t
+    return t.new_empty(t.shape).copy_(t)  # contiguous() keeps the stride of a dimension of size 1, whatever it is
 
 
 def _parents(parents: Optional[Tensor], batch: int, drafts: int, device) -> tuple:

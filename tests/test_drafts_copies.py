@@ -54,3 +54,20 @@ def test_copies_of_a_models_caches_share_a_count(how):
     c, d = how([a, b])
     assert c.counts is d.counts and c.counts is not a.counts
     assert c._tickets.data_ptr() not in (a._tickets.data_ptr(), d._tickets.data_ptr())
+
+
+@param("shape,strides,offset", [
+    ((1, 2, 1, 8), (5, 8, 3, 1), 0),    # dimensions of size 1 have any stride and count as contiguous
+    ((2, 1, 1, 8), (8, 7, 9, 1), 0),
+    ((2, 3, 4, 8), (96, 32, 8, 1), 3),  # rows not on 16 bytes
+    ((2, 3, 4, 8), (8, 16, 48, 2), 0),
+    ((2, 3, 4, 8), (0, 0, 9, 1), 0),
+])
+def test_rows_are_copied_where_they_do_not_start_on_16_bytes(shape, strides, offset):
+    from poly_attention.drafts import _rows16
+
+    t = torch.arange(400, dtype=torch.bfloat16).as_strided(shape, strides, offset)
+    r = _rows16(t)
+    assert torch.equal(r, t) and r.stride(3) == 1 and r.data_ptr() % 16 == 0
+    assert all(s * 2 % 16 == 0 for s in r.stride()[:3])
+    assert _rows16(r) is r

@@ -366,3 +366,23 @@ def test_module_rotary_of_a_layer_cast_whole(order, dtype, freqs_too):
             pair = raw.float().abs().unflatten(-1, (-1, 2)).sum(-1, keepdim=True).expand(*raw.shape[:-1], -1, 2).flatten(-2)
             off = (q[:, :, :404].float() - turned.float()).abs()
             assert bool((off <= 7 * half * pair).all()), float((off / pair).max())
+
+
+def test_rows_of_size_one_dimensions_of_any_stride():
+    """One row, one token, one head: a stride that nothing follows is no reason to refuse."""
+    from poly_attention import DraftCache
+
+    d = dev()
+    g = torch.Generator().manual_seed(6)
+    cache = DraftCache.empty(order=2, batch=1, kv_heads=1, dim_head=64, capacity=9, max_drafts=2, device=d,
+                             counts=torch.tensor([9], dtype=torch.int32, device=d))
+    fill_cache(cache, g, d)
+    rows = [torch.randn(64, generator=g).bfloat16().to(d) for _ in range(4)]
+    plain = [r.view(1, 1, 1, 64) for r in rows]
+    odd = [r.as_strided((1, 1, 1, 64), (3, 5, 7, 1)) for r in rows]
+    results = []
+    for qs in (plain, odd):
+        q1 = cache.append(qs[:3], qs[3:], [None] * 3, eps=1e-6)
+        results.append([q1.clone(), cache.attend(qs[0]).clone(), *[t.clone() for t in (*cache.draft_qs, *cache.draft_vs)]])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
