@@ -28,6 +28,7 @@ from typing import Optional, Sequence
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import DTYPE_CODE, PA_MAX_DRAFTS, PA_MAX_MOVES
@@ -55,6 +56,12 @@ def _call(fn, t: Tensor, what: str, *args) -> None:
 def _need(ok: bool, what: str, error=ValueError) -> None:
     if not ok:
         raise error(what)
+
+
+def _no_tangents(*tensors: Optional[Tensor]) -> None:
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise RuntimeError(_NO_GRAD)
 
 
 def _set_view(v, t: Tensor) -> None:
@@ -273,6 +280,7 @@ class DraftCache:
         q1 = qs[0]
         _need(len(qs) == self.order + 1 and len(vs) == self.order - 1 and len(weights) == len(qs),
               f"order {self.order}: {self.order + 1} qs and weights, {self.order - 1} vs")
+        _no_tangents(*qs, *vs, *weights, angles, inv_freq)
         plan = self._plans.get(("append", q1.shape)) or self._plan("append", q1)
         B, H, T, d = q1.shape
         dtype, device, grad = self.dtype, self.device, torch.is_grad_enabled()
@@ -371,6 +379,7 @@ class DraftCache:
         the other levels' queries, keys and values are in the draft slots.  Writes ``draft_msgs`` and
         ``draft_lses`` and returns the output [B, heads, T, d].  ``scale`` defaults to
         dim_head ** -0.5."""
+        _no_tangents(q1)
         plan = self._plans.get(("attend", q1.shape)) or self._plan("attend", q1)
         B, H, T, d = q1.shape
         dtype, device = self.dtype, self.device

@@ -71,3 +71,22 @@ def test_rows_are_copied_where_they_do_not_start_on_16_bytes(shape, strides, off
     assert torch.equal(r, t) and r.stride(3) == 1 and r.data_ptr() % 16 == 0
     assert all(s * 2 % 16 == 0 for s in r.stride()[:3])
     assert _rows16(r) is r
+
+
+def test_forward_mode_tangents_are_refused():
+    """A step has no derivative, forward or backward: a dual tensor raises as one that requires a gradient does."""
+    from torch.autograd import forward_ad
+
+    c = empty()
+    row = lambda: torch.zeros(2, 2, 3, 64)  # noqa: E731
+    w = [torch.ones(64) for _ in range(3)]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(row(), row())
+        with pytest.raises(RuntimeError, match="inference-only"):
+            c.attend(dual)
+        for qs, vs, ws in (([row(), dual, row()], [row()], w), ([row()] * 3, [dual], w),
+                           ([row()] * 3, [row()], [None, forward_ad.make_dual(w[0], w[1]), None])):
+            with pytest.raises(RuntimeError, match="inference-only"):
+                c.append(qs, vs, ws, eps=1e-6)
+        with pytest.raises(RuntimeError, match="GPU"):  # no tangent: the check behind it
+            c.attend(row())
