@@ -611,6 +611,10 @@ bool draft_dim(int d) { return d >= 8 && d <= 256 && d % 8 == 0 && (d <= 128 || 
 // k_draft_wide, 8 x 4096 of 128: as many as are in flight 69, twice as many 79 (64 rows); 84 and 90 (128 rows).
 constexpr int64_t kDraftMany = 4, kDraftFew = 2, kDraftWideMany = 2, kDraftUnitBytes = 64 * 1024, kDraftCus = 256;
 
+// Workgroups of a grid's first dimension, at most: its threads are counted in 32 bits, and a first launch that is
+// refused would leave the second one records that nothing has written.
+constexpr int64_t kDraftGroups = (int64_t(1) << 32) / kDraftThreads - 1;
+
 // geometry shared by the workspace query and the launch; false where the request is malformed
 bool draft_plan(const pa_draft* d, DraftDev& P, int& units, int& tiles) {
     if (d->batch < 1 || d->kv_heads < 1 || d->heads < 1 || d->heads % d->kv_heads != 0) return false;
@@ -647,7 +651,8 @@ bool draft_plan(const pa_draft* d, DraftDev& P, int& units, int& tiles) {
     P.target_min = (int)std::min(std::max<int64_t>(1, few), chunks);
     P.least = std::max(1, (int)(kDraftUnitBytes * tiles / ((int64_t)kDraftChunk * d->dim * (f32 ? 4 : 2))));
     units = (int)std::min(target + d->batch, chunks);
-    return (int64_t)d->kv_heads * P.row_blocks <= 65535 && (int64_t)d->batch * d->kv_heads <= INT32_MAX / 64;
+    return (int64_t)d->kv_heads * P.row_blocks <= 65535 && (int64_t)d->batch * d->kv_heads <= kDraftGroups &&
+           (int64_t)d->batch + units <= kDraftGroups;
 }
 
 // the workspace's arrays, and its size
@@ -814,7 +819,7 @@ int launch_draft_append(const pa_draft_rows* r, hipStream_t s) {
         I.heads = it.src.heads;
     }
     const int64_t nodes = (int64_t)r->batch * r->drafts;
-    if (nodes > (1 << 30)) return PA_EUNSUPPORTED;
+    if (nodes > kDraftGroups) return PA_EUNSUPPORTED;
     const dim3 grid((unsigned)nodes, r->count);
     ProfScope ps("draft_append", s);
     if (T == PA_F32) hipLaunchKernelGGL((k_draft_append<float>), grid, dim3(kDraftThreads), 0, s, P);
@@ -829,6 +834,7 @@ int launch_draft_commit(const pa_commit* c, hipStream_t s) {
         !c->path || !c->kept || !c->counts || (c->advance && !c->tickets))
         return PA_EINVAL;
     if (c->kv_heads > (1 << 14)) return PA_EUNSUPPORTED;  // 32-bit indexes of a row's vectors
+    if (c->batch > kDraftGroups) return PA_EUNSUPPORTED;
     DraftCommitDev P;
     P.batch = c->batch;
     P.kv_heads = c->kv_heads;

@@ -429,7 +429,7 @@ class DraftCache:
                 _set_view(L.out, cut(self.draft_msgs[t]))
                 _set_view(L.lse, cut(self.draft_lses[t]))
         D.workspace_bytes = _lib.load().pa_draft_attend_workspace(ctypes.byref(D))
-        _need(D.workspace_bytes > 0, f"{H} heads, {T} tokens over {self.kv_heads} kv_heads: too many",
+        _need(D.workspace_bytes > 0, f"{self.batch} rows, {H} heads, {T} tokens over {self.kv_heads} kv_heads: too many",
               NotImplementedError)
         last = D.levels[self.order - 1]
         strides = (T * H * self.dim_head, self.dim_head, H * self.dim_head, 1)
