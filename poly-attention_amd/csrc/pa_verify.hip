@@ -117,12 +117,11 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_stats(const VerifyDev P)
     // without a draft distribution the walk may take tokens out of p one by one: the node's children, whose loads are
     // on their way before the logits and looked at when the sum is known (1 us of 19 for 32 trees of 16 over 32000)
     const bool apart = P.uniforms && !P.probs;
-    const int lt = min(lane, P.T - 1);
     int64_t kid = -1;
-    int kid_of = lt - 1;
-    if (apart) {
-        kid = P.tokens[b * P.tokens_stride + lt];
-        if (P.parents) kid_of = P.parents[b * P.parents_stride + lt];
+    int kid_of = lane - 1;
+    if (apart && lane > t && lane < P.T) {
+        kid = P.tokens[b * P.tokens_stride + lane];
+        if (P.parents) kid_of = P.parents[b * P.parents_stride + lane];
     }
     const T* row = reinterpret_cast<const T*>(P.logits) + b * P.logits_sb + t * P.logits_sn;
     const int i0 = chunk * kVerChunk + tid * E;
@@ -171,7 +170,7 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_stats(const VerifyDev P)
         sum = rest = weights();
         // a token outside the vocabulary lies in no chunk, or behind the last one's entries
         const uint64_t in = (uint64_t)kid - (uint64_t)chunk * kVerChunk;
-        uint64_t kids = __ballot(apart && lane > t && lane < P.T && kid_of == t && in < kVerChunk);
+        uint64_t kids = __ballot(kid_of == t && in < kVerChunk);
         if (kids) {
             for (; kids; kids &= kids - 1) {
                 const int out = __builtin_amdgcn_readlane((int)in, __ffsll((unsigned long long)kids) - 1) - tid * E;
