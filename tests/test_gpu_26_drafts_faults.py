@@ -386,3 +386,49 @@ def test_rows_of_size_one_dimensions_of_any_stride():
         results.append([q1.clone(), cache.attend(qs[0]).clone(), *[t.clone() for t in (*cache.draft_qs, *cache.draft_vs)]])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@param("dtype", ("bf16", "f32"))
+@param("order,T,H,D", [(8, 64, 1, 8), (8, 5, 3, 16), (6, 17, 2, 40), (5, 33, 4, 136 + 8)])
+def test_attend_many_levels(dtype, order, T, H, D):
+    from test_gpu_25_drafts import check_attend
+
+    check_attend(order, 1, [37], T, H, 1, D, dtype, "tree")
+
+
+def test_offsets_past_32_bits():
+    """2.3e9 elements a buffer (4.6 GB): the last key head's positions, keys and records lie past 2^31 elements and 2^32
+    bytes, the committed ones too."""
+    from poly_attention import DraftCache, commit_drafts
+
+    d = dev()
+    hk, n, D, T = 17, 1 << 20, 128, 3
+    cache = DraftCache.empty(order=2, batch=1, kv_heads=hk, dim_head=D, capacity=n + 2, max_drafts=T, device=d,
+                             counts=torch.tensor([n], dtype=torch.int32, device=d))
+    g = torch.Generator(device=d).manual_seed(0)
+    for t in (*cache.qs, *cache.vs, *cache.msgs, *cache.draft_qs, *cache.draft_vs):
+        t.normal_(generator=g)
+    cache.lses[0].normal_(generator=g).add_(14.0)
+    q1 = torch.randn(1, hk, T, D, generator=g, device=d).bfloat16()
+    out = cache.attend(q1)
+    for h in (0, hk - 1):
+        def level(q, k, dk, v, dv, bias=None, dbias=None):
+            s = torch.cat([q.double() @ k[:n].double().t(), q.double() @ dk.double().t()], 1) * D ** -0.5
+            if bias is not None:
+                s = s + torch.cat([bias[:n].double(), dbias])
+            s[:, n:].masked_fill_(torch.ones(T, T, device=d).triu(1).bool(), -float("inf"))
+            w = torch.softmax(s, -1)
+            return w[:, :n] @ v[:n].double() + w[:, n:] @ dv.double(), torch.logsumexp(s, -1)
+
+        msg, lse = level(cache.draft_qs[0][0, h], cache.qs[1][0, h], cache.draft_qs[1][0, h], cache.vs[0][0, h],
+                         cache.draft_vs[0][0, h])
+        want, _ = level(q1[0, h], cache.qs[0][0, h], cache.draft_qs[0][0, h], cache.msgs[0][0, h], msg, cache.lses[0][0, h], lse)
+        # values of size 1 under 10^6 weights: outputs of 10^-3, and the sums' fp32 roundings of 2^-24 sqrt(n) n / n
+        assert float((out[0, h].double() - want).abs().max()) <= 2.0 ** -8 * float(want.abs().max()) + 2.0 ** -14
+        assert float((cache.draft_msgs[0][0, h].double() - msg).abs().max()) <= 2.0 ** -8 * float(msg.abs().max()) + 2.0 ** -14
+        assert float((cache.draft_lses[0][0, h].double() - lse).abs().max()) <= 2.0 ** -14
+    commit_drafts([cache], torch.tensor([[0, 2, 1]], dtype=torch.int32, device=d), torch.tensor([2], dtype=torch.int32, device=d))
+    assert cache.lengths() == [n + 2]
+    for name in BUFS:
+        for dst, src in zip(getattr(cache, name), getattr(cache, "draft_" + name)):
+            assert torch.equal(dst[0, :, n:], src[0][:, [0, 2]])
