@@ -347,7 +347,8 @@ typedef struct pa_linear {
  * its outputs are 0 and the walk of pa_draft_verify never reaches it.
  * The drafted tokens' keys, values, level outputs and logsumexps lie in draft slots [B, kv_heads,
  * T, dim] beside the cache until pa_draft_commit moves the kept ones behind the cached positions.
- * A count below 0 or above the capacity (at most 2^30) is taken as that bound. */
+ * A count below 0 or above the capacity (at most 2^30) is taken as that bound (by pa_draft_append, which
+ * knows no capacity, as it is).  batch * kv_heads, and batch * T of an append, stay below 2^24. */
 
 /* One level of pa_draft_attend. */
 typedef struct pa_draft_level {
@@ -367,8 +368,11 @@ typedef struct pa_draft_level {
  *   s_ij  = softclamp(scale <q_i, k_j>) + bias_j      j a cached position of the row, an ancestor of
  *   out_i = sum_j softmax_j(s_ij) v_j                  node i, or i itself
  *   lse_i = logsumexp_j(s_ij)
- * with the values of pa_poly_decode, a middle level's product not rounded (v; v * out of the level
- * below; out of the level below); the ancestors' level outputs are used as computed, in fp32.
+ * with the values of pa_poly_decode (v; v * out of the level below; out of the level below); the
+ * ancestors' level outputs are used as computed, in fp32.  In 16-bit types the weights of cached positions
+ * and a middle level's products with them enter as two numbers each, to 2^-16 of their value (fp16 weights
+ * 2^-21, and 2^-32 of the row's largest), and all sums are fp32: the outputs' own rounding is the largest
+ * error.  An infinite value gives the infinite output of the formula.
  * Rows and views start on 16 bytes; cached positions lie at most 2^22 elements apart. */
 typedef struct pa_draft {
     int32_t batch, kv_heads, heads, drafts, dim, order, capacity;
@@ -418,7 +422,8 @@ typedef struct pa_draft_rows {
  *   p := max(p - q, 0) / sum   with draft_probs, q = draft_probs[b, current node] the distribution
  *                              that the children of that node were drawn from, independently
  *   p := p without x / sum     without: the children were chosen, q(x) = 1
- * (p stays as it is where the sum is 0).  At the end token[b] is the i with the largest
+ * (p stays as it is where the sum is 0; without draft_probs, where what is left weighs no more than 2^-64
+ * of the largest).  At the end token[b] is the i with the largest
  * p_i / noise[b, i] among p_i > 0, the lowest of equals: with noise drawn from Exp(1) a sample of p.
  * path[b] lists the kept nodes in order, then -1; kept[b] is their number.  A row whose node 0 is
  * absent keeps nothing and gets token -1, and a p without a positive entry (logits that are NaN or

@@ -192,9 +192,9 @@ extern template void launch_draft_wide<f16>(const DraftDev& P, int units, bool v
 // its waves, and their 16-row tiles: what two waves per SIMD have registers for
 constexpr int kDraftWideWaves = 4;
 // Whether a group of `rows` rows at the final level goes to k_draft_wide (D: the padded head dim).  Both, in
-// us, behind cold caches: 40 rows of 128, 8 x 4096 positions 83 here, 68 there, 64 rows 85 and 69, 20 x 500
-// 48 rows 49 and 31; 64 rows of 64, 8 x 4096 48 and 48, 48 rows 20 x 500 26 and 24.  With a middle level
-// 64 rows of 64 (order 3, 8 x 2048) 84 and 105, 128 rows 33 and 31; 64 rows of 128 72 and 69.
+// us, behind cold caches: 40 rows of 128, 8 x 4096 positions 87 here, 73 there, 64 rows 94 and 76, 48 rows 20 x 500
+// 42 and 40; 64 rows of 64, 8 x 4096 61 and 53, 48 rows 20 x 500 34 and 29.  With a middle level (order 3, 8 x 2048)
+// 64 rows of 64 50 and 61, 128 rows 66 and 68; 64 rows of 128 102 and 100.
 constexpr bool draft_wide(int D, bool f32, bool middle, int rows) {
     return !f32 && D <= 128 && rows > (D == 64 && middle ? 64 : 32);
 }

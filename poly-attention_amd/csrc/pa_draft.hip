@@ -535,7 +535,7 @@ __device__ __forceinline__ void move_rows(const char* src, char* dst, int64_t sh
     }
 }
 
-// One workgroup per (row, move): 8 rows of 54 buffers 4.9 us, one of 5 3.9 (paths, rows, counts: three dependent
+// One workgroup per (row, move): 8 rows of 54 buffers 4.9 us, one of 5 4.2 (paths, rows, counts: three dependent
 // trips to memory).  With advance the workgroup of a row that draws the last ticket counts the
 // kept nodes: by then every other one has read the count, so one launch does both.  The first wave reads it
 // for the workgroup: a barrier does not wait for another wave's loads from memory, so a wave that read the
@@ -606,9 +606,10 @@ bool draft_dim(int d) { return d >= 8 && d <= 256 && d % 8 == 0 && (d <= 128 || 
 
 // Workgroups of the first launch aimed at, as multiples of those that are in flight together: kDraftMany,
 // but kDraftFew where a unit's keys are below kDraftUnitBytes per 16 rows, since a workgroup's start
-// and end and its record cost the more the more rows it has.  Behind cold caches: 32 x 8192 positions of
-// 128, 32 rows: 272 us with few, 249 with many; order 3, 8 x 2048 of 64, 16 rows: 41 with few, 45 with many.
-// k_draft_wide, 8 x 4096 of 128: as many as are in flight 69, twice as many 79 (64 rows); 84 and 90 (128 rows).
+// and end and its record cost the more the more rows it has.  Behind cold caches: 32 rows of up to 8192
+// positions of 128, 32 query rows: 250 us with few, 245 with many; order 3, 8 of up to 2048 of 64, 16 rows: 44 with few,
+// 46 with many.  k_draft_wide, 8 x 4096 of 128: as many as are in flight 76, twice as many 81 (64 rows); 90 and 93
+// (128 rows).
 constexpr int64_t kDraftMany = 4, kDraftFew = 2, kDraftWideMany = 2, kDraftUnitBytes = 64 * 1024, kDraftCus = 256;
 
 // Workgroups of a grid's first dimension, at most: its threads are counted in 32 bits, and a first launch that is

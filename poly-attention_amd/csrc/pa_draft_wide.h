@@ -13,10 +13,11 @@
 // results go to their records from registers, and nothing is joined.
 //
 // Bound by neither the loads nor the products alone but by how far they overlap, at two waves per SIMD.
-// 8 x 4096 positions of 128, 8 key heads, behind cold caches: 64 rows 69 us (loads alone 62, the rest alone
-// 41; k_draft_partial 85), 128 rows 84 (71, 49; 130), 256 rows in two blocks 135 (91, 79; 324).  Loads not
-// marked as streaming: 135 us for 128 rows.  A row tile's number tested inside the loop, which keeps LDS
-// reads from running ahead of it: 166 us for 256 rows, 155 without.  Eight waves with 256 rows: 154.
+// 8 x 4096 positions of 128, 8 key heads, behind cold caches: 64 rows 76 us (loads alone 62; k_draft_partial 94),
+// 128 rows 89 (71), 256 rows in two blocks 143 (91).  With one product per weight and value instead of two (weights
+// rounded to the type): 73, 86 and 131; at that stage, loads not marked as streaming: 135 us for 128 rows; a row
+// tile's number tested inside the loop, which keeps LDS reads from running ahead of it: 166 us for 256 rows, 155
+// without; eight waves with 256 rows: 154.
 #pragma once
 
 #include <type_traits>

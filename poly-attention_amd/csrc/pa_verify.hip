@@ -13,9 +13,9 @@
 // statistics keep beside the whole sum, and of the children that are left: sums of positive numbers, where
 // 1 - (rejected probabilities) would lose all its digits next to 0.
 //
-// 32 trees of 16 nodes over 32000 tokens (bf16): 10.2 us for the statistics (3.6 TB/s: 4096 short workgroups),
-// 10.0 for the walk (dependent trips to memory).  8 chains of 6 over 128256 (fp32) with the drafts'
-// distributions: 6.0 and 12.8.
+// 32 trees of 16 nodes over 32000 tokens (bf16): 10.8 us for the statistics (3.0 TB/s: 4096 short workgroups),
+// 10.4 for the walk (dependent trips to memory).  8 chains of 6 over 128256 (fp32) with the drafts'
+// distributions: 6.0 and 13.
 #include "pa_draft.h"
 
 namespace pa {
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_stats(const VerifyDev P)
     if (chunk == 0 && t == 0 && tid == 0) P.ticket[b * kTicketStride] = 0;  // before the walk's launch begins
     const float temp = row_temperature(P, b);
     // without a draft distribution the walk may take tokens out of p one by one: the node's children, whose loads are
-    // on their way before the logits and looked at when the sum is known (1 us of 19 for 32 trees of 16 over 32000)
+    // on their way before the logits and looked at when the sum is known (0.8 us of 18.4 behind cold caches, 32 trees of 16 over 32000)
     const bool apart = P.uniforms && !P.probs;
     int64_t kid = -1;
     int kid_of = lane - 1;
