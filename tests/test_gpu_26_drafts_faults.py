@@ -432,3 +432,31 @@ def test_offsets_past_32_bits():
     for name in BUFS:
         for dst, src in zip(getattr(cache, name), getattr(cache, "draft_" + name)):
             assert torch.equal(dst[0, :, n:], src[0][:, [0, 2]])
+
+
+# (seed, B, T, V): every node a child of node 0, tokens that repeat, numbers near 1: many rejections in a row
+STARS = [(1, 6, 64, 40), (2, 6, 64, 20000), (3, 8, 8, 30), (4, 8, 8, 500), (5, 4, 33, 4097), (6, 8, 5, 6)]
+
+
+def star_inputs(case):
+    seed, B, T, V = case
+    g = torch.Generator().manual_seed(seed)
+    logits = 3 * torch.randn(B, T, V, generator=g)
+    likely = logits[:, 0].topk(min(V, 24)).indices
+    tokens = likely.gather(1, torch.randint(0, likely.shape[1], (B, T), generator=g))
+    tokens[:, 1::5] = torch.randint(0, V, tokens[:, 1::5].shape, generator=g)
+    tokens[0, T // 2] = V
+    u = 1 - 0.15 * torch.rand(B, T, generator=g) ** 2
+    noise = -torch.log(torch.rand(B, V, generator=g).clamp(min=1e-30))
+    temperature = 0.5 + torch.rand(B, generator=g)
+    return logits, tokens, [[-1] + [0] * (T - 1)] * B, u, noise, temperature, None
+
+
+@param("case", STARS)
+def test_verify_many_children_of_one_node(case):
+    from test_gpu_25_drafts import assert_walk, run_verify
+
+    inputs = star_inputs(case)
+    want, margin = DO.verify(*inputs)
+    assert margin > 2.0 ** -17
+    assert_walk(run_verify(inputs, dev()), want)
