@@ -53,11 +53,12 @@
 extern "C" {
 #endif
 
-#define PA_ABI_VERSION 9
+#define PA_ABI_VERSION 10
 #define PA_MAX_ORDER 8
 #define PA_MAX_DRAFTS 64   /* drafted tokens per row of one step */
 #define PA_MAX_MOVES 128   /* array pairs of one pa_draft_commit */
 #define PA_TICKET_STRIDE 32  /* int32 per row of its tickets */
+#define PA_MAX_PAGE_ROWS 8192  /* rows of a page table */
 
 /* status codes (0 = success, negative = failure) */
 #define PA_OK            0
@@ -479,14 +480,115 @@ typedef struct pa_commit {
     pa_draft_move  moves[PA_MAX_MOVES];
 } pa_commit;
 
+/* ---- paged cache (no counterpart in the reference) -----------------------------------------
+ * The cached positions of `rows` rows lie in pages of `page_size` positions (a power of two, 16 to
+ * 4096) of one pool: position p of row b is place p % page_size of page
+ * table[b * max_pages + p / page_size].  An array of the cache is [pages, heads, page_size, dim]
+ * (logsumexps fp32 [pages, heads, page_size]), contiguous; all arrays of all layers share the table.
+ * counts[b] is a row's number of positions (at most max_pages * page_size, which is at most 2^30), of
+ * which the last fresh[b] are those of its chunk: the new tokens of the step.  refs[p] is the number of
+ * table entries that name page p; 0: the page is free.  Entries behind a row's pages are -1.
+ * The calls keep all of this; a page number outside the pool is never followed: reads give 0 and
+ * writes are dropped.  One call at a time may use a table. */
+typedef struct pa_page_table {
+    int32_t  rows, pages, page_size, max_pages;
+    int32_t* table;     /* device [rows, max_pages] */
+    int32_t* counts;    /* device [rows] */
+    int32_t* refs;      /* device [pages] */
+    int32_t* fresh;     /* device [rows] */
+    int32_t* starts;    /* device [rows + 1]: a chunk's first token where the chunks are packed */
+    int32_t* overflow;  /* device [1], or NULL: set to 1 when a row gets no pages */
+    int32_t* scratch;   /* device [pa_page_scratch bytes]: contents do not matter between calls */
+} pa_page_table;
+
+/* An array whose pages move: [pages, heads, page_size, row_bytes]; row_bytes 4 or a multiple of 16 (16-byte
+ * aligned then). */
+typedef struct pa_page_array {
+    void*   base;
+    int32_t heads, row_bytes;
+} pa_page_array;
+
+/* pa_page_select: row b becomes the first lengths[b] positions (all of them without lengths, and at most
+ * what there is) of what row index[b] was; any index outside [0, rows): an empty row.  All rows at
+ * once: index may repeat rows and permute them.  Pages are shared, not copied; fresh becomes 0.
+ * pa_page_extend: more[b] further positions for every row, as the chunk of the next step: fresh[b] and
+ * counts[b].  Pages are the free ones, lowest first, in the order of the rows; where the row's last
+ * page is partly filled and shared, the row first gets a copy of it (of the positions that it holds, in
+ * every array), and the last of the rows that write such a page keeps it.  A row whose pages are not
+ * to be had, or past max_pages, gets none of its positions (fresh 0, overflow set); rows behind it that
+ * need no page are not affected.  starts are the running sums of more (below 0: 0), granted or not.
+ * pa_page_compact: the pages in use become the first ones of the pool, those that lie there already
+ * unmoved, the others in their order into the free places in their order. */
+typedef struct pa_page_call {
+    pa_page_table        t;
+    const int32_t*       index;    /* select: device [rows] */
+    const int32_t*       lengths;  /* select: device [rows], or NULL */
+    const int32_t*       more;     /* extend: device [rows] */
+    const pa_page_array* arrays;   /* extend, compact: device [count] */
+    int32_t              count;
+} pa_page_call;
+
+/* The q RMSNorms and the rotary embedding of the chunks' tokens, into the rows' pages:
+ *   y = round(rotate(x * rsqrt(mean(x^2) + eps) * w))
+ * as pa_draft_append, at the tokens' positions counts[b] - fresh[b] + i.  `tokens` per row, or packed: in
+ * all, token starts[b] + i of a row of batch stride 0.  Tokens behind a chunk are not written to pages;
+ * out (the first item's) is 0 there. */
+typedef struct pa_page_item {
+    pa_view     src;            /* [rows or 1, heads, tokens, dim] */
+    const void* norm_weight;    /* [dim], or NULL: no normalisation */
+    int32_t     weight_dtype;
+    int32_t     rotate;
+    pa_view     out;            /* [rows or 1, heads, tokens, dim], or no ptr: pages */
+    void*       pages;          /* [pages, heads, page_size, dim] */
+} pa_page_item;
+typedef struct pa_page_rows {
+    pa_page_table t;
+    int32_t       tokens, packed, dim, count;
+    float         eps;
+    const void*   angles;       /* or NULL */
+    int32_t       angles_dtype;
+    int32_t       rot_dim;
+    int64_t       angles_sb, angles_sn;
+    const float*  inv_freq;     /* [rot_dim / 2], or NULL */
+    float         interp;
+    pa_page_item  items[PA_MAX_ORDER + 2];
+} pa_page_rows;
+
+/* One level of pa_paged_attend, the deepest first. */
+typedef struct pa_paged_level {
+    void*   keys;               /* [pages, kv_heads, page_size, dim] */
+    void*   values;             /* the same; written by the level below, except at the deepest */
+    float*  lses;               /* fp32 [pages, kv_heads, page_size], written (not at the final level) */
+    pa_view vmul;               /* middle levels: [rows or 1, kv_heads, tokens, dim], the tokens' projected values */
+} pa_paged_level;
+
+/* Every level of an order-`order` poly attention for the chunks' tokens: token i of row b at
+ * position p = counts[b] - fresh[b] + i, level t with queries keys[t + 1] (q at the final level):
+ *   s_j = softclamp(scale <query, keys[t]_j>) + lses[t - 1]_j     j = 0 .. p
+ *   o = sum_j softmax_j(s) values[t]_j,   lses[t]_p = logsumexp_j(s)
+ *   values[t + 1]_p = round(o * vmul[t + 1])  where level t + 1 is a middle one, else round(o)
+ * and the final o goes to out.  What a level leaves in the cache is what the next one reads, so that
+ * results do not depend on how a row's tokens were cut into chunks beyond the rounding of sums.  Sums,
+ * maxima and logsumexps are fp32.  out is 0 for tokens behind their chunk. */
+typedef struct pa_paged {
+    pa_page_table  t;
+    int32_t        tokens, packed, heads, kv_heads, dim, order, dtype;
+    float          scale, softclamp;
+    pa_view        q, out;      /* [rows or 1, heads, tokens, dim] */
+    pa_paged_level levels[PA_MAX_ORDER];
+    void*          workspace;
+    size_t         workspace_bytes;
+} pa_paged;
+
 int         pa_abi_version(void);
 const char* pa_strerror(int status);
 int         pa_last_hip_error(void);   /* hipError_t of the last PA_EHIP on this thread */
 /* sizeof of the ABI structs, for binding checks: 0 pa_view, 1 pa_mask, 2 pa_pass,
  * 3 pa_pass_grad, 4 pa_decode_level, 5 pa_decode, 6 pa_prologue_item, 7 pa_prologue,
  * 8 pa_rmsnorm, 9 pa_linear, 10 pa_linear_out, 11 pa_epilogue, 12 pa_qk_norm, 13 pa_draft_level,
- * 14 pa_draft, 15 pa_draft_item, 16 pa_draft_rows, 17 pa_verify, 18 pa_draft_move, 19 pa_commit;
- * 0 for other values */
+ * 14 pa_draft, 15 pa_draft_item, 16 pa_draft_rows, 17 pa_verify, 18 pa_draft_move, 19 pa_commit,
+ * 20 pa_page_table, 21 pa_page_array, 22 pa_page_call, 23 pa_page_item, 24 pa_page_rows,
+ * 25 pa_paged_level, 26 pa_paged; 0 for other values */
 size_t      pa_struct_size(int which);
 
 /* Kernel timing (no counterpart in the reference: a measurement facility for benchmarks).
@@ -566,6 +668,15 @@ int    pa_draft_attend(const pa_draft* d, void* stream);
 size_t pa_draft_verify_workspace(const pa_verify* v);
 int    pa_draft_verify(const pa_verify* v, void* stream);
 int    pa_draft_commit(const pa_commit* c, void* stream);
+
+/* The paged cache: the table's calls (per step of a model), append and attend (per layer). */
+size_t pa_page_scratch(const pa_page_table* t);
+int    pa_page_select(const pa_page_call* c, void* stream);
+int    pa_page_extend(const pa_page_call* c, void* stream);
+int    pa_page_compact(const pa_page_call* c, void* stream);
+int    pa_page_append(const pa_page_rows* r, void* stream);
+size_t pa_paged_attend_workspace(const pa_paged* p);
+int    pa_paged_attend(const pa_paged* p, void* stream);
 
 #ifdef __cplusplus
 }

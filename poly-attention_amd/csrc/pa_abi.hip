@@ -274,6 +274,13 @@ size_t pa_struct_size(int which) {
         case 17: return sizeof(pa_verify);
         case 18: return sizeof(pa_draft_move);
         case 19: return sizeof(pa_commit);
+        case 20: return sizeof(pa_page_table);
+        case 21: return sizeof(pa_page_array);
+        case 22: return sizeof(pa_page_call);
+        case 23: return sizeof(pa_page_item);
+        case 24: return sizeof(pa_page_rows);
+        case 25: return sizeof(pa_paged_level);
+        case 26: return sizeof(pa_paged);
         default: return 0;
     }
 }
@@ -721,6 +728,45 @@ int pa_draft_commit(const pa_commit* x, void* stream) {
     if (st != PA_OK) return st;
     return finish_launch();
 }
+
+int pa_page_select(const pa_page_call* x, void* stream) {
+    if (!x) return PA_EINVAL;
+    const int st = launch_page_select(x, static_cast<hipStream_t>(stream));
+    if (st != PA_OK) return st;
+    return finish_launch();
+}
+
+int pa_page_extend(const pa_page_call* x, void* stream) {
+    if (!x) return PA_EINVAL;
+    const int st = launch_page_extend(x, static_cast<hipStream_t>(stream));
+    if (st != PA_OK) return st;
+    return finish_launch();
+}
+
+int pa_page_compact(const pa_page_call* x, void* stream) {
+    if (!x) return PA_EINVAL;
+    const int st = launch_page_compact(x, static_cast<hipStream_t>(stream));
+    if (st != PA_OK) return st;
+    return finish_launch();
+}
+
+int pa_page_append(const pa_page_rows* x, void* stream) {
+    if (!x) return PA_EINVAL;
+    const int st = launch_page_append(x, static_cast<hipStream_t>(stream));
+    if (st != PA_OK) return st;
+    return finish_launch();
+}
+
+int pa_paged_attend(const pa_paged* x, void* stream) {
+    if (!x) return PA_EINVAL;
+    const int st = launch_paged_attend(x, static_cast<hipStream_t>(stream));
+    if (st != PA_OK) return st;
+    return finish_launch();
+}
+
+size_t pa_page_scratch(const pa_page_table* t) { return t ? page_scratch(t) : 0; }
+
+size_t pa_paged_attend_workspace(const pa_paged* p) { return p ? paged_attend_workspace(p) : 0; }
 
 size_t pa_draft_attend_workspace(const pa_draft* d) { return d ? draft_attend_workspace(d) : 0; }
 

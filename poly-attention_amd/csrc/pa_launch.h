@@ -83,6 +83,14 @@ int launch_draft_append(const pa_draft_rows* r, hipStream_t s);
 int launch_draft_commit(const pa_commit* c, hipStream_t s);
 size_t draft_verify_workspace(const pa_verify* v);
 int launch_draft_verify(const pa_verify* v, hipStream_t s);
+// paged cache
+size_t page_scratch(const pa_page_table* t);
+int launch_page_select(const pa_page_call* c, hipStream_t s);
+int launch_page_extend(const pa_page_call* c, hipStream_t s);
+int launch_page_compact(const pa_page_call* c, hipStream_t s);
+int launch_page_append(const pa_page_rows* r, hipStream_t s);
+size_t paged_attend_workspace(const pa_paged* p);
+int launch_paged_attend(const pa_paged* p, hipStream_t s);
 int launch_linear_small(const pa_linear* l, hipStream_t s);
 int launch_linear_rows(const pa_linear* l, hipStream_t s);
 

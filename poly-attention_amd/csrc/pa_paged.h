@@ -1,0 +1,295 @@
+// pa_paged.h -- attention of chunks of new tokens over a paged cache: what its kernels share.
+//
+// A level's query rows of one key head are its new tokens, at the final level times the query heads of
+// the group: row r of a chunk is token r / rep, head r % rep, so that a tile of rows covers few positions
+// and its causal ends lie together.  A tile's keys are the row's positions up to its last token; they are
+// split into units of `size` chunks of 128 positions where there are few tiles.  The rows' counts are known
+// on the device only: every workgroup finds its unit from them (a scan over the rows by a wave), and the
+// grid is the most units there can be.  A tile of one unit is finished where it is computed; the others
+// leave records (maximum, sum, weighted values) that k_paged_join joins.  The levels follow one another,
+// as each reads what the one below left in the cache.
+#pragma once
+
+#include "pa_draft_partial.h"
+#include "pa_page.h"
+
+namespace pa {
+
+constexpr int kPagedChunk = 128;
+constexpr int kPagedMost = (1 << 30) / kPagedChunk;  // chunks of a row, at most
+
+struct PagedDev {
+    PageDev p;
+    int32_t kv_heads, dim, rep;
+    int32_t last;              // the final level: queries from q, results to out
+    int32_t over, most;        // rows of a chunk, more than `over` and at most `most`, that a launch takes
+    int32_t tile;              // rows of its tiles
+    int32_t target;            // units aimed at over all rows ...
+    int32_t target_min, least; // ... or this many, where units are smaller than this many chunks
+    int64_t recs;              // records there are
+    float scale, softclamp;
+    DraftRow q, out, vmul;     // of the inputs; vmul: the next level's projected values, where it is a middle one
+    const char* keys;
+    const char* values;
+    const float* bias;         // the logsumexps of the level below, or null
+    const char* queries;       // not at the final level: the next level's keys, new tokens' queries
+    char* next;                // the next level's values
+    float* lses;
+    float* ws_o;               // [record][kv head][tile][dim]
+    float2* ws_s;              // [record][kv head][tile]: maximum (log2 units) and sum
+};
+
+__device__ __forceinline__ int64_t paged_base(const PagedDev& P, int id, int hk) {  // in positions
+    return ((int64_t)id * P.kv_heads + hk) << P.p.lg;
+}
+
+struct PagedUnit {
+    PageRow row;
+    int b, rows;         // the batch row, its query rows per key head
+    int tiles, tile;     // of the row, and the one asked for
+    int splits, split;   // units of a tile, and the one asked for
+    int size;            // chunks of a unit
+    int64_t rec;         // the record of the tile's first unit (splits > 1)
+    int at;              // what was asked for, from the row's first
+};
+
+// chunks per unit for a batch of `total` tiles times chunks
+__device__ __forceinline__ int paged_size(const PagedDev& P, uint64_t total) {
+    const uint64_t many = (total + P.target - 1) / P.target, few = (total + P.target_min - 1) / P.target_min;
+    const uint64_t s = max(many, min(few, (uint64_t)P.least));
+    return (int)min(max<uint64_t>(s, 1), (uint64_t)kPagedMost);
+}
+
+// One row's tiles and chunks, 0 for a row that the launch does not take.
+__device__ __forceinline__ void paged_tiles(const PagedDev& P, const PageRow& r, int& rows, int& tiles, int& chunks) {
+    rows = r.len * P.rep;
+    tiles = rows > P.over && rows <= P.most ? (rows + P.tile - 1) / P.tile : 0;
+    chunks = (r.n + kPagedChunk - 1) / kPagedChunk;
+}
+
+// What a row has of the things that are counted: kUnits, the records of its units, or (kRows) the query rows of tiles
+// that are to be joined.
+enum { kUnits, kRows };
+
+// Finds unit (or row) `want` over all rows of the batch, by the whole wave; false past the last one.
+template <int WHAT>
+__device__ __forceinline__ bool paged_find(const PagedDev& P, int64_t want, int lane, PagedUnit& U) {
+    uint64_t total = 0;
+    PageRow r0;
+    int rows0 = 0, tiles0 = 0, chunks0 = 0;  // this lane's row of the first 64
+    for (int b = lane; b < P.p.rows; b += 64) {
+        const PageRow r = page_row(P.p, b);
+        int rows, tiles, chunks;
+        paged_tiles(P, r, rows, tiles, chunks);
+        total += (uint64_t)tiles * chunks;
+        if (b < 64) {
+            r0 = r;
+            rows0 = rows;
+            tiles0 = tiles;
+            chunks0 = chunks;
+        }
+    }
+    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor((unsigned long long)total, off);
+    U.size = paged_size(P, total);
+    int64_t before = 0, recs = 0;
+    for (int b0 = 0; b0 < P.p.rows; b0 += 64) {
+        const int b = b0 + lane;
+        PageRow r = r0;
+        int rows = rows0, tiles = tiles0, chunks = chunks0;
+        if (b0 > 0) {
+            tiles = 0;
+            chunks = 0;
+            rows = 0;
+            if (b < P.p.rows) {
+                r = page_row(P.p, b);
+                paged_tiles(P, r, rows, tiles, chunks);
+            }
+        }
+        const int splits = (int)(((unsigned)chunks + U.size - 1) / U.size);
+        const int units = tiles * splits, rec = splits > 1 ? units : 0;
+        const int mine = WHAT == kUnits ? units : splits > 1 && tiles > 0 ? rows : 0;
+        int64_t incl = mine, incl_rec = rec;
+        for (int off = 1; off < 64; off <<= 1) {
+            const int64_t x = __shfl_up(incl, off), y = __shfl_up(incl_rec, off);
+            if (lane >= off) {
+                incl += x;
+                incl_rec += y;
+            }
+        }
+        const uint64_t past = __ballot(before + incl > want);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            U.b = __builtin_amdgcn_readfirstlane(b0 + l);
+            U.row.n = __builtin_amdgcn_readlane(r.n, l);
+            U.row.p0 = __builtin_amdgcn_readlane(r.p0, l);
+            U.row.len = __builtin_amdgcn_readlane(r.len, l);
+            U.row.start = __builtin_amdgcn_readlane(r.start, l);
+            U.rows = __builtin_amdgcn_readlane(rows, l);
+            U.tiles = __builtin_amdgcn_readlane(tiles, l);
+            U.splits = __builtin_amdgcn_readlane(splits, l);
+            U.rec = recs + __shfl(incl_rec - rec, l);
+            U.at = __builtin_amdgcn_readfirstlane((int)(want - before - __shfl(incl - mine, l)));
+            if (WHAT == kUnits) {
+                // the last tiles, which have most keys, first
+                const int t = U.at / U.splits;
+                U.split = U.at - t * U.splits;
+                U.tile = U.tiles - 1 - t;
+            } else {
+                U.tile = U.at / P.tile;
+                U.split = 0;
+            }
+            U.rec += (int64_t)U.tile * U.splits;
+            return true;
+        }
+        before += __shfl(incl, 63);
+        recs += __shfl(incl_rec, 63);
+    }
+    return false;
+}
+
+// the positions that a tile's last token sees
+__device__ __forceinline__ int paged_keys(const PagedDev& P, const PagedUnit& U) {
+    return U.row.p0 + (min((U.tile + 1) * P.tile, U.rows) - 1) / P.rep + 1;
+}
+
+// Where a query row's results go.
+struct PagedTo {
+    char* out;        // its features
+    const char* mul;  // or null
+    float* lse;       // or null
+};
+template <typename T>
+__device__ __forceinline__ PagedTo paged_to(const PagedDev& P, const PagedUnit& U, int hk, int r) {
+    PagedTo to = {nullptr, nullptr, nullptr};
+    const int i = r / P.rep, src_b = P.p.packed ? 0 : U.b, tok = U.row.start + i;
+    if (P.last) {
+        to.out = reinterpret_cast<char*>(P.out.at<T>(src_b, hk * P.rep + r - i * P.rep) + (int64_t)tok * P.out.sn);
+        return to;
+    }
+    const int64_t place = page_place(P.p, U.b, U.row.p0 + i);
+    if (place < 0) return to;
+    const int64_t at = paged_base(P, (int)(place >> P.p.lg), hk) + (place & ((1 << P.p.lg) - 1));
+    to.out = P.next + at * P.dim * (int64_t)sizeof(T);
+    to.lse = P.lses + at;
+    if (P.vmul.p) to.mul = reinterpret_cast<const char*>(P.vmul.at<T>(src_b, hk) + (int64_t)tok * P.vmul.sn);
+    return to;
+}
+
+// four features of a result
+template <typename T>
+__device__ __forceinline__ void paged_store(const PagedTo& to, int d, float4 y) {
+    if constexpr (sizeof(T) == 4) {
+        if (to.mul) {
+            const float4 m = *reinterpret_cast<const float4*>(to.mul + 4 * d);
+            y = make_float4(y.x * m.x, y.y * m.y, y.z * m.z, y.w * m.w);
+        }
+        *reinterpret_cast<float4*>(to.out + 4 * d) = y;
+    } else {
+        if (to.mul) {
+            typedef T t4 __attribute__((ext_vector_type(4)));
+            const t4 m = *reinterpret_cast<const t4*>(to.mul + 2 * d);
+            y = make_float4(y.x * (float)m[0], y.y * (float)m[1], y.z * (float)m[2], y.w * (float)m[3]);
+        }
+        u32x2_d w;
+        w[0] = draft_pack2<T>(y.x, y.y);
+        w[1] = draft_pack2<T>(y.z, y.w);
+        *reinterpret_cast<u32x2_d*>(to.out + 2 * d) = w;
+    }
+}
+
+// The first features of query row r: q at the final level, else the next level's keys at its position; null for
+// a page outside the pool.
+template <typename T>
+__device__ __forceinline__ const T* paged_query(const PagedDev& P, const PagedUnit& U, int hk, int r) {
+    const int i = r / P.rep;
+    if (P.last)
+        return P.q.at<T>(P.p.packed ? 0 : U.b, hk * P.rep + r - i * P.rep) + (int64_t)(U.row.start + i) * P.q.sn;
+    const int64_t place = page_place(P.p, U.b, U.row.p0 + i);
+    if (place < 0) return nullptr;
+    const int64_t at = paged_base(P, (int)(place >> P.p.lg), hk) + (place & ((1 << P.p.lg) - 1));
+    return reinterpret_cast<const T*>(P.queries) + at * P.dim;
+}
+
+// Whether a word of two 16-bit (or one 32-bit) numbers holds one that is not finite.
+template <typename T>
+__device__ __forceinline__ bool paged_odd(uint32_t w) {
+    if constexpr (sizeof(T) == 4) return (w & 0x7f800000u) == 0x7f800000u;
+    constexpr uint32_t e = std::is_same_v<T, f16> ? 0x7c00u : 0x7f80u;
+    return (w & e) == e || (w & (e << 16)) == e << 16;
+}
+
+// A unit's rows one after another, a wave each, position by position in fp32: the products of the matrix
+// instructions include a weight of 0 times the value of a position that a row does not see, which is no number where
+// the value is none.  Taken where such values lie behind a row's own position; 64 positions at a time, a
+// lane's score each, then a lane's features.
+template <typename T>
+__device__ __forceinline__ void paged_slow(const PagedDev& P, const PagedUnit& U, int hk, int begin, int cnt, int wave,
+                                                     int waves, int lane) {
+    const int r0 = U.tile * P.tile, nrows = min(P.tile, U.rows - r0);
+    for (int r = r0 + wave; r < r0 + nrows; r += waves) {
+        const T* const q = paged_query<T>(P, U, hk, r);
+        const int see = min(cnt, U.row.p0 + r / P.rep + 1 - begin);
+        float top = -INFINITY, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};  // features lane + 64 i
+        for (int j0 = 0; j0 < see; j0 += 64) {
+            const int j = min(j0 + lane, see - 1);
+            const int64_t place = page_place(P.p, U.b, begin + j);
+            int64_t at = -1;
+            float s = 0.f;
+            if (place >= 0) {
+                at = paged_base(P, (int)(place >> P.p.lg), hk) + (place & ((1 << P.p.lg) - 1));
+                const T* const k = reinterpret_cast<const T*>(P.keys) + at * P.dim;
+                if (q)
+                    for (int d = 0; d < P.dim; ++d) s = fmaf(to_f(q[d]), to_f(k[d]), s);
+            }
+            s *= P.scale;
+            if (P.softclamp > 0.f) s = P.softclamp * tanhf(s / P.softclamp);
+            if (P.bias && at >= 0) s += P.bias[at];
+            s = j0 + lane < see ? s * kLog2e : -INFINITY;
+            float t = fmaxf(top, s);
+            for (int off = 32; off > 0; off >>= 1) t = fmaxf(t, __shfl_xor(t, off));
+            const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t);
+            top = t;
+            const float w = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - (t == -INFINITY ? 0.f : t));
+            float add = w;
+            for (int off = 32; off > 0; off >>= 1) add += __shfl_xor(add, off);
+            sum = sum * f + add;
+            for (int i = 0; i < 4; ++i) y[i] *= f;
+            for (int k = 0; k < 64; ++k) {
+                const float wk = __shfl(w, k);
+                const int64_t ak = __shfl(at, k);
+                if (wk == 0.f || ak < 0) continue;
+                const T* const v = reinterpret_cast<const T*>(P.values) + ak * P.dim;
+                for (int i = 0; i < 4; ++i)
+                    if (lane + 64 * i < P.dim) y[i] = fmaf(wk, to_f(v[lane + 64 * i]), y[i]);
+            }
+        }
+        if (U.splits > 1) {
+            const int64_t rec = ((U.rec + U.split) * P.kv_heads + hk) * P.tile + r - r0;
+            if (lane == 0) P.ws_s[rec] = make_float2(top, sum);
+            for (int i = 0; i < 4; ++i)
+                if (lane + 64 * i < P.dim) P.ws_o[rec * P.dim + lane + 64 * i] = y[i];
+        } else {
+            const PagedTo to = paged_to<T>(P, U, hk, r);
+            if (lane == 0 && to.lse) *to.lse = (top + log2f(sum)) * kLn2;
+            for (int i = 0; i < 4; ++i)
+                if (to.out && lane + 64 * i < P.dim) {
+                    float x = y[i] / sum;
+                    if (to.mul) x *= to_f(reinterpret_cast<const T*>(to.mul)[lane + 64 * i]);
+                    reinterpret_cast<T*>(to.out)[lane + 64 * i] = from_f<T>(x);
+                }
+        }
+    }
+}
+
+// 16-row tiles of the workgroup's rows: what its registers hold
+template <typename T> constexpr int paged_row_tiles(int D) { return D > 128 ? 1 : 2; }
+// Waves per SIMD that the registers are held to
+constexpr int paged_waves(int D, int RT) { return D <= 128 && D * RT <= 256 ? 2 : 1; }
+
+template <typename T> void launch_paged_rows(const PagedDev& P, int64_t units, int tiles, hipStream_t s);
+// in source files of their own
+extern template void launch_paged_rows<bf16>(const PagedDev& P, int64_t units, int tiles, hipStream_t s);
+extern template void launch_paged_rows<f16>(const PagedDev& P, int64_t units, int tiles, hipStream_t s);
+extern template void launch_paged_rows<float>(const PagedDev& P, int64_t units, int tiles, hipStream_t s);
+
+}  // namespace pa

@@ -1,0 +1,6 @@
+// pa_paged_f16.hip -- attention over a paged cache, f16.
+#include "pa_paged_rows.h"
+
+namespace pa {
+template void launch_paged_rows<f16>(const PagedDev& P, int64_t units, int tiles, hipStream_t s);
+}  // namespace pa

@@ -15,5 +15,6 @@ from poly_attention.poly_vit import PolyViT  # noqa: E402
 from poly_attention.poly_transformer import PolyTransformer  # noqa: E402
 from poly_attention._cache import StaticCache  # noqa: E402
 from poly_attention.drafts import DraftCache, commit_drafts, verify_drafts  # noqa: E402
+from poly_attention.pages import PagedCache, PageTable  # noqa: E402
 
 __version__ = "0.3.6"

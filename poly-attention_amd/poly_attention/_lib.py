@@ -16,11 +16,12 @@ import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libpolyattn.so"
 
-PA_ABI_VERSION = 9
+PA_ABI_VERSION = 10
 PA_MAX_ORDER = 8
 PA_MAX_DRAFTS = 64
 PA_MAX_MOVES = 128
 PA_TICKET_STRIDE = 32
+PA_MAX_PAGE_ROWS = 8192
 
 PA_OK = 0
 PA_EINVAL = -1
@@ -76,6 +77,13 @@ EXPORTED_SYMBOLS = (
     "pa_draft_verify_workspace",
     "pa_draft_verify",
     "pa_draft_commit",
+    "pa_page_scratch",
+    "pa_page_select",
+    "pa_page_extend",
+    "pa_page_compact",
+    "pa_page_append",
+    "pa_paged_attend_workspace",
+    "pa_paged_attend",
 )
 
 
@@ -377,13 +385,99 @@ class PaCommit(ctypes.Structure):
     ]
 
 
+class PaPageTable(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int32),
+        ("pages", c_int32),
+        ("page_size", c_int32),
+        ("max_pages", c_int32),
+        ("table", c_void_p),
+        ("counts", c_void_p),
+        ("refs", c_void_p),
+        ("fresh", c_void_p),
+        ("starts", c_void_p),
+        ("overflow", c_void_p),
+        ("scratch", c_void_p),
+    ]
+
+
+class PaPageArray(ctypes.Structure):
+    _fields_ = [("base", c_void_p), ("heads", c_int32), ("row_bytes", c_int32)]
+
+
+class PaPageCall(ctypes.Structure):
+    _fields_ = [
+        ("t", PaPageTable),
+        ("index", c_void_p),
+        ("lengths", c_void_p),
+        ("more", c_void_p),
+        ("arrays", c_void_p),
+        ("count", c_int32),
+    ]
+
+
+class PaPageItem(ctypes.Structure):
+    _fields_ = [
+        ("src", PaView),
+        ("norm_weight", c_void_p),
+        ("weight_dtype", c_int32),
+        ("rotate", c_int32),
+        ("out", PaView),
+        ("pages", c_void_p),
+    ]
+
+
+class PaPageRows(ctypes.Structure):
+    _fields_ = [
+        ("t", PaPageTable),
+        ("tokens", c_int32),
+        ("packed", c_int32),
+        ("dim", c_int32),
+        ("count", c_int32),
+        ("eps", c_float),
+        ("angles", c_void_p),
+        ("angles_dtype", c_int32),
+        ("rot_dim", c_int32),
+        ("angles_sb", c_int64),
+        ("angles_sn", c_int64),
+        ("inv_freq", c_void_p),
+        ("interp", c_float),
+        ("items", PaPageItem * (PA_MAX_ORDER + 2)),
+    ]
+
+
+class PaPagedLevel(ctypes.Structure):
+    _fields_ = [("keys", c_void_p), ("values", c_void_p), ("lses", c_void_p), ("vmul", PaView)]
+
+
+class PaPaged(ctypes.Structure):
+    _fields_ = [
+        ("t", PaPageTable),
+        ("tokens", c_int32),
+        ("packed", c_int32),
+        ("heads", c_int32),
+        ("kv_heads", c_int32),
+        ("dim", c_int32),
+        ("order", c_int32),
+        ("dtype", c_int32),
+        ("scale", c_float),
+        ("softclamp", c_float),
+        ("q", PaView),
+        ("out", PaView),
+        ("levels", PaPagedLevel * PA_MAX_ORDER),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_size_t),
+    ]
+
+
 class PaKernelTime(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("launches", c_int64), ("total_ms", ctypes.c_double)]
 
 
 STRUCTS = (PaView, PaMask, PaPass, PaPassGrad, PaDecodeLevel, PaDecode, PaPrologueItem,
            PaPrologue, PaRmsNorm, PaLinear, PaLinearOut, PaEpilogue, PaQkNorm,
-           PaDraftLevel, PaDraft, PaDraftItem, PaDraftRows, PaVerify, PaDraftMove, PaCommit)
+           PaDraftLevel, PaDraft, PaDraftItem, PaDraftRows, PaVerify, PaDraftMove, PaCommit,
+           PaPageTable, PaPageArray, PaPageCall, PaPageItem, PaPageRows, PaPagedLevel, PaPaged)
 
 
 # The hot structs as one struct.pack each (assigning ctypes fields one by one was half of a pass's
@@ -476,6 +570,17 @@ def _configure(lib) -> None:
     lib.pa_draft_verify.argtypes = [c_void_p, c_void_p]  # packed structures
     lib.pa_draft_commit.restype = c_int
     lib.pa_draft_commit.argtypes = [c_void_p, c_void_p]
+    lib.pa_page_scratch.restype = c_size_t
+    lib.pa_page_scratch.argtypes = [ctypes.POINTER(PaPageTable)]
+    for call in (lib.pa_page_select, lib.pa_page_extend, lib.pa_page_compact):
+        call.restype = c_int
+        call.argtypes = [ctypes.POINTER(PaPageCall), c_void_p]
+    lib.pa_page_append.restype = c_int
+    lib.pa_page_append.argtypes = [ctypes.POINTER(PaPageRows), c_void_p]
+    lib.pa_paged_attend_workspace.restype = c_size_t
+    lib.pa_paged_attend_workspace.argtypes = [ctypes.POINTER(PaPaged)]
+    lib.pa_paged_attend.restype = c_int
+    lib.pa_paged_attend.argtypes = [ctypes.POINTER(PaPaged), c_void_p]
     lib.pa_linear_small.restype = c_int
     lib.pa_linear_small.argtypes = [ctypes.POINTER(PaLinear), c_void_p]
 

@@ -31,7 +31,8 @@ from ._helpers import (
     where_queries,
 )
 from .drafts import DraftCache
-from .poly_attention import (_DECODE_ROWS, _compute_dtype, _draft_step, _module_angles, _q_norms,
+from .pages import PagedCache
+from .poly_attention import (_DECODE_ROWS, _compute_dtype, _draft_step, _module_angles, _paged_step, _q_norms,
                              _static_decode_step, fused_available)
 from .rotary import RotaryEmbedding, apply_rotary_emb
 
@@ -146,13 +147,14 @@ class NPolyAttention(Module):
     def forward(self, x, context: Tensor | tuple[Tensor, ...] | None = None, mask=None,
                 context_mask: Tensor | tuple[Tensor | None, ...] | None = None,
                 rotary_pos_emb=None, cache=None, return_cache=False, parents=None):
-        """``parents``: the tree of the drafted tokens ``x`` (with a DraftCache; see drafts.py)."""
+        """``parents``: the tree of the drafted tokens ``x`` (with a DraftCache; see drafts.py).  With a
+        PagedCache ``x`` is a step's chunks of new tokens, padded or packed (see pages.py)."""
         seq_len, device = x.shape[-2], x.device
 
         has_cache = exists(cache)
-        drafted = isinstance(cache, DraftCache)
+        drafted, paged = isinstance(cache, DraftCache), isinstance(cache, PagedCache)
         assert drafted or not exists(parents), "parents describe drafted tokens: pass a DraftCache"
-        if has_cache and not drafted:
+        if has_cache and not (drafted or paged):
             assert seq_len == 1, "sequence length must be 1 when using kv cache"
 
         orig_x = x
@@ -220,9 +222,9 @@ class NPolyAttention(Module):
                     gates if self.attn_gate else None, self.use_root_value_as_attn_gate)
         epilogue_done = False
 
-        if drafted or isinstance(cache, _cache.StaticCache):
+        if drafted or paged or isinstance(cache, _cache.StaticCache):
             # fixed-capacity cache: norms, rotary and appends fused into the decode step
-            step = _static_decode_step
+            step = _paged_step if paged else _static_decode_step
             if drafted:
                 step = partial(_draft_step, parents=parents)
             out = step(self, qs, vs_for_aggregation, mask, context_mask, rotary_pos_emb,

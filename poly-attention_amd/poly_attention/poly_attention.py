@@ -20,6 +20,7 @@ from einops.layers.torch import Rearrange
 
 from . import _cache, _lib
 from .drafts import DraftCache
+from .pages import PagedCache
 from ._helpers import (
     add_key_bias,
     cast_tuple,
@@ -230,6 +231,16 @@ def _draft_step(module, qs, vs, mask, context_mask, rotary_pos_emb, cache: Draft
         raise NotImplementedError("masks are not supported with a DraftCache: rows hold their own counts")
     if cache.order != len(qs) - 1:
         raise ValueError(f"DraftCache of order {cache.order} passed to an order-{len(qs) - 1} module")
+    if not exists(rotary_pos_emb) and exists(module.rotary_emb):
+        cache.rotate_prefix(module.rotary_emb)
+    weights, kwargs = _step_norms(module, q1, rotary_pos_emb, lambda: cache.positions(q1.shape[-2], parents))
+    q1 = cache.append(qs, vs, weights, parents=parents, **kwargs)
+    return cache.attend(q1, parents=parents, scale=module.scale, softclamp=module.softclamp_value)
+
+
+def _step_norms(module, q1, rotary_pos_emb, positions):
+    """The norm weights and the eps and rotary arguments of a DraftCache's or a PagedCache's append, for a step of
+    q1's tokens at ``positions()``."""
     norms = list(module.q_norms)
     if len({n.eps for n in norms}) != 1:
         raise NotImplementedError("q norms with different eps")
@@ -238,7 +249,7 @@ def _draft_step(module, qs, vs, mask, context_mask, rotary_pos_emb, cache: Draft
         eps = torch.finfo(torch.float32).eps
     weights = [n.weight if n.weight is not None else torch.ones(q1.shape[-1], device=q1.device)
                for n in norms]
-    kwargs = {}
+    kwargs = {"eps": eps}
     if exists(rotary_pos_emb):
         # a table of more positions is read from its end, as apply_rotary_emb does
         T = q1.shape[-2]
@@ -247,14 +258,30 @@ def _draft_step(module, qs, vs, mask, context_mask, rotary_pos_emb, cache: Draft
         # a module's own rotary (poly_attention.py:302-304, n_poly_attention.py:224-229): the cache
         # holds its keys rotated, as a StaticCache does
         rot = module.rotary_emb
-        cache.rotate_prefix(rot)
         if type(rot) is RotaryEmbedding and rot.freqs.dtype == torch.float32:
             kwargs["inv_freq"], kwargs["interp"] = rot.freqs, rot.interpolate_factor
         else:  # frequencies of 16 bits (a layer cast whole) give angles of 16 bits, to the cached keys too
-            pos = cache.positions(q1.shape[-2], parents).to(q1.dtype) / rot.interpolate_factor
-            kwargs["angles"] = rot(pos).detach()
-    q1 = cache.append(qs, vs, weights, eps=eps, parents=parents, **kwargs)
-    return cache.attend(q1, parents=parents, scale=module.scale, softclamp=module.softclamp_value)
+            kwargs["angles"] = rot(positions().to(q1.dtype) / rot.interpolate_factor).detach()
+    return weights, kwargs
+
+
+def _paged_step(module, qs, vs, mask, context_mask, rotary_pos_emb, cache: PagedCache) -> Tensor:
+    """A step over chunks of new tokens on a PagedCache, for both module orders: the norms and the rotary into the
+    rows' pages, then every level of the attention.  ``qs`` = (q1, ..., q_{order+1}) are the raw projections
+    [rows, h, T, d] (or packed [1, h, total, d]), ``vs`` the aggregation values.  Returns the output like q1."""
+    q1 = qs[0]
+    if not (module.use_flash_kernel and q1.is_cuda):
+        raise RuntimeError("a PagedCache needs the fused GPU path (libpolyattn)")
+    _lib.load()
+    if exists(mask) or any(exists(m) for m in context_mask):
+        raise NotImplementedError("masks are not supported with a PagedCache: rows hold their own counts")
+    if cache.order != len(qs) - 1:
+        raise ValueError(f"PagedCache of order {cache.order} passed to an order-{len(qs) - 1} module")
+    table = cache.table
+    weights, kwargs = _step_norms(module, q1, rotary_pos_emb,
+                                  lambda: table.positions(q1.shape[-2], q1.shape[0] != table.rows))
+    q1 = cache.append(qs, vs[-1], weights, **kwargs)
+    return cache.attend(q1, vs[:-1], scale=module.scale, softclamp=module.softclamp_value)
 
 
 # attention
@@ -429,13 +456,14 @@ class Order2PolyAttention(Module):
     def forward(self, x, context: Tensor | tuple[Tensor, ...] | None = None, mask=None,
                 context_mask: Tensor | tuple[Tensor | None, ...] | None = None,
                 rotary_pos_emb=None, cache=None, return_cache=False, parents=None):
-        """``parents``: the tree of the drafted tokens ``x`` (with a DraftCache; see drafts.py)."""
+        """``parents``: the tree of the drafted tokens ``x`` (with a DraftCache; see drafts.py).  With a
+        PagedCache ``x`` is a step's chunks of new tokens, padded or packed (see pages.py)."""
         seq_len, device = x.shape[-2], x.device
 
         has_cache = exists(cache)
-        drafted = isinstance(cache, DraftCache)
+        drafted, paged = isinstance(cache, DraftCache), isinstance(cache, PagedCache)
         assert drafted or not exists(parents), "parents describe drafted tokens: pass a DraftCache"
-        if has_cache and not drafted:
+        if has_cache and not (drafted or paged):
             assert seq_len == 1, "sequence length must be 1 when using kv cache"
 
         orig_x = x
@@ -504,10 +532,12 @@ class Order2PolyAttention(Module):
                     gates if self.attn_gate else None, self.use_root_value_as_attn_gate)
         epilogue_done = False
 
-        if drafted or isinstance(cache, _cache.StaticCache):
+        if drafted or paged or isinstance(cache, _cache.StaticCache):
             # fixed-capacity cache: norms, rotary and appends fused into the decode step
             if drafted:
                 out = _draft_step(self, qs, (v3,), mask, context_mask, rotary_pos_emb, cache, parents)
+            elif paged:
+                out = _paged_step(self, qs, (v3,), mask, context_mask, rotary_pos_emb, cache)
             else:
                 out = _static_decode_step(self, qs, (v3,), mask, context_mask, rotary_pos_emb,
                                           cache)

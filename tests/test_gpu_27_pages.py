@@ -1,0 +1,834 @@
+"""GPU: the paged cache -- PageTable's calls against lists (pages_oracle.Table), PagedCache.append and attend against 64
+bits (pages_oracle, whose docstring derives the bounds), and the modules' steps over chunks against
+their forward over whole sequences."""
+
+import copy
+
+import pytest
+import torch
+
+import pages_oracle as PO
+from parity import assert_drift, assert_parity
+
+pytestmark = pytest.mark.gpu
+param = pytest.mark.parametrize
+
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    return torch.device("cuda")
+
+
+def assert_within(got, want, tol, what):
+    diff = (got.double().cpu() - want).abs()
+    over = diff - tol
+    assert bool((over <= 0).all()), (f"{what}: off by {diff.max().item():.3e}, over the bound by "
+                                     f"{over.max().item():.3e} at {(over == over.max()).nonzero()[:1].tolist()}")
+
+
+def make(counts, new, ps, g, spare=3, capacity=None, device="cuda"):
+    """A PageTable whose row b has counts[b] positions, the last new[b] of them its chunk, in scattered pages; and the
+    same as lists."""
+    from poly_attention import PageTable
+
+    cap = capacity or max(1, max(counts))
+    need = [-(-n // ps) for n in counts]
+    pool = sum(need) + spare
+    t = PageTable(len(counts), pages=pool, page_size=ps, capacity=cap, device=device)
+    o = PO.Table(len(counts), pool, ps, cap)
+    order = torch.randperm(pool, generator=g).tolist()
+    for b, k in enumerate(need):
+        o.pages[b], order = order[:k], order[k:]
+        for p in o.pages[b]:
+            o.refs[p] = 1
+    o.counts, o.new = list(counts), list(new)
+    o.starts = [sum(new[:k]) for k in range(len(new) + 1)]
+    load(t, o)
+    return t, o
+
+
+def load(t, o):
+    most = t.pages.shape[1]
+    t.pages.copy_(torch.tensor([row + [-1] * (most - len(row)) for row in o.pages]))
+    for name in ("counts", "new", "starts", "refs"):
+        getattr(t, name).copy_(torch.tensor(getattr(o, name)))
+
+
+def fill(cache, o, g, stale=float("nan")):
+    """Random contents at the rows' positions (chunks: keys and the deepest values alone); ``stale`` everywhere else."""
+    host = {}
+    for name in ("keys", "values", "lses"):
+        host[name] = []
+        for t, x in enumerate(getattr(cache, name)):
+            y = torch.full(x.shape, stale)
+            written = name == "keys" or (name == "values" and t == 0)
+            for b, n in enumerate(o.counts):
+                have = n if written else n - o.new[b]
+                for p in range(0, have, o.ps):
+                    k = min(o.ps, have - p)
+                    z = torch.randn(y.shape[1], k, *y.shape[3:], generator=g) * (0.3 if name == "values" and t else 1.0)
+                    if name == "lses":
+                        z += 2.0 * (t + 1)
+                    y[o.pages[b][p // o.ps], :, :k] = z
+            y = y.to(x.dtype)
+            x.copy_(y)
+            host[name].append(y)
+    return host
+
+
+def inputs(o, heads, d, dtype, packed, g, pad=0, stale=float("nan")):
+    """[rows or 1, heads, tokens, d] on the CPU as a projection's output seen per head; ``stale`` behind the chunks."""
+    B, T = (1, sum(o.new) + pad) if packed else (len(o.new), max(o.new) + pad)
+    x = torch.full((B, max(T, 1), heads, d), stale)
+    for b, i, sb, st in PO.places(o.starts, o.new, packed):
+        x[sb, st] = torch.randn(heads, d, generator=g)
+    return x.to(dtype).transpose(1, 2)
+
+
+def check_attend(order, counts, new, H, hk, D, dtype, ps=16, packed=False, softclamp=None, scale=None, pad=0,
+                 stale=float("nan"), change=None, capacity=None):
+    from poly_attention import PagedCache
+
+    d = dev()
+    g = torch.Generator().manual_seed(order * 1000 + len(counts) * 100 + sum(new))
+    t, o = make(counts, new, ps, g, capacity=capacity)
+    cache = PagedCache(t, order=order, kv_heads=hk, dim_head=D, dtype=DT[dtype])
+    host = fill(cache, o, g, stale)
+    q1 = inputs(o, H, D, DT[dtype], packed, g, pad)
+    vs = [inputs(o, hk, D, DT[dtype], packed, g, pad) for _ in range(order - 2)]
+    if change:
+        change(cache, host, o, q1, vs)
+    s = D ** -0.5 if scale is None else scale
+    got = cache.attend(q1.to(d), [v.to(d) for v in vs], scale=s, softclamp=softclamp)
+    assert got.shape == q1.shape
+    (out, out_tol), values, lses = PO.attend(q1, vs, host, o, packed, s, softclamp)
+    behind = torch.ones(q1.shape[0], q1.shape[2], dtype=torch.bool)
+    for b, i, sb, st in PO.places(o.starts, o.new, packed):
+        behind[sb, st] = False
+    assert bool((got.cpu().transpose(1, 2)[behind] == 0).all())
+    assert_within(got, out, out_tol, "out")
+    for lvl in range(order):
+        if lvl:
+            assert_pages(cache.values[lvl], *values[lvl], host["values"][lvl], f"values {lvl}")
+        else:
+            assert torch.equal(cache.values[0].cpu().nan_to_num(77), host["values"][0].nan_to_num(77))
+        if lvl < order - 1:
+            assert_pages(cache.lses[lvl], *lses[lvl], host["lses"][lvl], f"lses {lvl}")
+        assert torch.equal(cache.keys[lvl].cpu().nan_to_num(77), host["keys"][lvl].nan_to_num(77))
+    again = cache.attend(q1.to(d), [v.to(d) for v in vs], scale=s, softclamp=softclamp)
+    assert torch.equal(got, again), "the same bits each time"
+    return t, cache, o, q1, got
+
+
+def assert_pages(got, want, tol, was, what):
+    """The chunks' places within their bounds, all others untouched."""
+    got = got.cpu()
+    same = tol == 0
+    assert torch.equal(got[same].double().nan_to_num(77), was[same].double().nan_to_num(77)), f"{what}: another place changed"
+    assert_within(got[~same], want[~same], tol[~same], what)
+
+
+# ---------------------------------------------------------------------------------------
+# attention
+
+SHAPES = [
+    # order, counts, new, H, hk, D, dtype, page
+    (2, [1], [1], 1, 1, 64, "bf16", 16),                       # the first token there is
+    (2, [5], [5], 2, 2, 64, "f32", 16),                        # a whole prompt
+    (2, [300], [1], 8, 8, 64, "bf16", 64),
+    (2, [17, 0, 33, 128, 1], [1, 0, 17, 5, 1], 4, 2, 64, "f16", 16),
+    (3, [40, 129, 7], [8, 3, 7], 4, 4, 64, "bf16", 32),
+    (3, [64, 100], [64, 1], 6, 2, 40, "f32", 16),
+    (4, [50, 21], [20, 21], 2, 1, 32, "f16", 16),
+    (8, [30, 1], [4, 1], 2, 2, 8, "f32", 16),
+    (2, [700, 350], [33, 2], 8, 1, 128, "bf16", 128),
+    (2, [260, 513], [130, 1], 3, 3, 96, "f32", 64),
+    (2, [257, 200], [65, 200], 12, 4, 128, "f16", 256),
+    (2, [150, 90], [40, 2], 2, 2, 256, "bf16", 16),
+    (3, [150, 90], [12, 2], 2, 1, 160, "f32", 32),
+    (3, [600, 45, 1000], [200, 45, 1], 4, 2, 64, "bf16", 16),
+    (3, [400, 900], [300, 7], 4, 4, 128, "f16", 64),
+    (2, [1500], [1400], 2, 1, 64, "bf16", 64),
+    (2, [515, 300, 64], [515, 257, 64], 8, 2, 64, "f16", 16),
+    (2, [9000, 20], [1, 20], 4, 1, 128, "bf16", 64),
+    (2, [130] * 70, [2] * 69 + [130], 2, 1, 64, "bf16", 16),   # more rows than a wave's lanes
+    (2, [5000, 260], [200, 260], 16, 2, 128, "bf16", 4096),    # one page holds more than a tile's positions
+]
+
+
+@param("packed", [False, True])
+@param("order, counts, new, H, hk, D, dtype, ps", SHAPES)
+def test_attend(order, counts, new, H, hk, D, dtype, ps, packed):
+    check_attend(order, counts, new, H, hk, D, dtype, ps, packed)
+
+
+@param("dtype", ["bf16", "f16", "f32"])
+@param("counts, new", [([90, 35], [1, 3]), ([400, 200], [260, 31])])
+def test_attend_softclamp(dtype, counts, new):
+    check_attend(3, counts, new, 4, 2, 64, dtype, 16, softclamp=3.0)
+    check_attend(2, counts, new, 4, 2, 128, dtype, 16, softclamp=50.0, packed=True)
+
+
+def test_attend_scale_and_padding():
+    check_attend(2, [40, 3], [9, 3], 2, 2, 64, "f32", scale=0.0, pad=5)
+    check_attend(2, [40, 3], [9, 3], 2, 2, 64, "f32", scale=-0.3, pad=1, packed=True)
+    check_attend(2, [200, 300], [150, 3], 2, 2, 64, "bf16", pad=60)
+    check_attend(2, [20], [0], 2, 2, 64, "bf16", pad=3)        # nobody brings a token
+
+
+def test_rows_share_pages():
+    """Rows that share all but their last page."""
+    from poly_attention import PagedCache
+
+    g = torch.Generator().manual_seed(5)
+    t, o = make([70, 69, 66], [6, 5, 2], 16, g)
+    for b in (1, 2):
+        for k in range(4):
+            o.refs[o.pages[b][k]] -= 1
+            o.pages[b][k] = o.pages[0][k]
+            o.refs[o.pages[0][k]] += 1
+    load(t, o)
+    cache = PagedCache(t, order=2, kv_heads=2, dim_head=64, dtype=torch.float32)
+    host = fill(cache, o, g)
+    q1 = inputs(o, 4, 64, torch.float32, False, g)
+    got = cache.attend(q1.cuda())
+    (out, tol), values, lses = PO.attend(q1, [], host, o, False, 64 ** -0.5, None)
+    assert_within(got, out, tol, "out")
+
+
+@param("dtype", ["bf16", "f16", "f32"])
+@param("counts, new", [([100], [40]), ([300], [200])])
+def test_what_a_token_does_not_see(dtype, counts, new):
+    """Infinities and NaN in a later token's key, query, value and logsumexp reach no earlier token."""
+    from poly_attention import PagedCache
+
+    g = torch.Generator().manual_seed(3)
+    outs = []
+    for bad in (False, True):
+        g.manual_seed(3)
+        t, o = make(counts, new, 16, g)
+        cache = PagedCache(t, order=3, kv_heads=2, dim_head=64, dtype=DT[dtype])
+        fill(cache, o, g)
+        q1 = inputs(o, 4, 64, DT[dtype], False, g).cuda()
+        v = inputs(o, 2, 64, DT[dtype], False, g).cuda()
+        if bad:
+            for p, x in ((counts[0] - 3, float("inf")), (counts[0] - 1, float("nan")), (counts[0] - 2, -float("inf"))):
+                page, slot = o.pages[0][p // 16], p % 16
+                for a in (*cache.keys, cache.values[0]):
+                    a[page, :, slot] = x
+                v[:, :, new[0] - counts[0] + p] = x
+        outs.append((cache.attend(q1, [v]), cache, o))
+    (a, ca, o), (b, cb, _) = outs
+    m = new[0] - 3
+    assert bool(torch.isfinite(a[:, :, :m].float()).all())
+    tol = 0.02 if dtype != "f32" else 1e-4
+    diff = (a - b)[:, :, :m].float().abs().max().item()
+    assert diff <= tol, diff
+    # and the last token, which sees all of them, is no number
+    assert not bool(torch.isfinite(b[:, :, -1].float()).any())
+
+
+def test_values_and_weights_that_overflow_nothing():
+    """Scores and logsumexps of any size: softmaxes of one position, of far ones, of equal ones."""
+    def change(cache, host, o, q1, vs):
+        for b, n in enumerate(o.counts):
+            for p in range(n - o.new[b]):
+                page, slot = o.pages[b][p // o.ps], p % o.ps
+                host["lses"][0][page, :, slot] = [-1e5, 3e4, 0.0][p % 3] if p != 11 else 4e4
+        cache.lses[0].copy_(host["lses"][0])
+
+    check_attend(2, [60, 400], [3, 150], 2, 2, 64, "f32", change=change)
+    check_attend(2, [60, 400], [3, 150], 2, 2, 64, "bf16", change=change)
+
+
+@param("counts, new", [([90, 40], [5, 2]), ([300, 200], [200, 90])])
+def test_layouts(counts, new):
+    """Inputs of other strides, starts and types of heads give the same bits."""
+    from poly_attention import PagedCache
+
+    d = dev()
+    g = torch.Generator().manual_seed(8)
+    t, o = make(counts, new, 16, g)
+    cache = PagedCache(t, order=3, kv_heads=2, dim_head=64, dtype=torch.bfloat16)
+    fill(cache, o, g)
+    q1 = inputs(o, 4, 64, torch.bfloat16, False, g).to(d)
+    v = inputs(o, 2, 64, torch.bfloat16, False, g).to(d)
+    want = cache.attend(q1.contiguous(), [v.contiguous()])
+    for f in (lambda x: x, lambda x: x.transpose(2, 3).contiguous().transpose(2, 3),
+              lambda x: torch.nn.functional.pad(x, (1, 0))[..., 1:], lambda x: torch.stack([x, x], 3)[:, :, :, 1]):
+        assert torch.equal(cache.attend(f(q1), [f(v)]).nan_to_num(), want.nan_to_num())
+
+
+def test_long_rows_and_offsets_past_32_bits():
+    """A pool of more than 2^31 elements and 2^32 bytes, its last pages in use."""
+    from poly_attention import PagedCache, PageTable
+
+    d = dev()
+    ps, hk, D = 1024, 8, 128
+    pages = (1 << 31) // (ps * hk * D) + 6
+    t = PageTable(2, pages=pages, page_size=ps, capacity=4 * ps, device=d)
+    o = PO.Table(2, pages, ps, 4 * ps)
+    o.pages, o.counts, o.new, o.starts = [[pages - 1, 3], [pages - 2]], [1500, 900], [2, 1], [0, 2, 3]
+    for row in o.pages:
+        for p in row:
+            o.refs[p] = 1
+    load(t, o)
+    cache = PagedCache(t, order=2, kv_heads=hk, dim_head=D, dtype=torch.bfloat16)
+    g = torch.Generator().manual_seed(2)
+    used = [pages - 1, 3, pages - 2]
+    host = {k: [torch.randn(3, *x.shape[1:], generator=g).to(x.dtype) for x in getattr(cache, k)] for k in ("keys", "values", "lses")}
+    for k, xs in host.items():
+        for x, y in zip(getattr(cache, k), xs):
+            x[used] = y.to(d)
+    o.pages = [[0, 1], [2]]
+    q1 = inputs(o, 16, D, torch.bfloat16, False, g)
+    got = cache.attend(q1.to(d))
+    (out, tol), values, lses = PO.attend(q1, [], host, o, False, D ** -0.5, None)
+    assert_within(got, out, tol, "out")
+    assert_within(cache.lses[0][used], *lses[0], "lses")
+
+
+# ---------------------------------------------------------------------------------------
+# append
+
+
+@param("packed", [False, True])
+@param("order, counts, new, H, hk, D, rot, dtype, ps", [
+    (2, [1], [1], 1, 1, 64, 64, "bf16", 16),
+    (2, [20, 0, 40], [5, 0, 33], 4, 2, 64, 32, "f16", 16),
+    (3, [100, 31], [1, 31], 6, 3, 40, 0, "f32", 32),
+    (4, [9, 9], [9, 2], 2, 1, 8, 8, "f32", 16),
+    (2, [300, 700], [300, 250], 8, 2, 128, 128, "bf16", 64),
+    (2, [40, 17], [9, 17], 4, 4, 256, 100, "bf16", 16),
+    (2, [70] * 70, [3, 0] * 35, 2, 1, 96, 96, "f16", 16),
+])
+@param("kind", ["angles", "one", "none"])
+def test_append(order, counts, new, H, hk, D, rot, dtype, ps, packed, kind):
+    from poly_attention import PagedCache
+
+    d, dt = dev(), DT[dtype]
+    g = torch.Generator().manual_seed(sum(counts) + order)
+    t, o = make(counts, new, ps, g)
+    cache = PagedCache(t, order=order, kv_heads=hk, dim_head=D, dtype=dt)
+    for x in cache.arrays():
+        x.fill_(7.0)
+    qs = [inputs(o, h, D, dt, packed, g, pad=1) for h in (H, *[hk] * order)]
+    v = inputs(o, hk, D, dt, packed, g, pad=1)
+    weights = [None if k == 1 else 1 + 0.2 * torch.randn(D, generator=g) for k in range(order + 1)]
+    weights[0] = weights[0].to(dt)
+    B, T = qs[0].shape[0], qs[0].shape[2]
+    angles = None
+    if rot and kind != "none":
+        angles = torch.randn(*((B, T, rot) if kind == "angles" else (rot,)), generator=g) * 50
+    q1 = cache.append([q.to(d) for q in qs], v.to(d), [None if w is None else w.to(d) for w in weights], eps=1e-6,
+                      angles=None if angles is None else angles.to(d))
+    seen = torch.zeros(B, T, dtype=torch.bool)
+    left = [x.cpu().clone() for x in cache.arrays()]
+    for b, i, sb, st in PO.places(o.starts, o.new, packed):
+        seen[sb, st] = True
+        a = None if angles is None else angles[sb, st] if kind == "angles" else angles
+        p = counts[b] - new[b] + i
+        page, slot = o.pages[b][p // ps], p % ps
+        y, tol = PO.append(qs[0][sb, :, st], weights[0], 1e-6, a, dt)
+        assert_within(q1[sb, :, st], y, tol, "q1")
+        for k in range(1, order + 1):
+            y, tol = PO.append(qs[k][sb, :, st], weights[k], 1e-6, a, dt)
+            x = cache.keys[order - k][page, :, slot]
+            assert_within(x, y, tol, f"q{k + 1}")
+            left[order - k][page, :, slot] = 7.0
+        assert torch.equal(cache.values[0][page, :, slot].cpu(), v[sb, :, st])
+        left[order][page, :, slot] = 7.0
+    assert bool((q1.cpu().transpose(1, 2)[~seen] == 0).all())
+    assert all(bool((x == 7.0).all()) for x in left), "another place was written"
+
+
+@param("dtype", ["bf16", "f32"])
+@param("packed", [False, True])
+def test_append_module_frequencies(dtype, packed):
+    """A rotary module's frequencies at the tokens' positions."""
+    from poly_attention import PagedCache
+
+    d, dt = dev(), DT[dtype]
+    g = torch.Generator().manual_seed(4)
+    t, o = make([70, 9, 33], [6, 9, 1], 16, g)
+    cache = PagedCache(t, order=2, kv_heads=2, dim_head=64, dtype=dt)
+    qs = [inputs(o, 2, 64, dt, packed, g) for _ in range(3)]
+    v = inputs(o, 2, 64, dt, packed, g)
+    inv = 10000.0 ** -(torch.arange(0, 32, 2).float() / 32)
+    w = torch.ones(64)
+    q1 = cache.append([q.to(d) for q in qs], v.to(d), [w.to(d)] * 3, eps=1e-6, inv_freq=inv.to(d), interp=2.0)
+    for b, i, sb, st in PO.places(o.starts, o.new, packed):
+        p = o.counts[b] - o.new[b] + i
+        pos = torch.tensor(float(p)).to(dt).float().div(2.0).to(dt).float()
+        a = (pos * inv).repeat_interleave(2)
+        y, tol = PO.append(qs[0][sb, :, st], w, 1e-6, a, dt)
+        assert_within(q1[sb, :, st], y, tol, "q1")
+        y, tol = PO.append(qs[2][sb, :, st], w, 1e-6, a, dt)
+        assert_within(cache.keys[0][o.pages[b][p // 16], :, p % 16], y, tol, "q3")
+
+
+# ---------------------------------------------------------------------------------------
+# the table
+
+
+class Model:
+    """A table with a cache of one number per position (and two layers of other shapes), and what it has to hold."""
+
+    def __init__(self, rows, pool, ps, capacity):
+        from poly_attention import PagedCache, PageTable
+
+        self.t = PageTable(rows, pages=pool, page_size=ps, capacity=capacity)
+        self.caches = [PagedCache(self.t, order=2, kv_heads=1, dim_head=8, dtype=torch.float32),
+                       PagedCache(self.t, order=3, kv_heads=3, dim_head=24, dtype=torch.bfloat16)]
+        for c in self.caches:
+            for x in c.arrays():
+                x.fill_(-1.0)
+        self.o = PO.Table(rows, pool, ps, capacity)
+        self.text = [[] for _ in range(rows)]  # the numbers of a row's positions
+        self.next = 0
+
+    def write(self):
+        """Every granted position of the chunks gets a number of its own, below 256 (exact in every type)."""
+        o = self.o
+        for b, m in enumerate(o.new):
+            for i in range(m):
+                p = o.counts[b] - m + i
+                self.next = (self.next + 1) % 251
+                self.text[b].append(float(self.next))
+                for c in self.caches:
+                    for x in c.arrays():
+                        x[o.pages[b][p // o.ps], :, p % o.ps] = float(self.next)
+
+    def check(self):
+        self.o.check(self.t)
+        ps = self.o.ps
+        for c in self.caches:
+            for x in c.arrays():
+                x = x.cpu()
+                for b, n in enumerate(self.o.counts):
+                    got = PO.row_of(x, self.o.pages[b], n, ps)
+                    want = torch.tensor(self.text[b]).to(x.dtype)
+                    assert len(self.text[b]) == n
+                    if n:
+                        assert bool((got.transpose(0, 1).reshape(n, -1) == want[:, None]).all()), (b, n)
+
+    def extend(self, more, how):
+        self.o.extend(more)
+        self.t.extend(how(more))
+        self.write()
+
+    def select(self, index, lengths, how):
+        self.o.select(index, lengths)
+        self.t.select(how(index), None if lengths is None else how(lengths))
+        n = len(index)
+        self.text = [self.text[i][:self.o.counts[b]] if 0 <= i < n else [] for b, i in enumerate(index)]
+
+
+def as_int32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+@param("rows, pool, ps, capacity, seed", [(1, 3, 16, 64, 0), (3, 12, 16, 80, 1), (7, 20, 32, 300, 2), (40, 90, 16, 70, 3),
+                                          (70, 60, 16, 100, 4), (5, 9, 64, 640, 5)])
+def test_table(rows, pool, ps, capacity, seed):
+    dev()
+    import random
+
+    rng = random.Random(seed)
+    m = Model(rows, pool, ps, capacity)
+    for step in range(24):
+        what = rng.choice(["extend", "extend", "extend", "select", "compact", "fork"])
+        how = rng.choice([as_int32, list, lambda x: torch.tensor(x), lambda x: torch.tensor(x, device="cuda")])
+        if what == "extend":
+            big = rng.random() < 0.3
+            m.extend([rng.choice([0, 1, 1, rng.randrange(0, 2 * ps), -3 if how is as_int32 else 0]) if not big
+                      else rng.randrange(0, capacity) for _ in range(rows)], how)
+        elif what == "select":
+            index = [rng.choice([b, b, -1, rng.randrange(rows), rows + 2]) for b in range(rows)]
+            lengths = rng.choice([None, [rng.randrange(0, capacity) for _ in range(rows)]])
+            m.select(index, lengths, how)
+        elif what == "fork":  # rows that share partly filled pages
+            src = rng.randrange(rows)
+            m.select([src if rng.random() < 0.7 else b for b in range(rows)], None, how)
+            m.extend([rng.choice([0, 1, 1]) for _ in range(rows)], how)
+        else:
+            m.o.compact()
+            m.t.compact()
+        m.check()
+    assert bool(m.t.overflow.item()) == m.o.overflow
+
+
+def test_table_conveniences():
+    dev()
+    m = Model(4, 12, 16, 64)
+    m.extend([20, 33, 5, 0], list)
+    m.t.fork(1, [0, 3])
+    m.o.select([1, 1, 2, 1])
+    m.text = [list(m.text[1]), m.text[1], m.text[2], list(m.text[1])]
+    m.check()
+    m.t.free([1])
+    m.o.select([0, -1, 2, 3])
+    m.text[1] = []
+    m.check()
+    m.t.truncate([17, 4, 2, 99])
+    m.o.select([0, 1, 2, 3], [17, 4, 2, 99])
+    m.text = [x[:n] for x, n in zip(m.text, m.o.counts)]
+    m.check()
+    assert m.t.lengths() == m.o.counts and m.t.free_pages() == sum(r == 0 for r in m.o.refs)
+    m.t.check_overflow()
+    m.t.extend([100, 0, 0, 0])
+    with pytest.raises(RuntimeError):
+        m.t.check_overflow()
+    with pytest.raises(ValueError):
+        m.t.free([4])
+    with pytest.raises(ValueError):
+        m.t.extend([1, 1])
+    with pytest.raises(TypeError):
+        m.t.extend(torch.ones(4, device="cuda"))
+
+
+def test_large_pool():
+    """More pages than one round of the scans takes, the free ones last."""
+    dev()
+    from poly_attention import PageTable
+
+    pool = 70000
+    t = PageTable(3, pages=pool, page_size=16, capacity=1 << 20)
+    t.extend([900000, 16, 16])
+    n = -(-900000 // 16)
+    assert t.counts.tolist() == [900000, 16, 16]
+    assert torch.equal(t.pages[0, :n].cpu(), torch.arange(n, dtype=torch.int32))
+    assert t.pages[1:, 0].tolist() == [n, n + 1]
+    t.select([-1, 1, 2])
+    assert int(t.refs.sum()) == 2
+    t.extend([0, 17, 0])
+    assert t.pages[1, :3].tolist() == [n, 0, 1]
+    t.compact()
+    assert t.pages[:, :3].tolist() == [[-1, -1, -1], [2, 0, 1], [3, -1, -1]] and t.refs[:5].tolist() == [1, 1, 1, 1, 0]
+
+
+def test_copies():
+    """A deep copy goes on by itself."""
+    dev()
+    m = Model(2, 8, 16, 64)
+    m.extend([20, 3], as_int32)
+    other = copy.deepcopy(m)
+    other.o, other.text = copy.deepcopy(m.o), copy.deepcopy(m.text)
+    m.extend([1, 30], as_int32)
+    other.extend([2, 2], as_int32)
+    m.check()
+    other.check()
+
+
+def test_refusals():
+    from poly_attention import PagedCache, PageTable
+
+    d = dev()
+    t = PageTable(2, pages=8, page_size=16, capacity=64)
+    c = PagedCache(t, order=3, kv_heads=2, dim_head=64, dtype=torch.bfloat16)
+    z = lambda *s, dtype=torch.bfloat16, device=d: torch.zeros(*s, dtype=dtype, device=device)  # noqa: E731
+    q, v = z(2, 4, 3, 64), z(2, 2, 3, 64)
+    t.extend([3, 1])
+    w = [None] * 4
+    for bad in (z(3, 4, 3, 64), z(2, 3, 3, 64), z(2, 4, 0, 64), z(2, 4, 3, 32), z(4, 3, 64), q.cpu()):
+        with pytest.raises(ValueError):
+            c.attend(bad, [v])
+    with pytest.raises(TypeError):
+        c.attend(q.float(), [v])
+    for vs in ([], [v, v], [z(2, 4, 3, 64)], [z(2, 2, 2, 64)], [v.cpu()]):
+        with pytest.raises(ValueError):
+            c.attend(q, vs)
+    with pytest.raises(ValueError):
+        c.attend(q[:, :, :2], [v[:, :, :2]])  # fewer tokens than extend was given
+    with pytest.raises(ValueError):
+        c.attend(z(1, 4, 3, 64), [z(1, 2, 3, 64)])
+    with pytest.raises(RuntimeError):
+        c.attend(q.requires_grad_(), [v])
+    with torch.no_grad():
+        c.attend(q, [v])
+    q = q.detach()
+    with pytest.raises(ValueError):
+        c.append([q, v, v], v, w[:3], eps=1e-6)
+    with pytest.raises(ValueError):
+        c.append([q, v, v, q], v, w, eps=1e-6)
+    with pytest.raises(ValueError):
+        c.append([q, v, v, v], v, w, eps=1e-6, angles=z(2, 4, 64))
+    with pytest.raises(ValueError):
+        c.append([q, v, v, v], v, w, eps=1e-6, angles=z(3, 63))
+    with pytest.raises(ValueError):
+        c.append([q, v, v, v], v, w, eps=1e-6, angles=z(3, 64), inv_freq=z(32))
+    with pytest.raises(ValueError):
+        c.append([q, v, v, v], v, [z(32), None, None, None], eps=1e-6)
+    with pytest.raises(RuntimeError):
+        c.append([q, v, v, v.clone().requires_grad_()], v, w, eps=1e-6)
+
+
+# ---------------------------------------------------------------------------------------
+# modules
+
+
+def modules(order, d, **kw):
+    from poly_attention import NPolyAttention, PolyAttention
+
+    torch.manual_seed(7)
+    if order == 2:
+        m = PolyAttention(dim=96, heads=4, dim_head=d, causal=True, **kw)
+    else:
+        m = NPolyAttention(dim=96, order=order, heads=4, dim_head=d, causal=True, **kw)
+    return m.cuda().eval()
+
+
+@param("order, kw", [(2, {}), (2, dict(kv_heads=2)), (3, {}), (3, dict(kv_heads=2, use_rotary_embed=True)),
+                     (2, dict(use_rotary_embed=True, softclamp_value=20.0)), (4, dict(shared_kv=True)),
+                     (2, dict(multiply_root_value=True, attn_gate=True)), (3, dict(prenorm=True, multiply_root_value=True, kv_heads=1))])
+@param("packed", [False, True])
+def test_module_in_pieces(order, kw, packed):
+    """Sequences brought in chunks of all sizes have the outputs of the whole sequences."""
+    from poly_attention import PagedCache, PageTable
+
+    d = dev()
+    m = modules(order, 64, **kw)
+    g = torch.Generator().manual_seed(1)
+    lens = [150, 3, 77]
+    x = torch.randn(3, max(lens), 96, generator=g).to(d)
+    with torch.no_grad():
+        want = m(x)
+        t = PageTable(3, pages=20, page_size=16, capacity=160)
+        c = PagedCache(t, order=order, kv_heads=kw.get("kv_heads", 4), dim_head=64, dtype=torch.float32)
+        at = [0, 0, 0]
+        for step in ([1, 1, 5], [60, 0, 1], [80, 1, 64], [1, 1, 1], [7, 0, 6], [1, 0, 0]):
+            new = [min(s, n - a) for s, n, a in zip(step, lens, at)]
+            t.extend(new)
+            if packed:
+                piece = torch.cat([x[b, a:a + k] for b, (a, k) in enumerate(zip(at, new))])[None]
+            else:
+                piece = torch.stack([torch.nn.functional.pad(x[b, a:a + k], (0, 0, 0, max(new) - k)) for b, (a, k) in enumerate(zip(at, new))])
+            y = m(piece, cache=c)
+            first = 0
+            for b, (a, k) in enumerate(zip(at, new)):
+                got = y[0, first:first + k] if packed else y[b, :k]
+                first += k
+                assert_parity(got, want[b, a:a + k], torch.float32, f"row {b}, {k} tokens from {a}")
+            at = [a + k for a, k in zip(at, new)]
+        assert at == lens and t.lengths() == lens
+
+
+@param("dtype", ["bf16", "f16"])
+def test_module_16_bits(dtype):
+    """A layer cast whole to 16 bits, its own rotary with it, with an external one, and a fork."""
+    from poly_attention import PagedCache, PageTable
+
+    d, dt = dev(), DT[dtype]
+    for kw in (dict(use_rotary_embed=True), {}):
+        m = modules(2, 64, kv_heads=2, **kw).to(dt)
+        g = torch.Generator().manual_seed(1)
+        x = torch.randn(2, 90, 96, generator=g).to(d).to(dt)
+        with torch.no_grad():
+            want = m(x)  # another path in the same type, whose distance from 32 bits is the measure
+            exact = copy.deepcopy(m).float().cpu()(x.float().cpu())
+            t = PageTable(4, pages=20, page_size=16, capacity=128)
+            c = PagedCache(t, order=2, kv_heads=2, dim_head=64, dtype=dt)
+            t.extend([70, 70, 0, 0])
+            y = torch.zeros(4, 70, 96, device=d, dtype=dt)
+            y[:2] = x[:, :70]
+            a = m(y, cache=c)
+            assert_drift(a[:2], exact[:, :70], want[:, :70], "prompt")
+            t.select([0, 1, 0, 1])
+            t.extend([20] * 4)
+            b = m(torch.cat([x, x])[:, 70:], cache=c)
+            assert_drift(b[:2], exact[:, 70:], want[:, 70:], "rest")
+            assert_drift(b[2:], exact[:, 70:], want[:, 70:], "the forked rows'")
+
+
+def test_module_external_rotary():
+    from poly_attention import PagedCache, PageTable
+    from poly_attention.rotary import RotaryEmbedding
+
+    d = dev()
+    m, rot = modules(2, 64), RotaryEmbedding(32).to(d)
+    x = torch.randn(2, 40, 96, generator=torch.Generator().manual_seed(1)).to(d)
+    with torch.no_grad():
+        want = m(x, rotary_pos_emb=rot(torch.arange(40, device=d)))
+        t = PageTable(2, pages=20, page_size=16, capacity=64)
+        c = PagedCache(t, order=2, kv_heads=4, dim_head=64, dtype=torch.float32)
+        t.extend([25, 40])
+        piece = torch.cat([x[0, :25], x[1]])[None]
+        y = m(piece, cache=c, rotary_pos_emb=rot(t.positions(65, packed=True)))
+        assert_parity(y[0, :25], want[0, :25], torch.float32, "row 0")
+        assert_parity(y[0, 25:], want[1], torch.float32, "row 1")
+        t.extend([15, 0])
+        y = m(x[:, 25:], cache=c, rotary_pos_emb=rot(t.positions(15)))
+        assert_parity(y[0], want[0, 25:], torch.float32, "row 0's rest")
+
+
+def test_module_refusals():
+    from poly_attention import PagedCache, PageTable
+
+    d = dev()
+    m = modules(2, 64)
+    t = PageTable(2, pages=4, page_size=16, capacity=64)
+    c3 = PagedCache(t, order=3, kv_heads=4, dim_head=64, dtype=torch.float32)
+    c = PagedCache(t, order=2, kv_heads=4, dim_head=64, dtype=torch.float32)
+    t.extend([2, 2])
+    x = torch.zeros(2, 2, 96, device=d)
+    with torch.no_grad():
+        with pytest.raises(ValueError):
+            m(x, cache=c3)
+        with pytest.raises(NotImplementedError):
+            m(x, cache=c, mask=torch.ones(2, 2, dtype=torch.bool, device=d))
+        with pytest.raises(AssertionError):
+            m(x, cache=c, parents=torch.tensor([-1, 0], device=d))
+    with pytest.raises(RuntimeError):
+        m(x, cache=c)
+
+
+# ---------------------------------------------------------------------------------------
+# a step as it is used: captured, replayed, on other streams
+
+
+def serve(m, caches, t, tokens, more):
+    t.extend(more)
+    x = tokens
+    for c in caches:
+        x = x + m(x, cache=c)
+    return x
+
+
+@param("T", [1, 40])
+def test_captured_steps(T):
+    """A captured step replayed many times, between eager forks and frees, is the eager one."""
+    from poly_attention import PagedCache, PageTable
+
+    d = dev()
+    m = modules(2, 64, kv_heads=2, use_rotary_embed=True)
+    torch.manual_seed(3)
+    x = torch.randn(4, T, 96, device=d)
+    runs = []
+    for captured in (False, True):
+        t = PageTable(4, pages=60, page_size=16, capacity=400)
+        caches = [PagedCache(t, order=2, kv_heads=2, dim_head=64, dtype=torch.float32) for _ in range(2)]
+        more = torch.tensor([T, T, 0, 0], dtype=torch.int32, device=d)
+        tokens = x.clone()
+        outs = []
+        with torch.no_grad():
+            if captured:
+                side = torch.cuda.Stream()
+                side.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(side):
+                    serve(m, caches, t, tokens, more)
+                torch.cuda.current_stream().wait_stream(side)
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    y = serve(m, caches, t, tokens, more)
+                t.select([-1] * 4)
+            for step in range(7):
+                if step == 3:
+                    t.select([0, 1, 0, 1])
+                    more.copy_(torch.tensor([T, max(T - 3, 1), T, T]))
+                if step == 5:
+                    t.select([0, -1, 2, 0], [400, 0, T + 2, 3])
+                tokens.copy_(x * (1 + 0.1 * step))
+                if captured:
+                    graph.replay()
+                else:
+                    y = serve(m, caches, t, tokens, more)
+                outs.append((y.clone(), t.pages.clone(), t.counts.clone(), t.refs.clone()))
+                torch.cuda.synchronize()
+        runs.append(outs)
+    for a, b in zip(*runs):
+        for u, v in zip(a, b):
+            assert torch.equal(u, v)
+
+
+def test_two_pools_at_once():
+    """Two tables with their caches on two streams."""
+    from poly_attention import PagedCache, PageTable
+
+    d = dev()
+    m = modules(3, 64)
+    x = [torch.randn(3, 70, 96, generator=torch.Generator().manual_seed(k)).to(d) for k in range(2)]
+
+    def make_pool():
+        t = PageTable(3, pages=30, page_size=16, capacity=128)
+        return t, [PagedCache(t, order=3, kv_heads=4, dim_head=64, dtype=torch.float32) for _ in range(2)]
+
+    with torch.no_grad():
+        want = []
+        for k in range(2):
+            t, caches = make_pool()
+            want.append([serve(m, caches, t, x[k], torch.full((3,), 70, dtype=torch.int32, device=d)),
+                         serve(m, caches, t, x[k][:, :1], torch.ones(3, dtype=torch.int32, device=d))])
+        pools = [make_pool() for _ in range(2)]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        got = [[], []]
+        more = [torch.full((3,), n, dtype=torch.int32, device=d) for n in (70, 1)]
+        torch.cuda.synchronize()
+        for step in range(2):
+            for k in range(2):
+                with torch.cuda.stream(streams[k]):
+                    t, caches = pools[k]
+                    got[k].append(serve(m, caches, t, x[k] if step == 0 else x[k][:, :1], more[step]))
+        torch.cuda.synchronize()
+    for k in range(2):
+        for a, b in zip(want[k], got[k]):
+            assert torch.equal(a, b)
+
+
+def test_capture_needs_an_eager_call():
+    from poly_attention import PageTable
+
+    dev()
+    t = PageTable(2, pages=4, page_size=16, capacity=64)
+    more = torch.ones(2, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager"):
+        with torch.cuda.graph(graph):
+            t.extend(more)
+
+
+def test_whole_run():
+    """Prompts in pieces, a fork, single tokens, rows that end, a compaction and new rows: every token's output is that
+    of its whole sequence."""
+    from poly_attention import PagedCache, PageTable
+
+    d = dev()
+    m = modules(2, 64, kv_heads=2)
+    g = torch.Generator().manual_seed(9)
+    text = torch.randn(6, 130, 96, generator=g).to(d)
+    rows = 4
+    t = PageTable(rows, pages=24, page_size=16, capacity=160)
+    c = PagedCache(t, order=2, kv_heads=2, dim_head=64, dtype=torch.float32)
+    said = [torch.zeros(0, 96, device=d) for _ in range(rows)]  # what each row holds
+
+    def step(pieces):
+        new = [0 if p is None else p.shape[0] for p in pieces]
+        t.extend(new)
+        x = torch.cat([p for p in pieces if p is not None])[None]
+        y, at = m(x, cache=c)[0], 0
+        for b, p in enumerate(pieces):
+            if p is None:
+                continue
+            said[b] = torch.cat([said[b], p])
+            want = m(said[b][None])[0, -p.shape[0]:]
+            assert_parity(y[at:at + p.shape[0]], want, torch.float32, f"row {b}")
+            at += p.shape[0]
+
+    with torch.no_grad():
+        step([text[0, :70], text[1, :9], None, None])
+        step([text[0, 70:71], text[1, 9:60], text[2, :33], None])
+        t.fork(0, [3])
+        said[3] = said[0].clone()
+        step([text[0, 71:72], text[1, 60:61], text[2, 33:34], text[4, :5]])
+        t.free([1])
+        said[1] = said[1][:0]
+        t.compact()
+        step([text[0, 72:80], text[5, :20], text[2, 34:35], text[4, 5:6]])
+        t.truncate([50, 999, 20, 999])
+        said = [said[0][:50], said[1], said[2][:20], said[3]]
+        step([text[3, :1], text[5, 20:21], text[3, 1:2], text[4, 6:40]])
+    t.check_overflow()
+    assert t.lengths() == [x.shape[0] for x in said]
