@@ -32,7 +32,7 @@ namespace pa {
 // as dma16, marked as streaming
 __device__ __forceinline__ void dma16_nt(srd_t srd, uint32_t lds, uint32_t voff) {
     lds = __builtin_amdgcn_readfirstlane(lds);
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen nt lds"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %2, 0 offen nt lds"
                  :
                  : "v"(voff), "s"(lds), "s"(srd)
                  : "memory", "m0");
@@ -40,7 +40,7 @@ __device__ __forceinline__ void dma16_nt(srd_t srd, uint32_t lds, uint32_t voff)
 // as dma16, 4 bytes a lane
 __device__ __forceinline__ void dma4(srd_t srd, uint32_t lds, uint32_t voff) {
     lds = __builtin_amdgcn_readfirstlane(lds);
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %0, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dword %0, %2, 0 offen lds"
                  :
                  : "v"(voff), "s"(lds), "s"(srd)
                  : "memory", "m0");

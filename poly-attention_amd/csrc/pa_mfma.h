@@ -93,8 +93,8 @@ __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane
 // 41-52 us, dQ 62-76 -> 37-38 (with two workgroups per CU), dK/dV 65-68 -> 41-44.  Where nearly every
 // block leaves the range (softclamp 1, B = 4, H = 16, N = 2048, causal) a level's forward 252 -> 218,
 // its backward 364 -> 374: the range test, and dQ at two workgroups per CU instead of three.
-template <bool LOGIT, class Bias>
-__device__ __forceinline__ void soft_clamp16(f32x16_t& s, const PassDev& P, Bias bias) {
+template <bool LOGIT, class Pass, class Bias>
+__device__ __forceinline__ void soft_clamp16(f32x16_t& s, const Pass& P, Bias bias) {
     const SoftClampDev& c = P.sc;
     float mx = 0.f;
 #pragma unroll
@@ -227,10 +227,12 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 // Each active lane loads 16 bytes at byte offset `voff` of the buffer; lane i's bytes land at
-// LDS byte address lds + 16 * i (lds uniform across the wave).
+// LDS byte address lds + 16 * i (lds uniform across the wave).  A scalar register that a vector instruction wrote
+// (v_readfirstlane, a spilled one's v_readlane) may be read by a memory instruction five wait states later at the
+// earliest; the compiler does not see into the assembly, so the wait is in it.
 __device__ __forceinline__ void dma16(srd_t srd, uint32_t lds, uint32_t voff) {
     lds = __builtin_amdgcn_readfirstlane(lds);
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds"
                  :
                  : "v"(voff), "s"(lds), "s"(srd)
                  : "memory", "m0");
