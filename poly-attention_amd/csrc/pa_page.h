@@ -48,6 +48,21 @@ __device__ __forceinline__ int64_t page_place(const PageDev& P, int b, int p) {
     return (unsigned)id < (unsigned)P.pages ? ((int64_t)id << P.lg) + (p & ((1 << P.lg) - 1)) : -1;
 }
 
+// The row whose packed tokens `tok` belongs to: the last one that starts at or before it, by the whole wave.
+__device__ __forceinline__ int page_find(const PageDev& P, int tok, int lane) {
+    int lo = 0, n = P.rows;  // starts[lo] <= tok, as starts[0] is 0
+    while (n > 1) {
+        const int step = (n + 63) >> 6;
+        const int r = lo + lane * step;
+        const uint64_t below = __ballot(lane * step < n && P.starts[min(r, P.rows)] <= tok);
+        // starts do not fall, so the lanes are the first ones; none: a table that was never extended
+        const int k = max(__popcll(below) - 1, 0);
+        lo += k * step;
+        n = min(step, n - k * step);
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
 inline int page_lg(int size) {
     int lg = 0;
     while ((1 << lg) < size) ++lg;

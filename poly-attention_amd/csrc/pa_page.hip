@@ -377,21 +377,6 @@ struct PageRowsDev {
     PageItemDev it[PA_MAX_ORDER + 2];
 };
 
-// The row whose packed tokens `tok` belongs to: the last one that starts at or before it, by the whole wave.
-__device__ __forceinline__ int page_find(const PageDev& P, int tok, int lane) {
-    int lo = 0, n = P.rows;  // starts[lo] <= tok, as starts[0] is 0
-    while (n > 1) {
-        const int step = (n + 63) >> 6;
-        const int r = lo + lane * step;
-        const uint64_t below = __ballot(lane * step < n && P.starts[min(r, P.rows)] <= tok);
-        // starts do not fall, so the lanes are the first ones; none: a table that was never extended
-        const int k = max(__popcll(below) - 1, 0);
-        lo += k * step;
-        n = min(step, n - k * step);
-    }
-    return __builtin_amdgcn_readfirstlane(lo);
-}
-
 template <typename T>
 __global__ __launch_bounds__(kPageThreads) void k_page_append(const PageRowsDev P) {
     constexpr int E = 16 / sizeof(T), U = 2;

@@ -28,6 +28,7 @@ struct PagedDev {
     int32_t target_min, least; // ... or this many, where units are smaller than this many chunks
     int64_t recs;              // records there are
     float scale, softclamp;
+    SoftClampDev sc;           // of the logits
     DraftRow q, out, vmul;     // of the inputs; vmul: the next level's projected values, where it is a middle one
     const char* keys;
     const char* values;
@@ -37,6 +38,8 @@ struct PagedDev {
     float* lses;
     float* ws_o;               // [record][kv head][tile][dim]
     float2* ws_s;              // [record][kv head][tile]: maximum (log2 units) and sum
+    uint8_t* flags;            // [unit][kv head][4]
+    int32_t units;             // at most
 };
 
 __device__ __forceinline__ int64_t paged_base(const PagedDev& P, int id, int hk) {  // in positions
@@ -49,8 +52,9 @@ struct PagedUnit {
     int tiles, tile;     // of the row, and the one asked for
     int splits, split;   // units of a tile, and the one asked for
     int size;            // chunks of a unit
-    int64_t rec;         // the record of the tile's first unit (splits > 1)
+    int rec;             // the record of the tile's first unit (splits > 1)
     int at;              // what was asked for, from the row's first
+    int64_t before;      // how many there are, where there is no such one
 };
 
 // chunks per unit for a batch of `total` tiles times chunks
@@ -71,7 +75,8 @@ __device__ __forceinline__ void paged_tiles(const PagedDev& P, const PageRow& r,
 // that are to be joined.
 enum { kUnits, kRows };
 
-// Finds unit (or row) `want` over all rows of the batch, by the whole wave; false past the last one.
+// Finds unit (or row) `want` over all rows of the batch, by the whole wave; false past the last one.  What it finds
+// is held in scalar registers, so that the branches and loops over it are scalar ones.
 template <int WHAT>
 __device__ __forceinline__ bool paged_find(const PagedDev& P, int64_t want, int lane, PagedUnit& U) {
     uint64_t total = 0;
@@ -90,8 +95,9 @@ __device__ __forceinline__ bool paged_find(const PagedDev& P, int64_t want, int 
         }
     }
     for (int off = 32; off > 0; off >>= 1) total += __shfl_xor((unsigned long long)total, off);
-    U.size = paged_size(P, total);
-    int64_t before = 0, recs = 0;
+    U.size = __builtin_amdgcn_readfirstlane(paged_size(P, total));
+    int64_t before = 0;
+    int recs = 0;
     for (int b0 = 0; b0 < P.p.rows; b0 += 64) {
         const int b = b0 + lane;
         PageRow r = r0;
@@ -108,9 +114,11 @@ __device__ __forceinline__ bool paged_find(const PagedDev& P, int64_t want, int 
         const int splits = (int)(((unsigned)chunks + U.size - 1) / U.size);
         const int units = tiles * splits, rec = splits > 1 ? units : 0;
         const int mine = WHAT == kUnits ? units : splits > 1 && tiles > 0 ? rows : 0;
-        int64_t incl = mine, incl_rec = rec;
+        int64_t incl = mine;
+        int incl_rec = rec;
         for (int off = 1; off < 64; off <<= 1) {
-            const int64_t x = __shfl_up(incl, off), y = __shfl_up(incl_rec, off);
+            const int64_t x = __shfl_up(incl, off);
+            const int y = __shfl_up(incl_rec, off);
             if (lane >= off) {
                 incl += x;
                 incl_rec += y;
@@ -127,29 +135,34 @@ __device__ __forceinline__ bool paged_find(const PagedDev& P, int64_t want, int 
             U.rows = __builtin_amdgcn_readlane(rows, l);
             U.tiles = __builtin_amdgcn_readlane(tiles, l);
             U.splits = __builtin_amdgcn_readlane(splits, l);
-            U.rec = recs + __shfl(incl_rec - rec, l);
+            U.rec = recs + __builtin_amdgcn_readlane(incl_rec - rec, l);
             U.at = __builtin_amdgcn_readfirstlane((int)(want - before - __shfl(incl - mine, l)));
             if (WHAT == kUnits) {
                 // the last tiles, which have most keys, first
-                const int t = U.at / U.splits;
+                const int t = __builtin_amdgcn_readfirstlane(U.at / U.splits);
                 U.split = U.at - t * U.splits;
                 U.tile = U.tiles - 1 - t;
             } else {
-                U.tile = U.at / P.tile;
+                U.tile = __builtin_amdgcn_readfirstlane(U.at / P.tile);
                 U.split = 0;
             }
-            U.rec += (int64_t)U.tile * U.splits;
+            U.rec += U.tile * U.splits;
             return true;
         }
         before += __shfl(incl, 63);
-        recs += __shfl(incl_rec, 63);
+        recs += __builtin_amdgcn_readlane(incl_rec, 63);
     }
+    U.before = before;
     return false;
 }
 
 // the positions that a tile's last token sees
 __device__ __forceinline__ int paged_keys(const PagedDev& P, const PagedUnit& U) {
-    return U.row.p0 + (min((U.tile + 1) * P.tile, U.rows) - 1) / P.rep + 1;
+    return U.row.p0 + __builtin_amdgcn_readfirstlane((min((U.tile + 1) * P.tile, U.rows) - 1) / P.rep) + 1;
+}
+// whether there is a record for each of the tile's units: there are as many as there can be
+__device__ __forceinline__ bool paged_recorded(const PagedDev& P, const PagedUnit& U) {
+    return U.rec >= 0 && (int64_t)U.rec + U.splits <= P.recs;
 }
 
 // Where a query row's results go.
@@ -210,75 +223,25 @@ __device__ __forceinline__ const T* paged_query(const PagedDev& P, const PagedUn
     return reinterpret_cast<const T*>(P.queries) + at * P.dim;
 }
 
-// Whether a word of two 16-bit (or one 32-bit) numbers holds one that is not finite.
+// acc, no number once a word of two 16-bit numbers (of one of 32 bits) held one that is not finite.
 template <typename T>
-__device__ __forceinline__ bool paged_odd(uint32_t w) {
-    if constexpr (sizeof(T) == 4) return (w & 0x7f800000u) == 0x7f800000u;
-    constexpr uint32_t e = std::is_same_v<T, f16> ? 0x7c00u : 0x7f80u;
-    return (w & e) == e || (w & (e << 16)) == e << 16;
+__device__ __forceinline__ float paged_odd(uint32_t w, float acc) {
+    if constexpr (sizeof(T) == 4) {
+        return fmaf(__uint_as_float(w), 0.f, acc);
+    } else if constexpr (std::is_same_v<T, f16>) {
+        typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, w), __builtin_bit_cast(v2, 0u), acc, false);
+    } else {
+        typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, w), __builtin_bit_cast(v2, 0u), acc, false);
+    }
 }
 
-// A unit's rows one after another, a wave each, position by position in fp32: the products of the matrix
-// instructions include a weight of 0 times the value of a position that a row does not see, which is no number where
-// the value is none.  Taken where such values lie behind a row's own position; 64 positions at a time, a
-// lane's score each, then a lane's features.
-template <typename T>
-__device__ __forceinline__ void paged_slow(const PagedDev& P, const PagedUnit& U, int hk, int begin, int cnt, int wave,
-                                                     int waves, int lane) {
-    const int r0 = U.tile * P.tile, nrows = min(P.tile, U.rows - r0);
-    for (int r = r0 + wave; r < r0 + nrows; r += waves) {
-        const T* const q = paged_query<T>(P, U, hk, r);
-        const int see = min(cnt, U.row.p0 + r / P.rep + 1 - begin);
-        float top = -INFINITY, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};  // features lane + 64 i
-        for (int j0 = 0; j0 < see; j0 += 64) {
-            const int j = min(j0 + lane, see - 1);
-            const int64_t place = page_place(P.p, U.b, begin + j);
-            int64_t at = -1;
-            float s = 0.f;
-            if (place >= 0) {
-                at = paged_base(P, (int)(place >> P.p.lg), hk) + (place & ((1 << P.p.lg) - 1));
-                const T* const k = reinterpret_cast<const T*>(P.keys) + at * P.dim;
-                if (q)
-                    for (int d = 0; d < P.dim; ++d) s = fmaf(to_f(q[d]), to_f(k[d]), s);
-            }
-            s *= P.scale;
-            if (P.softclamp > 0.f) s = P.softclamp * tanhf(s / P.softclamp);
-            if (P.bias && at >= 0) s += P.bias[at];
-            s = j0 + lane < see ? s * kLog2e : -INFINITY;
-            float t = fmaxf(top, s);
-            for (int off = 32; off > 0; off >>= 1) t = fmaxf(t, __shfl_xor(t, off));
-            const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t);
-            top = t;
-            const float w = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - (t == -INFINITY ? 0.f : t));
-            float add = w;
-            for (int off = 32; off > 0; off >>= 1) add += __shfl_xor(add, off);
-            sum = sum * f + add;
-            for (int i = 0; i < 4; ++i) y[i] *= f;
-            for (int k = 0; k < 64; ++k) {
-                const float wk = __shfl(w, k);
-                const int64_t ak = __shfl(at, k);
-                if (wk == 0.f || ak < 0) continue;
-                const T* const v = reinterpret_cast<const T*>(P.values) + ak * P.dim;
-                for (int i = 0; i < 4; ++i)
-                    if (lane + 64 * i < P.dim) y[i] = fmaf(wk, to_f(v[lane + 64 * i]), y[i]);
-            }
-        }
-        if (U.splits > 1) {
-            const int64_t rec = ((U.rec + U.split) * P.kv_heads + hk) * P.tile + r - r0;
-            if (lane == 0) P.ws_s[rec] = make_float2(top, sum);
-            for (int i = 0; i < 4; ++i)
-                if (lane + 64 * i < P.dim) P.ws_o[rec * P.dim + lane + 64 * i] = y[i];
-        } else {
-            const PagedTo to = paged_to<T>(P, U, hk, r);
-            if (lane == 0 && to.lse) *to.lse = (top + log2f(sum)) * kLn2;
-            for (int i = 0; i < 4; ++i)
-                if (to.out && lane + 64 * i < P.dim) {
-                    float x = y[i] / sum;
-                    if (to.mul) x *= to_f(reinterpret_cast<const T*>(to.mul)[lane + 64 * i]);
-                    reinterpret_cast<T*>(to.out)[lane + 64 * i] = from_f<T>(x);
-                }
-        }
-    }
+// Where values that are not finite lie behind some row's own position, the products are no numbers: a weight of 0
+// times such a value.  A unit says so by a sum that is no number, in its records, or where it is its tile's only one by
+// a byte for each of its waves; k_paged_join then forms the rows again, one after another.
+__device__ __forceinline__ uint8_t* paged_flag(const PagedDev& P, int wave) {
+    return P.flags + 4 * (int64_t)blockIdx.x + wave;
 }
 
 // 16-row tiles of the workgroup's rows: what its registers hold
@@ -291,5 +254,10 @@ template <typename T> void launch_paged_rows(const PagedDev& P, int64_t units, i
 extern template void launch_paged_rows<bf16>(const PagedDev& P, int64_t units, int tiles, hipStream_t s);
 extern template void launch_paged_rows<f16>(const PagedDev& P, int64_t units, int tiles, hipStream_t s);
 extern template void launch_paged_rows<float>(const PagedDev& P, int64_t units, int tiles, hipStream_t s);
+// 16-bit chunks of more rows (k_paged_tiles), head dims up to 128
+constexpr int paged_tile_rows(int D) { return 256; }
+template <typename T> void launch_paged_tiles(const PagedDev& P, int64_t units, hipStream_t s);
+extern template void launch_paged_tiles<bf16>(const PagedDev& P, int64_t units, hipStream_t s);
+extern template void launch_paged_tiles<f16>(const PagedDev& P, int64_t units, hipStream_t s);
 
 }  // namespace pa

@@ -6,24 +6,98 @@
 
 namespace pa {
 
-// A query row of a tile that was split, per workgroup: its units dealt out over parts of the workgroup, four
-// features a thread.  The final level's launch also clears the outputs of tokens behind their chunk.
+// A query row position by position in fp32, by the workgroup: its waves take 64 positions at a time in turn, a lane's
+// score each, then a lane's features.  A position that the row does not see takes no part.
+struct SlowRow {
+    float top[4], sum[4], y[4][256];
+};
 template <typename T>
-__global__ __launch_bounds__(kPageThreads) void k_paged_join(const PagedDev P) {
-    __shared__ float s_red[kPageThreads][6];
+__device__ __forceinline__ void paged_slow(const PagedDev& P, const PagedUnit& U, int hk, int r, SlowRow& S) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const T* const q = paged_query<T>(P, U, hk, r);
+    const int see = U.row.p0 + r / P.rep + 1;
+    float top = -INFINITY, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};  // features lane + 64 i
+    for (int j0 = 64 * wave; j0 < see; j0 += 256) {
+        const int64_t place = page_place(P.p, U.b, min(j0 + lane, see - 1));
+        int64_t at = -1;
+        float s = 0.f;
+        if (place >= 0) {
+            at = paged_base(P, (int)(place >> P.p.lg), hk) + (place & ((1 << P.p.lg) - 1));
+            const T* const k = reinterpret_cast<const T*>(P.keys) + at * P.dim;
+            if (q)
+                for (int d = 0; d < P.dim; ++d) s = fmaf(to_f(q[d]), to_f(k[d]), s);
+        }
+        s *= P.scale;
+        if (P.softclamp > 0.f) s = P.softclamp * tanhf(s / P.softclamp);
+        if (P.bias && at >= 0) s += P.bias[at];
+        s = j0 + lane < see ? s * kLog2e : -INFINITY;
+        float t = fmaxf(top, s);
+        for (int off = 32; off > 0; off >>= 1) t = fmaxf(t, __shfl_xor(t, off));
+        const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t);
+        top = t;
+        const float w = s == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s - t);
+        float add = w;
+        for (int off = 32; off > 0; off >>= 1) add += __shfl_xor(add, off);
+        sum = sum * f + add;
+        for (int i = 0; i < 4; ++i) y[i] *= f;
+        for (int k = 0; k < min(64, see - j0); ++k) {
+            const float wk = __shfl(w, k);
+            const int64_t ak = __shfl(at, k);
+            if (wk == 0.f || ak < 0) continue;
+            const T* const v = reinterpret_cast<const T*>(P.values) + ak * P.dim;
+            for (int i = 0; i < 4; ++i)
+                if (lane + 64 * i < P.dim) y[i] = fmaf(wk, to_f(v[lane + 64 * i]), y[i]);
+        }
+    }
+    __syncthreads();  // S has been read
+    if (lane == 0) {
+        S.top[wave] = top;
+        S.sum[wave] = sum;
+    }
+    for (int i = 0; i < 4; ++i) S.y[wave][lane + 64 * i] = y[i];
+    __syncthreads();
+    if (wave) return;
+    // a maximum that is no number is passed over above, and shows in the sums
+    const float t = fmaxf(fmaxf(S.top[0], S.top[1]), fmaxf(S.top[2], S.top[3]));
+    sum = 0.f;
+    for (int i = 0; i < 4; ++i) y[i] = 0.f;
+    for (int w = 0; w < 4; ++w) {
+        if (64 * w >= see) break;  // had no position
+        const float f = __builtin_amdgcn_exp2f(S.top[w] - t);
+        if (f == 0.f) continue;
+        sum += S.sum[w] * f;
+        for (int i = 0; i < 4; ++i) y[i] += S.y[w][lane + 64 * i] * f;
+    }
+    const PagedTo to = paged_to<T>(P, U, hk, r);
+    if (lane == 0 && to.lse) *to.lse = (t + log2f(sum)) * kLn2;
+    for (int i = 0; i < 4; ++i)
+        if (to.out && lane + 64 * i < P.dim) {
+            float x = y[i] / sum;
+            if (to.mul) x *= to_f(reinterpret_cast<const T*>(to.mul)[lane + 64 * i]);
+            reinterpret_cast<T*>(to.out)[lane + 64 * i] = from_f<T>(x);
+        }
+}
+
+// A query row of a tile that was split, per workgroup: its units dealt out over parts of the workgroup, four
+// features a thread.  A level's two launches (few rows, many) leave their records to one join.
+template <typename T>
+__device__ __forceinline__ void paged_join(const PagedDev& P, int64_t& item, int64_t step_items, float (*s_red)[6], SlowRow& S) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int quads = P.dim >> 2;
     int lgq = 0;
     while ((1 << lgq) < quads) ++lgq;                        // at most 64
     const int parts = kPageThreads >> lgq, part = tid >> lgq, d = (tid & ((1 << lgq) - 1)) * 4;
-    for (int64_t item = blockIdx.x;; item += gridDim.x) {
+    for (;; item += step_items) {
         const int hk = (int)(item % P.kv_heads);
         PagedUnit U;
-        if (!paged_find<kRows>(P, item / P.kv_heads, lane, U)) break;
+        if (!paged_find<kRows>(P, item / P.kv_heads, lane, U)) {
+            item -= U.before * P.kv_heads;  // the next launch's, from its first
+            return;
+        }
         const int live = min(U.splits, (paged_keys(P, U) + U.size * kPagedChunk - 1) / (U.size * kPagedChunk));
-        if (U.rec + live > P.recs) continue;  // there are as many as there can be
+        if (!paged_recorded(P, U)) continue;
         const int r = U.at - U.tile * P.tile;
-        const int64_t rec = (U.rec * P.kv_heads + hk) * P.tile + r, step = (int64_t)P.kv_heads * P.tile;
+        const int64_t rec = ((int64_t)U.rec * P.kv_heads + hk) * P.tile + r, step = (int64_t)P.kv_heads * P.tile;
         float top = -INFINITY, sum = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         if (d < P.dim) {
@@ -60,7 +134,11 @@ __global__ __launch_bounds__(kPageThreads) void k_paged_join(const PagedDev P) {
         mine[3] = y.y;
         mine[4] = y.z;
         mine[5] = y.w;
-        __syncthreads();
+        // in every thread alike: a unit's sum is one number for all its features
+        if (__syncthreads_or(sum != sum)) {
+            paged_slow<T>(P, U, hk, U.at, S);
+            continue;
+        }
         if (part == 0 && d < P.dim) {
             float t = top;
             for (int k = 1; k < parts; ++k) t = fmaxf(t, s_red[(k << lgq) + tid][0]);
@@ -82,6 +160,28 @@ __global__ __launch_bounds__(kPageThreads) void k_paged_join(const PagedDev P) {
         __syncthreads();  // s_red is written again
     }
 }
+// The tiles of one unit that asked to be formed again.  Units that there are not have any flags.
+template <typename T>
+__device__ __forceinline__ void paged_again(const PagedDev& P, SlowRow& S) {
+    const int64_t all = (int64_t)P.units * P.kv_heads;
+    for (int64_t x = blockIdx.x; x < all; x += gridDim.x) {
+        if (reinterpret_cast<const uint32_t*>(P.flags)[x] == 0) continue;
+        PagedUnit U;
+        if (!paged_find<kUnits>(P, x / P.kv_heads, threadIdx.x & 63, U) || U.splits > 1) continue;
+        for (int r = U.tile * P.tile; r < min((U.tile + 1) * P.tile, U.rows); ++r)
+            paged_slow<T>(P, U, (int)(x % P.kv_heads), r, S);
+    }
+}
+template <typename T>
+__global__ __launch_bounds__(kPageThreads) void k_paged_join(const PagedDev A, const PagedDev B) {
+    __shared__ float s_red[kPageThreads][6];
+    __shared__ SlowRow s_slow;
+    int64_t item = blockIdx.x;
+    if (A.recs > 0) paged_join<T>(A, item, gridDim.x, s_red, s_slow);
+    if (B.recs > 0) paged_join<T>(B, item, gridDim.x, s_red, s_slow);
+    paged_again<T>(A, s_slow);
+    paged_again<T>(B, s_slow);
+}
 
 // Outputs of tokens behind their chunk: 0.  A wave per token.
 template <typename T>
@@ -89,33 +189,14 @@ __global__ __launch_bounds__(kPageThreads) void k_paged_clear(const PagedDev P) 
     const int lane = threadIdx.x & 63;
     const int64_t all = (int64_t)P.p.tokens * (P.p.packed ? 1 : P.p.rows), step = (int64_t)gridDim.x * (kPageThreads / 64);
     for (int64_t x = (int64_t)blockIdx.x * (kPageThreads / 64) + (threadIdx.x >> 6); x < all; x += step) {
-        int b, i;
-        if (P.p.packed) {
-            b = 0;
-            i = (int)x;
-            // the last row that starts at or before it
-            int lo = 0, n = P.p.rows;
-            while (n > 1) {
-                const int half = n >> 1;
-                if (P.p.starts[lo + half] <= i) {
-                    lo += half;
-                    n -= half;
-                } else {
-                    n = half;
-                }
-            }
-            b = lo;
-        } else {
-            b = (int)(x / P.p.tokens);
-            i = (int)(x - (int64_t)b * P.p.tokens);
-        }
+        const int b = P.p.packed ? page_find(P.p, (int)x, lane) : (int)(x / P.p.tokens);
+        const int i = (int)(P.p.packed ? x : x - (int64_t)b * P.p.tokens);
         const PageRow r = page_row(P.p, b);
-        if (i - r.start >= 0 && i - r.start < r.len) continue;
+        if (i >= r.start && i - r.start < r.len) continue;
         const int quads = P.dim >> 2, items = P.kv_heads * P.rep * quads;
-        const PagedTo to = {nullptr, nullptr, nullptr};
+        PagedTo at = {nullptr, nullptr, nullptr};
         for (int k = lane; k < items; k += 64) {
             const int h = k / quads, d = (k - h * quads) * 4;
-            PagedTo at = to;
             at.out = reinterpret_cast<char*>(P.out.at<T>(P.p.packed ? 0 : b, h) + (int64_t)i * P.out.sn);
             paged_store<T>(at, d, make_float4(0.f, 0.f, 0.f, 0.f));
         }
@@ -142,16 +223,19 @@ DraftRow paged_view(const pa_view& v) {
     return r;
 }
 
-constexpr int64_t kPagedCus = 256, kPagedMany = 4, kPagedFew = 2, kPagedUnitBytes = 64 * 1024;
+constexpr int64_t kPagedCus = 256, kPagedMany = 4, kPagedFew = 2, kPagedUnitBytes = 64 * 1024, kTilesMany = 2;
+// chunks of more query rows per key head than this go to k_paged_tiles, where it applies
+constexpr int kPagedFewRows = 32;
 
-// What a level's launch takes: its tiles and their split.
+// What a launch of a level takes: its tiles and their split.
 struct PagedPlan {
     int64_t units;  // at most
-    int tiles;      // 16-row tiles of a workgroup
-    size_t bytes;   // of its records
+    int tiles;      // 16-row tiles of a workgroup (few rows)
+    size_t records, flags;
 };
 
-PagedPlan paged_plan(const pa_paged* p, bool last, PagedDev& P) {
+// many: the launch of k_paged_tiles, or else that of k_paged_rows; both: there is the other one too
+PagedPlan paged_plan(const pa_paged* p, bool last, bool many, bool both, PagedDev& P) {
     const int rep = last ? p->heads / p->kv_heads : 1;
     const bool f32 = p->dtype == PA_F32;
     const int D = p->dim <= 64 ? 64 : p->dim <= 128 ? 128 : 256;
@@ -159,24 +243,40 @@ PagedPlan paged_plan(const pa_paged* p, bool last, PagedDev& P) {
     PagedPlan plan;
     plan.tiles = rows <= 16 ? 1 : f32 ? paged_row_tiles<float>(D) : paged_row_tiles<bf16>(D);
     P.rep = rep;
-    P.over = 0;
-    P.most = 1 << 30;
-    P.tile = 16 * plan.tiles;
-    const int64_t flight = kPagedCus * paged_waves(D, plan.tiles);
-    P.target = (int)std::max<int64_t>(1, kPagedMany * flight / p->kv_heads);
-    P.target_min = (int)std::max<int64_t>(1, kPagedFew * flight / p->kv_heads);
-    P.least = std::max(1, (int)(kPagedUnitBytes * plan.tiles / ((int64_t)kPagedChunk * p->dim * (f32 ? 4 : 2))));
-    const int64_t tiles = p->packed ? (rows + P.tile - 1) / P.tile + p->t.rows : (rows + P.tile - 1) / P.tile * p->t.rows;
+    P.over = many ? kPagedFewRows : 0;
+    P.most = many || !both ? 1 << 30 : kPagedFewRows;
+    P.tile = many ? paged_tile_rows(D) : 16 * plan.tiles;
+    const int64_t flight = kPagedCus * (many ? (D == 128 ? 1 : 2) : paged_waves(D, plan.tiles));
+    P.target = (int)std::max<int64_t>(1, (many ? kTilesMany : kPagedMany) * flight / p->kv_heads);
+    P.target_min = (int)std::max<int64_t>(1, (many ? 1 : kPagedFew) * flight / p->kv_heads);
+    P.least = many ? 4 : std::max(1, (int)(kPagedUnitBytes * plan.tiles / ((int64_t)kPagedChunk * p->dim * (f32 ? 4 : 2))));
+    // tiles of all rows: of chunks of at most P.most rows
+    const int64_t each = (std::min<int64_t>(rows, P.most) + P.tile - 1) / P.tile;
+    const int64_t tiles = p->packed ? std::min<int64_t>((rows + P.tile - 1) / P.tile + p->t.rows, each * p->t.rows)
+                                    : each * p->t.rows;
     // no more units than tiles times the table's chunks
     const int64_t chunks = ((int64_t)p->t.max_pages * p->t.page_size + kPagedChunk - 1) / kPagedChunk;
     plan.units = std::min(tiles + P.target, tiles * chunks);
     // a tile's units are at most twice their chunks over the unit's size where there are two or more
     P.recs = chunks > 1 ? std::min<int64_t>(2 * (int64_t)P.target, tiles * chunks) : 0;
-    plan.bytes = (size_t)P.recs * p->kv_heads * P.tile;  // records
+    plan.records = (size_t)P.recs * p->kv_heads * P.tile;
+    plan.flags = 4 * (size_t)plan.units * p->kv_heads;
+    P.units = (int)std::min<int64_t>(plan.units, 1 << 30);
     return plan;
 }
 
-size_t paged_bytes(size_t records, int dim) { return ((records * dim * 4 + 255) & ~size_t(255)) + records * sizeof(float2); }
+// Which launches a level has: one of few rows, unless every chunk has more; one of many, where chunks can have
+// them.  The scores' initial value is a logsumexp over the scale, so that has to be an ordinary number.
+void paged_launches(const pa_paged* p, bool last, bool& few, bool& many) {
+    const int64_t rows = (int64_t)p->tokens * (last ? p->heads / p->kv_heads : 1);
+    many = p->dtype != PA_F32 && p->dim <= 128 && p->scale >= 1e-6f && p->scale <= 1e6f && rows > kPagedFewRows;
+    few = true;
+}
+
+size_t paged_whole(size_t n) { return (n + 255) & ~size_t(255); }
+size_t paged_bytes(const PagedPlan& plan, int dim) {
+    return paged_whole(plan.records * dim * 4) + paged_whole(plan.records * sizeof(float2)) + paged_whole(plan.flags);
+}
 
 }  // namespace
 
@@ -184,7 +284,12 @@ size_t paged_attend_workspace(const pa_paged* p) {
     if (p->kv_heads < 1 || p->heads < 1 || p->tokens < 1 || p->t.rows < 1 || p->t.max_pages < 1 || !paged_dim(p->dim)) return 0;
     PagedDev P;
     size_t n = 16;
-    for (int last = 0; last < 2; ++last) n = std::max(n, paged_bytes(paged_plan(p, last, P).bytes, p->dim));
+    for (int last = 0; last < 2; ++last) {
+        // whatever the scale, which says whether there is a launch of many rows
+        const size_t a = paged_bytes(paged_plan(p, last, false, true, P), p->dim) +
+                         paged_bytes(paged_plan(p, last, true, true, P), p->dim);
+        n = std::max(n, std::max(a, paged_bytes(paged_plan(p, last, false, false, P), p->dim)));
+    }
     return n;
 }
 
@@ -216,15 +321,13 @@ int launch_paged_attend(const pa_paged* p, hipStream_t s) {
     P.softclamp = p->softclamp > 0.f ? p->softclamp : 0.f;
     if (!p->workspace || (uintptr_t)p->workspace % 16 != 0 || p->workspace_bytes < paged_attend_workspace(p))
         return PA_EWORKSPACE;
-    for (int t = 0; t < p->order; ++t) {
-        const bool last = t == p->order - 1;
-        const PagedPlan plan = paged_plan(p, last, P);
-        if (plan.units * p->kv_heads > kPageGroups) return PA_EUNSUPPORTED;
-    }
+    P.sc = soft_clamp_dev(P.scale, P.softclamp, true);
+    for (int last = 0; last < 2; ++last)
+        for (int many = 0; many < 2; ++many)
+            if (paged_plan(p, last, many, true, P).units * p->kv_heads > kPageGroups) return PA_EUNSUPPORTED;
     for (int t = 0; t < p->order; ++t) {
         const bool last = t == p->order - 1, middle_next = t + 1 < p->order - 1;
         const pa_paged_level& l = p->levels[t];
-        const PagedPlan plan = paged_plan(p, last, P);
         P.last = last;
         P.q = paged_view(p->q);
         P.out = paged_view(p->out);
@@ -236,22 +339,43 @@ int launch_paged_attend(const pa_paged* p, hipStream_t s) {
         P.queries = last ? nullptr : static_cast<const char*>(p->levels[t + 1].keys);
         P.next = last ? nullptr : static_cast<char*>(p->levels[t + 1].values);
         P.lses = last ? nullptr : l.lses;
-        P.ws_o = static_cast<float*>(p->workspace);
-        P.ws_s = reinterpret_cast<float2*>(static_cast<char*>(p->workspace) + ((plan.bytes * p->dim * 4 + 255) & ~size_t(255)));
-        {
+        char* ws = static_cast<char*>(p->workspace);
+        auto records = [&](PagedDev& Q, const PagedPlan& plan) {
+            Q.ws_o = reinterpret_cast<float*>(ws);
+            char* at = ws + paged_whole(plan.records * p->dim * 4);
+            Q.ws_s = reinterpret_cast<float2*>(at);
+            Q.flags = reinterpret_cast<uint8_t*>(at + paged_whole(plan.records * sizeof(float2)));
+            ws += paged_bytes(plan, p->dim);
+        };
+        bool few, many;
+        paged_launches(p, last, few, many);
+        PagedDev A = P, B = P;
+        A.recs = B.recs = 0;
+        A.units = B.units = 0;
+        if (few) {
+            const PagedPlan plan = paged_plan(p, last, false, many, A);
+            records(A, plan);
             ProfScope ps("paged_rows", s);
-            if (p->dtype == PA_F32) launch_paged_rows<float>(P, plan.units, plan.tiles, s);
-            else if (p->dtype == PA_F16) launch_paged_rows<f16>(P, plan.units, plan.tiles, s);
-            else launch_paged_rows<bf16>(P, plan.units, plan.tiles, s);
+            if (p->dtype == PA_F32) launch_paged_rows<float>(A, plan.units, plan.tiles, s);
+            else if (p->dtype == PA_F16) launch_paged_rows<f16>(A, plan.units, plan.tiles, s);
+            else launch_paged_rows<bf16>(A, plan.units, plan.tiles, s);
         }
-        if (P.recs > 0) {
-            const int64_t items = std::min<int64_t>(P.recs * P.tile, (int64_t)p->tokens * rep * rows) * p->kv_heads;
-            const dim3 grid((unsigned)std::min<int64_t>(items, 2048)), block(kPageThreads);
+        if (many) {
+            const PagedPlan plan = paged_plan(p, last, true, few, B);
+            records(B, plan);
+            ProfScope ps("paged_tiles", s);
+            if (p->dtype == PA_F16) launch_paged_tiles<f16>(B, plan.units, s);
+            else launch_paged_tiles<bf16>(B, plan.units, s);
+        }
+        {
+            const int64_t items = std::min<int64_t>(A.recs * A.tile + B.recs * B.tile, (int64_t)p->tokens * rep * rows) * p->kv_heads;
+            const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>(items, p->kv_heads), 2048)), block(kPageThreads);
             ProfScope ps("paged_join", s);
-            if (p->dtype == PA_F32) hipLaunchKernelGGL((k_paged_join<float>), grid, block, 0, s, P);
-            else if (p->dtype == PA_F16) hipLaunchKernelGGL((k_paged_join<f16>), grid, block, 0, s, P);
-            else hipLaunchKernelGGL((k_paged_join<bf16>), grid, block, 0, s, P);
+            if (p->dtype == PA_F32) hipLaunchKernelGGL((k_paged_join<float>), grid, block, 0, s, A, B);
+            else if (p->dtype == PA_F16) hipLaunchKernelGGL((k_paged_join<f16>), grid, block, 0, s, A, B);
+            else hipLaunchKernelGGL((k_paged_join<bf16>), grid, block, 0, s, A, B);
         }
+        P.rep = last ? (int)rep : 1;
     }
     const int64_t tokens = (int64_t)p->tokens * rows;
     const dim3 grid((unsigned)std::min<int64_t>((tokens + 3) / 4, 1024)), block(kPageThreads);

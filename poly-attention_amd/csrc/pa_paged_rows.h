@@ -31,7 +31,7 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int hk = blockIdx.x % P.kv_heads;
+    const int hk = __builtin_amdgcn_readfirstlane(blockIdx.x % P.kv_heads);
     PagedUnit U;
     if (!paged_find<kUnits>(P, blockIdx.x / P.kv_heads, lane, U)) return;
     const int r0 = U.tile * P.tile, nrows = min(P.tile, U.rows - r0), nrt = (nrows + 15) / 16;
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
     int see[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) see[rt] = U.row.p0 + min(r0 + 16 * rt + c, U.rows - 1) / P.rep - begin;
-    const int all_see = U.row.p0 + r0 / P.rep - begin;
+    const int all_see = U.row.p0 + __builtin_amdgcn_readfirstlane(r0 / P.rep) - begin;
 
     f32x4_t o[RT][VE];
     float m[RT], l[RT];
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
         for (int j = 0; j < VE; ++j) o[rt][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    bool odd = false;  // a value that is no number among those that some row does not see
+    float odd = 0.f;  // no number: a value that is not finite lies among those that some row does not see
     for (int j0 = first; j0 < cnt; j0 += STEP) {
         f32x4_t bias[KT];
 #pragma unroll
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
 #pragma unroll
             for (int n = 0; n < G::NP; ++n)
 #pragma unroll
-                for (int w = 0; w < G::VW; ++w) odd = odd || paged_odd<T>(v[n][w]);
+                for (int w = 0; w < G::VW; ++w) odd = paged_odd<T>(v[n][w], odd);
         }
         if (j0 + 16 * KT > cnt) {  // the unit's last positions
 #pragma unroll
@@ -336,8 +336,11 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
             s_l[wave][16 * rt + c] = l[rt];
         }
     }
-    const bool any = __any(odd);
-    if (lane == 0) s_odd[wave] = any;
+    const bool any = __any(odd != 0.f);
+    if (lane == 0) {
+        s_odd[wave] = any;
+        if (U.splits == 1) *paged_flag(P, wave) = any;
+    }
     __syncthreads();
     float f[RT];
 #pragma unroll
@@ -348,7 +351,7 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
         f[rt] = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - top);
     }
     const bool done = U.splits == 1;
-    const int64_t rec = ((U.rec + U.split) * P.kv_heads + hk) * P.tile;
+    const int64_t rec = ((int64_t)(U.rec + U.split) * P.kv_heads + hk) * P.tile;
     auto row_sum = [&](int r, float& top) __attribute__((always_inline)) -> float {
         top = s_m[0][r];
         for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][r]);
@@ -357,16 +360,12 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
             sum += s_m[w][r] == -INFINITY ? 0.f : s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - top);
         return sum;
     };
-    if (!done && U.rec + U.split >= P.recs) return;  // there are as many as there can be
-    if (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3]) {
-        paged_slow<T>(P, U, hk, begin, cnt, wave, 4, lane);
-        return;
-    }
+    if (!done && !paged_recorded(P, U)) return;
     if (tid < nrows) {
         float top;
         const float sum = row_sum(tid, top);
         if (!done) {
-            P.ws_s[rec + tid] = make_float2(top, sum);
+            P.ws_s[rec + tid] = make_float2(top, s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3] ? NAN : sum);
         } else if (!P.last) {
             const PagedTo to = paged_to<T>(P, U, hk, r0 + tid);
             if (to.lse) *to.lse = (top + log2f(sum)) * kLn2;
