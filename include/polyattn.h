@@ -59,6 +59,7 @@ extern "C" {
 #define PA_MAX_MOVES 128   /* array pairs of one pa_draft_commit */
 #define PA_TICKET_STRIDE 32  /* int32 per row of its tickets */
 #define PA_MAX_PAGE_ROWS 8192  /* rows of a page table */
+#define PA_PAGED_TICKETS 8192  /* tickets of pa_paged_attend; kv_heads up to half of it */
 
 /* status codes (0 = success, negative = failure) */
 #define PA_OK            0
@@ -576,6 +577,7 @@ typedef struct pa_paged {
     float          scale, softclamp;
     pa_view        q, out;      /* [rows or 1, heads, tokens, dim] */
     pa_paged_level levels[PA_MAX_ORDER];
+    int32_t*       tickets;     /* device [PA_PAGED_TICKETS * PA_TICKET_STRIDE], 0 before the first call and after each */
     void*          workspace;
     size_t         workspace_bytes;
 } pa_paged;

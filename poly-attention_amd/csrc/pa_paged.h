@@ -38,8 +38,10 @@ struct PagedDev {
     float* lses;
     float* ws_o;               // [record][kv head][tile][dim]
     float2* ws_s;              // [record][kv head][tile]: maximum (log2 units) and sum
-    uint8_t* flags;            // [unit][kv head][4]
+    uint8_t* flags;            // [unit][kv head][8]: its waves'
+    int32_t* tickets;          // [record][kv head][kTicketStride], 0 between launches
     int32_t units;             // at most
+    int32_t lgr;               // log2 of the rows that a workgroup of k_paged_join takes at once
 };
 
 __device__ __forceinline__ int64_t paged_base(const PagedDev& P, int id, int hk) {  // in positions
@@ -53,7 +55,7 @@ struct PagedUnit {
     int splits, split;   // units of a tile, and the one asked for
     int size;            // chunks of a unit
     int rec;             // the record of the tile's first unit (splits > 1)
-    int at;              // what was asked for, from the row's first
+    int at;              // what was asked for, from the row's first (kRows: its first row)
     int64_t before;      // how many there are, where there is no such one
 };
 
@@ -71,8 +73,8 @@ __device__ __forceinline__ void paged_tiles(const PagedDev& P, const PageRow& r,
     chunks = (r.n + kPagedChunk - 1) / kPagedChunk;
 }
 
-// What a row has of the things that are counted: kUnits, the records of its units, or (kRows) the query rows of tiles
-// that are to be joined.
+// What a row has of the things that are counted: kUnits, its units, or (kRows) blocks of 2^P.lgr query rows of tiles that
+// are to be joined.
 enum { kUnits, kRows };
 
 // Finds unit (or row) `want` over all rows of the batch, by the whole wave; false past the last one.  What it finds
@@ -113,7 +115,7 @@ __device__ __forceinline__ bool paged_find(const PagedDev& P, int64_t want, int 
         }
         const int splits = (int)(((unsigned)chunks + U.size - 1) / U.size);
         const int units = tiles * splits, rec = splits > 1 ? units : 0;
-        const int mine = WHAT == kUnits ? units : splits > 1 && tiles > 0 ? rows : 0;
+        const int mine = WHAT == kUnits ? units : splits > 1 && tiles > 0 ? (rows + (1 << P.lgr) - 1) >> P.lgr : 0;
         int64_t incl = mine;
         int incl_rec = rec;
         for (int off = 1; off < 64; off <<= 1) {
@@ -143,6 +145,7 @@ __device__ __forceinline__ bool paged_find(const PagedDev& P, int64_t want, int 
                 U.split = U.at - t * U.splits;
                 U.tile = U.tiles - 1 - t;
             } else {
+                U.at <<= P.lgr;  // the first of the rows
                 U.tile = __builtin_amdgcn_readfirstlane(U.at / P.tile);
                 U.split = 0;
             }
@@ -237,11 +240,129 @@ __device__ __forceinline__ float paged_odd(uint32_t w, float acc) {
     }
 }
 
-// Where values that are not finite lie behind some row's own position, the products are no numbers: a weight of 0
-// times such a value.  A unit says so by a sum that is no number, in its records, or where it is its tile's only one by
-// a byte for each of its waves; k_paged_join then forms the rows again, one after another.
+// Joins the units of `n` query rows of a tile, r first, and finishes them, by the workgroup: 2^lgr rows at a time, four
+// features a thread, the units dealt out over what is left of the threads.  RAW: the records may still be in another
+// XCD's way and are read at the GPU's level.  True where a unit's sum is no number (in every thread).
+template <typename T, bool RAW>
+__device__ __forceinline__ bool paged_join_rows(const PagedDev& P, const PagedUnit& U, int hk, int r, int n, int lgr, float (*s_red)[6]) {
+    const int tid = threadIdx.x;
+    const int quads = P.dim >> 2;
+    int lgq = 0;
+    while ((1 << lgq) < quads) ++lgq;  // at most 64
+    const int lgp = lgq + lgr, parts = kPageThreads >> lgp, part = tid >> lgp, d = (tid & ((1 << lgq) - 1)) * 4;
+    const int live = min(U.splits, (paged_keys(P, U) + U.size * kPagedChunk - 1) / (U.size * kPagedChunk));
+    const int64_t step = (int64_t)P.kv_heads * P.tile;
+    bool none = false;
+    for (int i = (tid >> lgq) & ((1 << lgr) - 1); i - ((tid >> lgq) & ((1 << lgr) - 1)) < n; i += 1 << lgr) {
+        const bool in = i < n && d < P.dim;
+        const int64_t rec = ((int64_t)U.rec * P.kv_heads + hk) * P.tile + r - U.tile * P.tile + i;
+        float top = -INFINITY, sum = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (in) {
+            constexpr int N = 4;
+            for (int u0 = part; u0 < live; u0 += N * parts) {
+                float2 ms[N];
+                float4 z[N];
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const int64_t at = rec + min(u0 + k * parts, live - 1) * step;
+                    if constexpr (RAW) {
+                        auto raw = [](const void* p) __attribute__((always_inline)) -> float2 {
+                            return __builtin_bit_cast(float2, __hip_atomic_load(static_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                                                                __HIP_MEMORY_SCOPE_AGENT));
+                        };
+                        ms[k] = raw(P.ws_s + at);
+                        const float2 a = raw(P.ws_o + at * P.dim + d), b = raw(P.ws_o + at * P.dim + d + 2);
+                        z[k] = make_float4(a.x, a.y, b.x, b.y);
+                    } else {
+                        ms[k] = P.ws_s[at];
+                        z[k] = *reinterpret_cast<const float4*>(P.ws_o + at * P.dim + d);
+                    }
+                }
+                float t = top;
+#pragma unroll
+                for (int k = 0; k < N; ++k) t = u0 + k * parts < live ? fmaxf(t, ms[k].x) : t;
+                const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t);
+                top = t;
+                sum *= f;
+                y = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    if (u0 + k * parts >= live || ms[k].x == -INFINITY) continue;
+                    const float w = __builtin_amdgcn_exp2f(ms[k].x - top);
+                    sum += ms[k].y * w;
+                    y = make_float4(fmaf(z[k].x, w, y.x), fmaf(z[k].y, w, y.y), fmaf(z[k].z, w, y.z), fmaf(z[k].w, w, y.w));
+                }
+            }
+        }
+        none = none || sum != sum;
+        if (parts > 1) {
+            float* const mine = s_red[tid];
+            mine[0] = top;
+            mine[1] = sum;
+            mine[2] = y.x;
+            mine[3] = y.y;
+            mine[4] = y.z;
+            mine[5] = y.w;
+            __syncthreads();
+            if (part == 0) {
+                float t = top;
+                for (int k = 1; k < parts; ++k) t = fmaxf(t, s_red[(k << lgp) + tid][0]);
+                const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t);
+                top = t;
+                sum *= f0;
+                y = make_float4(y.x * f0, y.y * f0, y.z * f0, y.w * f0);
+                for (int k = 1; k < parts; ++k) {
+                    const float* z = s_red[(k << lgp) + tid];
+                    if (z[0] == -INFINITY) continue;
+                    const float w = __builtin_amdgcn_exp2f(z[0] - t);
+                    sum += z[1] * w;
+                    y = make_float4(fmaf(z[2], w, y.x), fmaf(z[3], w, y.y), fmaf(z[4], w, y.z), fmaf(z[5], w, y.w));
+                }
+            }
+            __syncthreads();  // s_red is written again
+        }
+        if (part == 0 && in) {
+            const PagedTo to = paged_to<T>(P, U, hk, r + i);
+            const float inv = 1.f / sum;
+            if (to.out) paged_store<T>(to, d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+            if (d == 0 && to.lse) *to.lse = (top + log2f(sum)) * kLn2;
+        }
+    }
+    return none;
+}
+
+// A record's maximum and sum, and four of its features, at the GPU's level: read by whichever workgroup ends last.
+__device__ __forceinline__ void paged_raw(void* p, float a, float b) {
+    __hip_atomic_store(static_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, make_float2(a, b)), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Where values that are not finite lie behind some row's own position, the products of k_paged_tiles are no numbers: a
+// weight of 0 times such a value.  A unit says so by a sum that is no number, in its records, or where it is its tile's
+// only one by a byte for each of its waves; k_paged_join then forms the rows again, one after another.
 __device__ __forceinline__ uint8_t* paged_flag(const PagedDev& P, int wave) {
-    return P.flags + 4 * (int64_t)blockIdx.x + wave;
+    return P.flags + 8 * (int64_t)blockIdx.x + wave;
+}
+
+// Outputs of tokens behind their chunk: 0.  A wave per token, workgroup `group` of `groups`.
+template <typename T>
+__device__ __forceinline__ void paged_clear(const PagedDev& P, int group, int groups) {
+    const int lane = threadIdx.x & 63;
+    const int64_t all = (int64_t)P.p.tokens * (P.p.packed ? 1 : P.p.rows), step = (int64_t)groups * (kPageThreads / 64);
+    for (int64_t x = (int64_t)group * (kPageThreads / 64) + (threadIdx.x >> 6); x < all; x += step) {
+        const int b = P.p.packed ? page_find(P.p, (int)x, lane) : (int)(x / P.p.tokens);
+        const int i = (int)(P.p.packed ? x : x - (int64_t)b * P.p.tokens);
+        const PageRow r = page_row(P.p, b);
+        if (i >= r.start && i - r.start < r.len) continue;
+        const int quads = P.dim >> 2, items = P.kv_heads * P.rep * quads;
+        PagedTo at = {nullptr, nullptr, nullptr};
+        for (int k = lane; k < items; k += 64) {
+            const int h = k / quads, d = (k - h * quads) * 4;
+            at.out = reinterpret_cast<char*>(P.out.at<T>(P.p.packed ? 0 : b, h) + (int64_t)i * P.out.sn);
+            paged_store<T>(at, d, make_float4(0.f, 0.f, 0.f, 0.f));
+        }
+    }
 }
 
 // 16-row tiles of the workgroup's rows: what its registers hold
@@ -249,11 +370,12 @@ template <typename T> constexpr int paged_row_tiles(int D) { return D > 128 ? 1 
 // Waves per SIMD that the registers are held to
 constexpr int paged_waves(int D, int RT) { return D <= 128 && D * RT <= 256 ? 2 : 1; }
 
-template <typename T> void launch_paged_rows(const PagedDev& P, int64_t units, int tiles, hipStream_t s);
+// clear: workgroups that clear outputs, behind those of the units
+template <typename T> void launch_paged_rows(const PagedDev& P, int64_t units, int clear, int tiles, hipStream_t s);
 // in source files of their own
-extern template void launch_paged_rows<bf16>(const PagedDev& P, int64_t units, int tiles, hipStream_t s);
-extern template void launch_paged_rows<f16>(const PagedDev& P, int64_t units, int tiles, hipStream_t s);
-extern template void launch_paged_rows<float>(const PagedDev& P, int64_t units, int tiles, hipStream_t s);
+extern template void launch_paged_rows<bf16>(const PagedDev& P, int64_t units, int clear, int tiles, hipStream_t s);
+extern template void launch_paged_rows<f16>(const PagedDev& P, int64_t units, int clear, int tiles, hipStream_t s);
+extern template void launch_paged_rows<float>(const PagedDev& P, int64_t units, int clear, int tiles, hipStream_t s);
 // 16-bit chunks of more rows (k_paged_tiles), head dims up to 128
 constexpr int paged_tile_rows(int D) { return 256; }
 template <typename T> void launch_paged_tiles(const PagedDev& P, int64_t units, hipStream_t s);

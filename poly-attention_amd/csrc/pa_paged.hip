@@ -78,94 +78,26 @@ __device__ __forceinline__ void paged_slow(const PagedDev& P, const PagedUnit& U
         }
 }
 
-// A query row of a tile that was split, per workgroup: its units dealt out over parts of the workgroup, four
-// features a thread.  A level's two launches (few rows, many) leave their records to one join.
+// Blocks of rows of tiles that were split, a workgroup each.
 template <typename T>
-__device__ __forceinline__ void paged_join(const PagedDev& P, int64_t& item, int64_t step_items, float (*s_red)[6], SlowRow& S) {
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int quads = P.dim >> 2;
-    int lgq = 0;
-    while ((1 << lgq) < quads) ++lgq;                        // at most 64
-    const int parts = kPageThreads >> lgq, part = tid >> lgq, d = (tid & ((1 << lgq) - 1)) * 4;
-    for (;; item += step_items) {
+__device__ __forceinline__ void paged_join(const PagedDev& P, float (*s_red)[6], SlowRow& S) {
+    for (int64_t item = blockIdx.x;; item += gridDim.x) {
         const int hk = (int)(item % P.kv_heads);
         PagedUnit U;
-        if (!paged_find<kRows>(P, item / P.kv_heads, lane, U)) {
-            item -= U.before * P.kv_heads;  // the next launch's, from its first
-            return;
-        }
-        const int live = min(U.splits, (paged_keys(P, U) + U.size * kPagedChunk - 1) / (U.size * kPagedChunk));
+        if (!paged_find<kRows>(P, item / P.kv_heads, threadIdx.x & 63, U)) return;
         if (!paged_recorded(P, U)) continue;
-        const int r = U.at - U.tile * P.tile;
-        const int64_t rec = ((int64_t)U.rec * P.kv_heads + hk) * P.tile + r, step = (int64_t)P.kv_heads * P.tile;
-        float top = -INFINITY, sum = 0.f;
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (d < P.dim) {
-            constexpr int N = 4;
-            for (int u0 = part; u0 < live; u0 += N * parts) {
-                float2 ms[N];
-                float4 z[N];
-#pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    const int u = min(u0 + k * parts, live - 1);
-                    ms[k] = P.ws_s[rec + u * step];
-                    z[k] = *reinterpret_cast<const float4*>(P.ws_o + (rec + u * step) * P.dim + d);
-                }
-                float t = top;
-#pragma unroll
-                for (int k = 0; k < N; ++k) t = u0 + k * parts < live ? fmaxf(t, ms[k].x) : t;
-                const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t);
-                top = t;
-                sum *= f;
-                y = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
-#pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    if (u0 + k * parts >= live || ms[k].x == -INFINITY) continue;
-                    const float w = __builtin_amdgcn_exp2f(ms[k].x - top);
-                    sum += ms[k].y * w;
-                    y = make_float4(fmaf(z[k].x, w, y.x), fmaf(z[k].y, w, y.y), fmaf(z[k].z, w, y.z), fmaf(z[k].w, w, y.w));
-                }
-            }
-        }
-        float* const mine = s_red[tid];
-        mine[0] = top;
-        mine[1] = sum;
-        mine[2] = y.x;
-        mine[3] = y.y;
-        mine[4] = y.z;
-        mine[5] = y.w;
-        // in every thread alike: a unit's sum is one number for all its features
-        if (__syncthreads_or(sum != sum)) {
-            paged_slow<T>(P, U, hk, U.at, S);
-            continue;
-        }
-        if (part == 0 && d < P.dim) {
-            float t = top;
-            for (int k = 1; k < parts; ++k) t = fmaxf(t, s_red[(k << lgq) + tid][0]);
-            const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t);
-            sum *= f0;
-            y = make_float4(y.x * f0, y.y * f0, y.z * f0, y.w * f0);
-            for (int k = 1; k < parts; ++k) {
-                const float* z = s_red[(k << lgq) + tid];
-                if (z[0] == -INFINITY) continue;
-                const float w = __builtin_amdgcn_exp2f(z[0] - t);
-                sum += z[1] * w;
-                y = make_float4(fmaf(z[2], w, y.x), fmaf(z[3], w, y.y), fmaf(z[4], w, y.z), fmaf(z[5], w, y.w));
-            }
-            const PagedTo to = paged_to<T>(P, U, hk, U.at);
-            const float inv = 1.f / sum;
-            if (to.out) paged_store<T>(to, d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
-            if (d == 0 && to.lse) *to.lse = (t + log2f(sum)) * kLn2;
-        }
-        __syncthreads();  // s_red is written again
+        const int n = min(1 << P.lgr, U.rows - U.at);
+        if (__syncthreads_or(paged_join_rows<T, false>(P, U, hk, U.at, n, P.lgr, s_red)))
+            for (int r = U.at; r < U.at + n; ++r) paged_slow<T>(P, U, hk, r, S);
     }
 }
+
 // The tiles of one unit that asked to be formed again.  Units that there are not have any flags.
 template <typename T>
 __device__ __forceinline__ void paged_again(const PagedDev& P, SlowRow& S) {
     const int64_t all = (int64_t)P.units * P.kv_heads;
     for (int64_t x = blockIdx.x; x < all; x += gridDim.x) {
-        if (reinterpret_cast<const uint32_t*>(P.flags)[x] == 0) continue;
+        if (reinterpret_cast<const uint64_t*>(P.flags)[x] == 0) continue;
         PagedUnit U;
         if (!paged_find<kUnits>(P, x / P.kv_heads, threadIdx.x & 63, U) || U.splits > 1) continue;
         for (int r = U.tile * P.tile; r < min((U.tile + 1) * P.tile, U.rows); ++r)
@@ -173,34 +105,11 @@ __device__ __forceinline__ void paged_again(const PagedDev& P, SlowRow& S) {
     }
 }
 template <typename T>
-__global__ __launch_bounds__(kPageThreads) void k_paged_join(const PagedDev A, const PagedDev B) {
+__global__ __launch_bounds__(kPageThreads) void k_paged_join(const PagedDev P) {
     __shared__ float s_red[kPageThreads][6];
     __shared__ SlowRow s_slow;
-    int64_t item = blockIdx.x;
-    if (A.recs > 0) paged_join<T>(A, item, gridDim.x, s_red, s_slow);
-    if (B.recs > 0) paged_join<T>(B, item, gridDim.x, s_red, s_slow);
-    paged_again<T>(A, s_slow);
-    paged_again<T>(B, s_slow);
-}
-
-// Outputs of tokens behind their chunk: 0.  A wave per token.
-template <typename T>
-__global__ __launch_bounds__(kPageThreads) void k_paged_clear(const PagedDev P) {
-    const int lane = threadIdx.x & 63;
-    const int64_t all = (int64_t)P.p.tokens * (P.p.packed ? 1 : P.p.rows), step = (int64_t)gridDim.x * (kPageThreads / 64);
-    for (int64_t x = (int64_t)blockIdx.x * (kPageThreads / 64) + (threadIdx.x >> 6); x < all; x += step) {
-        const int b = P.p.packed ? page_find(P.p, (int)x, lane) : (int)(x / P.p.tokens);
-        const int i = (int)(P.p.packed ? x : x - (int64_t)b * P.p.tokens);
-        const PageRow r = page_row(P.p, b);
-        if (i >= r.start && i - r.start < r.len) continue;
-        const int quads = P.dim >> 2, items = P.kv_heads * P.rep * quads;
-        PagedTo at = {nullptr, nullptr, nullptr};
-        for (int k = lane; k < items; k += 64) {
-            const int h = k / quads, d = (k - h * quads) * 4;
-            at.out = reinterpret_cast<char*>(P.out.at<T>(P.p.packed ? 0 : b, h) + (int64_t)i * P.out.sn);
-            paged_store<T>(at, d, make_float4(0.f, 0.f, 0.f, 0.f));
-        }
-    }
+    if (P.recs > 0) paged_join<T>(P, s_red, s_slow);
+    paged_again<T>(P, s_slow);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -260,17 +169,19 @@ PagedPlan paged_plan(const pa_paged* p, bool last, bool many, bool both, PagedDe
     // a tile's units are at most twice their chunks over the unit's size where there are two or more
     P.recs = chunks > 1 ? std::min<int64_t>(2 * (int64_t)P.target, tiles * chunks) : 0;
     plan.records = (size_t)P.recs * p->kv_heads * P.tile;
-    plan.flags = 4 * (size_t)plan.units * p->kv_heads;
+    plan.flags = 8 * (size_t)plan.units * p->kv_heads;
     P.units = (int)std::min<int64_t>(plan.units, 1 << 30);
+    // as many rows as the workgroup has threads for (many rows: the units are few), within a tile
+    P.lgr = 0;
+    while (P.lgr < 4 && (((p->dim >> 2) - 1) >> (8 - P.lgr - 1)) == 0) ++P.lgr;
     return plan;
 }
 
-// Which launches a level has: one of few rows, unless every chunk has more; one of many, where chunks can have
-// them.  The scores' initial value is a logsumexp over the scale, so that has to be an ordinary number.
-void paged_launches(const pa_paged* p, bool last, bool& few, bool& many) {
+// Whether a level has a launch of many rows beside that of few: where chunks can have them.  The scores' initial value
+// is a logsumexp over the scale, so that has to be an ordinary number.
+bool paged_many(const pa_paged* p, bool last) {
     const int64_t rows = (int64_t)p->tokens * (last ? p->heads / p->kv_heads : 1);
-    many = p->dtype != PA_F32 && p->dim <= 128 && p->scale >= 1e-6f && p->scale <= 1e6f && rows > kPagedFewRows;
-    few = true;
+    return p->dtype != PA_F32 && p->dim <= 128 && p->scale >= 1e-6f && p->scale <= 1e6f && rows > kPagedFewRows;
 }
 
 size_t paged_whole(size_t n) { return (n + 255) & ~size_t(255); }
@@ -303,6 +214,7 @@ int launch_paged_attend(const pa_paged* p, hipStream_t s) {
     const int64_t rep = p->heads / p->kv_heads;
     if (p->tokens * rep > (1 << 30)) return PA_EUNSUPPORTED;
     auto view_ok = [&](const pa_view& v, int heads) { return v.ptr && v.heads == heads && v.dtype == p->dtype; };
+    if (!p->tickets || p->kv_heads > PA_PAGED_TICKETS / 2) return p->tickets ? PA_EUNSUPPORTED : PA_EINVAL;
     if (!view_ok(p->q, p->heads) || !view_ok(p->out, p->heads)) return PA_EINVAL;
     if (!paged_rows16(p->q) || !paged_rows16(p->out)) return PA_EUNSUPPORTED;
     for (int t = 0; t < p->order; ++t) {
@@ -347,42 +259,35 @@ int launch_paged_attend(const pa_paged* p, hipStream_t s) {
             Q.flags = reinterpret_cast<uint8_t*>(at + paged_whole(plan.records * sizeof(float2)));
             ws += paged_bytes(plan, p->dim);
         };
-        bool few, many;
-        paged_launches(p, last, few, many);
-        PagedDev A = P, B = P;
-        A.recs = B.recs = 0;
-        A.units = B.units = 0;
-        if (few) {
+        const bool many = paged_many(p, last);
+        {
+            PagedDev A = P;
             const PagedPlan plan = paged_plan(p, last, false, many, A);
             records(A, plan);
+            A.tickets = p->tickets;
+            // the final level's launch clears the outputs of tokens behind their chunk, too
+            const int clear = last ? (int)std::min<int64_t>(((int64_t)p->tokens * rows + 3) / 4, 512) : 0;
             ProfScope ps("paged_rows", s);
-            if (p->dtype == PA_F32) launch_paged_rows<float>(A, plan.units, plan.tiles, s);
-            else if (p->dtype == PA_F16) launch_paged_rows<f16>(A, plan.units, plan.tiles, s);
-            else launch_paged_rows<bf16>(A, plan.units, plan.tiles, s);
+            if (p->dtype == PA_F32) launch_paged_rows<float>(A, plan.units, clear, plan.tiles, s);
+            else if (p->dtype == PA_F16) launch_paged_rows<f16>(A, plan.units, clear, plan.tiles, s);
+            else launch_paged_rows<bf16>(A, plan.units, clear, plan.tiles, s);
         }
         if (many) {
-            const PagedPlan plan = paged_plan(p, last, true, few, B);
+            PagedDev B = P;
+            const PagedPlan plan = paged_plan(p, last, true, true, B);
             records(B, plan);
-            ProfScope ps("paged_tiles", s);
-            if (p->dtype == PA_F16) launch_paged_tiles<f16>(B, plan.units, s);
-            else launch_paged_tiles<bf16>(B, plan.units, s);
-        }
-        {
-            const int64_t items = std::min<int64_t>(A.recs * A.tile + B.recs * B.tile, (int64_t)p->tokens * rep * rows) * p->kv_heads;
-            const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>(items, p->kv_heads), 2048)), block(kPageThreads);
+            {
+                ProfScope ps("paged_tiles", s);
+                if (p->dtype == PA_F16) launch_paged_tiles<f16>(B, plan.units, s);
+                else launch_paged_tiles<bf16>(B, plan.units, s);
+            }
+            const int64_t blocks = ((int64_t)p->tokens * rows * B.rep >> B.lgr) + p->t.rows;
+            const dim3 grid((unsigned)std::min<int64_t>(blocks * p->kv_heads, 2048)), block(kPageThreads);
             ProfScope ps("paged_join", s);
-            if (p->dtype == PA_F32) hipLaunchKernelGGL((k_paged_join<float>), grid, block, 0, s, A, B);
-            else if (p->dtype == PA_F16) hipLaunchKernelGGL((k_paged_join<f16>), grid, block, 0, s, A, B);
-            else hipLaunchKernelGGL((k_paged_join<bf16>), grid, block, 0, s, A, B);
+            if (p->dtype == PA_F16) hipLaunchKernelGGL((k_paged_join<f16>), grid, block, 0, s, B);
+            else hipLaunchKernelGGL((k_paged_join<bf16>), grid, block, 0, s, B);
         }
-        P.rep = last ? (int)rep : 1;
     }
-    const int64_t tokens = (int64_t)p->tokens * rows;
-    const dim3 grid((unsigned)std::min<int64_t>((tokens + 3) / 4, 1024)), block(kPageThreads);
-    ProfScope ps("paged_clear", s);
-    if (p->dtype == PA_F32) hipLaunchKernelGGL((k_paged_clear<float>), grid, block, 0, s, P);
-    else if (p->dtype == PA_F16) hipLaunchKernelGGL((k_paged_clear<f16>), grid, block, 0, s, P);
-    else hipLaunchKernelGGL((k_paged_clear<bf16>), grid, block, 0, s, P);
     return PA_OK;
 }
 

@@ -11,6 +11,23 @@
 
 namespace pa {
 
+// one of a word's numbers, and the word without those that are not finite
+template <typename T>
+__device__ __forceinline__ float paged_number(uint32_t w, int half) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+    else return (float)__builtin_bit_cast(T, (uint16_t)(half ? w >> 16 : w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t paged_finite(uint32_t w) {
+    if constexpr (sizeof(T) == 4) {
+        return paged_number<T>(w, 0) * 0.f == 0.f ? w : 0u;
+    } else {
+        return (paged_number<T>(w, 0) * 0.f == 0.f ? w & 0xffffu : 0u) | (paged_number<T>(w, 1) * 0.f == 0.f ? w & 0xffff0000u : 0u);
+    }
+}
+// keeps a rarely taken branch one
+__device__ __forceinline__ void keep_branch_rows() { asm volatile("" ::: "memory"); }
+
 template <typename T, int D, int RT>
 __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows(const PagedDev P) {
     typedef DraftGeo<T, D> G;
@@ -26,11 +43,16 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
     __shared__ __align__(16) float s_o[NB * OWORDS > INWORDS ? NB * OWORDS : INWORDS];  // queries and keys, then these
     u32x4_d* const s_q = reinterpret_cast<u32x4_d*>(s_o);
     __shared__ float s_m[4][16 * RT], s_l[4][16 * RT];
-    __shared__ int s_odd[4];
+    __shared__ int s_last;
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
+    const int main = P.units * P.kv_heads;
+    if ((int)blockIdx.x >= main) {
+        paged_clear<T>(P, blockIdx.x - main, gridDim.x - main);
+        return;
+    }
     const int hk = __builtin_amdgcn_readfirstlane(blockIdx.x % P.kv_heads);
     PagedUnit U;
     if (!paged_find<kUnits>(P, blockIdx.x / P.kv_heads, lane, U)) return;
@@ -163,7 +185,6 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
         for (int j = 0; j < VE; ++j) o[rt][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    float odd = 0.f;  // no number: a value that is not finite lies among those that some row does not see
     for (int j0 = first; j0 < cnt; j0 += STEP) {
         f32x4_t bias[KT];
 #pragma unroll
@@ -226,6 +247,7 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) x[rt][t][i] = fmaf(bias[t][i], kLog2e, x[rt][t][i]);
         }
+        bool odd = false;  // a value that is not finite lies among positions that some row does not see
         if (j0 + 16 * KT - 1 > all_see) {  // positions that some row does not see, those past the unit among them
 #pragma unroll
             for (int t = 0; t < KT; ++t)
@@ -234,10 +256,12 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
                         if (j0 + 16 * t + 4 * g + i > see[rt]) x[rt][t][i] = -INFINITY;
+            float none = 0.f;
 #pragma unroll
             for (int n = 0; n < G::NP; ++n)
 #pragma unroll
-                for (int w = 0; w < G::VW; ++w) odd = paged_odd<T>(v[n][w], odd);
+                for (int w = 0; w < G::VW; ++w) none = paged_odd<T>(v[n][w], none);
+            odd = __any(none != 0.f);
         }
         if (j0 + 16 * KT > cnt) {  // the unit's last positions
 #pragma unroll
@@ -296,6 +320,37 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
                 }
             }
         }
+        if (odd) {
+            // a weight of 0 times such a value would be no number: they leave the products, and are added to the
+            // rows that see them one position after another
+            keep_branch_rows();
+#pragma unroll
+            for (int n = 0; n < G::NP; ++n) {
+                float none = 0.f;
+#pragma unroll
+                for (int w = 0; w < G::VW; ++w) none = paged_odd<T>(v[n][w], none);
+                const uint64_t who = __ballot(none != 0.f);
+                if (!who) continue;
+                for (int g2 = 0; g2 < 4; ++g2) {  // position 16 (n / 4) + 4 g2 + n % 4
+                    if (!((who >> (16 * g2)) & 0xffff)) continue;
+                    float p[RT];
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) p[rt] = __shfl(x[rt][n / 4][n % 4], 16 * g2 + c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < VE; ++j) {
+                            const uint32_t word = __shfl(v[n][G::F32 ? j : j / 2], 16 * g2 + 4 * g + i);
+                            const float z = paged_number<T>(word, G::F32 ? 0 : j & 1);
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt)
+                                if (z * 0.f != 0.f && p[rt] > 0.f) o[rt][j][i] += p[rt] * z;
+                        }
+                }
+#pragma unroll
+                for (int w = 0; w < G::VW; ++w) v[n][w] = paged_finite<T>(v[n][w]);
+            }
+        }
         // O^T += V^T P^T, feature j of every lane's VE per tile
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
@@ -336,11 +391,6 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
             s_l[wave][16 * rt + c] = l[rt];
         }
     }
-    const bool any = __any(odd != 0.f);
-    if (lane == 0) {
-        s_odd[wave] = any;
-        if (U.splits == 1) *paged_flag(P, wave) = any;
-    }
     __syncthreads();
     float f[RT];
 #pragma unroll
@@ -365,7 +415,7 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
         float top;
         const float sum = row_sum(tid, top);
         if (!done) {
-            P.ws_s[rec + tid] = make_float2(top, s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3] ? NAN : sum);
+            paged_raw(P.ws_s + rec + tid, top, sum);
         } else if (!P.last) {
             const PagedTo to = paged_to<T>(P, U, hk, r0 + tid);
             if (to.lse) *to.lse = (top + log2f(sum)) * kLn2;
@@ -415,17 +465,38 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
                     y.z += z.z;
                     y.w += z.w;
                 }
-                if (!done) *reinterpret_cast<float4*>(P.ws_o + (rec + 16 * rt + r) * P.dim + d) = y;
-                else if (to.out) paged_store<T>(to, d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+                if (!done) {
+                    float* const at = P.ws_o + (rec + 16 * rt + r) * P.dim + d;
+                    paged_raw(at, y.x, y.y);
+                    paged_raw(at + 2, y.z, y.w);
+                } else if (to.out) paged_store<T>(to, d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
             }
         }
         if (rt + 1 < RT) __syncthreads();
     }
+    if (done) return;
+    // The unit that ends last joins its tile's.  The records were written at the GPU's level, past this XCD's cache, and
+    // are there once the waves' stores have returned; a release would write the cache back, at several us.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int32_t* const ticket = P.tickets + ((int64_t)U.rec * P.kv_heads + hk) * kTicketStride;
+    const int live = min(U.splits, (paged_keys(P, U) + U.size * kPagedChunk - 1) / (U.size * kPagedChunk));
+    if (tid == 0) {
+        const int drawn = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_last = drawn == live - 1;
+        if (drawn == live - 1) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!s_last) return;
+    int lgr = 0;
+    while ((1 << lgr) < nrows && (P.dim << lgr) < 4 * kPageThreads) ++lgr;  // a quad of threads' features each
+    while (lgr > 0 && ((P.dim + 3) / 4 - 1) >> (8 - lgr)) --lgr;
+    paged_join_rows<T, true>(P, U, hk, r0, nrows, lgr, reinterpret_cast<float(*)[6]>(s_o));
 }
 
 template <typename T, int D>
-void launch_paged_rows_d(const PagedDev& P, int64_t units, int tiles, hipStream_t s) {
-    const dim3 grid((unsigned)(units * P.kv_heads)), block(kPageThreads);
+void launch_paged_rows_d(const PagedDev& P, int64_t units, int clear, int tiles, hipStream_t s) {
+    const dim3 grid((unsigned)(units * P.kv_heads + clear)), block(kPageThreads);
     if constexpr (paged_row_tiles<T>(D) >= 2)
         if (tiles == 2) {
             hipLaunchKernelGGL((k_paged_rows<T, D, 2>), grid, block, 0, s, P);
@@ -434,10 +505,10 @@ void launch_paged_rows_d(const PagedDev& P, int64_t units, int tiles, hipStream_
     hipLaunchKernelGGL((k_paged_rows<T, D, 1>), grid, block, 0, s, P);
 }
 template <typename T>
-void launch_paged_rows(const PagedDev& P, int64_t units, int tiles, hipStream_t s) {
-    if (P.dim <= 64) launch_paged_rows_d<T, 64>(P, units, tiles, s);
-    else if (P.dim <= 128) launch_paged_rows_d<T, 128>(P, units, tiles, s);
-    else launch_paged_rows_d<T, 256>(P, units, tiles, s);
+void launch_paged_rows(const PagedDev& P, int64_t units, int clear, int tiles, hipStream_t s) {
+    if (P.dim <= 64) launch_paged_rows_d<T, 64>(P, units, clear, tiles, s);
+    else if (P.dim <= 128) launch_paged_rows_d<T, 128>(P, units, clear, tiles, s);
+    else launch_paged_rows_d<T, 256>(P, units, clear, tiles, s);
 }
 
 }  // namespace pa

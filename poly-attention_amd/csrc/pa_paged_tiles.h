@@ -7,8 +7,10 @@
 // page: the loads of a wave go to one page each, whose number is a scalar from a register of 64 that is
 // loaded ahead.
 //
-// With two blocks of rows a wave, one's products run beside the other's exponentials, and each fragment read from
-// LDS feeds two products: with one, the reads of LDS alone would take as long as the products at head dim 128.
+// A wave works on two blocks of 32 x 32 scores at once, one's products beside the other's exponentials: two blocks of
+// rows at head dim 64, where each fragment read from LDS feeds two products; two of positions at 128, eight waves of 32
+// rows, since two blocks of rows there pass 256 registers, and copies between the two halves of the register file took
+// more than half the time (4096 tokens behind 4096, 32/8 heads: 672 us at the final level, ...).
 // No maximum is taken per tile: the probabilities are formed against the running one, and a tile whose sums
 // say that it was passed by far, or a row that has none yet, is formed again (kTileCap).  Scores get the logsumexp
 // of the level below as the products' initial value.
@@ -24,18 +26,23 @@ namespace pa {
 constexpr int kTileKeys = 64, kTileStages = 4;
 constexpr float kTileCap = 8192.f;  // of a lane's sum of a tile's probabilities
 
-template <typename T, int D, int QB, bool SOFTCLAMP, bool BIAS, bool LAST>
-__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void k_paged_tiles(const PagedDev P) {
+// waves of a workgroup, and 32-row blocks of a wave
+constexpr int paged_tile_waves(int D) { return D == 128 ? 8 : 4; }
+constexpr int paged_tile_blocks(int D) { return 8 / paged_tile_waves(D); }
+
+template <typename T, int D, bool SOFTCLAMP, bool BIAS, bool LAST>
+__global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(const PagedDev P) {
+    constexpr int NW = paged_tile_waves(D), QB = paged_tile_blocks(D), NT = 64 * NW;
     using M = Mma<T>;
     typedef typename M::frag frag;
-    constexpr int BN = kTileKeys, CPR = D / 8, NL = BN * CPR / 256, NSTG = kTileStages;
+    constexpr int BN = kTileKeys, CPR = D / 8, NL = BN * CPR / NT, NSTG = kTileStages;
     constexpr int ELEMS = BN * D;
     // fp16's smallest numbers are near: its weights are held 2^7 times larger
     constexpr float LIFT = draft_lift<T>();
     __shared__ __attribute__((aligned(16))) T sK[NSTG * ELEMS];
     __shared__ __attribute__((aligned(16))) T sV[NSTG * ELEMS];
     __shared__ __attribute__((aligned(16))) float sBraw[NSTG][BN];
-    __shared__ __attribute__((aligned(16))) float sBw[4][2][BN];  // a wave's, of a pair of tiles, in the scores' unit
+    __shared__ __attribute__((aligned(16))) float sBw[NW][2][BN];  // a wave's, of a pair of tiles, in the scores' unit
 
     const int tid = threadIdx.x, lane = tid & 63, w = wave_id();
     const int hh = lane >> 5, col = lane & 31;
@@ -88,7 +95,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void k_paged_tiles(const Pag
     ids_next = opaque(ids_next);
 
     const int rowb = P.dim * 2;
-    // a thread's 16-byte chunks of a tile, n * 256 + tid: row p / CPR, chunk p % CPR permuted by the row
+    // a thread's 16-byte chunks of a tile, n * NT + tid: row p / CPR, chunk p % CPR permuted by the row
     auto swz_key = [](int r) __attribute__((always_inline)) -> int {
         if (D == 64) {
             const int v = (r >> 1) & 7;
@@ -100,7 +107,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void k_paged_tiles(const Pag
     uint32_t offk[NL], offv[NL];
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
-        const int p = n * 256 + tid, r = p / CPR, ph = p % CPR;
+        const int p = n * NT + tid, r = p / CPR, ph = p % CPR;
         const int ck = ph ^ swz_key(r), cv = ph ^ swz_val(r);
         offk[n] = ck * 8 < P.dim ? (r & 15) * rowb + ck * 16 : kDraftOut;
         offv[n] = cv * 8 < P.dim ? (r & 15) * rowb + cv * 16 : kDraftOut;
@@ -115,15 +122,15 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void k_paged_tiles(const Pag
         const uint32_t kd = lds_k + (uint32_t)(stage * ELEMS * 2), vd = lds_v + (uint32_t)(stage * ELEMS * 2);
 #pragma unroll
         for (int n = 0; n < NL; ++n) {
-            const int j = j0 + ((n * 256 + w * 64) / CPR & ~15);  // the block of 16 that the wave's rows lie in
+            const int j = j0 + ((n * NT + w * 64) / CPR & ~15);  // the block of 16 that the wave's rows lie in
             const int id = __builtin_amdgcn_readlane(ids, (j >> 4) & 63);
             const bool ok = (unsigned)id < (unsigned)P.p.pages;
             const int64_t at = (paged_base(P, ok ? id : 0, hk) + ((begin + j) & inside)) * rowb;
             const uint32_t bytes = ok && j < cnt ? min(16, cnt - j) * rowb : 0;
-            dma16(make_srd(P.keys + at, bytes), kd + (uint32_t)((n * 256 + w * 64) * 16), offk[n]);
-            dma16(make_srd(P.values + at, bytes), vd + (uint32_t)((n * 256 + w * 64) * 16), offv[n]);
+            dma16(make_srd(P.keys + at, bytes), kd + (uint32_t)((n * NT + w * 64) * 16), offk[n]);
+            dma16(make_srd(P.values + at, bytes), vd + (uint32_t)((n * NT + w * 64) * 16), offv[n]);
         }
-        if (BIAS) {
+        if (BIAS && w < 4) {
             const int j = j0 + 16 * w;  // a quarter of the tile's
             const int id = __builtin_amdgcn_readlane(ids, (j >> 4) & 63);
             const bool ok = (unsigned)id < (unsigned)P.p.pages;
@@ -221,111 +228,120 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void k_paged_tiles(const Pag
         }
         l[u] += lt;
     };
-    constexpr int NK = D / 16, NV = 2 * (D / 32);  // products of a step's scores and averages, per block of rows
-    frag kf[NK];
-    auto load_keys = [&](int stage, int kb) __attribute__((always_inline)) {
+    constexpr int NK = D / 16, NV = 2 * (D / 32);  // products of 32 x 32 scores, and of their part of the averages
+    auto load_keys = [&](frag (&kf)[NK], int stage, int kb) __attribute__((always_inline)) {
 #pragma unroll
         for (int c = 0; c < NK; ++c) kf[c] = ld_frag<T>(sK + stage * ELEMS + kb * 32 * D + koff[c]);
     };
-    // 32 positions, keys in kf; the next step's are read on the way (next: its stage, or -1)
-    auto step = [&](int stage, int kb, int j0, int next, int next_kb) __attribute__((always_inline)) {
-        const T* const V = sV + stage * ELEMS + kb * 32 * D;
-        const float* const bias = &sBw[w][stage & 1][kb * 32 + 4 * hh];
-        const bool edge = j0 + 31 > all_see || j0 + 32 > cnt;
-        f32x16_t s[QB];
-        {
-            f32x16_t init = zero16();
-            if (BIAS && !SOFTCLAMP) {
+    auto load_values = [&](frag (&vf)[2][D / 32], int stage, int kb) __attribute__((always_inline)) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const float4 bb = *reinterpret_cast<const float4*>(bias + 8 * g);
-                    init[4 * g] = bb.x;
-                    init[4 * g + 1] = bb.y;
-                    init[4 * g + 2] = bb.z;
-                    init[4 * g + 3] = bb.w;
-                }
+        for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+                const T* base = sV + stage * ELEMS + (kb * 32 + 16 * t2) * D + voff[x];
+                const u32x2_t lo = lds_read_tr(base), hi = lds_read_tr(base + 8 * D);
+                const u32x4_t v4 = {lo[0], lo[1], hi[0], hi[1]};
+                vf[t2][x] = __builtin_bit_cast(frag, v4);
             }
+    };
+    auto check_values = [&](const frag (&vf)[2][D / 32]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < QB; ++u) s[u] = init;
+        for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+                const u32x4_t v4 = __builtin_bit_cast(u32x4_t, vf[t2][x]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd = paged_odd<T>(v4[e], odd);
+            }
+    };
+    auto first_scores = [&](const float* bias) __attribute__((always_inline)) -> f32x16_t {
+        f32x16_t init = zero16();
+        if (BIAS && !SOFTCLAMP) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 bb = *reinterpret_cast<const float4*>(bias + 8 * g);
+                init[4 * g] = bb.x;
+                init[4 * g + 1] = bb.y;
+                init[4 * g + 2] = bb.z;
+                init[4 * g + 3] = bb.w;
+            }
         }
-        // (A) scores of block 0
+        return init;
+    };
+    // Two blocks of 32 x 32 scores, of two blocks of rows (QB 2) or of positions: one's products run beside the other's
+    // exponentials.  (A) scores of the first; (B) scores of the second, probabilities of the first; (C) averages of
+    // the first, probabilities of the second; (D) averages of the second.
+    auto step = [&](int stage, int kb, int j0) __attribute__((always_inline)) {
+        constexpr int R1 = QB - 1;  // the second one's rows ...
+        const int kb1 = QB == 2 ? kb : 1, j1 = QB == 2 ? j0 : j0 + 32;  // ... and positions
+        const float* const bias = &sBw[w][stage & 1][4 * hh];
+        const bool edge = j0 + (QB == 2 ? 31 : 63) > all_see || j0 + (QB == 2 ? 32 : 64) > cnt;
+        frag k0[NK], k1[QB == 2 ? 1 : NK];
+        load_keys(k0, stage, kb);
+        f32x16_t s0 = first_scores(bias + 32 * kb);
 #pragma unroll
-        for (int c = 0; c < NK; ++c) s[0] = M::run(kf[c], qf[0][c], s[0]);
-        clamp(s[0], bias);
+        for (int c = 0; c < NK; ++c) s0 = M::run(k0[c], qf[0][c], s0);
+        if constexpr (QB == 1) {
+            __builtin_amdgcn_sched_barrier(0);
+            load_keys(k1, stage, 1);
+        }
+        f32x16_t s1 = first_scores(bias + 32 * kb1);
+        clamp(s0, bias + 32 * kb);
         if (edge) {
             keep_branch();
-            mask(s[0], 0, j0);
+            mask(s0, 0, j0);
         }
-        begin_rows(s[0], 0);
+        begin_rows(s0, 0);
         __builtin_amdgcn_sched_barrier(0);
-        // (B) scores of block 1 beside block 0's probabilities
-        u32x4_t pk0[2];
-        float lt0;
+        u32x4_t pk0[2], pk1[2];
+        float lt;
         {
             const float msub = without(m[0]);
             float lts[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
-                if constexpr (QB == 2) s[1] = M::run(kf[i], qf[1][i], s[1]);
-                if (i % (NK / 4) == 0) four(s[0], i / (NK / 4), msub, pk0, lts);
+                s1 = M::run(QB == 2 ? k0[i] : k1[QB == 2 ? 0 : i], qf[R1][i], s1);
+                if (i % (NK / 4) == 0) four(s0, i / (NK / 4), msub, pk0, lts);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            lt0 = (lts[0] + lts[1]) + (lts[2] + lts[3]);
+            lt = (lts[0] + lts[1]) + (lts[2] + lts[3]);
         }
-        frag vf[2][D / 32];
-#pragma unroll
-        for (int t2 = 0; t2 < 2; ++t2)
-#pragma unroll
-            for (int x = 0; x < D / 32; ++x) {
-                const T* base = V + 16 * t2 * D + voff[x];
-                const u32x2_t lo = lds_read_tr(base), hi = lds_read_tr(base + 8 * D);
-                const u32x4_t v4 = {lo[0], lo[1], hi[0], hi[1]};
-                vf[t2][x] = __builtin_bit_cast(frag, v4);
-            }
-        again(s[0], 0, lt0, pk0);
-        if (next >= 0) load_keys(next, next_kb);
+        frag v0[2][D / 32], v1[QB == 2 ? 1 : 2][D / 32];
+        load_values(v0, stage, kb);
+        again(s0, 0, lt, pk0);
+        clamp(s1, bias + 32 * kb1);
         if (edge) {
             keep_branch();
-#pragma unroll
-            for (int t2 = 0; t2 < 2; ++t2)
-#pragma unroll
-                for (int x = 0; x < D / 32; ++x) {
-                    const u32x4_t v4 = __builtin_bit_cast(u32x4_t, vf[t2][x]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) odd = paged_odd<T>(v4[e], odd);
-                }
+            check_values(v0);
+            mask(s1, R1, j1);
         }
-        if constexpr (QB == 2) {
-            clamp(s[1], bias);
-            if (edge) {
-                keep_branch();
-                mask(s[1], 1, j0);
-            }
-            begin_rows(s[1], 1);
-            __builtin_amdgcn_sched_barrier(0);
-            // (C) block 0's averages beside block 1's probabilities
-            u32x4_t pk1[2];
-            const float msub = without(m[1]);
+        begin_rows(s1, R1);
+        __builtin_amdgcn_sched_barrier(0);
+        {
+            const float msub = without(m[R1]);
             float lts[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int t2 = i / (D / 32), x = i % (D / 32);
-                o[0][x] = M::run(vf[t2][x], __builtin_bit_cast(frag, pk0[t2]), o[0][x]);
-                if (i % (NV / 4) == 0) four(s[1], i / (NV / 4), msub, pk1, lts);
+                o[0][x] = M::run(v0[t2][x], __builtin_bit_cast(frag, pk0[t2]), o[0][x]);
+                if (i % (NV / 4) == 0) four(s1, i / (NV / 4), msub, pk1, lts);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            again(s[1], 1, (lts[0] + lts[1]) + (lts[2] + lts[3]), pk1);
-            // (D) block 1's averages
-#pragma unroll
-            for (int t2 = 0; t2 < 2; ++t2)
-#pragma unroll
-                for (int x = 0; x < D / 32; ++x) o[1][x] = M::run(vf[t2][x], __builtin_bit_cast(frag, pk1[t2]), o[1][x]);
-        } else {
-#pragma unroll
-            for (int t2 = 0; t2 < 2; ++t2)
-#pragma unroll
-                for (int x = 0; x < D / 32; ++x) o[0][x] = M::run(vf[t2][x], __builtin_bit_cast(frag, pk0[t2]), o[0][x]);
+            lt = (lts[0] + lts[1]) + (lts[2] + lts[3]);
         }
+        if constexpr (QB == 1) load_values(v1, stage, 1);
+        again(s1, R1, lt, pk1);
+        if constexpr (QB == 1) {
+            if (edge) {
+                keep_branch();
+                check_values(v1);
+            }
+        }
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x)
+                o[R1][x] = M::run(QB == 2 ? v0[t2][x] : v1[QB == 2 ? 0 : t2][x], __builtin_bit_cast(frag, pk1[t2]), o[R1][x]);
     };
 
     // pairs of tiles, a barrier each: both have landed, and the pair before has been read
@@ -335,7 +351,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void k_paged_tiles(const Pag
         lds_barrier();
         if (t + 2 < ntl) issue((t + 2) * BN, st ^ 2);
         if (t + 3 < ntl) issue((t + 3) * BN, (st ^ 2) + 1);
-        const int j0 = t * BN, left = nact - 2 * t;  // steps of this pair, and further ones
+        const int j0 = t * BN, left = nact - 2 * t;  // 32-position steps of this pair, and further ones
         if (left <= 0) continue;  // the same barriers in every wave
         if (BIAS)
 #pragma unroll
@@ -343,16 +359,15 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void k_paged_tiles(const Pag
                 const int j = j0 + BN * k + lane;
                 sBw[w][k][lane] = j < cnt ? sBraw[st + k][lane] * bmul : -INFINITY;
             }
-        load_keys(st, 0);
-        step(st, 0, j0, left > 1 ? st : -1, 1);
-        if (left > 1) step(st, 1, j0 + 32, left > 2 ? st + 1 : -1, 0);
-        if (left > 2) step(st + 1, 0, j0 + 64, left > 3 ? st + 1 : -1, 1);
-        if (left > 3) step(st + 1, 1, j0 + 96, -1, 0);
+        step(st, 0, j0);
+        if (QB == 2 && left > 1) step(st, 1, j0 + 32);
+        if (left > 2) step(st + 1, 0, j0 + 64);
+        if (QB == 2 && left > 3) step(st + 1, 1, j0 + 96);
     }
 
     if (U.splits > 1 && !paged_recorded(P, U)) return;
     const bool any = __any(odd != 0.f);
-    if (U.splits == 1 && lane == 0) *paged_flag(P, w) = any;
+    if (U.splits == 1 && lane < 8 / NW) *paged_flag(P, w + NW * lane) = any;  // eight of them, whatever the waves
     const int64_t rec = ((int64_t)(U.rec + U.split) * P.kv_heads + hk) * P.tile;
 #pragma unroll
     for (int u = 0; u < QB; ++u) {
@@ -391,10 +406,10 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void k_paged_tiles(const Pag
 
 template <typename T, int D, bool SOFTCLAMP>
 void launch_paged_tiles_d(const PagedDev& P, int64_t units, hipStream_t s) {
-    const dim3 grid((unsigned)(units * P.kv_heads)), block(256);
-    if (P.last) hipLaunchKernelGGL((k_paged_tiles<T, D, 2, SOFTCLAMP, true, true>), grid, block, 0, s, P);
-    else if (P.bias) hipLaunchKernelGGL((k_paged_tiles<T, D, 2, SOFTCLAMP, true, false>), grid, block, 0, s, P);
-    else hipLaunchKernelGGL((k_paged_tiles<T, D, 2, SOFTCLAMP, false, false>), grid, block, 0, s, P);
+    const dim3 grid((unsigned)(units * P.kv_heads)), block(64 * paged_tile_waves(D));
+    if (P.last) hipLaunchKernelGGL((k_paged_tiles<T, D, SOFTCLAMP, true, true>), grid, block, 0, s, P);
+    else if (P.bias) hipLaunchKernelGGL((k_paged_tiles<T, D, SOFTCLAMP, true, false>), grid, block, 0, s, P);
+    else hipLaunchKernelGGL((k_paged_tiles<T, D, SOFTCLAMP, false, false>), grid, block, 0, s, P);
 }
 template <typename T>
 void launch_paged_tiles(const PagedDev& P, int64_t units, hipStream_t s) {

@@ -22,6 +22,7 @@ PA_MAX_DRAFTS = 64
 PA_MAX_MOVES = 128
 PA_TICKET_STRIDE = 32
 PA_MAX_PAGE_ROWS = 8192
+PA_PAGED_TICKETS = 8192
 
 PA_OK = 0
 PA_EINVAL = -1
@@ -465,6 +466,7 @@ class PaPaged(ctypes.Structure):
         ("q", PaView),
         ("out", PaView),
         ("levels", PaPagedLevel * PA_MAX_ORDER),
+        ("tickets", c_void_p),
         ("workspace", c_void_p),
         ("workspace_bytes", c_size_t),
     ]

@@ -224,6 +224,8 @@ class PagedCache:
         self.keys, self.values = rows(order), rows(order)
         self.lses = tuple(torch.empty(table.pool, kv_heads, table.page_size, dtype=torch.float32, device=table.device)
                           for _ in range(order - 1))
+        # of attend, 0 between calls
+        self._tickets = torch.zeros(_lib.PA_PAGED_TICKETS * _lib.PA_TICKET_STRIDE, dtype=torch.int32, device=table.device)
         self._plans: dict = {}
         table.caches.append(self)
         table._call_struct = None  # its list of arrays grows
@@ -428,5 +430,6 @@ class PagedCache:
         for x in (D.q, D.out):
             x.heads, x.dtype = H, code
         D.out.sb, D.out.sh, D.out.sn, _ = strides
+        D.tickets = self._tickets.data_ptr()
         D.workspace_bytes = _lib.load().pa_paged_attend_workspace(ctypes.byref(D))
         return D, strides, (B, self.kv_heads, T, d)

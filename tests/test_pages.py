@@ -107,7 +107,7 @@ def attend_args(order=3):
         if 0 < t < order - 1:
             view(L.vmul, 2)
     P.workspace_bytes = _lib.load().pa_paged_attend_workspace(ctypes.byref(P))
-    P.workspace = FAKE
+    P.workspace = P.tickets = FAKE
     return P
 
 
@@ -129,7 +129,7 @@ TABLE_REFUSALS = [("t.rows", 0, -1), ("t.pages", 0, -1), ("t.max_pages", 0, -1),
     ("dim", 0, -1), ("dim", 20, -2), ("dim", 264, -2), ("q.ptr", None, -1), ("out.ptr", None, -1), ("q.heads", 2, -1),
     ("q.dtype", _lib.PA_F16, -1), ("q.sn", 63, -2), ("out.ptr", FAKE + 8, -2), ("levels.0.keys", None, -1),
     ("levels.1.values", None, -1), ("levels.0.lses", None, -1), ("levels.1.vmul.ptr", None, -1),
-    ("levels.1.vmul.heads", 4, -1), ("levels.2.keys", FAKE + 4, -2), ("workspace", None, -4),
+    ("levels.1.vmul.heads", 4, -1), ("levels.2.keys", FAKE + 4, -2), ("workspace", None, -4), ("tickets", None, -1),
     ("workspace", FAKE + 8, -4), ("workspace_bytes", 15, -4), ("tokens", 1 << 30, -2)])
 def test_attend_refuses(path, value, want):
     lib = _lib.load()
