@@ -25,7 +25,8 @@ struct PagedDev {
     int32_t over, most;        // rows of a chunk, more than `over` and at most `most`, that a launch takes
     int32_t tile;              // rows of its tiles
     int32_t target;            // units aimed at over all rows ...
-    int32_t target_min, least; // ... or this many, where units are smaller than this many chunks
+    int32_t target_min, least; // ... or this many, where units are of at most so many chunks
+    int32_t fewest;            // chunks of a unit, at least
     int64_t recs;              // records there are
     float scale, softclamp;
     SoftClampDev sc;           // of the logits
@@ -53,17 +54,32 @@ struct PagedUnit {
     int b, rows;         // the batch row, its query rows per key head
     int tiles, tile;     // of the row, and the one asked for
     int splits, split;   // units of a tile, and the one asked for
-    int size;            // chunks of a unit
+    int size;            // chunks of the row's units
     int rec;             // the record of the tile's first unit (splits > 1)
     int at;              // what was asked for, from the row's first (kRows: its first row)
-    int64_t before;      // how many there are, where there is no such one
 };
 
-// chunks per unit for a batch of `total` tiles times chunks
-__device__ __forceinline__ int paged_size(const PagedDev& P, uint64_t total) {
-    const uint64_t many = (total + P.target - 1) / P.target, few = (total + P.target_min - 1) / P.target_min;
-    const uint64_t s = max(many, min(few, (uint64_t)P.least));
-    return (int)min(max<uint64_t>(s, 1), (uint64_t)kPagedMost);
+// Chunks per unit for `tiles` tiles of `total` chunks together: P.target units in all, or P.target_min where
+// those are of at most P.least chunks.  Each tile's last unit is half one on
+// average: there are total / size + tiles / 2 or so.
+__device__ __forceinline__ int paged_size(const PagedDev& P, uint64_t total, int tiles) {
+    auto chunks = [&](int target) __attribute__((always_inline)) -> uint32_t {
+        const uint32_t aim = max(target - tiles / 2, target / 2 + 1);
+        const uint64_t n = total >> 31 ? (total + aim - 1) / aim : (uint64_t)(((uint32_t)total + aim - 1) / aim);
+        return (uint32_t)min(n, (uint64_t)kPagedMost);
+    };
+    return (int)max(max(chunks(P.target), min(chunks(P.target_min), (uint32_t)P.least)), (uint32_t)P.fewest);
+}
+
+// sums of the lanes up to each, whole waves
+__device__ __forceinline__ int paged_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // rows of 16 lanes: shifted by 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // a row's last into the next row
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // the second row's into the upper half
+    return x;
 }
 
 // One row's tiles and chunks, 0 for a row that the launch does not take.
@@ -80,8 +96,9 @@ enum { kUnits, kRows };
 // Finds unit (or row) `want` over all rows of the batch, by the whole wave; false past the last one.  What it finds
 // is held in scalar registers, so that the branches and loops over it are scalar ones.
 template <int WHAT>
-__device__ __forceinline__ bool paged_find(const PagedDev& P, int64_t want, int lane, PagedUnit& U) {
+__device__ __forceinline__ bool paged_find(const PagedDev& P, int want, int lane, PagedUnit& U) {
     uint64_t total = 0;
+    int all_tiles = 0;
     PageRow r0;
     int rows0 = 0, tiles0 = 0, chunks0 = 0;  // this lane's row of the first 64
     for (int b = lane; b < P.p.rows; b += 64) {
@@ -89,6 +106,7 @@ __device__ __forceinline__ bool paged_find(const PagedDev& P, int64_t want, int 
         int rows, tiles, chunks;
         paged_tiles(P, r, rows, tiles, chunks);
         total += (uint64_t)tiles * chunks;
+        all_tiles += tiles;
         if (b < 64) {
             r0 = r;
             rows0 = rows;
@@ -96,10 +114,12 @@ __device__ __forceinline__ bool paged_find(const PagedDev& P, int64_t want, int 
             chunks0 = chunks;
         }
     }
-    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor((unsigned long long)total, off);
-    U.size = __builtin_amdgcn_readfirstlane(paged_size(P, total));
-    int64_t before = 0;
-    int recs = 0;
+    if (P.p.rows > 1)
+        for (int off = 32; off > 0; off >>= 1) total += __shfl_xor((unsigned long long)total, off);
+    const int all = __builtin_amdgcn_readlane(paged_scan(all_tiles), 63);
+    total = ((uint64_t)__builtin_amdgcn_readfirstlane((int)(total >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)total);
+    U.size = __builtin_amdgcn_readfirstlane(paged_size(P, total, all));
+    int before = 0, recs = 0;  // units are at most the grid's, and blocks of rows fewer than memory holds outputs of
     for (int b0 = 0; b0 < P.p.rows; b0 += 64) {
         const int b = b0 + lane;
         PageRow r = r0;
@@ -116,16 +136,7 @@ __device__ __forceinline__ bool paged_find(const PagedDev& P, int64_t want, int 
         const int splits = (int)(((unsigned)chunks + U.size - 1) / U.size);
         const int units = tiles * splits, rec = splits > 1 ? units : 0;
         const int mine = WHAT == kUnits ? units : splits > 1 && tiles > 0 ? (rows + (1 << P.lgr) - 1) >> P.lgr : 0;
-        int64_t incl = mine;
-        int incl_rec = rec;
-        for (int off = 1; off < 64; off <<= 1) {
-            const int64_t x = __shfl_up(incl, off);
-            const int y = __shfl_up(incl_rec, off);
-            if (lane >= off) {
-                incl += x;
-                incl_rec += y;
-            }
-        }
+        const int incl = paged_scan(mine), incl_rec = paged_scan(rec);
         const uint64_t past = __ballot(before + incl > want);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
@@ -137,8 +148,10 @@ __device__ __forceinline__ bool paged_find(const PagedDev& P, int64_t want, int 
             U.rows = __builtin_amdgcn_readlane(rows, l);
             U.tiles = __builtin_amdgcn_readlane(tiles, l);
             U.splits = __builtin_amdgcn_readlane(splits, l);
+            // the row's units of one size
+            U.size = __builtin_amdgcn_readfirstlane((int)(((unsigned)__builtin_amdgcn_readlane(chunks, l) + U.splits - 1) / U.splits));
             U.rec = recs + __builtin_amdgcn_readlane(incl_rec - rec, l);
-            U.at = __builtin_amdgcn_readfirstlane((int)(want - before - __shfl(incl - mine, l)));
+            U.at = want - before - __builtin_amdgcn_readlane(incl - mine, l);
             if (WHAT == kUnits) {
                 // the last tiles, which have most keys, first
                 const int t = __builtin_amdgcn_readfirstlane(U.at / U.splits);
@@ -152,10 +165,9 @@ __device__ __forceinline__ bool paged_find(const PagedDev& P, int64_t want, int 
             U.rec += U.tile * U.splits;
             return true;
         }
-        before += __shfl(incl, 63);
+        before += __builtin_amdgcn_readlane(incl, 63);
         recs += __builtin_amdgcn_readlane(incl_rec, 63);
     }
-    U.before = before;
     return false;
 }
 
@@ -240,93 +252,107 @@ __device__ __forceinline__ float paged_odd(uint32_t w, float acc) {
     }
 }
 
-// Joins the units of `n` query rows of a tile, r first, and finishes them, by the workgroup: 2^lgr rows at a time, four
-// features a thread, the units dealt out over what is left of the threads.  RAW: the records may still be in another
-// XCD's way and are read at the GPU's level.  True where a unit's sum is no number (in every thread).
-template <typename T, bool RAW>
+// a maximum and sum, or two features, of a record; RAW: read at the GPU's level, past this XCD's caches
+template <bool RAW>
+__device__ __forceinline__ float2 paged_pair(const void* p) {
+    if constexpr (RAW)
+        return __builtin_bit_cast(float2, __hip_atomic_load(static_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    else
+        return *static_cast<const float2*>(p);
+}
+
+// Joins the units of `n` query rows of a tile, r first, and finishes them, by the workgroup: M 2^lgr rows at a time, M of
+// them and four features a thread, the units dealt out over what is left of the threads, so that eight loads or so are
+// under way.  True where a unit's sum is no number (in every thread).
+template <typename T, bool RAW, int M>
 __device__ __forceinline__ bool paged_join_rows(const PagedDev& P, const PagedUnit& U, int hk, int r, int n, int lgr, float (*s_red)[6]) {
+    constexpr int N = M >= 4 ? 2 : M == 2 ? 4 : 6;
     const int tid = threadIdx.x;
     const int quads = P.dim >> 2;
     int lgq = 0;
     while ((1 << lgq) < quads) ++lgq;  // at most 64
     const int lgp = lgq + lgr, parts = kPageThreads >> lgp, part = tid >> lgp, d = (tid & ((1 << lgq) - 1)) * 4;
     const int live = min(U.splits, (paged_keys(P, U) + U.size * kPagedChunk - 1) / (U.size * kPagedChunk));
-    const int64_t step = (int64_t)P.kv_heads * P.tile;
+    const int64_t step = (int64_t)P.kv_heads * P.tile, first = ((int64_t)U.rec * P.kv_heads + hk) * P.tile + r - U.tile * P.tile;
     bool none = false;
-    for (int i = (tid >> lgq) & ((1 << lgr) - 1); i - ((tid >> lgq) & ((1 << lgr) - 1)) < n; i += 1 << lgr) {
-        const bool in = i < n && d < P.dim;
-        const int64_t rec = ((int64_t)U.rec * P.kv_heads + hk) * P.tile + r - U.tile * P.tile + i;
-        float top = -INFINITY, sum = 0.f;
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (in) {
-            constexpr int N = 4;
-            for (int u0 = part; u0 < live; u0 += N * parts) {
-                float2 ms[N];
-                float4 z[N];
+    for (int i0 = 0; i0 < n; i0 += M << lgr) {
+        const int i = i0 + ((tid >> lgq) & ((1 << lgr) - 1));
+        float top[M], sum[M];
+        float4 y[M];
 #pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    const int64_t at = rec + min(u0 + k * parts, live - 1) * step;
-                    if constexpr (RAW) {
-                        auto raw = [](const void* p) __attribute__((always_inline)) -> float2 {
-                            return __builtin_bit_cast(float2, __hip_atomic_load(static_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
-                                                                                __HIP_MEMORY_SCOPE_AGENT));
-                        };
-                        ms[k] = raw(P.ws_s + at);
-                        const float2 a = raw(P.ws_o + at * P.dim + d), b = raw(P.ws_o + at * P.dim + d + 2);
-                        z[k] = make_float4(a.x, a.y, b.x, b.y);
-                    } else {
-                        ms[k] = P.ws_s[at];
-                        z[k] = *reinterpret_cast<const float4*>(P.ws_o + at * P.dim + d);
+        for (int q = 0; q < M; ++q) {
+            top[q] = -INFINITY;
+            sum[q] = 0.f;
+            y[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        if (d < P.dim)
+            for (int u0 = part; u0 < live; u0 += N * parts) {
+                float2 ms[M][N];
+                float4 z[M][N];
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+#pragma unroll
+                    for (int q = 0; q < M; ++q) {
+                        const int64_t at = first + min(i + (q << lgr), n - 1) + min(u0 + k * parts, live - 1) * step;
+                        ms[q][k] = paged_pair<RAW>(P.ws_s + at);
+                        const float2 a = paged_pair<RAW>(P.ws_o + at * P.dim + d), b = paged_pair<RAW>(P.ws_o + at * P.dim + d + 2);
+                        z[q][k] = make_float4(a.x, a.y, b.x, b.y);
+                    }
+#pragma unroll
+                for (int q = 0; q < M; ++q) {
+                    float t = top[q];
+#pragma unroll
+                    for (int k = 0; k < N; ++k) t = u0 + k * parts < live ? fmaxf(t, ms[q][k].x) : t;
+                    const float f = top[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[q] - t);
+                    top[q] = t;
+                    sum[q] *= f;
+                    y[q] = make_float4(y[q].x * f, y[q].y * f, y[q].z * f, y[q].w * f);
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        if (u0 + k * parts >= live || ms[q][k].x == -INFINITY) continue;
+                        const float w = __builtin_amdgcn_exp2f(ms[q][k].x - t);
+                        sum[q] += ms[q][k].y * w;
+                        y[q] = make_float4(fmaf(z[q][k].x, w, y[q].x), fmaf(z[q][k].y, w, y[q].y), fmaf(z[q][k].z, w, y[q].z),
+                                           fmaf(z[q][k].w, w, y[q].w));
                     }
                 }
-                float t = top;
-#pragma unroll
-                for (int k = 0; k < N; ++k) t = u0 + k * parts < live ? fmaxf(t, ms[k].x) : t;
-                const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t);
-                top = t;
-                sum *= f;
-                y = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
-#pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    if (u0 + k * parts >= live || ms[k].x == -INFINITY) continue;
-                    const float w = __builtin_amdgcn_exp2f(ms[k].x - top);
-                    sum += ms[k].y * w;
-                    y = make_float4(fmaf(z[k].x, w, y.x), fmaf(z[k].y, w, y.y), fmaf(z[k].z, w, y.z), fmaf(z[k].w, w, y.w));
-                }
             }
-        }
-        none = none || sum != sum;
-        if (parts > 1) {
-            float* const mine = s_red[tid];
-            mine[0] = top;
-            mine[1] = sum;
-            mine[2] = y.x;
-            mine[3] = y.y;
-            mine[4] = y.z;
-            mine[5] = y.w;
-            __syncthreads();
-            if (part == 0) {
-                float t = top;
-                for (int k = 1; k < parts; ++k) t = fmaxf(t, s_red[(k << lgp) + tid][0]);
-                const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t);
-                top = t;
-                sum *= f0;
-                y = make_float4(y.x * f0, y.y * f0, y.z * f0, y.w * f0);
-                for (int k = 1; k < parts; ++k) {
-                    const float* z = s_red[(k << lgp) + tid];
-                    if (z[0] == -INFINITY) continue;
-                    const float w = __builtin_amdgcn_exp2f(z[0] - t);
-                    sum += z[1] * w;
-                    y = make_float4(fmaf(z[2], w, y.x), fmaf(z[3], w, y.y), fmaf(z[4], w, y.z), fmaf(z[5], w, y.w));
+#pragma unroll
+        for (int q = 0; q < M; ++q) {
+            none = none || sum[q] != sum[q];
+            if (i0 + (q << lgr) >= n) break;  // no row in any thread
+            if (parts > 1) {
+                float* const mine = s_red[tid];
+                mine[0] = top[q];
+                mine[1] = sum[q];
+                mine[2] = y[q].x;
+                mine[3] = y[q].y;
+                mine[4] = y[q].z;
+                mine[5] = y[q].w;
+                __syncthreads();
+                if (part == 0) {
+                    float t = top[q];
+                    for (int k = 1; k < parts; ++k) t = fmaxf(t, s_red[(k << lgp) + tid][0]);
+                    const float f0 = top[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[q] - t);
+                    top[q] = t;
+                    sum[q] *= f0;
+                    y[q] = make_float4(y[q].x * f0, y[q].y * f0, y[q].z * f0, y[q].w * f0);
+                    for (int k = 1; k < parts; ++k) {
+                        const float* z = s_red[(k << lgp) + tid];
+                        if (z[0] == -INFINITY) continue;
+                        const float w = __builtin_amdgcn_exp2f(z[0] - t);
+                        sum[q] += z[1] * w;
+                        y[q] = make_float4(fmaf(z[2], w, y[q].x), fmaf(z[3], w, y[q].y), fmaf(z[4], w, y[q].z), fmaf(z[5], w, y[q].w));
+                    }
                 }
+                __syncthreads();  // s_red is written again
             }
-            __syncthreads();  // s_red is written again
-        }
-        if (part == 0 && in) {
-            const PagedTo to = paged_to<T>(P, U, hk, r + i);
-            const float inv = 1.f / sum;
-            if (to.out) paged_store<T>(to, d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
-            if (d == 0 && to.lse) *to.lse = (top + log2f(sum)) * kLn2;
+            if (part == 0 && i + (q << lgr) < n && d < P.dim) {
+                const PagedTo to = paged_to<T>(P, U, hk, r + i + (q << lgr));
+                const float inv = 1.f / sum[q];
+                if (to.out) paged_store<T>(to, d, make_float4(y[q].x * inv, y[q].y * inv, y[q].z * inv, y[q].w * inv));
+                if (d == 0 && to.lse) *to.lse = (top[q] + log2f(sum[q])) * kLn2;
+            }
         }
     }
     return none;

@@ -87,7 +87,7 @@ __device__ __forceinline__ void paged_join(const PagedDev& P, float (*s_red)[6],
         if (!paged_find<kRows>(P, item / P.kv_heads, threadIdx.x & 63, U)) return;
         if (!paged_recorded(P, U)) continue;
         const int n = min(1 << P.lgr, U.rows - U.at);
-        if (__syncthreads_or(paged_join_rows<T, false>(P, U, hk, U.at, n, P.lgr, s_red)))
+        if (__syncthreads_or(paged_join_rows<T, false, 1>(P, U, hk, U.at, n, P.lgr, s_red)))
             for (int r = U.at; r < U.at + n; ++r) paged_slow<T>(P, U, hk, r, S);
     }
 }
@@ -132,7 +132,16 @@ DraftRow paged_view(const pa_view& v) {
     return r;
 }
 
-constexpr int64_t kPagedCus = 256, kPagedMany = 4, kPagedFew = 2, kPagedUnitBytes = 64 * 1024, kTilesMany = 2;
+constexpr int64_t kPagedCus = 256;
+// Units of k_paged_rows: each has its latencies (some 6 us alone), so they are of 64 KB of keys at least, and
+// no more than there is room for at once where that leaves them at most 256 KB; beyond, twice as many, which the uneven
+// ends of rows fill better.  Measured, us: 32 ragged rows of up to 8192 positions, 32/8 heads of 128, 227 so, 236 with
+// three times as many, 247 with up to 512 KB; one row of 65536 116, 129 with up to 128 KB only, 109 with 512; 6 ragged
+// chunks behind 5003, 12/4 heads of 128, 111, with 32 KB at least 124, 128 KB 117.
+constexpr int64_t kPagedMany = 2, kPagedLarge = 256 * 1024, kPagedSmall = 64 * 1024;
+// Units of k_paged_tiles: two chunks at least, and no more than there is room for at once (4 ragged chunks of 512 behind
+// 2048, 32/8 heads of 128: 164 us, with twice as many 220; 512 behind 32768: 436 and 491).
+constexpr int kTilesFewest = 2;
 // chunks of more query rows per key head than this go to k_paged_tiles, where it applies
 constexpr int kPagedFewRows = 32;
 
@@ -156,9 +165,11 @@ PagedPlan paged_plan(const pa_paged* p, bool last, bool many, bool both, PagedDe
     P.most = many || !both ? 1 << 30 : kPagedFewRows;
     P.tile = many ? paged_tile_rows(D) : 16 * plan.tiles;
     const int64_t flight = kPagedCus * (many ? (D == 128 ? 1 : 2) : paged_waves(D, plan.tiles));
-    P.target = (int)std::max<int64_t>(1, (many ? kTilesMany : kPagedMany) * flight / p->kv_heads);
-    P.target_min = (int)std::max<int64_t>(1, (many ? 1 : kPagedFew) * flight / p->kv_heads);
-    P.least = many ? 4 : std::max(1, (int)(kPagedUnitBytes * plan.tiles / ((int64_t)kPagedChunk * p->dim * (f32 ? 4 : 2))));
+    P.target = (int)std::max<int64_t>(1, (many ? 1 : kPagedMany) * flight / p->kv_heads);
+    const int64_t chunk = (int64_t)kPagedChunk * p->dim * (f32 ? 4 : 2);  // bytes of its keys
+    P.target_min = (int)std::max<int64_t>(1, flight / p->kv_heads);
+    P.least = many ? 0 : (int)(kPagedLarge / chunk);
+    P.fewest = many ? kTilesFewest : (int)std::max<int64_t>(1, kPagedSmall / chunk);
     // tiles of all rows: of chunks of at most P.most rows
     const int64_t each = (std::min<int64_t>(rows, P.most) + P.tile - 1) / P.tile;
     const int64_t tiles = p->packed ? std::min<int64_t>((rows + P.tile - 1) / P.tile + p->t.rows, each * p->t.rows)

@@ -488,10 +488,10 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
     }
     __syncthreads();
     if (!s_last) return;
+    // rows at once, as there are rows, and threads for four features each
     int lgr = 0;
-    while ((1 << lgr) < nrows && (P.dim << lgr) < 4 * kPageThreads) ++lgr;  // a quad of threads' features each
-    while (lgr > 0 && ((P.dim + 3) / 4 - 1) >> (8 - lgr)) --lgr;
-    paged_join_rows<T, true>(P, U, hk, r0, nrows, lgr, reinterpret_cast<float(*)[6]>(s_o));
+    while ((1 << lgr) < nrows && (((P.dim >> 2) - 1) >> (7 - lgr)) == 0) ++lgr;
+    paged_join_rows<T, true, RT * D >= 256 ? 4 : RT * D / 64>(P, U, hk, r0, nrows, lgr, reinterpret_cast<float(*)[6]>(s_o));
 }
 
 template <typename T, int D>
