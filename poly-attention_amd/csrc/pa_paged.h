@@ -93,7 +93,7 @@ __device__ __forceinline__ void paged_tiles(const PagedDev& P, const PageRow& r,
 // are to be joined.
 enum { kUnits, kRows };
 
-// Finds unit (or row) `want` over all rows of the batch, by the whole wave; false past the last one.  What it finds
+// Finds unit (or block of rows) `want` over all rows of the batch, by the whole wave; false past the last one.  What it finds
 // is held in scalar registers, so that the branches and loops over it are scalar ones.
 template <int WHAT>
 __device__ __forceinline__ bool paged_find(const PagedDev& P, int want, int lane, PagedUnit& U) {
@@ -252,28 +252,57 @@ __device__ __forceinline__ float paged_odd(uint32_t w, float acc) {
     }
 }
 
-// a maximum and sum, or two features, of a record; RAW: read at the GPU's level, past this XCD's caches
-template <bool RAW>
-__device__ __forceinline__ float2 paged_pair(const void* p) {
-    if constexpr (RAW)
-        return __builtin_bit_cast(float2, __hip_atomic_load(static_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    else
-        return *static_cast<const float2*>(p);
-}
+// Records that the same launch reads (GPU) are written and read at the GPU's level, past their XCD's cache.
+constexpr int kPagedGpu = 16;  // sc1
+// a tile's records, from its first unit's
+template <bool GPU>
+struct PagedRecords {
+    __amdgpu_buffer_rsrc_t o;
+    float2* s;
+    int step;  // rows from a unit's record to the next one's
+    int dim;
+    __device__ __forceinline__ PagedRecords(const PagedDev& P, const PagedUnit& U, int hk) {
+        const int64_t first = ((int64_t)U.rec * P.kv_heads + hk) * P.tile;
+        step = P.kv_heads * P.tile;
+        dim = P.dim;
+        s = P.ws_s + first;
+        o = draft_buffer(reinterpret_cast<const char*>(P.ws_o + first * P.dim), (int64_t)U.splits * step * P.dim * 4);
+    }
+    __device__ __forceinline__ float4 get(int row, int d) const {
+        return __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(o, (row * dim + d) * 4, 0, GPU ? kPagedGpu : 0));
+    }
+    __device__ __forceinline__ void put(int row, int d, float4 y) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_d, y), o, (row * dim + d) * 4, 0, GPU ? kPagedGpu : 0);
+    }
+    __device__ __forceinline__ float2 get_sum(int row) const {
+        if (!GPU) return s[row];
+        return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(s + row), __ATOMIC_RELAXED,
+                                                            __HIP_MEMORY_SCOPE_AGENT));
+    }
+    __device__ __forceinline__ void put_sum(int row, float top, float sum) const {
+        if (!GPU)
+            s[row] = make_float2(top, sum);
+        else
+            __hip_atomic_store(reinterpret_cast<uint64_t*>(s + row), __builtin_bit_cast(uint64_t, make_float2(top, sum)),
+                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+};
 
-// Joins the units of `n` query rows of a tile, r first, and finishes them, by the workgroup: M 2^lgr rows at a time, M of
-// them and four features a thread, the units dealt out over what is left of the threads, so that eight loads or so are
-// under way.  True where a unit's sum is no number (in every thread).
-template <typename T, bool RAW, int M>
-__device__ __forceinline__ bool paged_join_rows(const PagedDev& P, const PagedUnit& U, int hk, int r, int n, int lgr, float (*s_red)[6]) {
+// Joins `count` records, `first` and every `ustep`-th after it, of n query rows of a tile, r first, by the workgroup:
+// M 2^lgr rows at a time, M of them and four features a thread, the records dealt out over what is left of the
+// threads, so that eight loads or so are under way.  The rows are finished, or the first record takes what was
+// joined.  True where a record's sum is no number.
+template <typename T, int M, bool GPU>
+__device__ __forceinline__ bool paged_join(const PagedDev& P, const PagedUnit& U, int hk, int first, int ustep, int count, bool finish,
+                                           int r, int n, int lgr, float (*s_red)[6]) {
     constexpr int N = M >= 4 ? 2 : M == 2 ? 4 : 6;
+    const PagedRecords<GPU> R(P, U, hk);
     const int tid = threadIdx.x;
     const int quads = P.dim >> 2;
     int lgq = 0;
     while ((1 << lgq) < quads) ++lgq;  // at most 64
     const int lgp = lgq + lgr, parts = kPageThreads >> lgp, part = tid >> lgp, d = (tid & ((1 << lgq) - 1)) * 4;
-    const int live = min(U.splits, (paged_keys(P, U) + U.size * kPagedChunk - 1) / (U.size * kPagedChunk));
-    const int64_t step = (int64_t)P.kv_heads * P.tile, first = ((int64_t)U.rec * P.kv_heads + hk) * P.tile + r - U.tile * P.tile;
+    const int row0 = first * R.step + r - U.tile * P.tile;
     bool none = false;
     for (int i0 = 0; i0 < n; i0 += M << lgr) {
         const int i = i0 + ((tid >> lgq) & ((1 << lgr) - 1));
@@ -286,30 +315,29 @@ __device__ __forceinline__ bool paged_join_rows(const PagedDev& P, const PagedUn
             y[q] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
         if (d < P.dim)
-            for (int u0 = part; u0 < live; u0 += N * parts) {
+            for (int u0 = part; u0 < count; u0 += N * parts) {
                 float2 ms[M][N];
                 float4 z[M][N];
 #pragma unroll
                 for (int k = 0; k < N; ++k)
 #pragma unroll
                     for (int q = 0; q < M; ++q) {
-                        const int64_t at = first + min(i + (q << lgr), n - 1) + min(u0 + k * parts, live - 1) * step;
-                        ms[q][k] = paged_pair<RAW>(P.ws_s + at);
-                        const float2 a = paged_pair<RAW>(P.ws_o + at * P.dim + d), b = paged_pair<RAW>(P.ws_o + at * P.dim + d + 2);
-                        z[q][k] = make_float4(a.x, a.y, b.x, b.y);
+                        const int at = row0 + min(i + (q << lgr), n - 1) + min(u0 + k * parts, count - 1) * ustep * R.step;
+                        ms[q][k] = R.get_sum(at);
+                        z[q][k] = R.get(at, d);
                     }
 #pragma unroll
                 for (int q = 0; q < M; ++q) {
                     float t = top[q];
 #pragma unroll
-                    for (int k = 0; k < N; ++k) t = u0 + k * parts < live ? fmaxf(t, ms[q][k].x) : t;
+                    for (int k = 0; k < N; ++k) t = u0 + k * parts < count ? fmaxf(t, ms[q][k].x) : t;
                     const float f = top[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[q] - t);
                     top[q] = t;
                     sum[q] *= f;
                     y[q] = make_float4(y[q].x * f, y[q].y * f, y[q].z * f, y[q].w * f);
 #pragma unroll
                     for (int k = 0; k < N; ++k) {
-                        if (u0 + k * parts >= live || ms[q][k].x == -INFINITY) continue;
+                        if (u0 + k * parts >= count || ms[q][k].x == -INFINITY) continue;
                         const float w = __builtin_amdgcn_exp2f(ms[q][k].x - t);
                         sum[q] += ms[q][k].y * w;
                         y[q] = make_float4(fmaf(z[q][k].x, w, y[q].x), fmaf(z[q][k].y, w, y[q].y), fmaf(z[q][k].z, w, y[q].z),
@@ -317,51 +345,82 @@ __device__ __forceinline__ bool paged_join_rows(const PagedDev& P, const PagedUn
                     }
                 }
             }
-#pragma unroll
-        for (int q = 0; q < M; ++q) {
-            none = none || sum[q] != sum[q];
-            if (i0 + (q << lgr) >= n) break;  // no row in any thread
-            if (parts > 1) {
+        if (!finish) __syncthreads();  // the first record has been read
+        auto end = [&](float& top, float& sum, float4& y, int row) __attribute__((always_inline)) {
+            none = none || sum != sum;
+            if (row - i + i0 < n && parts > 1) {  // a row in some thread
                 float* const mine = s_red[tid];
-                mine[0] = top[q];
-                mine[1] = sum[q];
-                mine[2] = y[q].x;
-                mine[3] = y[q].y;
-                mine[4] = y[q].z;
-                mine[5] = y[q].w;
+                mine[0] = top;
+                mine[1] = sum;
+                mine[2] = y.x;
+                mine[3] = y.y;
+                mine[4] = y.z;
+                mine[5] = y.w;
                 __syncthreads();
                 if (part == 0) {
-                    float t = top[q];
+                    float t = top;
                     for (int k = 1; k < parts; ++k) t = fmaxf(t, s_red[(k << lgp) + tid][0]);
-                    const float f0 = top[q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top[q] - t);
-                    top[q] = t;
-                    sum[q] *= f0;
-                    y[q] = make_float4(y[q].x * f0, y[q].y * f0, y[q].z * f0, y[q].w * f0);
+                    const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - t);
+                    top = t;
+                    sum *= f0;
+                    y = make_float4(y.x * f0, y.y * f0, y.z * f0, y.w * f0);
                     for (int k = 1; k < parts; ++k) {
                         const float* z = s_red[(k << lgp) + tid];
                         if (z[0] == -INFINITY) continue;
                         const float w = __builtin_amdgcn_exp2f(z[0] - t);
-                        sum[q] += z[1] * w;
-                        y[q] = make_float4(fmaf(z[2], w, y[q].x), fmaf(z[3], w, y[q].y), fmaf(z[4], w, y[q].z), fmaf(z[5], w, y[q].w));
+                        sum += z[1] * w;
+                        y = make_float4(fmaf(z[2], w, y.x), fmaf(z[3], w, y.y), fmaf(z[4], w, y.z), fmaf(z[5], w, y.w));
                     }
                 }
                 __syncthreads();  // s_red is written again
             }
-            if (part == 0 && i + (q << lgr) < n && d < P.dim) {
-                const PagedTo to = paged_to<T>(P, U, hk, r + i + (q << lgr));
-                const float inv = 1.f / sum[q];
-                if (to.out) paged_store<T>(to, d, make_float4(y[q].x * inv, y[q].y * inv, y[q].z * inv, y[q].w * inv));
-                if (d == 0 && to.lse) *to.lse = (top[q] + log2f(sum[q])) * kLn2;
+            if (part != 0 || row >= n || d >= P.dim) return;
+            if (finish) {
+                const PagedTo to = paged_to<T>(P, U, hk, r + row);
+                const float inv = 1.f / sum;
+                if (to.out) paged_store<T>(to, d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+                if (d == 0 && to.lse) *to.lse = (top + log2f(sum)) * kLn2;
+            } else {
+                R.put(row0 + row, d, y);
+                if (d == 0) R.put_sum(row0 + row, top, sum);
             }
+        };
+        end(top[0], sum[0], y[0], i);
+        if constexpr (M > 1) end(top[1], sum[1], y[1], i + (1 << lgr));
+        if constexpr (M > 2) {
+            end(top[2], sum[2], y[2], i + (2 << lgr));
+            end(top[3], sum[3], y[3], i + (3 << lgr));
         }
     }
     return none;
 }
 
-// A record's maximum and sum, and four of its features, at the GPU's level: read by whichever workgroup ends last.
-__device__ __forceinline__ void paged_raw(void* p, float a, float b) {
-    __hip_atomic_store(static_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, make_float2(a, b)), __ATOMIC_RELAXED,
-                       __HIP_MEMORY_SCOPE_AGENT);
+// The end of a unit of the tile's n query rows, r first, its records written: the last one of its tile joins them, as a
+// ticket says.  More than eight units join in two steps, groups first, as one workgroup reads but 25 to 100 GB/s
+// (one row of 65536 positions 116 us in one step, 109 in two).
+template <typename T, int M>
+__device__ __forceinline__ void paged_end(const PagedDev& P, const PagedUnit& U, int hk, int r, int n, float (*s_red)[6], int& s_last) {
+    const int live = min(U.splits, (paged_keys(P, U) + U.size * kPagedChunk - 1) / (U.size * kPagedChunk));
+    const int size = live <= 8 ? live : live <= 64 ? 8 : 16;
+    const int first = U.split - U.split % size, groups = (live + size - 1) / size, in = min(size, live - first);
+    int lgr = 0;  // rows at once, as there are rows, and threads for four features each
+    while ((1 << lgr) < n && (((P.dim >> 2) - 1) >> (7 - lgr)) == 0) ++lgr;
+    for (bool whole = groups == 1;; whole = true) {
+        int32_t* const ticket = P.tickets + ((int64_t)(U.rec + (whole ? 0 : first)) * P.kv_heads + hk) * kTicketStride + (whole ? 0 : 1);
+        const int all = groups == 1 ? live : whole ? groups : in;
+        // the records are there once the waves' stores have returned; a release would write the cache back, at several us
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            const int drawn = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            s_last = drawn == all - 1;
+            if (drawn == all - 1) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!__builtin_amdgcn_readfirstlane(s_last)) return;
+        paged_join<T, M, true>(P, U, hk, whole ? 0 : first, whole && groups > 1 ? size : 1, all, whole, r, n, lgr, s_red);
+        if (whole) return;
+    }
 }
 
 // Where values that are not finite lie behind some row's own position, the products of k_paged_tiles are no numbers: a

@@ -80,14 +80,15 @@ __device__ __forceinline__ void paged_slow(const PagedDev& P, const PagedUnit& U
 
 // Blocks of rows of tiles that were split, a workgroup each.
 template <typename T>
-__device__ __forceinline__ void paged_join(const PagedDev& P, float (*s_red)[6], SlowRow& S) {
+__device__ __forceinline__ void paged_join_tiles(const PagedDev& P, float (*s_red)[6], SlowRow& S) {
     for (int64_t item = blockIdx.x;; item += gridDim.x) {
         const int hk = (int)(item % P.kv_heads);
         PagedUnit U;
         if (!paged_find<kRows>(P, item / P.kv_heads, threadIdx.x & 63, U)) return;
         if (!paged_recorded(P, U)) continue;
         const int n = min(1 << P.lgr, U.rows - U.at);
-        if (__syncthreads_or(paged_join_rows<T, false, 1>(P, U, hk, U.at, n, P.lgr, s_red)))
+        const int live = min(U.splits, (paged_keys(P, U) + U.size * kPagedChunk - 1) / (U.size * kPagedChunk));
+        if (__syncthreads_or(paged_join<T, 1, false>(P, U, hk, 0, 1, live, true, U.at, n, P.lgr, s_red)))
             for (int r = U.at; r < U.at + n; ++r) paged_slow<T>(P, U, hk, r, S);
     }
 }
@@ -108,7 +109,7 @@ template <typename T>
 __global__ __launch_bounds__(kPageThreads) void k_paged_join(const PagedDev P) {
     __shared__ float s_red[kPageThreads][6];
     __shared__ SlowRow s_slow;
-    if (P.recs > 0) paged_join<T>(P, s_red, s_slow);
+    if (P.recs > 0) paged_join_tiles<T>(P, s_red, s_slow);
     paged_again<T>(P, s_slow);
 }
 

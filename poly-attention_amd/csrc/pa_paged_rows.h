@@ -401,7 +401,7 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
         f[rt] = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - top);
     }
     const bool done = U.splits == 1;
-    const int64_t rec = ((int64_t)(U.rec + U.split) * P.kv_heads + hk) * P.tile;
+    const PagedRecords<true> R(P, U, hk);
     auto row_sum = [&](int r, float& top) __attribute__((always_inline)) -> float {
         top = s_m[0][r];
         for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][r]);
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
         float top;
         const float sum = row_sum(tid, top);
         if (!done) {
-            paged_raw(P.ws_s + rec + tid, top, sum);
+            R.put_sum(U.split * R.step + tid, top, sum);
         } else if (!P.last) {
             const PagedTo to = paged_to<T>(P, U, hk, r0 + tid);
             if (to.lse) *to.lse = (top + log2f(sum)) * kLn2;
@@ -466,32 +466,13 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
                     y.w += z.w;
                 }
                 if (!done) {
-                    float* const at = P.ws_o + (rec + 16 * rt + r) * P.dim + d;
-                    paged_raw(at, y.x, y.y);
-                    paged_raw(at + 2, y.z, y.w);
+                    R.put(U.split * R.step + 16 * rt + r, d, y);
                 } else if (to.out) paged_store<T>(to, d, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
             }
         }
         if (rt + 1 < RT) __syncthreads();
     }
-    if (done) return;
-    // The unit that ends last joins its tile's.  The records were written at the GPU's level, past this XCD's cache, and
-    // are there once the waves' stores have returned; a release would write the cache back, at several us.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    int32_t* const ticket = P.tickets + ((int64_t)U.rec * P.kv_heads + hk) * kTicketStride;
-    const int live = min(U.splits, (paged_keys(P, U) + U.size * kPagedChunk - 1) / (U.size * kPagedChunk));
-    if (tid == 0) {
-        const int drawn = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = drawn == live - 1;
-        if (drawn == live - 1) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (!s_last) return;
-    // rows at once, as there are rows, and threads for four features each
-    int lgr = 0;
-    while ((1 << lgr) < nrows && (((P.dim >> 2) - 1) >> (7 - lgr)) == 0) ++lgr;
-    paged_join_rows<T, true, RT * D >= 256 ? 4 : RT * D / 64>(P, U, hk, r0, nrows, lgr, reinterpret_cast<float(*)[6]>(s_o));
+    if (!done) paged_end<T, RT * D >= 256 ? 4 : RT * D / 64>(P, U, hk, r0, nrows, reinterpret_cast<float(*)[6]>(s_o), s_last);
 }
 
 template <typename T, int D>

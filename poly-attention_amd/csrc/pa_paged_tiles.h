@@ -368,23 +368,22 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
     if (U.splits > 1 && !paged_recorded(P, U)) return;
     const bool any = __any(odd != 0.f);
     if (U.splits == 1 && lane < 8 / NW) *paged_flag(P, w + NW * lane) = any;  // eight of them, whatever the waves
-    const int64_t rec = ((int64_t)(U.rec + U.split) * P.kv_heads + hk) * P.tile;
+    const PagedRecords<false> R(P, U, hk);
 #pragma unroll
     for (int u = 0; u < QB; ++u) {
         const int r = r0 + 32 * u + col;
         const float sum = xhalf_sum(l[u]);
         if (r >= rend) continue;
         if (U.splits > 1) {
-            const int64_t at = rec + r - U.tile * P.tile;
-            if (hh == 0) P.ws_s[at] = make_float2(m[u], any ? NAN : sum);
+            const int at = U.split * R.step + r - U.tile * P.tile;
+            if (hh == 0) R.put_sum(at, m[u], any ? NAN : sum);
 #pragma unroll
             for (int x = 0; x < D / 32; ++x)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const int d = x * 32 + 8 * g + 4 * hh;
                     if (d < P.dim)
-                        *reinterpret_cast<float4*>(P.ws_o + at * P.dim + d) =
-                            make_float4(o[u][x][4 * g], o[u][x][4 * g + 1], o[u][x][4 * g + 2], o[u][x][4 * g + 3]);
+                        R.put(at, d, make_float4(o[u][x][4 * g], o[u][x][4 * g + 1], o[u][x][4 * g + 2], o[u][x][4 * g + 3]));
                 }
             continue;
         }
