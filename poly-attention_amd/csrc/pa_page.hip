@@ -14,6 +14,7 @@ namespace pa {
 
 constexpr int kPlanThreads = 1024;  // of the kernels of one workgroup
 constexpr int kPlanWaves = kPlanThreads / 64;
+constexpr int kCopyParts = 64;  // of a page's copy, at most
 
 struct PagePlan {  // a table, and a call's arguments
     int32_t rows, pages, lg, max_pages;
@@ -31,8 +32,6 @@ struct PagePlan {  // a table, and a call's arguments
     int4* moves;     // [max(rows, pages / 2 + 1)]: from, to, positions
     int32_t* list;   // [pages]: the free pages that are handed out, or where a page went
     int32_t* need;   // [rows]
-    int32_t* upto;   // [rows]
-    int32_t* after;  // [rows]
     int32_t* copy;   // [rows, max_pages]
     const pa_page_array* arrays;
     int32_t count;
@@ -71,6 +70,20 @@ __device__ __forceinline__ Sums block_sums(int a, int b, int64_t (*part)[2], int
     return s;
 }
 
+// 16 references from place `first`, a multiple of 16; `none` past the last page
+__device__ __forceinline__ void plan_refs(const PagePlan& P, int64_t first, int none, int (&r)[16]) {
+    if (first + 16 <= P.pages && (uintptr_t)P.refs % 16 == 0) {
+#pragma unroll
+        for (int k = 0; k < 16; k += 4) {
+            const int4 x = *reinterpret_cast<const int4*>(P.refs + first + k);
+            r[k] = x.x, r[k + 1] = x.y, r[k + 2] = x.z, r[k + 3] = x.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) r[k] = first + k < P.pages ? P.refs[first + k] : none;
+    }
+}
+
 __device__ __forceinline__ int plan_count(const PagePlan& P, int b) {
     return min(max(P.counts[b], 0), P.max_pages << P.lg);
 }
@@ -89,8 +102,11 @@ __device__ __forceinline__ void plan_asked(const PagePlan& P, int b, int& n, int
 __global__ __launch_bounds__(kPlanThreads) void k_page_extend(const PagePlan P) {
     __shared__ int64_t s_part[kPlanWaves][2];
     __shared__ int s_tail[PA_MAX_PAGE_ROWS];  // the partly filled page that a row is about to write, or -1
+    __shared__ int s_need[PA_MAX_PAGE_ROWS], s_upto[PA_MAX_PAGE_ROWS], s_after[PA_MAX_PAGE_ROWS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int size = 1 << P.lg;
+    int r[16];
+    plan_refs(P, (int64_t)tid * 16, 1, r);  // nothing below writes them before they have been looked at
     for (int b = tid; b < P.rows; b += kPlanThreads) {
         int n, m;
         bool past;
@@ -134,9 +150,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_extend(const PagePlan P) 
         const int asked = b < P.rows ? max(P.more[b], 0) : 0;
         const Sums s = block_sums(want, asked, s_part, tid);
         if (b < P.rows) {
-            P.need[b] = want << 3 | flags;
-            P.after[b] = after;
-            P.upto[b] = clip(needed + s.a + want);
+            s_need[b] = want << 3 | flags;
+            s_after[b] = after;
+            s_upto[b] = clip(needed + s.a + want);
             P.starts[b] = clip(tokens + s.b);
         }
         needed += s.all_a;
@@ -148,19 +164,17 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_extend(const PagePlan P) 
     }
     // the first `needed` free pages
     int64_t found = 0;
-    constexpr int U = 4;
-    for (int64_t p0 = 0; p0 < P.pages && found < needed; p0 += kPlanThreads * 4 * U) {
-        const int64_t first = p0 + (int64_t)tid * 4 * U;
-        int r[4 * U];
-#pragma unroll
-        for (int k = 0; k < 4 * U; ++k) r[k] = first + k < P.pages ? P.refs[first + k] : 1;
+    constexpr int U = 16;
+    for (int64_t p0 = 0; p0 < P.pages && found < needed; p0 += kPlanThreads * U) {
+        const int64_t first = p0 + (int64_t)tid * U;
+        if (p0 > 0) plan_refs(P, first, 1, r);
         int mine = 0;
 #pragma unroll
-        for (int k = 0; k < 4 * U; ++k) mine += r[k] == 0;
+        for (int k = 0; k < U; ++k) mine += r[k] == 0;
         const Sums s = block_sums(mine, 0, s_part, tid);
         int64_t at = found + s.a;
 #pragma unroll
-        for (int k = 0; k < 4 * U; ++k)
+        for (int k = 0; k < U; ++k)
             if (r[k] == 0) {
                 if (at < needed) P.list[at] = (int)(first + k);
                 ++at;
@@ -173,11 +187,11 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_extend(const PagePlan P) 
         int n, m;
         bool past;
         plan_asked(P, b, n, m, past);
-        const int need = P.need[b], want = need >> 3;
-        const int first = P.upto[b] - want;
+        const int need = s_need[b], want = need >> 3;
+        const int first = s_upto[b] - want;
         // a row that keeps a page needs the last of those that copied it to have got theirs, and so the others
-        const int after = P.after[b];
-        const bool ok = m > 0 && (want > 0 ? P.upto[b] <= found : after < 0 || P.upto[after] <= found);
+        const int after = s_after[b];
+        const bool ok = m > 0 && (want > 0 ? s_upto[b] <= found : after < 0 || s_upto[after] <= found);
         const bool copies = need & 1;
         if (ok) {
             const int at = copies ? n >> P.lg : (n + size - 1) >> P.lg;
@@ -204,29 +218,23 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_extend(const PagePlan P) 
     }
 }
 
-// Rows as the beginnings of other rows, in two launches: what the rows become, beside the references; then
-// into the table.  One workgroup per row.
-__device__ __forceinline__ void select_row(const PagePlan& P, int b, int& old_pages, int& new_count, int& src) {
-    src = P.index[b];
-    const int size = 1 << P.lg, n = plan_count(P, b);
-    old_pages = (n + size - 1) >> P.lg;
+// Rows as the beginnings of other rows: what the rows become, beside the references; then, when all rows have been
+// read, into the table.  A workgroup per row in two launches, or one for a small table, which saves the second
+// launch's 4 us or so.
+__device__ __forceinline__ void select_new(const PagePlan& P, int b, int tid, int threads) {
+    const int size = 1 << P.lg, old_pages = (plan_count(P, b) + size - 1) >> P.lg;
+    int src = P.index[b], n = 0;
     if (src < 0 || src >= P.rows) {
         src = -1;
-        new_count = 0;
-        return;
+    } else {
+        n = plan_count(P, src);
+        if (P.lengths) n = min(n, max(P.lengths[b], 0));
     }
-    new_count = plan_count(P, src);
-    if (P.lengths) new_count = min(new_count, max(P.lengths[b], 0));
-}
-__global__ __launch_bounds__(kPageThreads) void k_page_select(const PagePlan P) {
-    const int b = blockIdx.x, size = 1 << P.lg;
-    int old_pages, n, src;
-    select_row(P, b, old_pages, n, src);
     const int used = (n + size - 1) >> P.lg, most = max(used, old_pages);
     const int32_t* from = P.table + (int64_t)max(src, 0) * P.max_pages;
     const int32_t* own = P.table + (int64_t)b * P.max_pages;
     int32_t* to = P.copy + (int64_t)b * P.max_pages;
-    for (int k = threadIdx.x; k < most; k += kPageThreads) {
+    for (int k = tid; k < most; k += threads) {
         const int was = k < old_pages ? own[k] : -1, is = k < used ? from[k] : -1;
         to[k] = is;
         if (was != is) {
@@ -234,19 +242,40 @@ __global__ __launch_bounds__(kPageThreads) void k_page_select(const PagePlan P) 
             if (plan_page(P, is)) atomicAdd(P.refs + is, 1);
         }
     }
-    if (threadIdx.x == 0) P.need[b] = n;
+    if (tid == 0) P.need[b] = n;
 }
-__global__ __launch_bounds__(kPageThreads) void k_page_selected(const PagePlan P) {
-    const int b = blockIdx.x, size = 1 << P.lg;
+// the count, which the callers write when all threads of the row have read it
+__device__ __forceinline__ int select_row(const PagePlan& P, int b, int tid, int threads) {
+    const int size = 1 << P.lg;
     const int n = P.need[b], old = plan_count(P, b);
     const int most = max((n + size - 1) >> P.lg, (old + size - 1) >> P.lg);
     int32_t* row = P.table + (int64_t)b * P.max_pages;
     const int32_t* from = P.copy + (int64_t)b * P.max_pages;
-    for (int k = threadIdx.x; k < most; k += kPageThreads) row[k] = from[k];
-    __syncthreads();  // the row's count has been read by every wave: it bounds the loop above
+    for (int k = tid; k < most; k += threads) row[k] = from[k];
+    return n;
+}
+__global__ __launch_bounds__(kPageThreads) void k_page_select(const PagePlan P) {
+    select_new(P, blockIdx.x, threadIdx.x, kPageThreads);
+}
+__global__ __launch_bounds__(kPageThreads) void k_page_selected(const PagePlan P) {
+    const int b = blockIdx.x, n = select_row(P, b, threadIdx.x, kPageThreads);
+    __syncthreads();
     if (threadIdx.x == 0) {
         P.counts[b] = n;
         P.fresh[b] = 0;
+    }
+}
+__global__ __launch_bounds__(kPlanThreads) void k_page_select_all(const PagePlan P) {  // a wave per row
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int b = wave; b < P.rows; b += kPlanWaves) select_new(P, b, lane, 64);
+    __syncthreads();
+    for (int b = wave; b < P.rows; b += kPlanWaves) {
+        const int n = select_row(P, b, lane, 64);
+        __builtin_amdgcn_wave_barrier();
+        if (lane == 0) {
+            P.counts[b] = n;
+            P.fresh[b] = 0;
+        }
     }
 }
 
@@ -258,20 +287,17 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_plan(const PagePlan P) {
     constexpr int U = 16;
     int used = 0;
     for (int64_t p0 = 0; p0 < P.pages; p0 += kPlanThreads * U) {
-        int mine = 0;
+        int mine = 0, r[U];
+        plan_refs(P, p0 + (int64_t)tid * U, 0, r);
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-            const int64_t p = p0 + (int64_t)k * kPlanThreads + tid;
-            mine += p < P.pages && P.refs[p] > 0;
-        }
+        for (int k = 0; k < U; ++k) mine += r[k] > 0;
         used += (int)block_sums(mine, 0, s_part, tid).all_a;
     }
     int holes = 0, movers = 0;
     for (int64_t p0 = 0; p0 < P.pages; p0 += kPlanThreads * U) {
         const int64_t first = p0 + (int64_t)tid * U;
         int free = 0, moving = 0, r[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k) r[k] = first + k < P.pages ? P.refs[first + k] : 0;
+        plan_refs(P, first, 0, r);
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             const bool in = first + k < used;
@@ -303,12 +329,13 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_plan(const PagePlan P) {
     }
 }
 
-// The moves of pages, in every array, a wave for each move, array and head; and with `remap` the table's
-// entries that follow them.  Bound by memory: 16 bytes a lane, eight loads in flight.
+// The moves of pages, in every array, and with `remap` the table's entries that follow them.  Bound by memory: 16 bytes a
+// lane, eight loads in flight.  A wave takes a part of a page at a time: as many parts as give each wave four or so,
+// at least 8 KB of the largest pages.
 __global__ __launch_bounds__(kPageThreads) void k_page_copy(const PagePlan P, int remap) {
     const int lane = threadIdx.x & 63;
     const int64_t waves = (int64_t)gridDim.x * (kPageThreads / 64);
-    const int64_t wave = (int64_t)blockIdx.x * (kPageThreads / 64) + (threadIdx.x >> 6);
+    const int64_t wave = (int64_t)blockIdx.x * (kPageThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int moves = P.head[0];
     if (remap && moves > 0) {
         const int used = P.head[1];
@@ -321,51 +348,57 @@ __global__ __launch_bounds__(kPageThreads) void k_page_copy(const PagePlan P, in
             }
         }
     }
-    const int64_t items = (int64_t)moves * P.count;
-    for (int64_t it = wave; it < items; it += waves) {
+    const int64_t pages = (int64_t)moves * P.count;
+    if (pages == 0) return;
+    const int parts = (int)min(max(4 * waves / pages, (int64_t)1), (int64_t)kCopyParts);
+    for (int64_t it = wave; it < pages * parts; it += waves) {
         // neighbours in time copy one page's arrays
-        const int mv = (int)(it / P.count), a = (int)(it - (int64_t)mv * P.count);
+        const int64_t x = it / parts;
+        const int part = (int)(it - x * parts), mv = (int)(x / P.count), a = (int)(x - (int64_t)mv * P.count);
         const int4 m = P.moves[mv];
         const pa_page_array A = P.arrays[a];
         const int64_t head = (int64_t)A.row_bytes << P.lg, page = head * A.heads;
         const char* src = static_cast<const char*>(A.base) + m.x * page;
         char* dst = static_cast<char*>(A.base) + m.y * page;
         const int bytes = m.z * A.row_bytes;  // of a head
-        if (A.row_bytes % 16 == 0) {
-            constexpr int U = 8;
-            const int per = bytes >> 4, all = per * A.heads;
+        constexpr int U = 8;
+        auto move = [&](auto word) __attribute__((always_inline)) {
+            typedef decltype(word) W;
+            const int per = bytes / (int)sizeof(W), all = per * A.heads;
+            const int each = (all + parts * 64 - 1) / (parts * 64) * 64, end = min((part + 1) * each, all);
             const int64_t skip = head - bytes;  // between heads
-            for (int x0 = 0; x0 < all; x0 += 64 * U) {
-                u32x4_d v[U];
+            for (int x0 = part * each; x0 < end; x0 += 64 * U) {
+                W v[U];
                 int64_t at[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const int x = min(x0 + 64 * u + lane, all - 1);
-                    at[u] = 16ll * x + (skip ? skip * (x / per) : 0);
-                    v[u] = load16u(src + at[u]);
+                    const int k = min(x0 + 64 * u + lane, end - 1);
+                    at[u] = (int64_t)sizeof(W) * k + (skip ? skip * (k / per) : 0);
+                    v[u] = *reinterpret_cast<const W*>(src + at[u]);
                 }
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    if (x0 + 64 * u + lane < all) *reinterpret_cast<u32x4_d*>(dst + at[u]) = v[u];
+                    if (x0 + 64 * u + lane < end) *reinterpret_cast<W*>(dst + at[u]) = v[u];
             }
-        } else {
-            for (int h = 0; h < A.heads; ++h)
-                for (int x = lane; x < m.z; x += 64)
-                    reinterpret_cast<uint32_t*>(dst + h * head)[x] = reinterpret_cast<const uint32_t*>(src + h * head)[x];
-        }
+        };
+        if (bytes % 16 == 0) move(u32x4_d{});  // a head of a page has 16 rows or more
+        else move(uint32_t{});
     }
 }
 
 // ---------------------------------------------------------------------------------------
-// Norms and rotary of the chunks' tokens, into their pages.  A workgroup per token (and, where there are
-// few, per tensor), a lane holding 16 bytes of a row: its features are the same in all rows, so the sines
-// and cosines are computed once per lane and token.
+// Norms and rotary of the chunks' tokens, into their pages.  A wave per token and four groups of 64 / lpr rows of one
+// tensor, a lane holding 16 bytes of a row: the tensor, its weights and the lane's features are the same for all of
+// them.  The token's sines and cosines are dealt out over the wave's lanes.  Bound by memory, behind it by
+// instructions: 4096 tokens of 56 heads of 128 (117 MB) 24 us; 57 with a workgroup per token whose waves look the
+// tensors up, 58 with a workgroup for several tokens, which has too few waves.
 
 struct PageItemDev {
     DraftRow src, out;
     const void* w;
     char* pages;
     int32_t wdt, rotate, heads;
+    int32_t wide;  // the weights are of 32 bits or of the rows' type, and can be read 16 bytes at a time
 };
 struct PageRowsDev {
     PageDev p;
@@ -374,129 +407,187 @@ struct PageRowsDev {
     int64_t angles_sb, angles_sn;
     const void* angles;
     const float* inv_freq;
+    int32_t all;                      // tokens
+    int32_t first[PA_MAX_ORDER + 2];  // an item's first four groups of rows; of those past the last INT32_MAX
     PageItemDev it[PA_MAX_ORDER + 2];
 };
 
+// 16 bytes of a row as E numbers, and E numbers of another type
+template <typename T, int E>
+__device__ __forceinline__ void page_numbers(u32x4_d raw, float (&x)[E]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(raw[e]);
+    } else {
+        typedef T t2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t word = raw[e];  // a value: a bit cast of the element reads element 0
+            const t2 z = __builtin_bit_cast(t2, word);
+            x[2 * e] = (float)z[0];
+            x[2 * e + 1] = (float)z[1];
+        }
+    }
+}
+
+// the sum over a group of `n` neighbouring lanes, a power of two
+__device__ __forceinline__ float page_sum(float x, int n) {
+    auto dpp = [](float x, auto ctrl) __attribute__((always_inline)) -> float {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    if (n > 1) x += dpp(x, std::integral_constant<int, 0xb1>());   // neighbours
+    if (n > 2) x += dpp(x, std::integral_constant<int, 0x4e>());   // pairs
+    if (n > 4) x += dpp(x, std::integral_constant<int, 0x141>());  // the halves of a row of 16, mirrored
+    if (n > 8) x += dpp(x, std::integral_constant<int, 0x140>());  // the row, mirrored
+    if (n > 16) x += __shfl_xor(x, 16);
+    if (n > 32) x += __shfl_xor(x, 32);
+    return x;
+}
+
+// sin and cos: of an angle that is reduced by Cody and Waite's two parts of 2 pi, by the instructions, which
+// are within 2^-20 or so: far less than a 16-bit type's rounding
+template <typename T>
+__device__ __forceinline__ void page_sincos(float a, float& sn, float& cs) {
+    if constexpr (sizeof(T) == 4) {
+        sincosf(a, &sn, &cs);
+    } else {
+        const float q = rintf(a * 0.15915494309189535f);
+        const float r = fmaf(-q, -1.7484555e-7f, fmaf(-q, 6.2831855f, a)) * 0.15915494309189535f;
+        sn = __builtin_amdgcn_sinf(r);
+        cs = __builtin_amdgcn_cosf(r);
+    }
+}
+
+constexpr int kAppendGroups = 4;
+
 template <typename T>
 __global__ __launch_bounds__(kPageThreads) void k_page_append(const PageRowsDev P) {
-    constexpr int E = 16 / sizeof(T), U = 2;
-    const int tid = threadIdx.x, lane = tid & 63;
-    int b = 0, i;
+    constexpr int E = 16 / sizeof(T), U = kAppendGroups;
+    __shared__ __align__(16) float s_cos[kPageThreads / 64][256], s_sin[kPageThreads / 64][256];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int k = 0, from = 0;
+#pragma unroll
+    for (int j = 1; j < PA_MAX_ORDER + 2; ++j)
+        if ((int)blockIdx.y >= P.first[j]) {
+            k = j;
+            from = P.first[j];
+        }
+    const PageItemDev& I = P.it[k];
+    const int group = 64 / P.lpr, h0 = ((int)blockIdx.y - from) * U * group + lane / P.lpr;
+    const int x = blockIdx.x * (kPageThreads / 64) + wave;
+    if (x >= P.all) return;
+    int b, tok;
     if (P.p.packed) {
-        i = blockIdx.x;
-        b = page_find(P.p, i, lane);
+        tok = x;
+        b = page_find(P.p, x, lane);
     } else {
-        b = blockIdx.x / P.p.tokens;
-        i = blockIdx.x - b * P.p.tokens;
+        b = x / P.p.tokens;
+        tok = x - b * P.p.tokens;
     }
     const PageRow row = page_row(P.p, b);
-    const int tok = i;  // place in the inputs
-    i -= row.start;
+    const int i = tok - row.start, pos = row.p0 + i, src_b = P.p.packed ? 0 : b;
     const bool here = i >= 0 && i < row.len;
-    const int64_t place = here ? page_place(P.p, b, row.p0 + i) : -1;
-    const int src_b = P.p.packed ? 0 : b;
-    const int sub = tid & (P.lpr - 1), d0 = sub * E;
+    if (!here && I.pages) return;
+    const int d0 = (lane & (P.lpr - 1)) * E;
     const bool in = d0 < P.dim;
-    const int per = kPageThreads / P.lpr, first = tid / P.lpr;
-    float cs[E], sn[E];
+    u32x4_d raw[U];
+    const T* const src = I.src.at<T>(src_b, 0) + (int64_t)tok * I.src.sn + d0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        cs[e] = 1.f;
-        sn[e] = 0.f;
+    for (int u = 0; u < U; ++u) {
+        raw[u] = u32x4_d{0u, 0u, 0u, 0u};
+        if (here && in && h0 + u * group < I.heads) raw[u] = load16u(src + (h0 + u * group) * I.src.sh);
     }
-    if (P.rot_dim > 0 && here) {
-        float a[E];
-        if (P.angles) {
-            const int64_t at = src_b * P.angles_sb + tok * P.angles_sn;
+    float w[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                a[e] = d0 + e < P.rot_dim ? load_any(P.angles, P.adt, at + d0 + e) : 0.f;
-        } else {  // the position as the rotary module builds it, rounded to the rows' type
-            const float pos = round_to<T>(round_to<T>((float)(row.p0 + i)) / P.interp);
+    for (int e = 0; e < E; ++e) w[e] = 0.f;
+    if (I.w && in) {
+        const char* const at = static_cast<const char*>(I.w) + d0 * (I.wdt == PA_F32 ? 4 : 2);
+        if (!I.wide) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) a[e] = d0 + e < P.rot_dim ? pos * P.inv_freq[(d0 + e) >> 1] : 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-            sincosf(a[e], &sn[e], &cs[e]);
-            sn[e + 1] = sn[e];
-            cs[e + 1] = cs[e];
-            // a pair's features usually turn by one angle
-            if (a[e + 1] != a[e]) sincosf(a[e + 1], &sn[e + 1], &cs[e + 1]);
-        }
-    }
-    const int64_t head = (int64_t)P.dim << P.p.lg;  // elements between a page's heads
-    const int64_t inside = place & ((1 << P.p.lg) - 1), id = place >> P.p.lg;
-    for (int k = blockIdx.y; k < P.count; k += gridDim.y) {
-        const PageItemDev& I = P.it[k];
-        const T* src = I.src.at<T>(src_b, 0) + (int64_t)tok * I.src.sn + d0;
-        T* out;
-        int64_t sh;
-        if (I.pages) {
-            if (place < 0) continue;
-            out = reinterpret_cast<T*>(I.pages) + id * I.heads * head + inside * P.dim + d0;
-            sh = head;
+            for (int e = 0; e < E; ++e) w[e] = load_any(I.w, I.wdt, d0 + e);
+        } else if (sizeof(T) == 4 || I.wdt != PA_F32) {
+            page_numbers<T>(load16u(at), w);
         } else {
-            out = I.out.at<T>(src_b, 0) + (int64_t)tok * I.out.sn + d0;
-            sh = I.out.sh;
+            const u32x4_d a = load16u(at), b = load16u(at + 16);
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[e] = __uint_as_float(e < 4 ? a[e & 3] : b[e & 3]);
         }
-        float w[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) w[e] = I.w && in ? load_any(I.w, I.wdt, d0 + e) : 0.f;
-        const bool turn = I.rotate && P.rot_dim > 0;
-        for (int h0 = first; h0 - first < I.heads; h0 += U * per) {
-            u32x4_d raw[U], y[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                raw[u] = u32x4_d{0u, 0u, 0u, 0u};
-                if (here && in && h0 + u * per < I.heads) raw[u] = load16u(src + (h0 + u * per) * I.src.sh);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float x[E];
-                if constexpr (E == 4) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(raw[u][e]);
+    }
+    const int64_t place = here ? page_place(P.p, b, pos) : -1;
+    if (I.pages && place < 0) return;
+    const bool turn = I.rotate && P.rot_dim > 0 && here;
+    float cs[E], sn[E];
+    if (turn) {
+        float *const c = s_cos[wave], *const s = s_sin[wave];
+        // the position as the rotary module builds it, rounded to the rows' type
+        const float at = round_to<T>(round_to<T>((float)pos) / P.interp);
+        for (int p = lane; 2 * p < P.dim; p += 64) {  // a pair of features
+            float a = 0.f, a1 = 0.f, s0, c0;
+            if (2 * p < P.rot_dim) {
+                if (P.angles) {
+                    const int64_t from = src_b * P.angles_sb + tok * P.angles_sn + 2 * p;
+                    a = load_any(P.angles, P.adt, from);
+                    a1 = load_any(P.angles, P.adt, from + 1);
                 } else {
-                    typedef T t2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t word = raw[u][e];  // a value: a bit cast of the element reads element 0
-                        const t2 z = __builtin_bit_cast(t2, word);
-                        x[2 * e] = (float)z[0];
-                        x[2 * e + 1] = (float)z[1];
-                    }
+                    a = a1 = at * P.inv_freq[p];
                 }
-                if (I.w) {
-                    float ss = 0.f;
-#pragma unroll
-                    for (int e = 0; e < E; ++e) ss += x[e] * x[e];
-                    for (int off = 1; off < P.lpr; off <<= 1) ss += __shfl_xor(ss, off);
-                    const float r = rsqrtf(ss / (float)P.dim + P.eps);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) x[e] = x[e] * r * w[e];
-                }
-                if (turn) {
-#pragma unroll
-                    for (int e = 0; e < E; e += 2) {
-                        const float z = x[e] * cs[e] - x[e + 1] * sn[e];
-                        x[e + 1] = x[e + 1] * cs[e + 1] + x[e] * sn[e + 1];
-                        x[e] = z;
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (E == 4) y[u][e] = __float_as_uint(x[e]);
-                    else y[u][e] = draft_pack2<T>(x[2 * e], x[2 * e + 1]);
-                }
-                if (!here) y[u] = u32x4_d{0u, 0u, 0u, 0u};
             }
+            page_sincos<T>(a, s0, c0);
+            float s1 = s0, c1 = c0;
+            if (__any(a1 != a)) page_sincos<T>(a1, s1, c1);  // usually they turn by one angle
+            *reinterpret_cast<float2*>(s + 2 * p) = make_float2(s0, s1);
+            *reinterpret_cast<float2*>(c + 2 * p) = make_float2(c0, c1);
+        }
+        // other lanes of the wave read them: LDS keeps a wave's order, the compiler has to as well
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int h = h0 + u * per;
-                if (in && h < I.heads) *reinterpret_cast<u32x4_d*>(out + h * sh) = y[u];
+        for (int e = 0; e < E; e += 4) {
+            const int at = in ? d0 + e : 0;
+            const float4 x = *reinterpret_cast<const float4*>(c + at), y = *reinterpret_cast<const float4*>(s + at);
+            cs[e] = x.x, cs[e + 1] = x.y, cs[e + 2] = x.z, cs[e + 3] = x.w;
+            sn[e] = y.x, sn[e + 1] = y.y, sn[e + 2] = y.z, sn[e + 3] = y.w;
+        }
+    }
+    T* out;
+    int64_t sh;
+    if (I.pages) {
+        sh = (int64_t)P.dim << P.p.lg;
+        out = reinterpret_cast<T*>(I.pages) + (place >> P.p.lg) * I.heads * sh + (place & ((1 << P.p.lg) - 1)) * P.dim + d0;
+    } else {
+        sh = I.out.sh;
+        out = I.out.at<T>(src_b, 0) + (int64_t)tok * I.out.sn + d0;
+    }
+    const float rdim = 1.f / (float)P.dim;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float v[E];
+        page_numbers<T>(raw[u], v);
+        if (I.w) {
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) ss = fmaf(v[e], v[e], ss);
+            const float r = rsqrtf(fmaf(page_sum(ss, P.lpr), rdim, P.eps));
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = v[e] * r * w[e];
+        }
+        if (turn) {
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float z = v[e] * cs[e] - v[e + 1] * sn[e];
+                v[e + 1] = v[e + 1] * cs[e + 1] + v[e] * sn[e + 1];
+                v[e] = z;
             }
         }
+        u32x4_d y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (E == 4) y[e] = __float_as_uint(v[e]);
+            else y[e] = draft_pack2<T>(v[2 * e], v[2 * e + 1]);
+        }
+        if (!here) y = u32x4_d{0u, 0u, 0u, 0u};
+        if (in && h0 + u * group < I.heads) *reinterpret_cast<u32x4_d*>(out + (h0 + u * group) * sh) = y;
     }
 }
 
@@ -521,8 +612,6 @@ size_t plan_scratch(const pa_page_table& t, PagePlan* P) {
     P->moves = reinterpret_cast<int4*>(take(std::max<size_t>(t.rows, t.pages / 2 + 1) * sizeof(int4)));
     P->list = reinterpret_cast<int32_t*>(take((size_t)t.pages * 4));
     P->need = reinterpret_cast<int32_t*>(take((size_t)t.rows * 4));
-    P->upto = reinterpret_cast<int32_t*>(take((size_t)t.rows * 4));
-    P->after = reinterpret_cast<int32_t*>(take((size_t)t.rows * 4));
     P->copy = reinterpret_cast<int32_t*>(take((size_t)t.rows * t.max_pages * 4));
     return n;
 }
@@ -562,11 +651,18 @@ size_t page_scratch(const pa_page_table* t) {
 // workgroups of the copies: four waves each, the whole card where a pool is compacted; a step's copies are few
 // and mostly none
 constexpr int kCopyGroups = 2048, kStepGroups = 256;
+// entries of a table that one workgroup selects
+constexpr int64_t kSelectSmall = 8192;
 
 int launch_page_select(const pa_page_call* c, hipStream_t s) {
     PagePlan P;
     if (const int st = plan_dev(c, P)) return st;
     if (!P.index) return PA_EINVAL;
+    if ((int64_t)P.rows * P.max_pages <= kSelectSmall) {
+        ProfScope ps("page_select", s);
+        hipLaunchKernelGGL(k_page_select_all, dim3(1), dim3(kPlanThreads), 0, s, P);
+        return PA_OK;
+    }
     {
         ProfScope ps("page_select", s);
         hipLaunchKernelGGL(k_page_select, dim3(P.rows), dim3(kPageThreads), 0, s, P);
@@ -646,6 +742,7 @@ int launch_page_append(const pa_page_rows* r, hipStream_t s) {
     const int E = T == PA_F32 ? 4 : 8;
     P.lpr = 1;
     while (P.lpr * E < r->dim) P.lpr <<= 1;
+    int64_t groups = 0;  // four groups of rows each
     for (int k = 0; k < r->count; ++k) {
         const pa_page_item& it = r->items[k];
         if (!it.src.ptr || it.src.heads < 1 || it.src.dtype != T || !it.out.ptr == !it.pages ||
@@ -661,10 +758,17 @@ int launch_page_append(const pa_page_rows* r, hipStream_t s) {
         I.wdt = it.weight_dtype;
         I.rotate = it.rotate;
         I.heads = it.src.heads;
+        I.wide = (uintptr_t)it.norm_weight % 16 == 0 && (it.weight_dtype == PA_F32 || it.weight_dtype == T);
+        P.first[k] = (int)groups;
+        const int rows = kAppendGroups * (64 / P.lpr);
+        groups += (I.heads + rows - 1) / rows;
     }
+    if (groups > 65535) return PA_EUNSUPPORTED;
+    for (int k = r->count; k < PA_MAX_ORDER + 2; ++k) P.first[k] = INT32_MAX;
     const int64_t tokens = (int64_t)r->tokens * (r->packed ? 1 : r->t.rows);
     if (tokens > kPageGroups) return PA_EUNSUPPORTED;
-    const dim3 grid((unsigned)tokens, tokens < 512 ? r->count : 1);
+    P.all = (int)tokens;
+    const dim3 grid((unsigned)((tokens + kPageThreads / 64 - 1) / (kPageThreads / 64)), (unsigned)groups);
     ProfScope ps("page_append", s);
     if (T == PA_F32) hipLaunchKernelGGL((k_page_append<float>), grid, dim3(kPageThreads), 0, s, P);
     else if (T == PA_F16) hipLaunchKernelGGL((k_page_append<f16>), grid, dim3(kPageThreads), 0, s, P);
