@@ -330,8 +330,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_plan(const PagePlan P) {
 }
 
 // The moves of pages, in every array, and with `remap` the table's entries that follow them.  Bound by memory: 16 bytes a
-// lane, eight loads in flight.  A wave takes a part of a page at a time: as many parts as give each wave four or so,
-// at least 8 KB of the largest pages.
+// lane, eight loads in flight, stores past the caches (half a GB moved in a pool 245 us without, 235 with).  A wave takes
+// a part of a page at a time: as many parts as give each wave four or so.
 __global__ __launch_bounds__(kPageThreads) void k_page_copy(const PagePlan P, int remap) {
     const int lane = threadIdx.x & 63;
     const int64_t waves = (int64_t)gridDim.x * (kPageThreads / 64);
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(kPageThreads) void k_page_copy(const PagePlan P, in
                 }
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    if (x0 + 64 * u + lane < end) *reinterpret_cast<W*>(dst + at[u]) = v[u];
+                    if (x0 + 64 * u + lane < end) __builtin_nontemporal_store(v[u], reinterpret_cast<W*>(dst + at[u]));
             }
         };
         if (bytes % 16 == 0) move(u32x4_d{});  // a head of a page has 16 rows or more
@@ -648,9 +648,9 @@ size_t page_scratch(const pa_page_table* t) {
     return plan_scratch(x, nullptr);
 }
 
-// workgroups of the copies: four waves each, the whole card where a pool is compacted; a step's copies are few
-// and mostly none
-constexpr int kCopyGroups = 2048, kStepGroups = 256;
+// Workgroups of the copies, four waves each.  Half a GB moved in a pool: 1024 235 us, 512 278, 2048 260; 24 pages of 40
+// arrays, partly filled: 256 24 us, 512 17, 1024 18.
+constexpr int kCopyGroups = 1024, kStepGroups = 512;
 // entries of a table that one workgroup selects
 constexpr int64_t kSelectSmall = 8192;
 

@@ -291,30 +291,35 @@ class PagedCache:
         P, kv = plan
         B, H, T, d = q1.shape
         dtype, device, grad = self.dtype, self.device, torch.is_grad_enabled()
+        index, unit = device.index, dtype.itemsize
         keep = []
         P.eps = eps
         self._set_angles(P, angles, inv_freq, interp, B, T, keep)
-        shape = q1.shape
+        shape, items = q1.shape, P.items
         for k, src in enumerate((*qs, v)):
-            if src.shape != shape or src.dtype is not dtype or src.device != device:
+            if src.shape != shape or src.dtype is not dtype or src.get_device() != index:
                 self._check_rows(src, f"q{k + 1}" if k <= order else "v", shape)
             w = weights[k] if k <= order else None
             if grad and (src.requires_grad or (w is not None and w.requires_grad)):
                 raise RuntimeError(_NO_GRAD)
             shape = kv
-            src = _rows16(src)
-            keep.append(src)
-            it = P.items[k]
+            s0, s1, s2, s3 = src.stride()
+            ptr = src.data_ptr()
+            if s3 != 1 or ((s0 | s1 | s2) * unit | ptr) & 15:
+                src = _rows16(src)
+                keep.append(src)
+                s0, s1, s2, _ = src.stride()
+                ptr = src.data_ptr()
+            it = items[k]
             view = it.src
-            view.ptr = src.data_ptr()
-            view.sb, view.sh, view.sn, _ = src.stride()
+            view.ptr, view.sb, view.sh, view.sn = ptr, s0, s1, s2
             if w is None:
                 it.norm_weight = None
                 continue
             code = DTYPE_CODE.get(w.dtype)
-            if code is None or w.dim() != 1 or w.numel() != d or w.device != device:
+            if code is None or w.shape != (d,) or w.get_device() != index:
                 _need(False, f"norm weight {k}: [{d}] on the cache's device")
-            if w.stride(0) != 1:
+            if not w.is_contiguous():
                 w = w.contiguous()
                 keep.append(w)
             it.norm_weight, it.weight_dtype = w.data_ptr(), code
