@@ -84,6 +84,14 @@ __device__ __forceinline__ void plan_refs(const PagePlan& P, int64_t first, int 
     }
 }
 
+// the free ones among them, a bit each
+__device__ __forceinline__ uint32_t plan_free(const int (&r)[16]) {
+    uint32_t free = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) free |= (uint32_t)(r[k] == 0) << k;
+    return free;
+}
+
 __device__ __forceinline__ int plan_count(const PagePlan& P, int b) {
     return min(max(P.counts[b], 0), P.max_pages << P.lg);
 }
@@ -106,7 +114,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_extend(const PagePlan P) 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int size = 1 << P.lg;
     int r[16];
-    plan_refs(P, (int64_t)tid * 16, 1, r);  // nothing below writes them before they have been looked at
+    plan_refs(P, (int64_t)tid * 16, 1, r);
+    uint32_t free = plan_free(r);  // nothing below writes them before they have been looked at
     for (int b = tid; b < P.rows; b += kPlanThreads) {
         int n, m;
         bool past;
@@ -167,18 +176,13 @@ __global__ __launch_bounds__(kPlanThreads) void k_page_extend(const PagePlan P) 
     constexpr int U = 16;
     for (int64_t p0 = 0; p0 < P.pages && found < needed; p0 += kPlanThreads * U) {
         const int64_t first = p0 + (int64_t)tid * U;
-        if (p0 > 0) plan_refs(P, first, 1, r);
-        int mine = 0;
-#pragma unroll
-        for (int k = 0; k < U; ++k) mine += r[k] == 0;
-        const Sums s = block_sums(mine, 0, s_part, tid);
+        if (p0 > 0) {
+            plan_refs(P, first, 1, r);
+            free = plan_free(r);
+        }
+        const Sums s = block_sums(__popc(free), 0, s_part, tid);
         int64_t at = found + s.a;
-#pragma unroll
-        for (int k = 0; k < U; ++k)
-            if (r[k] == 0) {
-                if (at < needed) P.list[at] = (int)(first + k);
-                ++at;
-            }
+        for (; free && at < needed; free &= free - 1, ++at) P.list[at] = (int)(first + __ffs(free) - 1);
         found += s.all_a;
     }
     __syncthreads();

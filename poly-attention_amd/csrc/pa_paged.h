@@ -346,7 +346,7 @@ __device__ __forceinline__ bool paged_join(const PagedDev& P, const PagedUnit& U
                 }
             }
         if (!finish) __syncthreads();  // the first record has been read
-        auto end = [&](float& top, float& sum, float4& y, int row) __attribute__((always_inline)) {
+        auto end = [&](float top, float sum, float4 y, int row) __attribute__((always_inline)) {
             none = none || sum != sum;
             if (row - i + i0 < n && parts > 1) {  // a row in some thread
                 float* const mine = s_red[tid];
