@@ -290,12 +290,12 @@ struct PagedRecords {
 
 // Joins `count` records, `first` and every `ustep`-th after it, of n query rows of a tile, r first, by the workgroup:
 // M 2^lgr rows at a time, M of them and four features a thread, the records dealt out over what is left of the
-// threads, so that eight loads or so are under way.  The rows are finished, or the first record takes what was
+// threads, so that 8 to 16 loads are under way.  The rows are finished, or the first record takes what was
 // joined.  True where a record's sum is no number.
 template <typename T, int M, bool GPU>
 __device__ __forceinline__ bool paged_join(const PagedDev& P, const PagedUnit& U, int hk, int first, int ustep, int count, bool finish,
                                            int r, int n, int lgr, float (*s_red)[6]) {
-    constexpr int N = M >= 4 ? 2 : M == 2 ? 4 : 6;
+    constexpr int N = M >= 2 ? 4 : 6;
     const PagedRecords<GPU> R(P, U, hk);
     const int tid = threadIdx.x;
     const int quads = P.dim >> 2;

@@ -237,7 +237,11 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[rt][t][i] = cl2 * tanhf(x[rt][t][i]);
+                    for (int i = 0; i < 4; ++i) {
+                        // tanh(x) = 1 - 2 / (e^2x + 1) to 2^-23 or so absolutely, which 16-bit operands do not see
+                        if constexpr (G::F32) x[rt][t][i] = cl2 * tanhf(x[rt][t][i]);
+                        else x[rt][t][i] = fmaf(-2.f * cl2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.f * kLog2e * x[rt][t][i]) + 1.f), cl2);
+                    }
         }
         if (P.bias) {
 #pragma unroll
