@@ -246,9 +246,12 @@ int launch_paged_attend(const pa_paged* p, hipStream_t s) {
     if (!p->workspace || (uintptr_t)p->workspace % 16 != 0 || p->workspace_bytes < paged_attend_workspace(p))
         return PA_EWORKSPACE;
     P.sc = soft_clamp_dev(P.scale, P.softclamp, true);
-    for (int last = 0; last < 2; ++last)
-        for (int many = 0; many < 2; ++many)
-            if (paged_plan(p, last, many, true, P).units * p->kv_heads > kPageGroups) return PA_EUNSUPPORTED;
+    for (int last = 0; last < 2; ++last) {
+        const bool many = paged_many(p, last);
+        if (paged_plan(p, last, false, many, P).units * p->kv_heads > kPageGroups ||
+            (many && paged_plan(p, last, true, true, P).units * p->kv_heads > kPageGroups))
+            return PA_EUNSUPPORTED;
+    }
     for (int t = 0; t < p->order; ++t) {
         const bool last = t == p->order - 1, middle_next = t + 1 < p->order - 1;
         const pa_paged_level& l = p->levels[t];

@@ -220,3 +220,20 @@ def test_oracle_table_waits():
     t.select([0, 0, -1])
     t.overflow = False
     assert t.extend([1, 1, 0]) == [] and t.new == [0, 0, 0] and t.overflow
+
+
+@pytest.mark.parametrize("dtype, tokens", [(_lib.PA_F32, 1 << 27), (_lib.PA_BF16, 1 << 29)])
+def test_attend_refuses_more_units_than_a_launch_has(dtype, tokens):
+    P = attend_args(2)
+    P.dtype = P.q.dtype = P.out.dtype = dtype
+    P.heads = P.q.heads = P.out.heads = 2
+    P.tokens = tokens
+    P.workspace_bytes = _lib.load().pa_paged_attend_workspace(ctypes.byref(P))
+    assert _lib.load().pa_paged_attend(ctypes.byref(P), None) == _lib.PA_EUNSUPPORTED
+
+
+def test_attend_refuses_more_heads_than_tickets():
+    P = attend_args(2)
+    P.heads = P.q.heads = P.out.heads = P.kv_heads = 5000
+    P.workspace_bytes = _lib.load().pa_paged_attend_workspace(ctypes.byref(P))
+    assert _lib.load().pa_paged_attend(ctypes.byref(P), None) == _lib.PA_EUNSUPPORTED
