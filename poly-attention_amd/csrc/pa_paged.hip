@@ -143,8 +143,10 @@ constexpr int64_t kPagedMany = 2, kPagedLarge = 256 * 1024, kPagedSmall = 64 * 1
 // Units of k_paged_tiles: two chunks at least, and no more than there is room for at once (4 ragged chunks of 512 behind
 // 2048, 32/8 heads of 128: 164 us, with twice as many 220; 512 behind 32768: 436 and 491).
 constexpr int kTilesFewest = 2;
-// chunks of more query rows per key head than this go to k_paged_tiles, where it applies
-constexpr int kPagedFewRows = 32;
+// Chunks of more query rows per key head than this go to k_paged_tiles, where it applies.  8 rows behind 4096 positions, both
+// levels of order 2, 32/8 heads of 128, us: 12 tokens (48 rows at the final level) 67 so and 74 with k_paged_tiles there,
+// 16 68 and 75, 24 (96 rows) 96 with k_paged_rows there and 81 so; 16 heads of 64, 40 tokens 89 so and 99.
+constexpr int kPagedFewRows = 64;
 
 // What a launch of a level takes: its tiles and their split.
 struct PagedPlan {

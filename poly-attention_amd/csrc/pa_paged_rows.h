@@ -1,4 +1,4 @@
-// pa_paged_rows.h -- k_paged_rows: a unit of positions for up to 32 query rows.
+// pa_paged_rows.h -- k_paged_rows: a unit of positions for up to 32 query rows of a chunk.
 //
 // One workgroup per (unit, key head), four waves, each on its own 32 (fp32: 16) positions at a time; nothing
 // is shared until the end, so there is no barrier in the loop.  The products and the lane layout are those
