@@ -502,8 +502,7 @@ typedef struct pa_page_table {
     int32_t* scratch;   /* device [pa_page_scratch bytes]: contents do not matter between calls */
 } pa_page_table;
 
-/* An array whose pages move: [pages, heads, page_size, row_bytes]; row_bytes 4 or a multiple of 16 (16-byte
- * aligned then). */
+/* An array whose pages move: [pages, heads, page_size, row_bytes], 16-byte aligned; row_bytes 4 or a multiple of 16. */
 typedef struct pa_page_array {
     void*   base;
     int32_t heads, row_bytes;
@@ -570,7 +569,8 @@ typedef struct pa_paged_level {
  *   values[t + 1]_p = round(o * vmul[t + 1])  where level t + 1 is a middle one, else round(o)
  * and the final o goes to out.  What a level leaves in the cache is what the next one reads, so that
  * results do not depend on how a row's tokens were cut into chunks beyond the rounding of sums.  Sums,
- * maxima and logsumexps are fp32.  out is 0 for tokens behind their chunk. */
+ * maxima and logsumexps are fp32.  out is 0 for tokens behind their chunk.  kv_heads up to PA_PAGED_TICKETS / 2.  Calls
+ * that may overlap need tickets and a workspace of their own. */
 typedef struct pa_paged {
     pa_page_table  t;
     int32_t        tokens, packed, heads, kv_heads, dim, order, dtype;

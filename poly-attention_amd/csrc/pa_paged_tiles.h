@@ -14,6 +14,11 @@
 // No maximum is taken per tile: the probabilities are formed against the running one, and a tile whose sums
 // say that it was passed by far, or a row that has none yet, is formed again (kTileCap).  Scores get the logsumexp
 // of the level below as the products' initial value.
+//
+// A weight enters its product rounded once to the operands' type (k_paged_rows takes it as two numbers): of a row's many
+// weights each is off by at most half a step, and the output, 2^-9 off by its own rounding in bf16, is some 1.3 times as far
+// off (0.0023 against 0.0017 in norm over three levels), where a second product would make half as many products more.  The
+// final level divides by the sum of the rounded weights; a level whose logsumexp is kept by that of the fp32 ones.
 #pragma once
 
 #include <type_traits>

@@ -2,8 +2,9 @@
 
 Public names as the reference's ``poly_attention/__init__.py:1-7``.  The attention core runs
 in libpolyattn.so (hand-written HIP kernels for gfx950) on GPU tensors.  Additions:
-``StaticCache``, a fixed-capacity KV cache for decode loops captured into a HIP graph, and
-``DraftCache``, ``verify_drafts`` and ``commit_drafts`` for decoding with drafted tokens.
+``StaticCache``, a fixed-capacity KV cache for decode loops captured into a HIP graph,
+``DraftCache``, ``verify_drafts`` and ``commit_drafts`` for decoding with drafted tokens, and
+``PageTable`` and ``PagedCache``, rows of any lengths in the pages of one pool, for serving.
 """
 
 from poly_attention.poly_attention import Order2PolyAttention
