@@ -457,12 +457,12 @@ template <typename T> constexpr int paged_row_tiles(int D) { return D > 128 ? 1 
 // Waves per SIMD that the registers are held to
 constexpr int paged_waves(int D, int RT) { return D <= 128 && D * RT <= 256 ? 2 : 1; }
 
-// clear: workgroups that clear outputs, behind those of the units
-template <typename T> void launch_paged_rows(const PagedDev& P, int64_t units, int clear, int tiles, hipStream_t s);
+// joins: workgroups that join the tiles of B; clear: those that clear outputs
+template <typename T> void launch_paged_rows(const PagedDev& P, const PagedDev& B, int64_t units, int joins, int clear, int tiles, hipStream_t s);
 // in source files of their own
-extern template void launch_paged_rows<bf16>(const PagedDev& P, int64_t units, int clear, int tiles, hipStream_t s);
-extern template void launch_paged_rows<f16>(const PagedDev& P, int64_t units, int clear, int tiles, hipStream_t s);
-extern template void launch_paged_rows<float>(const PagedDev& P, int64_t units, int clear, int tiles, hipStream_t s);
+extern template void launch_paged_rows<bf16>(const PagedDev& P, const PagedDev& B, int64_t units, int joins, int clear, int tiles, hipStream_t s);
+extern template void launch_paged_rows<f16>(const PagedDev& P, const PagedDev& B, int64_t units, int joins, int clear, int tiles, hipStream_t s);
+extern template void launch_paged_rows<float>(const PagedDev& P, const PagedDev& B, int64_t units, int joins, int clear, int tiles, hipStream_t s);
 // 16-bit chunks of more rows (k_paged_tiles), head dims up to 128
 constexpr int paged_tile_rows(int D) { return 256; }
 template <typename T> void launch_paged_tiles(const PagedDev& P, int64_t units, hipStream_t s);

@@ -2,5 +2,5 @@
 #include "pa_paged_rows.h"
 
 namespace pa {
-template void launch_paged_rows<float>(const PagedDev& P, int64_t units, int clear, int tiles, hipStream_t s);
+template void launch_paged_rows<float>(const PagedDev& P, const PagedDev& B, int64_t units, int joins, int clear, int tiles, hipStream_t s);
 }  // namespace pa

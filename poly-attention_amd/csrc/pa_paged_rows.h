@@ -7,7 +7,7 @@
 // their page is a scalar, read from a register of 64 of them that is loaded ahead.
 #pragma once
 
-#include "pa_paged.h"
+#include "pa_paged_join.h"
 
 namespace pa {
 
@@ -28,8 +28,9 @@ __device__ __forceinline__ uint32_t paged_finite(uint32_t w) {
 // keeps a rarely taken branch one
 __device__ __forceinline__ void keep_branch_rows() { asm volatile("" ::: "memory"); }
 
-template <typename T, int D, int RT>
-__global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows(const PagedDev P) {
+// workgroups: the units', with JOIN `joins` for B's tiles of many rows (whose launch came before), and those that clear outputs
+template <typename T, int D, int RT, bool JOIN>
+__global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows(const PagedDev P, const PagedDev B, int joins) {
     typedef DraftGeo<T, D> G;
     constexpr int KT = G::KT, KS = G::KS, VE = G::VE, KE = G::KE, CPR = G::CPR, LOADS = KT * KS;
     constexpr int PITCH = D + 4;
@@ -50,7 +51,15 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
     const int c = lane & 15, g = lane >> 4;
     const int main = P.units * P.kv_heads;
     if ((int)blockIdx.x >= main) {
-        paged_clear<T>(P, blockIdx.x - main, gridDim.x - main);
+        const int group = blockIdx.x - main;
+        if constexpr (JOIN)
+            if (group < joins) {
+                SlowRow& slow = *reinterpret_cast<SlowRow*>(s_o);
+                if (B.recs > 0) paged_join_tiles<T>(B, group, joins, reinterpret_cast<float(*)[6]>(&slow + 1), slow);
+                paged_again<T>(B, group, joins, slow);
+                return;
+            }
+        paged_clear<T>(P, group - joins, gridDim.x - main - joins);
         return;
     }
     const int hk = __builtin_amdgcn_readfirstlane(blockIdx.x % P.kv_heads);
@@ -480,20 +489,25 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
 }
 
 template <typename T, int D>
-void launch_paged_rows_d(const PagedDev& P, int64_t units, int clear, int tiles, hipStream_t s) {
-    const dim3 grid((unsigned)(units * P.kv_heads + clear)), block(kPageThreads);
-    if constexpr (paged_row_tiles<T>(D) >= 2)
-        if (tiles == 2) {
-            hipLaunchKernelGGL((k_paged_rows<T, D, 2>), grid, block, 0, s, P);
+void launch_paged_rows_d(const PagedDev& P, const PagedDev& B, int64_t units, int joins, int clear, int tiles, hipStream_t s) {
+    const dim3 grid((unsigned)(units * P.kv_heads + joins + clear)), block(kPageThreads);
+    if constexpr (sizeof(T) == 2 && D <= 128)
+        if (joins) {
+            hipLaunchKernelGGL((k_paged_rows<T, D, 2, true>), grid, block, 0, s, P, B, joins);
             return;
         }
-    hipLaunchKernelGGL((k_paged_rows<T, D, 1>), grid, block, 0, s, P);
+    if constexpr (paged_row_tiles<T>(D) >= 2)
+        if (tiles == 2) {
+            hipLaunchKernelGGL((k_paged_rows<T, D, 2, false>), grid, block, 0, s, P, B, joins);
+            return;
+        }
+    hipLaunchKernelGGL((k_paged_rows<T, D, 1, false>), grid, block, 0, s, P, B, joins);
 }
 template <typename T>
-void launch_paged_rows(const PagedDev& P, int64_t units, int clear, int tiles, hipStream_t s) {
-    if (P.dim <= 64) launch_paged_rows_d<T, 64>(P, units, clear, tiles, s);
-    else if (P.dim <= 128) launch_paged_rows_d<T, 128>(P, units, clear, tiles, s);
-    else launch_paged_rows_d<T, 256>(P, units, clear, tiles, s);
+void launch_paged_rows(const PagedDev& P, const PagedDev& B, int64_t units, int joins, int clear, int tiles, hipStream_t s) {
+    if (P.dim <= 64) launch_paged_rows_d<T, 64>(P, B, units, joins, clear, tiles, s);
+    else if (P.dim <= 128) launch_paged_rows_d<T, 128>(P, B, units, joins, clear, tiles, s);
+    else launch_paged_rows_d<T, 256>(P, B, units, joins, clear, tiles, s);
 }
 
 }  // namespace pa
