@@ -7,7 +7,7 @@
 // on the device only: every workgroup finds its unit from them (a scan over the rows by a wave), and the
 // grid is the most units there can be (one without a unit is gone after 2 us; a launch of such 4.7).  A tile of one unit
 // is finished where it is computed; the others leave records (maximum, sum, weighted values), which few rows' last unit
-// joins, and k_paged_join those of many rows: a workgroup reads some 25 GB/s, as each CU does that has work of its own,
+// joins, and workgroups of the next launch those of many rows: a workgroup reads some 25 GB/s, as each CU does that has work of its own,
 // so 256 rows of 8 units took 20 us in the last unit and take 9 in a launch of their own, 28 rows of 9 units 10.
 // The levels follow one another, as each reads what the one below left in the cache.
 #pragma once
@@ -427,7 +427,7 @@ __device__ __forceinline__ void paged_end(const PagedDev& P, const PagedUnit& U,
 
 // Where values that are not finite lie behind some row's own position, the products of k_paged_tiles are no numbers: a
 // weight of 0 times such a value.  A unit says so by a sum that is no number, in its records, or where it is its tile's
-// only one by a byte for each of its waves; k_paged_join then forms the rows again, one after another.
+// only one by a byte for each of its waves; the join then forms the rows again, one after another.
 __device__ __forceinline__ uint8_t* paged_flag(const PagedDev& P, int wave) {
     return P.flags + 8 * (int64_t)blockIdx.x + wave;
 }

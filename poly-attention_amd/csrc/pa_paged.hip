@@ -34,20 +34,23 @@ DraftRow paged_view(const pa_view& v) {
 constexpr int64_t kPagedCus = 256;
 // Units of k_paged_rows: each has its latencies (some 6 us alone), so they are of 64 KB of keys at least, and
 // no more than there is room for at once where that leaves them at most 256 KB; beyond, twice as many, which the uneven
-// ends of rows fill better.  Measured, us: 32 ragged rows of up to 8192 positions, 32/8 heads of 128, 227 so, 236 with
-// three times as many, 247 with up to 512 KB; one row of 65536 116, 129 with up to 128 KB only, 109 with 512; 6 ragged
-// chunks behind 5003, 12/4 heads of 128, 111, with 32 KB at least 124, 128 KB 117.
+// ends of rows fill better.  Measured, us: 32 ragged rows of up to 8192 positions, 32/8 heads of 128, 227 so, 266 with
+// only as many as there is room for, 234 with three times as many, 244 with up to 512 KB; one row of 65536 109, with up to
+// 128 KB 119, 512 KB 106.  With 128 KB at least 6 ragged chunks behind 5003, 12/4 heads of 128, 83 and 75 so; fp32
+// chunks behind 1111, 8/2 heads of 96, 69 and 63.
 constexpr int64_t kPagedMany = 2, kPagedLarge = 256 * 1024, kPagedSmall = 64 * 1024;
 // Units of k_paged_tiles: two chunks at least, and no more than there is room for at once (4 ragged chunks of 512 behind
-// 2048, 32/8 heads of 128: 164 us, with twice as many 220; 512 behind 32768: 436 and 491).
+// 2048, 32/8 heads of 128: 173 us, with twice as many 236; 512 behind 32768: 489 and 525; a prompt's 512 among 15 tokens, order
+// 3, 16 heads of 64: 141, with four chunks at least 160).
 constexpr int kTilesFewest = 2;
 // Up to so many workgroups that join tiles share the launch of the few rows', behind those: 512 of them beside 15 rows' tokens
-// (order 3, 16 heads of 64) 142 us so, 160 in a launch of their own.  More would wait for its registers: 2048 of a prompt's
-// 4096 tokens, 32/8 heads of 128, take 30 us in a launch of their own, 47 with it.
+// (order 3, 16 heads of 64) 141 us so, 161 in a launch of their own; beside idle ones (8 rows' 24 tokens) 85 and 81.  More
+// would wait for that launch's registers: 2048 of 4096 tokens, 32/8 heads of 128, 677 us so and 650 in their own.
 constexpr int kPagedJoins = 1024;
 // Chunks of more query rows per key head than this go to k_paged_tiles, where it applies.  8 rows behind 4096 positions, both
-// levels of order 2, 32/8 heads of 128, us: 12 tokens (48 rows at the final level) 67 so and 74 with k_paged_tiles there,
-// 16 68 and 75, 24 (96 rows) 96 with k_paged_rows there and 81 so; 16 heads of 64, 40 tokens 89 so and 99.
+// levels of order 2, us: 32/8 heads of 128, 12 tokens (48 rows at the final level) 68 so and 73 with k_paged_tiles there,
+// 64 tokens (64 rows at the first) 110 and 120, 24 (96 rows) 96 with k_paged_rows there and 85 so; 16 heads of 64, 40
+// tokens 88 so and 97.
 constexpr int kPagedFewRows = 64;
 
 // What a launch of a level takes: its tiles and their split.
