@@ -238,16 +238,12 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
 #pragma unroll
         for (int c = 0; c < NK; ++c) kf[c] = ld_frag<T>(sK + stage * ELEMS + kb * 32 * D + koff[c]);
     };
-    auto load_values = [&](frag (&vf)[2][D / 32], int stage, int kb) __attribute__((always_inline)) {
-#pragma unroll
-        for (int t2 = 0; t2 < 2; ++t2)
-#pragma unroll
-            for (int x = 0; x < D / 32; ++x) {
-                const T* base = sV + stage * ELEMS + (kb * 32 + 16 * t2) * D + voff[x];
-                const u32x2_t lo = lds_read_tr(base), hi = lds_read_tr(base + 8 * D);
-                const u32x4_t v4 = {lo[0], lo[1], hi[0], hi[1]};
-                vf[t2][x] = __builtin_bit_cast(frag, v4);
-            }
+    auto load_value = [&](frag (&vf)[2][D / 32], int stage, int kb, int i) __attribute__((always_inline)) {
+        const int t2 = i / (D / 32), x = i % (D / 32);
+        const T* base = sV + stage * ELEMS + (kb * 32 + 16 * t2) * D + voff[x];
+        const u32x2_t lo = lds_read_tr(base), hi = lds_read_tr(base + 8 * D);
+        const u32x4_t v4 = {lo[0], lo[1], hi[0], hi[1]};
+        vf[t2][x] = __builtin_bit_cast(frag, v4);
     };
     auto check_values = [&](const frag (&vf)[2][D / 32]) __attribute__((always_inline)) {
 #pragma unroll
@@ -299,6 +295,8 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
         begin_rows(s0, 0);
         __builtin_amdgcn_sched_barrier(0);
         u32x4_t pk0[2], pk1[2];
+        frag v0[2][D / 32], v1[QB == 2 ? 1 : 2][D / 32];
+        static_assert(NK == NV, "a fragment of the values takes the place of one of the keys");
         float lt;
         {
             const float msub = without(m[0]);
@@ -306,13 +304,12 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
 #pragma unroll
             for (int i = 0; i < NK; ++i) {
                 s1 = M::run(QB == 2 ? k0[i] : k1[QB == 2 ? 0 : i], qf[R1][i], s1);
+                load_value(v0, stage, kb, i);
                 if (i % (NK / 4) == 0) four(s0, i / (NK / 4), msub, pk0, lts);
                 __builtin_amdgcn_sched_barrier(0);
             }
             lt = (lts[0] + lts[1]) + (lts[2] + lts[3]);
         }
-        frag v0[2][D / 32], v1[QB == 2 ? 1 : 2][D / 32];
-        load_values(v0, stage, kb);
         again(s0, 0, lt, pk0);
         clamp(s1, bias + 32 * kb1);
         if (edge) {
@@ -329,12 +326,12 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
             for (int i = 0; i < NV; ++i) {
                 const int t2 = i / (D / 32), x = i % (D / 32);
                 o[0][x] = M::run(v0[t2][x], __builtin_bit_cast(frag, pk0[t2]), o[0][x]);
+                if constexpr (QB == 1) load_value(v1, stage, 1, i);
                 if (i % (NV / 4) == 0) four(s1, i / (NV / 4), msub, pk1, lts);
                 __builtin_amdgcn_sched_barrier(0);
             }
             lt = (lts[0] + lts[1]) + (lts[2] + lts[3]);
         }
-        if constexpr (QB == 1) load_values(v1, stage, 1);
         again(s1, R1, lt, pk1);
         if constexpr (QB == 1) {
             if (edge) {
