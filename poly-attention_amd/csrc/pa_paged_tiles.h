@@ -234,9 +234,12 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
         l[u] += lt;
     };
     constexpr int NK = D / 16, NV = 2 * (D / 32);  // products of 32 x 32 scores, and of their part of the averages
+    auto load_key = [&](frag (&kf)[NK], int stage, int kb, int c) __attribute__((always_inline)) {
+        kf[c] = ld_frag<T>(sK + stage * ELEMS + kb * 32 * D + koff[c]);
+    };
     auto load_keys = [&](frag (&kf)[NK], int stage, int kb) __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < NK; ++c) kf[c] = ld_frag<T>(sK + stage * ELEMS + kb * 32 * D + koff[c]);
+        for (int c = 0; c < NK; ++c) load_key(kf, stage, kb, c);
     };
     auto load_value = [&](frag (&vf)[2][D / 32], int stage, int kb, int i) __attribute__((always_inline)) {
         const int t2 = i / (D / 32), x = i % (D / 32);
@@ -271,14 +274,14 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
     };
     // Two blocks of 32 x 32 scores, of two blocks of rows (QB 2) or of positions: one's products run beside the other's
     // exponentials.  (A) scores of the first; (B) scores of the second, probabilities of the first; (C) averages of
-    // the first, probabilities of the second; (D) averages of the second.
-    auto step = [&](int stage, int kb, int j0) __attribute__((always_inline)) {
+    // the first, probabilities of the second; (D) averages of the second.  Each fragment is read from LDS when the one that it
+    // follows in its registers has gone into a product: the next step's first keys (k0) in (D), with MORE.
+    auto step = [&](int stage, int kb, int j0, frag (&k0)[NK], auto MORE) __attribute__((always_inline)) {
         constexpr int R1 = QB - 1;  // the second one's rows ...
         const int kb1 = QB == 2 ? kb : 1, j1 = QB == 2 ? j0 : j0 + 32;  // ... and positions
         const float* const bias = &sBw[w][stage & 1][4 * hh];
         const bool edge = j0 + (QB == 2 ? 31 : 63) > all_see || j0 + (QB == 2 ? 32 : 64) > cnt;
-        frag k0[NK], k1[QB == 2 ? 1 : NK];
-        load_keys(k0, stage, kb);
+        frag k1[QB == 2 ? 1 : NK];
         f32x16_t s0 = first_scores(bias + 32 * kb);
 #pragma unroll
         for (int c = 0; c < NK; ++c) s0 = M::run(k0[c], qf[0][c], s0);
@@ -339,11 +342,14 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
                 check_values(v1);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int t2 = 0; t2 < 2; ++t2)
-#pragma unroll
-            for (int x = 0; x < D / 32; ++x)
-                o[R1][x] = M::run(QB == 2 ? v0[t2][x] : v1[QB == 2 ? 0 : t2][x], __builtin_bit_cast(frag, pk1[t2]), o[R1][x]);
+        for (int i = 0; i < NV; ++i) {
+            const int t2 = i / (D / 32), x = i % (D / 32);
+            o[R1][x] = M::run(QB == 2 ? v0[t2][x] : v1[QB == 2 ? 0 : t2][x], __builtin_bit_cast(frag, pk1[t2]), o[R1][x]);
+            if constexpr (MORE) load_key(k0, QB == 2 && !kb ? stage : stage + 1, QB == 2 ? !kb : 0, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
 
     // pairs of tiles, a barrier each: both have landed, and the pair before has been read
@@ -361,10 +367,18 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
                 const int j = j0 + BN * k + lane;
                 sBw[w][k][lane] = j < cnt ? sBraw[st + k][lane] * bmul : -INFINITY;
             }
-        step(st, 0, j0);
-        if (QB == 2 && left > 1) step(st, 1, j0 + 32);
-        if (left > 2) step(st + 1, 0, j0 + 64);
-        if (QB == 2 && left > 3) step(st + 1, 1, j0 + 96);
+        const std::true_type more;
+        const std::false_type last;
+        frag k0[NK];
+        load_keys(k0, st, 0);
+        step(st, 0, j0, k0, more);  // the keys of a step that there is not are read in vain
+        if constexpr (QB == 1) {
+            if (left > 2) step(st + 1, 0, j0 + 64, k0, last);
+        } else {
+            if (left > 1) step(st, 1, j0 + 32, k0, more);
+            if (left > 2) step(st + 1, 0, j0 + 64, k0, more);
+            if (left > 3) step(st + 1, 1, j0 + 96, k0, last);
+        }
     }
 
     if (U.splits > 1 && !paged_recorded(P, U)) return;
