@@ -118,24 +118,23 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
         offv[n] = cv * 8 < P.dim ? (r & 15) * rowb + cv * 16 : kDraftOut;
     }
     const uint32_t lds_k = lds_addr(sK), lds_v = lds_addr(sV), lds_b = lds_addr(&sBraw[0][0]);
-    auto issue = [&](int j0, int stage) __attribute__((always_inline)) {
-        if (j0 >> 10 != block) {
-            block = j0 >> 10;
-            ids = ids_next;
-            if (j0 + 1024 < cnt) ids_next = load_pages((block + 1) << 10);
-        }
+    auto turn_page = [&](int j0) __attribute__((always_inline)) {
+        if (j0 >> 10 == block) return;
+        block = j0 >> 10;
+        ids = ids_next;
+        if (j0 + 1024 < cnt) ids_next = load_pages((block + 1) << 10);
+    };
+    // a wave's part n of NL of a tile's loads; 0 past the unit's end
+    auto issue_part = [&](int j0, int stage, int n) __attribute__((always_inline)) {
         const uint32_t kd = lds_k + (uint32_t)(stage * ELEMS * 2), vd = lds_v + (uint32_t)(stage * ELEMS * 2);
-#pragma unroll
-        for (int n = 0; n < NL; ++n) {
-            const int j = j0 + ((n * NT + w * 64) / CPR & ~15);  // the block of 16 that the wave's rows lie in
-            const int id = __builtin_amdgcn_readlane(ids, (j >> 4) & 63);
-            const bool ok = (unsigned)id < (unsigned)P.p.pages;
-            const int64_t at = (paged_base(P, ok ? id : 0, hk) + ((begin + j) & inside)) * rowb;
-            const uint32_t bytes = ok && j < cnt ? min(16, cnt - j) * rowb : 0;
-            dma16(make_srd(P.keys + at, bytes), kd + (uint32_t)((n * NT + w * 64) * 16), offk[n]);
-            dma16(make_srd(P.values + at, bytes), vd + (uint32_t)((n * NT + w * 64) * 16), offv[n]);
-        }
-        if (BIAS && w < 4) {
+        const int j = j0 + ((n * NT + w * 64) / CPR & ~15);  // the block of 16 that the wave's rows lie in
+        const int id = __builtin_amdgcn_readlane(ids, (j >> 4) & 63);
+        const bool ok = (unsigned)id < (unsigned)P.p.pages;
+        const int64_t at = (paged_base(P, ok ? id : 0, hk) + ((begin + j) & inside)) * rowb;
+        const uint32_t bytes = ok && j < cnt ? min(16, cnt - j) * rowb : 0;
+        dma16(make_srd(P.keys + at, bytes), kd + (uint32_t)((n * NT + w * 64) * 16), offk[n]);
+        dma16(make_srd(P.values + at, bytes), vd + (uint32_t)((n * NT + w * 64) * 16), offv[n]);
+        if (BIAS && n == NL - 1 && w < 4) {
             const int j = j0 + 16 * w;  // a quarter of the tile's
             const int id = __builtin_amdgcn_readlane(ids, (j >> 4) & 63);
             const bool ok = (unsigned)id < (unsigned)P.p.pages;
@@ -143,6 +142,10 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
             if (lane < 4)
                 dma16(make_srd(P.bias + at, ok && j < cnt ? 64 : 0), lds_b + (uint32_t)(stage * BN * 4 + w * 64), 16 * lane);
         }
+    };
+    auto issue = [&](int j0, int stage) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < NL; ++n) issue_part(j0, stage, n);
     };
 
     int koff[D / 16];  // rows col (+ 32 kb), chunk 2c + hh
@@ -276,7 +279,9 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
     // exponentials.  (A) scores of the first; (B) scores of the second, probabilities of the first; (C) averages of
     // the first, probabilities of the second; (D) averages of the second.  Each fragment is read from LDS when the one that it
     // follows in its registers has gone into a product: the next step's first keys (k0) in (D), with MORE.
-    auto step = [&](int stage, int kb, int j0, frag (&k0)[NK], auto MORE) __attribute__((always_inline)) {
+    // (A) has no exponentials beside it, but the loads of the next pair of tiles (side), whose addresses are a good many scalar
+    // instructions.
+    auto step = [&](int stage, int kb, int j0, frag (&k0)[NK], auto MORE, auto side) __attribute__((always_inline)) {
         constexpr int R1 = QB - 1;  // the second one's rows ...
         const int kb1 = QB == 2 ? kb : 1, j1 = QB == 2 ? j0 : j0 + 32;  // ... and positions
         const float* const bias = &sBw[w][stage & 1][4 * hh];
@@ -284,7 +289,10 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
         frag k1[QB == 2 ? 1 : NK];
         f32x16_t s0 = first_scores(bias + 32 * kb);
 #pragma unroll
-        for (int c = 0; c < NK; ++c) s0 = M::run(k0[c], qf[0][c], s0);
+        for (int c = 0; c < NK; ++c) {
+            s0 = M::run(k0[c], qf[0][c], s0);
+            side(c);
+        }
         if constexpr (QB == 1) {
             __builtin_amdgcn_sched_barrier(0);
             load_keys(k1, stage, 1);
@@ -353,14 +361,25 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
     };
 
     // pairs of tiles, a barrier each: both have landed, and the pair before has been read
-    for (int t = 0; t < ntl; t += 2) {
-        const int st = t & 3;
+    int t = 0;
+    auto pair = [&]() __attribute__((always_inline)) {
         wait_vmcnt<0>();
         lds_barrier();
-        if (t + 2 < ntl) issue((t + 2) * BN, st ^ 2);
-        if (t + 3 < ntl) issue((t + 3) * BN, (st ^ 2) + 1);
+        turn_page((t + 2) * BN);  // a pair's tiles lie in one block of 1024
+    };
+    for (; 2 * t < nact; t += 2) {
+        pair();
+        const int st = t & 3;
         const int j0 = t * BN, left = nact - 2 * t;  // 32-position steps of this pair, and further ones
-        if (left <= 0) continue;  // the same barriers in every wave
+        auto next = [&](int c) __attribute__((always_inline)) {
+            constexpr int PER = NK / (2 * NL);  // products between two parts
+            if (c % PER != PER - 1) return;
+            const int n = c / PER % NL, u = c / (PER * NL);
+            __builtin_amdgcn_sched_barrier(0);
+            issue_part((t + 2 + u) * BN, (st ^ 2) + u, n);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto none = [](int) __attribute__((always_inline)) {};
         if (BIAS)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -371,15 +390,21 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
         const std::false_type last;
         frag k0[NK];
         load_keys(k0, st, 0);
-        step(st, 0, j0, k0, more);  // the keys of a step that there is not are read in vain
+        step(st, 0, j0, k0, more, next);  // the keys of a step that there is not are read in vain
         if constexpr (QB == 1) {
-            if (left > 2) step(st + 1, 0, j0 + 64, k0, last);
+            if (left > 2) step(st + 1, 0, j0 + 64, k0, last, none);
         } else {
-            if (left > 1) step(st, 1, j0 + 32, k0, more);
-            if (left > 2) step(st + 1, 0, j0 + 64, k0, more);
-            if (left > 3) step(st + 1, 1, j0 + 96, k0, last);
+            if (left > 1) step(st, 1, j0 + 32, k0, more, none);
+            if (left > 2) step(st + 1, 0, j0 + 64, k0, more, none);
+            if (left > 3) step(st + 1, 1, j0 + 96, k0, last, none);
         }
     }
+    for (; t < ntl; t += 2) {  // the same barriers in every wave
+        pair();
+        issue((t + 2) * BN, (t & 3) ^ 2);
+        issue((t + 3) * BN, ((t & 3) ^ 2) + 1);
+    }
+    wait_vmcnt<0>();  // the loads past the end
 
     if (U.splits > 1 && !paged_recorded(P, U)) return;
     const bool any = __any(odd != 0.f);
