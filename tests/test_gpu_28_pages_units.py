@@ -156,3 +156,33 @@ def test_copies_of_any_page(ps, hk, D, dtype, held):
     assert t.pages[2, 0].item() == 0
     for x, y in zip(now, was):
         assert torch.equal(x[0], y[1]) and torch.equal(x[1:], y[1:])
+
+
+@param("D", [64, 128])
+def test_captured_chunks(D):
+    """Chunks of many and of few rows, captured and replayed between eager calls over other contents."""
+    from poly_attention import PagedCache
+
+    d = dev()
+    g = torch.Generator().manual_seed(21)
+    t, o = make([900, 300, 2000], [400, 1, 30], 64, g)
+    cache = PagedCache(t, order=3, kv_heads=2, dim_head=D, dtype=torch.bfloat16)
+    fill(cache, o, g)
+    xs = [(inputs(o, 8, D, torch.bfloat16, True, g).to(d), inputs(o, 2, D, torch.bfloat16, True, g).to(d)) for _ in range(4)]
+    want = [cache.attend(q, [v]) for q, v in xs]
+    q, v = (x.clone() for x in xs[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.attend(q, [v])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = cache.attend(q, [v])
+    for k in (1, 3, 0, 2, 2):
+        q.copy_(xs[k][0])
+        v.copy_(xs[k][1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[k])
+        assert torch.equal(cache.attend(*[xs[3 - k][0], [xs[3 - k][1]]]), want[3 - k])
