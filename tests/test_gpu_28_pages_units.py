@@ -186,3 +186,53 @@ def test_captured_chunks(D):
         torch.cuda.synchronize()
         assert torch.equal(y, want[k])
         assert torch.equal(cache.attend(*[xs[3 - k][0], [xs[3 - k][1]]]), want[3 - k])
+
+
+@param("rows", [1000, 8192])
+def test_thousands_of_rows(rows):
+    """Every row finds its chunk and its pages: packed and padded steps give the same, and each row what it gives alone."""
+    from poly_attention import PagedCache, PageTable
+
+    d = dev()
+    g = torch.Generator().manual_seed(rows)
+    more = torch.randint(0, 4, (rows,), generator=g)
+    more[0], more[-1] = 3, 2
+    T, hk, D = 3, 2, 64
+    steps = [more, (more + 1) % 4]
+    total = [int(m.sum()) for m in steps]
+    qs = [[torch.randn(rows, hk, T, D, generator=g).to(torch.bfloat16).to(d) for _ in range(4)] for _ in steps]
+    got = []
+    for packed in (False, True):
+        t = PageTable(rows, pages=rows + 40, page_size=16, capacity=32, device=d)
+        c = PagedCache(t, order=2, kv_heads=hk, dim_head=D)
+        outs = []
+        for m, q in zip(steps, qs):
+            t.extend(m.to(d, torch.int32))
+            here = (torch.arange(T) < m[:, None]).to(d)                                  # [rows, T]
+            if packed:
+                q = [x.transpose(1, 2)[here].transpose(0, 1)[None].contiguous() for x in q]
+            q1 = c.append(q[:3], q[3], [None] * 3, eps=1e-6)
+            y = c.attend(q1)
+            if packed:
+                z = torch.zeros(rows, T, hk, D, dtype=y.dtype, device=d)
+                z[here] = y[0].transpose(0, 1)
+                y = z.transpose(1, 2)
+            outs.append(y)
+        assert t.counts.tolist() == (steps[0] + steps[1]).tolist() and not t.overflow.item()
+        assert t.starts[-1].item() == total[1]
+        used = t.pages[t.pages >= 0]
+        assert used.numel() == used.unique().numel() == int((t.refs > 0).sum())
+        got.append(outs)
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    for b in (0, 1, 63, 64, rows // 2, rows - 1):                                        # alone
+        t = PageTable(1, pages=4, page_size=16, capacity=32, device=d)
+        c = PagedCache(t, order=2, kv_heads=hk, dim_head=D)
+        for k, (m, q) in enumerate(zip(steps, qs)):
+            n = int(m[b])
+            t.extend([n])
+            if not n:
+                continue
+            one = [x[b:b + 1, :, :n].contiguous() for x in q]
+            y = c.attend(c.append(one[:3], one[3], [None] * 3, eps=1e-6))
+            assert torch.equal(y, got[0][k][b:b + 1, :, :n])
