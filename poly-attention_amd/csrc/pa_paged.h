@@ -116,10 +116,13 @@ __device__ __forceinline__ bool paged_find(const PagedDev& P, int want, int lane
             chunks0 = chunks;
         }
     }
-    if (P.p.rows > 1)
-        for (int off = 32; off > 0; off >>= 1) total += __shfl_xor((unsigned long long)total, off);
     const int all = __builtin_amdgcn_readlane(paged_scan(all_tiles), 63);
-    total = ((uint64_t)__builtin_amdgcn_readfirstlane((int)(total >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)total);
+    if (!__any(total >> 25 != 0)) {  // the sum is below 2^31
+        total = (uint32_t)__builtin_amdgcn_readlane(paged_scan((int)total), 63);
+    } else {
+        for (int off = 32; off > 0; off >>= 1) total += __shfl_xor((unsigned long long)total, off);
+        total = ((uint64_t)__builtin_amdgcn_readfirstlane((int)(total >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)total);
+    }
     U.size = __builtin_amdgcn_readfirstlane(paged_size(P, total, all));
     int before = 0, recs = 0;  // units are at most the grid's, and blocks of rows fewer than memory holds outputs of
     for (int b0 = 0; b0 < P.p.rows; b0 += 64) {
