@@ -401,12 +401,15 @@ __device__ __forceinline__ bool paged_join(const PagedDev& P, const PagedUnit& U
 }
 
 // The end of a unit of the tile's n query rows, r first, its records written: the last one of its tile joins them, as a
-// ticket says.  More than eight units join in two steps, groups first, as one workgroup reads but 25 to 100 GB/s
-// (one row of 65536 positions 116 us in one step, 109 in two).
+// ticket says.  More than eight units, or than 128 rows of records, join in two steps, groups of about the square root of
+// their number first, as one workgroup reads but 25 GB/s or so: one row of 65536 positions 116 us in one step, 110 in two; 32
+// query rows behind up to 4096 59 with groups of eight, 57 so.
 template <typename T, int M>
 __device__ __forceinline__ void paged_end(const PagedDev& P, const PagedUnit& U, int hk, int r, int n, float (*s_red)[6], int& s_last) {
     const int live = min(U.splits, (paged_keys(P, U) + U.size * kPagedChunk - 1) / (U.size * kPagedChunk));
-    const int size = live <= 8 ? live : live <= 64 ? 8 : 16;
+    int size = live;  // of a group
+    if (live > 8 || live * n > 128)
+        for (size = 2; size * size < live;) ++size;
     const int first = U.split - U.split % size, groups = (live + size - 1) / size, in = min(size, live - first);
     int lgr = 0;  // rows at once, as there are rows, and threads for four features each
     while ((1 << lgr) < n && (((P.dim >> 2) - 1) >> (7 - lgr)) == 0) ++lgr;
