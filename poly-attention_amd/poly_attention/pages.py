@@ -47,8 +47,8 @@ class PageTable:
     free) and ``overflow`` [1].  ``pages``, ``counts`` and ``refs`` together are the state: a copy of the three can be
     written back, as long as the caches' pages were not given to others in between.
 
-    A table and its caches take one call at a time; others may be used at once, on any streams.  ``copy.deepcopy`` of a
-    table, or of the list of its caches, copies the pool."""
+    A table and its caches take one call at a time; others may be used at once, on any streams.  A table whose calls were
+    captured takes no further caches.  ``copy.deepcopy`` of a table, or of the list of its caches, copies the pool."""
 
     def __init__(self, rows: int, *, pages: int, page_size: int = 64, capacity: int, device="cuda"):
         _need(1 <= rows <= PA_MAX_PAGE_ROWS, f"rows {rows}: 1 to {PA_MAX_PAGE_ROWS}")
@@ -75,10 +75,12 @@ class PageTable:
         t.rows, t.pages, t.page_size, t.max_pages = self.rows, self.pool, self.page_size, self.pages.shape[1]
         t.table, t.counts, t.refs = self.pages.data_ptr(), self.counts.data_ptr(), self.refs.data_ptr()
         t.fresh, t.starts, t.overflow = self.new.data_ptr(), self.starts.data_ptr(), self.overflow.data_ptr()
-        self._call_struct = None
+        self._call_struct = self._scratch = self._arrays = None
+        self._captured = False
 
     def __getstate__(self):
-        return {k: v for k, v in self.__dict__.items() if k not in ("_t", "_call_struct", "_scratch", "_arrays")}
+        gone = ("_t", "_call_struct", "_scratch", "_arrays", "_captured")
+        return {k: v for k, v in self.__dict__.items() if k not in gone}
 
     def __setstate__(self, state) -> None:
         self.__dict__.update(state)
@@ -86,16 +88,18 @@ class PageTable:
         self._setup()
 
     def _struct(self):
-        """The structure of the table's own calls; its scratch and the list of arrays live as long as the table."""
+        """The structure of the table's own calls.  Captured steps hold the addresses of its scratch and of the list of
+        arrays: the scratch stays as long as the table, and the list from the first captured call on."""
         c = self._call_struct
         if c is None:
             _need(self.device.type == "cuda", "a PageTable's calls need the GPU (libpolyattn)", RuntimeError)
-            if torch.cuda.is_current_stream_capturing():
+            if self._capturing():
                 raise RuntimeError("PageTable: run one eager call before capturing steps (the list of its caches is "
                                    "written then)")
-            size = _lib.load().pa_page_scratch(ctypes.byref(self._t))
-            self._scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
-            self._t.scratch = self._scratch.data_ptr()
+            if self._scratch is None:
+                size = _lib.load().pa_page_scratch(ctypes.byref(self._t))
+                self._scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
+                self._t.scratch = self._scratch.data_ptr()
             arrays = b"".join(bytes(_lib.PaPageArray(x.data_ptr(), x.shape[1], x.element_size() * (x.shape[3] if x.dim() == 4 else 1)))
                               for cache in self.caches for x in cache.arrays())
             c = _lib.PaPageCall()
@@ -105,7 +109,15 @@ class PageTable:
                 c.arrays = self._arrays.data_ptr()
             c.t = self._t
             self._call_struct = c
+        elif not self._captured:
+            self._captured = self._capturing()
         return c
+
+    def _capturing(self) -> bool:
+        if self.device.index == torch._C._cuda_getDevice():
+            return torch.cuda.is_current_stream_capturing()
+        with torch.cuda.device(self.device):
+            return torch.cuda.is_current_stream_capturing()
 
     def _rows_tensor(self, x, what: str) -> Tensor:
         if isinstance(x, Tensor):
@@ -216,6 +228,9 @@ class PagedCache:
         _need(8 <= dim_head <= 256 and dim_head % (8 if dim_head <= 128 else 16) == 0,
               f"dim_head {dim_head}: a multiple of 8 up to 128, of 16 up to 256")
         self.table, self.order, self.kv_heads, self.dim_head, self.dtype = table, order, kv_heads, dim_head, dtype
+        # a captured step would go on without it: a page of it that rows share would not be copied before one of them writes
+        _need(not table._captured, "a call of the table was captured, and its graph copies the pages of the caches that the "
+              "table had then: make the caches before, or take another table", RuntimeError)
 
         def rows(m):
             return tuple(torch.empty(table.pool, kv_heads, table.page_size, dim_head, dtype=dtype, device=table.device)
