@@ -23,7 +23,9 @@ into a HIP graph.  The calls are for the GPU and for inference.
 
 from __future__ import annotations
 
+import copy
 import ctypes
+import weakref
 from typing import Optional, Sequence
 
 import torch
@@ -47,8 +49,12 @@ class PageTable:
     free) and ``overflow`` [1].  ``pages``, ``counts`` and ``refs`` together are the state: a copy of the three can be
     written back, as long as the caches' pages were not given to others in between.
 
-    A table and its caches take one call at a time; others may be used at once, on any streams.  A table whose calls were
-    captured takes no further caches.  ``copy.deepcopy`` of a table, or of the list of its caches, copies the pool."""
+    ``caches`` are those that there are: a cache holds its table, not the table its caches, and the pages of one that is given
+    up are free memory again, at the latest when the table goes where a call of it was captured.  A table whose calls
+    were captured takes no further caches.
+
+    A table and its caches take one call at a time; others may be used at once, on any streams.  ``copy.deepcopy`` of
+    the list of its caches, or of the table, copies the pool; a table copied by itself holds its copies of the caches."""
 
     def __init__(self, rows: int, *, pages: int, page_size: int = 64, capacity: int, device="cuda"):
         _need(1 <= rows <= PA_MAX_PAGE_ROWS, f"rows {rows}: 1 to {PA_MAX_PAGE_ROWS}")
@@ -65,33 +71,56 @@ class PageTable:
         self.refs, self.starts = torch.zeros(pages, **i32), torch.zeros(rows + 1, **i32)
         self.overflow = torch.zeros(1, **i32)
         self.device = self.counts.device
-        self.caches: list = []
         self._expected = None  # the chunks' tokens, where the host knows them
-        self._setup()
+        self._setup(())
 
-    def _setup(self) -> None:
-        """What holds addresses."""
+    def _setup(self, caches) -> None:
+        """What holds addresses, and the caches."""
         self._t = t = _lib.PaPageTable()
         t.rows, t.pages, t.page_size, t.max_pages = self.rows, self.pool, self.page_size, self.pages.shape[1]
         t.table, t.counts, t.refs = self.pages.data_ptr(), self.counts.data_ptr(), self.refs.data_ptr()
         t.fresh, t.starts, t.overflow = self.new.data_ptr(), self.starts.data_ptr(), self.overflow.data_ptr()
         self._call_struct = self._scratch = self._arrays = None
-        self._captured = False
+        self._captured = None  # the arrays that a captured call has
+        self._caches = weakref.WeakValueDictionary(enumerate(caches))
+        self._listed = 0  # caches whose arrays are on the list
+
+    @property
+    def caches(self) -> list:
+        return list(self._caches.values())
+
+    def _add(self, cache) -> None:
+        self._caches[max(self._caches, default=-1) + 1] = cache
+        self._call_struct = None  # its list of arrays grows
+
+    def _state(self) -> dict:
+        gone = ("_t", "_call_struct", "_scratch", "_arrays", "_captured", "_caches", "_listed", "_own")
+        return {k: v for k, v in self.__dict__.items() if k not in gone}
 
     def __getstate__(self):
-        gone = ("_t", "_call_struct", "_scratch", "_arrays", "_captured")
-        return {k: v for k, v in self.__dict__.items() if k not in gone}
+        return {**self._state(), "_own": self.caches}
 
     def __setstate__(self, state) -> None:
         self.__dict__.update(state)
         self.device = self.counts.device
-        self._setup()
+        self._setup(self._own)
+
+    def _copy(self, memo):
+        """A copy without caches."""
+        other = memo[id(self)] = object.__new__(type(self))
+        other.__setstate__({**copy.deepcopy(self._state(), memo), "_own": []})
+        return other
+
+    def __deepcopy__(self, memo):
+        other = self._copy(memo)
+        other._own = [copy.deepcopy(c, memo) for c in self.caches]
+        return other
 
     def _struct(self):
         """The structure of the table's own calls.  Captured steps hold the addresses of its scratch and of the list of
         arrays: the scratch stays as long as the table, and the list from the first captured call on."""
         c = self._call_struct
-        if c is None:
+        if c is None or (self._listed != len(self._caches) and self._captured is None):
             _need(self.device.type == "cuda", "a PageTable's calls need the GPU (libpolyattn)", RuntimeError)
             if self._capturing():
                 raise RuntimeError("PageTable: run one eager call before capturing steps (the list of its caches is "
@@ -100,17 +129,18 @@ class PageTable:
                 size = _lib.load().pa_page_scratch(ctypes.byref(self._t))
                 self._scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
                 self._t.scratch = self._scratch.data_ptr()
+            caches = self.caches
             arrays = b"".join(bytes(_lib.PaPageArray(x.data_ptr(), x.shape[1], x.element_size() * (x.shape[3] if x.dim() == 4 else 1)))
-                              for cache in self.caches for x in cache.arrays())
+                              for cache in caches for x in cache.arrays())
             c = _lib.PaPageCall()
             c.count = len(arrays) // ctypes.sizeof(_lib.PaPageArray)
             if arrays:
                 self._arrays = torch.frombuffer(bytearray(arrays), dtype=torch.uint8).to(self.device)
                 c.arrays = self._arrays.data_ptr()
             c.t = self._t
-            self._call_struct = c
-        elif not self._captured:
-            self._captured = self._capturing()
+            self._call_struct, self._listed = c, len(caches)
+        elif self._captured is None and self._capturing():
+            self._captured = [x for cache in self.caches for x in cache.arrays()]
         return c
 
     def _capturing(self) -> bool:
@@ -229,7 +259,7 @@ class PagedCache:
               f"dim_head {dim_head}: a multiple of 8 up to 128, of 16 up to 256")
         self.table, self.order, self.kv_heads, self.dim_head, self.dtype = table, order, kv_heads, dim_head, dtype
         # a captured step would go on without it: a page of it that rows share would not be copied before one of them writes
-        _need(not table._captured, "a call of the table was captured, and its graph copies the pages of the caches that the "
+        _need(table._captured is None, "a call of the table was captured, and its graph copies the pages of the caches that the "
               "table had then: make the caches before, or take another table", RuntimeError)
 
         def rows(m):
@@ -242,8 +272,7 @@ class PagedCache:
         # of attend, 0 between calls
         self._tickets = torch.zeros(_lib.PA_PAGED_TICKETS * _lib.PA_TICKET_STRIDE, dtype=torch.int32, device=table.device)
         self._plans: dict = {}
-        table.caches.append(self)
-        table._call_struct = None  # its list of arrays grows
+        table._add(self)
 
     def __getstate__(self):
         return {k: v for k, v in self.__dict__.items() if k != "_plans"}
@@ -251,6 +280,13 @@ class PagedCache:
     def __setstate__(self, state) -> None:
         self.__dict__.update(state)
         self._plans = {}
+
+    def __deepcopy__(self, memo):
+        table = memo.get(id(self.table)) or self.table._copy(memo)
+        other = memo[id(self)] = object.__new__(type(self))
+        other.__setstate__({**copy.deepcopy({k: v for k, v in self.__getstate__().items() if k != "table"}, memo), "table": table})
+        table._add(other)
+        return other
 
     @property
     def device(self):

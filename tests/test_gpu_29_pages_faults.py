@@ -1,5 +1,7 @@
 """GPU: faults that the paged cache had, one test each."""
 
+import weakref
+
 import pytest
 import torch
 
@@ -88,3 +90,56 @@ def test_captured_table_calls_after_much_else():
     for a, b in zip(*runs):
         for x, y in zip(a, b):
             assert torch.equal(x, y)
+
+
+# ---------------------------------------------------------------------------------------
+# caches that are given up
+
+
+def test_a_cache_that_is_gone_is_not_copied():
+    """Its memory is others' at once, and the table's calls leave it alone."""
+    from poly_attention import PagedCache, PageTable
+
+    d = dev()
+    t = PageTable(3, pages=8, page_size=16, capacity=64)
+    caches = [PagedCache(t, order=2, kv_heads=1, dim_head=64, dtype=torch.float32) for _ in range(2)]
+    t.extend([5, 40, 0])
+    gone = [weakref.ref(x) for x in caches[0].arrays()]
+    assert t._call_struct.count == 10
+    del caches[0]
+    assert all(r() is None for r in gone)
+    theirs = [torch.full((8, 1, 16, 64), 7.0, device=d) for _ in range(200)]
+    t.select([0, 1, 0])
+    t.extend([1, 0, 1])                        # row 0 copies the page that it shares
+    t.free([0])
+    t.compact()
+    assert t._call_struct.count == 5
+    assert all(bool((x == 7).all()) for x in theirs)
+    assert t.counts.tolist() == [0, 40, 6]
+
+
+def test_a_captured_call_keeps_its_arrays():
+    from poly_attention import PagedCache, PageTable
+
+    d = dev()
+    t = PageTable(3, pages=8, page_size=16, capacity=64)
+    caches = [PagedCache(t, order=2, kv_heads=1, dim_head=64, dtype=torch.float32) for _ in range(2)]
+    index = torch.tensor([0, 1, 0], dtype=torch.int32, device=d)
+    more = torch.tensor([1, 0, 1], dtype=torch.int32, device=d)
+    t.extend([5, 40, 0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        t.select(index)
+        t.extend(more)
+    keys = weakref.ref(caches[0].keys[0])
+    del caches[0]
+    assert keys() is not None and len(t.caches) == 1
+    theirs = [torch.full((8, 1, 16, 64), 7.0, device=d) for _ in range(200)]
+    for step in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert t.counts.tolist() == [6 + step, 40, 6 + step]
+    t.extend([1, 1, 1])                        # eager calls go on
+    assert all(bool((x == 7).all()) for x in theirs)
+    del t, caches, graph

@@ -1,5 +1,10 @@
 """Faults that the paged cache had and that show without a GPU, one test each."""
 
+import copy
+import gc
+import io
+import weakref
+
 import pytest
 import torch
 
@@ -9,7 +14,67 @@ from test_pages import cache, table
 def test_no_cache_joins_a_captured_table():
     t = table()
     first = cache(t)
-    t._captured = True                         # as a captured call leaves it
+    t._captured = []                           # as a captured call leaves it
     with pytest.raises(RuntimeError, match="captured"):
         cache(t)
     assert t.caches == [first]
+
+
+@pytest.fixture
+def no_collector():
+    gc.collect()
+    gc.disable()
+    yield
+    gc.enable()
+
+
+def test_what_is_given_up_is_gone(no_collector):
+    """Caches and their table are let go without the collector of cycles, and a cache alone while its table lives."""
+    t = table()
+    caches = [cache(t), cache(t, order=3), cache(t)]
+    kept = [weakref.ref(x) for x in (t, caches[1], caches[1].keys[0], caches[2].values[1], t.counts)]
+    caches[1:2] = []
+    assert [r() is None for r in kept] == [False, True, True, False, False]
+    assert t.caches == caches
+    caches.append(cache(t))
+    assert t.caches == caches
+    del t, caches
+    assert all(r() is None for r in kept)
+
+
+def test_copies_are_let_go_too(no_collector):
+    t = table()
+    caches = [cache(t), cache(t)]
+    other = copy.deepcopy(caches)
+    assert other[0].table is other[1].table is not t and other[0].table.caches == other and t.caches == caches
+    kept = weakref.ref(other[0].table), weakref.ref(other[1].keys[0])
+    del other
+    assert all(r() is None for r in kept)
+    assert copy.deepcopy(caches[1]).table.caches[0:] != caches
+
+
+def test_a_table_copied_by_itself_has_its_caches():
+    t = table()
+    caches = [cache(t), cache(t)]
+    t.counts.fill_(3)
+    caches[1].keys[0].fill_(5.0)
+    for other in (copy.deepcopy(t), copy.deepcopy({"t": t, "c": caches})["t"]):
+        assert len(other.caches) == 2 and all(c.table is other for c in other.caches)
+        assert bool((other.caches[1].keys[0] == 5).all()) and other.counts.tolist() == [3, 3]
+        assert other.caches[1].keys[0].data_ptr() != caches[1].keys[0].data_ptr()
+    again = copy.deepcopy(other)
+    assert len(again.caches) == 2 and again.caches[0] is not other.caches[0]
+
+
+def test_saved_and_loaded():
+    t = table()
+    caches = [cache(t), cache(t, order=3)]
+    caches[1].keys[2].fill_(5.0)
+    for what in (t, caches):
+        file = io.BytesIO()
+        torch.save(what, file)
+        file.seek(0)
+        got = torch.load(file, weights_only=False)
+        got = got.caches if what is t else got
+        assert [c.order for c in got] == [2, 3] and got[0].table is got[1].table and got[0].table.caches == got
+        assert bool((got[1].keys[2] == 5).all()) and got[0].table._t.counts == got[0].table.counts.data_ptr()
