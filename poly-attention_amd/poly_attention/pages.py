@@ -35,6 +35,7 @@ from . import _lib
 from ._lib import DTYPE_CODE, PA_MAX_PAGE_ROWS
 from .drafts import _call, _need, _no_tangents, _rows16, _set_view
 
+_PLANS = 32  # shapes of steps that a cache keeps the calls' structures for: packed steps may each have another
 _NO_GRAD = "PagedCache steps are inference-only: run them under torch.no_grad()"
 
 
@@ -298,6 +299,12 @@ class PagedCache:
 
     # -------------------------------------------------------------------------------------
 
+    def _keep(self, kind: str, shape, plan):
+        if len(self._plans) >= _PLANS:
+            del self._plans[next(iter(self._plans))]
+        self._plans[kind, shape] = plan
+        return plan
+
     def _check_rows(self, t: Tensor, what: str, shape: tuple) -> None:
         _need(t.shape == shape, f"{what}: {list(shape)}, not {list(t.shape)}")
         _need(t.dtype == self.dtype, f"{what}: {t.dtype}, the cache holds {self.dtype}", TypeError)
@@ -337,7 +344,7 @@ class PagedCache:
         plan = self._plans.get(("append", q1.shape))
         if plan is None:
             self._check_q1(q1)
-            plan = self._plans["append", q1.shape] = self._append_plan(q1)
+            plan = self._keep("append", q1.shape, self._append_plan(q1))
         self._check_tokens(q1.shape)
         P, kv = plan
         B, H, T, d = q1.shape
@@ -434,7 +441,7 @@ class PagedCache:
         plan = self._plans.get(("attend", q1.shape))
         if plan is None:
             self._check_q1(q1)
-            plan = self._plans["attend", q1.shape] = self._attend_plan(q1)
+            plan = self._keep("attend", q1.shape, self._attend_plan(q1))
         self._check_tokens(q1.shape)
         D, strides, kv = plan
         dtype, device = self.dtype, self.device

@@ -78,3 +78,25 @@ def test_saved_and_loaded():
         got = got.caches if what is t else got
         assert [c.order for c in got] == [2, 3] and got[0].table is got[1].table and got[0].table.caches == got
         assert bool((got[1].keys[2] == 5).all()) and got[0].table._t.counts == got[0].table.counts.data_ptr()
+
+
+def test_steps_of_many_shapes_are_not_kept(monkeypatch):
+    """A packed step has another total each time."""
+    c = cache()
+    monkeypatch.setattr(c, "_check_q1", lambda q1: None)  # it wants the GPU
+
+    class Planned(Exception):
+        pass
+
+    def attend(n):
+        c.attend(torch.zeros(1, 2, n, 64))
+
+    made = []
+    monkeypatch.setattr(c, "_attend_plan", lambda q1: made.append(q1.shape[2]) or "plan")
+    monkeypatch.setattr(c, "_check_tokens", lambda shape: (_ for _ in ()).throw(Planned))
+    for n in range(1, 400):
+        with pytest.raises(Planned):
+            attend(n)
+    with pytest.raises(Planned):
+        attend(399)                            # a shape of late
+    assert made == list(range(1, 400)) and 1 <= len(c._plans) <= 64
