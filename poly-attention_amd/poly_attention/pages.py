@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import copy
 import ctypes
+import operator
 import weakref
 from typing import Optional, Sequence
 
@@ -156,11 +157,21 @@ class PageTable:
             _need(x.shape == (self.rows,), f"{what}: [{self.rows}], not {list(x.shape)}")
             if x.device == self.device:
                 if x.dtype != torch.int32:  # whatever does not fit is far outside every range
-                    x = x.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32) if x.dtype == torch.int64 else x.to(torch.int32)
+                    y, most = x.to(torch.int64), (1 << 31) - 1
+                    if x.dtype == torch.uint64:
+                        y = torch.where(y < 0, most, y)
+                    x = y.clamp(-most, most).to(torch.int32)
                 return x.contiguous()
             x = x.tolist()
         _need(len(x) == self.rows, f"{what}: one for each of the {self.rows} rows")
-        return torch.tensor([max(-1, min(int(v), (1 << 31) - 1)) for v in x], dtype=torch.int32, device=self.device)
+        return torch.tensor([max(-1, min(v, (1 << 31) - 1)) for v in self._whole(x, what)], dtype=torch.int32, device=self.device)
+
+    @staticmethod
+    def _whole(x, what: str) -> list:
+        try:
+            return [operator.index(v) for v in x]
+        except TypeError:
+            raise TypeError(f"{what}: whole numbers") from None
 
     def extend(self, more) -> None:
         """``more[b]`` new tokens for every row (whole numbers, an int32 tensor on the device or a list): their pages are
@@ -173,7 +184,7 @@ class PageTable:
         host = not isinstance(more, Tensor) or more.device.type == "cpu"
         tensor = self._rows_tensor(more, "more")
         if host:
-            each = [max(int(v), 0) for v in (more.tolist() if isinstance(more, Tensor) else more)]
+            each = [max(v, 0) for v in (more.tolist() if isinstance(more, Tensor) else self._whole(more, "more"))]
             self._expected = (max(each), sum(each))
         else:
             self._expected = None

@@ -100,3 +100,20 @@ def test_steps_of_many_shapes_are_not_kept(monkeypatch):
     with pytest.raises(Planned):
         attend(399)                            # a shape of late
     assert made == list(range(1, 400)) and 1 <= len(c._plans) <= 64
+
+
+@pytest.mark.parametrize("dtype, x, want", [
+    (torch.uint64, [(1 << 32) + 1, 5], [(1 << 31) - 1, 5]), (torch.uint64, [(1 << 64) - 1, 0], [(1 << 31) - 1, 0]),
+    (torch.uint32, [(1 << 32) - 1, 1 << 31], [(1 << 31) - 1] * 2), (torch.uint16, [65535, 1], [65535, 1]),
+    (torch.int64, [(1 << 40), -(1 << 40)], [(1 << 31) - 1, -(1 << 31) + 1]), (torch.int8, [-1, 3], [-1, 3]),
+])
+def test_numbers_of_any_type(dtype, x, want):
+    """Numbers that do not fit stay outside every range, instead of becoming others."""
+    got = table()._rows_tensor(torch.tensor(x, dtype=dtype), "more")
+    assert got.dtype == torch.int32 and got.tolist() == want
+
+
+@pytest.mark.parametrize("x", [[1.5, 2], [1, 2.0], ["1", 2], [None, 1]])
+def test_lists_hold_whole_numbers(x):
+    with pytest.raises(TypeError, match="whole"):
+        table()._rows_tensor(x, "lengths")
