@@ -342,7 +342,11 @@ __device__ __forceinline__ bool paged_join(const PagedDev& P, const PagedUnit& U
                     y[q] = make_float4(y[q].x * f, y[q].y * f, y[q].z * f, y[q].w * f);
 #pragma unroll
                     for (int k = 0; k < N; ++k) {
-                        if (u0 + k * parts >= count || ms[q][k].x == -INFINITY) continue;
+                        if (u0 + k * parts >= count) continue;
+                        if (ms[q][k].x == -INFINITY) {  // its sum is 0, or no number as its scores are
+                            sum[q] += ms[q][k].y;
+                            continue;
+                        }
                         const float w = __builtin_amdgcn_exp2f(ms[q][k].x - t);
                         sum[q] += ms[q][k].y * w;
                         y[q] = make_float4(fmaf(z[q][k].x, w, y[q].x), fmaf(z[q][k].y, w, y[q].y), fmaf(z[q][k].z, w, y[q].z),
@@ -371,7 +375,10 @@ __device__ __forceinline__ bool paged_join(const PagedDev& P, const PagedUnit& U
                     y = make_float4(y.x * f0, y.y * f0, y.z * f0, y.w * f0);
                     for (int k = 1; k < parts; ++k) {
                         const float* z = s_red[(k << lgp) + tid];
-                        if (z[0] == -INFINITY) continue;
+                        if (z[0] == -INFINITY) {
+                            sum += z[1];
+                            continue;
+                        }
                         const float w = __builtin_amdgcn_exp2f(z[0] - t);
                         sum += z[1] * w;
                         y = make_float4(fmaf(z[2], w, y.x), fmaf(z[3], w, y.y), fmaf(z[4], w, y.z), fmaf(z[5], w, y.w));

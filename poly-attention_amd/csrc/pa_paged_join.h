@@ -56,15 +56,15 @@ __device__ __forceinline__ void paged_slow(const PagedDev& P, const PagedUnit& U
     for (int i = 0; i < 4; ++i) S.y[wave][lane + 64 * i] = y[i];
     __syncthreads();
     if (wave) return;
-    // a maximum that is no number is passed over above, and shows in the sums
+    // a maximum that is no number is passed over above, and shows in the sums, also of a wave that has no other
     const float t = fmaxf(fmaxf(S.top[0], S.top[1]), fmaxf(S.top[2], S.top[3]));
     sum = 0.f;
     for (int i = 0; i < 4; ++i) y[i] = 0.f;
     for (int w = 0; w < 4; ++w) {
         if (64 * w >= see) break;  // had no position
-        const float f = __builtin_amdgcn_exp2f(S.top[w] - t);
-        if (f == 0.f) continue;
+        const float f = S.top[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(S.top[w] - t);
         sum += S.sum[w] * f;
+        if (f == 0.f) continue;
         for (int i = 0; i < 4; ++i) y[i] += S.y[w][lane + 64 * i] * f;
     }
     const PagedTo to = paged_to<T>(P, U, hk, r);

@@ -421,8 +421,9 @@ __global__ __launch_bounds__(kPageThreads, paged_waves(D, RT)) void k_paged_rows
         top = s_m[0][r];
         for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][r]);
         float sum = 0.f;
+        // a wave without a maximum has a sum of 0, or none where its scores are no numbers
         for (int w = 0; w < 4; ++w)
-            sum += s_m[w][r] == -INFINITY ? 0.f : s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - top);
+            sum += s_m[w][r] == -INFINITY ? s_l[w][r] : s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - top);
         return sum;
     };
     if (!done && !paged_recorded(P, U)) return;

@@ -5,7 +5,7 @@ import weakref
 import pytest
 import torch
 
-from test_gpu_27_pages import dev
+from test_gpu_27_pages import DT, dev, fill, inputs, make
 
 pytestmark = pytest.mark.gpu
 param = pytest.mark.parametrize
@@ -143,3 +143,59 @@ def test_a_captured_call_keeps_its_arrays():
     t.extend([1, 1, 1])                        # eager calls go on
     assert all(bool((x == 7).all()) for x in theirs)
     del t, caches, graph
+
+
+@param("dtype", [torch.uint64, torch.uint32, torch.int64])
+def test_counts_of_any_type(dtype):
+    from poly_attention import PageTable
+
+    d = dev()
+    t = PageTable(2, pages=8, page_size=16, capacity=64)
+    t.extend(torch.tensor([3, 17], dtype=dtype).to(d))
+    assert t.counts.tolist() == [3, 17]
+    t.extend(torch.tensor([(1 << 31) + 1 if dtype == torch.uint32 else (1 << 32) + 1, 1], dtype=dtype).to(d))
+    assert t.counts.tolist() == [3, 18] and t.new.tolist() == [0, 1] and bool(t.overflow.item())
+
+
+# ---------------------------------------------------------------------------------------
+# numbers that are none
+
+
+@param("dtype", ["bf16", "f16", "f32"])
+@param("counts, new, heads, D, lo, hi", [
+    ([100], [1], 2, 64, 0, 32),                # all that one wave has, of a unit
+    ([100], [1], 2, 64, 0, 16),                # a half of it (fp32: the same)
+    ([100], [100], 2, 64, 0, 100),             # all there is
+    ([9000], [3], 4, 64, 0, 8000),             # whole units of several
+    ([9000], [40], 2, 128, 4000, 8000),        # in two steps of the join
+    ([300], [200], 2, 64, 0, 64),              # many rows, one unit
+    ([5000], [300], 2, 64, 0, 2048),           # many rows, several units
+    ([5000], [300], 2, 128, 0, 4500),
+    ([5000], [300], 4, 96, 2048, 4500),
+])
+def test_keys_that_are_no_numbers(counts, new, heads, D, dtype, lo, hi):
+    """Softmaxes over a score that is no number are none, wherever the others of its wave or unit are none either."""
+    from poly_attention import PagedCache
+
+    dev()
+    g = torch.Generator().manual_seed(4)
+    t, o = make(counts, new, 16, g)
+    cache = PagedCache(t, order=3, kv_heads=2, dim_head=D, dtype=DT[dtype])
+    fill(cache, o, g)
+    n, m = counts[0], new[0]
+    for p in range(lo, hi):
+        cache.keys[0][o.pages[0][p // 16], 1, p % 16] = float("nan")
+    q1 = inputs(o, heads, D, DT[dtype], False, g).cuda()
+    v = inputs(o, 2, D, DT[dtype], False, g).cuda()
+    out = cache.attend(q1, [v]).float().cpu()
+    sees = torch.arange(n - m, n) >= lo
+    half = heads // 2
+    assert bool(torch.isfinite(out[0, :half]).all())
+    assert bool(torch.isnan(out[0, half:, sees]).all())
+    assert bool(torch.isfinite(out[0, half:, ~sees]).all())
+    for lse, value in zip(cache.lses, cache.values[1:]):
+        where = [(o.pages[0][p // 16], p % 16) for p in range(n - m, n)]
+        got = torch.stack([lse[page, 1, slot] for page, slot in where]).cpu()
+        assert torch.equal(torch.isnan(got), sees)
+        got = torch.stack([value[page, 1, slot] for page, slot in where]).float().cpu()
+        assert torch.equal(torch.isnan(got).all(-1), sees)
