@@ -1,0 +1,80 @@
+"""GPU: chunks of many query rows (k_paged_tiles): head dims between the kernels' own, units of a few positions, and what is
+not finite behind a token, with and without a soft clamp, in one unit and in several."""
+
+import pytest
+import torch
+
+import pages_oracle as PO
+from test_gpu_27_pages import DT, assert_within, check_attend, dev, fill, inputs, make
+
+pytestmark = pytest.mark.gpu
+param = pytest.mark.parametrize
+
+
+@param("dtype", ["bf16", "f16"])
+@param("D", [8, 40, 72, 96, 120])
+@param("counts, new, packed", [([200, 150], [150, 70], False),             # one unit of a row each
+                               ([3000, 90, 700], [200, 90, 1], True)])     # several, and few rows beside them
+def test_head_dims_between(counts, new, packed, D, dtype):
+    check_attend(3, counts, new, 4, 2, D, dtype, 32, packed)
+    check_attend(2, counts, new, 4, 2, D, dtype, 16, not packed, softclamp=4.0)
+
+
+def last_unit(n, m, rep, kv_heads, D):
+    """Positions of the last unit of a single row's tiles, as the launch of many rows splits them: chunks of 128 positions, two
+    at least to a unit, and no more units than the card has room for."""
+    rows = m * rep
+    tiles, chunks = -(-rows // 256), -(-n // 128)
+    target = max(1, 256 * (1 if D > 64 else 2) // kv_heads)
+    aim = max(target - tiles // 2, target // 2 + 1)
+    size = max(-(-tiles * chunks // aim), 2)
+    splits = -(-chunks // size)
+    size = -(-chunks // splits)
+    return n - (splits - 1) * size * 128
+
+
+@param("softclamp", [None, 5.0])
+@param("dtype", ["bf16", "f16"])
+@param("D", [64, 128])
+@param("n, m, H, hk, want", [(257, 200, 1, 1, 1), (320, 250, 1, 1, 64), (290, 90, 2, 1, 34), (1537, 300, 2, 2, 1)])
+def test_units_of_a_few_positions(n, m, H, hk, want, D, dtype, softclamp):
+    """One tile of 64 positions, or a part of one, is all that a workgroup of many rows has: where the GPU once faulted."""
+    assert last_unit(n, m, 1, hk, D) == want <= 64
+    check_attend(2, [n], [m], H, hk, D, dtype, 64, softclamp=softclamp)
+
+
+@param("softclamp", [None, 4.0])
+@param("dtype", ["bf16", "f16"])
+@param("D", [64, 96, 128])
+@param("counts, new", [([240], [100]), ([700], [200]), ([4000, 180], [300, 90])])
+def test_what_a_token_does_not_see(counts, new, D, dtype, softclamp):
+    """Infinities and NaN in the last tokens' keys, queries and values reach no earlier token: those stay within the bounds of
+    what they see."""
+    from poly_attention import PagedCache
+
+    dev()
+    g = torch.Generator().manual_seed(3)
+    t, o = make(counts, new, 16, g)
+    cache = PagedCache(t, order=3, kv_heads=2, dim_head=D, dtype=DT[dtype])
+    host = fill(cache, o, g)
+    q1, v = inputs(o, 4, D, DT[dtype], False, g), inputs(o, 2, D, DT[dtype], False, g)
+    (out, tol), values, lses = PO.attend(q1, [v], host, o, False, D ** -0.5, softclamp)
+    bad = [(3, float("inf")), (1, float("nan")), (2, -float("inf"))]
+    q, w = q1.cuda(), v.cuda()
+    for b, n in enumerate(counts):
+        for k, x in bad:
+            page, slot = o.pages[b][(n - k) // 16], (n - k) % 16
+            for a in (*cache.keys, cache.values[0]):
+                a[page, :, slot] = x
+            w[b, :, new[b] - k] = x
+            q[b, :, new[b] - k] = x
+    got = cache.attend(q, [w], softclamp=softclamp)
+    for b, n in enumerate(counts):
+        m = new[b] - 3
+        assert_within(got[b, :, :m], out[b, :, :m], tol[b, :, :m], f"row {b}")
+        for x, (y, y_tol) in [*zip(cache.values[1:], values[1:]), *zip(cache.lses, lses)]:
+            for p in range(n - new[b], n - 3):
+                at = o.pages[b][p // 16], slice(None), p % 16
+                assert_within(x[at], y[at], y_tol[at], f"position {p}")
+        # the last token sees all of them
+        assert not bool(torch.isfinite(got[b, :, new[b] - 1].float()).any())
