@@ -16,10 +16,12 @@
 // say that it was passed by far, or a row that has none yet, is formed again (kTileCap).  Scores get the logsumexp
 // of the level below as the products' initial value.
 //
-// A weight enters its product rounded once to the operands' type (k_paged_rows takes it as two numbers): of a row's many
-// weights each is off by at most half a step, and the output, 2^-9 off by its own rounding in bf16, is some 1.3 times as far
-// off (0.0023 against 0.0017 in norm over three levels), where a second product would make half as many products more.  The
-// final level divides by the sum of the rounded weights; a level whose logsumexp is kept by that of the fp32 ones.
+// What a level leaves in the cache is kept, and read by every later token: its weights enter the products as two numbers of the
+// operands' type, as in k_paged_rows, so that it does not depend on how many tokens a chunk has. The final level's weights are
+// rounded once, and divided by the sum of the rounded ones: of a row's many weights each is off by at most half a step, and the
+// output, 2^-9 off by its own rounding in bf16, 1.2 to 1.4 times as far off as that alone (fp16 the same). 4096 tokens behind
+// 4096, 32/8 heads of 128: 631 us so, 800 with two numbers at the final level too, 587 with one at both, which left the cached
+// values 1.4 times as far off, at each level anew.
 #pragma once
 
 #include <type_traits>
@@ -60,6 +62,10 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
     if (cnt <= 0) return;  // past the tile's last token: the join knows
     const int r0 = U.tile * P.tile + w * 32 * QB, rend = min((U.tile + 1) * P.tile, U.rows);
 
+    constexpr bool TWO = !LAST;  // numbers of the type that a weight is in its product
+    struct Weights {
+        u32x4_t hi[2], lo[TWO ? 2 : 1];
+    };
     frag qf[QB][D / 16];
     f32x16_t o[QB][D / 32];
     float m[QB], l[QB];
@@ -200,17 +206,27 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
         }
     };
     // four probabilities of a block of rows into the packed operands and the sums
-    auto four = [&](const f32x16_t& s, int i, float msub, u32x4_t (&pk)[2], float (&lts)[4]) __attribute__((always_inline)) {
+    auto four = [&](const f32x16_t& s, int i, float msub, Weights& pk, float (&lts)[4]) __attribute__((always_inline)) {
         const int a = 4 * i;
         const float p0 = fast_exp2(fmaf(s[a], sl2, -msub)), p1 = fast_exp2(fmaf(s[a + 1], sl2, -msub));
         const float p2 = fast_exp2(fmaf(s[a + 2], sl2, -msub)), p3 = fast_exp2(fmaf(s[a + 3], sl2, -msub));
-        const uint32_t w0 = pack2<T>(p0, p1), w1 = pack2<T>(p2, p3);
-        pk[a / 8][(a % 8) / 2] = w0;
-        pk[a / 8][(a % 8) / 2 + 1] = w1;
+        uint32_t w0, w1;
+        if constexpr (TWO) {
+            uint32_t r0, r1;
+            draft_split2<T>(p0, p1, w0, r0);
+            draft_split2<T>(p2, p3, w1, r1);
+            pk.lo[a / 8][(a % 8) / 2] = r0;
+            pk.lo[a / 8][(a % 8) / 2 + 1] = r1;
+        } else {
+            w0 = pack2<T>(p0, p1);
+            w1 = pack2<T>(p2, p3);
+        }
+        pk.hi[a / 8][(a % 8) / 2] = w0;
+        pk.hi[a / 8][(a % 8) / 2 + 1] = w1;
         if constexpr (LAST) {  // the weights as the products take them
             lts[(2 * i) % 4] = sum_pair<T>(w0, lts[(2 * i) % 4]);
             lts[(2 * i + 1) % 4] = sum_pair<T>(w1, lts[(2 * i + 1) % 4]);
-        } else {  // a logsumexp is kept: rounded weights would leave it 2^-9 off
+        } else {
             lts[0] += p0;
             lts[1] += p1;
             lts[2] += p2;
@@ -219,7 +235,7 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
     };
     auto without = [](float x) __attribute__((always_inline)) -> float { return x == -INFINITY ? 0.f : x; };
     // the rare path of a block whose sums passed the cap
-    auto again = [&](const f32x16_t& s, int u, float lt, u32x4_t (&pk)[2]) __attribute__((always_inline)) {
+    auto again = [&](const f32x16_t& s, int u, float lt, Weights& pk) __attribute__((always_inline)) {
         if (__any(!(lt <= kTileCap))) {
             keep_branch();
             const float mn = fmaxf(m[u], top(s));
@@ -306,7 +322,7 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
         }
         begin_rows(s0, 0);
         __builtin_amdgcn_sched_barrier(0);
-        u32x4_t pk0[2], pk1[2];
+        Weights pk0, pk1;
         frag v0[2][D / 32], v1[QB == 2 ? 1 : 2][D / 32];
         static_assert(NK == NV, "a fragment of the values takes the place of one of the keys");
         float lt;
@@ -337,7 +353,8 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int t2 = i / (D / 32), x = i % (D / 32);
-                o[0][x] = M::run(v0[t2][x], __builtin_bit_cast(frag, pk0[t2]), o[0][x]);
+                o[0][x] = M::run(v0[t2][x], __builtin_bit_cast(frag, pk0.hi[t2]), o[0][x]);
+                if constexpr (TWO) o[0][x] = M::run(v0[t2][x], __builtin_bit_cast(frag, pk0.lo[t2]), o[0][x]);
                 if constexpr (QB == 1) load_value(v1, stage, 1, i);
                 if (i % (NV / 4) == 0) four(s1, i / (NV / 4), msub, pk1, lts);
                 __builtin_amdgcn_sched_barrier(0);
@@ -355,7 +372,9 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int t2 = i / (D / 32), x = i % (D / 32);
-            o[R1][x] = M::run(QB == 2 ? v0[t2][x] : v1[QB == 2 ? 0 : t2][x], __builtin_bit_cast(frag, pk1[t2]), o[R1][x]);
+            const frag v = QB == 2 ? v0[t2][x] : v1[QB == 2 ? 0 : t2][x];
+            o[R1][x] = M::run(v, __builtin_bit_cast(frag, pk1.hi[t2]), o[R1][x]);
+            if constexpr (TWO) o[R1][x] = M::run(v, __builtin_bit_cast(frag, pk1.lo[t2]), o[R1][x]);
             if constexpr (MORE) load_key(k0, QB == 2 && !kb ? stage : stage + 1, QB == 2 ? !kb : 0, i);
             __builtin_amdgcn_sched_barrier(0);
         }

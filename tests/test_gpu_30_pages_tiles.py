@@ -78,3 +78,37 @@ def test_what_a_token_does_not_see(counts, new, D, dtype, softclamp):
                 assert_within(x[at], y[at], y_tol[at], f"position {p}")
         # the last token sees all of them
         assert not bool(torch.isfinite(got[b, :, new[b] - 1].float()).any())
+
+
+@param("softclamp", [None, 6.0])
+@param("dtype", ["bf16", "f16"])
+@param("D", [64, 128])
+@param("n, m", [(250, 200), (3000, 300)])
+def test_what_is_cached_holds_more_than_one_rounding(n, m, D, dtype, softclamp):
+    """Values that a level leaves in the cache for later levels and tokens are its averages, rounded once: weights that were
+    rounded to the type as well would leave them sqrt(2) times as far from 64 bits (in norm).  Two numbers hold a weight to 2^-16,
+    which beside the result's 2^-9 (fp16: 2^-22 beside 2^-12) is below a hundredth, and fp32 scores of some 10 are within 2^-19."""
+    from poly_attention import PagedCache
+
+    dev()
+    g = torch.Generator().manual_seed(9)
+    t, o = make([n], [m], 64, g)
+    cache = PagedCache(t, order=3, kv_heads=2, dim_head=D, dtype=DT[dtype])
+    fill(cache, o, g)
+    q1, v = inputs(o, 4, D, DT[dtype], False, g).cuda(), inputs(o, 2, D, DT[dtype], False, g).cuda()
+    cache.attend(q1, [v], softclamp=softclamp)
+    rows = lambda x: PO.row_of(x, o.pages[0], n, 64).double()  # noqa: E731
+    hidden = torch.arange(n, device="cuda") > torch.arange(n - m, n, device="cuda")[:, None]
+    for lvl in range(2):
+        s = rows(cache.keys[lvl + 1])[:, n - m:] @ rows(cache.keys[lvl]).transpose(1, 2) * D ** -0.5
+        if softclamp:
+            s = softclamp * torch.tanh(s / softclamp)
+        if lvl:
+            s = s + rows(cache.lses[0])[:, None]
+        s = s.masked_fill(hidden, -float("inf"))
+        want = s.softmax(-1) @ rows(cache.values[lvl])
+        if not lvl:
+            want = want * v[0].double()
+        off = (rows(cache.values[lvl + 1])[:, n - m:] - want).norm()
+        least = (want.to(DT[dtype]).double() - want).norm()
+        assert off <= 1.1 * least, (lvl, (off / least).item())
