@@ -92,14 +92,14 @@ __device__ __forceinline__ void paged_join_tiles(const PagedDev& P, int group, i
     }
 }
 
-// The tiles of one unit that asked to be formed again.  Units that there are not have any flags.
+// The tiles of one unit that asked to be formed again.
 template <typename T>
 __device__ __forceinline__ void paged_again(const PagedDev& P, int group, int groups, SlowRow& S) {
     const int64_t all = (int64_t)P.units * P.kv_heads;
     for (int64_t x = group; x < all; x += groups) {
         if (reinterpret_cast<const uint64_t*>(P.flags)[x] == 0) continue;
         PagedUnit U;
-        if (!paged_find<kUnits>(P, x / P.kv_heads, threadIdx.x & 63, U) || U.splits > 1) continue;
+        if (!paged_find<kUnits>(P, x / P.kv_heads, threadIdx.x & 63, U)) continue;
         for (int r = U.tile * P.tile; r < min((U.tile + 1) * P.tile, U.rows); ++r)
             paged_slow<T>(P, U, (int)(x % P.kv_heads), r, S);
     }

@@ -55,11 +55,15 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
     const int tid = threadIdx.x, lane = tid & 63, w = wave_id();
     const int hh = lane >> 5, col = lane & 31;
     const int hk = __builtin_amdgcn_readfirstlane(blockIdx.x % P.kv_heads);
+    // eight of them, whatever the waves; 0 too where there is no unit, so that the join looks for none
+    auto flag = [&](bool any) __attribute__((always_inline)) {
+        if (lane < 8 / NW) *paged_flag(P, w + NW * lane) = any;
+    };
     PagedUnit U;
-    if (!paged_find<kUnits>(P, blockIdx.x / P.kv_heads, lane, U)) return;
+    if (!paged_find<kUnits>(P, blockIdx.x / P.kv_heads, lane, U)) return flag(false);
     const int begin = U.split * U.size * kPagedChunk;
     const int cnt = min(U.size * kPagedChunk, paged_keys(P, U) - begin);
-    if (cnt <= 0) return;  // past the tile's last token: the join knows
+    if (cnt <= 0) return flag(false);  // past the tile's last token: the join knows
     const int r0 = U.tile * P.tile + w * 32 * QB, rend = min((U.tile + 1) * P.tile, U.rows);
 
     constexpr bool TWO = !LAST;  // numbers of the type that a weight is in its product
@@ -426,9 +430,9 @@ __global__ __launch_bounds__(64 * paged_tile_waves(D), 2) void k_paged_tiles(con
     }
     wait_vmcnt<0>();  // the loads past the end
 
-    if (U.splits > 1 && !paged_recorded(P, U)) return;
     const bool any = __any(odd != 0.f);
-    if (U.splits == 1 && lane < 8 / NW) *paged_flag(P, w + NW * lane) = any;  // eight of them, whatever the waves
+    flag(U.splits == 1 && any);
+    if (U.splits > 1 && !paged_recorded(P, U)) return;
     const PagedRecords<false> R(P, U, hk);
 #pragma unroll
     for (int u = 0; u < QB; ++u) {

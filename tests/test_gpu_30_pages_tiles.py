@@ -112,3 +112,23 @@ def test_what_is_cached_holds_more_than_one_rounding(n, m, D, dtype, softclamp):
         off = (rows(cache.values[lvl + 1])[:, n - m:] - want).norm()
         least = (want.to(DT[dtype]).double() - want).norm()
         assert off <= 1.1 * least, (lvl, (off / least).item())
+
+
+@param("counts, new, packed", [([250, 100], [200, 1], True), ([6000, 130], [300, 90], False), ([90] * 40, [90] * 40, False)])
+@param("D", [64, 128])
+def test_whatever_the_workspace_held(counts, new, packed, D):
+    """Every byte of a workspace that a call reads was written by it."""
+    from poly_attention import PagedCache
+
+    dev()
+    g = torch.Generator().manual_seed(2)
+    t, o = make(counts, new, 64, g)
+    cache = PagedCache(t, order=2, kv_heads=2, dim_head=D, dtype=torch.bfloat16)
+    fill(cache, o, g)
+    q1 = inputs(o, 4, D, torch.bfloat16, packed, g).cuda()
+    want = cache.attend(q1)
+    size = cache._plans["attend", q1.shape][0].workspace_bytes
+    for byte in (0, 255, 127, 1):
+        torch.cuda.synchronize()
+        torch.full((size,), byte, dtype=torch.uint8, device="cuda")  # the block that the call takes next
+        assert torch.equal(cache.attend(q1), want)
