@@ -532,8 +532,9 @@ __global__ __launch_bounds__(kDraftThreads, draft_waves(D, RT, VM)) void k_draft
     if (tid < nrows) {
         float top = s_m[0][tid], sum = 0.f;
         for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][tid]);
+        // a wave without a maximum has a sum of 0, or none where its scores are no numbers
         for (int w = 0; w < 4; ++w)
-            sum += s_m[w][tid] == -INFINITY ? 0.f : s_l[w][tid] * __builtin_amdgcn_exp2f(s_m[w][tid] - top);
+            sum += s_m[w][tid] == -INFINITY ? s_l[w][tid] : s_l[w][tid] * __builtin_amdgcn_exp2f(s_m[w][tid] - top);
         P.ws_s[rec + tid] = make_float2(top, sum);
     }
     // 16 rows at a time, the waves side by side in NB buffers

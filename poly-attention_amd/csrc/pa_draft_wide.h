@@ -317,7 +317,7 @@ __global__ __launch_bounds__(64 * kDraftWideWaves, 2) void k_draft_wide(const Dr
             l[rt] += __shfl_xor(l[rt], 32);
             const int r = 16 * rt + c;
             if (r >= nrows) continue;
-            if (g == 0) P.ws_s[rec + r] = make_float2(m[rt], m[rt] == -INFINITY ? 0.f : l[rt]);
+            if (g == 0) P.ws_s[rec + r] = make_float2(m[rt], l[rt]);  // without a maximum 0, or no number
 #pragma unroll
             for (int j = 0; j < VE; ++j)
                 if (16 * j + 4 * g < P.dim) *reinterpret_cast<f32x4_t*>(P.ws_o + (rec + r) * P.dim + 16 * j + 4 * g) = o[rt][j];
