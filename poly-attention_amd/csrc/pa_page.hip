@@ -579,6 +579,7 @@ __global__ __launch_bounds__(kPageThreads) void k_page_append(const PageRowsDev 
         if (turn) {
 #pragma unroll
             for (int e = 0; e < E; e += 2) {
+                if (d0 + e >= P.rot_dim) continue;  // as it is: a sine of 0 times an infinity is no number
                 const float z = v[e] * cs[e] - v[e + 1] * sn[e];
                 v[e + 1] = v[e + 1] * cs[e + 1] + v[e] * sn[e + 1];
                 v[e] = z;

@@ -199,3 +199,24 @@ def test_keys_that_are_no_numbers(counts, new, heads, D, dtype, lo, hi):
         assert torch.equal(torch.isnan(got), sees)
         got = torch.stack([value[page, 1, slot] for page, slot in where]).float().cpu()
         assert torch.equal(torch.isnan(got).all(-1), sees)
+
+
+@param("dtype", ["bf16", "f16", "f32"])
+@param("D, rot", [(64, 32), (128, 2), (40, 14)])
+def test_features_that_are_not_turned(D, rot, dtype):
+    """They are as they were beside an infinite one."""
+    from poly_attention import PagedCache
+
+    d = dev()
+    g = torch.Generator().manual_seed(5)
+    t, o = make([20, 9], [7, 9], 16, g)
+    cache = PagedCache(t, order=2, kv_heads=2, dim_head=D, dtype=DT[dtype])
+    qs = [inputs(o, 2, D, DT[dtype], False, g).to(d) for _ in range(3)]
+    v = inputs(o, 2, D, DT[dtype], False, g).to(d)
+    for x in qs:
+        x[..., rot + 1::4] = float("inf")
+        x[..., rot + 2::4] = float("nan")
+    q1 = cache.append(qs, v, [None] * 3, eps=1e-6, angles=torch.randn(rot, generator=g).to(d))
+    for b, n in enumerate(o.new):
+        assert torch.equal(q1[b, :, :n, rot:].nan_to_num(77), qs[0][b, :, :n, rot:].nan_to_num(77))
+        assert bool(torch.isfinite(q1[b, :, :n, :rot]).all())
