@@ -515,8 +515,9 @@ typedef struct pa_page_array {
  * counts[b].  Pages are the free ones, lowest first, in the order of the rows; where the row's last
  * page is partly filled and shared, the row first gets a copy of it (of the positions that it holds, in
  * every array), and the last of the rows that write such a page keeps it.  A row whose pages are not
- * to be had, or past max_pages, gets none of its positions (fresh 0, overflow set); rows behind it that
- * need no page are not affected.  starts are the running sums of more (below 0: 0), granted or not.
+ * to be had, or past max_pages, gets none of its positions (fresh 0, overflow set).  Behind a row that
+ * did not find its pages, no row that needs one gets any, nor does a row that was to keep a page which
+ * such a row still shares; rows that need none, and rows behind one past max_pages, get theirs.  starts are the running sums of more (below 0: 0), granted or not.
  * pa_page_compact: the pages in use become the first ones of the pool, those that lie there already
  * unmoved, the others in their order into the free places in their order. */
 typedef struct pa_page_call {

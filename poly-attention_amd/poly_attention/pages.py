@@ -178,8 +178,10 @@ class PageTable:
         taken from the free ones, lowest first, in the order of the rows, and ``counts``, ``new`` and ``starts``
         follow.  A row whose last page is partly filled and shared first gets a copy of it, in every cache; the
         last of the rows that write such a page keeps it.  A row whose pages are not to be had, or that would pass
-        the capacity, gets none of its tokens and sets ``overflow``: nothing of them is cached and their outputs
-        are 0.  Rows behind it that need no new page are not affected."""
+        the capacity, gets none of its tokens and sets ``overflow`` (which stays until it is cleared): nothing of them is
+        cached and their outputs are 0.  Pages are dealt out in the order of the rows: behind a row that did not
+        find its pages none that needs one gets any, however few, nor does a row that was to keep a page which such a
+        row still shares.  The others, and rows behind one that passes the capacity, get theirs."""
         c = self._struct()
         host = not isinstance(more, Tensor) or more.device.type == "cpu"
         tensor = self._rows_tensor(more, "more")

@@ -220,3 +220,37 @@ def test_features_that_are_not_turned(D, rot, dtype):
     for b, n in enumerate(o.new):
         assert torch.equal(q1[b, :, :n, rot:].nan_to_num(77), qs[0][b, :, :n, rot:].nan_to_num(77))
         assert bool(torch.isfinite(q1[b, :, :n, :rot]).all())
+
+
+# ---------------------------------------------------------------------------------------
+# rows that do not get their pages
+
+
+def test_rows_behind_one_that_finds_no_pages():
+    """As the documentation says: behind it none that needs a page, with free ones there, and those that need none do."""
+    from poly_attention import PageTable
+
+    dev()
+    t = PageTable(5, pages=8, page_size=16, capacity=160)
+    t.extend([10, 10, 16, 5, 0])
+    assert t.pages[:, 0].tolist() == [0, 1, 2, 3, -1] and t.free_pages() == 4
+    t.extend([100, 3, 1, 12, 1])               # row 0 needs six pages of the four, row 1 none, row 2 one, rows 3 and 4 one each
+    assert t.new.tolist() == [0, 3, 0, 0, 0] and t.counts.tolist() == [10, 13, 16, 5, 0] and t.free_pages() == 4
+    assert t.starts.tolist() == [0, 100, 103, 104, 116, 117] and bool(t.overflow.item())
+    t.overflow.zero_()
+    t.extend([151, 3, 1, 12, 1])               # row 0 passes its capacity: the others are not affected
+    assert t.new.tolist() == [0, 3, 1, 12, 1] and t.free_pages() == 1 and bool(t.overflow.item())
+
+
+def test_a_row_that_waits_for_a_shared_page():
+    from poly_attention import PageTable
+
+    dev()
+    t = PageTable(3, pages=3, page_size=16, capacity=64)
+    t.extend([20, 0, 5])
+    t.select([0, 0, 2])
+    t.extend([1, 1, 1])                        # rows 0 and 1 write page 1, no page is free for row 0's copy
+    assert t.new.tolist() == [0, 0, 1] and t.refs.tolist() == [2, 2, 1] and bool(t.overflow.item())
+    t.free([0])
+    t.extend([0, 1, 1])
+    assert t.new.tolist() == [0, 1, 1] and t.refs.tolist() == [1, 1, 1]

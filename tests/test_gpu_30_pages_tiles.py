@@ -132,3 +132,11 @@ def test_whatever_the_workspace_held(counts, new, packed, D):
         torch.cuda.synchronize()
         torch.full((size,), byte, dtype=torch.uint8, device="cuda")  # the block that the call takes next
         assert torch.equal(cache.attend(q1), want)
+
+
+@param("counts, new, H, hk, D", [([300, 5000], [1, 1], 128, 1, 128), ([40, 700, 64], [1, 0, 2], 160, 2, 64), ([513], [1], 72, 1, 96)])
+@param("packed", [False, True])
+def test_single_tokens_of_many_heads(counts, new, H, hk, D, packed):
+    """More query heads of a key head than a few rows: single tokens are many rows too, with and without other levels'."""
+    check_attend(2, counts, new, H, hk, D, "bf16", 64, packed)
+    check_attend(3, counts, new, H, hk, D, "f16", 16, packed, softclamp=8.0)
