@@ -2,6 +2,7 @@
 #pragma once
 
 #include "pa_common.h"
+#include "pa_draft_partial.h"
 #include "pa_launch.h"
 
 namespace pa {
@@ -92,6 +93,22 @@ inline PageDev page_dev(const pa_page_table& t, int tokens, int packed) {
     P.fresh = t.fresh;
     P.starts = t.starts;
     return P;
+}
+
+// the types, head dims and inputs that the calls take
+inline bool page_dtype(int d) { return d == PA_F32 || d == PA_F16 || d == PA_BF16; }
+inline bool page_dim(int d) { return d >= 8 && d <= 256 && d % 8 == 0 && (d <= 128 || d % 16 == 0); }
+inline bool page_rows16(const pa_view& v) {
+    const int E = v.dtype == PA_F32 ? 4 : 8;
+    return (uintptr_t)v.ptr % 16 == 0 && v.sb % E == 0 && v.sh % E == 0 && v.sn % E == 0;
+}
+inline DraftRow page_view(const pa_view& v) {
+    DraftRow r;
+    r.p = static_cast<char*>(v.ptr);
+    r.sb = v.sb;
+    r.sh = v.sh;
+    r.sn = v.sn;
+    return r;
 }
 
 }  // namespace pa

@@ -7,7 +7,6 @@
 // order in which atomics arrive.
 #include <algorithm>
 
-#include "pa_draft_partial.h"
 #include "pa_page.h"
 
 namespace pa {
@@ -704,23 +703,6 @@ int launch_page_compact(const pa_page_call* c, hipStream_t s) {
     hipLaunchKernelGGL(k_page_copy, dim3(kCopyGroups), dim3(kPageThreads), 0, s, P, 1);
     return PA_OK;
 }
-
-namespace {
-bool page_dtype(int d) { return d == PA_F32 || d == PA_F16 || d == PA_BF16; }
-bool page_dim(int d) { return d >= 8 && d <= 256 && d % 8 == 0 && (d <= 128 || d % 16 == 0); }
-bool page_rows16(const pa_view& v) {
-    const int E = v.dtype == PA_F32 ? 4 : 8;
-    return (uintptr_t)v.ptr % 16 == 0 && v.sb % E == 0 && v.sh % E == 0 && v.sn % E == 0;
-}
-DraftRow page_view(const pa_view& v) {
-    DraftRow r;
-    r.p = static_cast<char*>(v.ptr);
-    r.sb = v.sb;
-    r.sh = v.sh;
-    r.sn = v.sn;
-    return r;
-}
-}  // namespace
 
 int launch_page_append(const pa_page_rows* r, hipStream_t s) {
     if (const int st = page_check(r->t)) return st;

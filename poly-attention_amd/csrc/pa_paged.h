@@ -12,7 +12,6 @@
 // The levels follow one another, as each reads what the one below left in the cache.
 #pragma once
 
-#include "pa_draft_partial.h"
 #include "pa_page.h"
 
 namespace pa {
@@ -477,7 +476,7 @@ extern template void launch_paged_rows<bf16>(const PagedDev& P, const PagedDev& 
 extern template void launch_paged_rows<f16>(const PagedDev& P, const PagedDev& B, int64_t units, int joins, int clear, int tiles, hipStream_t s);
 extern template void launch_paged_rows<float>(const PagedDev& P, const PagedDev& B, int64_t units, int joins, int clear, int tiles, hipStream_t s);
 // 16-bit chunks of more rows (k_paged_tiles), head dims up to 128
-constexpr int paged_tile_rows(int D) { return 256; }
+constexpr int kTileRows = 256;  // of a tile
 template <typename T> void launch_paged_tiles(const PagedDev& P, int64_t units, hipStream_t s);
 extern template void launch_paged_tiles<bf16>(const PagedDev& P, int64_t units, hipStream_t s);
 extern template void launch_paged_tiles<f16>(const PagedDev& P, int64_t units, hipStream_t s);

@@ -16,21 +16,6 @@ __global__ __launch_bounds__(kPageThreads) void k_paged_join(const PagedDev P) {
 
 namespace {
 
-bool paged_dtype(int d) { return d == PA_F32 || d == PA_F16 || d == PA_BF16; }
-bool paged_dim(int d) { return d >= 8 && d <= 256 && d % 8 == 0 && (d <= 128 || d % 16 == 0); }
-bool paged_rows16(const pa_view& v) {
-    const int E = v.dtype == PA_F32 ? 4 : 8;
-    return (uintptr_t)v.ptr % 16 == 0 && v.sb % E == 0 && v.sh % E == 0 && v.sn % E == 0;
-}
-DraftRow paged_view(const pa_view& v) {
-    DraftRow r;
-    r.p = static_cast<char*>(v.ptr);
-    r.sb = v.sb;
-    r.sh = v.sh;
-    r.sn = v.sn;
-    return r;
-}
-
 constexpr int64_t kPagedCus = 256;
 // Units of k_paged_rows: each has its latencies (some 6 us alone), so they are of 64 KB of keys at least, and
 // no more than there is room for at once where that leaves them at most 256 KB; beyond, twice as many, which the uneven
@@ -71,7 +56,7 @@ PagedPlan paged_plan(const pa_paged* p, bool last, bool many, bool both, PagedDe
     P.rep = rep;
     P.over = many ? kPagedFewRows : 0;
     P.most = many || !both ? 1 << 30 : kPagedFewRows;
-    P.tile = many ? paged_tile_rows(D) : 16 * plan.tiles;
+    P.tile = many ? kTileRows : 16 * plan.tiles;
     const int64_t flight = kPagedCus * (many ? (D == 128 ? 1 : 2) : paged_waves(D, plan.tiles));
     P.target = (int)std::max<int64_t>(1, (many ? 1 : kPagedMany) * flight / p->kv_heads);
     const int64_t chunk = (int64_t)kPagedChunk * p->dim * (f32 ? 4 : 2);  // bytes of its keys
@@ -111,7 +96,7 @@ size_t paged_bytes(const PagedPlan& plan, int dim) {
 }  // namespace
 
 size_t paged_attend_workspace(const pa_paged* p) {
-    if (p->kv_heads < 1 || p->heads < 1 || p->tokens < 1 || p->t.rows < 1 || p->t.max_pages < 1 || !paged_dim(p->dim)) return 0;
+    if (p->kv_heads < 1 || p->heads < 1 || p->tokens < 1 || p->t.rows < 1 || p->t.max_pages < 1 || !page_dim(p->dim)) return 0;
     PagedDev P;
     size_t n = 16;
     for (int last = 0; last < 2; ++last) {
@@ -126,22 +111,22 @@ size_t paged_attend_workspace(const pa_paged* p) {
 int launch_paged_attend(const pa_paged* p, hipStream_t s) {
     if (const int st = page_check(p->t)) return st;
     if (p->tokens < 1 || p->kv_heads < 1 || p->heads < 1 || p->heads % p->kv_heads != 0 || p->order < 2 ||
-        p->order > PA_MAX_ORDER || p->dim < 1 || !paged_dtype(p->dtype))
+        p->order > PA_MAX_ORDER || p->dim < 1 || !page_dtype(p->dtype))
         return PA_EINVAL;
-    if (!paged_dim(p->dim)) return PA_EUNSUPPORTED;
+    if (!page_dim(p->dim)) return PA_EUNSUPPORTED;
     const int rows = p->packed ? 1 : p->t.rows;
     const int64_t rep = p->heads / p->kv_heads;
     if (p->tokens * rep > (1 << 30)) return PA_EUNSUPPORTED;
     auto view_ok = [&](const pa_view& v, int heads) { return v.ptr && v.heads == heads && v.dtype == p->dtype; };
     if (!p->tickets || p->kv_heads > PA_PAGED_TICKETS / 2) return p->tickets ? PA_EUNSUPPORTED : PA_EINVAL;
     if (!view_ok(p->q, p->heads) || !view_ok(p->out, p->heads)) return PA_EINVAL;
-    if (!paged_rows16(p->q) || !paged_rows16(p->out)) return PA_EUNSUPPORTED;
+    if (!page_rows16(p->q) || !page_rows16(p->out)) return PA_EUNSUPPORTED;
     for (int t = 0; t < p->order; ++t) {
         const pa_paged_level& l = p->levels[t];
         const bool middle = t > 0 && t < p->order - 1;
         if (!l.keys || !l.values || (t < p->order - 1 && !l.lses) || (middle && !view_ok(l.vmul, p->kv_heads)))
             return PA_EINVAL;
-        if ((uintptr_t)l.keys % 16 || (uintptr_t)l.values % 16 || (uintptr_t)l.lses % 16 || (middle && !paged_rows16(l.vmul)))
+        if ((uintptr_t)l.keys % 16 || (uintptr_t)l.values % 16 || (uintptr_t)l.lses % 16 || (middle && !page_rows16(l.vmul)))
             return PA_EUNSUPPORTED;
     }
     PagedDev P;
@@ -163,10 +148,10 @@ int launch_paged_attend(const pa_paged* p, hipStream_t s) {
         const bool last = t == p->order - 1, middle_next = t + 1 < p->order - 1;
         const pa_paged_level& l = p->levels[t];
         P.last = last;
-        P.q = paged_view(p->q);
-        P.out = paged_view(p->out);
+        P.q = page_view(p->q);
+        P.out = page_view(p->out);
         P.vmul = DraftRow{nullptr, 0, 0, 0};
-        if (middle_next) P.vmul = paged_view(p->levels[t + 1].vmul);
+        if (middle_next) P.vmul = page_view(p->levels[t + 1].vmul);
         P.keys = static_cast<const char*>(l.keys);
         P.values = static_cast<const char*>(l.values);
         P.bias = t ? p->levels[t - 1].lses : nullptr;
