@@ -569,8 +569,10 @@ typedef struct pa_paged_level {
  *   o = sum_j softmax_j(s) values[t]_j,   lses[t]_p = logsumexp_j(s)
  *   values[t + 1]_p = round(o * vmul[t + 1])  where level t + 1 is a middle one, else round(o)
  * and the final o goes to out.  What a level leaves in the cache is what the next one reads, so that
- * results do not depend on how a row's tokens were cut into chunks beyond the rounding of sums.  Sums,
- * maxima and logsumexps are fp32.  out is 0 for tokens behind their chunk.  kv_heads up to PA_PAGED_TICKETS / 2.  Calls
+ * it does not depend on how a row's tokens were cut into chunks beyond the rounding of sums.  Sums,
+ * maxima and logsumexps are fp32; in 16-bit types a weight is two numbers of the type, but for out of chunks of
+ * more than 64 query rows a key head (head dims to 128), whose weights are rounded once.  out is 0 for tokens behind
+ * their chunk.  kv_heads up to PA_PAGED_TICKETS / 2.  Calls
  * that may overlap need tickets and a workspace of their own. */
 typedef struct pa_paged {
     pa_page_table  t;

@@ -25,17 +25,17 @@ constexpr int64_t kPagedCus = 256;
 // chunks behind 1111, 8/2 heads of 96, 69 and 63.
 constexpr int64_t kPagedMany = 2, kPagedLarge = 256 * 1024, kPagedSmall = 64 * 1024;
 // Units of k_paged_tiles: two chunks at least, and no more than there is room for at once (4 ragged chunks of 512 behind
-// 2048, 32/8 heads of 128: 173 us, with twice as many 236; 512 behind 32768: 489 and 525; a prompt's 512 among 15 tokens, order
-// 3, 16 heads of 64: 141, with four chunks at least 160).
+// 2048, 32/8 heads of 128: 171 us, with twice as many 237; 512 behind 32768: 483 and 525; a prompt's 512 among 15 tokens, order
+// 3, 16 heads of 64: 150, with four chunks at least 171).
 constexpr int kTilesFewest = 2;
 // Up to so many workgroups that join tiles share the launch of the few rows', behind those: 512 of them beside 15 rows' tokens
-// (order 3, 16 heads of 64) 141 us so, 161 in a launch of their own; beside idle ones (8 rows' 24 tokens) 85 and 81.  More
-// would wait for that launch's registers: 2048 of 4096 tokens, 32/8 heads of 128, 677 us so and 650 in their own.
+// (order 3, 16 heads of 64) 150 us so, 165 in a launch of their own; beside idle ones (8 rows' 24 tokens behind 2048, 32/8 heads
+// of 128) 66 and 61.  More would wait for that launch's registers: 2048 of 4096 tokens behind 4096 658 us so and 640 in their own.
 constexpr int kPagedJoins = 1024;
 // Chunks of more query rows per key head than this go to k_paged_tiles, where it applies.  8 rows behind 4096 positions, both
-// levels of order 2, us: 32/8 heads of 128, 12 tokens (48 rows at the final level) 68 so and 73 with k_paged_tiles there,
-// 64 tokens (64 rows at the first) 110 and 120, 24 (96 rows) 96 with k_paged_rows there and 85 so; 16 heads of 64, 40
-// tokens 88 so and 97.
+// levels of order 2, us: 32/8 heads of 128, 12 tokens (48 rows at the final level) 68 so and 70 with k_paged_tiles there,
+// 64 tokens (64 rows at the first) 109 and 118, 24 (96 rows) 97 with k_paged_rows there and 82 so; 16 heads of 64, 40
+// tokens 88 so and 98.
 constexpr int kPagedFewRows = 64;
 
 // What a launch of a level takes: its tiles and their split.
