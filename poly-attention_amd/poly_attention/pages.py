@@ -14,7 +14,8 @@ piece of one, a single token, or none::
 
 ``x`` is [rows, T, dim], row b's tokens first and padding behind them, or packed, [1, sum(more), dim], one
 row's tokens behind the other's.  A token attends to its row's cached positions and to the tokens of its own chunk
-up to itself.  Rows are forked, freed, cut and reordered with ``PageTable.select``; pages are shared until
+up to itself.  T holds the longest chunk, packed all of them: tokens of a chunk behind it would count as cached without
+having been written (a list given to ``extend`` is checked for it, device numbers cannot be).  Rows are forked, freed, cut and reordered with ``PageTable.select``; pages are shared until
 one of their rows writes to them.
 
 All of it works on the device's counts, without a host synchronisation, so a step of fixed shapes can be captured
