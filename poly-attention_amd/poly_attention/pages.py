@@ -41,6 +41,13 @@ _PLANS = 32  # shapes of steps that a cache keeps the calls' structures for: pac
 _NO_GRAD = "PagedCache steps are inference-only: run them under torch.no_grad()"
 
 
+def _capturing(device) -> bool:
+    if device.index == torch._C._cuda_getDevice():
+        return torch._C._cuda_isCurrentStreamCapturing()
+    with torch.cuda.device(device):
+        return torch._C._cuda_isCurrentStreamCapturing()
+
+
 class PageTable:
     """Which pages each of ``rows`` rows has, out of a pool of ``pages`` pages of ``page_size`` positions (a power
     of two, 16 to 4096); a row holds at most ``capacity`` positions (whole pages).
@@ -53,8 +60,8 @@ class PageTable:
     written back, as long as the caches' pages were not given to others in between.
 
     ``caches`` are those that there are: a cache holds its table, not the table its caches, and the pages of one that is given
-    up are free memory again, at the latest when the table goes where a call of it was captured.  A table whose calls
-    were captured takes no further caches.
+    up are free memory again, but for pages that a captured call has (of the cache, or of the table), which stay as long as the
+    table.  A table whose own calls were captured takes no further caches.
 
     A table and its caches take one call at a time; others may be used at once, on any streams.  ``copy.deepcopy`` of
     the list of its caches, or of the table, copies the pool; a table copied by itself holds its copies of the caches."""
@@ -84,7 +91,8 @@ class PageTable:
         t.table, t.counts, t.refs = self.pages.data_ptr(), self.counts.data_ptr(), self.refs.data_ptr()
         t.fresh, t.starts, t.overflow = self.new.data_ptr(), self.starts.data_ptr(), self.overflow.data_ptr()
         self._call_struct = self._scratch = self._arrays = None
-        self._captured = None  # the arrays that a captured call has
+        self._captured = False  # a call of the table
+        self._kept: list = []  # tensors that captured calls have, of the table and of its caches
         self._caches = weakref.WeakValueDictionary(enumerate(caches))
         self._listed = 0  # caches whose arrays are on the list
 
@@ -97,7 +105,7 @@ class PageTable:
         self._call_struct = None  # its list of arrays grows
 
     def _state(self) -> dict:
-        gone = ("_t", "_call_struct", "_scratch", "_arrays", "_captured", "_caches", "_listed", "_own")
+        gone = ("_t", "_call_struct", "_scratch", "_arrays", "_captured", "_kept", "_caches", "_listed", "_own")
         return {k: v for k, v in self.__dict__.items() if k not in gone}
 
     def __getstate__(self):
@@ -123,9 +131,9 @@ class PageTable:
         """The structure of the table's own calls.  Captured steps hold the addresses of its scratch and of the list of
         arrays: the scratch stays as long as the table, and the list from the first captured call on."""
         c = self._call_struct
-        if c is None or (self._listed != len(self._caches) and self._captured is None):
+        if c is None or (self._listed != len(self._caches) and not self._captured):
             _need(self.device.type == "cuda", "a PageTable's calls need the GPU (libpolyattn)", RuntimeError)
-            if self._capturing():
+            if _capturing(self.device):
                 raise RuntimeError("PageTable: run one eager call before capturing steps (the list of its caches is "
                                    "written then)")
             if self._scratch is None:
@@ -142,15 +150,10 @@ class PageTable:
                 c.arrays = self._arrays.data_ptr()
             c.t = self._t
             self._call_struct, self._listed = c, len(caches)
-        elif self._captured is None and self._capturing():
-            self._captured = [x for cache in self.caches for x in cache.arrays()]
+        elif not self._captured and _capturing(self.device):
+            self._captured = True
+            self._kept += [x for cache in self.caches for x in cache.arrays()]
         return c
-
-    def _capturing(self) -> bool:
-        if self.device.index == torch._C._cuda_getDevice():
-            return torch.cuda.is_current_stream_capturing()
-        with torch.cuda.device(self.device):
-            return torch.cuda.is_current_stream_capturing()
 
     def _rows_tensor(self, x, what: str) -> Tensor:
         if isinstance(x, Tensor):
@@ -274,7 +277,7 @@ class PagedCache:
               f"dim_head {dim_head}: a multiple of 8 up to 128, of 16 up to 256")
         self.table, self.order, self.kv_heads, self.dim_head, self.dtype = table, order, kv_heads, dim_head, dtype
         # a captured step would go on without it: a page of it that rows share would not be copied before one of them writes
-        _need(table._captured is None, "a call of the table was captured, and its graph copies the pages of the caches that the "
+        _need(not table._captured, "a call of the table was captured, and its graph copies the pages of the caches that the "
               "table had then: make the caches before, or take another table", RuntimeError)
 
         def rows(m):
@@ -287,14 +290,16 @@ class PagedCache:
         # of attend, 0 between calls
         self._tickets = torch.zeros(_lib.PA_PAGED_TICKETS * _lib.PA_TICKET_STRIDE, dtype=torch.int32, device=table.device)
         self._plans: dict = {}
+        self._captured = False
         table._add(self)
 
     def __getstate__(self):
-        return {k: v for k, v in self.__dict__.items() if k != "_plans"}
+        return {k: v for k, v in self.__dict__.items() if k not in ("_plans", "_captured")}
 
     def __setstate__(self, state) -> None:
         self.__dict__.update(state)
         self._plans = {}
+        self._captured = False
 
     def __deepcopy__(self, memo):
         table = memo.get(id(self.table)) or self.table._copy(memo)
@@ -312,6 +317,11 @@ class PagedCache:
         return (*self.keys, *self.values, *self.lses)
 
     # -------------------------------------------------------------------------------------
+
+    def _hold(self) -> None:
+        """A captured call has the cache's addresses: its tensors stay as long as the table."""
+        self._captured = True
+        self.table._kept += [*self.arrays(), self._tickets]
 
     def _keep(self, kind: str, shape, plan):
         if len(self._plans) >= _PLANS:
@@ -360,6 +370,8 @@ class PagedCache:
             self._check_q1(q1)
             plan = self._keep("append", q1.shape, self._append_plan(q1))
         self._check_tokens(q1.shape)
+        if not self._captured and torch._C._cuda_isCurrentStreamCapturing():
+            self._hold()
         P, kv = plan
         B, H, T, d = q1.shape
         dtype, device, grad = self.dtype, self.device, torch.is_grad_enabled()
@@ -457,6 +469,8 @@ class PagedCache:
             self._check_q1(q1)
             plan = self._keep("attend", q1.shape, self._attend_plan(q1))
         self._check_tokens(q1.shape)
+        if not self._captured and torch._C._cuda_isCurrentStreamCapturing():
+            self._hold()
         D, strides, kv = plan
         dtype, device = self.dtype, self.device
         if q1.dtype is not dtype or q1.device != device:

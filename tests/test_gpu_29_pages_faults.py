@@ -145,6 +145,41 @@ def test_a_captured_call_keeps_its_arrays():
     del t, caches, graph
 
 
+@param("what", ["append", "attend"])
+def test_a_captured_step_keeps_its_cache(what):
+    """The step alone is captured, and the cache given up while its table lives."""
+    from poly_attention import PagedCache, PageTable
+
+    d = dev()
+    g = torch.Generator().manual_seed(1)
+    t = PageTable(2, pages=8, page_size=16, capacity=64)
+    cache = PagedCache(t, order=2, kv_heads=1, dim_head=64, dtype=torch.float32)
+    qs = [torch.randn(2, 1, 4, 64, generator=g).to(d) for _ in range(4)]
+    t.extend([4, 3])
+
+    def step():
+        q1 = cache.append(qs[:3], qs[3], [None] * 3, eps=1e-6)
+        return cache.attend(q1) if what == "attend" else q1
+
+    want = step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step()
+    kept = [weakref.ref(x) for x in (*cache.arrays(), cache._tickets)]
+    del step, cache
+    assert not t.caches and all(r() is not None for r in kept)
+    theirs = [torch.full((8, 1, 16, 64), 7.0, device=d) for _ in range(200)]
+    for _ in range(3):
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+    assert all(bool((x == 7).all()) for x in theirs)
+    del graph, t
+    assert all(r() is None for r in kept)
+
+
 @param("dtype", [torch.uint64, torch.uint32, torch.int64])
 def test_counts_of_any_type(dtype):
     from poly_attention import PageTable
